@@ -237,6 +237,97 @@ TENZO_API int tenzo_cuda_repetition_penalty(float* logits, int vocab, const int*
 TENZO_API int tenzo_cuda_topk_candidates(const float* logits, int vocab, int k, int* count, float* values, int* indices, void* stream);
 TENZO_API int tenzo_cuda_topk_max_candidates(void);
 
+/* ---- 4-bit paged KV cache: append, read, attention, and the tables of beams -----------------------------
+ * No counterpart in the reference (its caches hold 8 bits). Pool: uint8 [block][layer][kv_head][K, V][16 slots][80], 16-byte
+ * aligned. A row is 64 bytes of codes - dim d in nibble d % 2 of byte d / 2, the low nibble first - and four pairs (scale, minimum)
+ * of fp16, one for each 32 dims; a value is minimum + scale * code. 160 bytes a token and kv head (the INT8 caches: 264).
+ * Token t of table row s lives in block block_table[s * table_stride + t / 16], slot t % 16. head_dim is 128.
+ *
+ * A position outside its range, a table row outside [0, table_rows) or a table entry outside [0, n_blocks) touches no memory: that row is
+ * left out and a flag is raised, which tenzo_cuda_kv4_take_errors() returns and clears. Calls on one device share the flags only. */
+typedef struct {
+    uint8_t* pool;
+    int n_blocks, n_layers, n_kv;
+    const int* block_table;  /* device int32 [table_rows][table_stride] */
+    int table_rows, table_stride;
+} tenzo_kv4_cache;
+
+/* Stores `rows` rows of keys and values: k, v [rows][kv_stride] fp32 (n_kv*128 used; rows may be strided, kv_stride >= n_kv*128), row i
+ * at position pos[i] of table row seq[i] (seq NULL: table row i). pos[i] < 0 marks padding: nothing is stored. No two rows of a call may name
+ * the same token. Keys are rotated first (rope tables [rope_len][64], position < rope_len; both NULL: no rotation) as pairs (i, i + 64):
+ *   r_i = fma(x_i, c, -(x_{i+64} * s)),  r_{i+64} = fma(x_i, s, x_{i+64} * c).
+ * Then per 32 dims, each step rounded to fp32: x = clamp(x, +-65504), minimum = fp16(min x), scale = fp16((max x - minimum) * (1/15)),
+ * code = clamp(rint((x - minimum) * (1/scale)), 0, 15), ties to even; scale 0 gives codes 0. Values have to be finite (others spoil their own
+ * 32 dims only). */
+TENZO_API int tenzo_cuda_kv4_append(const tenzo_kv4_cache* cache, int layer, const float* k, const float* v, int kv_stride, const int* pos,
+                                    const int* seq, int rows, const float* rope_cos, const float* rope_sin, int rope_len, int use_pdl, void* stream);
+/* The stored rows as fp32: k, v [rows][kv_stride] (either may be NULL) receive minimum + scale * code, zeros for padding and for rows that are
+ * refused. Keys come back rotated, as they are stored. */
+TENZO_API int tenzo_cuda_kv4_read(const tenzo_kv4_cache* cache, int layer, float* k, float* v, int kv_stride, const int* pos, const int* seq, int rows,
+                                  int use_pdl, void* stream);
+
+/* out[row] = softmax(q K^T / sqrt(128)) V per query head over the keys 0 .. pos[row] of table row seq[row] (seq NULL: row), the query rotated at
+ * pos[row] as above; query head h reads kv head h / (n_q / n_kv), any n_q that n_kv divides. Several rows may name one sequence
+ * (a prompt's or a draft's rows, each with its own position). pos[row] < 0: zeros. A row whose position is max_len or more, or whose table row is
+ * out of range, is not written and raises the flag; a table entry out of range leaves its 16 keys out and raises it. Sums and softmax in
+ * fp32; products with the query and with the weights keep 22 bits (two fp16 parts), outputs agree with 64 bits to about 1e-6 of the output's norm. */
+typedef struct {
+    const float* q;          /* [rows][q_stride], n_q*128 used, before rotation */
+    float* out;              /* [rows][n_q*128] */
+    tenzo_kv4_cache cache;
+    const int* pos;          /* [rows] device */
+    const int* seq;          /* [rows] device, or NULL */
+    const float* rope_cos; const float* rope_sin;   /* [rope_len][64], rope_len >= max_len; both NULL: no rotation */
+    int rope_len;
+    int q_stride;            /* floats between rows; 0 = n_q*128 */
+    int layer, n_q, rows;
+    int max_len;             /* upper bound on pos + 1 (sizes the grid); at most 16 * table_stride */
+    int split_keys;          /* keys a CTA takes (rounded up to 128); 0 = choose */
+    int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
+    void* workspace;         /* 16-byte aligned, contents need not be kept: partial results of splits. tenzo_cuda_attention_kv4_workspace_bytes(...) */
+    size_t workspace_bytes;  /* bytes; with less (or NULL) fewer splits are taken, and split_keys that need more are refused (-1) */
+} tenzo_attention_kv4_args;
+TENZO_API int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, void* stream);
+TENZO_API size_t tenzo_cuda_attention_kv4_workspace_bytes(int rows, int n_q, int n_kv, int max_len);
+/* Error flags of the four calls above and below this one since the last call (bit 0: a bounded wait was given up, bit 1: an index out of range);
+ * -1 if the query failed. Synchronises with the device. */
+TENZO_API int tenzo_cuda_kv4_take_errors(void);
+
+/* The cache's half of a beam-search step. Table rows g*beams .. g*beams + beams - 1 are the beams of group g and hold length[g] tokens each; beam i goes
+ * on from beam parent[g*beams + i] (0 .. beams - 1). With j = length / 16 and r = length % 16, row i of table_out gets its parent's entries below j (full
+ * blocks are shared) and its own above j. The block being filled, entry j if r > 0, belongs to one beam alone (they must differ): the first child of a
+ * parent takes its parent's; the n-th of the further children, by index, takes that of the n-th beam without children, and the r filled slots of all layers and heads are copied
+ * into it. If r = 0, entry j stays the beam's own. No block is allocated or freed, and a prompt is forked the same way: parent 0 for
+ * all. table_out [groups*beams][table_stride] must not overlap the table; groups*beams = table_rows, beams <= TENZO_BEAMS_MOST (-5 otherwise).
+ * A group with a parent or a length out of range is copied as it is and raises the flag. */
+enum { TENZO_BEAMS_MOST = 32 };
+TENZO_API int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_out, const int* parent, const int* length, int groups, int beams, int use_pdl,
+                                     void* stream);
+
+/* ---- beam search: the k best continuations over beams x vocabulary -----------------------------------------
+ * Beside the greedy argmax and the sampler (:1722-1807); the reference has no beam search. logits [groups*beams][row_stride] fp32,
+ * scores [groups*beams] the beams' sums of log-probabilities. Per group, over all beams b and tokens t,
+ *   score(b, t) = scores[b] + (x_t - log sum_u exp x_u)   in 64 bits,
+ * the k best go to parent_out / token_out / score_out [groups][k], best first; of equal scores the lower beam, in a beam the larger logit, then the
+ * lower token. score_out is rounded to fp32.
+ * A finished beam (finished[row] != 0) has its end token `eos` alone, at scores[b]. -inf masks a token; NaN counts as -inf, +inf as the largest finite
+ * number. A beam with score -inf or NaN, or with no token left, has score -inf for every token (chosen only when nothing else is left, lowest index
+ * first). beams <= TENZO_BEAMS_MOST and k <= 2 * TENZO_BEAMS_MOST (-5 otherwise); k <= beams * vocab. */
+typedef struct {
+    const float* logits;
+    const float* scores;
+    const int* finished;     /* [groups*beams] device, or NULL */
+    int eos;                 /* used with `finished` only */
+    int row_stride;          /* floats between rows of logits; 0 = vocab */
+    int groups, beams, vocab, k;
+    int use_pdl;
+    int* parent_out; int* token_out; float* score_out;
+    void* workspace;         /* tenzo_cuda_beam_select_workspace_bytes(...) bytes, 16-byte aligned, contents need not be kept */
+    size_t workspace_bytes;
+} tenzo_beam_select_args;
+TENZO_API int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* stream);
+TENZO_API size_t tenzo_cuda_beam_select_workspace_bytes(int groups, int beams, int vocab, int k);
+
 /* ---- INT8 embedding row dequantisation ---------------------------------------------------------
  * Replaces embedding_lookup's int8 branch (:1299-1315): x = (float)W8[tok] * scale[tok].
  * vocab > 0: token ids outside [0, vocab) are read as row 0 rather than past the table; 0 = unchecked. */

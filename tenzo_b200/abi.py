@@ -69,6 +69,29 @@ class AttentionArgs(C.Structure):
     ]
 
 
+class Kv4Cache(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("n_blocks", C.c_int), ("n_layers", C.c_int), ("n_kv", C.c_int), ("block_table", C.c_void_p),
+                ("table_rows", C.c_int), ("table_stride", C.c_int)]
+
+
+class AttentionKv4Args(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("cache", Kv4Cache), ("pos", C.c_void_p), ("seq", C.c_void_p),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rope_len", C.c_int), ("q_stride", C.c_int),
+        ("layer", C.c_int), ("n_q", C.c_int), ("rows", C.c_int), ("max_len", C.c_int), ("split_keys", C.c_int), ("use_pdl", C.c_int),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("scores", C.c_void_p), ("finished", C.c_void_p), ("eos", C.c_int), ("row_stride", C.c_int),
+        ("groups", C.c_int), ("beams", C.c_int), ("vocab", C.c_int), ("k", C.c_int), ("use_pdl", C.c_int),
+        ("parent_out", C.c_void_p), ("token_out", C.c_void_p), ("score_out", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 ENGINE_SYMBOLS = [
     "tenzo_get_version", "tenzo_default_config", "tenzo_default_sampling_params", "tenzo_create_engine",
     "tenzo_destroy_engine", "tenzo_reset", "tenzo_get_seq_len", "tenzo_set_layer_weights", "tenzo_set_final_norm",
@@ -88,6 +111,8 @@ KERNEL_SYMBOLS = [
     "tenzo_cuda_embedding_i8", "tenzo_cuda_tl1_pack_rows2bit", "tenzo_cuda_lm_head_i8_static",
     "tenzo_cuda_lm_head_static_max_batch", "tenzo_cuda_lm_head_take_timeouts", "tenzo_cuda_repetition_penalty",
     "tenzo_cuda_topk_candidates", "tenzo_cuda_topk_max_candidates",
+    "tenzo_cuda_kv4_append", "tenzo_cuda_kv4_read", "tenzo_cuda_kv4_reorder", "tenzo_cuda_kv4_take_errors", "tenzo_cuda_attention_kv4",
+    "tenzo_cuda_attention_kv4_workspace_bytes", "tenzo_cuda_beam_select", "tenzo_cuda_beam_select_workspace_bytes",
 ]
 HAL_SYMBOLS = ["tenzo_hal_initialize", "tenzo_hal_bitlinear_tl1_host", "tenzo_hal_rmsnorm_host", "tenzo_hal_gemm_f32_host", "tenzo_hal_call_count"]
 
@@ -176,6 +201,16 @@ def declare_kernel_abi(L):
     L.tenzo_cuda_repetition_penalty.restype, L.tenzo_cuda_repetition_penalty.argtypes = i32, [vp, i32, vp, vp, i32, f32, vp]
     L.tenzo_cuda_topk_candidates.restype, L.tenzo_cuda_topk_candidates.argtypes = i32, [vp, i32, i32, vp, vp, vp, vp]
     L.tenzo_cuda_topk_max_candidates.restype, L.tenzo_cuda_topk_max_candidates.argtypes = i32, []
+    cache = C.POINTER(Kv4Cache)
+    L.tenzo_cuda_kv4_append.restype = L.tenzo_cuda_kv4_read.restype = L.tenzo_cuda_kv4_reorder.restype = i32
+    L.tenzo_cuda_kv4_append.argtypes = [cache, i32, vp, vp, i32, vp, vp, i32, vp, vp, i32, i32, vp]
+    L.tenzo_cuda_kv4_read.argtypes = [cache, i32, vp, vp, i32, vp, vp, i32, i32, vp]
+    L.tenzo_cuda_kv4_reorder.argtypes = [cache, vp, vp, vp, i32, i32, i32, vp]
+    L.tenzo_cuda_kv4_take_errors.restype, L.tenzo_cuda_kv4_take_errors.argtypes = i32, []
+    L.tenzo_cuda_attention_kv4.restype, L.tenzo_cuda_attention_kv4.argtypes = i32, [C.POINTER(AttentionKv4Args), vp]
+    L.tenzo_cuda_attention_kv4_workspace_bytes.restype, L.tenzo_cuda_attention_kv4_workspace_bytes.argtypes = sz, [i32, i32, i32, i32]
+    L.tenzo_cuda_beam_select.restype, L.tenzo_cuda_beam_select.argtypes = i32, [C.POINTER(BeamSelectArgs), vp]
+    L.tenzo_cuda_beam_select_workspace_bytes.restype, L.tenzo_cuda_beam_select_workspace_bytes.argtypes = sz, [i32, i32, i32, i32]
     L.tenzo_cuda_lm_head_scratch_bytes.restype, L.tenzo_cuda_lm_head_scratch_bytes.argtypes = sz, [i32]
     L.tenzo_cuda_embedding_i8.restype, L.tenzo_cuda_embedding_i8.argtypes = i32, [vp, vp, i32, vp, i32, vp, i32, i32, vp]
     L.tenzo_cuda_tl1_pack_rows2bit.restype, L.tenzo_cuda_tl1_pack_rows2bit.argtypes = i32, [vp, i32, i32, vp, vp]

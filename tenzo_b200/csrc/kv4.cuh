@@ -1,0 +1,46 @@
+// The 4-bit paged cache: what its kernels (kv4_rows.cu, attention_kv4.cu) share.
+//
+// Pool: uint8 [block][layer][kv head][K, V][16 slots][80]. A row (one token, one kv head, keys or values) is 64 bytes of codes, dim d
+// in nibble d % 2 of byte d / 2 (the low one first), and four pairs (scale, minimum) of fp16 for the dims 32g .. 32g + 31; a value
+// is minimum + scale * code. Rows of 80 bytes are what makes the attention kernel's shared memory free of bank conflicts
+// without a swizzle: 20 words apart, eight consecutive rows start at eight different multiples of four banks. And a page of one
+// head, keys and values, is 2560 contiguous bytes: one bulk copy.
+#pragma once
+#include "common.cuh"
+#include "../../include/tenzo_kernels.h"
+
+namespace tz {
+
+constexpr int kK4Slots = 16, kK4Row = 80, kK4Codes = 64;
+constexpr int kK4Half = kK4Slots * kK4Row;              // the keys of a page, or its values
+constexpr int kK4Page = 2 * kK4Half;
+
+constexpr int kK4ErrWait = 1, kK4ErrIndex = 2;          // bits of the error flags
+
+// Byte offset of the page of `kvh` in block `block`.
+__device__ __forceinline__ size_t kv4_page(const tenzo_kv4_cache& c, int layer, int kvh, int block) {
+    return (((size_t)block * c.n_layers + layer) * c.n_kv + kvh) * kK4Page;
+}
+
+inline bool kv4_cache_ok(const tenzo_kv4_cache& c) {
+    return c.pool && c.block_table && !(reinterpret_cast<uintptr_t>(c.pool) & 15) && c.n_blocks > 0 && c.n_layers > 0 && c.n_kv > 0 && c.table_rows > 0 &&
+           c.table_stride > 0;
+}
+
+// Launch, with (or without) the attribute that lets the kernel become resident while its predecessor drains.
+template <typename... KArgs, typename... Args>
+inline int kv4_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool pdl, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace tz

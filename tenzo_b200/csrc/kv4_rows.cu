@@ -1,0 +1,244 @@
+// Rows of the 4-bit paged cache (kv4.cuh): appending them, reading them back, and handing the tables of parents on to the beams that
+// continue them.
+//
+// Append: one warp per (row, kv head), lanes 0-15 the key, 16-31 the value, eight dims a lane. The rotation pairs dims i and i + 64, that
+// is lanes 8 apart; a group of 32 dims is four lanes, so its minimum and maximum take two shuffles each. Every step is rounded to
+// fp32 in the order the header gives (a code next to a border must not depend on who computes it); only the two parameters are
+// rounded further, to fp16: at 32 dims a pair a third format of 32 bits would cost 10 % of the cache's bytes.
+// Bound by memory: 1024 bytes in and 160 out a row and head.
+#include "kv4.cuh"
+
+#include <cuda_fp16.h>
+
+namespace tz {
+
+constexpr int kRowWarps = 4;                             // rows a CTA, one warp each
+constexpr float kFp16Most = 65504.0f;
+
+__device__ int g_kv4_rows_error = 0;
+
+// The page and slot of a row's token; null for padding (a negative position), and for an index outside its range (which is flagged).
+__device__ __forceinline__ uint8_t* row_place(const tenzo_kv4_cache& c, int layer, int kvh, int pos, int seq, int rope_len) {
+    if (pos < 0) return nullptr;
+    const int col = pos / kK4Slots;
+    int block = -1;
+    if (seq >= 0 && seq < c.table_rows && col < c.table_stride && pos < rope_len) block = __ldg(c.block_table + (size_t)seq * c.table_stride + col);
+    if (block < 0 || block >= c.n_blocks) {
+        atomicOr(&g_kv4_rows_error, kK4ErrIndex);
+        return nullptr;
+    }
+    return c.pool + kv4_page(c, layer, kvh, block) + (size_t)(pos % kK4Slots) * kK4Row;
+}
+
+struct RowsArgs {
+    tenzo_kv4_cache c;
+    int layer, rows, kv_stride, rope_len, use_pdl;
+    const int *pos, *seq;
+    const float *cs, *sn;
+};
+
+template <bool VEC>
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+    if (VEC) {
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __ldcg(p + j);
+    }
+}
+
+template <bool VEC, bool ROPE>
+__global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsArgs a, const float* __restrict__ k, const float* __restrict__ v) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
+    if (a.use_pdl) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
+    if (row >= a.rows) return;
+    const int pos = a.pos[row];
+    float x[8];
+    load8<VEC>((is_v ? v : k) + (size_t)row * a.kv_stride + kvh * 128 + 8 * l, x);      // (padding rows are there to be read too)
+    uint8_t* at = row_place(a.c, a.layer, kvh, pos, a.seq ? a.seq[row] : row, ROPE ? a.rope_len : 0x7fffffff);
+    if (!at) return;                                     // the whole warp
+    if (ROPE) {
+        const float* cs = a.cs + (size_t)pos * 64 + ((8 * l) & 63);
+        const float* sn = a.sn + (size_t)pos * 64 + ((8 * l) & 63);
+        float c[8], s[8];
+        load8<VEC>(cs, c);
+        load8<VEC>(sn, s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float o = __shfl_xor_sync(0xffffffffu, x[j], 8);
+            const float r = l < 8 ? __fmaf_rn(x[j], c[j], -(o * s[j])) : __fmaf_rn(o, s[j], x[j] * c[j]);
+            if (!is_v) x[j] = r;
+        }
+    }
+    float lo, hi;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        x[j] = fminf(fmaxf(x[j], -kFp16Most), kFp16Most);
+        lo = j ? fminf(lo, x[j]) : x[j];
+        hi = j ? fmaxf(hi, x[j]) : x[j];
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const __half low = __float2half_rn(lo), scale = __float2half_rn((hi - __half2float(low)) * (1.0f / 15.0f));
+    const float m = __half2float(low), s = __half2float(scale);
+    uint32_t word = 0;
+    if (s > 0.0f) {
+        const float inv = 1.0f / s;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = __float2int_rn(fminf(fmaxf((x[j] - m) * inv, 0.0f), 15.0f));   // nearest, ties to even
+            word |= (uint32_t)c << (4 * j);
+        }
+    }
+    at += is_v * kK4Half;
+    reinterpret_cast<uint32_t*>(at)[l] = word;
+    if ((l & 3) == 0) reinterpret_cast<__half2*>(at + kK4Codes)[l >> 2] = __halves2half2(scale, low);
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kRowWarps * 32) kv4_read_kernel(const RowsArgs a, float* __restrict__ k, float* __restrict__ v) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
+    if (a.use_pdl) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
+    if (row >= a.rows) return;
+    const uint8_t* at = row_place(a.c, a.layer, kvh, a.pos[row], a.seq ? a.seq[row] : row, 0x7fffffff);
+    float x[8] = {};
+    if (at) {
+        at += is_v * kK4Half;
+        const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(at) + l);
+        const uint32_t pair = __ldcg(reinterpret_cast<const uint32_t*>(at + kK4Codes) + (l >> 2));
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = p.y + p.x * (float)((word >> (4 * j)) & 15u);
+    }
+    float* out = (is_v ? v : k);
+    if (!out) return;
+    out += (size_t)row * a.kv_stride + kvh * 128 + 8 * l;
+    if (VEC) {
+        reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j] = x[j];
+    }
+}
+
+// ---- the tables of the beams after a selection ---------------------------------------------------------------------------
+// A group's beams all hold `length` tokens. Full blocks are shared, so a table row is its parent's; the block being filled is every
+// beam's own: the first child keeps its parent's, a further one gets that of a beam without children and the filled rows are copied
+// into it. Nothing is read that this launch writes: sources have children, targets have none, and the tables are two.
+// CTA (x, y): beam x, part y of the copy. Bound by memory: length % 16 rows of 80 bytes, layers x heads x 2 times, in and out.
+constexpr int kReorderThreads = 256, kReorderParts = 8;
+
+__global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenzo_kv4_cache c, int* __restrict__ table_out, const int* __restrict__ parent,
+                                                                      const int* __restrict__ length, int beams, int use_pdl) {
+    const int g = blockIdx.x / beams, i = blockIdx.x % beams, lane = threadIdx.x & 31;
+    if (use_pdl) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
+    const int* rows = c.block_table + (size_t)g * beams * c.table_stride;      // the group's
+    const int len = length[g], col = len / kK4Slots, filled = len < 0 ? 0 : len % kK4Slots;
+    const bool mine = lane < beams;
+    int p = mine ? parent[(size_t)g * beams + lane] : lane;
+    const bool bad = (mine && (p < 0 || p >= beams)) || len < 0 || col + (filled > 0) > c.table_stride;
+    const bool refused = __any_sync(0xffffffffu, bad);
+    if (refused) {                                       // the group stays as it is
+        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&g_kv4_rows_error, kK4ErrIndex);
+        p = lane;
+    }
+    const unsigned all = beams == 32 ? 0xffffffffu : (1u << beams) - 1u;
+    const unsigned alike = __match_any_sync(0xffffffffu, p) & all, below = (1u << lane) - 1u;
+    const unsigned further = __ballot_sync(0xffffffffu, mine && (alike & below));
+    const unsigned childless = all & ~__reduce_or_sync(0xffffffffu, mine ? 1u << p : 0u);
+    const int from = __shfl_sync(0xffffffffu, p, i);
+    const bool copies = filled > 0 && ((further >> i) & 1u);
+    int giver = filled > 0 ? from : i;                   // whose block the beam goes on filling
+    if (copies) {
+        unsigned left = childless;                       // as many beams are without children as there are further ones
+        for (int n = __popc(further & ((1u << i) - 1u)); n > 0; --n) left &= left - 1u;
+        giver = __ffs((int)left) - 1;
+    }
+    if (blockIdx.y == 0) {
+        int* out = table_out + ((size_t)g * beams + i) * c.table_stride;
+        for (int x = threadIdx.x; x < c.table_stride; x += kReorderThreads)
+            out[x] = refused ? rows[(size_t)i * c.table_stride + x] : rows[(size_t)(x < col ? from : x == col ? giver : i) * c.table_stride + x];
+    }
+    if (!copies) return;
+    const int source = rows[(size_t)from * c.table_stride + col], target = rows[(size_t)giver * c.table_stride + col];
+    if (source < 0 || source >= c.n_blocks || target < 0 || target >= c.n_blocks) {
+        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&g_kv4_rows_error, kK4ErrIndex);
+        return;
+    }
+    const int halves = c.n_layers * c.n_kv * 2, units = filled * (kK4Row / 16);          // 16-byte units of a half page
+    const uint4* src = reinterpret_cast<const uint4*>(c.pool + (size_t)source * halves * kK4Half);
+    uint4* dst = reinterpret_cast<uint4*>(c.pool + (size_t)target * halves * kK4Half);
+    constexpr int kUnits = kK4Half / 16;
+    for (int h = blockIdx.y * (kReorderThreads / 32) + (threadIdx.x >> 5); h < halves; h += kReorderParts * (kReorderThreads / 32))
+        for (int u = lane; u < units; u += 32) dst[(size_t)h * kUnits + u] = __ldcg(src + (size_t)h * kUnits + u);
+}
+
+static bool aligned16(const void* p) { return !(reinterpret_cast<uintptr_t>(p) & 15); }
+
+static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, const int* pos, const int* seq, int rows, RowsArgs* a) {
+    if (!cache || !kv4_cache_ok(*cache) || layer < 0 || layer >= cache->n_layers || !pos || rows < 1 || cache->n_kv > 65535) return false;
+    if (kv_stride < cache->n_kv * 128) return false;
+    if (!seq && rows > cache->table_rows) return false;
+    a->c = *cache;
+    a->layer = layer; a->rows = rows; a->kv_stride = kv_stride; a->pos = pos; a->seq = seq;
+    return true;
+}
+
+int kv4_rows_take_error() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_kv4_rows_error, sizeof v) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_kv4_rows_error, &zero, sizeof zero);
+    return v;
+}
+
+}  // namespace tz
+
+extern "C" int tenzo_cuda_kv4_append(const tenzo_kv4_cache* cache, int layer, const float* k, const float* v, int kv_stride, const int* pos, const int* seq,
+                                     int rows, const float* rope_cos, const float* rope_sin, int rope_len, int use_pdl, void* stream) {
+    using namespace tz;
+    RowsArgs a = {};
+    if (rows == 0) return 0;
+    if (!rows_args(cache, layer, kv_stride, pos, seq, rows, &a) || !k || !v) return -1;
+    if ((rope_cos == nullptr) != (rope_sin == nullptr) || (rope_cos && rope_len <= 0)) return -1;
+    a.cs = rope_cos; a.sn = rope_sin; a.rope_len = rope_len; a.use_pdl = use_pdl != 0;
+    const bool vec = aligned16(k) && aligned16(v) && kv_stride % 4 == 0 && aligned16(rope_cos) && aligned16(rope_sin);
+    auto* kernel = rope_cos ? (vec ? kv4_append_kernel<true, true> : kv4_append_kernel<false, true>)
+                            : (vec ? kv4_append_kernel<true, false> : kv4_append_kernel<false, false>);
+    return kv4_launch(kernel, dim3((unsigned)((rows + kRowWarps - 1) / kRowWarps), (unsigned)cache->n_kv), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl, a, k, v);
+}
+
+extern "C" int tenzo_cuda_kv4_read(const tenzo_kv4_cache* cache, int layer, float* k, float* v, int kv_stride, const int* pos, const int* seq, int rows,
+                                   int use_pdl, void* stream) {
+    using namespace tz;
+    RowsArgs a = {};
+    if (rows == 0) return 0;
+    if (!rows_args(cache, layer, kv_stride, pos, seq, rows, &a) || (!k && !v)) return -1;
+    a.use_pdl = use_pdl != 0;
+    const bool vec = aligned16(k) && aligned16(v) && kv_stride % 4 == 0;
+    return kv4_launch(vec ? kv4_read_kernel<true> : kv4_read_kernel<false>, dim3((unsigned)((rows + kRowWarps - 1) / kRowWarps), (unsigned)cache->n_kv),
+                      kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl, a, k, v);
+}
+
+extern "C" int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_out, const int* parent, const int* length, int groups, int beams, int use_pdl,
+                                      void* stream) {
+    using namespace tz;
+    if (!cache || !kv4_cache_ok(*cache) || !table_out || table_out == cache->block_table || !parent || !length || groups < 1) return -1;
+    if (beams < 1 || beams > TENZO_BEAMS_MOST) return -5;
+    if ((long long)groups * beams != cache->table_rows) return -1;
+    return kv4_launch(kv4_reorder_kernel, dim3((unsigned)(groups * beams), kReorderParts), kReorderThreads, 0, static_cast<cudaStream_t>(stream), use_pdl != 0, *cache,
+                      table_out, parent, length, beams, use_pdl != 0);
+}

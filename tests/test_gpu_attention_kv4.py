@@ -1,0 +1,227 @@
+"""Attention over the 4-bit paged cache against the formula in 64 bits (kv4_reference.attention derives the bound)."""
+import numpy as np
+import pytest
+import torch
+import kv4_reference as ref
+from gpu_helpers import Guarded, dev, host
+
+pytestmark = pytest.mark.gpu
+
+
+def setup(rng, lens, n_kv, columns, layers=1, spread=1.0, garbage=True):
+    """A pool whose slots behind a sequence's last key, and whose other blocks, hold anything (NaN parameters among it)."""
+    n_seq = len(lens)
+    blocks = n_seq * columns + 2
+    table = rng.permutation(blocks)[: n_seq * columns].astype(np.int32).reshape(n_seq, columns)
+    pool = rng.integers(0, 256, (blocks, layers, n_kv, 2, 16, 80), dtype=np.uint8) if garbage else np.zeros((blocks, layers, n_kv, 2, 16, 80), np.uint8)
+    if garbage:
+        pool[..., 64:] = np.array([0x7E00, 0x7C00], np.uint16).view(np.uint8).tolist() * 4           # NaN, infinity
+    good = ref.random_pool(rng, blocks, layers, n_kv, spread)
+    for s, n in enumerate(lens):
+        for c in range((n + 15) // 16):
+            m = min(16, n - 16 * c)
+            pool[table[s, c], :, :, :, :m] = good[table[s, c], :, :, :, :m]
+    return table, pool
+
+
+def check(out, q, pool, table, layer, pos, seq, cos=None, sin=None):
+    n_q = q.shape[1] // 128
+    for i, (p, s) in enumerate(zip(pos, seq)):
+        k, v = ref.cached(pool, layer, table[s], max(0, p + 1))
+        turn = (cos[p], sin[p]) if cos is not None and p >= 0 else (None, None)
+        want, bound = ref.attention(q[i].reshape(n_q, 128), k, v, *turn)
+        err = abs(out[i].reshape(n_q, 128).astype(np.float64) - want)
+        assert (err <= bound).all(), (i, p, float((err / bound).max()))
+        if p >= 0:                                               # and on the whole, to the type's own accuracy
+            rel = np.linalg.norm(out[i].reshape(n_q, 128) - want) / np.linalg.norm(want)
+            assert rel <= 2e-6, (i, p, rel)
+
+
+LENS = [1, 2, 8, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 0, 200, 255, 256, 257, 300]
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(20, 5), (4, 4), (2, 1), (3, 1), (6, 1), (7, 1), (8, 1), (16, 2), (9, 1), (16, 1), (20, 1), (33, 1)])
+@pytest.mark.parametrize("split", [0, 128])
+def test_lengths_and_heads(cuda_lib, n_q, n_kv, split):
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(n_q * 100 + n_kv)
+    table, pool = setup(rng, LENS, n_kv, 20)
+    q = rng.standard_normal((len(LENS), n_q * 128)).astype(np.float32) * 2
+    pos = np.array(LENS, np.int32) - 1
+    cos, sin = ref.rope(320)
+    g = Guarded()
+    out = g.empty((len(LENS), n_q * 128), torch.float32)
+    ws = g.empty((kernels.attention_kv4_workspace_bytes(len(LENS), n_q, n_kv, 320),), torch.uint8)
+    kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=n_q, block_table=dev(table), rope_cos=dev(cos), rope_sin=dev(sin), out=out, split_keys=split,
+                          workspace=ws)
+    check(host(out), q, pool, table, 0, pos, range(len(LENS)), cos, sin)
+    g.check()
+    assert kernels.kv4_take_errors() == 0
+
+
+@pytest.mark.parametrize("n_q,n_kv,lens", [(20, 5, [5000, 4097, 1]), (16, 2, [9001]), (12, 4, [1234, 3000, 2048, 77]), (32, 8, [16000])])
+def test_long_contexts(cuda_lib, n_q, n_kv, lens):
+    """Every way of splitting gives the result: chosen, forced, and with a workspace that allows some splits or none."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(sum(lens))
+    most = max(lens)
+    table, pool = setup(rng, lens, n_kv, (most + 15) // 16, layers=2)
+    q = rng.standard_normal((len(lens), n_q * 128)).astype(np.float32)
+    pos = np.array(lens, np.int32) - 1
+    dq, dp, dpos, dt = dev(q), dev(pool), dev(pos), dev(table)
+    full = kernels.attention_kv4_workspace_bytes(len(lens), n_q, n_kv, most)
+    for split, room in ((0, full), (256, full), (1000, full), (0, full // 3), (0, 0), (most, 0)):
+        ws = torch.empty(max(room, 16), dtype=torch.uint8, device="cuda")[:room]
+        out = kernels.attention_kv4(dq, dp, dpos, layer=1, n_q=n_q, block_table=dt, max_len=most, split_keys=split, workspace=ws)
+        check(host(out), q, pool, table, 1, pos, range(len(lens)))
+    assert kernels.kv4_take_errors() == 0
+
+
+@pytest.mark.parametrize("scale_q,spread", [(1e-6, 1.0), (1.0, 1e-3), (1.0, 300.0), (30.0, 1.0), (0.0, 1.0), (1e4, 1e-4)])
+def test_magnitudes(cuda_lib, scale_q, spread):
+    """Queries and values far from 1: nothing overflows or fades in the 16-bit parts of the products."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(3)
+    lens = [33, 700]
+    table, pool = setup(rng, lens, 2, 44, spread=spread)
+    keys = ref.random_pool(rng, len(pool), 1, 2, 1.0)
+    pool[:, :, :, 0] = keys[:, :, :, 0]                                   # keys of ordinary size, values of `spread`
+    q = rng.standard_normal((2, 8 * 128)).astype(np.float32) * np.float32(scale_q)
+    pos = np.array(lens, np.int32) - 1
+    out = kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=8, block_table=dev(table))
+    for i, p in enumerate(pos):
+        k, v = ref.cached(pool, 0, table[i], p + 1)
+        want, bound = ref.attention(q[i].reshape(8, 128), k, v)
+        err = abs(host(out)[i].reshape(8, 128).astype(np.float64) - want)
+        assert (err <= bound).all(), float((err / bound).max())
+
+
+def test_values_that_grow_along_the_sequence(cuda_lib):
+    """The scale of the values rises by a factor of a million from the first key to the last, and falls in the second sequence."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(8)
+    n = 640
+    x = rng.standard_normal((2, n, 128)).astype(np.float32)
+    grow = np.exp(np.linspace(-7, 7, n)).astype(np.float32)[:, None]
+    rows_v = np.stack([ref.quantise(x[0] * grow), ref.quantise(x[1] * grow[::-1])])
+    rows_k = ref.quantise(rng.standard_normal((2, n, 128)).astype(np.float32))
+    pool = np.stack([rows_k, rows_v], 2).reshape(2, n // 16, 16, 2, 80).transpose(0, 1, 3, 2, 4).reshape(2 * n // 16, 1, 1, 2, 16, 80).copy()
+    table = np.arange(2 * n // 16, dtype=np.int32).reshape(2, -1)
+    q = rng.standard_normal((2, 4 * 128)).astype(np.float32) * 3
+    pos = np.full(2, n - 1, np.int32)
+    for split in (0, 128, 640):
+        out = kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=4, block_table=dev(table), split_keys=split)
+        check(host(out), q, pool, table, 0, pos, range(2))
+
+
+def test_one_key_far_above_the_others(cuda_lib):
+    """A score far above all others, at the first key, at the last, and growing scores (the running maximum moves at every step)."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(4)
+    n = 333
+    base = rng.standard_normal(128).astype(np.float32)
+    x = rng.standard_normal((3, n, 128)).astype(np.float32)
+    x[0, 0] = base * 6
+    x[1, n - 1] = base * 6
+    x[2] = base * np.linspace(-5, 5, n)[:, None].astype(np.float32) + 0.1 * x[2]
+    columns = (n + 15) // 16
+    rows = np.zeros((3, columns * 16, 2, 80), np.uint8)
+    rows[:, :n, 0] = ref.quantise(x)
+    rows[:, :n, 1] = ref.quantise(rng.standard_normal((3, n, 128)).astype(np.float32))
+    pool = rows.reshape(3 * columns, 16, 2, 80).transpose(0, 2, 1, 3).reshape(3 * columns, 1, 1, 2, 16, 80).copy()
+    table = np.arange(3 * columns, dtype=np.int32).reshape(3, -1)
+    q = np.tile(base, (3, 2)).astype(np.float32) * np.float32(0.3)
+    pos = np.full(3, n - 1, np.int32)
+    out = kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=2, block_table=dev(table))
+    check(host(out), q, pool, table, 0, pos, range(3))
+
+
+def test_rows_of_one_sequence_and_shared_blocks(cuda_lib):
+    """A draft's rows, each at its own position, from strided queries; tables that share blocks, as beams do; padding rows."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(12)
+    table, pool = setup(rng, [100, 100], 2, 7)
+    table[1, :5] = table[0, :5]
+    seq = np.array([0, 0, 0, 1, 1, 1, 0, 1], np.int32)
+    pos = np.array([95, 96, 97, 40, 98, 99, -1, -5], np.int32)
+    wide = rng.standard_normal((8, 12 * 128)).astype(np.float32)
+    d = dev(wide)
+    cos, sin = ref.rope(112)
+    out = kernels.attention_kv4(d[:, 128: 9 * 128], dev(pool), dev(pos), layer=0, n_q=8, block_table=dev(table), seq=dev(seq), rope_cos=dev(cos), rope_sin=dev(sin))
+    check(host(out), wide[:, 128: 9 * 128], pool, table, 0, pos, seq, cos, sin)
+    assert bool((out[6:] == 0).all())
+
+
+def test_indices_out_of_range(cuda_lib):
+    """A position past max_len or a sequence that is not there: the row stays as it was. A table entry out of range: its keys are left out."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(2)
+    lens = [60, 60, 60, 60]
+    table, pool = setup(rng, lens, 2, 4)
+    broken = table.copy()
+    broken[1, 2], broken[3, 0] = len(pool), -3
+    seq = np.array([0, 1, 2, 3, 7, -1], np.int32)
+    pos = np.array([59, 59, 64, 59, 3, 3], np.int32)
+    q = rng.standard_normal((6, 4 * 128)).astype(np.float32)
+    for split in (0, 128):
+        out = torch.full((6, 4 * 128), 5.0, device="cuda")
+        kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=4, block_table=dev(broken), seq=dev(seq), out=out, max_len=64, split_keys=split)
+        assert kernels.kv4_take_errors() == 2 and kernels.kv4_take_errors() == 0
+        got = host(out)
+        check(got[:1], q[:1], pool, table, 0, pos[:1], seq[:1])
+        assert (got[[2, 4, 5]] == 5.0).all()
+        for i, gone in ((1, 2), (3, 0)):
+            k, v = ref.cached(pool, 0, table[i], 60)
+            keep = np.r_[0: 16 * gone, 16 * gone + 16: 60]
+            want, bound = ref.attention(q[i].reshape(4, 128), k[:, keep], v[:, keep])
+            assert (abs(got[i].reshape(4, 128) - want) <= bound).all()
+    only_bad = np.full((1, 4), -1, np.int32)
+    out = kernels.attention_kv4(dev(q[:1]), dev(pool), dev(pos[:1]), layer=0, n_q=4, block_table=dev(only_bad))
+    assert kernels.kv4_take_errors() == 2 and bool((out == 0).all())
+
+
+def test_two_graphs_on_one_workspace_and_a_side_stream(cuda_lib):
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(21)
+    table, pool = setup(rng, [700, 650], 2, 44)
+    q = [rng.standard_normal((2, 4 * 128)).astype(np.float32) for _ in range(2)]
+    pos = np.array([699, 649], np.int32)
+    dq, dp, dpos, dt = [dev(x) for x in q], dev(pool), dev(pos), dev(table)
+    ws = torch.empty(kernels.attention_kv4_workspace_bytes(2, 4, 2, 704), dtype=torch.uint8, device="cuda")
+    graphs, outs = [], [torch.zeros(2, 4 * 128, device="cuda") for _ in range(2)]
+    side = torch.cuda.Stream()
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            for _ in range(2):
+                kernels.attention_kv4(dq[i], dp, dpos, layer=0, n_q=4, block_table=dt, out=outs[i], workspace=ws, split_keys=128, use_pdl=True)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        check(host(outs[i]), q[i], pool, table, 0, pos, range(2))
+        assert torch.equal(outs[i], kernels.attention_kv4(dq[i], dp, dpos, layer=0, n_q=4, block_table=dt, split_keys=128))
+    assert kernels.kv4_take_errors() == 0
+
+
+def test_pools_beyond_32_bits(cuda_lib):
+    """Blocks whose bytes lie past 2^31 and 2^32 of the pool's start."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(6)
+    per_block = 4 * 8 * 2560
+    blocks = (2 ** 32 + 2 ** 30) // per_block
+    pool = torch.zeros(blocks, 4, 8, 2, 16, 80, dtype=torch.uint8, device="cuda")
+    table = np.array([[blocks - 1, 2 ** 31 // per_block + 1, 2 ** 32 // per_block + 1, 0]], np.int32)
+    n = 60
+    k, v = (rng.standard_normal((n, 8 * 128)).astype(np.float32) for _ in range(2))
+    pos = np.arange(n, dtype=np.int32)
+    dt, dpos, seq = dev(table), dev(pos), torch.zeros(n, dtype=torch.int32, device="cuda")
+    kernels.kv4_append(dev(k), dev(v), pool, dpos, layer=3, block_table=dt, seq=seq)
+    rk, rv = kernels.kv4_read(pool, dpos, layer=3, block_table=dt, seq=seq)
+    assert np.array_equal(host(rk).reshape(n, 8, 128), ref.values(ref.quantise(k.reshape(n, 8, 128))).astype(np.float32))
+    small = host(pool[dt[0].long()])
+    q = rng.standard_normal((1, 16 * 128)).astype(np.float32)
+    out = kernels.attention_kv4(dev(q), pool, dev(np.array([n - 1], np.int32)), layer=3, n_q=16, block_table=dt)
+    check(host(out), q, small, np.arange(4)[None], 3, [n - 1], [0])
+    assert kernels.kv4_take_errors() == 0

@@ -1,0 +1,169 @@
+"""Beam selection against a full sort in 64 bits: parents and tokens equal, scores rounded once."""
+import numpy as np
+import pytest
+import torch
+import kv4_reference as ref
+from gpu_helpers import Guarded, dev, host
+
+pytestmark = pytest.mark.gpu
+LOWEST = np.finfo(np.float32).min
+
+
+def check(logits, scores, beams, k, finished=None, eos=0, logits_dev=None):
+    from tenzo_b200 import kernels
+    want_parent, want_token, want_score = ref.select(logits, scores, beams, k, finished, eos)
+    g, groups = Guarded(), len(scores) // beams
+    ws = g.empty((int(kernels.load_library().tenzo_cuda_beam_select_workspace_bytes(groups, beams, logits.shape[1], k)),), torch.uint8)
+    got = kernels.beam_select(dev(logits) if logits_dev is None else logits_dev, dev(scores), beams=beams, k=k, finished=None if finished is None else dev(finished),
+                              eos=eos, workspace=ws)
+    parent, token, score = (host(t) for t in got)
+    g.check()
+    assert np.array_equal(parent, want_parent) and np.array_equal(token, want_token), (parent, want_parent, token, want_token)
+    both = np.isfinite(want_score)
+    assert np.array_equal(both, np.isfinite(score)) and np.array_equal(score[~both], want_score[~both].astype(np.float32))
+    # rounded once to fp32 (2^-24), and the sum of exponentials is good to 2^-30 or better
+    assert (abs(score[both] - want_score[both]) <= 2.0 ** -24 * abs(want_score[both]) + 2.0 ** -30).all()
+    return parent, token, score
+
+
+@pytest.mark.parametrize("groups,beams,vocab,k", [
+    (1, 1, 1, 1), (1, 1, 2, 2), (2, 3, 5, 15), (1, 4, 1024, 8), (3, 2, 1000, 4), (2, 5, 8191, 10), (1, 3, 8192, 3), (1, 3, 8193, 6), (2, 32, 4001, 64), (1, 1, 50001, 64),
+    (1, 4, 128256, 8), (5, 8, 30011, 16), (70, 2, 2048, 4), (1, 16, 333, 32), (300, 1, 77, 1), (2, 12, 50001, 24), (1, 2, 300007, 4),
+])
+def test_shapes(cuda_lib, groups, beams, vocab, k):
+    rng = np.random.default_rng(vocab + k)
+    logits = (rng.standard_normal((groups * beams, vocab)) * 2.5).astype(np.float32)
+    scores = (-20 - 3 * rng.random(groups * beams)).astype(np.float32)
+    check(logits, scores, beams, k)
+
+
+@pytest.mark.parametrize("vocab", [64, 1023, 20000, 128256])
+def test_masked_tokens(cuda_lib, vocab):
+    """Masks of -infinity, of the lowest number and of NaN; rows with fewer tokens left than are asked for, with one, and with none."""
+    rng = np.random.default_rng(vocab)
+    beams, k = 6, 12
+    logits = (rng.standard_normal((2 * beams, vocab)) * 3).astype(np.float32)
+    logits[0, rng.random(vocab) < 0.9] = -np.inf
+    logits[1] = -np.inf
+    logits[2] = -np.inf
+    logits[2, vocab - 1] = 1.5
+    logits[3, rng.random(vocab) < 0.5] = np.nan
+    logits[4] = LOWEST
+    logits[4, [3, 5]] = -2.0
+    logits[5] = np.nan
+    logits[6] = LOWEST                                   # every token alike: uniform
+    logits[7, 10:] = -np.inf
+    logits[8] = -np.inf
+    logits[8, : 5] = [1, 1, 1, 1, 1]
+    scores = (-5 * rng.random(2 * beams)).astype(np.float32)
+    check(logits, scores, beams, k)
+
+
+def test_rows_with_nothing_left(cuda_lib):
+    """All beams masked, dead (score -inf or NaN), or both: the lowest indices, at -infinity."""
+    rng = np.random.default_rng(0)
+    logits = rng.standard_normal((9, 500)).astype(np.float32)
+    logits[:3] = -np.inf
+    scores = np.array([-1, -2, -3, -np.inf, -np.inf, -np.inf, -np.inf, np.nan, -4], np.float32)
+    logits[8, 3:] = -np.inf
+    parent, token, score = check(logits, scores, 3, 6)
+    assert (score[:2] == -np.inf).all() and (parent[:2] == 0).all() and (token[:2] == np.arange(6)).all()
+    assert (score[2, 3:] == -np.inf).all()
+
+
+def test_ties(cuda_lib):
+    """Equal logits within a row, equal rows, zeros of both signs, first steps (all beams alike, all but one dead): the lowest index first."""
+    rng = np.random.default_rng(1)
+    vocab = 9001
+    row = np.round(rng.standard_normal(vocab) * 2).astype(np.float32)
+    same = np.tile(row, (4, 1))
+    check(same, np.full(4, -1.0, np.float32), 4, 8)
+    check(same, np.array([0, -np.inf, -np.inf, -np.inf], np.float32), 4, 8)
+    check(np.zeros((4, vocab), np.float32), np.zeros(4, np.float32), 4, 64)
+    check(np.full((4, vocab), -7.25, np.float32), np.array([-1, 0, 0, -1], np.float32), 4, 64)
+    signs = np.where(rng.random((2, vocab)) < 0.5, -0.0, 0.0).astype(np.float32)
+    signs[:, ::3] = -1
+    check(signs, np.zeros(2, np.float32), 2, 64)
+
+
+def test_many_large_values_side_by_side(cuda_lib):
+    """The largest logits lie next to one another, or a fixed distance apart (whatever way the row is dealt out, some threads hold many), ascending or descending."""
+    rng = np.random.default_rng(2)
+    vocab = 20011
+    for step in (1, 4, 32, 128, 256, 512, 1024, 2048):
+        logits = rng.standard_normal((4, vocab)).astype(np.float32)
+        at = (7 + step * np.arange(2000)) % vocab
+        logits[:, at] += 50 + np.arange(2000, dtype=np.float32) / 64
+        logits[2:] = logits[2:, ::-1]
+        check(logits, np.zeros(4, np.float32), 2, 64)
+    ramp = np.arange(vocab, dtype=np.float32)
+    check(np.stack([ramp, -ramp, ramp[::-1], np.sin(ramp)]), np.zeros(4, np.float32), 4, 64)
+
+
+def test_extreme_numbers(cuda_lib):
+    rng = np.random.default_rng(3)
+    logits = (rng.standard_normal((4, 3000)) * 1e4).astype(np.float32)
+    logits[1] = rng.standard_normal(3000).astype(np.float32) * np.float32(1e-40)        # denormals
+    logits[2, 17] = np.inf
+    logits[2, 900] = np.inf
+    logits[3, 5] = np.finfo(np.float32).max
+    check(logits, np.array([-1e6, 0, -1e30, 3.0], np.float32), 4, 8)
+    check(logits, np.zeros(4, np.float32), 1, 8)
+
+
+def test_finished_beams(cuda_lib):
+    rng = np.random.default_rng(4)
+    beams, vocab, k = 4, 700, 8
+    logits = rng.standard_normal((3 * beams, vocab)).astype(np.float32)
+    scores = (-30 + 5 * rng.random(3 * beams)).astype(np.float32)
+    finished = np.zeros(3 * beams, np.int32)
+    finished[[0, 2, 3]] = 1
+    finished[4:8] = 5                                   # all of a group: their end tokens, then the lowest indices at -infinity
+    scores[2], scores[3] = scores[0], -40.0
+    for eos in (0, 5, 2, vocab - 1):
+        check(logits, scores, beams, k, finished, eos)
+    scores[4] = -np.inf
+    check(logits, scores, beams, k, finished, 9)
+    check(logits[:, :3].copy(), scores, beams, 6, finished, 2)
+
+
+def test_beams_whose_scores_lie_close(cuda_lib):
+    """Long sums: 32 bits hold steps of 2^-12 there, the order goes by 64."""
+    rng = np.random.default_rng(5)
+    logits = rng.standard_normal((8, 5000)).astype(np.float32)
+    logits[1:] = logits[0] + rng.standard_normal((7, 5000)).astype(np.float32) * np.float32(1e-5)
+    check(logits, np.full(8, -30000.0, np.float32), 8, 16)
+
+
+def test_rows_of_a_wider_buffer(cuda_lib):
+    rng = np.random.default_rng(6)
+    for offset, width in ((0, 3001), (1, 3004), (4, 3004)):
+        wide = rng.standard_normal((6, width + 8)).astype(np.float32)
+        d = dev(wide)
+        view = wide[:, offset: offset + 2999]
+        check(view, np.zeros(6, np.float32), 3, 6, logits_dev=d[:, offset: offset + 2999])
+
+
+def test_graph_and_side_stream(cuda_lib):
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(7)
+    a, b = ((rng.standard_normal((4, 40000))).astype(np.float32) for _ in range(2))
+    scores = np.zeros(4, np.float32)
+    d, s = dev(a), dev(scores)
+    kernels.beam_select(d, s, beams=4, k=8)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        for _ in range(2):
+            parent, token, _ = kernels.beam_select(d, s, beams=4, k=8, use_pdl=True)
+    for x in (a, b, a):
+        d.copy_(dev(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ref.select(x, scores, 4, 8)
+        assert np.array_equal(host(parent), want[0]) and np.array_equal(host(token), want[1])
+
+
+def test_no_groups(cuda_lib):
+    from tenzo_b200 import kernels
+    parent, token, score = kernels.beam_select(torch.empty(0, 10, device="cuda"), torch.empty(0, device="cuda"), beams=2, k=3)
+    assert parent.shape == token.shape == score.shape == (0, 3)
