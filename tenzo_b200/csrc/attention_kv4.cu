@@ -1,77 +1,517 @@
 // GQA decode attention over the 4-bit paged cache (kv4.cuh): softmax(q K^T / sqrt(128)) V over the keys 0 .. pos of a row's sequence,
 // the query rotated on the way.
 //
-// One warp per query head and share of the keys: a lane holds four dims, the warps of a CTA join their (maximum, sum, output).
+//   * The keys of a (row, kv head) are split over CTAs and, inside a CTA, over four warps that never wait for one another: each streams
+//     steps of 32 keys, two pages of 2560 bytes by one bulk copy each, through a ring of its own and keeps a running
+//     (maximum, sum, output) per query head. The triples meet by log-sum-exp, first the warps', then the splits' in a second kernel.
+//   * A nibble in the low bits of a 16-bit word is the fp16 number code * 2^-24, one field further up code * 2^-20; one packed multiplication
+//     makes two of them normal numbers. (The tensor cores take subnormal operands too, exactly, but line the products up by the
+//     exponent they are written with: sums lose the leading zeros' bits, 1e-5 instead of 4e-7 over 100 keys.) With
+//     value = minimum + scale * code per group of 32 dims,
+//       q.k   = sum_g scale_g (q_g . c_g) + minimum_g (sum of q over g)
+//       p.v_d = sum_t (p_t scale_tg) c_td + sum_t p_t minimum_tg
+//     the products with codes are one chain of MMAs a group, whose sums (or weights) take the scale in fp32; the terms with the minima
+//     are one MMA more, over the parameters as they lie.
+//   * The other operands have 22 bits: queries and weights enter as two fp16 parts each (the query scaled to a maximum near 2^7, the
+//     weights to at most 2^14 with the largest scale of the values seen so far). Outputs agree with 64 bits to a few 1e-7.
+//   * S = Q K^T has heads as rows (rows 0-7 the first parts, 8-15 the second, so a lane adds the two itself) and its accumulators are, lane
+//     by lane, the weights' B operand of O^T = V^T P^T, whose columns are heads. Up to four heads a kv head, columns 4-7 carry the
+//     weights' second parts; with five to eight a second MMA does.
+#include "attn_common.cuh"
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>
 
 namespace tz {
 
-constexpr int kA4Warps = 8, kA4Hd = 128;
+constexpr int kA4Hd = 128, kA4Warps = 4, kA4Threads = kA4Warps * 32;
+constexpr int kA4Step = 32;                              // keys a warp takes at a time
+constexpr int kA4Stages = 2, kA4StepBytes = 2 * kK4Page;
+constexpr int kA4Resident = 4;                           // CTAs an SM
 
 __device__ int g_kv4_attention_error = 0;
 
-__global__ void __launch_bounds__(kA4Warps * 32) attention_kv4_simple_kernel(const tenzo_attention_kv4_args a) {
-    __shared__ float s_q[kA4Hd], s_o[kA4Warps][kA4Hd], s_m[kA4Warps], s_l[kA4Warps];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y, row = blockIdx.x, kvh = head / (a.n_q / a.cache.n_kv);
-    if (a.use_pdl) {
-        pdl_launch_dependents();
-        pdl_wait();
-    }
+struct A4Launch {
+    tenzo_attention_kv4_args a;
+    int n_splits, split_keys, group, head_blocks;        // query heads a kv head, and blocks of them that a CTA takes
+    float* part_o;                                       // [row][head][split][128]
+    float2* part_ml;                                     // [row][head][split]: maximum (log2), sum
+};
+
+__device__ __forceinline__ float a4_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t a4_pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float a4_low(uint32_t pair) { return __low2float(*reinterpret_cast<const __half2*>(&pair)); }
+__device__ __forceinline__ float a4_high(uint32_t pair) { return __high2float(*reinterpret_cast<const __half2*>(&pair)); }
+// D = A B (+ D); the accumulators of the first form start at zero.
+__device__ __forceinline__ void a4_mma16_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void a4_mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void a4_mma8_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
+}
+__device__ __forceinline__ f32x2 a4_mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 a4_fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+// The eleven leading bits of two numbers as fp16 (towards zero).
+__device__ __forceinline__ uint32_t a4_pack_cut(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// Codes of a word as two fp16 numbers (code - 8) * 2^-9: nibbles 0 and 4, nibbles 1 and 5.
+__device__ __forceinline__ uint32_t a4_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+constexpr uint32_t kMinus8 = 0xa400a400u;                                                     // -2^-6
+__device__ __forceinline__ uint32_t a4_even(uint32_t w) { return a4_fma(w & 0x000f000fu, 0x78007800u, kMinus8); }    // code * 2^-24, times 2^15
+__device__ __forceinline__ uint32_t a4_odd(uint32_t w) { return a4_fma(w & 0x00f000f0u, 0x68006800u, kMinus8); }     // code * 2^-20, times 2^11
+
+// Rows that are left alone (a position or a sequence out of range); the same rule in both kernels.
+__device__ __forceinline__ bool a4_refused(const tenzo_attention_kv4_args& a, int pos, int seq) { return pos >= a.max_len || seq < 0 || seq >= a.cache.table_rows; }
+
+template <int HB>
+__global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(const A4Launch L) {
+    static_assert(HB == 4 || HB == 8, "heads a CTA takes");
+    const tenzo_attention_kv4_args& a = L.a;
+    extern __shared__ __align__(128) unsigned char a4_smem[];
+    __shared__ float s_q[HB][kA4Hd], s_qsum[HB][4], s_f[HB], s_ml[kA4Warps][HB][2];
+    __shared__ uint64_t s_bar[kA4Warps][kA4Stages];
+    __shared__ __align__(16) float s_scale[kA4Warps][2][kA4Step / 2][4][2];      // a step's scales, keys and values: [pair of keys][group][key]
+    __shared__ __align__(16) uint4 s_centre[kA4Warps][kA4Step];                  // minimum + 8 scale of the values: four first parts, four second ones
+    __shared__ __align__(16) uint4 s_qa[8][32];          // the queries' A fragments, the same in every warp
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int row = blockIdx.x / L.n_splits, split = blockIdx.x % L.n_splits;
+    const int kvh = blockIdx.y / L.head_blocks, head0 = blockIdx.y % L.head_blocks * HB, heads = min(HB, L.group - head0);
+    if (lane == 0)
+        for (int s = 0; s < kA4Stages; ++s) mbar_init(&s_bar[warp][s], 1);
+    mbar_init_fence();
+    if (a.use_pdl || L.n_splits > 1) pdl_launch_dependents();       // the second kernel waits for this one whatever its neighbours do
+    if (a.use_pdl) pdl_wait();
     const int pos = a.pos[row], seq = a.seq ? a.seq[row] : row;
-    float* out = a.out + ((size_t)row * a.n_q + head) * kA4Hd;
-    if (pos >= a.max_len || seq < 0 || seq >= a.cache.table_rows) {
+    if (a4_refused(a, pos, seq)) {
         if (tid == 0) atomicOr(&g_kv4_attention_error, kK4ErrIndex);
         return;
     }
-    const float* q = a.q + (size_t)row * a.q_stride + (size_t)head * kA4Hd;
-    if (tid < 64) {
-        const float x0 = q[tid], x1 = q[tid + 64];
-        const bool turn = a.rope_cos && pos >= 0;
-        const float c = turn ? a.rope_cos[(size_t)pos * 64 + tid] : 1.0f, s = turn ? a.rope_sin[(size_t)pos * 64 + tid] : 0.0f;
-        s_q[tid] = __fmaf_rn(x0, c, -(x1 * s));
-        s_q[tid + 64] = __fmaf_rn(x0, s, x1 * c);
+    const int c_begin = split * L.split_keys, c_end = min(pos + 1, c_begin + L.split_keys);
+    float* out = a.out + ((size_t)row * a.n_q + (size_t)kvh * L.group + head0) * kA4Hd;
+    if (c_begin >= c_end) {                              // the second kernel knows which splits there are
+        if (L.n_splits == 1)
+            for (int i = tid; i < heads * kA4Hd; i += kA4Threads) out[i] = 0.0f;
+        return;
     }
-    __syncthreads();
-    float qv[4], o[4] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) qv[j] = s_q[4 * lane + j] * 0.08838834764831845f;
-    for (int t = warp; t <= pos; t += kA4Warps) {
-        const int block = a.cache.block_table[(size_t)seq * a.cache.table_stride + t / kK4Slots];
-        if (block < 0 || block >= a.cache.n_blocks) {
-            if (lane == 0) atomicOr(&g_kv4_attention_error, kK4ErrIndex);
-            continue;
+    const int steps = (c_end - c_begin + kA4Step - 1) / kA4Step;
+    const int my_steps = warp < steps ? (steps - warp + kA4Warps - 1) / kA4Warps : 0;
+    const int* table = a.cache.block_table + (size_t)seq * a.cache.table_stride + c_begin / kK4Slots;
+    const int pages = (c_end - c_begin + kK4Slots - 1) / kK4Slots;
+    const uint8_t* pool = a.cache.pool + kv4_page(a.cache, a.layer, kvh, 0);
+    const size_t block_bytes = (size_t)a.cache.n_layers * a.cache.n_kv * kK4Page;
+    unsigned char* ring = a4_smem + (size_t)warp * kA4Stages * kA4StepBytes;
+    uint64_t* bar = s_bar[warp];
+
+    // Table entries of sixteen of the warp's steps, one a lane (-1: no such page, or an entry out of range), and of the next sixteen.
+    auto entries = [&](int k0) {
+        const int page = 2 * (warp + (k0 + (lane >> 1)) * kA4Warps) + (lane & 1);
+        int id = -1;
+        if (page < pages) {
+            id = __ldg(table + page);
+            if (id < 0 || id >= a.cache.n_blocks) {
+                atomicOr(&g_kv4_attention_error, kK4ErrIndex);
+                id = -1;
+            }
         }
-        const uint8_t* kr = a.cache.pool + kv4_page(a.cache, a.layer, kvh, block) + (size_t)(t % kK4Slots) * kK4Row;
-        const uint8_t* vr = kr + kK4Half;
-        const uint32_t kc = reinterpret_cast<const uint16_t*>(kr)[lane], vc = reinterpret_cast<const uint16_t*>(vr)[lane];
-        const float2 kp = __half22float2(reinterpret_cast<const __half2*>(kr + kK4Codes)[lane >> 3]);
-        const float2 vp = __half22float2(reinterpret_cast<const __half2*>(vr + kK4Codes)[lane >> 3]);
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s = __fmaf_rn(qv[j], __fmaf_rn(kp.x, (float)((kc >> (4 * j)) & 15u), kp.y), s);
-        s = warp_sum(s);
-        const float n = fmaxf(m, s), f = expf(m - n), e = expf(s - n);
-        m = n;
-        l = __fmaf_rn(l, f, e);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = __fmaf_rn(o[j], f, e * __fmaf_rn(vp.x, (float)((vc >> (4 * j)) & 15u), vp.y));
+        return id;
+    };
+    int ids = entries(0), ids_next = entries(16);
+    unsigned there = 0;                                  // two bits a stage: which of its pages were copied
+    auto issue = [&](int k) {                            // the warp's k-th step into stage k % kA4Stages
+        const int st = k % kA4Stages;
+        const int id0 = __shfl_sync(0xffffffffu, ids, 2 * (k & 15)), id1 = __shfl_sync(0xffffffffu, ids, 2 * (k & 15) + 1);
+        there = (there & ~(3u << (2 * st))) | ((id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u)) << (2 * st);
+        if (lane == 0) {
+            unsigned char* to = ring + (size_t)st * kA4StepBytes;
+            mbar_expect_tx(&bar[st], ((id0 >= 0) + (id1 >= 0)) * (unsigned)kK4Page);
+            if (id0 >= 0) bulk_g2s(to, pool + (size_t)id0 * block_bytes, kK4Page, &bar[st]);
+            if (id1 >= 0) bulk_g2s(to + kK4Page, pool + (size_t)id1 * block_bytes, kK4Page, &bar[st]);
+        }
+        if ((k & 15) == 15) {
+            ids = ids_next;
+            ids_next = entries(k + 17);
+        }
+    };
+    for (int k = 0; k < kA4Stages && k < my_steps; ++k) issue(k);
+
+    // ---- the heads' queries: rotated, scaled by a power of two to a maximum in [2^7, 2^8), and their sums over each group of dims --------
+    const float* q = a.q + (size_t)row * a.q_stride + ((size_t)kvh * L.group + head0) * kA4Hd;
+    for (int i = tid; i < HB * 64; i += kA4Threads) {
+        const int h = i >> 6, d = i & 63;
+        float r0 = 0.0f, r1 = 0.0f;
+        if (h < heads) {
+            const float x0 = __ldcg(q + h * kA4Hd + d), x1 = __ldcg(q + h * kA4Hd + d + 64);
+            r0 = x0;
+            r1 = x1;
+            if (a.rope_cos) {
+                const float c = __ldg(a.rope_cos + (size_t)pos * 64 + d), s = __ldg(a.rope_sin + (size_t)pos * 64 + d);
+                r0 = __fmaf_rn(x0, c, -(x1 * s));
+                r1 = __fmaf_rn(x0, s, x1 * c);
+            }
+        }
+        s_q[h][d] = r0;
+        s_q[h][d + 64] = r1;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s_o[warp][4 * lane + j] = o[j];
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
     __syncthreads();
-    if (tid < kA4Hd) {
-        float top = -INFINITY, sum = 0.0f, v = 0.0f;
-        for (int w = 0; w < kA4Warps; ++w) top = fmaxf(top, s_m[w]);
+    for (int h = warp; h < HB; h += kA4Warps) {
+        float4 v = *reinterpret_cast<const float4*>(&s_q[h][4 * lane]);
+        const float m = warp_max(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        const int e = max(15, (int)(__float_as_uint(m) >> 23));
+        const float up = __uint_as_float((uint32_t)(127 + 7 - (e - 127)) << 23), down = __uint_as_float((uint32_t)(127 - 7 + (e - 127)) << 23);
+        v.x *= up; v.y *= up; v.z *= up; v.w *= up;
+        *reinterpret_cast<float4*>(&s_q[h][4 * lane]) = v;
+        float sum = (v.x + v.y) + (v.z + v.w);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if ((lane & 7) == 0) s_qsum[h][lane >> 3] = sum;
+        if (lane == 0) s_f[h] = down * (512.0f * 0.08838834764831845f * 1.4426950408889634f);  // the unit of the products, 1/sqrt(128) and log2(e)
+    }
+    __syncthreads();
+    const int mine = g & (HB - 1);                       // the head of rows g and g + 8
+    for (int i = warp; i < 8; i += kA4Warps) {           // group i / 2, nibbles 2 (i % 2) and + 1 of the lane's word
+        const float* p = &s_q[mine][32 * (i >> 1) + 8 * t + 2 * (i & 1)];
+        const float x[4] = {p[0], p[4], p[1], p[5]};
+        const uint32_t a0 = a4_pack(x[0], x[1]), a2 = a4_pack(x[2], x[3]);
+        s_qa[i][lane] = make_uint4(a0, a4_pack(x[0] - a4_low(a0), x[1] - a4_high(a0)), a2, a4_pack(x[2] - a4_low(a2), x[3] - a4_high(a2)));
+    }
+    uint32_t qm[2];
+    {                                                    // beside the scale (8-fold), beside the minimum; in units of 2^9, as the codes
+        const float sum = s_qsum[mine][t] * 0.001953125f, first = __half2float(__float2half_rn(sum));
+        qm[0] = a4_pack(8.0f * first, first);
+        qm[1] = a4_pack(8.0f * (sum - first), sum - first);
+    }
+    const float f = s_f[mine];
+    __syncthreads();
+
+    float m_run = -INFINITY, top = 0.0f, l_run = 0.0f;   // head `mine`: largest product so far, its score (log2) less 14, this lane's share of the sum
+    float vs = 1.0f;                                     // values' scales are multiplied by this power of two, to at most 1
+    uint32_t v_most = 0;                                 // the largest exponent of a scale so far, as fp16 bits
+    f32x2 acc[8][2], accm = 0;                           // group i / 2: dims 4g + 2 (i % 2), and + 1; heads 2t, 2t + 1
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = 0;
+    const uint32_t cut = HB == 8 || g >= 4 ? 0xffffe000u : 0u;                                  // columns 4-7: what the first eleven bits leave
+    const f32x2 minus = pack2(-1.0f, -1.0f), f2 = pack2(f, f);
+    bool gave_up = false;
+
+    for (int k = 0; k < my_steps; ++k) {
+        const int st = k % kA4Stages, t0 = c_begin + (warp + k * kA4Warps) * kA4Step;
+        unsigned char* step = ring + (size_t)st * kA4StepBytes;
+        if (!mbar_wait_bounded(&bar[st], (unsigned)(k / kA4Stages) & 1u)) gave_up = true;
+        const unsigned copied = (there >> (2 * st)) & 3u;
+        const bool ragged = t0 + kA4Step > c_end || copied != 3u;
+        unsigned char* own = step + (lane >> 4) * kK4Page + (lane & 15) * kK4Row + kK4Codes;    // the parameters of key t0 + lane
+        if (ragged) {                                    // keys that do not count: parameters of zero, whatever lies there
+            if (t0 + lane >= c_end || !((copied >> (lane >> 4)) & 1u)) {
+                *reinterpret_cast<uint4*>(own) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(own + kK4Half) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");                   // a later copy into the stage comes after these
+            }
+            __syncwarp();
+        }
+        // ---- the step's scales in fp32, one key a lane ---------------------------------------------------------------------
+        bool v_grown;
+        float ratio = 1.0f;
+        {
+            const uint4 pk = *reinterpret_cast<const uint4*>(own), pv = *reinterpret_cast<const uint4*>(own + kK4Half);
+            const uint32_t v_max = __reduce_max_sync(0xffffffffu, max(max(pv.x & 0x7c00u, pv.y & 0x7c00u), max(pv.z & 0x7c00u, pv.w & 0x7c00u)));
+            v_grown = v_max > v_most || k == 0;
+            if (v_grown) {                               // a scale below 2^(e - 14) times 2^(14 - e) is below 1
+                v_most = v_max;
+                const float now = __uint_as_float((127u + 14u - max(v_max >> 10, 1u)) << 23);
+                ratio = k == 0 ? 1.0f : now / vs;
+                vs = now;
+            }
+            float* ks = &s_scale[warp][0][lane >> 1][0][lane & 1];
+            float* vt = &s_scale[warp][1][lane >> 1][0][lane & 1];
+            ks[0] = a4_low(pk.x); ks[2] = a4_low(pk.y); ks[4] = a4_low(pk.z); ks[6] = a4_low(pk.w);
+            const float sv[4] = {a4_low(pv.x), a4_low(pv.y), a4_low(pv.z), a4_low(pv.w)};
+            vt[0] = sv[0] * vs; vt[2] = sv[1] * vs; vt[4] = sv[2] * vs; vt[6] = sv[3] * vs;
+            const float c[4] = {__fmaf_rn(8.0f, sv[0], a4_high(pv.x)), __fmaf_rn(8.0f, sv[1], a4_high(pv.y)), __fmaf_rn(8.0f, sv[2], a4_high(pv.z)),
+                                __fmaf_rn(8.0f, sv[3], a4_high(pv.w))};
+            const uint32_t c01 = a4_pack(c[0], c[1]), c23 = a4_pack(c[2], c[3]);
+            s_centre[warp][lane] = make_uint4(c01, c23, a4_pack(c[0] - a4_low(c01), c[1] - a4_high(c01)), a4_pack(c[2] - a4_low(c23), c[3] - a4_high(c23)));
+            __syncwarp();
+        }
+        // ---- products with the keys: columns are eight keys a tile ----------------------------------------------------------
+        f32x2 x[4];
+        const unsigned char* kr = step + g * kK4Row + 4 * t;
+        auto tile = [](int nt) { return (nt >> 1) * kK4Page + (nt & 1) * 8 * kK4Row; };
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+            float c[4];
+            a4_mma8_new(c, qm[0], qm[1], *reinterpret_cast<const uint32_t*>(kr + tile(nt) + kK4Codes));
+            x[nt] = add2(pack2(c[0], c[1]), pack2(c[2], c[3]));
+        }
+#pragma unroll
+        for (int gr = 0; gr < 4; ++gr) {
+            const uint4 qa = s_qa[2 * gr][lane], qb = s_qa[2 * gr + 1][lane];
+            const uint32_t a0[4] = {qa.x, qa.y, qa.z, qa.w}, a1[4] = {qb.x, qb.y, qb.z, qb.w};
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) {
+                uint32_t w = *reinterpret_cast<const uint32_t*>(kr + tile(nt) + 16 * gr);
+                float c[4];
+                a4_mma16_new(c, a0, a4_even(w), a4_odd(w));
+                w >>= 8;
+                a4_mma16(c, a1, a4_even(w), a4_odd(w));
+                x[nt] = a4_fma2(*reinterpret_cast<const f32x2*>(&s_scale[warp][0][4 * nt + t][gr][0]), add2(pack2(c[0], c[1]), pack2(c[2], c[3])), x[nt]);
+            }
+        }
+        float s[4][2];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) unpack2(x[nt], s[nt][0], s[nt][1]);
+        if (ragged) {
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (t0 + nt * 8 + 2 * t + j >= c_end || !((copied >> (nt >> 1)) & 1u)) s[nt][j] = -INFINITY;
+                x[nt] = pack2(s[nt][0], s[nt][1]);
+            }
+        }
+        // ---- the running maximum ---------------------------------------------------------------------------------------------
+        float mx = s[0][0];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) mx = fmaxf(mx, fmaxf(s[nt][0], s[nt][1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (__any_sync(0xffffffffu, mx > m_run || v_grown)) {
+            float alpha = 1.0f;
+            if (mx > m_run) {
+                const float now = __fmaf_rn(mx, f, -14.0f);
+                alpha = m_run == -INFINITY ? 0.0f : a4_ex2(top - now);
+                m_run = mx;
+                top = now;
+            }
+            l_run *= alpha;
+            const f32x2 a01 = pack2(__shfl_sync(0xffffffffu, alpha, 8 * t), __shfl_sync(0xffffffffu, alpha, 8 * t + 4));
+            accm = a4_mul2(accm, a01);
+            const f32x2 scaled = a4_mul2(a01, pack2(ratio, ratio));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                acc[i][0] = a4_mul2(acc[i][0], scaled);
+                acc[i][1] = a4_mul2(acc[i][1], scaled);
+            }
+        }
+        // ---- weights (2^14-fold) and O^T += V^T P^T --------------------------------------------------------------------------
+        const f32x2 down = pack2(-top, -top);
+        f32x2 e[4];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+            float e0, e1;
+            unpack2(a4_fma2(x[nt], f2, down), e0, e1);
+            e0 = a4_ex2(e0);
+            e1 = a4_ex2(e1);
+            l_run += e0 + e1;
+            e[nt] = pack2(e0, e1);
+        }
+        // The two fp16 parts of a pair of weights: the first eleven bits, and what they leave (cut off in turn: 2^-22 less on average,
+        // in all products alike).
+        auto parts = [&](f32x2 w, uint32_t& first, uint32_t& second) {
+            float w0, w1, r0, r1;
+            unpack2(w, w0, w1);
+            unpack2(a4_fma2(pack2(__uint_as_float(__float_as_uint(w0) & cut), __uint_as_float(__float_as_uint(w1) & cut)), minus, w), r0, r1);
+            if (HB == 8) {
+                first = a4_pack_cut(w0, w1);
+                second = a4_pack_cut(r0, r1);
+            } else {
+                first = a4_pack_cut(r0, r1);             // columns 0-3 nothing was taken off, columns 4-7 the first part
+            }
+        };
+        uint32_t b[4], c[4];
+        auto product = [&](float (&o)[4], const uint32_t (&v0)[4], const uint32_t (&v1)[4]) {       // the step's 32 keys
+            a4_mma16_new(o, v0, b[0], b[1]);
+            a4_mma16(o, v1, b[2], b[3]);
+            if (HB == 8) {
+                a4_mma16(o, v0, c[0], c[1]);
+                a4_mma16(o, v1, c[2], c[3]);
+            }
+        };
+        {
+            uint32_t v0[4] = {}, v1[4] = {};
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(v0[0]), "=r"(v0[2]), "=r"(v1[0]), "=r"(v1[2]) : "r"(smem_addr(&s_centre[warp][lane])) : "memory");
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) parts(e[nt], b[nt], c[nt]);
+            float m[4];
+            product(m, v0, v1);
+            accm = add2(accm, pack2(m[0], m[1]));
+        }
+        const uint32_t at = smem_addr(step) + (uint32_t)((lane >> 4) * kK4Page + kK4Half + (8 * ((lane >> 3) & 1) + (lane & 7)) * kK4Row);
+#pragma unroll
+        for (int gr = 0; gr < 4; ++gr) {
+            uint32_t r[4];                               // the tiles' keys; dims 32 gr + 4g ..
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at + 16 * gr) : "memory");
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) parts(a4_mul2(e[nt], *reinterpret_cast<const f32x2*>(&s_scale[warp][1][4 * nt + t][gr][0])), b[nt], c[nt]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t v0[4] = {a4_even(r[0]), a4_odd(r[0]), a4_even(r[1]), a4_odd(r[1])};
+                const uint32_t v1[4] = {a4_even(r[2]), a4_odd(r[2]), a4_even(r[3]), a4_odd(r[3])};
+                float o[4];                              // added in fp32: the tensor cores' own sums are cut off, not rounded
+                product(o, v0, v1);
+                acc[2 * gr + i][0] = add2(acc[2 * gr + i][0], pack2(o[0], o[1]));
+                acc[2 * gr + i][1] = add2(acc[2 * gr + i][1], pack2(o[2], o[3]));
+#pragma unroll
+                for (int n = 0; n < 4; ++n) r[n] >>= 8;
+            }
+        }
+        __syncwarp();                                    // every lane is done with the stage and the scales
+        if (k + kA4Stages < my_steps) issue(k + kA4Stages);
+    }
+    if (gave_up && lane == 0) atomicOr(&g_kv4_attention_error, kK4ErrWait);
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+
+    // ---- the warps' outputs in one unit, then their triples into one --------------------------------------------------------
+    __syncthreads();                                     // all rings are idle: reuse them
+    float* w_o = reinterpret_cast<float*>(a4_smem);      // [warp][HB][128]
+    float am[2];
+    unpack2(accm, am[0], am[1]);
+    const float unit = 512.0f / vs;
+#pragma unroll
+    for (int gr = 0; gr < 4; ++gr) {
+        const float m0 = __shfl_sync(0xffffffffu, am[0], 4 * gr + t) + __shfl_sync(0xffffffffu, am[0], 16 + 4 * gr + t);
+        const float m1 = __shfl_sync(0xffffffffu, am[1], 4 * gr + t) + __shfl_sync(0xffffffffu, am[1], 16 + 4 * gr + t);
+        float o[2][4];                                   // [head 2t, 2t + 1][dims 32 gr + 4g ..]
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float c[4];
+            unpack2(acc[2 * gr + i][0], c[0], c[1]);
+            unpack2(acc[2 * gr + i][1], c[2], c[3]);
+            o[0][2 * i] = __fmaf_rn(c[0], unit, m0);
+            o[1][2 * i] = __fmaf_rn(c[1], unit, m1);
+            o[0][2 * i + 1] = __fmaf_rn(c[2], unit, m0);
+            o[1][2 * i + 1] = __fmaf_rn(c[3], unit, m1);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (HB == 4) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) o[h][d] += __shfl_xor_sync(0xffffffffu, o[h][d], 2);
+            }
+            if (HB == 8 || t < 2) *reinterpret_cast<float4*>(w_o + ((size_t)warp * HB + 2 * t + h) * kA4Hd + 32 * gr + 4 * g) = make_float4(o[h][0], o[h][1], o[h][2], o[h][3]);
+        }
+    }
+    if (t == 0 && g < HB) {
+        s_ml[warp][g][0] = m_run == -INFINITY ? -INFINITY : top;
+        s_ml[warp][g][1] = l_run;
+    }
+    __syncthreads();
+    for (int i = tid; i < heads * kA4Hd; i += kA4Threads) {
+        const int h = i / kA4Hd, d = i % kA4Hd;
+        float m = -INFINITY, o = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kA4Warps; ++w) m = fmaxf(m, s_ml[w][h][0]);
+        const float m_use = m == -INFINITY ? 0.0f : m;
+#pragma unroll
         for (int w = 0; w < kA4Warps; ++w) {
-            const float f = s_m[w] == -INFINITY ? 0.0f : expf(s_m[w] - top);
-            sum = __fmaf_rn(s_l[w], f, sum);
-            v = __fmaf_rn(s_o[w][tid], f, v);
+            const float x = a4_ex2(s_ml[w][h][0] - m_use);
+            o = __fmaf_rn(w_o[((size_t)w * HB + h) * kA4Hd + d], x, o);
+            l = __fmaf_rn(s_ml[w][h][1], x, l);
         }
-        out[tid] = sum > 0.0f ? v / sum : 0.0f;
+        if (L.n_splits == 1) {
+            out[i] = l > 0.0f ? o / l : 0.0f;
+        } else {
+            const size_t at = ((size_t)row * a.n_q + (size_t)kvh * L.group + head0 + h) * L.n_splits + split;
+            L.part_o[at * kA4Hd + d] = o;
+            if (d == 0) L.part_ml[at] = make_float2(m, l);
+        }
     }
+}
+
+// The splits of a (row, head): one warp each, four dims a lane.
+__global__ void __launch_bounds__(kA4Threads) attention_kv4_merge_kernel(const A4Launch L) {
+    const tenzo_attention_kv4_args& a = L.a;
+    const int lane = threadIdx.x & 31, head = blockIdx.y * kA4Warps + (threadIdx.x >> 5), row = blockIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
+    if (head >= a.n_q) return;
+    const int pos = a.pos[row], seq = a.seq ? a.seq[row] : row;
+    if (a4_refused(a, pos, seq)) return;
+    const int n = pos < 0 ? 0 : pos / L.split_keys + 1;
+    const size_t at = ((size_t)row * a.n_q + head) * L.n_splits;
+    const float2* ml = L.part_ml + at;
+    const float4* po = reinterpret_cast<const float4*>(L.part_o) + at * (kA4Hd / 4) + lane;
+    float m = -INFINITY;
+    for (int s = lane; s < n; s += 32) m = fmaxf(m, __ldcg(ml + s).x);
+    m = warp_max(m);
+    const float m_use = m == -INFINITY ? 0.0f : m;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+    constexpr int kBatch = 8;                            // loads in flight
+    for (int s0 = 0; s0 < n; s0 += kBatch) {
+        float2 v[kBatch];
+        float4 p[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            v[u] = s0 + u < n ? __ldcg(ml + s0 + u) : make_float2(-INFINITY, 0.0f);
+            p[u] = s0 + u < n ? __ldcg(po + (size_t)(s0 + u) * (kA4Hd / 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const float x = a4_ex2(v[u].x - m_use);
+            o.x = __fmaf_rn(p[u].x, x, o.x);
+            o.y = __fmaf_rn(p[u].y, x, o.y);
+            o.z = __fmaf_rn(p[u].z, x, o.z);
+            o.w = __fmaf_rn(p[u].w, x, o.w);
+            l = __fmaf_rn(v[u].y, x, l);
+        }
+    }
+    const float r = l > 0.0f ? 1.0f / l : 0.0f;
+    reinterpret_cast<float4*>(a.out + ((size_t)row * a.n_q + head) * kA4Hd)[lane] = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
+}
+
+static size_t a4_part_bytes(int rows, int n_q) { return (size_t)rows * n_q * (kA4Hd + 2) * sizeof(float); }
+
+// Keys a CTA takes: the number of splits whose rounds of CTAs take least at the longest length, a CTA's own cost counted as some
+// hundred keys and a split's as some in the second kernel. `most`: as many splits as there is room for partial results.
+static void a4_pick_split(long long items, int max_len, int most, int* n_splits, int* split_keys) {
+    const long long places = 148 * kA4Resident;
+    double best = 0.0;
+    for (int want = 1; want <= 64 && (want == 1 || (max_len + want - 1) / want > 128); ++want) {
+        const int keys = ((max_len + want - 1) / want + 127) / 128 * 128, splits = (max_len + keys - 1) / keys;
+        if (splits > most) continue;
+        const long long ctas = items * splits;
+        const double rounds = ctas <= 3 * places ? (double)((ctas + places - 1) / places) : (double)ctas / places + 0.5;
+        const double cost = rounds * (keys + 500.0) + (splits > 1 ? 300.0 + 16.0 * (splits - 1) : 0.0);
+        if (want == 1 || cost < best) {
+            best = cost;
+            *split_keys = keys;
+            *n_splits = splits;
+        }
+    }
+}
+
+template <int HB>
+static int a4_run(const A4Launch& L, cudaStream_t st) {
+    const size_t smem = (size_t)kA4Warps * kA4Stages * kA4StepBytes;
+    if (cudaError_t e = allow_smem(attention_kv4_kernel<HB>, smem)) return (int)e;
+    const dim3 grid((unsigned)L.a.rows * (unsigned)L.n_splits, (unsigned)(L.a.cache.n_kv * L.head_blocks));
+    return kv4_launch(attention_kv4_kernel<HB>, grid, kA4Threads, smem, st, L.a.use_pdl != 0, L);
 }
 
 int kv4_attention_take_error() {
@@ -86,13 +526,16 @@ int kv4_rows_take_error();
 
 extern "C" size_t tenzo_cuda_attention_kv4_workspace_bytes(int rows, int n_q, int n_kv, int max_len) {
     if (rows <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_len <= 0) return 0;
-    return 64;
+    const size_t splits = ((size_t)max_len + 127) / 128;     // the finest split that may be asked for
+    return tz::a4_part_bytes(rows, n_q) * splits;
 }
 
 extern "C" int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, void* stream) {
     using namespace tz;
     if (!args) return -1;
-    tenzo_attention_kv4_args a = *args;
+    A4Launch L = {};
+    L.a = *args;
+    tenzo_attention_kv4_args& a = L.a;
     if (a.rows == 0) return 0;
     if (!kv4_cache_ok(a.cache) || !a.q || !a.out || !a.pos) return -1;
     if (a.layer < 0 || a.layer >= a.cache.n_layers || a.n_q <= 0 || a.n_q % a.cache.n_kv || a.rows < 0 || a.max_len <= 0) return -1;
@@ -101,7 +544,27 @@ extern "C" int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, vo
     if (a.split_keys < 0 || (reinterpret_cast<uintptr_t>(a.out) & 15)) return -1;
     if (a.q_stride == 0) a.q_stride = a.n_q * kA4Hd;
     if (a.q_stride < a.n_q * kA4Hd) return -1;
-    return kv4_launch(attention_kv4_simple_kernel, dim3((unsigned)a.rows, (unsigned)a.n_q), kA4Warps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl != 0, a);
+    L.group = a.n_q / a.cache.n_kv;
+    const int hb = L.group <= 4 ? 4 : 8;
+    L.head_blocks = (L.group + hb - 1) / hb;
+    const long long items = (long long)a.rows * a.cache.n_kv * L.head_blocks;
+    if ((long long)a.cache.n_kv * L.head_blocks > 65535) return -1;
+    const bool ws_ok = a.workspace && !(reinterpret_cast<uintptr_t>(a.workspace) & 15);
+    const size_t room = ws_ok ? a.workspace_bytes / a4_part_bytes(a.rows, a.n_q) : 0;
+    if (a.split_keys > 0) {
+        L.split_keys = (int)(((long long)a.split_keys + 127) / 128 * 128 < a.max_len ? ((long long)a.split_keys + 127) / 128 * 128 : ((long long)a.max_len + 127) / 128 * 128);
+        L.n_splits = (a.max_len + L.split_keys - 1) / L.split_keys;
+        if (L.n_splits > 1 && room < (size_t)L.n_splits) return -1;
+    } else {
+        a4_pick_split(items, a.max_len, room > 1 ? (int)(room < 64 ? room : 64) : 1, &L.n_splits, &L.split_keys);
+    }
+    if ((long long)a.rows * L.n_splits > 0x7fffffffLL) return -1;
+    L.part_o = static_cast<float*>(a.workspace);
+    L.part_ml = reinterpret_cast<float2*>(L.part_o + (size_t)a.rows * a.n_q * L.n_splits * kA4Hd);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (int rc = hb == 4 ? a4_run<4>(L, st) : a4_run<8>(L, st)) return rc;
+    if (L.n_splits == 1) return 0;
+    return kv4_launch(attention_kv4_merge_kernel, dim3((unsigned)a.rows, (unsigned)((a.n_q + kA4Warps - 1) / kA4Warps)), kA4Threads, 0, st, true, L);
 }
 
 extern "C" int tenzo_cuda_kv4_take_errors(void) {
