@@ -1,122 +1,391 @@
 // The k best continuations of a group of beams over beams x vocabulary.
 //
 // score(beam, token) = cum[beam] + (x - log sum exp x), in 64 bits: sums of log-probabilities lie close together between beams, and 32
-// bits would order some of them wrongly. A row's k best are found by its logits alone (same order), the rows' lists then meet.
+// bits would order some of them wrongly. Within a row the order is that of the logits. Two kernels:
+//
+//   1. A CTA takes a chunk of a row, each thread up to 32 logits in registers, read once. The k-th largest of the 256 threads' maxima is a
+//      lower bound of the chunk's k-th largest logit, and hardly more logits reach it: those are listed, ranked, and their
+//      exponentials summed in 64 bits. All others' exponentials are summed in 32 (hardware ex2, about 1e-7 each, and the largest of them is one of 17 at
+//      least): the logarithm of the whole is good to some 1e-9 whether a few tokens have all the weight or thousands share it.
+//      Everything is added in an order that the data alone decides, so that equal rows get equal sums and tie.
+//   2. A CTA a group: a warp merges each row's lists, then an entry's place is its place in its row and, by bisection, the number of better ones
+//      in each other row.
+//
+// The first kernel reads 4 bytes a logit; what bounds it besides is some ten instructions and an ex2 (8 cycles of its unit a warp) for each.
 #include "common.cuh"
-#include "../../include/tenzo_kernels.h"
+#include "kv4.cuh"
 
 #include <cfloat>
 
 namespace tz {
 
-constexpr int kBsThreads = 512;
+constexpr int kBsThreads = 256, kBsWarps = kBsThreads / 32;
+constexpr int kBsLeast = 16;                              // at least so many candidates are asked for in a chunk
+constexpr int kBsWindow = 8;                              // and up to so many threads more are let in
+constexpr int kBsMostK = 2 * TENZO_BEAMS_MOST;
+constexpr int kBsMostPer = 32;                            // logits a thread holds at most
+constexpr int kBsList = (kBsMostK + kBsWindow) * kBsMostPer;      // candidates lie in that many threads' logits
+constexpr int kBsMergeWarps = 8, kBsMergeRoom = 1024;     // entries of a row that a warp of the second kernel keeps in shared memory
 
-// A logit as it counts: NaN never chosen before anything else, infinity as the largest number.
-__device__ __forceinline__ float beam_logit(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
-// Order of the floats as integers, and -0 as +0.
+typedef unsigned long long u64;
+
+// Order of the floats as integers above 0 (0: nothing there), and -0 as +0.
 __device__ __forceinline__ uint32_t beam_key(float f) {
     const uint32_t b = f == 0.0f ? 0u : __float_as_uint(f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+__device__ __forceinline__ float beam_unkey(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+__device__ __forceinline__ u64 beam_entry(uint32_t key, int token) { return ((u64)key << 32) | (uint32_t)~token; }      // larger key, then lower token
+__device__ __forceinline__ int entry_token(u64 e) { return (int)~(uint32_t)e; }
+__device__ __forceinline__ float entry_logit(u64 e) { return beam_unkey((uint32_t)(e >> 32)); }
 
-struct BeamRow {                                          // one of a row's best
-    double score;
-    int token;
+struct __align__(16) BeamPart {                           // of a chunk
+    double sum;                                           // of exp(x - most)
+    float most;
+};
+struct BeamLaunch {
+    tenzo_beam_select_args a;
+    int per, chunks;                                      // logits a thread takes, chunks a row
+    BeamPart* parts;                                      // [row][chunk]
+    u64* lists;                                           // [row][chunk][k], best first; 0 behind the last
 };
 
-// One CTA a row: the sum of exponentials, then k times the largest of what is left.
-__global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const tenzo_beam_select_args a) {
-    __shared__ double s_sum[kBsThreads / 32];
-    __shared__ unsigned long long s_key[kBsThreads / 32];
-    __shared__ float s_max[kBsThreads / 32];
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// Rows that the first kernel leaves out: finished beams, and those whose score is -infinity (or NaN).
+__device__ __forceinline__ bool beam_dead(float cum) { return !(cum > -INFINITY); }
+__device__ __forceinline__ bool beam_done(const tenzo_beam_select_args& a, int row, float cum) { return a.finished && a.finished[row] != 0 && !beam_dead(cum); }
+
+template <bool VEC, int PER>
+__global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch L) {
+    __shared__ uint32_t s_keys[kBsThreads];
+    __shared__ u64 s_list[kBsList], s_sorted[kBsList];
+    __shared__ double s_sum[kBsWarps];
+    __shared__ float s_red[kBsWarps];
+    __shared__ uint32_t s_bound;
+    __shared__ int s_short, s_last, s_n;
+    const tenzo_beam_select_args& a = L.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / L.chunks, chunk = blockIdx.x % L.chunks;
+    pdl_launch_dependents();                              // the second kernel waits for this one, whatever its neighbours do
+    if (a.use_pdl) pdl_wait();
+    const float cum = a.scores[row];
+    if (beam_dead(cum) || beam_done(a, row, cum)) return;
     const float* x = a.logits + (size_t)row * a.row_stride;
-    const double cum = (double)a.scores[row];
-    BeamRow* out = static_cast<BeamRow*>(a.workspace) + (size_t)row * a.k;
-    const bool done = a.finished && a.finished[row] != 0 && cum > -INFINITY;
-    float m = -INFINITY;
-    for (int i = tid; i < a.vocab; i += kBsThreads) m = fmaxf(m, beam_logit(x[i]));
-    m = block_max(m, s_max);
-    const bool none = done || m == -INFINITY || !(cum > -INFINITY);
-    double sum = 0.0;
-    if (!none)
-        for (int i = tid; i < a.vocab; i += kBsThreads) sum += exp((double)beam_logit(x[i]) - (double)m);
+    const int base = chunk * kBsThreads * PER;
+    // place of the j-th logit of a thread: consecutive fours (or ones) go to consecutive threads
+    auto place = [&](int j) { return base + (VEC ? 4 * (tid + kBsThreads * (j >> 2)) + (j & 3) : tid + kBsThreads * j); };
+    float v[PER];                                         // NaN: nothing there
+    if (VEC) {
+#pragma unroll
+        for (int j = 0; j < PER; j += 4) {
+            float4 f = make_float4(NAN, NAN, NAN, NAN);
+            const int i = place(j);
+            if (i + 3 < a.vocab) {
+                f = __ldcs(reinterpret_cast<const float4*>(x + i));
+            } else {
+                if (i < a.vocab) f.x = x[i];
+                if (i + 1 < a.vocab) f.y = x[i + 1];
+                if (i + 2 < a.vocab) f.z = x[i + 2];
+            }
+            v[j] = f.x; v[j + 1] = f.y; v[j + 2] = f.z; v[j + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = place(j) < a.vocab ? __ldcs(x + place(j)) : NAN;
+    }
+    if (tid == 0) s_n = 0;
+    // ---- what counts: NaN as -infinity, infinity as the largest number; the largest of all ------------------------------------
+    float top = -INFINITY;
+    const bool whole = base + kBsThreads * PER <= a.vocab;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const float c = fminf(fmaxf(v[j], -INFINITY), FLT_MAX);
+        v[j] = whole || place(j) < a.vocab ? c : NAN;
+        top = fmaxf(top, c);                              // (an absent one counts as -infinity here)
+    }
+    s_keys[tid] = place(0) < a.vocab ? beam_key(top) : 0u;
+    float most = warp_max(top);
+    if (lane == 0) s_red[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kBsWarps; ++w) most = fmaxf(most, s_red[w]);
+    // ---- a bound that `want` threads' maxima reach, and hardly more -------------------------------------------------------------
+    const int want = max(a.k, kBsLeast);
+    auto at_least = [&](const uint32_t (&key)[kBsWarps], uint32_t b) {
+        int n = 0;
+#pragma unroll
+        for (int w = 0; w < kBsWarps; ++w) n += key[w] >= b;
+        return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+    };
+    if (warp == 0) {
+        uint32_t key[kBsWarps], least = 0xffffffffu;
+#pragma unroll
+        for (int w = 0; w < kBsWarps; ++w) {
+            key[w] = s_keys[32 * w + lane];
+            least = min(least, key[w]);
+        }
+        uint32_t lo = __reduce_min_sync(0xffffffffu, least), hi = beam_key(most) + 1;       // all reach lo, none hi
+        int reach = kBsThreads;
+        while (reach > want + kBsWindow && hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int n = at_least(key, mid);
+            if (n >= want) { lo = mid; reach = n; } else hi = mid;
+        }
+        const int above = reach > want + kBsWindow ? at_least(key, hi) : 0;
+        if (lane == 0) {
+            s_bound = lo;
+            s_short = lo > 0 && reach > want + kBsWindow ? want - above : 0;      // too many alike: so many of them, by index
+            s_last = 0x7fffffff;
+        }
+    }
+    __syncthreads();
+    const float bound = s_bound <= beam_key(-INFINITY) ? -INFINITY : beam_unkey(s_bound);      // (no float below that one: all that is there is listed)
+    if (s_short) {                                        // the first place of each thread's largest, then a place that enough of them reach
+        int first = 0x7fffffff;
+        if (s_keys[tid] == s_bound) {
+#pragma unroll
+            for (int j = PER - 1; j >= 0; --j)
+                if (v[j] == bound) first = place(j);
+        }
+        __syncthreads();
+        s_keys[tid] = (uint32_t)first;
+        __syncthreads();
+        if (warp == 0) {
+            uint32_t key[kBsWarps];
+#pragma unroll
+            for (int w = 0; w < kBsWarps; ++w) key[w] = ~s_keys[32 * w + lane];
+            uint32_t lo = ~(uint32_t)(base + kBsThreads * PER), hi = ~(uint32_t)base + 1u;     // (complements: a lower place is a larger key)
+            int reach = at_least(key, lo);
+            while (reach > s_short + kBsWindow && hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                const int n = at_least(key, mid);
+                if (n >= s_short) { lo = mid; reach = n; } else hi = mid;
+            }
+            if (lane == 0) s_last = (int)~lo;
+        }
+        __syncthreads();
+    }
+    const int last = s_last;
+    // ---- the others' exponentials, and the list of candidates -------------------------------------------------------------------
+    const float from = most == -INFINITY ? 0.0f : most;
+    float rest = 0.0f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const float d = v[j] - from;                      // times log2(e), whose second part is 1.9e-8
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmaf_rn(d, 1.4426950216293335f, d * 1.9259629911e-8f)));
+        rest += v[j] < bound || (v[j] == bound && place(j) > last) ? e : 0.0f;
+    }
+    if (top >= bound) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (v[j] > bound || (v[j] == bound && place(j) <= last)) {
+                const int at = atomicAdd(&s_n, 1);
+                if (at < kBsList) s_list[at] = beam_entry(beam_key(v[j]), place(j));
+            }
+    }
+    double sum = (double)rest;
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    sum = 0.0;
-    for (int w = 0; w < kBsThreads / 32; ++w) sum += s_sum[w];
-    if (none) {                                           // the lowest tokens, all with -inf; a finished beam's end token in front
-        for (int i = tid; i < a.k; i += kBsThreads) {
-            const int token = !done ? i : i == 0 ? a.eos : i - 1 < a.eos ? i - 1 : i;
-            out[i] = {done && i == 0 ? cum : -(double)INFINITY, token < a.vocab ? token : -1};
-        }
-        return;
+    const int n = min(s_n, kBsList);
+    for (int i = tid; i < n; i += kBsThreads) {
+        const u64 e = s_list[i];
+        int before = 0;
+        for (int j = 0; j < n; ++j) before += s_list[j] > e;
+        s_sorted[before] = e;
     }
-    const double lse = (double)m + log(sum);
-    unsigned long long last = ~0ull;
-    for (int r = 0; r < a.k; ++r) {
-        unsigned long long best = 0;
-        for (int i = tid; i < a.vocab; i += kBsThreads) {
-            const unsigned long long key = ((unsigned long long)beam_key(beam_logit(x[i])) << 32) | (0xffffffffu - (unsigned)i);
-            if (key < last && key > best) best = key;
-        }
-        for (int o = 16; o > 0; o >>= 1) { const unsigned long long v = __shfl_xor_sync(0xffffffffu, best, o); best = v > best ? v : best; }
-        __syncthreads();
-        if (lane == 0) s_key[warp] = best;
-        __syncthreads();
-        for (int w = 0; w < kBsThreads / 32; ++w) best = s_key[w] > best ? s_key[w] : best;
-        last = best;
-        if (tid == 0) {
-            const int token = best ? (int)(0xffffffffu - (unsigned)best) : -1;
-            out[r] = {token < 0 ? -(double)INFINITY : cum + ((double)beam_logit(x[token]) - lse), token};
-        }
-        if (!best) last = 0;
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < kBsWarps; ++w) sum += s_sum[w];
+    __syncthreads();
+    double listed = 0.0;
+    if (most > -INFINITY)
+        for (int i = tid; i < n; i += kBsThreads) listed += exp((double)entry_logit(s_sorted[i]) - (double)most);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) listed += __shfl_xor_sync(0xffffffffu, listed, o);
+    if (lane == 0) s_sum[warp] = listed;
+    u64* to = L.lists + ((size_t)row * L.chunks + chunk) * a.k;
+    for (int i = tid; i < a.k; i += kBsThreads) to[i] = i < n ? s_sorted[i] : 0ull;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 0; w < kBsWarps; ++w) sum += s_sum[w];
+        BeamPart p;
+        p.sum = sum;
+        p.most = most;
+        L.parts[(size_t)row * L.chunks + chunk] = p;
     }
 }
 
-// One CTA a group: a candidate's place is the number of candidates in front of it.
-__global__ void __launch_bounds__(kBsThreads) beam_groups_kernel(const tenzo_beam_select_args a) {
-    const int g = blockIdx.x, n = a.beams * a.k;
-    const BeamRow* in = static_cast<const BeamRow*>(a.workspace) + (size_t)g * n;
-    for (int i = threadIdx.x; i < n; i += kBsThreads) {
-        const BeamRow c = in[i];
-        if (c.token < 0) continue;
-        int before = 0;
-        for (int j = 0; j < n; ++j) {
-            const BeamRow o = in[j];
-            if (o.token >= 0 && (o.score > c.score || (o.score == c.score && j < i))) ++before;
+struct BeamGroup {
+    double score[TENZO_BEAMS_MOST][kBsMostK];             // a row's best, in order
+    int token[TENZO_BEAMS_MOST][kBsMostK];
+    int count[TENZO_BEAMS_MOST];
+    u64 pick[kBsMergeWarps][kBsMostK + 2 * kBsWindow];    // what a warp found, unsorted
+    int picked[kBsMergeWarps];
+    u64 room[kBsMergeWarps][kBsMergeRoom];                // a row's lists
+};
+
+__global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const BeamLaunch L) {
+    extern __shared__ __align__(16) unsigned char bs_smem[];
+    BeamGroup& G = *reinterpret_cast<BeamGroup*>(bs_smem);
+    const tenzo_beam_select_args& a = L.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, k = a.k;
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int b = warp; b < a.beams; b += kBsMergeWarps) {
+        const int row = g * a.beams + b, most_tokens = min(k, a.vocab);
+        const float cum = a.scores[row];
+        const bool done = beam_done(a, row, cum);
+        const BeamPart* parts = L.parts + (size_t)row * L.chunks;
+        float most = -INFINITY;
+        double sum = 0.0;
+        if (!done && !beam_dead(cum)) {
+            for (int c = lane; c < L.chunks; c += 32) most = fmaxf(most, __ldcg(&parts[c].most));
+            most = warp_max(most);
+            for (int c = lane; c < L.chunks; c += 32) {
+                const float m = __ldcg(&parts[c].most);
+                if (m > -INFINITY) sum += __ldcg(&parts[c].sum) * exp((double)m - (double)most);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        if (before < a.k) {
-            const size_t to = (size_t)g * a.k + before;
-            a.parent_out[to] = i / a.k;
-            a.token_out[to] = c.token;
-            a.score_out[to] = (float)c.score;
+        if (most == -INFINITY) {                          // finished, or nothing left: the lowest tokens at -infinity; in front of them a finished beam's end
+            for (int i = lane; i < most_tokens; i += 32) {
+                G.token[b][i] = !done ? i : i == 0 ? a.eos : i - 1 < a.eos ? i - 1 : i;
+                G.score[b][i] = done && i == 0 ? (double)cum : -(double)INFINITY;
+            }
+            if (lane == 0) G.count[b] = most_tokens;
+            continue;
+        }
+        const double lse = (double)most + log(sum);
+        const u64* list = L.lists + (size_t)row * L.chunks * k;
+        const int n = L.chunks * k;
+        const bool fits = n <= kBsMergeRoom;
+        // every chunk's k-th is a lower bound of the row's k-th
+        u64 lo = 0, hi = 0;
+        for (int c = lane; c < L.chunks; c += 32) {
+            const u64 first = __ldcg(list + (size_t)c * k), kth = __ldcg(list + (size_t)c * k + k - 1);
+            hi = first > hi ? first : hi;
+            lo = kth > lo ? kth : lo;
+        }
+        if (fits)
+            for (int i = lane; i < n; i += 32) G.room[warp][i] = __ldcg(list + i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const u64 h = __shfl_xor_sync(0xffffffffu, hi, o), l = __shfl_xor_sync(0xffffffffu, lo, o);
+            hi = h > hi ? h : hi;
+            lo = l > lo ? l : lo;
+        }
+        if (lo == 0) lo = 1;                              // (0: nothing there)
+        hi += 1;
+        if (lane == 0) G.picked[warp] = 0;
+        __syncwarp();
+        auto entry = [&](int i) { return fits ? G.room[warp][i] : __ldcg(list + i); };
+        auto at_least = [&](u64 x) {
+            int m = 0;
+            for (int i = lane; i < n; i += 32) m += entry(i) >= x;
+            return (int)__reduce_add_sync(0xffffffffu, (unsigned)m);
+        };
+        int reach = at_least(lo);
+        while (reach > k + kBsWindow && hi - lo > 1) {    // entries differ: it ends
+            const u64 mid = lo + (hi - lo) / 2;
+            const int m = at_least(mid);
+            if (m >= k) { lo = mid; reach = m; } else hi = mid;
+        }
+        for (int i = lane; i < n; i += 32) {
+            const u64 e = entry(i);
+            if (e >= lo) {
+                const int at = atomicAdd(&G.picked[warp], 1);
+                if (at < kBsMostK + 2 * kBsWindow) G.pick[warp][at] = e;
+            }
+        }
+        __syncwarp();
+        const int m = min(G.picked[warp], kBsMostK + 2 * kBsWindow);
+        for (int i = lane; i < m; i += 32) {
+            const u64 e = G.pick[warp][i];
+            int before = 0;
+            for (int j = 0; j < m; ++j) before += G.pick[warp][j] > e;
+            if (before < k) {
+                const float x = entry_logit(e);
+                G.token[b][before] = entry_token(e);
+                G.score[b][before] = x == -INFINITY ? -(double)INFINITY : (double)cum + ((double)x - lse);
+            }
+        }
+        if (lane == 0) G.count[b] = min(m, k);
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int i = tid; i < a.beams * k; i += kBsMergeWarps * 32) {
+        const int b = i / k, p = i % k;
+        if (p >= G.count[b]) continue;
+        const double score = G.score[b][p];
+        int before = p;
+        for (int o = 0; o < a.beams && before < k; ++o) {
+            if (o == b) continue;
+            int lo = 0, hi = G.count[o];                  // the number in front: larger scores, and equal ones of lower beams
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                const double s = G.score[o][mid];
+                if (s > score || (s == score && o < b)) lo = mid + 1; else hi = mid;
+            }
+            before += lo;
+        }
+        if (before < k) {
+            const size_t to = (size_t)g * k + before;
+            a.parent_out[to] = b;
+            a.token_out[to] = G.token[b][p];
+            a.score_out[to] = (float)score;
         }
     }
+}
+
+// Logits a thread takes: 32, or fewer where that would leave SMs without a CTA.
+static int beam_per(int rows, int vocab) {
+    int per = kBsMostPer;
+    while (per > 4 && (long long)rows * ((vocab + kBsThreads * per - 1) / (kBsThreads * per)) < 128) per /= 2;
+    return per;
+}
+
+template <bool VEC>
+static int beam_rows_run(const BeamLaunch& L, cudaStream_t st) {
+    auto* kernel = L.per == 32 ? beam_rows_kernel<VEC, 32> : L.per == 16 ? beam_rows_kernel<VEC, 16> : L.per == 8 ? beam_rows_kernel<VEC, 8> : beam_rows_kernel<VEC, 4>;
+    return kv4_launch(kernel, dim3((unsigned)(L.a.groups * L.a.beams) * (unsigned)L.chunks), kBsThreads, 0, st, L.a.use_pdl != 0, L);
 }
 
 }  // namespace tz
 
 extern "C" size_t tenzo_cuda_beam_select_workspace_bytes(int groups, int beams, int vocab, int k) {
-    if (groups <= 0 || beams <= 0 || vocab <= 0 || k <= 0) return 0;
-    return (size_t)groups * beams * k * sizeof(tz::BeamRow);
+    if (groups <= 0 || beams <= 0 || vocab <= 0 || k <= 0 || (long long)groups * beams > 0x7fffffffLL) return 0;
+    const int per = tz::beam_per(groups * beams, vocab);
+    const size_t chunks = ((size_t)vocab + tz::kBsThreads * per - 1) / ((size_t)tz::kBsThreads * per);
+    return (size_t)groups * beams * chunks * (sizeof(tz::BeamPart) + (size_t)k * sizeof(tz::u64));
 }
 
 extern "C" int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* stream) {
     using namespace tz;
     if (!args) return -1;
-    tenzo_beam_select_args a = *args;
+    BeamLaunch L = {};
+    L.a = *args;
+    tenzo_beam_select_args& a = L.a;
     if (a.groups == 0) return 0;
     if (!a.logits || !a.scores || !a.parent_out || !a.token_out || !a.score_out || !a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 15)) return -1;
     if (a.groups < 0 || a.vocab <= 0 || a.beams < 1 || a.k < 1 || a.k > (long long)a.beams * a.vocab) return -1;
     if (a.finished && (a.eos < 0 || a.eos >= a.vocab)) return -1;
-    if (a.beams > TENZO_BEAMS_MOST || a.k > 2 * TENZO_BEAMS_MOST) return -5;
+    if (a.beams > TENZO_BEAMS_MOST || a.k > kBsMostK) return -5;
     if (a.row_stride == 0) a.row_stride = a.vocab;
     if (a.row_stride < a.vocab) return -1;
+    const long long rows = (long long)a.groups * a.beams;
+    if (rows > 0x7fffffffLL) return -1;
+    L.per = beam_per((int)rows, a.vocab);
+    L.chunks = (int)(((long long)a.vocab + kBsThreads * L.per - 1) / (kBsThreads * L.per));
+    if (rows * L.chunks > 0x7fffffffLL || (long long)L.chunks * a.k > 0x7fffffffLL || (long long)L.chunks * kBsThreads * L.per > 0x7fffffffLL) return -1;
     if (a.workspace_bytes < tenzo_cuda_beam_select_workspace_bytes(a.groups, a.beams, a.vocab, a.k)) return -1;
+    L.parts = static_cast<BeamPart*>(a.workspace);
+    L.lists = reinterpret_cast<u64*>(L.parts + (size_t)rows * L.chunks);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    beam_rows_kernel<<<a.groups * a.beams, kBsThreads, 0, st>>>(a);
-    beam_groups_kernel<<<a.groups, kBsThreads, 0, st>>>(a);
-    return (int)cudaGetLastError();
+    const bool vec = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.row_stride % 4 == 0;
+    if (cudaError_t e = allow_smem(beam_groups_kernel, sizeof(BeamGroup))) return (int)e;
+    if (int rc = vec ? beam_rows_run<true>(L, st) : beam_rows_run<false>(L, st)) return rc;
+    return kv4_launch(beam_groups_kernel, dim3((unsigned)a.groups), kBsMergeWarps * 32, sizeof(BeamGroup), st, true, L);
 }
