@@ -178,15 +178,32 @@ _BEAM_SELECT = struct.Struct("@PPPiiiiiiiPPPPN")                # abi.BeamSelect
 assert _KV4_CACHE.size == C.sizeof(abi.Kv4Cache) and _KV4_ATTENTION.size == C.sizeof(abi.AttentionKv4Args) and _BEAM_SELECT.size == C.sizeof(abi.BeamSelectArgs)
 
 
-@functools.cache
-def _packed(name, argtypes):
-    """A prototype of `name` of this module's own, whose structs are the bytes of a struct.Struct (c_char_p in argtypes)."""
-    fn = load_library()[name]
-    fn.restype, fn.argtypes = C.c_int, list(argtypes)
-    return fn
-
-
 _PI, _PP, _PB = C.c_int, C.c_void_p, C.c_char_p
+
+
+@functools.cache
+def _beam_calls():
+    """The entry points with prototypes of this module's own, whose structs are the bytes of a struct.Struct; tenzo_cuda_kv4_append, _read, _reorder,
+    tenzo_cuda_attention_kv4, tenzo_cuda_beam_select, and the two workspace sizes."""
+    def fn(name, *argtypes, restype=C.c_int):
+        f = load_library()[name]
+        f.restype, f.argtypes = restype, list(argtypes)
+        return f
+    return (fn("tenzo_cuda_kv4_append", _PB, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PI, _PP),
+            fn("tenzo_cuda_kv4_read", _PB, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PI, _PP),
+            fn("tenzo_cuda_kv4_reorder", _PB, _PP, _PP, _PP, _PI, _PI, _PI, _PP),
+            fn("tenzo_cuda_attention_kv4", _PB, _PP), fn("tenzo_cuda_beam_select", _PB, _PP),
+            fn("tenzo_cuda_attention_kv4_workspace_bytes", _PI, _PI, _PI, _PI, restype=C.c_size_t),
+            fn("tenzo_cuda_beam_select_workspace_bytes", _PI, _PI, _PI, _PI, restype=C.c_size_t))
+
+
+# (These calls take as long as their kernels at small sizes: attributes of a tensor are read once, 0.05 us each, and the stream's handle comes from
+# the raw getter, 0.07 us against 0.76 by way of a stream object.)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _refuse(t, what, need):
+    raise ValueError(f"{what}: {need} on the current CUDA device is needed, not {t.dtype} {tuple(t.shape)} of strides {t.stride()} on {t.device}")
 
 
 def _arg(t: torch.Tensor | None, dtype, device: int, what: str) -> int:
@@ -194,119 +211,117 @@ def _arg(t: torch.Tensor | None, dtype, device: int, what: str) -> int:
     if t is None:
         return 0
     if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{what}: a contiguous {dtype} tensor on the current CUDA device is needed, not {t.dtype} of strides {t.stride()} on {t.device}")
+        _refuse(t, what, f"a contiguous {dtype} tensor")
     return t.data_ptr()
 
 
-def _arg_rows(t: torch.Tensor, device: int, columns: int, what: str) -> tuple[int, int]:
-    """Address and row stride of fp32 rows that may lie apart (a column slice of a wider buffer)."""
-    if t.dtype is not torch.float32 or t.get_device() != device or t.dim() != 2 or t.shape[1] != columns or (columns > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: fp32 rows of {columns} values on the current CUDA device are needed, not {t.dtype} {tuple(t.shape)} of strides {t.stride()} on {t.device}")
-    stride = t.stride(0)
-    return t.data_ptr(), stride if t.shape[0] > 1 else max(stride, columns)
+def _arg_rows(t: torch.Tensor, device: int, columns: int, what: str) -> tuple[int, int, int]:
+    """Address, row stride and number of fp32 rows that may lie apart (a column slice of a wider buffer)."""
+    shape, strides = t.shape, t.stride()
+    if t.dtype is not torch.float32 or t.get_device() != device or len(shape) != 2 or shape[1] != columns or (columns > 1 and strides[1] != 1):
+        _refuse(t, what, f"fp32 rows of {columns} values")
+    n = shape[0]
+    return t.data_ptr(), strides[0] if n > 1 else max(strides[0], columns), n
 
 
 def _kv4_cache(pool: torch.Tensor, block_table: torch.Tensor, device: int):
-    """The fields of abi.Kv4Cache."""
-    shape = pool.shape
-    if len(shape) != 6 or tuple(shape[3:]) != (2, 16, 80) or block_table.dim() != 2:
-        raise ValueError(f"a pool [blocks, layers, kv heads, 2, 16, 80] and a table [rows, columns] are needed, not {tuple(shape)} and {tuple(block_table.shape)}")
-    rows, columns = block_table.shape
-    return (_arg(pool, torch.uint8, device, "pool"), shape[0], shape[1], shape[2], _arg(block_table, torch.int32, device, "block_table"), rows, columns)
+    """The bytes of abi.Kv4Cache, kv heads, table rows and columns."""
+    shape, table = pool.shape, block_table.shape
+    if len(shape) != 6 or len(table) != 2 or shape[3] != 2 or shape[4] != 16 or shape[5] != 80:
+        raise ValueError(f"a pool [blocks, layers, kv heads, 2, 16, 80] and a table [rows, columns] are needed, not {tuple(shape)} and {tuple(table)}")
+    n_kv, (rows, columns) = shape[2], table
+    return (_KV4_CACHE.pack(_arg(pool, torch.uint8, device, "pool"), shape[0], shape[1], n_kv, _arg(block_table, torch.int32, device, "block_table"), rows, columns),
+            n_kv, rows, columns)
 
 
-def _row_count(pos, seq, n, what):
-    if pos.shape != (n,) or (seq is not None and seq.shape != (n,)):
-        raise ValueError(f"{what}: pos and seq have one entry for each of {n} rows")
+def _arg_entries(t, n: int, device: int, what: str) -> int:
+    """Address of int32 [n]; 0 for None."""
+    if t is not None and t.shape != (n,):
+        raise ValueError(f"{what} has one entry for each of {n} rows, not {tuple(t.shape)}")
+    return _arg(t, torch.int32, device, what)
 
 
-def _current_device() -> int:
-    return torch._C._cuda_getDevice()
+def _arg_rope(cos, sin, device: int) -> tuple[int, int, int]:
+    if cos is None and sin is None:
+        return 0, 0, 0
+    if cos is None or sin is None or cos.dim() != 2 or cos.shape[1] != 64 or sin.shape != cos.shape:
+        raise ValueError("rope_cos and rope_sin are tables of the same number of rows of 64")
+    return _arg(cos, torch.float32, device, "rope_cos"), _arg(sin, torch.float32, device, "rope_sin"), cos.shape[0]
 
 
 def kv4_append(k, v, pool, pos, *, layer, block_table, seq=None, rope_cos=None, rope_sin=None, use_pdl=False):
     """Rotates the rows k [n, n_kv*128], quantises k and v to 4 bits and stores them in `pool` (uint8 [blocks, layers, n_kv, 2, 16, 80]) at
     positions pos int32 [n] of the sequences seq int32 [n] (default: row i is sequence i) of block_table int32 [sequences, columns].
     A negative position marks a padding row, for which nothing is stored."""
-    dev, n = _current_device(), k.shape[0]
-    cache = _kv4_cache(pool, block_table, dev)
-    (kp, ks), (vp, vs) = _arg_rows(k, dev, cache[3] * 128, "k"), _arg_rows(v, dev, cache[3] * 128, "v")
-    if v.shape[0] != n or (ks != vs and n > 1):
+    dev = _current_device()
+    cache, n_kv, _, _ = _kv4_cache(pool, block_table, dev)
+    (kp, ks, n), (vp, vs, m) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
+    if n != m or (ks != vs and n > 1):
         raise ValueError("k and v have the same number of rows, equally far apart")
-    _row_count(pos, seq, n, "kv4_append")
-    if rope_cos is not None and (rope_cos.shape[1:] != (64,) or rope_sin is None or rope_sin.shape != rope_cos.shape):
-        raise ValueError("rope_cos and rope_sin are tables of the same number of rows of 64")
-    fn = _packed("tenzo_cuda_kv4_append", (_PB, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PI, _PP))
-    _ok(fn(_KV4_CACHE.pack(*cache), layer, kp, vp, ks, _arg(pos, torch.int32, dev, "pos"), _arg(seq, torch.int32, dev, "seq"), n,
-           _arg(rope_cos, torch.float32, dev, "rope_cos"), _arg(rope_sin, torch.float32, dev, "rope_sin"), 0 if rope_cos is None else rope_cos.shape[0], use_pdl,
-           _stream()), "tenzo_cuda_kv4_append")
+    cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
+    _ok(_beam_calls()[0](cache, layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, cos, sin, length, use_pdl, _raw_stream(dev)),
+        "tenzo_cuda_kv4_append")
 
 
 def kv4_read(pool, pos, *, layer, block_table, seq=None, use_pdl=False, k=None, v=None):
     """The rows at positions pos int32 [n] of the sequences seq as the cache holds them: (k, v), fp32 [n, n_kv*128], the keys rotated; zeros for
     negative positions. k and v may be given (both) to be written into."""
-    dev, n = _current_device(), pos.shape[0]
-    cache = _kv4_cache(pool, block_table, dev)
-    width = cache[3] * 128
+    dev, n = _current_device(), len(pos)
+    cache, n_kv, _, _ = _kv4_cache(pool, block_table, dev)
     if k is None and v is None:
-        k, v = torch.empty(2, n, width, dtype=torch.float32, device=pool.device)
-        kp, vp, stride = k.data_ptr(), v.data_ptr(), width
-    else:
-        (kp, stride), (vp, vs) = _arg_rows(k, dev, width, "k"), _arg_rows(v, dev, width, "v")
-        if k.shape[0] != n or v.shape[0] != n or (stride != vs and n > 1):
-            raise ValueError("k and v have one row for each position, equally far apart")
-    _row_count(pos, seq, n, "kv4_read")
-    fn = _packed("tenzo_cuda_kv4_read", (_PB, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PI, _PP))
-    _ok(fn(_KV4_CACHE.pack(*cache), layer, kp, vp, stride, _arg(pos, torch.int32, dev, "pos"), _arg(seq, torch.int32, dev, "seq"), n, use_pdl, _stream()),
-        "tenzo_cuda_kv4_read")
+        k = torch.empty(n, n_kv * 128, dtype=torch.float32, device=pool.device)
+        v = torch.empty_like(k)
+    (kp, ks, m), (vp, vs, o) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
+    if n != m or n != o or (ks != vs and n > 1):
+        raise ValueError("k and v have one row for each position, equally far apart")
+    _ok(_beam_calls()[1](cache, layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, use_pdl, _raw_stream(dev)), "tenzo_cuda_kv4_read")
     return k, v
 
 
 def attention_kv4_workspace_bytes(rows, n_q, n_kv, max_len) -> int:
-    return int(load_library().tenzo_cuda_attention_kv4_workspace_bytes(rows, n_q, n_kv, max_len))
+    return _beam_calls()[5](rows, n_q, n_kv, max_len)
 
 
 def attention_kv4(q, pool, pos, *, layer, n_q, block_table, seq=None, rope_cos=None, rope_sin=None, max_len=None, split_keys=0, use_pdl=False, out=None,
                   workspace=None):
     """GQA attention of the query rows q [rows, n_q*128] over the keys 0 .. pos[row] of their sequences in the 4-bit pool, the queries rotated first.
     Returns out [rows, n_q*128]; zeros where pos is negative. max_len: an upper bound on pos + 1 (default: what the table has room for)."""
-    dev, rows = _current_device(), q.shape[0]
-    cache = _kv4_cache(pool, block_table, dev)
-    qp, q_stride = _arg_rows(q, dev, n_q * 128, "q")
-    _row_count(pos, seq, rows, "attention_kv4")
-    if rope_cos is not None and (rope_cos.shape[1:] != (64,) or rope_sin is None or rope_sin.shape != rope_cos.shape):
-        raise ValueError("rope_cos and rope_sin are tables of the same number of rows of 64")
+    dev = _current_device()
+    cache, n_kv, _, columns = _kv4_cache(pool, block_table, dev)
+    qp, q_stride, rows = _arg_rows(q, dev, n_q * 128, "q")
+    cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
     if max_len is None:
-        max_len = cache[6] * 16 if rope_cos is None else min(cache[6] * 16, rope_cos.shape[0])
+        max_len = min(columns * 16, length) if cos else columns * 16
     if out is None:
         out = torch.empty(rows, n_q * 128, dtype=torch.float32, device=q.device)
     elif out.shape != (rows, n_q * 128):
         raise ValueError(f"out is [{rows}, {n_q * 128}]")
     if workspace is None:
-        workspace = torch.empty(attention_kv4_workspace_bytes(rows, n_q, cache[3], max_len), dtype=torch.uint8, device=q.device)
-    args = _KV4_ATTENTION.pack(qp, _arg(out, torch.float32, dev, "out"), *cache, _arg(pos, torch.int32, dev, "pos"), _arg(seq, torch.int32, dev, "seq"),
-                               _arg(rope_cos, torch.float32, dev, "rope_cos"), _arg(rope_sin, torch.float32, dev, "rope_sin"),
-                               0 if rope_cos is None else rope_cos.shape[0], q_stride, layer, n_q, rows, max_len, split_keys, use_pdl,
-                               _arg(workspace, torch.uint8, dev, "workspace"), workspace.numel())
-    _ok(_packed("tenzo_cuda_attention_kv4", (_PB, _PP))(args, _stream()), "tenzo_cuda_attention_kv4")
+        need = _beam_calls()[5](rows, n_q, n_kv, max_len)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    args = _KV4_ATTENTION.pack(qp, _arg(out, torch.float32, dev, "out"), *_KV4_CACHE.unpack(cache), _arg_entries(pos, rows, dev, "pos"), _arg_entries(seq, rows, dev, "seq"),
+                               cos, sin, length, q_stride, layer, n_q, rows, max_len, split_keys, use_pdl, _arg(workspace, torch.uint8, dev, "workspace"),
+                               0 if workspace is None else workspace.numel())
+    _ok(_beam_calls()[3](args, _raw_stream(dev)), "tenzo_cuda_attention_kv4")
     return out
 
 
 def beam_select(logits, scores, *, beams, k, finished=None, eos=0, use_pdl=False, workspace=None):
     """The k best continuations of each group of `beams` rows of logits [groups*beams, vocab], given the beams' sums of log-probabilities scores
     fp32 [groups*beams]. Returns (parent, token, score), [groups, k], best first. finished int32 [groups*beams]: beams that only go on with `eos`."""
-    dev, (rows, vocab) = _current_device(), logits.shape
+    dev, vocab = _current_device(), logits.shape[-1]
+    lp, stride, rows = _arg_rows(logits, dev, vocab, "logits")
     groups = rows // beams
-    if groups * beams != rows or scores.shape != (rows,) or (finished is not None and finished.shape != (rows,)):
+    if groups * beams != rows or scores.shape != (rows,):
         raise ValueError(f"{rows} rows of logits are no groups of {beams} beams with one score each")
-    lp, stride = _arg_rows(logits, dev, vocab, "logits")
-    out = torch.empty(3, groups, k, dtype=torch.int32, device=logits.device)
-    parent, token, score = out[0], out[1], out[2].view(torch.float32)
+    device = logits.device
+    parent = torch.empty(groups, k, dtype=torch.int32, device=device)
+    token, score = torch.empty_like(parent), torch.empty(groups, k, dtype=torch.float32, device=device)
     if workspace is None:
-        workspace = torch.empty(load_library().tenzo_cuda_beam_select_workspace_bytes(groups, beams, vocab, k), dtype=torch.uint8, device=logits.device)
-    args = _BEAM_SELECT.pack(lp, _arg(scores, torch.float32, dev, "scores"), _arg(finished, torch.int32, dev, "finished"), eos, stride, groups, beams, vocab, k,
+        workspace = torch.empty(_beam_calls()[6](groups, beams, vocab, k), dtype=torch.uint8, device=device)
+    args = _BEAM_SELECT.pack(lp, _arg(scores, torch.float32, dev, "scores"), _arg_entries(finished, rows, dev, "finished"), eos, stride, groups, beams, vocab, k,
                              use_pdl, parent.data_ptr(), token.data_ptr(), score.data_ptr(), _arg(workspace, torch.uint8, dev, "workspace"), workspace.numel())
-    _ok(_packed("tenzo_cuda_beam_select", (_PB, _PP))(args, _stream()), "tenzo_cuda_beam_select")
+    _ok(_beam_calls()[4](args, _raw_stream(dev)), "tenzo_cuda_beam_select")
     return parent, token, score
 
 
@@ -314,16 +329,15 @@ def kv4_reorder(pool, block_table, parent, length, *, out=None, use_pdl=False):
     """The block table of the beams that go on from parent int32 [groups, beams] of beams that hold length int32 [groups] tokens each. Full blocks are
     shared; the block being filled is copied within `pool` for the second and further children of a beam, into those of beams without children."""
     dev, (groups, beams) = _current_device(), parent.shape
-    cache = _kv4_cache(pool, block_table, dev)
-    if length.shape != (groups,) or block_table.shape[0] != groups * beams:
-        raise ValueError(f"{groups} groups of {beams} beams need as many lengths and table rows, not {tuple(length.shape)} and {block_table.shape[0]}")
+    cache, _, rows, _ = _kv4_cache(pool, block_table, dev)
+    if rows != groups * beams:
+        raise ValueError(f"{groups} groups of {beams} beams need as many table rows, not {rows}")
     if out is None:
         out = torch.empty_like(block_table)
     elif out.shape != block_table.shape:
         raise ValueError("out has the table's shape")
-    fn = _packed("tenzo_cuda_kv4_reorder", (_PB, _PP, _PP, _PP, _PI, _PI, _PI, _PP))
-    _ok(fn(_KV4_CACHE.pack(*cache), _arg(out, torch.int32, dev, "out"), _arg(parent, torch.int32, dev, "parent"), _arg(length, torch.int32, dev, "length"), groups, beams,
-           use_pdl, _stream()), "tenzo_cuda_kv4_reorder")
+    _ok(_beam_calls()[2](cache, _arg(out, torch.int32, dev, "out"), _arg(parent, torch.int32, dev, "parent"), _arg_entries(length, groups, dev, "length"), groups, beams,
+                         use_pdl, _raw_stream(dev)), "tenzo_cuda_kv4_reorder")
     return out
 
 
