@@ -25,7 +25,9 @@ constexpr int kBsWindow = 8;                              // and up to so many t
 constexpr int kBsMostK = 2 * TENZO_BEAMS_MOST;
 constexpr int kBsMostPer = 32;                            // logits a thread holds at most
 constexpr int kBsList = (kBsMostK + kBsWindow) * kBsMostPer;      // candidates lie in that many threads' logits
-constexpr int kBsMergeWarps = 8, kBsMergeRoom = 1024;     // entries of a row that a warp of the second kernel keeps in shared memory
+constexpr int kBsMergeWarps = 16;                         // rows that the second kernel merges at a time
+constexpr int kBsHeads = 4;                               // leading entries of a row's lists, a lane
+constexpr int kBsPicks = 96;                              // entries that are ranked; more than k + kBsWindow
 
 typedef unsigned long long u64;
 
@@ -72,11 +74,11 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     const int base = chunk * kBsThreads * PER;
     // place of the j-th logit of a thread: consecutive fours (or ones) go to consecutive threads
     auto place = [&](int j) { return base + (VEC ? 4 * (tid + kBsThreads * (j >> 2)) + (j & 3) : tid + kBsThreads * j); };
-    float v[PER];                                         // NaN: nothing there
+    float v[PER];                                         // -infinity where there is nothing
     if (VEC) {
 #pragma unroll
         for (int j = 0; j < PER; j += 4) {
-            float4 f = make_float4(NAN, NAN, NAN, NAN);
+            float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             const int i = place(j);
             if (i + 3 < a.vocab) {
                 f = __ldcs(reinterpret_cast<const float4*>(x + i));
@@ -89,17 +91,15 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = place(j) < a.vocab ? __ldcs(x + place(j)) : NAN;
+        for (int j = 0; j < PER; ++j) v[j] = place(j) < a.vocab ? __ldcs(x + place(j)) : -INFINITY;
     }
     if (tid == 0) s_n = 0;
     // ---- what counts: NaN as -infinity, infinity as the largest number; the largest of all ------------------------------------
     float top = -INFINITY;
-    const bool whole = base + kBsThreads * PER <= a.vocab;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const float c = fminf(fmaxf(v[j], -INFINITY), FLT_MAX);
-        v[j] = whole || place(j) < a.vocab ? c : NAN;
-        top = fmaxf(top, c);                              // (an absent one counts as -infinity here)
+        v[j] = fminf(fmaxf(v[j], -INFINITY), FLT_MAX);
+        top = fmaxf(top, v[j]);
     }
     s_keys[tid] = place(0) < a.vocab ? beam_key(top) : 0u;
     float most = warp_max(top);
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
         if (s_keys[tid] == s_bound) {
 #pragma unroll
             for (int j = PER - 1; j >= 0; --j)
-                if (v[j] == bound) first = place(j);
+                if (v[j] == bound && place(j) < a.vocab) first = place(j);
         }
         __syncthreads();
         s_keys[tid] = (uint32_t)first;
@@ -169,18 +169,20 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     float rest = 0.0f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
+        bool other = v[j] < bound;
+        if (!other) {
+            const int i = place(j);
+            if (v[j] > bound || i <= last) {
+                const int at = i < a.vocab ? atomicAdd(&s_n, 1) : kBsList;
+                if (at < kBsList) s_list[at] = beam_entry(beam_key(v[j]), i);
+            } else {
+                other = true;
+            }
+        }
         const float d = v[j] - from;                      // times log2(e), whose second part is 1.9e-8
         float e;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmaf_rn(d, 1.4426950216293335f, d * 1.9259629911e-8f)));
-        rest += v[j] < bound || (v[j] == bound && place(j) > last) ? e : 0.0f;
-    }
-    if (top >= bound) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (v[j] > bound || (v[j] == bound && place(j) <= last)) {
-                const int at = atomicAdd(&s_n, 1);
-                if (at < kBsList) s_list[at] = beam_entry(beam_key(v[j]), place(j));
-            }
+        rest += other ? e : 0.0f;
     }
     double sum = (double)rest;
 #pragma unroll
@@ -221,23 +223,30 @@ struct BeamGroup {
     double score[TENZO_BEAMS_MOST][kBsMostK];             // a row's best, in order
     int token[TENZO_BEAMS_MOST][kBsMostK];
     int count[TENZO_BEAMS_MOST];
-    u64 pick[kBsMergeWarps][kBsMostK + 2 * kBsWindow];    // what a warp found, unsorted
+    u64 pick[kBsMergeWarps][kBsPicks];                    // what a warp found, unsorted
     int picked[kBsMergeWarps];
-    u64 room[kBsMergeWarps][kBsMergeRoom];                // a row's lists
 };
 
 __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const BeamLaunch L) {
-    extern __shared__ __align__(16) unsigned char bs_smem[];
-    BeamGroup& G = *reinterpret_cast<BeamGroup*>(bs_smem);
+    __shared__ BeamGroup G;
     const tenzo_beam_select_args& a = L.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, k = a.k;
     pdl_launch_dependents();
     pdl_wait();
     for (int b = warp; b < a.beams; b += kBsMergeWarps) {
-        const int row = g * a.beams + b, most_tokens = min(k, a.vocab);
+        const int row = g * a.beams + b, most_tokens = min(k, a.vocab), n = L.chunks * k;
+        const BeamPart* parts = L.parts + (size_t)row * L.chunks;
+        const u64* list = L.lists + (size_t)row * L.chunks * k;
+        // The first `deep` of every list, 2 k or more in all, bound the row's k-th from below. (Asked for first: of a row left out they mean nothing.)
+        const int deep = min(k, (2 * k + L.chunks - 1) / L.chunks), heads = L.chunks * deep;
+        uint32_t head[kBsHeads];
+#pragma unroll
+        for (int i = 0; i < kBsHeads; ++i) {
+            const int at = lane + 32 * i;
+            head[i] = at < heads ? (uint32_t)(__ldcg(list + (size_t)(at / deep) * k + at % deep) >> 32) : 0u;
+        }
         const float cum = a.scores[row];
         const bool done = beam_done(a, row, cum);
-        const BeamPart* parts = L.parts + (size_t)row * L.chunks;
         float most = -INFINITY;
         double sum = 0.0;
         if (!done && !beam_dead(cum)) {
@@ -258,50 +267,57 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
             if (lane == 0) G.count[b] = most_tokens;
             continue;
         }
-        const double lse = (double)most + log(sum);
-        const u64* list = L.lists + (size_t)row * L.chunks * k;
-        const int n = L.chunks * k;
-        const bool fits = n <= kBsMergeRoom;
-        // every chunk's k-th is a lower bound of the row's k-th
-        u64 lo = 0, hi = 0;
-        for (int c = lane; c < L.chunks; c += 32) {
-            const u64 first = __ldcg(list + (size_t)c * k), kth = __ldcg(list + (size_t)c * k + k - 1);
-            hi = first > hi ? first : hi;
-            lo = kth > lo ? kth : lo;
-        }
-        if (fits)
-            for (int i = lane; i < n; i += 32) G.room[warp][i] = __ldcg(list + i);
+        u64 lo = 1;                                       // (0: nothing there)
+        int reach = kBsPicks + 1;
+        if (heads <= 32 * kBsHeads) {
+            auto at_least = [&](uint32_t x) {
+                int m = 0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const u64 h = __shfl_xor_sync(0xffffffffu, hi, o), l = __shfl_xor_sync(0xffffffffu, lo, o);
-            hi = h > hi ? h : hi;
-            lo = l > lo ? l : lo;
+                for (int i = 0; i < kBsHeads; ++i) m += __popc(__ballot_sync(0xffffffffu, head[i] >= x));
+                return m;
+            };
+            uint32_t low = 1, high = beam_key(most) + 1;
+            int r = at_least(low);
+            while (r > k + kBsWindow && high - low > 1) {
+                const uint32_t mid = low + (high - low) / 2;
+                const int m = at_least(mid);
+                if (m >= k) { low = mid; r = m; } else high = mid;
+            }
+            if (r >= k) lo = (u64)low << 32;              // (fewer: the row has no k)
         }
-        if (lo == 0) lo = 1;                              // (0: nothing there)
-        hi += 1;
-        if (lane == 0) G.picked[warp] = 0;
-        __syncwarp();
-        auto entry = [&](int i) { return fits ? G.room[warp][i] : __ldcg(list + i); };
-        auto at_least = [&](u64 x) {
-            int m = 0;
-            for (int i = lane; i < n; i += 32) m += entry(i) >= x;
-            return (int)__reduce_add_sync(0xffffffffu, (unsigned)m);
-        };
-        int reach = at_least(lo);
-        while (reach > k + kBsWindow && hi - lo > 1) {    // entries differ: it ends
-            const u64 mid = lo + (hi - lo) / 2;
-            const int m = at_least(mid);
-            if (m >= k) { lo = mid; reach = m; } else hi = mid;
-        }
-        for (int i = lane; i < n; i += 32) {
-            const u64 e = entry(i);
-            if (e >= lo) {
-                const int at = atomicAdd(&G.picked[warp], 1);
-                if (at < kBsMostK + 2 * kBsWindow) G.pick[warp][at] = e;
+        for (int pass = 0; pass < 2; ++pass) {
+            if (lane == 0) G.picked[warp] = 0;
+            __syncwarp();
+            for (int i0 = 0; i0 < n; i0 += 32 * 8) {
+                u64 e[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) e[u] = i0 + 32 * u + lane < n ? __ldcg(list + i0 + 32 * u + lane) : 0ull;
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (e[u] >= lo) {
+                        const int at = atomicAdd(&G.picked[warp], 1);
+                        if (at < kBsPicks) G.pick[warp][at] = e[u];
+                    }
+            }
+            __syncwarp();
+            reach = G.picked[warp];
+            __syncwarp();
+            if (reach <= kBsPicks || pass) break;
+            // Too many alike, or a great many lists: the k-th of all entries, which differ, by bisection over the memory.
+            auto at_least = [&](u64 x) {
+                int m = 0;
+                for (int i = lane; i < n; i += 32) m += __ldcg(list + i) >= x;
+                return (int)__reduce_add_sync(0xffffffffu, (unsigned)m);
+            };
+            u64 hi = ((u64)beam_key(most) + 1) << 32;
+            while (reach > kBsPicks && hi - lo > 1) {
+                const u64 mid = lo + (hi - lo) / 2;
+                const int m = at_least(mid);
+                if (m >= k) { lo = mid; reach = m; } else hi = mid;
             }
         }
-        __syncwarp();
-        const int m = min(G.picked[warp], kBsMostK + 2 * kBsWindow);
+        const double lse = (double)most + log(sum);
+        const int m = min(reach, kBsPicks);
         for (int i = lane; i < m; i += 32) {
             const u64 e = G.pick[warp][i];
             int before = 0;
@@ -385,7 +401,6 @@ extern "C" int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* 
     L.lists = reinterpret_cast<u64*>(L.parts + (size_t)rows * L.chunks);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool vec = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.row_stride % 4 == 0;
-    if (cudaError_t e = allow_smem(beam_groups_kernel, sizeof(BeamGroup))) return (int)e;
     if (int rc = vec ? beam_rows_run<true>(L, st) : beam_rows_run<false>(L, st)) return rc;
-    return kv4_launch(beam_groups_kernel, dim3((unsigned)a.groups), kBsMergeWarps * 32, sizeof(BeamGroup), st, true, L);
+    return kv4_launch(beam_groups_kernel, dim3((unsigned)a.groups), kBsMergeWarps * 32, 0, st, true, L);
 }
