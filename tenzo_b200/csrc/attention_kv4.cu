@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     mbar_init_fence();
     if (a.use_pdl || L.n_splits > 1) pdl_launch_dependents();       // the second kernel waits for this one whatever its neighbours do
     if (a.use_pdl) pdl_wait();
-    const int pos = a.pos[row], seq = a.seq ? a.seq[row] : row;
+    const int pos = ld_l2(a.pos + row), seq = a.seq ? ld_l2(a.seq + row) : row;
     if (a4_refused(a, pos, seq)) {
         if (tid == 0) atomicOr(&g_kv4_attention_error, kK4ErrIndex);
         return;
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         const int page = 2 * (warp + (k0 + (lane >> 1)) * kA4Warps) + (lane & 1);
         int id = -1;
         if (page < pages) {
-            id = __ldg(table + page);
+            id = ld_l2(table + page);
             if (id < 0 || id >= a.cache.n_blocks) {
                 atomicOr(&g_kv4_attention_error, kK4ErrIndex);
                 id = -1;
@@ -163,11 +163,11 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         const int h = i >> 6, d = i & 63;
         float r0 = 0.0f, r1 = 0.0f;
         if (h < heads) {
-            const float x0 = __ldcg(q + h * kA4Hd + d), x1 = __ldcg(q + h * kA4Hd + d + 64);
+            const float x0 = ld_l2(q + h * kA4Hd + d), x1 = ld_l2(q + h * kA4Hd + d + 64);
             r0 = x0;
             r1 = x1;
             if (a.rope_cos) {
-                const float c = __ldg(a.rope_cos + (size_t)pos * 64 + d), s = __ldg(a.rope_sin + (size_t)pos * 64 + d);
+                const float c = ld_l2(a.rope_cos + (size_t)pos * 64 + d), s = ld_l2(a.rope_sin + (size_t)pos * 64 + d);
                 r0 = __fmaf_rn(x0, c, -(x1 * s));
                 r1 = __fmaf_rn(x0, s, x1 * c);
             }
@@ -450,14 +450,14 @@ __global__ void __launch_bounds__(kA4Threads) attention_kv4_merge_kernel(const A
     pdl_launch_dependents();
     pdl_wait();
     if (head >= a.n_q) return;
-    const int pos = a.pos[row], seq = a.seq ? a.seq[row] : row;
+    const int pos = ld_l2(a.pos + row), seq = a.seq ? ld_l2(a.seq + row) : row;
     if (a4_refused(a, pos, seq)) return;
     const int n = pos < 0 ? 0 : pos / L.split_keys + 1;
     const size_t at = ((size_t)row * a.n_q + head) * L.n_splits;
     const float2* ml = L.part_ml + at;
     const float4* po = reinterpret_cast<const float4*>(L.part_o) + at * (kA4Hd / 4) + lane;
     float m = -INFINITY;
-    for (int s = lane; s < n; s += 32) m = fmaxf(m, __ldcg(ml + s).x);
+    for (int s = lane; s < n; s += 32) m = fmaxf(m, ld_l2(ml + s).x);
     m = warp_max(m);
     const float m_use = m == -INFINITY ? 0.0f : m;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -468,8 +468,8 @@ __global__ void __launch_bounds__(kA4Threads) attention_kv4_merge_kernel(const A
         float4 p[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            v[u] = s0 + u < n ? __ldcg(ml + s0 + u) : make_float2(-INFINITY, 0.0f);
-            p[u] = s0 + u < n ? __ldcg(po + (size_t)(s0 + u) * (kA4Hd / 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            v[u] = s0 + u < n ? ld_l2(ml + s0 + u) : make_float2(-INFINITY, 0.0f);
+            p[u] = s0 + u < n ? ld_l2(po + (size_t)(s0 + u) * (kA4Hd / 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {

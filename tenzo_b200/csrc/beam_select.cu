@@ -4,12 +4,12 @@
 // bits would order some of them wrongly. Within a row the order is that of the logits. Two kernels:
 //
 //   1. A CTA takes a chunk of a row, each thread up to 32 logits in registers, read once. The k-th largest of the 256 threads' maxima is a
-//      lower bound of the chunk's k-th largest logit, and hardly more logits reach it: those are listed, ranked, and their
-//      exponentials summed in 64 bits. All others' exponentials are summed in 32 (hardware ex2, about 1e-7 each, and the largest of them is one of 17 at
-//      least): the logarithm of the whole is good to some 1e-9 whether a few tokens have all the weight or thousands share it.
-//      Everything is added in an order that the data alone decides, so that equal rows get equal sums and tie.
-//   2. A CTA a group: a warp merges each row's lists, then an entry's place is its place in its row and, by bisection, the number of better ones
-//      in each other row.
+//      lower bound of the chunk's k-th largest logit, and hardly more logits reach it: those are listed, and their exponentials summed in 64
+//      bits. All others' are summed in 32 (hardware ex2, about 1e-7 each, and 16 larger ones at least are on the list): the
+//      logarithm of the whole is good to some 1e-9 whether a few tokens have all the weight or thousands share it.
+//   2. A CTA a group, a warp a row: the k best of the lists. An entry's place in the group is its place in its row and, by bisection, the
+//      number of better ones in each other row.
+// Sums are taken in an order that the data alone decides, or as integers, so that equal rows get equal sums and tie.
 //
 // The first kernel reads 4 bytes a logit; what bounds it besides is some ten instructions and an ex2 (8 cycles of its unit a warp) for each.
 #include "common.cuh"
@@ -26,8 +26,10 @@ constexpr int kBsMostK = 2 * TENZO_BEAMS_MOST;
 constexpr int kBsMostPer = 32;                            // logits a thread holds at most
 constexpr int kBsList = (kBsMostK + kBsWindow) * kBsMostPer;      // candidates lie in that many threads' logits
 constexpr int kBsMergeWarps = 16;                         // rows that the second kernel merges at a time
-constexpr int kBsHeads = 4;                               // leading entries of a row's lists, a lane
+constexpr int kBsHold = 32;                               // entries of a row's lists that a lane keeps
 constexpr int kBsPicks = 96;                              // entries that are ranked; more than k + kBsWindow
+
+constexpr double kBsUnit = 281474976710656.0;             // 2^48
 
 typedef unsigned long long u64;
 
@@ -47,20 +49,21 @@ struct __align__(16) BeamPart {                           // of a chunk
 };
 struct BeamLaunch {
     tenzo_beam_select_args a;
-    int per, chunks;                                      // logits a thread takes, chunks a row
+    int per, chunks, slots;                               // logits a thread takes, chunks a row, entries a chunk's list has room for
     BeamPart* parts;                                      // [row][chunk]
-    u64* lists;                                           // [row][chunk][k], best first; 0 behind the last
+    u64* lists;                                           // [row][chunk][slots], in any order; 0 where there is none
 };
 
 // Rows that the first kernel leaves out: finished beams, and those whose score is -infinity (or NaN).
 __device__ __forceinline__ bool beam_dead(float cum) { return !(cum > -INFINITY); }
-__device__ __forceinline__ bool beam_done(const tenzo_beam_select_args& a, int row, float cum) { return a.finished && a.finished[row] != 0 && !beam_dead(cum); }
+__device__ __forceinline__ bool beam_done(const tenzo_beam_select_args& a, int row, float cum) { return a.finished && ld_l2(a.finished + row) != 0 && !beam_dead(cum); }
 
 template <bool VEC, int PER>
 __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch L) {
     __shared__ uint32_t s_keys[kBsThreads];
     __shared__ u64 s_list[kBsList], s_sorted[kBsList];
     __shared__ double s_sum[kBsWarps];
+    __shared__ u64 s_listed;
     __shared__ float s_red[kBsWarps];
     __shared__ uint32_t s_bound;
     __shared__ int s_short, s_last, s_n;
@@ -68,12 +71,13 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / L.chunks, chunk = blockIdx.x % L.chunks;
     pdl_launch_dependents();                              // the second kernel waits for this one, whatever its neighbours do
     if (a.use_pdl) pdl_wait();
-    const float cum = a.scores[row];
+    const float cum = ld_l2(a.scores + row);
     if (beam_dead(cum) || beam_done(a, row, cum)) return;
     const float* x = a.logits + (size_t)row * a.row_stride;
     const int base = chunk * kBsThreads * PER;
     // place of the j-th logit of a thread: consecutive fours (or ones) go to consecutive threads
     auto place = [&](int j) { return base + (VEC ? 4 * (tid + kBsThreads * (j >> 2)) + (j & 3) : tid + kBsThreads * j); };
+    static_assert(PER <= 32, "one bit each");
     float v[PER];                                         // -infinity where there is nothing
     if (VEC) {
 #pragma unroll
@@ -81,25 +85,33 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
             float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             const int i = place(j);
             if (i + 3 < a.vocab) {
-                f = __ldcs(reinterpret_cast<const float4*>(x + i));
+                f = ld_l2(reinterpret_cast<const float4*>(x + i));
             } else {
-                if (i < a.vocab) f.x = x[i];
-                if (i + 1 < a.vocab) f.y = x[i + 1];
-                if (i + 2 < a.vocab) f.z = x[i + 2];
+                if (i < a.vocab) f.x = ld_l2(x + i);
+                if (i + 1 < a.vocab) f.y = ld_l2(x + i + 1);
+                if (i + 2 < a.vocab) f.z = ld_l2(x + i + 2);
             }
             v[j] = f.x; v[j + 1] = f.y; v[j + 2] = f.z; v[j + 3] = f.w;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = place(j) < a.vocab ? __ldcs(x + place(j)) : -INFINITY;
+        for (int j = 0; j < PER; ++j) v[j] = place(j) < a.vocab ? ld_l2(x + place(j)) : -INFINITY;
     }
-    if (tid == 0) s_n = 0;
+    if (tid == 0) {
+        s_n = 0;
+        s_listed = 0;
+    }
     // ---- what counts: NaN as -infinity, infinity as the largest number; the largest of all ------------------------------------
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        v[j] = fminf(fmaxf(v[j], -INFINITY), FLT_MAX);
+        v[j] = fmaxf(v[j], -INFINITY);                    // (drops NaN)
         top = fmaxf(top, v[j]);
+    }
+    if (top == INFINITY) {
+        top = FLT_MAX;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = fminf(v[j], FLT_MAX);
     }
     s_keys[tid] = place(0) < a.vocab ? beam_key(top) : 0u;
     float most = warp_max(top);
@@ -167,53 +179,55 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     // ---- the others' exponentials, and the list of candidates -------------------------------------------------------------------
     const float from = most == -INFINITY ? 0.0f : most;
     float rest = 0.0f;
+    uint32_t reach_it = 0;                                // one bit a logit
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        bool other = v[j] < bound;
-        if (!other) {
-            const int i = place(j);
-            if (v[j] > bound || i <= last) {
-                const int at = i < a.vocab ? atomicAdd(&s_n, 1) : kBsList;
-                if (at < kBsList) s_list[at] = beam_entry(beam_key(v[j]), i);
-            } else {
-                other = true;
-            }
-        }
         const float d = v[j] - from;                      // times log2(e), whose second part is 1.9e-8
         float e;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmaf_rn(d, 1.4426950216293335f, d * 1.9259629911e-8f)));
-        rest += other ? e : 0.0f;
+        if (v[j] >= bound) reach_it |= 1u << j; else rest += e;
+    }
+    for (const bool one = (reach_it & (reach_it - 1u)) == 0u; reach_it; reach_it &= reach_it - 1u) {
+        const int i = place(__ffs((int)reach_it) - 1);
+        if (i >= a.vocab) continue;
+        const float c = one ? top : fminf(fmaxf(ld_l2(x + i), -INFINITY), FLT_MAX);      // (read again: a register's number is no variable)
+        if (c == bound && i > last) {
+            rest += from == bound ? 1.0f : exp2f((c - from) * 1.4426950408889634f);
+        } else {
+            const int at = atomicAdd(&s_n, 1);
+            if (at < kBsList) s_list[at] = beam_entry(beam_key(c), i);
+        }
     }
     double sum = (double)rest;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    const int n = min(s_n, kBsList);
-    for (int i = tid; i < n; i += kBsThreads) {
-        const u64 e = s_list[i];
-        int before = 0;
-        for (int j = 0; j < n; ++j) before += s_list[j] > e;
-        s_sorted[before] = e;
+    int n = min(s_n, kBsList);
+    const u64* list = s_list;
+    if (most > -INFINITY) {                               // the listed ones' exponentials, in units of 2^-48: whole numbers add up the same in any order
+        u64 mine = 0;
+        for (int i = tid; i < n; i += kBsThreads) mine += (u64)__double2ll_rn(exp((double)entry_logit(s_list[i]) - (double)most) * kBsUnit);
+        if (mine) atomicAdd(&s_listed, mine);
     }
-    sum = 0.0;
-#pragma unroll
-    for (int w = 0; w < kBsWarps; ++w) sum += s_sum[w];
+    if (n > L.slots) {                                    // (many large ones in few threads) the best k go on
+        for (int i = tid; i < n; i += kBsThreads) {
+            const u64 e = s_list[i];
+            int before = 0;
+            for (int j = 0; j < n; ++j) before += s_list[j] > e;
+            s_sorted[before] = e;
+        }
+        n = a.k;
+        list = s_sorted;
+    }
     __syncthreads();
-    double listed = 0.0;
-    if (most > -INFINITY)
-        for (int i = tid; i < n; i += kBsThreads) listed += exp((double)entry_logit(s_sorted[i]) - (double)most);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) listed += __shfl_xor_sync(0xffffffffu, listed, o);
-    if (lane == 0) s_sum[warp] = listed;
-    u64* to = L.lists + ((size_t)row * L.chunks + chunk) * a.k;
-    for (int i = tid; i < a.k; i += kBsThreads) to[i] = i < n ? s_sorted[i] : 0ull;
-    __syncthreads();
+    u64* to = L.lists + ((size_t)row * L.chunks + chunk) * L.slots;
+    if (tid < L.slots) to[tid] = tid < n ? list[tid] : 0ull;
     if (tid == 0) {
-#pragma unroll
-        for (int w = 0; w < kBsWarps; ++w) sum += s_sum[w];
         BeamPart p;
-        p.sum = sum;
+        p.sum = (double)s_listed * (1.0 / kBsUnit);
+#pragma unroll
+        for (int w = 0; w < kBsWarps; ++w) p.sum += s_sum[w];
         p.most = most;
         L.parts[(size_t)row * L.chunks + chunk] = p;
     }
@@ -234,30 +248,27 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
     pdl_launch_dependents();
     pdl_wait();
     for (int b = warp; b < a.beams; b += kBsMergeWarps) {
-        const int row = g * a.beams + b, most_tokens = min(k, a.vocab), n = L.chunks * k;
+        const int row = g * a.beams + b, most_tokens = min(k, a.vocab), n = L.chunks * L.slots;
         const BeamPart* parts = L.parts + (size_t)row * L.chunks;
-        const u64* list = L.lists + (size_t)row * L.chunks * k;
-        // The first `deep` of every list, 2 k or more in all, bound the row's k-th from below. (Asked for first: of a row left out they mean nothing.)
-        const int deep = min(k, (2 * k + L.chunks - 1) / L.chunks), heads = L.chunks * deep;
-        uint32_t head[kBsHeads];
+        const u64* list = L.lists + (size_t)row * n;
+        const bool held = n <= 32 * kBsHold;              // in registers; more are read again whenever they are needed
+        u64 mine[kBsHold];                                // (asked for first: of a row left out they mean nothing)
 #pragma unroll
-        for (int i = 0; i < kBsHeads; ++i) {
-            const int at = lane + 32 * i;
-            head[i] = at < heads ? (uint32_t)(__ldcg(list + (size_t)(at / deep) * k + at % deep) >> 32) : 0u;
-        }
-        const float cum = a.scores[row];
+        for (int i = 0; i < kBsHold; ++i) mine[i] = held && lane + 32 * i < n ? ld_l2(list + lane + 32 * i) : 0ull;
+        auto each = [&](auto&& f) {
+            if (held) {
+#pragma unroll
+                for (int i = 0; i < kBsHold; ++i) f(mine[i]);
+            } else {
+                for (int i = lane; i < n; i += 32) f(ld_l2(list + i));
+            }
+        };
+        const float cum = ld_l2(a.scores + row);
         const bool done = beam_done(a, row, cum);
         float most = -INFINITY;
-        double sum = 0.0;
         if (!done && !beam_dead(cum)) {
-            for (int c = lane; c < L.chunks; c += 32) most = fmaxf(most, __ldcg(&parts[c].most));
+            for (int c = lane; c < L.chunks; c += 32) most = fmaxf(most, ld_l2(&parts[c].most));
             most = warp_max(most);
-            for (int c = lane; c < L.chunks; c += 32) {
-                const float m = __ldcg(&parts[c].most);
-                if (m > -INFINITY) sum += __ldcg(&parts[c].sum) * exp((double)m - (double)most);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
         if (most == -INFINITY) {                          // finished, or nothing left: the lowest tokens at -infinity; in front of them a finished beam's end
             for (int i = lane; i < most_tokens; i += 32) {
@@ -267,57 +278,58 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
             if (lane == 0) G.count[b] = most_tokens;
             continue;
         }
-        u64 lo = 1;                                       // (0: nothing there)
-        int reach = kBsPicks + 1;
-        if (heads <= 32 * kBsHeads) {
-            auto at_least = [&](uint32_t x) {
-                int m = 0;
-#pragma unroll
-                for (int i = 0; i < kBsHeads; ++i) m += __popc(__ballot_sync(0xffffffffu, head[i] >= x));
-                return m;
-            };
-            uint32_t low = 1, high = beam_key(most) + 1;
-            int r = at_least(low);
-            while (r > k + kBsWindow && high - low > 1) {
-                const uint32_t mid = low + (high - low) / 2;
-                const int m = at_least(mid);
-                if (m >= k) { low = mid; r = m; } else high = mid;
-            }
-            if (r >= k) lo = (u64)low << 32;              // (fewer: the row has no k)
+        double sum = 0.0;
+        for (int c = lane; c < L.chunks; c += 32) {
+            const float m = ld_l2(&parts[c].most);
+            if (m > -INFINITY) sum += ld_l2(&parts[c].sum) * exp((double)m - (double)most);
         }
-        for (int pass = 0; pass < 2; ++pass) {
-            if (lane == 0) G.picked[warp] = 0;
-            __syncwarp();
-            for (int i0 = 0; i0 < n; i0 += 32 * 8) {
-                u64 e[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) e[u] = i0 + 32 * u + lane < n ? __ldcg(list + i0 + 32 * u + lane) : 0ull;
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if (e[u] >= lo) {
-                        const int at = atomicAdd(&G.picked[warp], 1);
-                        if (at < kBsPicks) G.pick[warp][at] = e[u];
-                    }
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const double lse = (double)most + log(sum);
+        // ---- a bound that k entries reach, and hardly more: the k-th of every lane's two largest logits ----------------------------
+        uint32_t one = 0, two = 0;
+        each([&](u64 e) {
+            const uint32_t x = (uint32_t)(e >> 32);
+            two = max(two, min(one, x));
+            one = max(one, x);
+        });
+        u64 lo = 1;                                       // (0: nothing there)
+        {
+            auto at_least = [&](uint32_t x) { return __popc(__ballot_sync(0xffffffffu, one >= x)) + __popc(__ballot_sync(0xffffffffu, two >= x)); };
+            uint32_t low = 1, high = beam_key(most) + 1;
+            int reach = at_least(low);
+            if (reach >= k) {                             // (else all there is: fewer than two a lane)
+                while (reach > k && high - low > 1) {
+                    const uint32_t mid = low + (high - low) / 2;
+                    const int m = at_least(mid);
+                    if (m >= k) { low = mid; reach = m; } else high = mid;
+                }
+                lo = (u64)low << 32;
             }
-            __syncwarp();
-            reach = G.picked[warp];
-            __syncwarp();
-            if (reach <= kBsPicks || pass) break;
-            // Too many alike, or a great many lists: the k-th of all entries, which differ, by bisection over the memory.
-            auto at_least = [&](u64 x) {
+            // More than can be ranked (many alike, or in few lanes): the k-th of all entries, which differ.
+            auto entries = [&](u64 x) {
                 int m = 0;
-                for (int i = lane; i < n; i += 32) m += __ldcg(list + i) >= x;
+                each([&](u64 e) { m += e >= x; });
                 return (int)__reduce_add_sync(0xffffffffu, (unsigned)m);
             };
+            reach = entries(lo);
             u64 hi = ((u64)beam_key(most) + 1) << 32;
             while (reach > kBsPicks && hi - lo > 1) {
                 const u64 mid = lo + (hi - lo) / 2;
-                const int m = at_least(mid);
+                const int m = entries(mid);
                 if (m >= k) { lo = mid; reach = m; } else hi = mid;
             }
         }
-        const double lse = (double)most + log(sum);
-        const int m = min(reach, kBsPicks);
+        if (lane == 0) G.picked[warp] = 0;
+        __syncwarp();
+        each([&](u64 e) {
+            if (e >= lo) {
+                const int at = atomicAdd(&G.picked[warp], 1);
+                if (at < kBsPicks) G.pick[warp][at] = e;
+            }
+        });
+        __syncwarp();
+        const int m = min(G.picked[warp], kBsPicks);
         for (int i = lane; i < m; i += 32) {
             const u64 e = G.pick[warp][i];
             int before = 0;
@@ -357,9 +369,12 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
 }
 
 // Logits a thread takes: 32, or fewer where that would leave SMs without a CTA.
-static int beam_per(int rows, int vocab) {
+// (and lists would no longer be held in registers by the second kernel).
+static int beam_chunks(int per, int vocab) { return (int)(((long long)vocab + kBsThreads * per - 1) / (kBsThreads * per)); }
+static int beam_slots(int k) { return (k > kBsLeast ? k : kBsLeast) + 2 * kBsWindow; }
+static int beam_per(int rows, int vocab, int k) {
     int per = kBsMostPer;
-    while (per > 4 && (long long)rows * ((vocab + kBsThreads * per - 1) / (kBsThreads * per)) < 128) per /= 2;
+    while (per > 4 && (long long)rows * beam_chunks(per, vocab) < 128 && (long long)beam_chunks(per / 2, vocab) * beam_slots(k) <= 32 * kBsHold) per /= 2;
     return per;
 }
 
@@ -373,9 +388,8 @@ static int beam_rows_run(const BeamLaunch& L, cudaStream_t st) {
 
 extern "C" size_t tenzo_cuda_beam_select_workspace_bytes(int groups, int beams, int vocab, int k) {
     if (groups <= 0 || beams <= 0 || vocab <= 0 || k <= 0 || (long long)groups * beams > 0x7fffffffLL) return 0;
-    const int per = tz::beam_per(groups * beams, vocab);
-    const size_t chunks = ((size_t)vocab + tz::kBsThreads * per - 1) / ((size_t)tz::kBsThreads * per);
-    return (size_t)groups * beams * chunks * (sizeof(tz::BeamPart) + (size_t)k * sizeof(tz::u64));
+    const size_t chunks = (size_t)tz::beam_chunks(tz::beam_per(groups * beams, vocab, k), vocab);
+    return (size_t)groups * beams * chunks * (sizeof(tz::BeamPart) + (size_t)tz::beam_slots(k) * sizeof(tz::u64));
 }
 
 extern "C" int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* stream) {
@@ -393,9 +407,10 @@ extern "C" int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* 
     if (a.row_stride < a.vocab) return -1;
     const long long rows = (long long)a.groups * a.beams;
     if (rows > 0x7fffffffLL) return -1;
-    L.per = beam_per((int)rows, a.vocab);
-    L.chunks = (int)(((long long)a.vocab + kBsThreads * L.per - 1) / (kBsThreads * L.per));
-    if (rows * L.chunks > 0x7fffffffLL || (long long)L.chunks * a.k > 0x7fffffffLL || (long long)L.chunks * kBsThreads * L.per > 0x7fffffffLL) return -1;
+    L.per = beam_per((int)rows, a.vocab, a.k);
+    L.chunks = beam_chunks(L.per, a.vocab);
+    L.slots = beam_slots(a.k);
+    if (rows * L.chunks > 0x7fffffffLL || (long long)L.chunks * L.slots > 0x7fffffffLL || (long long)L.chunks * kBsThreads * L.per > 0x7fffffffLL) return -1;
     if (a.workspace_bytes < tenzo_cuda_beam_select_workspace_bytes(a.groups, a.beams, a.vocab, a.k)) return -1;
     L.parts = static_cast<BeamPart*>(a.workspace);
     L.lists = reinterpret_cast<u64*>(L.parts + (size_t)rows * L.chunks);

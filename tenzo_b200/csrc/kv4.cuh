@@ -22,6 +22,26 @@ __device__ __forceinline__ size_t kv4_page(const tenzo_kv4_cache& c, int layer, 
     return (((size_t)block * c.n_layers + layer) * c.n_kv + kvh) * kK4Page;
 }
 
+// Loads of what the kernel in front may have written, from L2. They are volatile so that none moves in front of the wait for that kernel: the
+// compiler may hoist a load through a const __restrict__ pointer, an __ldg or an __ldcg above it (a table of parents was read early that way, once in some
+// hundred launches).
+__device__ __forceinline__ int ld_l2(const int* p) { int v; asm volatile("ld.global.cg.b32 %0, [%1];" : "=r"(v) : "l"(p)); return v; }
+__device__ __forceinline__ uint32_t ld_l2(const uint32_t* p) { uint32_t v; asm volatile("ld.global.cg.b32 %0, [%1];" : "=r"(v) : "l"(p)); return v; }
+__device__ __forceinline__ float ld_l2(const float* p) { float v; asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p)); return v; }
+__device__ __forceinline__ double ld_l2(const double* p) { double v; asm volatile("ld.global.cg.f64 %0, [%1];" : "=d"(v) : "l"(p)); return v; }
+__device__ __forceinline__ unsigned long long ld_l2(const unsigned long long* p) { unsigned long long v; asm volatile("ld.global.cg.b64 %0, [%1];" : "=l"(v) : "l"(p)); return v; }
+__device__ __forceinline__ float2 ld_l2(const float2* p) { float2 v; asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p)); return v; }
+__device__ __forceinline__ float4 ld_l2(const float4* p) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 ld_l2(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 inline bool kv4_cache_ok(const tenzo_kv4_cache& c) {
     return c.pool && c.block_table && !(reinterpret_cast<uintptr_t>(c.pool) & 15) && c.n_blocks > 0 && c.n_layers > 0 && c.n_kv > 0 && c.table_rows > 0 &&
            c.table_stride > 0;

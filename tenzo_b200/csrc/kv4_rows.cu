@@ -22,7 +22,7 @@ __device__ __forceinline__ uint8_t* row_place(const tenzo_kv4_cache& c, int laye
     if (pos < 0) return nullptr;
     const int col = pos / kK4Slots;
     int block = -1;
-    if (seq >= 0 && seq < c.table_rows && col < c.table_stride && pos < rope_len) block = __ldg(c.block_table + (size_t)seq * c.table_stride + col);
+    if (seq >= 0 && seq < c.table_rows && col < c.table_stride && pos < rope_len) block = ld_l2(c.block_table + (size_t)seq * c.table_stride + col);
     if (block < 0 || block >= c.n_blocks) {
         atomicOr(&g_kv4_rows_error, kK4ErrIndex);
         return nullptr;
@@ -40,26 +40,26 @@ struct RowsArgs {
 template <bool VEC>
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
     if (VEC) {
-        const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
+        const float4 a = ld_l2(reinterpret_cast<const float4*>(p)), b = ld_l2(reinterpret_cast<const float4*>(p) + 1);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __ldcg(p + j);
+        for (int j = 0; j < 8; ++j) x[j] = ld_l2(p + j);
     }
 }
 
 template <bool VEC, bool ROPE>
-__global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsArgs a, const float* __restrict__ k, const float* __restrict__ v) {
+__global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsArgs a, const float* k, const float* v) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
     if (a.use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
     if (row >= a.rows) return;
-    const int pos = a.pos[row];
+    const int pos = ld_l2(a.pos + row);
     float x[8];
     load8<VEC>((is_v ? v : k) + (size_t)row * a.kv_stride + kvh * 128 + 8 * l, x);      // (padding rows are there to be read too)
-    uint8_t* at = row_place(a.c, a.layer, kvh, pos, a.seq ? a.seq[row] : row, ROPE ? a.rope_len : 0x7fffffff);
+    uint8_t* at = row_place(a.c, a.layer, kvh, pos, a.seq ? ld_l2(a.seq + row) : row, ROPE ? a.rope_len : 0x7fffffff);
     if (!at) return;                                     // the whole warp
     if (ROPE) {
         const float* cs = a.cs + (size_t)pos * 64 + ((8 * l) & 63);
@@ -103,19 +103,19 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsAr
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kRowWarps * 32) kv4_read_kernel(const RowsArgs a, float* __restrict__ k, float* __restrict__ v) {
+__global__ void __launch_bounds__(kRowWarps * 32) kv4_read_kernel(const RowsArgs a, float* k, float* v) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
     if (a.use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
     if (row >= a.rows) return;
-    const uint8_t* at = row_place(a.c, a.layer, kvh, a.pos[row], a.seq ? a.seq[row] : row, 0x7fffffff);
+    const uint8_t* at = row_place(a.c, a.layer, kvh, ld_l2(a.pos + row), a.seq ? ld_l2(a.seq + row) : row, 0x7fffffff);
     float x[8] = {};
     if (at) {
         at += is_v * kK4Half;
-        const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(at) + l);
-        const uint32_t pair = __ldcg(reinterpret_cast<const uint32_t*>(at + kK4Codes) + (l >> 2));
+        const uint32_t word = ld_l2(reinterpret_cast<const uint32_t*>(at) + l);
+        const uint32_t pair = ld_l2(reinterpret_cast<const uint32_t*>(at + kK4Codes) + (l >> 2));
         const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&pair));
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = p.y + p.x * (float)((word >> (4 * j)) & 15u);
@@ -139,17 +139,17 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_read_kernel(const RowsArgs
 // CTA (x, y): beam x, part y of the copy. Bound by memory: length % 16 rows of 80 bytes, layers x heads x 2 times, in and out.
 constexpr int kReorderThreads = 256, kReorderParts = 8;
 
-__global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenzo_kv4_cache c, int* __restrict__ table_out, const int* __restrict__ parent,
-                                                                      const int* __restrict__ length, int beams, int use_pdl) {
+__global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenzo_kv4_cache c, int* table_out, const int* parent,
+                                                                      const int* length, int beams, int use_pdl) {
     const int g = blockIdx.x / beams, i = blockIdx.x % beams, lane = threadIdx.x & 31;
     if (use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
     const int* rows = c.block_table + (size_t)g * beams * c.table_stride;      // the group's
-    const int len = length[g], col = len / kK4Slots, filled = len < 0 ? 0 : len % kK4Slots;
+    const int len = ld_l2(length + g), col = len / kK4Slots, filled = len < 0 ? 0 : len % kK4Slots;
     const bool mine = lane < beams;
-    int p = mine ? parent[(size_t)g * beams + lane] : lane;
+    int p = mine ? ld_l2(parent + (size_t)g * beams + lane) : lane;
     const bool bad = (mine && (p < 0 || p >= beams)) || len < 0 || col + (filled > 0) > c.table_stride;
     const bool refused = __any_sync(0xffffffffu, bad);
     if (refused) {                                       // the group stays as it is
@@ -171,10 +171,10 @@ __global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenz
     if (blockIdx.y == 0) {
         int* out = table_out + ((size_t)g * beams + i) * c.table_stride;
         for (int x = threadIdx.x; x < c.table_stride; x += kReorderThreads)
-            out[x] = refused ? rows[(size_t)i * c.table_stride + x] : rows[(size_t)(x < col ? from : x == col ? giver : i) * c.table_stride + x];
+            out[x] = ld_l2(rows + (size_t)(refused ? i : x < col ? from : x == col ? giver : i) * c.table_stride + x);
     }
     if (!copies) return;
-    const int source = rows[(size_t)from * c.table_stride + col], target = rows[(size_t)giver * c.table_stride + col];
+    const int source = ld_l2(rows + (size_t)from * c.table_stride + col), target = ld_l2(rows + (size_t)giver * c.table_stride + col);
     if (source < 0 || source >= c.n_blocks || target < 0 || target >= c.n_blocks) {
         if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&g_kv4_rows_error, kK4ErrIndex);
         return;
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenz
     uint4* dst = reinterpret_cast<uint4*>(c.pool + (size_t)target * halves * kK4Half);
     constexpr int kUnits = kK4Half / 16;
     for (int h = blockIdx.y * (kReorderThreads / 32) + (threadIdx.x >> 5); h < halves; h += kReorderParts * (kReorderThreads / 32))
-        for (int u = lane; u < units; u += 32) dst[(size_t)h * kUnits + u] = __ldcg(src + (size_t)h * kUnits + u);
+        for (int u = lane; u < units; u += 32) dst[(size_t)h * kUnits + u] = ld_l2(src + (size_t)h * kUnits + u);
 }
 
 static bool aligned16(const void* p) { return !(reinterpret_cast<uintptr_t>(p) & 15); }
