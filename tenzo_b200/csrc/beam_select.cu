@@ -7,8 +7,8 @@
 //      lower bound of the chunk's k-th largest logit, and hardly more logits reach it: those are listed, and their exponentials summed in 64
 //      bits. All others' are summed in 32 (hardware ex2, about 1e-7 each, and 16 larger ones at least are on the list): the
 //      logarithm of the whole is good to some 1e-9 whether a few tokens have all the weight or thousands share it.
-//   2. A CTA a group, a warp a row: the k best of the lists. An entry's place in the group is its place in its row and, by bisection, the
-//      number of better ones in each other row.
+//   2. A CTA a group, a warp a row: the k best of the lists, with their scores; then the rows' scores that reach a common border are ranked
+//      among one another.
 // Sums are taken in an order that the data alone decides, or as integers, so that equal rows get equal sums and tie.
 //
 // The first kernel reads 4 bytes a logit; what bounds it besides is some ten instructions and an ex2 (8 cycles of its unit a warp) for each.
@@ -26,7 +26,7 @@ constexpr int kBsMostK = 2 * TENZO_BEAMS_MOST;
 constexpr int kBsMostPer = 32;                            // logits a thread holds at most
 constexpr int kBsList = (kBsMostK + kBsWindow) * kBsMostPer;      // candidates lie in that many threads' logits
 constexpr int kBsMergeWarps = 16;                         // rows that the second kernel merges at a time
-constexpr int kBsHold = 32;                               // entries of a row's lists that a lane keeps
+constexpr int kBsHold = 1280;                             // entries of a row's lists that a warp keeps: 16 chunks of the most slots
 constexpr int kBsPicks = 96;                              // entries that are ranked; more than k + kBsWindow
 
 constexpr double kBsUnit = 281474976710656.0;             // 2^48
@@ -50,13 +50,14 @@ struct __align__(16) BeamPart {                           // of a chunk
 struct BeamLaunch {
     tenzo_beam_select_args a;
     int per, chunks, slots;                               // logits a thread takes, chunks a row, entries a chunk's list has room for
+    int eager;                                            // few CTAs: time counts, not the bytes of rows that are left out
     BeamPart* parts;                                      // [row][chunk]
     u64* lists;                                           // [row][chunk][slots], in any order; 0 where there is none
 };
 
 // Rows that the first kernel leaves out: finished beams, and those whose score is -infinity (or NaN).
 __device__ __forceinline__ bool beam_dead(float cum) { return !(cum > -INFINITY); }
-__device__ __forceinline__ bool beam_done(const tenzo_beam_select_args& a, int row, float cum) { return a.finished && ld_l2(a.finished + row) != 0 && !beam_dead(cum); }
+__device__ __forceinline__ bool beam_finished(const tenzo_beam_select_args& a, int row) { return a.finished && ld_l2(a.finished + row) != 0; }
 
 template <bool VEC, int PER>
 __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch L) {
@@ -72,7 +73,8 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     pdl_launch_dependents();                              // the second kernel waits for this one, whatever its neighbours do
     if (a.use_pdl) pdl_wait();
     const float cum = ld_l2(a.scores + row);
-    if (beam_dead(cum) || beam_done(a, row, cum)) return;
+    const bool out = beam_finished(a, row) || beam_dead(cum);
+    if (!L.eager && out) return;                          // (eager: the logits are asked for meanwhile)
     const float* x = a.logits + (size_t)row * a.row_stride;
     const int base = chunk * kBsThreads * PER;
     // place of the j-th logit of a thread: consecutive fours (or ones) go to consecutive threads
@@ -97,6 +99,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
 #pragma unroll
         for (int j = 0; j < PER; ++j) v[j] = place(j) < a.vocab ? ld_l2(x + place(j)) : -INFINITY;
     }
+    if (out) return;
     if (tid == 0) {
         s_n = 0;
         s_listed = 0;
@@ -233,137 +236,193 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     }
 }
 
+// Order of the scores as integers, and back. (No score is NaN.)
+__device__ __forceinline__ u64 score_key(double f) {
+    const u64 b = f == 0.0 ? 0ull : (u64)__double_as_longlong(f);
+    return (b >> 63) ? ~b : (b | 1ull << 63);
+}
+__device__ __forceinline__ double score_of(u64 k) { return __longlong_as_double((long long)((k >> 63) ? (k & ~(1ull << 63)) : ~k)); }
+
 struct BeamGroup {
-    double score[TENZO_BEAMS_MOST][kBsMostK];             // a row's best, in order
+    u64 score[TENZO_BEAMS_MOST][kBsMostK];                // keys of a row's best, in order
     int token[TENZO_BEAMS_MOST][kBsMostK];
     int count[TENZO_BEAMS_MOST];
     u64 pick[kBsMergeWarps][kBsPicks];                    // what a warp found, unsorted
-    int picked[kBsMergeWarps];
+    u64 live[TENZO_BEAMS_MOST * kBsMostK];                // scores that may be among the group's best, and whose they are: 64 beam + place
+    unsigned short whose[TENZO_BEAMS_MOST * kBsMostK];
+    int n_live;
 };
 
-__global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const BeamLaunch L) {
-    __shared__ BeamGroup G;
+// Its loops are not unrolled further than their loads ask for: every instruction runs a few times only, and a kernel's first pass through its
+// code waits for the code. Dynamic shared memory: the group, then `hold` entries a warp (0: the lists are longer and read from L2).
+__global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const BeamLaunch L, const int hold) {
+    extern __shared__ __align__(16) unsigned char bs_smem[];
+    BeamGroup& G = *reinterpret_cast<BeamGroup*>(bs_smem);
     const tenzo_beam_select_args& a = L.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, k = a.k;
+    const unsigned below = (1u << lane) - 1u;
+    u64* room = reinterpret_cast<u64*>(bs_smem + (sizeof(BeamGroup) + 15) / 16 * 16) + (size_t)warp * hold;
     pdl_launch_dependents();
     pdl_wait();
+    if (tid == 0) G.n_live = 0;
+#pragma unroll 1
     for (int b = warp; b < a.beams; b += kBsMergeWarps) {
-        const int row = g * a.beams + b, most_tokens = min(k, a.vocab), n = L.chunks * L.slots;
+        const int row = g * a.beams + b, most_tokens = min(k, a.vocab), n = L.chunks * L.slots;      // (an even number)
         const BeamPart* parts = L.parts + (size_t)row * L.chunks;
         const u64* list = L.lists + (size_t)row * n;
-        const bool held = n <= 32 * kBsHold;              // in registers; more are read again whenever they are needed
-        u64 mine[kBsHold];                                // (asked for first: of a row left out they mean nothing)
-#pragma unroll
-        for (int i = 0; i < kBsHold; ++i) mine[i] = held && lane + 32 * i < n ? ld_l2(list + lane + 32 * i) : 0ull;
-        auto each = [&](auto&& f) {
-            if (held) {
-#pragma unroll
-                for (int i = 0; i < kBsHold; ++i) f(mine[i]);
-            } else {
-                for (int i = lane; i < n; i += 32) f(ld_l2(list + i));
-            }
-        };
         const float cum = ld_l2(a.scores + row);
-        const bool done = beam_done(a, row, cum);
+        const bool finished = beam_finished(a, row), done = finished && !beam_dead(cum);
+        float first_most = -INFINITY;                     // of the lane's first chunk
+        double first_sum = 0.0;
+        if (lane < L.chunks) {
+            first_most = ld_l2(&parts[lane].most);
+            first_sum = ld_l2(&parts[lane].sum);
+        }
+        // the row's entries, and each lane's two largest logits (of a row that was left out they mean nothing)
+        uint32_t one = 0, two = 0;
+#pragma unroll 8
+        for (int i = lane; i < n / 2; i += 32) {
+            const uint4 e = ld_l2(reinterpret_cast<const uint4*>(list) + i);                       // two entries: token, logit, token, logit
+            if (hold) reinterpret_cast<uint4*>(room)[i] = e;
+            two = max(two, min(one, e.y));
+            one = max(one, e.y);
+            two = max(two, min(one, e.w));
+            one = max(one, e.w);
+        }
+        auto entry = [&](int i) { return hold ? room[i] : ld_l2(list + i); };
         float most = -INFINITY;
-        if (!done && !beam_dead(cum)) {
-            for (int c = lane; c < L.chunks; c += 32) most = fmaxf(most, ld_l2(&parts[c].most));
+        if (!finished && !beam_dead(cum)) {
+            most = first_most;
+#pragma unroll 1
+            for (int c = lane + 32; c < L.chunks; c += 32) most = fmaxf(most, ld_l2(&parts[c].most));
             most = warp_max(most);
         }
         if (most == -INFINITY) {                          // finished, or nothing left: the lowest tokens at -infinity; in front of them a finished beam's end
             for (int i = lane; i < most_tokens; i += 32) {
                 G.token[b][i] = !done ? i : i == 0 ? a.eos : i - 1 < a.eos ? i - 1 : i;
-                G.score[b][i] = done && i == 0 ? (double)cum : -(double)INFINITY;
+                G.score[b][i] = score_key(done && i == 0 ? (double)cum : -(double)INFINITY);
             }
             if (lane == 0) G.count[b] = most_tokens;
             continue;
         }
         double sum = 0.0;
+#pragma unroll 1
         for (int c = lane; c < L.chunks; c += 32) {
-            const float m = ld_l2(&parts[c].most);
-            if (m > -INFINITY) sum += ld_l2(&parts[c].sum) * exp((double)m - (double)most);
+            if (c >= 32) {
+                first_most = ld_l2(&parts[c].most);
+                first_sum = ld_l2(&parts[c].sum);
+            }
+            if (first_most > -INFINITY) sum += first_sum * exp((double)first_most - (double)most);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const double lse = (double)most + log(sum);
-        // ---- a bound that k entries reach, and hardly more: the k-th of every lane's two largest logits ----------------------------
-        uint32_t one = 0, two = 0;
-        each([&](u64 e) {
-            const uint32_t x = (uint32_t)(e >> 32);
-            two = max(two, min(one, x));
-            one = max(one, x);
-        });
-        u64 lo = 1;                                       // (0: nothing there)
+        // ---- a bound that k of the lanes' two largest logits reach, and hardly more -------------------------------------------------
+        u64 lo = 1, hi = ((u64)beam_key(most) + 1) << 32; // (0: nothing there)
         {
             auto at_least = [&](uint32_t x) { return __popc(__ballot_sync(0xffffffffu, one >= x)) + __popc(__ballot_sync(0xffffffffu, two >= x)); };
             uint32_t low = 1, high = beam_key(most) + 1;
             int reach = at_least(low);
-            if (reach >= k) {                             // (else all there is: fewer than two a lane)
-                while (reach > k && high - low > 1) {
+            if (reach >= k) {                             // (else all there is)
+                const uint32_t least = max(1u, __reduce_min_sync(0xffffffffu, k <= 32 ? one : two));
+                if (at_least(least) >= k) low = least;
+                reach = at_least(low);
+#pragma unroll 1
+                while (reach > k + kBsWindow && high - low > 1) {
                     const uint32_t mid = low + (high - low) / 2;
                     const int m = at_least(mid);
                     if (m >= k) { low = mid; reach = m; } else high = mid;
                 }
                 lo = (u64)low << 32;
             }
-            // More than can be ranked (many alike, or in few lanes): the k-th of all entries, which differ.
-            auto entries = [&](u64 x) {
-                int m = 0;
-                each([&](u64 e) { m += e >= x; });
-                return (int)__reduce_add_sync(0xffffffffu, (unsigned)m);
-            };
-            reach = entries(lo);
-            u64 hi = ((u64)beam_key(most) + 1) << 32;
-            while (reach > kBsPicks && hi - lo > 1) {
+        }
+        // ---- the entries that reach it; more than can be ranked (many alike, or in few lanes): the k-th of all, which differ -------
+        __syncwarp();                                     // (the room)
+        int m;
+#pragma unroll 1
+        for (;;) {
+            m = 0;
+#pragma unroll 4
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const u64 e = i0 + lane < n ? entry(i0 + lane) : 0ull;
+                const unsigned in = __ballot_sync(0xffffffffu, e >= lo);
+                if (in) {
+                    const int at = m + __popc(in & below);
+                    if (e >= lo && at < kBsPicks) G.pick[warp][at] = e;
+                    m += __popc(in);
+                }
+            }
+            if (m <= kBsPicks) break;
+#pragma unroll 1
+            for (int reach = m; reach > kBsPicks && hi - lo > 1;) {
                 const u64 mid = lo + (hi - lo) / 2;
-                const int m = entries(mid);
-                if (m >= k) { lo = mid; reach = m; } else hi = mid;
+                int c = 0;
+#pragma unroll 4
+                for (int i = lane; i < n; i += 32) c += entry(i) >= mid;
+                c = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+                if (c >= k) { lo = mid; reach = c; } else hi = mid;
             }
         }
-        if (lane == 0) G.picked[warp] = 0;
         __syncwarp();
-        each([&](u64 e) {
-            if (e >= lo) {
-                const int at = atomicAdd(&G.picked[warp], 1);
-                if (at < kBsPicks) G.pick[warp][at] = e;
-            }
-        });
-        __syncwarp();
-        const int m = min(G.picked[warp], kBsPicks);
+#pragma unroll 1
         for (int i = lane; i < m; i += 32) {
             const u64 e = G.pick[warp][i];
             int before = 0;
+#pragma unroll 8
             for (int j = 0; j < m; ++j) before += G.pick[warp][j] > e;
             if (before < k) {
                 const float x = entry_logit(e);
                 G.token[b][before] = entry_token(e);
-                G.score[b][before] = x == -INFINITY ? -(double)INFINITY : (double)cum + ((double)x - lse);
+                G.score[b][before] = score_key(x == -INFINITY ? -(double)INFINITY : (double)cum + ((double)x - lse));
             }
         }
         if (lane == 0) G.count[b] = min(m, k);
         __syncwarp();
     }
     __syncthreads();
-    for (int i = tid; i < a.beams * k; i += kBsMergeWarps * 32) {
-        const int b = i / k, p = i % k;
-        if (p >= G.count[b]) continue;
-        const double score = G.score[b][p];
-        int before = p;
-        for (int o = 0; o < a.beams && before < k; ++o) {
-            if (o == b) continue;
-            int lo = 0, hi = G.count[o];                  // the number in front: larger scores, and equal ones of lower beams
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                const double s = G.score[o][mid];
-                if (s > score || (s == score && o < b)) lo = mid + 1; else hi = mid;
+    // ---- a score that k entries reach: the worst of the rows' ceil(k / beams)-th, or the best of their k-th. What lies below is out. ----
+    u64 worst = ~0ull, best = 0;
+    if (lane < a.beams) {
+        const int each = (k + a.beams - 1) / a.beams, n = G.count[lane];
+        worst = n >= each ? G.score[lane][each - 1] : 0;
+        if (n >= k) best = G.score[lane][k - 1];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const u64 w = __shfl_xor_sync(0xffffffffu, worst, o), h = __shfl_xor_sync(0xffffffffu, best, o);
+        worst = w < worst ? w : worst;
+        best = h > best ? h : best;
+    }
+    const u64 border = worst > best ? worst : best;
+#pragma unroll 1
+    for (int b = warp; b < a.beams; b += kBsMergeWarps)
+#pragma unroll 1
+        for (int p = lane; p < G.count[b]; p += 32) {
+            const u64 score = G.score[b][p];
+            if (score >= border) {
+                const int at = atomicAdd(&G.n_live, 1);
+                G.live[at] = score;
+                G.whose[at] = (unsigned short)(kBsMostK * b + p);
             }
-            before += lo;
+        }
+    __syncthreads();
+    const int n = G.n_live;
+#pragma unroll 1
+    for (int i = tid; i < n; i += kBsMergeWarps * 32) {
+        const u64 score = G.live[i];
+        const int whose = G.whose[i];
+        int before = 0;                                   // larger scores, and equal ones of lower beams, or in front in its own
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+            const u64 other = G.live[j];
+            before += other > score;
+            if (other == score) before += G.whose[j] < whose;
         }
         if (before < k) {
             const size_t to = (size_t)g * k + before;
-            a.parent_out[to] = b;
-            a.token_out[to] = G.token[b][p];
-            a.score_out[to] = (float)score;
+            a.parent_out[to] = whose / kBsMostK;
+            a.token_out[to] = G.token[whose / kBsMostK][whose % kBsMostK];
+            a.score_out[to] = (float)score_of(score);
         }
     }
 }
@@ -374,9 +433,12 @@ static int beam_chunks(int per, int vocab) { return (int)(((long long)vocab + kB
 static int beam_slots(int k) { return (k > kBsLeast ? k : kBsLeast) + 2 * kBsWindow; }
 static int beam_per(int rows, int vocab, int k) {
     int per = kBsMostPer;
-    while (per > 4 && (long long)rows * beam_chunks(per, vocab) < 128 && (long long)beam_chunks(per / 2, vocab) * beam_slots(k) <= 32 * kBsHold) per /= 2;
+    while (per > 4 && (long long)rows * beam_chunks(per, vocab) < 128 && (long long)beam_chunks(per / 2, vocab) * beam_slots(k) <= kBsHold) per /= 2;
     return per;
 }
+
+static size_t beam_groups_smem(int hold) { return (sizeof(BeamGroup) + 15) / 16 * 16 + (size_t)kBsMergeWarps * hold * sizeof(u64); }
+static_assert((sizeof(BeamGroup) + 15) / 16 * 16 + (size_t)kBsMergeWarps * kBsHold * sizeof(u64) <= kMaxSmem, "what an SM has");
 
 template <bool VEC>
 static int beam_rows_run(const BeamLaunch& L, cudaStream_t st) {
@@ -410,12 +472,15 @@ extern "C" int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* 
     L.per = beam_per((int)rows, a.vocab, a.k);
     L.chunks = beam_chunks(L.per, a.vocab);
     L.slots = beam_slots(a.k);
+    L.eager = rows * L.chunks <= 592;
     if (rows * L.chunks > 0x7fffffffLL || (long long)L.chunks * L.slots > 0x7fffffffLL || (long long)L.chunks * kBsThreads * L.per > 0x7fffffffLL) return -1;
     if (a.workspace_bytes < tenzo_cuda_beam_select_workspace_bytes(a.groups, a.beams, a.vocab, a.k)) return -1;
     L.parts = static_cast<BeamPart*>(a.workspace);
     L.lists = reinterpret_cast<u64*>(L.parts + (size_t)rows * L.chunks);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool vec = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.row_stride % 4 == 0;
+    if (cudaError_t e = allow_smem(beam_groups_kernel, beam_groups_smem(kBsHold))) return (int)e;
     if (int rc = vec ? beam_rows_run<true>(L, st) : beam_rows_run<false>(L, st)) return rc;
-    return kv4_launch(beam_groups_kernel, dim3((unsigned)a.groups), kBsMergeWarps * 32, 0, st, true, L);
+    const int entries = L.chunks * L.slots, hold = entries <= kBsHold ? (entries + 1) / 2 * 2 : 0;
+    return kv4_launch(beam_groups_kernel, dim3((unsigned)a.groups), kBsMergeWarps * 32, beam_groups_smem(hold), st, true, L, hold);
 }
