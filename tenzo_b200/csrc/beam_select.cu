@@ -60,11 +60,11 @@ __device__ __forceinline__ bool beam_dead(float cum) { return !(cum > -INFINITY)
 __device__ __forceinline__ bool beam_finished(const tenzo_beam_select_args& a, int row) { return a.finished && ld_l2(a.finished + row) != 0; }
 
 template <bool VEC, int PER>
-__global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch L) {
+__global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaunch L) {
     __shared__ uint32_t s_keys[kBsThreads];
     __shared__ u64 s_list[kBsList], s_sorted[kBsList];
     __shared__ double s_sum[kBsWarps];
-    __shared__ u64 s_listed;
+    __shared__ u64 s_listed[kBsWarps];
     __shared__ float s_red[kBsWarps];
     __shared__ uint32_t s_bound;
     __shared__ int s_short, s_last, s_n;
@@ -102,7 +102,6 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     if (out) return;
     if (tid == 0) {
         s_n = 0;
-        s_listed = 0;
     }
     // ---- what counts: NaN as -infinity, infinity as the largest number; the largest of all ------------------------------------
     float top = -INFINITY;
@@ -206,12 +205,17 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    int n = min(s_n, kBsList);
+    const int listed_n = min(s_n, kBsList);
+    int n = listed_n;
     const u64* list = s_list;
-    if (most > -INFINITY) {                               // the listed ones' exponentials, in units of 2^-48: whole numbers add up the same in any order
+    if (32 * warp < n) {                                  // the listed ones' exponentials, in units of 2^-48: whole numbers add up the same in any order
         u64 mine = 0;
-        for (int i = tid; i < n; i += kBsThreads) mine += (u64)__double2ll_rn(exp((double)entry_logit(s_list[i]) - (double)most) * kBsUnit);
-        if (mine) atomicAdd(&s_listed, mine);
+#pragma unroll 1
+        for (int i = tid; i < n; i += kBsThreads)
+            if (most > -INFINITY) mine += (u64)__double2ll_rn(exp((double)entry_logit(s_list[i]) - (double)most) * kBsUnit);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        if (lane == 0) s_listed[warp] = mine;
     }
     if (n > L.slots) {                                    // (many large ones in few threads) the best k go on
         for (int i = tid; i < n; i += kBsThreads) {
@@ -228,7 +232,9 @@ __global__ void __launch_bounds__(kBsThreads) beam_rows_kernel(const BeamLaunch 
     if (tid < L.slots) to[tid] = tid < n ? list[tid] : 0ull;
     if (tid == 0) {
         BeamPart p;
-        p.sum = (double)s_listed * (1.0 / kBsUnit);
+        u64 listed = 0;
+        for (int w = 0; w < kBsWarps && 32 * w < listed_n; ++w) listed += s_listed[w];
+        p.sum = (double)listed * (1.0 / kBsUnit);
 #pragma unroll
         for (int w = 0; w < kBsWarps; ++w) p.sum += s_sum[w];
         p.most = most;
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
             two = max(two, min(one, e.w));
             one = max(one, e.w);
         }
-        auto entry = [&](int i) { return hold ? room[i] : ld_l2(list + i); };
+        const u64* entry = hold ? room : list;
         float most = -INFINITY;
         if (!finished && !beam_dead(cum)) {
             most = first_most;
@@ -342,14 +348,16 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
 #pragma unroll 1
         for (;;) {
             m = 0;
-#pragma unroll 4
-            for (int i0 = 0; i0 < n; i0 += 32) {
-                const u64 e = i0 + lane < n ? entry(i0 + lane) : 0ull;
-                const unsigned in = __ballot_sync(0xffffffffu, e >= lo);
-                if (in) {
-                    const int at = m + __popc(in & below);
-                    if (e >= lo && at < kBsPicks) G.pick[warp][at] = e;
-                    m += __popc(in);
+#pragma unroll 2
+            for (int i0 = 0; i0 < n; i0 += 64) {          // two entries a lane
+                const int i = i0 + 2 * lane;
+                const ulonglong2 e = i < n ? *reinterpret_cast<const ulonglong2*>(entry + i) : make_ulonglong2(0, 0);
+                const unsigned in0 = __ballot_sync(0xffffffffu, e.x >= lo), in1 = __ballot_sync(0xffffffffu, e.y >= lo);
+                if (in0 | in1) {
+                    const int at0 = m + __popc(in0 & below), at1 = m + __popc(in0) + __popc(in1 & below);
+                    if (e.x >= lo && at0 < kBsPicks) G.pick[warp][at0] = e.x;
+                    if (e.y >= lo && at1 < kBsPicks) G.pick[warp][at1] = e.y;
+                    m += __popc(in0) + __popc(in1);
                 }
             }
             if (m <= kBsPicks) break;
@@ -358,7 +366,7 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
                 const u64 mid = lo + (hi - lo) / 2;
                 int c = 0;
 #pragma unroll 4
-                for (int i = lane; i < n; i += 32) c += entry(i) >= mid;
+                for (int i = lane; i < n; i += 32) c += entry[i] >= mid;
                 c = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
                 if (c >= k) { lo = mid; reach = c; } else hi = mid;
             }

@@ -315,8 +315,8 @@ def beam_select(logits, scores, *, beams, k, finished=None, eos=0, use_pdl=False
     if groups * beams != rows or scores.shape != (rows,):
         raise ValueError(f"{rows} rows of logits are no groups of {beams} beams with one score each")
     device = logits.device
-    parent = torch.empty(groups, k, dtype=torch.int32, device=device)
-    token, score = torch.empty_like(parent), torch.empty(groups, k, dtype=torch.float32, device=device)
+    parent, token, score = torch.empty(3, groups, k, dtype=torch.int32, device=device).unbind(0)
+    score = score.view(torch.float32)
     if workspace is None:
         workspace = torch.empty(_beam_calls()[6](groups, beams, vocab, k), dtype=torch.uint8, device=device)
     args = _BEAM_SELECT.pack(lp, _arg(scores, torch.float32, dev, "scores"), _arg_entries(finished, rows, dev, "finished"), eos, stride, groups, beams, vocab, k,
