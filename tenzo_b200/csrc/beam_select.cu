@@ -389,30 +389,46 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
     }
     __syncthreads();
     // ---- a score that k entries reach: the worst of the rows' ceil(k / beams)-th, or the best of their k-th. What lies below is out. ----
-    u64 worst = ~0ull, best = 0;
+    u64 worst = ~0ull, best = 0, first = 0;
     if (lane < a.beams) {
         const int each = (k + a.beams - 1) / a.beams, n = G.count[lane];
         worst = n >= each ? G.score[lane][each - 1] : 0;
+        first = n ? G.score[lane][0] : 0;
         if (n >= k) best = G.score[lane][k - 1];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const u64 w = __shfl_xor_sync(0xffffffffu, worst, o), h = __shfl_xor_sync(0xffffffffu, best, o);
+        const u64 w = __shfl_xor_sync(0xffffffffu, worst, o), h = __shfl_xor_sync(0xffffffffu, best, o), f = __shfl_xor_sync(0xffffffffu, first, o);
         worst = w < worst ? w : worst;
         best = h > best ? h : best;
+        first = f > first ? f : first;
     }
-    const u64 border = worst > best ? worst : best;
+    u64 border = worst > best ? worst : best, high = first + 1;
+    // ... and closer to the k-th, by bisection over all (a place of the rows' lists a thread).
+    auto place = [&](int i) { return i < a.beams * kBsMostK && i % kBsMostK < G.count[i / kBsMostK] ? G.score[i / kBsMostK][i % kBsMostK] : 0ull; };
+    auto reaching = [&](u64 x) {
+        int c = 0;
 #pragma unroll 1
-    for (int b = warp; b < a.beams; b += kBsMergeWarps)
+        for (int i0 = 0; i0 < a.beams * kBsMostK; i0 += kBsMergeWarps * 32) c += __syncthreads_count(place(i0 + tid) >= x);
+        return c;
+    };
+    if (border == 0) border = 1;                          // (no score has the key 0)
+    int reach = reaching(border);
 #pragma unroll 1
-        for (int p = lane; p < G.count[b]; p += 32) {
-            const u64 score = G.score[b][p];
-            if (score >= border) {
-                const int at = atomicAdd(&G.n_live, 1);
-                G.live[at] = score;
-                G.whose[at] = (unsigned short)(kBsMostK * b + p);
-            }
+    while (reach > k + 64 && high - border > 1) {       // (so many are ranked in less time than another step takes)
+        const u64 mid = border + (high - border) / 2;
+        const int c = reaching(mid);
+        if (c >= k) { border = mid; reach = c; } else high = mid;
+    }
+#pragma unroll 1
+    for (int i = tid; i < a.beams * kBsMostK; i += kBsMergeWarps * 32) {
+        const u64 score = place(i);
+        if (score >= border) {
+            const int at = atomicAdd(&G.n_live, 1);
+            G.live[at] = score;
+            G.whose[at] = (unsigned short)i;
         }
+    }
     __syncthreads();
     const int n = G.n_live;
 #pragma unroll 1
