@@ -12,7 +12,7 @@
 
 namespace tz {
 
-constexpr int kRowWarps = 4;                             // rows a CTA, one warp each
+constexpr int kRowWarps = 4;                             // warps a CTA; a warp takes R consecutive rows of one kv head
 constexpr float kFp16Most = 65504.0f;
 
 __device__ int g_kv4_rows_error = 0;
@@ -48,87 +48,118 @@ __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
     }
 }
 
-template <bool VEC, bool ROPE>
+// Lane r < R looks up the warp's r-th row; its position (-1: leave it alone) and place go to all by shuffles.
+template <int R>
+struct RowPlaces {
+    int pos;
+    uint8_t* at;
+    __device__ __forceinline__ RowPlaces(const RowsArgs& a, int row0, int kvh, int rope_len) : pos(-1), at(nullptr) {
+        const int lane = threadIdx.x & 31, row = row0 + lane;
+        if (lane < R && row < a.rows) {
+            pos = ld_l2(a.pos + row);
+            at = row_place(a.c, a.layer, kvh, pos, a.seq ? ld_l2(a.seq + row) : row, rope_len);
+        }
+    }
+    __device__ __forceinline__ uint8_t* place(int r) const { return reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), r)); }
+    __device__ __forceinline__ int position(int r) const { return __shfl_sync(0xffffffffu, pos, r); }
+};
+
+template <bool VEC, bool ROPE, int R>
 __global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsArgs a, const float* k, const float* v) {
-    const int lane = threadIdx.x & 31, row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
+    const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * R, kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
     if (a.use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
-    if (row >= a.rows) return;
-    const int pos = ld_l2(a.pos + row);
-    float x[8];
-    load8<VEC>((is_v ? v : k) + (size_t)row * a.kv_stride + kvh * 128 + 8 * l, x);      // (padding rows are there to be read too)
-    uint8_t* at = row_place(a.c, a.layer, kvh, pos, a.seq ? ld_l2(a.seq + row) : row, ROPE ? a.rope_len : 0x7fffffff);
-    if (!at) return;                                     // the whole warp
-    if (ROPE) {
-        const float* cs = a.cs + (size_t)pos * 64 + ((8 * l) & 63);
-        const float* sn = a.sn + (size_t)pos * 64 + ((8 * l) & 63);
-        float c[8], s[8];
-        load8<VEC>(cs, c);
-        load8<VEC>(sn, s);
+    if (row0 >= a.rows) return;
+    float x[R][8];
+#pragma unroll
+    for (int r = 0; r < R; ++r)                          // (padding rows are there to be read too)
+        if (row0 + r < a.rows) load8<VEC>((is_v ? v : k) + (size_t)(row0 + r) * a.kv_stride + kvh * 128 + 8 * l, x[r]);
+    const RowPlaces<R> places(a, row0, kvh, ROPE ? a.rope_len : 0x7fffffff);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        uint8_t* at = places.place(r);
+        if (!at) continue;                               // the whole warp
+        if (ROPE) {
+            const size_t of = (size_t)places.position(r) * 64 + ((8 * l) & 63);
+            float c[8], s[8];
+            load8<VEC>(a.cs + of, c);
+            load8<VEC>(a.sn + of, s);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float o = __shfl_xor_sync(0xffffffffu, x[r][j], 8);
+                const float turned = l < 8 ? __fmaf_rn(x[r][j], c[j], -(o * s[j])) : __fmaf_rn(o, s[j], x[r][j] * c[j]);
+                if (!is_v) x[r][j] = turned;
+            }
+        }
+        float lo, hi;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float o = __shfl_xor_sync(0xffffffffu, x[j], 8);
-            const float r = l < 8 ? __fmaf_rn(x[j], c[j], -(o * s[j])) : __fmaf_rn(o, s[j], x[j] * c[j]);
-            if (!is_v) x[j] = r;
+            x[r][j] = fminf(fmaxf(x[r][j], -kFp16Most), kFp16Most);
+            lo = j ? fminf(lo, x[r][j]) : x[r][j];
+            hi = j ? fmaxf(hi, x[r][j]) : x[r][j];
         }
-    }
-    float lo, hi;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        x[j] = fminf(fmaxf(x[j], -kFp16Most), kFp16Most);
-        lo = j ? fminf(lo, x[j]) : x[j];
-        hi = j ? fmaxf(hi, x[j]) : x[j];
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const __half low = __float2half_rn(lo), scale = __float2half_rn((hi - __half2float(low)) * (1.0f / 15.0f));
-    const float m = __half2float(low), s = __half2float(scale);
-    uint32_t word = 0;
-    if (s > 0.0f) {
-        const float inv = 1.0f / s;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = __float2int_rn(fminf(fmaxf((x[j] - m) * inv, 0.0f), 15.0f));   // nearest, ties to even
-            word |= (uint32_t)c << (4 * j);
+        for (int o = 1; o < 4; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
+        const __half low = __float2half_rn(lo), scale = __float2half_rn((hi - __half2float(low)) * (1.0f / 15.0f));
+        const float m = __half2float(low), s = __half2float(scale);
+        uint32_t word = 0;
+        if (s > 0.0f) {
+            const float inv = 1.0f / s;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int c = __float2int_rn(fminf(fmaxf((x[r][j] - m) * inv, 0.0f), 15.0f));      // nearest, ties to even
+                word |= (uint32_t)c << (4 * j);
+            }
+        }
+        at += is_v * kK4Half;
+        reinterpret_cast<uint32_t*>(at)[l] = word;
+        if ((l & 3) == 0) reinterpret_cast<__half2*>(at + kK4Codes)[l >> 2] = __halves2half2(scale, low);
     }
-    at += is_v * kK4Half;
-    reinterpret_cast<uint32_t*>(at)[l] = word;
-    if ((l & 3) == 0) reinterpret_cast<__half2*>(at + kK4Codes)[l >> 2] = __halves2half2(scale, low);
 }
 
-template <bool VEC>
+template <bool VEC, int R>
 __global__ void __launch_bounds__(kRowWarps * 32) kv4_read_kernel(const RowsArgs a, float* k, float* v) {
-    const int lane = threadIdx.x & 31, row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
+    const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * R, kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
     if (a.use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
-    if (row >= a.rows) return;
-    const uint8_t* at = row_place(a.c, a.layer, kvh, ld_l2(a.pos + row), a.seq ? ld_l2(a.seq + row) : row, 0x7fffffff);
-    float x[8] = {};
-    if (at) {
-        at += is_v * kK4Half;
-        const uint32_t word = ld_l2(reinterpret_cast<const uint32_t*>(at) + l);
-        const uint32_t pair = ld_l2(reinterpret_cast<const uint32_t*>(at + kK4Codes) + (l >> 2));
-        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+    if (row0 >= a.rows) return;
+    const RowPlaces<R> places(a, row0, kvh, 0x7fffffff);
+    uint32_t word[R], pair[R];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = p.y + p.x * (float)((word >> (4 * j)) & 15u);
+    for (int r = 0; r < R; ++r) {
+        const uint8_t* at = places.place(r);
+        word[r] = pair[r] = 0;
+        if (at) {
+            at += is_v * kK4Half;
+            word[r] = ld_l2(reinterpret_cast<const uint32_t*>(at) + l);
+            pair[r] = ld_l2(reinterpret_cast<const uint32_t*>(at + kK4Codes) + (l >> 2));
+        }
     }
-    float* out = (is_v ? v : k);
-    if (!out) return;
-    out += (size_t)row * a.kv_stride + kvh * 128 + 8 * l;
-    if (VEC) {
-        reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
+    float* to = is_v ? v : k;
+    if (!to) return;
+    to += (size_t)row0 * a.kv_stride + kvh * 128 + 8 * l;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = x[j];
+    for (int r = 0; r < R; ++r) {
+        if (row0 + r >= a.rows) break;
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&pair[r]));
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = p.y + p.x * (float)((word[r] >> (4 * j)) & 15u);
+        float* out = to + (size_t)r * a.kv_stride;
+        if (VEC) {
+            reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) out[j] = x[j];
+        }
     }
 }
 
@@ -179,12 +210,25 @@ __global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenz
         if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&g_kv4_rows_error, kK4ErrIndex);
         return;
     }
-    const int halves = c.n_layers * c.n_kv * 2, units = filled * (kK4Row / 16);          // 16-byte units of a half page
+    const unsigned halves = c.n_layers * c.n_kv * 2, units = filled * (kK4Row / 16), total = halves * units;         // 16-byte units of a half page, and in all
+    const unsigned by_units = 0xffffffffu / units + 1u;  // i / units for i below 2^32 / units
     const uint4* src = reinterpret_cast<const uint4*>(c.pool + (size_t)source * halves * kK4Half);
     uint4* dst = reinterpret_cast<uint4*>(c.pool + (size_t)target * halves * kK4Half);
-    constexpr int kUnits = kK4Half / 16;
-    for (int h = blockIdx.y * (kReorderThreads / 32) + (threadIdx.x >> 5); h < halves; h += kReorderParts * (kReorderThreads / 32))
-        for (int u = lane; u < units; u += 32) dst[(size_t)h * kUnits + u] = ld_l2(src + (size_t)h * kUnits + u);
+    constexpr unsigned kUnits = kK4Half / 16, kStep = kReorderParts * kReorderThreads;
+    constexpr int kBatch = 8;                            // loads in flight
+    for (unsigned i0 = blockIdx.y * kReorderThreads + threadIdx.x; i0 < total; i0 += kBatch * kStep) {
+        uint4 w[kBatch];
+        size_t at[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            const unsigned i = i0 + n * kStep, h = __umulhi(i, by_units);
+            at[n] = (size_t)h * kUnits + (i - h * units);
+            if (i < total) w[n] = ld_l2(src + at[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n)
+            if (i0 + n * kStep < total) dst[at[n]] = w[n];
+    }
 }
 
 static bool aligned16(const void* p) { return !(reinterpret_cast<uintptr_t>(p) & 15); }
@@ -197,6 +241,10 @@ static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, co
     a->layer = layer; a->rows = rows; a->kv_stride = kv_stride; a->pos = pos; a->seq = seq;
     return true;
 }
+
+// Rows a warp takes: four where that still leaves every SM 16 warps (their loads are in flight together), else one.
+static int rows_a_warp(int rows, int n_kv) { return (long long)rows * n_kv >= 4LL * 148 * 16 ? 4 : 1; }
+static dim3 rows_grid(int rows, int n_kv, int r) { return dim3((unsigned)(((long long)rows + r * kRowWarps - 1) / (r * kRowWarps)), (unsigned)n_kv); }
 
 int kv4_rows_take_error() {
     int v = 0, zero = 0;
@@ -216,9 +264,10 @@ extern "C" int tenzo_cuda_kv4_append(const tenzo_kv4_cache* cache, int layer, co
     if ((rope_cos == nullptr) != (rope_sin == nullptr) || (rope_cos && rope_len <= 0)) return -1;
     a.cs = rope_cos; a.sn = rope_sin; a.rope_len = rope_len; a.use_pdl = use_pdl != 0;
     const bool vec = aligned16(k) && aligned16(v) && kv_stride % 4 == 0 && aligned16(rope_cos) && aligned16(rope_sin);
-    auto* kernel = rope_cos ? (vec ? kv4_append_kernel<true, true> : kv4_append_kernel<false, true>)
-                            : (vec ? kv4_append_kernel<true, false> : kv4_append_kernel<false, false>);
-    return kv4_launch(kernel, dim3((unsigned)((rows + kRowWarps - 1) / kRowWarps), (unsigned)cache->n_kv), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl, a, k, v);
+    const int r = rows_a_warp(rows, cache->n_kv);
+    auto* kernel = r == 1 ? (rope_cos ? (vec ? kv4_append_kernel<true, true, 1> : kv4_append_kernel<false, true, 1>) : (vec ? kv4_append_kernel<true, false, 1> : kv4_append_kernel<false, false, 1>))
+                          : (rope_cos ? (vec ? kv4_append_kernel<true, true, 4> : kv4_append_kernel<false, true, 4>) : (vec ? kv4_append_kernel<true, false, 4> : kv4_append_kernel<false, false, 4>));
+    return kv4_launch(kernel, rows_grid(rows, cache->n_kv, r), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl, a, k, v);
 }
 
 extern "C" int tenzo_cuda_kv4_read(const tenzo_kv4_cache* cache, int layer, float* k, float* v, int kv_stride, const int* pos, const int* seq, int rows,
@@ -229,8 +278,9 @@ extern "C" int tenzo_cuda_kv4_read(const tenzo_kv4_cache* cache, int layer, floa
     if (!rows_args(cache, layer, kv_stride, pos, seq, rows, &a) || (!k && !v)) return -1;
     a.use_pdl = use_pdl != 0;
     const bool vec = aligned16(k) && aligned16(v) && kv_stride % 4 == 0;
-    return kv4_launch(vec ? kv4_read_kernel<true> : kv4_read_kernel<false>, dim3((unsigned)((rows + kRowWarps - 1) / kRowWarps), (unsigned)cache->n_kv),
-                      kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl, a, k, v);
+    const int r = rows_a_warp(rows, cache->n_kv);
+    auto* kernel = r == 1 ? (vec ? kv4_read_kernel<true, 1> : kv4_read_kernel<false, 1>) : (vec ? kv4_read_kernel<true, 4> : kv4_read_kernel<false, 4>);
+    return kv4_launch(kernel, rows_grid(rows, cache->n_kv, r), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl, a, k, v);
 }
 
 extern "C" int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_out, const int* parent, const int* length, int groups, int beams, int use_pdl,
