@@ -27,6 +27,7 @@ __device__ __forceinline__ size_t kv4_page(const tenzo_kv4_cache& c, int layer, 
 // hundred launches).
 __device__ __forceinline__ int ld_l2(const int* p) { int v; asm volatile("ld.global.cg.b32 %0, [%1];" : "=r"(v) : "l"(p)); return v; }
 __device__ __forceinline__ uint32_t ld_l2(const uint32_t* p) { uint32_t v; asm volatile("ld.global.cg.b32 %0, [%1];" : "=r"(v) : "l"(p)); return v; }
+__device__ __forceinline__ uint32_t ld_l2(const unsigned short* p) { unsigned short v; asm volatile("ld.global.cg.u16 %0, [%1];" : "=h"(v) : "l"(p)); return v; }
 __device__ __forceinline__ float ld_l2(const float* p) { float v; asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p)); return v; }
 __device__ __forceinline__ double ld_l2(const double* p) { double v; asm volatile("ld.global.cg.f64 %0, [%1];" : "=d"(v) : "l"(p)); return v; }
 __device__ __forceinline__ unsigned long long ld_l2(const unsigned long long* p) { unsigned long long v; asm volatile("ld.global.cg.b64 %0, [%1];" : "=l"(v) : "l"(p)); return v; }

@@ -1,8 +1,8 @@
 // Rows of the 4-bit paged cache (kv4.cuh): appending them, reading them back, and handing the tables of parents on to the beams that
 // continue them.
 //
-// Append: one warp per (row, kv head), lanes 0-15 the key, 16-31 the value, eight dims a lane. The rotation pairs dims i and i + 64, that
-// is lanes 8 apart; a group of 32 dims is four lanes, so its minimum and maximum take two shuffles each. Every step is rounded to
+// A warp takes one kv head of one row (or of four), lanes 0-15 the key, 16-31 the value, dims 4l .. 4l + 3 and 64 more a lane: the pairs that the
+// rotation turns lie in one lane, and every load and store is of whole sectors. Neighbouring warps take neighbouring heads. Every step is rounded to
 // fp32 in the order the header gives (a code next to a border must not depend on who computes it); only the two parameters are
 // rounded further, to fp16: at 32 dims a pair a third format of 32 bits would cost 10 % of the cache's bytes.
 // Bound by memory: 1024 bytes in and 160 out a row and head.
@@ -38,13 +38,13 @@ struct RowsArgs {
 };
 
 template <bool VEC>
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+__device__ __forceinline__ void load4(const float* p, float* x) {
     if (VEC) {
-        const float4 a = ld_l2(reinterpret_cast<const float4*>(p)), b = ld_l2(reinterpret_cast<const float4*>(p) + 1);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        const float4 v = ld_l2(reinterpret_cast<const float4*>(p));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = ld_l2(p + j);
+        for (int j = 0; j < 4; ++j) x[j] = ld_l2(p + j);
     }
 }
 
@@ -64,101 +64,118 @@ struct RowPlaces {
     __device__ __forceinline__ int position(int r) const { return __shfl_sync(0xffffffffu, pos, r); }
 };
 
+// The four codes of x, a nibble each.
+__device__ __forceinline__ uint32_t row_codes(const float* x, float m, float inv) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w |= (uint32_t)__float2int_rn(fminf(fmaxf((x[j] - m) * inv, 0.0f), 15.0f)) << (4 * j);     // nearest, ties to even
+    return w;
+}
+
 template <bool VEC, bool ROPE, int R>
 __global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsArgs a, const float* k, const float* v) {
-    const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * R, kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
+    const int lane = threadIdx.x & 31, unit = blockIdx.x * kRowWarps + (threadIdx.x >> 5), kvh = unit % a.c.n_kv, row0 = unit / a.c.n_kv * R;
+    const int is_v = lane >> 4, l = lane & 15;
     if (a.use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
     if (row0 >= a.rows) return;
-    float x[R][8];
+    float x[R][8];                                       // dims 4l .. 4l + 3, and 64 more
 #pragma unroll
-    for (int r = 0; r < R; ++r)                          // (padding rows are there to be read too)
-        if (row0 + r < a.rows) load8<VEC>((is_v ? v : k) + (size_t)(row0 + r) * a.kv_stride + kvh * 128 + 8 * l, x[r]);
+    for (int r = 0; r < R; ++r) {                        // (padding rows are there to be read too)
+        if (row0 + r < a.rows) {
+            const float* p = (is_v ? v : k) + (size_t)(row0 + r) * a.kv_stride + kvh * 128 + 4 * l;
+            load4<VEC>(p, x[r]);
+            load4<VEC>(p + 64, x[r] + 4);
+        }
+    }
     const RowPlaces<R> places(a, row0, kvh, ROPE ? a.rope_len : 0x7fffffff);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         uint8_t* at = places.place(r);
         if (!at) continue;                               // the whole warp
         if (ROPE) {
-            const size_t of = (size_t)places.position(r) * 64 + ((8 * l) & 63);
-            float c[8], s[8];
-            load8<VEC>(a.cs + of, c);
-            load8<VEC>(a.sn + of, s);
+            const size_t of = (size_t)places.position(r) * 64 + 4 * l;
+            if (!is_v) {
+                float c[4], s[4];
+                load4<VEC>(a.cs + of, c);
+                load4<VEC>(a.sn + of, s);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float o = __shfl_xor_sync(0xffffffffu, x[r][j], 8);
-                const float turned = l < 8 ? __fmaf_rn(x[r][j], c[j], -(o * s[j])) : __fmaf_rn(o, s[j], x[r][j] * c[j]);
-                if (!is_v) x[r][j] = turned;
+                for (int j = 0; j < 4; ++j) {
+                    const float p = x[r][j], q = x[r][4 + j];
+                    x[r][j] = __fmaf_rn(p, c[j], -(q * s[j]));
+                    x[r][4 + j] = __fmaf_rn(p, s[j], q * c[j]);
+                }
             }
         }
-        float lo, hi;
+        // Group l / 8 of the first 64 dims and of the others: lanes with an even l gather the first's minimum and maximum, the others
+        // the second's. (Clamped afterwards: what lies outside gets the first or the last code all the same.)
+        const bool odd = l & 1;
+        const float lo_a = fminf(fminf(x[r][0], x[r][1]), fminf(x[r][2], x[r][3])), hi_a = fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]));
+        const float lo_b = fminf(fminf(x[r][4], x[r][5]), fminf(x[r][6], x[r][7])), hi_b = fmaxf(fmaxf(x[r][4], x[r][5]), fmaxf(x[r][6], x[r][7]));
+        float lo = fminf(odd ? lo_b : lo_a, __shfl_xor_sync(0xffffffffu, odd ? lo_a : lo_b, 1));
+        float hi = fmaxf(odd ? hi_b : hi_a, __shfl_xor_sync(0xffffffffu, odd ? hi_a : hi_b, 1));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[r][j] = fminf(fmaxf(x[r][j], -kFp16Most), kFp16Most);
-            lo = j ? fminf(lo, x[r][j]) : x[r][j];
-            hi = j ? fmaxf(hi, x[r][j]) : x[r][j];
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
+        for (int o = 2; o < 8; o <<= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
+        lo = fminf(fmaxf(lo, -kFp16Most), kFp16Most);
+        hi = fminf(fmaxf(hi, -kFp16Most), kFp16Most);
         const __half low = __float2half_rn(lo), scale = __float2half_rn((hi - __half2float(low)) * (1.0f / 15.0f));
-        const float m = __half2float(low), s = __half2float(scale);
-        uint32_t word = 0;
-        if (s > 0.0f) {
-            const float inv = 1.0f / s;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = __float2int_rn(fminf(fmaxf((x[r][j] - m) * inv, 0.0f), 15.0f));      // nearest, ties to even
-                word |= (uint32_t)c << (4 * j);
-            }
-        }
+        const float m = __half2float(low), s = __half2float(scale), inv = s > 0.0f ? 1.0f / s : 0.0f;
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, 1), inv2 = __shfl_xor_sync(0xffffffffu, inv, 1);     // the other group's
         at += is_v * kK4Half;
-        reinterpret_cast<uint32_t*>(at)[l] = word;
-        if ((l & 3) == 0) reinterpret_cast<__half2*>(at + kK4Codes)[l >> 2] = __halves2half2(scale, low);
+        reinterpret_cast<unsigned short*>(at)[l] = (unsigned short)row_codes(x[r], odd ? m2 : m, odd ? inv2 : inv);
+        reinterpret_cast<unsigned short*>(at + 32)[l] = (unsigned short)row_codes(x[r] + 4, odd ? m : m2, odd ? inv : inv2);
+        if ((l & 6) == 0) reinterpret_cast<__half2*>(at + kK4Codes)[2 * odd + (l >> 3)] = __halves2half2(scale, low);
     }
 }
 
 template <bool VEC, int R>
 __global__ void __launch_bounds__(kRowWarps * 32) kv4_read_kernel(const RowsArgs a, float* k, float* v) {
-    const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * R, kvh = blockIdx.y, is_v = lane >> 4, l = lane & 15;
+    const int lane = threadIdx.x & 31, unit = blockIdx.x * kRowWarps + (threadIdx.x >> 5), kvh = unit % a.c.n_kv, row0 = unit / a.c.n_kv * R;
+    const int is_v = lane >> 4, l = lane & 15;
     if (a.use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
     if (row0 >= a.rows) return;
     const RowPlaces<R> places(a, row0, kvh, 0x7fffffff);
-    uint32_t word[R], pair[R];
+    uint32_t word[R][2], pair[R][2];                     // of dims 4l .. 4l + 3, and 64 more
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const uint8_t* at = places.place(r);
-        word[r] = pair[r] = 0;
+        word[r][0] = word[r][1] = pair[r][0] = pair[r][1] = 0;
         if (at) {
             at += is_v * kK4Half;
-            word[r] = ld_l2(reinterpret_cast<const uint32_t*>(at) + l);
-            pair[r] = ld_l2(reinterpret_cast<const uint32_t*>(at + kK4Codes) + (l >> 2));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                word[r][h] = ld_l2(reinterpret_cast<const unsigned short*>(at + 32 * h) + l);
+                pair[r][h] = ld_l2(reinterpret_cast<const uint32_t*>(at + kK4Codes) + 2 * h + (l >> 3));
+            }
         }
     }
     float* to = is_v ? v : k;
     if (!to) return;
-    to += (size_t)row0 * a.kv_stride + kvh * 128 + 8 * l;
+    to += (size_t)row0 * a.kv_stride + kvh * 128 + 4 * l;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (row0 + r >= a.rows) break;
-        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&pair[r]));
-        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = p.y + p.x * (float)((word[r] >> (4 * j)) & 15u);
-        float* out = to + (size_t)r * a.kv_stride;
-        if (VEC) {
-            reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
-            reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
-        } else {
+        for (int h = 0; h < 2; ++h) {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&pair[r][h]));
+            float x[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = x[j];
+            for (int j = 0; j < 4; ++j) x[j] = p.y + p.x * (float)((word[r][h] >> (4 * j)) & 15u);
+            float* out = to + (size_t)r * a.kv_stride + 64 * h;
+            if (VEC) {
+                *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) out[j] = x[j];
+            }
         }
     }
 }
@@ -234,7 +251,7 @@ __global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenz
 static bool aligned16(const void* p) { return !(reinterpret_cast<uintptr_t>(p) & 15); }
 
 static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, const int* pos, const int* seq, int rows, RowsArgs* a) {
-    if (!cache || !kv4_cache_ok(*cache) || layer < 0 || layer >= cache->n_layers || !pos || rows < 1 || cache->n_kv > 65535) return false;
+    if (!cache || !kv4_cache_ok(*cache) || layer < 0 || layer >= cache->n_layers || !pos || rows < 1 || (long long)rows * cache->n_kv > 0x7fffffffLL) return false;
     if (kv_stride < cache->n_kv * 128) return false;
     if (!seq && rows > cache->table_rows) return false;
     a->c = *cache;
@@ -244,7 +261,7 @@ static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, co
 
 // Rows a warp takes: four where that still leaves every SM 16 warps (their loads are in flight together), else one.
 static int rows_a_warp(int rows, int n_kv) { return (long long)rows * n_kv >= 4LL * 148 * 16 ? 4 : 1; }
-static dim3 rows_grid(int rows, int n_kv, int r) { return dim3((unsigned)(((long long)rows + r * kRowWarps - 1) / (r * kRowWarps)), (unsigned)n_kv); }
+static dim3 rows_grid(int rows, int n_kv, int r) { return dim3((unsigned)((((long long)rows + r - 1) / r * n_kv + kRowWarps - 1) / kRowWarps)); }
 
 int kv4_rows_take_error() {
     int v = 0, zero = 0;
