@@ -1,7 +1,7 @@
 // Rows of the 4-bit paged cache (kv4.cuh): appending them, reading them back, and handing the tables of parents on to the beams that
 // continue them.
 //
-// A warp takes one kv head of one row (or of four), lanes 0-15 the key, 16-31 the value, dims 4l .. 4l + 3 and 64 more a lane: the pairs that the
+// A warp takes one kv head of one row (or of two), lanes 0-15 the key, 16-31 the value, dims 4l .. 4l + 3 and 64 more a lane: the pairs that the
 // rotation turns lie in one lane, and every load and store is of whole sectors. Neighbouring warps take neighbouring heads. Every step is rounded to
 // fp32 in the order the header gives (a code next to a border must not depend on who computes it); only the two parameters are
 // rounded further, to fp16: at 32 dims a pair a third format of 32 bits would cost 10 % of the cache's bytes.
@@ -16,19 +16,6 @@ constexpr int kRowWarps = 4;                             // warps a CTA; a warp 
 constexpr float kFp16Most = 65504.0f;
 
 __device__ int g_kv4_rows_error = 0;
-
-// The page and slot of a row's token; null for padding (a negative position), and for an index outside its range (which is flagged).
-__device__ __forceinline__ uint8_t* row_place(const tenzo_kv4_cache& c, int layer, int kvh, int pos, int seq, int rope_len) {
-    if (pos < 0) return nullptr;
-    const int col = pos / kK4Slots;
-    int block = -1;
-    if (seq >= 0 && seq < c.table_rows && col < c.table_stride && pos < rope_len) block = ld_l2(c.block_table + (size_t)seq * c.table_stride + col);
-    if (block < 0 || block >= c.n_blocks) {
-        atomicOr(&g_kv4_rows_error, kK4ErrIndex);
-        return nullptr;
-    }
-    return c.pool + kv4_page(c, layer, kvh, block) + (size_t)(pos % kK4Slots) * kK4Row;
-}
 
 struct RowsArgs {
     tenzo_kv4_cache c;
@@ -48,20 +35,33 @@ __device__ __forceinline__ void load4(const float* p, float* x) {
     }
 }
 
-// Lane r < R looks up the warp's r-th row; its position (-1: leave it alone) and place go to all by shuffles.
+// Lane r < R looks up the warp's r-th row: the position (-1: padding) and the table's entry are asked for at once, the place comes from them. Null for padding
+// and for an index outside its range, which is flagged.
 template <int R>
 struct RowPlaces {
-    int pos;
-    uint8_t* at;
-    __device__ __forceinline__ RowPlaces(const RowsArgs& a, int row0, int kvh, int rope_len) : pos(-1), at(nullptr) {
+    const RowsArgs& a;
+    int kvh, pos, block;
+    __device__ __forceinline__ RowPlaces(const RowsArgs& args, int row0, int head, int rope_len) : a(args), kvh(head), pos(-1), block(-1) {
         const int lane = threadIdx.x & 31, row = row0 + lane;
         if (lane < R && row < a.rows) {
             pos = ld_l2(a.pos + row);
-            at = row_place(a.c, a.layer, kvh, pos, a.seq ? ld_l2(a.seq + row) : row, rope_len);
+            const int seq = a.seq ? ld_l2(a.seq + row) : row;
+            if (pos >= 0) {
+                const bool there = seq >= 0 && seq < a.c.table_rows && pos / kK4Slots < a.c.table_stride && pos < rope_len;
+                if (there) block = ld_l2(a.c.block_table + (size_t)seq * a.c.table_stride + pos / kK4Slots);
+            }
         }
     }
-    __device__ __forceinline__ uint8_t* place(int r) const { return reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), r)); }
     __device__ __forceinline__ int position(int r) const { return __shfl_sync(0xffffffffu, pos, r); }
+    __device__ __forceinline__ uint8_t* finish(int r) const {
+        const int p = __shfl_sync(0xffffffffu, pos, r), b = __shfl_sync(0xffffffffu, block, r);
+        if (p < 0) return nullptr;
+        if (b < 0 || b >= a.c.n_blocks) {
+            if ((threadIdx.x & 31) == 0) atomicOr(&g_kv4_rows_error, kK4ErrIndex);
+            return nullptr;
+        }
+        return a.c.pool + kv4_page(a.c, a.layer, kvh, b) + (size_t)(p % kK4Slots) * kK4Row;
+    }
 };
 
 // The four codes of x, a nibble each.
@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsAr
         pdl_wait();
     }
     if (row0 >= a.rows) return;
-    float x[R][8];                                       // dims 4l .. 4l + 3, and 64 more
+    const RowPlaces<R> places(a, row0, kvh, ROPE ? a.rope_len : 0x7fffffff);
+    float x[R][8], c[R][4], s[R][4];                     // dims 4l .. 4l + 3, and 64 more
 #pragma unroll
     for (int r = 0; r < R; ++r) {                        // (padding rows are there to be read too)
         if (row0 + r < a.rows) {
@@ -90,23 +91,26 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsAr
             load4<VEC>(p + 64, x[r] + 4);
         }
     }
-    const RowPlaces<R> places(a, row0, kvh, ROPE ? a.rope_len : 0x7fffffff);
+    if (ROPE) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int pos = places.position(r);
+            if (!is_v && pos >= 0 && pos < a.rope_len) {
+                load4<VEC>(a.cs + (size_t)pos * 64 + 4 * l, c[r]);
+                load4<VEC>(a.sn + (size_t)pos * 64 + 4 * l, s[r]);
+            }
+        }
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        uint8_t* at = places.place(r);
+        uint8_t* at = places.finish(r);
         if (!at) continue;                               // the whole warp
-        if (ROPE) {
-            const size_t of = (size_t)places.position(r) * 64 + 4 * l;
-            if (!is_v) {
-                float c[4], s[4];
-                load4<VEC>(a.cs + of, c);
-                load4<VEC>(a.sn + of, s);
+        if (ROPE && !is_v) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float p = x[r][j], q = x[r][4 + j];
-                    x[r][j] = __fmaf_rn(p, c[j], -(q * s[j]));
-                    x[r][4 + j] = __fmaf_rn(p, s[j], q * c[j]);
-                }
+            for (int j = 0; j < 4; ++j) {
+                const float p = x[r][j], q = x[r][4 + j];
+                x[r][j] = __fmaf_rn(p, c[r][j], -(q * s[r][j]));
+                x[r][4 + j] = __fmaf_rn(p, s[r][j], q * c[r][j]);
             }
         }
         // Group l / 8 of the first 64 dims and of the others: lanes with an even l gather the first's minimum and maximum, the others
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_append_kernel(const RowsAr
         lo = fminf(fmaxf(lo, -kFp16Most), kFp16Most);
         hi = fminf(fmaxf(hi, -kFp16Most), kFp16Most);
         const __half low = __float2half_rn(lo), scale = __float2half_rn((hi - __half2float(low)) * (1.0f / 15.0f));
-        const float m = __half2float(low), s = __half2float(scale), inv = s > 0.0f ? 1.0f / s : 0.0f;
+        const float m = __half2float(low), step = __half2float(scale), inv = step > 0.0f ? 1.0f / step : 0.0f;
         const float m2 = __shfl_xor_sync(0xffffffffu, m, 1), inv2 = __shfl_xor_sync(0xffffffffu, inv, 1);     // the other group's
         at += is_v * kK4Half;
         reinterpret_cast<unsigned short*>(at)[l] = (unsigned short)row_codes(x[r], odd ? m2 : m, odd ? inv2 : inv);
@@ -146,7 +150,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_read_kernel(const RowsArgs
     uint32_t word[R][2], pair[R][2];                     // of dims 4l .. 4l + 3, and 64 more
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const uint8_t* at = places.place(r);
+        const uint8_t* at = places.finish(r);
         word[r][0] = word[r][1] = pair[r][0] = pair[r][1] = 0;
         if (at) {
             at += is_v * kK4Half;
@@ -259,8 +263,8 @@ static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, co
     return true;
 }
 
-// Rows a warp takes: four where that still leaves every SM 16 warps (their loads are in flight together), else one.
-static int rows_a_warp(int rows, int n_kv) { return (long long)rows * n_kv >= 4LL * 148 * 16 ? 4 : 1; }
+// Rows a warp takes: two where that still leaves every SM 16 warps (their loads are in flight together), else one.
+static int rows_a_warp(int rows, int n_kv) { return (long long)rows * n_kv >= 4LL * 148 * 16 ? 2 : 1; }
 static dim3 rows_grid(int rows, int n_kv, int r) { return dim3((unsigned)((((long long)rows + r - 1) / r * n_kv + kRowWarps - 1) / kRowWarps)); }
 
 int kv4_rows_take_error() {
@@ -283,7 +287,7 @@ extern "C" int tenzo_cuda_kv4_append(const tenzo_kv4_cache* cache, int layer, co
     const bool vec = aligned16(k) && aligned16(v) && kv_stride % 4 == 0 && aligned16(rope_cos) && aligned16(rope_sin);
     const int r = rows_a_warp(rows, cache->n_kv);
     auto* kernel = r == 1 ? (rope_cos ? (vec ? kv4_append_kernel<true, true, 1> : kv4_append_kernel<false, true, 1>) : (vec ? kv4_append_kernel<true, false, 1> : kv4_append_kernel<false, false, 1>))
-                          : (rope_cos ? (vec ? kv4_append_kernel<true, true, 4> : kv4_append_kernel<false, true, 4>) : (vec ? kv4_append_kernel<true, false, 4> : kv4_append_kernel<false, false, 4>));
+                          : (rope_cos ? (vec ? kv4_append_kernel<true, true, 2> : kv4_append_kernel<false, true, 2>) : (vec ? kv4_append_kernel<true, false, 2> : kv4_append_kernel<false, false, 2>));
     return kv4_launch(kernel, rows_grid(rows, cache->n_kv, r), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl, a, k, v);
 }
 
@@ -296,7 +300,7 @@ extern "C" int tenzo_cuda_kv4_read(const tenzo_kv4_cache* cache, int layer, floa
     a.use_pdl = use_pdl != 0;
     const bool vec = aligned16(k) && aligned16(v) && kv_stride % 4 == 0;
     const int r = rows_a_warp(rows, cache->n_kv);
-    auto* kernel = r == 1 ? (vec ? kv4_read_kernel<true, 1> : kv4_read_kernel<false, 1>) : (vec ? kv4_read_kernel<true, 4> : kv4_read_kernel<false, 4>);
+    auto* kernel = r == 1 ? (vec ? kv4_read_kernel<true, 1> : kv4_read_kernel<false, 1>) : (vec ? kv4_read_kernel<true, 2> : kv4_read_kernel<false, 2>);
     return kv4_launch(kernel, rows_grid(rows, cache->n_kv, r), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl, a, k, v);
 }
 
