@@ -86,6 +86,17 @@ __device__ __forceinline__ uint32_t a4_odd(uint32_t w) { return a4_fma(w & 0x00f
 // Rows that are left alone (a position or a sequence out of range); the same rule in both kernels.
 __device__ __forceinline__ bool a4_refused(const tenzo_attention_kv4_args& a, int pos, int seq) { return pos >= a.max_len || seq < 0 || seq >= a.cache.table_rows; }
 
+// D = A B + c in every place.
+__device__ __forceinline__ void a4_imma_from(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, int c) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c));
+}
+// The upper nibbles of a word's bytes as signed numbers 16 (code - 8).
+__device__ __forceinline__ uint32_t a4_signed(uint32_t w) { return (w & 0xf0f0f0f0u) ^ 0x80808080u; }
+__device__ __forceinline__ f32x2 a4_pair(int lo, int hi) { return pack2(__int_as_float(lo), __int_as_float(hi)); }
+
+constexpr int kA4FromFloat = 0x4B400000;                  // 1.5 * 2^23 as a float
+
 template <int HB>
 __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(const A4Launch L) {
     static_assert(HB == 4 || HB == 8, "heads a CTA takes");
@@ -95,12 +106,12 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     __shared__ uint64_t s_bar[kA4Warps][kA4Stages];
     __shared__ __align__(16) float s_scale[kA4Warps][2][kA4Step / 2][4][2];      // a step's scales, keys and values: [pair of keys][group][key]
     __shared__ __align__(16) uint4 s_centre[kA4Warps][kA4Step];                  // minimum + 8 scale of the values: four first parts, four second ones
-    __shared__ __align__(16) uint4 s_qa[8][32];          // the queries' A fragments, the same in every warp
+    __shared__ __align__(16) uint4 s_qa[4][HB == 8 ? 2 : 1][32];      // the queries' A fragments, the same in every warp
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int row = blockIdx.x / L.n_splits, split = blockIdx.x % L.n_splits;
     const int kvh = blockIdx.y / L.head_blocks, head0 = blockIdx.y % L.head_blocks * HB, heads = min(HB, L.group - head0);
     if (lane == 0)
-        for (int s = 0; s < kA4Stages; ++s) mbar_init(&s_bar[warp][s], 1);
+        for (int s = 0; s < kA4Stages; ++s) mbar_init(&s_bar[warp][s], 2);
     mbar_init_fence();
     if (a.use_pdl || L.n_splits > 1) pdl_launch_dependents();       // the second kernel waits for this one whatever its neighbours do
     if (a.use_pdl) pdl_wait();
@@ -120,44 +131,43 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     const int my_steps = warp < steps ? (steps - warp + kA4Warps - 1) / kA4Warps : 0;
     const int* table = a.cache.block_table + (size_t)seq * a.cache.table_stride + c_begin / kK4Slots;
     const int pages = (c_end - c_begin + kK4Slots - 1) / kK4Slots;
-    const uint8_t* pool = a.cache.pool + kv4_page(a.cache, a.layer, kvh, 0);
-    const size_t block_bytes = (size_t)a.cache.n_layers * a.cache.n_kv * kK4Page;
     unsigned char* ring = a4_smem + (size_t)warp * kA4Stages * kA4StepBytes;
     uint64_t* bar = s_bar[warp];
 
-    // Table entries of sixteen of the warp's steps, one a lane (-1: no such page, or an entry out of range), and of the next sixteen.
-    auto entries = [&](int k0) {
+    // A lane has the address of one page of sixteen of the warp's steps (null: no such page, or a table entry out of range) and copies it when its step's turn comes.
+    auto page_at = [&](int k0) -> const uint8_t* {
         const int page = 2 * (warp + (k0 + (lane >> 1)) * kA4Warps) + (lane & 1);
-        int id = -1;
-        if (page < pages) {
-            id = ld_l2(table + page);
-            if (id < 0 || id >= a.cache.n_blocks) {
-                atomicOr(&g_kv4_attention_error, kK4ErrIndex);
-                id = -1;
-            }
+        if (page >= pages) return nullptr;
+        const int id = ld_l2(table + page);
+        if (id < 0 || id >= a.cache.n_blocks) {
+            atomicOr(&g_kv4_attention_error, kK4ErrIndex);
+            return nullptr;
         }
-        return id;
+        return a.cache.pool + kv4_page(a.cache, a.layer, kvh, id);
     };
-    int ids = entries(0), ids_next = entries(16);
-    unsigned there = 0;                                  // two bits a stage: which of its pages were copied
+    __syncwarp();                                        // (the barriers)
+    const uint8_t *from = page_at(0), *from_next = my_steps > 16 ? page_at(16) : nullptr;
+    unsigned there = __ballot_sync(0xffffffffu, from != nullptr), there_before = 0;       // of the pages: of these sixteen steps, of those before
     auto issue = [&](int k) {                            // the warp's k-th step into stage k % kA4Stages
         const int st = k % kA4Stages;
-        const int id0 = __shfl_sync(0xffffffffu, ids, 2 * (k & 15)), id1 = __shfl_sync(0xffffffffu, ids, 2 * (k & 15) + 1);
-        there = (there & ~(3u << (2 * st))) | ((id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u)) << (2 * st);
-        if (lane == 0) {
-            unsigned char* to = ring + (size_t)st * kA4StepBytes;
-            mbar_expect_tx(&bar[st], ((id0 >= 0) + (id1 >= 0)) * (unsigned)kK4Page);
-            if (id0 >= 0) bulk_g2s(to, pool + (size_t)id0 * block_bytes, kK4Page, &bar[st]);
-            if (id1 >= 0) bulk_g2s(to + kK4Page, pool + (size_t)id1 * block_bytes, kK4Page, &bar[st]);
+        if ((lane >> 1) == (k & 15)) {
+            if (from) {
+                mbar_expect_tx(&bar[st], (unsigned)kK4Page);
+                bulk_g2s(ring + (size_t)st * kA4StepBytes + (lane & 1) * kK4Page, from, kK4Page, &bar[st]);
+            } else {
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&bar[st])) : "memory");
+            }
         }
         if ((k & 15) == 15) {
-            ids = ids_next;
-            ids_next = entries(k + 17);
+            from = from_next;
+            there_before = there;
+            there = __ballot_sync(0xffffffffu, from != nullptr);
+            from_next = page_at(k + 17);
         }
     };
     for (int k = 0; k < kA4Stages && k < my_steps; ++k) issue(k);
 
-    // ---- the heads' queries: rotated, scaled by a power of two to a maximum in [2^7, 2^8), and their sums over each group of dims --------
+    // ---- the heads' queries: rotated, scaled by a power of two to a maximum in [2^21, 2^22) and rounded, and their sums over each group of dims ----
     const float* q = a.q + (size_t)row * a.q_stride + ((size_t)kvh * L.group + head0) * kA4Hd;
     for (int i = tid; i < HB * 64; i += kA4Threads) {
         const int h = i >> 6, d = i & 63;
@@ -179,48 +189,59 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     for (int h = warp; h < HB; h += kA4Warps) {
         float4 v = *reinterpret_cast<const float4*>(&s_q[h][4 * lane]);
         const float m = warp_max(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        const int e = max(15, (int)(__float_as_uint(m) >> 23));
-        const float up = __uint_as_float((uint32_t)(127 + 7 - (e - 127)) << 23), down = __uint_as_float((uint32_t)(127 - 7 + (e - 127)) << 23);
-        v.x *= up; v.y *= up; v.z *= up; v.w *= up;
+        const int e = max(22, (int)(__float_as_uint(m) >> 23));
+        const float up = __uint_as_float((uint32_t)(127 + 21 - (e - 127)) << 23), down = __uint_as_float((uint32_t)(127 - 21 + (e - 127)) << 23);
+        v.x = rintf(v.x * up); v.y = rintf(v.y * up); v.z = rintf(v.z * up); v.w = rintf(v.w * up);
         *reinterpret_cast<float4*>(&s_q[h][4 * lane]) = v;
         float sum = (v.x + v.y) + (v.z + v.w);
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if ((lane & 7) == 0) s_qsum[h][lane >> 3] = sum;
-        if (lane == 0) s_f[h] = down * (512.0f * 0.08838834764831845f * 1.4426950408889634f);  // the unit of the products, 1/sqrt(128) and log2(e)
+        if (lane == 0) s_f[h] = down * (4096.0f * 0.08838834764831845f * 1.4426950408889634f); // the unit of the first bytes' sums, 1/sqrt(128) and log2(e)
     }
     __syncthreads();
-    const int mine = g & (HB - 1);                       // the head of rows g and g + 8
-    for (int i = warp; i < 8; i += kA4Warps) {           // group i / 2, nibbles 2 (i % 2) and + 1 of the lane's word
-        const float* p = &s_q[mine][32 * (i >> 1) + 8 * t + 2 * (i & 1)];
-        const float x[4] = {p[0], p[4], p[1], p[5]};
-        const uint32_t a0 = a4_pack(x[0], x[1]), a2 = a4_pack(x[2], x[3]);
-        s_qa[i][lane] = make_uint4(a0, a4_pack(x[0] - a4_low(a0), x[1] - a4_high(a0)), a2, a4_pack(x[2] - a4_low(a2), x[3] - a4_high(a2)));
+    const int mine = g & (HB - 1);                       // the head of a lane's scores
+    {                                                    // group `warp`: byte i of a word is dim 8t + 2i, of the other word 8t + 2i + 1
+        uint32_t w[4] = {0, 0, 0, 0}, w2[2] = {0, 0};    // rows g, rows g + 8 (see above)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int x = (int)s_q[mine][32 * warp + 8 * t + i];
+            const int d3 = ((x + 128) & 255) - 128, r = (x - d3) >> 8, d2 = ((r + 128) & 255) - 128, d1 = (r - d2) >> 8;
+            const int up = HB == 8 || g < 4 ? d1 : d2, down = HB == 8 || g < 4 ? d3 : 0, at = 2 * (i & 1), by = 8 * (i >> 1);
+            w[at] |= (uint32_t)(up & 255) << by;
+            w[at + 1] |= (uint32_t)(down & 255) << by;
+            w2[i & 1] |= (uint32_t)(d2 & 255) << by;
+        }
+        s_qa[warp][0][lane] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (HB == 8) s_qa[warp][HB == 8 ? 1 : 0][lane] = make_uint4(w2[0], 0, w2[1], 0);
     }
-    uint32_t qm[2];
-    {                                                    // beside the scale (8-fold), beside the minimum; in units of 2^9, as the codes
-        const float sum = s_qsum[mine][t] * 0.001953125f, first = __half2float(__float2half_rn(sum));
+    uint32_t qm[2] = {0, 0};                             // beside the scale (8-fold), beside the minimum; 2^-6 of the others' unit
+    if (HB == 8 || g < 4) {
+        const float sum = s_qsum[mine][t] * 3.814697265625e-6f, first = __half2float(__float2half_rn(sum));    // 2^-18
         qm[0] = a4_pack(8.0f * first, first);
         qm[1] = a4_pack(8.0f * (sum - first), sum - first);
     }
     const float f = s_f[mine];
     __syncthreads();
 
-    float m_run = -INFINITY, top = 0.0f, l_run = 0.0f;   // head `mine`: largest product so far, its score (log2) less 14, this lane's share of the sum
+    float m_run = -INFINITY, top = 0.0f;                 // head `mine`: largest product so far, its score (log2) less 14
+    f32x2 l_pair = 0;                                    // this lane's share of the sum
     float vs = 1.0f;                                     // values' scales are multiplied by this power of two, to at most 1
     uint32_t v_most = 0;                                 // the largest exponent of a scale so far, as fp16 bits
     f32x2 acc[8][2], accm = 0;                           // group i / 2: dims 4g + 2 (i % 2), and + 1; heads 2t, 2t + 1
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = 0;
     const uint32_t cut = HB == 8 || g >= 4 ? 0xffffe000u : 0u;                                  // columns 4-7: what the first eleven bits leave
-    const f32x2 minus = pack2(-1.0f, -1.0f), f2 = pack2(f, f);
+    const f32x2 minus = pack2(-1.0f, -1.0f), f2 = pack2(f, f), from_float = pack2(-12582912.0f, -12582912.0f), third = pack2(1.52587890625e-5f, 1.52587890625e-5f);
+    const f32x2 second = pack2(0.00390625f, 0.00390625f), part = HB == 8 || g < 4 ? pack2(1.0f, 1.0f) : second, sixty_four = pack2(64.0f, 64.0f);
     bool gave_up = false;
 
     for (int k = 0; k < my_steps; ++k) {
         const int st = k % kA4Stages, t0 = c_begin + (warp + k * kA4Warps) * kA4Step;
         unsigned char* step = ring + (size_t)st * kA4StepBytes;
         if (!mbar_wait_bounded(&bar[st], (unsigned)(k / kA4Stages) & 1u)) gave_up = true;
-        const unsigned copied = (there >> (2 * st)) & 3u;
+        // (copies run ahead of the products, so `there` may be of the next sixteen steps already)
+        const unsigned copied = ((min(k + kA4Stages, my_steps) >> 4) == (k >> 4) ? there : there_before) >> (2 * (k & 15)) & 3u;
         const bool ragged = t0 + kA4Step > c_end || copied != 3u;
         unsigned char* own = step + (lane >> 4) * kK4Page + (lane & 15) * kK4Row + kK4Codes;    // the parameters of key t0 + lane
         if (ragged) {                                    // keys that do not count: parameters of zero, whatever lies there
@@ -236,11 +257,11 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         float ratio = 1.0f;
         {
             const uint4 pk = *reinterpret_cast<const uint4*>(own), pv = *reinterpret_cast<const uint4*>(own + kK4Half);
-            const uint32_t v_max = __reduce_max_sync(0xffffffffu, max(max(pv.x & 0x7c00u, pv.y & 0x7c00u), max(pv.z & 0x7c00u, pv.w & 0x7c00u)));
-            v_grown = v_max > v_most || k == 0;
+            const uint32_t v_max = max(max(pv.x & 0x7c00u, pv.y & 0x7c00u), max(pv.z & 0x7c00u, pv.w & 0x7c00u));
+            v_grown = __any_sync(0xffffffffu, v_max > v_most) || k == 0;
             if (v_grown) {                               // a scale below 2^(e - 14) times 2^(14 - e) is below 1
-                v_most = v_max;
-                const float now = __uint_as_float((127u + 14u - max(v_max >> 10, 1u)) << 23);
+                v_most = __reduce_max_sync(0xffffffffu, v_max);
+                const float now = __uint_as_float((127u + 14u - max(v_most >> 10, 1u)) << 23);
                 ratio = k == 0 ? 1.0f : now / vs;
                 vs = now;
             }
@@ -256,28 +277,31 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
             __syncwarp();
         }
         // ---- products with the keys: columns are eight keys a tile ----------------------------------------------------------
-        f32x2 x[4];
+        f32x2 x[4] = {0, 0, 0, 0};
         const unsigned char* kr = step + g * kK4Row + 4 * t;
         auto tile = [](int nt) { return (nt >> 1) * kK4Page + (nt & 1) * 8 * kK4Row; };
+#pragma unroll
+        for (int gr = 0; gr < 4; ++gr) {
+            const uint4 qa = s_qa[gr][0][lane], qb = s_qa[gr][HB == 8 ? 1 : 0][lane];
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(kr + tile(nt) + 16 * gr), even = a4_signed(w << 4), odd = a4_signed(w);
+                int c[4];
+                a4_imma_from(c, qa, even, odd, kA4FromFloat);
+                f32x2 sum = a4_fma2(add2(a4_pair(c[2], c[3]), from_float), third, add2(a4_pair(c[0], c[1]), from_float));
+                if (HB == 8) {
+                    a4_imma_from(c, qb, even, odd, kA4FromFloat);
+                    sum = a4_fma2(add2(a4_pair(c[0], c[1]), from_float), second, sum);
+                }
+                x[nt] = a4_fma2(*reinterpret_cast<const f32x2*>(&s_scale[warp][0][4 * nt + t][gr][0]), sum, x[nt]);
+            }
+        }
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
             float c[4];
             a4_mma8_new(c, qm[0], qm[1], *reinterpret_cast<const uint32_t*>(kr + tile(nt) + kK4Codes));
-            x[nt] = add2(pack2(c[0], c[1]), pack2(c[2], c[3]));
-        }
-#pragma unroll
-        for (int gr = 0; gr < 4; ++gr) {
-            const uint4 qa = s_qa[2 * gr][lane], qb = s_qa[2 * gr + 1][lane];
-            const uint32_t a0[4] = {qa.x, qa.y, qa.z, qa.w}, a1[4] = {qb.x, qb.y, qb.z, qb.w};
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                uint32_t w = *reinterpret_cast<const uint32_t*>(kr + tile(nt) + 16 * gr);
-                float c[4];
-                a4_mma16_new(c, a0, a4_even(w), a4_odd(w));
-                w >>= 8;
-                a4_mma16(c, a1, a4_even(w), a4_odd(w));
-                x[nt] = a4_fma2(*reinterpret_cast<const f32x2*>(&s_scale[warp][0][4 * nt + t][gr][0]), add2(pack2(c[0], c[1]), pack2(c[2], c[3])), x[nt]);
-            }
+            x[nt] = a4_fma2(add2(pack2(c[0], c[1]), pack2(c[2], c[3])), sixty_four, HB == 8 ? x[nt] : a4_mul2(x[nt], part));
+            if (HB == 4) x[nt] = add2(x[nt], __shfl_xor_sync(0xffffffffu, x[nt], 16));
         }
         float s[4][2];
 #pragma unroll
@@ -305,7 +329,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
                 m_run = mx;
                 top = now;
             }
-            l_run *= alpha;
+            l_pair = a4_mul2(l_pair, pack2(alpha, alpha));
             const f32x2 a01 = pack2(__shfl_sync(0xffffffffu, alpha, 8 * t), __shfl_sync(0xffffffffu, alpha, 8 * t + 4));
             accm = a4_mul2(accm, a01);
             const f32x2 scaled = a4_mul2(a01, pack2(ratio, ratio));
@@ -322,10 +346,8 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         for (int nt = 0; nt < 4; ++nt) {
             float e0, e1;
             unpack2(a4_fma2(x[nt], f2, down), e0, e1);
-            e0 = a4_ex2(e0);
-            e1 = a4_ex2(e1);
-            l_run += e0 + e1;
-            e[nt] = pack2(e0, e1);
+            e[nt] = pack2(a4_ex2(e0), a4_ex2(e1));
+            l_pair = add2(l_pair, e[nt]);
         }
         // The two fp16 parts of a pair of weights: the first eleven bits, and what they leave (cut off in turn: 2^-22 less on average,
         // in all products alike).
@@ -383,6 +405,9 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         if (k + kA4Stages < my_steps) issue(k + kA4Stages);
     }
     if (gave_up && lane == 0) atomicOr(&g_kv4_attention_error, kK4ErrWait);
+    float l_run, l_other;
+    unpack2(l_pair, l_run, l_other);
+    l_run += l_other;
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
 
@@ -443,6 +468,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     }
 }
 
+
 // The splits of a (row, head): one warp each, four dims a lane.
 __global__ void __launch_bounds__(kA4Threads) attention_kv4_merge_kernel(const A4Launch L) {
     const tenzo_attention_kv4_args& a = L.a;
@@ -489,8 +515,8 @@ static size_t a4_part_bytes(int rows, int n_q) { return (size_t)rows * n_q * (kA
 
 // Keys a CTA takes: the number of splits whose rounds of CTAs take least at the longest length, a CTA's own cost counted as some
 // hundred keys and a split's as some in the second kernel. `most`: as many splits as there is room for partial results.
-static void a4_pick_split(long long items, int max_len, int most, int* n_splits, int* split_keys) {
-    const long long places = 148 * kA4Resident;
+static void a4_pick_split(long long items, int resident, int max_len, int most, int* n_splits, int* split_keys) {
+    const long long places = 148 * resident;
     double best = 0.0;
     for (int want = 1; want <= 64 && (want == 1 || (max_len + want - 1) / want > 128); ++want) {
         const int keys = ((max_len + want - 1) / want + 127) / 128 * 128, splits = (max_len + keys - 1) / keys;
@@ -556,7 +582,7 @@ extern "C" int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, vo
         L.n_splits = (a.max_len + L.split_keys - 1) / L.split_keys;
         if (L.n_splits > 1 && room < (size_t)L.n_splits) return -1;
     } else {
-        a4_pick_split(items, a.max_len, room > 1 ? (int)(room < 64 ? room : 64) : 1, &L.n_splits, &L.split_keys);
+        a4_pick_split(items, kA4Resident, a.max_len, room > 1 ? (int)(room < 64 ? room : 64) : 1, &L.n_splits, &L.split_keys);
     }
     if ((long long)a.rows * L.n_splits > 0x7fffffffLL) return -1;
     L.part_o = static_cast<float*>(a.workspace);
