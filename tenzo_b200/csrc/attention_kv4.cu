@@ -28,12 +28,14 @@ constexpr int kA4Hd = 128, kA4Warps = 4, kA4Threads = kA4Warps * 32;
 constexpr int kA4Step = 32;                              // keys a warp takes at a time
 constexpr int kA4Stages = 2, kA4StepBytes = 2 * kK4Page;
 constexpr int kA4Resident = 4;                           // CTAs an SM
+constexpr int kA4Cluster = 8;                            // splits that a cluster may take
 
 __device__ int g_kv4_attention_error = 0;
 
 struct A4Launch {
     tenzo_attention_kv4_args a;
     int n_splits, split_keys, group, head_blocks;        // query heads a kv head, and blocks of them that a CTA takes
+    int cluster;                                         // the splits of an item are a thread-block cluster, which joins them itself
     float* part_o;                                       // [row][head][split][128]
     float2* part_ml;                                     // [row][head][split]: maximum (log2), sum
 };
@@ -86,16 +88,11 @@ __device__ __forceinline__ uint32_t a4_odd(uint32_t w) { return a4_fma(w & 0x00f
 // Rows that are left alone (a position or a sequence out of range); the same rule in both kernels.
 __device__ __forceinline__ bool a4_refused(const tenzo_attention_kv4_args& a, int pos, int seq) { return pos >= a.max_len || seq < 0 || seq >= a.cache.table_rows; }
 
-// D = A B + c in every place.
-__device__ __forceinline__ void a4_imma_from(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, int c) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c));
+// D = A B, signed bytes times codes.
+__device__ __forceinline__ void a4_imma(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(0));
 }
-// The upper nibbles of a word's bytes as signed numbers 16 (code - 8).
-__device__ __forceinline__ uint32_t a4_signed(uint32_t w) { return (w & 0xf0f0f0f0u) ^ 0x80808080u; }
-__device__ __forceinline__ f32x2 a4_pair(int lo, int hi) { return pack2(__int_as_float(lo), __int_as_float(hi)); }
-
-constexpr int kA4FromFloat = 0x4B400000;                  // 1.5 * 2^23 as a float
 
 template <int HB>
 __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(const A4Launch L) {
@@ -113,7 +110,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     if (lane == 0)
         for (int s = 0; s < kA4Stages; ++s) mbar_init(&s_bar[warp][s], 2);
     mbar_init_fence();
-    if (a.use_pdl || L.n_splits > 1) pdl_launch_dependents();       // the second kernel waits for this one whatever its neighbours do
+    if (a.use_pdl || (L.n_splits > 1 && !L.cluster)) pdl_launch_dependents();       // the second kernel waits for this one whatever its neighbours do
     if (a.use_pdl) pdl_wait();
     const int pos = ld_l2(a.pos + row), seq = a.seq ? ld_l2(a.seq + row) : row;
     if (a4_refused(a, pos, seq)) {
@@ -122,15 +119,16 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     }
     const int c_begin = split * L.split_keys, c_end = min(pos + 1, c_begin + L.split_keys);
     float* out = a.out + ((size_t)row * a.n_q + (size_t)kvh * L.group + head0) * kA4Hd;
-    if (c_begin >= c_end) {                              // the second kernel knows which splits there are
-        if (L.n_splits == 1)
+    if (c_begin >= c_end && (!L.cluster || pos < 0)) {   // the second kernel knows which splits there are
+        if (L.n_splits == 1 || (L.cluster && split == 0))
             for (int i = tid; i < heads * kA4Hd; i += kA4Threads) out[i] = 0.0f;
         return;
     }
-    const int steps = (c_end - c_begin + kA4Step - 1) / kA4Step;
+    // (a cluster's CTAs without keys go the same way, with no step: 0 outputs, a maximum of -infinity)
+    const int steps = max(0, c_end - c_begin + kA4Step - 1) / kA4Step;
     const int my_steps = warp < steps ? (steps - warp + kA4Warps - 1) / kA4Warps : 0;
     const int* table = a.cache.block_table + (size_t)seq * a.cache.table_stride + c_begin / kK4Slots;
-    const int pages = (c_end - c_begin + kK4Slots - 1) / kK4Slots;
+    const int pages = max(0, c_end - c_begin + kK4Slots - 1) / kK4Slots;
     unsigned char* ring = a4_smem + (size_t)warp * kA4Stages * kA4StepBytes;
     uint64_t* bar = s_bar[warp];
 
@@ -167,7 +165,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     };
     for (int k = 0; k < kA4Stages && k < my_steps; ++k) issue(k);
 
-    // ---- the heads' queries: rotated, scaled by a power of two to a maximum in [2^21, 2^22) and rounded, and their sums over each group of dims ----
+    // ---- the heads' queries: rotated, scaled to a maximum of 2^22 - 1 and rounded, and their sums over each group of dims ----
     const float* q = a.q + (size_t)row * a.q_stride + ((size_t)kvh * L.group + head0) * kA4Hd;
     for (int i = tid; i < HB * 64; i += kA4Threads) {
         const int h = i >> 6, d = i & 63;
@@ -189,15 +187,14 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
     for (int h = warp; h < HB; h += kA4Warps) {
         float4 v = *reinterpret_cast<const float4*>(&s_q[h][4 * lane]);
         const float m = warp_max(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        const int e = max(22, (int)(__float_as_uint(m) >> 23));
-        const float up = __uint_as_float((uint32_t)(127 + 21 - (e - 127)) << 23), down = __uint_as_float((uint32_t)(127 - 21 + (e - 127)) << 23);
+        const float most = fmaxf(m, 1e-25f), up = 4194303.0f / most, down = most / 4194303.0f;
         v.x = rintf(v.x * up); v.y = rintf(v.y * up); v.z = rintf(v.z * up); v.w = rintf(v.w * up);
         *reinterpret_cast<float4*>(&s_q[h][4 * lane]) = v;
         float sum = (v.x + v.y) + (v.z + v.w);
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if ((lane & 7) == 0) s_qsum[h][lane >> 3] = sum;
-        if (lane == 0) s_f[h] = down * (4096.0f * 0.08838834764831845f * 1.4426950408889634f); // the unit of the first bytes' sums, 1/sqrt(128) and log2(e)
+        if (lane == 0) s_f[h] = down * (0.08838834764831845f * 1.4426950408889634f);           // (the unit of the products), 1/sqrt(128) and log2(e)
     }
     __syncthreads();
     const int mine = g & (HB - 1);                       // the head of a lane's scores
@@ -215,11 +212,11 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         s_qa[warp][0][lane] = make_uint4(w[0], w[1], w[2], w[3]);
         if (HB == 8) s_qa[warp][HB == 8 ? 1 : 0][lane] = make_uint4(w2[0], 0, w2[1], 0);
     }
-    uint32_t qm[2] = {0, 0};                             // beside the scale (8-fold), beside the minimum; 2^-6 of the others' unit
+    uint32_t qm[2] = {0, 0};                             // beside the minimum (the scale has 0); 2^-18 of the products' unit
     if (HB == 8 || g < 4) {
-        const float sum = s_qsum[mine][t] * 3.814697265625e-6f, first = __half2float(__float2half_rn(sum));    // 2^-18
-        qm[0] = a4_pack(8.0f * first, first);
-        qm[1] = a4_pack(8.0f * (sum - first), sum - first);
+        const float sum = s_qsum[mine][t] * 3.814697265625e-6f, first = __half2float(__float2half_rn(sum));
+        qm[0] = a4_pack(0.0f, first);
+        qm[1] = a4_pack(0.0f, sum - first);
     }
     const float f = s_f[mine];
     __syncthreads();
@@ -232,8 +229,8 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = 0;
     const uint32_t cut = HB == 8 || g >= 4 ? 0xffffe000u : 0u;                                  // columns 4-7: what the first eleven bits leave
-    const f32x2 minus = pack2(-1.0f, -1.0f), f2 = pack2(f, f), from_float = pack2(-12582912.0f, -12582912.0f), third = pack2(1.52587890625e-5f, 1.52587890625e-5f);
-    const f32x2 second = pack2(0.00390625f, 0.00390625f), part = HB == 8 || g < 4 ? pack2(1.0f, 1.0f) : second, sixty_four = pack2(64.0f, 64.0f);
+    const f32x2 minus = pack2(-1.0f, -1.0f), f2 = pack2(f, f), qm_unit = pack2(262144.0f, 262144.0f);
+    const int shifted = HB == 8 || g < 4 ? 65536 : 256;  // what the row's digits count
     bool gave_up = false;
 
     for (int k = 0; k < my_steps; ++k) {
@@ -285,22 +282,24 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
             const uint4 qa = s_qa[gr][0][lane], qb = s_qa[gr][HB == 8 ? 1 : 0][lane];
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(kr + tile(nt) + 16 * gr), even = a4_signed(w << 4), odd = a4_signed(w);
-                int c[4];
-                a4_imma_from(c, qa, even, odd, kA4FromFloat);
-                f32x2 sum = a4_fma2(add2(a4_pair(c[2], c[3]), from_float), third, add2(a4_pair(c[0], c[1]), from_float));
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(kr + tile(nt) + 16 * gr), even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+                int c[4], d[4];
+                a4_imma(c, qa, even, odd);               // 32 codes times 22 bits and a sign: 31 bits at most
+                c[0] = c[0] * shifted + c[2];
+                c[1] = c[1] * shifted + c[3];
                 if (HB == 8) {
-                    a4_imma_from(c, qb, even, odd, kA4FromFloat);
-                    sum = a4_fma2(add2(a4_pair(c[0], c[1]), from_float), second, sum);
+                    a4_imma(d, qb, even, odd);
+                    c[0] += d[0] * 256;
+                    c[1] += d[1] * 256;
                 }
-                x[nt] = a4_fma2(*reinterpret_cast<const f32x2*>(&s_scale[warp][0][4 * nt + t][gr][0]), sum, x[nt]);
+                x[nt] = a4_fma2(*reinterpret_cast<const f32x2*>(&s_scale[warp][0][4 * nt + t][gr][0]), pack2((float)c[0], (float)c[1]), x[nt]);
             }
         }
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
             float c[4];
             a4_mma8_new(c, qm[0], qm[1], *reinterpret_cast<const uint32_t*>(kr + tile(nt) + kK4Codes));
-            x[nt] = a4_fma2(add2(pack2(c[0], c[1]), pack2(c[2], c[3])), sixty_four, HB == 8 ? x[nt] : a4_mul2(x[nt], part));
+            x[nt] = a4_fma2(add2(pack2(c[0], c[1]), pack2(c[2], c[3])), qm_unit, x[nt]);
             if (HB == 4) x[nt] = add2(x[nt], __shfl_xor_sync(0xffffffffu, x[nt], 16));
         }
         float s[4][2];
@@ -446,6 +445,8 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         s_ml[warp][g][1] = l_run;
     }
     __syncthreads();
+    float* part = w_o + kA4Warps * HB * kA4Hd;            // the CTA's outputs and (maximum, sum), for the cluster
+    float2* part_ml = reinterpret_cast<float2*>(part + HB * kA4Hd);
     for (int i = tid; i < heads * kA4Hd; i += kA4Threads) {
         const int h = i / kA4Hd, d = i % kA4Hd;
         float m = -INFINITY, o = 0.0f, l = 0.0f;
@@ -460,14 +461,46 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         }
         if (L.n_splits == 1) {
             out[i] = l > 0.0f ? o / l : 0.0f;
+        } else if (L.cluster) {
+            part[i] = o;
+            if (d == 0) part_ml[h] = make_float2(m, l);
         } else {
             const size_t at = ((size_t)row * a.n_q + (size_t)kvh * L.group + head0 + h) * L.n_splits + split;
             L.part_o[at * kA4Hd + d] = o;
             if (d == 0) L.part_ml[at] = make_float2(m, l);
         }
     }
+    if (L.cluster) {                                     // each CTA joins a share of the outputs, from all of the cluster's shared memory
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        auto of = [](uint32_t at, int rank) {
+            uint32_t r;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+            return v;
+        };
+        const int share = (heads * kA4Hd + L.n_splits - 1) / L.n_splits;
+        for (int i = split * share + tid; i < min(heads * kA4Hd, (split + 1) * share); i += kA4Threads) {
+            const uint32_t ml = smem_addr(part_ml + i / kA4Hd), at = smem_addr(part + i);
+            float m = -INFINITY, o = 0.0f, l = 0.0f, pm[kA4Cluster];
+#pragma unroll
+            for (int r = 0; r < kA4Cluster; ++r) {
+                pm[r] = r < L.n_splits ? of(ml, r) : -INFINITY;
+                m = fmaxf(m, pm[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < kA4Cluster; ++r) {
+                const float x = a4_ex2(pm[r] - (m == -INFINITY ? 0.0f : m));
+                if (r < L.n_splits) {
+                    o = __fmaf_rn(of(at, r), x, o);
+                    l = __fmaf_rn(of(ml + 4, r), x, l);
+                }
+            }
+            out[i] = l > 0.0f ? o / l : 0.0f;
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");       // until all have read
+    }
 }
-
 
 // The splits of a (row, head): one warp each, four dims a lane.
 __global__ void __launch_bounds__(kA4Threads) attention_kv4_merge_kernel(const A4Launch L) {
@@ -514,30 +547,33 @@ __global__ void __launch_bounds__(kA4Threads) attention_kv4_merge_kernel(const A
 static size_t a4_part_bytes(int rows, int n_q) { return (size_t)rows * n_q * (kA4Hd + 2) * sizeof(float); }
 
 // Keys a CTA takes: the number of splits whose rounds of CTAs take least at the longest length, a CTA's own cost counted as some
-// hundred keys and a split's as some in the second kernel. `most`: as many splits as there is room for partial results.
-static void a4_pick_split(long long items, int resident, int max_len, int most, int* n_splits, int* split_keys) {
-    const long long places = 148 * resident;
+// hundred keys. `most`: as many splits as there is room for partial results; `join`: what joining them costs, in keys.
+static double a4_pick_split(long long items, int max_len, int most, double join, int* n_splits, int* split_keys) {
+    const long long places = 148 * kA4Resident;
     double best = 0.0;
-    for (int want = 1; want <= 64 && (want == 1 || (max_len + want - 1) / want > 128); ++want) {
+    for (int want = 1; want <= most; ++want) {
         const int keys = ((max_len + want - 1) / want + 127) / 128 * 128, splits = (max_len + keys - 1) / keys;
         if (splits > most) continue;
         const long long ctas = items * splits;
         const double rounds = ctas <= 3 * places ? (double)((ctas + places - 1) / places) : (double)ctas / places + 0.5;
-        const double cost = rounds * (keys + 500.0) + (splits > 1 ? 300.0 + 16.0 * (splits - 1) : 0.0);
+        const double cost = rounds * (keys + 500.0) + (splits > 1 ? join + 16.0 * (splits - 1) : 0.0);
         if (want == 1 || cost < best) {
             best = cost;
             *split_keys = keys;
             *n_splits = splits;
         }
+        if (keys == 128) break;
     }
+    return best;
 }
 
 template <int HB>
 static int a4_run(const A4Launch& L, cudaStream_t st) {
     const size_t smem = (size_t)kA4Warps * kA4Stages * kA4StepBytes;
+    static_assert(kA4Warps * HB * kA4Hd * 4 + HB * (kA4Hd + 2) * 4 <= kA4Warps * kA4Stages * kA4StepBytes, "outputs where the rings were");
     if (cudaError_t e = allow_smem(attention_kv4_kernel<HB>, smem)) return (int)e;
     const dim3 grid((unsigned)L.a.rows * (unsigned)L.n_splits, (unsigned)(L.a.cache.n_kv * L.head_blocks));
-    return kv4_launch(attention_kv4_kernel<HB>, grid, kA4Threads, smem, st, L.a.use_pdl != 0, L);
+    return kv4_launch_cluster(attention_kv4_kernel<HB>, grid, kA4Threads, L.cluster ? L.n_splits : 1, smem, st, L.a.use_pdl != 0, L);
 }
 
 int kv4_attention_take_error() {
@@ -582,14 +618,22 @@ extern "C" int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, vo
         L.n_splits = (a.max_len + L.split_keys - 1) / L.split_keys;
         if (L.n_splits > 1 && room < (size_t)L.n_splits) return -1;
     } else {
-        a4_pick_split(items, kA4Resident, a.max_len, room > 1 ? (int)(room < 64 ? room : 64) : 1, &L.n_splits, &L.split_keys);
+        const double apart = a4_pick_split(items, a.max_len, room > 1 ? (int)(room < 64 ? room : 64) : 1, 300.0, &L.n_splits, &L.split_keys);
+        // Joined by clusters: 1 x 1000 keys 7.0 us and 9.2 by a second kernel, 12 x 8192 of 40/5 heads 36.3 and 38.1; but where CTAs come in several rounds
+        // a cluster waits for room for all of its own (256 x 4095 ragged: 218 and 174).
+        int splits, keys;
+        if (a4_pick_split(items, a.max_len, kA4Cluster, 100.0, &splits, &keys) < apart && splits > 1 && items * splits <= 148 * kA4Resident) {
+            L.n_splits = splits;
+            L.split_keys = keys;
+            L.cluster = 1;
+        }
     }
     if ((long long)a.rows * L.n_splits > 0x7fffffffLL) return -1;
     L.part_o = static_cast<float*>(a.workspace);
     L.part_ml = reinterpret_cast<float2*>(L.part_o + (size_t)a.rows * a.n_q * L.n_splits * kA4Hd);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (int rc = hb == 4 ? a4_run<4>(L, st) : a4_run<8>(L, st)) return rc;
-    if (L.n_splits == 1) return 0;
+    if (L.n_splits == 1 || L.cluster) return 0;
     return kv4_launch(attention_kv4_merge_kernel, dim3((unsigned)a.rows, (unsigned)((a.n_q + kA4Warps - 1) / kA4Warps)), kA4Threads, 0, st, true, L);
 }
 

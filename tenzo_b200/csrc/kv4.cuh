@@ -48,20 +48,33 @@ inline bool kv4_cache_ok(const tenzo_kv4_cache& c) {
            c.table_stride > 0;
 }
 
-// Launch, with (or without) the attribute that lets the kernel become resident while its predecessor drains.
+// Launch in clusters of `cluster` blocks along x, with (or without) the attribute that lets the kernel become resident while its predecessor drains.
 template <typename... KArgs, typename... Args>
-inline int kv4_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool pdl, Args&&... args) {
+inline int kv4_launch_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, int cluster, size_t smem, cudaStream_t st, bool pdl, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    unsigned n = 0;
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = (unsigned)cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
+    cfg.numAttrs = n;
     return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <typename... KArgs, typename... Args>
+inline int kv4_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool pdl, Args&&... args) {
+    return kv4_launch_cluster(kernel, grid, threads, 1, smem, st, pdl, args...);
 }
 
 }  // namespace tz

@@ -296,9 +296,8 @@ def attention_kv4(q, pool, pos, *, layer, n_q, block_table, seq=None, rope_cos=N
         out = torch.empty(rows, n_q * 128, dtype=torch.float32, device=q.device)
     elif out.shape != (rows, n_q * 128):
         raise ValueError(f"out is [{rows}, {n_q * 128}]")
-    if workspace is None:
-        need = _beam_calls()[5](rows, n_q, n_kv, max_len)
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    if workspace is None and (split_keys or max_len > 1024):       # (up to 1024 keys the call does as well without)
+        workspace = torch.empty(_beam_calls()[5](rows, n_q, n_kv, max_len), dtype=torch.uint8, device=q.device)
     args = _KV4_ATTENTION.pack(qp, _arg(out, torch.float32, dev, "out"), *_KV4_CACHE.unpack(cache), _arg_entries(pos, rows, dev, "pos"), _arg_entries(seq, rows, dev, "seq"),
                                cos, sin, length, q_stride, layer, n_q, rows, max_len, split_keys, use_pdl, _arg(workspace, torch.uint8, dev, "workspace"),
                                0 if workspace is None else workspace.numel())
