@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
 // Logits a thread takes: 32, or fewer where that would leave SMs without a CTA.
 // (and lists would no longer be held in registers by the second kernel).
 static int beam_chunks(int per, int vocab) { return (int)(((long long)vocab + kBsThreads * per - 1) / (kBsThreads * per)); }
-static int beam_slots(int k) { return (k > kBsLeast ? k : kBsLeast) + 2 * kBsWindow; }
+static int beam_slots(int k) { return ((k > kBsLeast ? k : kBsLeast) + 2 * kBsWindow + 1) / 2 * 2; }      // (even: they are read two at a time)
 static int beam_per(int rows, int vocab, int k) {
     int per = kBsMostPer;
     while (per > 4 && (long long)rows * beam_chunks(per, vocab) < 128 && (long long)beam_chunks(per / 2, vocab) * beam_slots(k) <= kBsHold) per /= 2;

@@ -163,6 +163,34 @@ def test_graph_and_side_stream(cuda_lib):
         assert np.array_equal(host(parent), want[0]) and np.array_equal(host(token), want[1])
 
 
+@pytest.mark.parametrize("k", [15, 17, 19, 31, 33, 47, 63])
+def test_odd_numbers_of_candidates(cuda_lib, k):
+    rng = np.random.default_rng(k)
+    for beams, vocab in ((32, 1000), (3, 40001), (1, 128256)):
+        logits = (rng.standard_normal((2 * beams, vocab)) * 2).astype(np.float32)
+        logits[:, ::5] = np.round(logits[:, ::5])
+        check(logits, (-9 * rng.random(2 * beams)).astype(np.float32), beams, k)
+
+
+def test_two_at_once(cuda_lib):
+    """Calls on two streams, each with a workspace of its own."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(8)
+    rows = [(rng.standard_normal((8, 60000)) * 2).astype(np.float32) for _ in range(2)]
+    want = [ref.select(x, np.zeros(8, np.float32), 4, 8) for x in rows]
+    d, scores, streams = [dev(x) for x in rows], torch.zeros(8, device="cuda"), [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(kernels.beam_select(d[i], scores, beams=4, k=8, use_pdl=True))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for parent, token, _ in got[i]:
+            assert np.array_equal(host(parent), want[i][0]) and np.array_equal(host(token), want[i][1])
+
+
 def test_no_groups(cuda_lib):
     from tenzo_b200 import kernels
     parent, token, score = kernels.beam_select(torch.empty(0, 10, device="cuda"), torch.empty(0, device="cuda"), beams=2, k=3)
