@@ -603,6 +603,7 @@ extern "C" int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, vo
     if (a.layer < 0 || a.layer >= a.cache.n_layers || a.n_q <= 0 || a.n_q % a.cache.n_kv || a.rows < 0 || a.max_len <= 0) return -1;
     if (a.max_len > (long long)a.cache.table_stride * kK4Slots || (!a.seq && a.rows > a.cache.table_rows)) return -1;
     if ((a.rope_cos == nullptr) != (a.rope_sin == nullptr) || (a.rope_cos && a.rope_len < a.max_len)) return -1;
+    if (a.max_len > 1 << 30 || a.n_q > 4 * 65535) return -1;
     if (a.split_keys < 0 || (reinterpret_cast<uintptr_t>(a.out) & 15)) return -1;
     if (a.q_stride == 0) a.q_stride = a.n_q * kA4Hd;
     if (a.q_stride < a.n_q * kA4Hd) return -1;

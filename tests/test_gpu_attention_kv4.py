@@ -205,6 +205,45 @@ def test_two_graphs_on_one_workspace_and_a_side_stream(cuda_lib):
     assert kernels.kv4_take_errors() == 0
 
 
+@pytest.mark.parametrize("n_q,n_kv", [(4, 2), (8, 1), (12, 1)])
+def test_a_prompts_rows(cuda_lib, n_q, n_kv):
+    """Every position of one sequence as a row of its own, in any order."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(n_q)
+    n = 700
+    table, pool = setup(rng, [n], n_kv, 44)
+    pos = rng.permutation(n).astype(np.int32)
+    q = rng.standard_normal((n, n_q * 128)).astype(np.float32)
+    cos, sin = ref.rope(n)
+    out = host(kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=n_q, block_table=dev(table), seq=torch.zeros(n, dtype=torch.int32, device="cuda"),
+                                     rope_cos=dev(cos), rope_sin=dev(sin)))
+    some = rng.choice(n, 60, replace=False)
+    check(out[some], q[some], pool, table, 0, pos[some], np.zeros(60, int), cos, sin)
+
+
+def test_two_at_once(cuda_lib):
+    """Calls on two streams, joined by clusters, by a second kernel, and not at all; each with a workspace of its own."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(31)
+    for lens, split in (([900, 1000], 0), ([5000, 4000], 0), ([300, 200], 512)):
+        table, pool = setup(rng, lens, 2, (max(lens) + 15) // 16)
+        q = [rng.standard_normal((2, 8 * 128)).astype(np.float32) for _ in range(2)]
+        pos = np.array(lens, np.int32) - 1
+        dq, dp, dpos, dt = [dev(x) for x in q], dev(pool), dev(pos), dev(table)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        got = [[], []]
+        for _ in range(10):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(kernels.attention_kv4(dq[i], dp, dpos, layer=0, n_q=8, block_table=dt, split_keys=split, use_pdl=True))
+        torch.cuda.synchronize()
+        for i in range(2):
+            check(host(got[i][0]), q[i], pool, table, 0, pos, range(2))
+            assert all(torch.equal(got[i][0], x) for x in got[i])
+    assert kernels.kv4_take_errors() == 0
+
+
 def test_pools_beyond_32_bits(cuda_lib):
     """Blocks whose bytes lie past 2^31 and 2^32 of the pool's start."""
     from tenzo_b200 import kernels
