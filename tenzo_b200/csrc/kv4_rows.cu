@@ -188,20 +188,23 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_read_kernel(const RowsArgs
 // A group's beams all hold `length` tokens. Full blocks are shared, so a table row is its parent's; the block being filled is every
 // beam's own: the first child keeps its parent's, a further one gets that of a beam without children and the filled rows are copied
 // into it. Nothing is read that this launch writes: sources have children, targets have none, and the tables are two.
-// CTA (x, y): beam x, part y of the copy. Bound by memory: length % 16 rows of 80 bytes, layers x heads x 2 times, in and out.
-constexpr int kReorderThreads = 256, kReorderParts = 8;
+// CTA (x, y): part y of all that group x copies, and every gridDim.y-th of its table rows: each CTA has its share of the work, and the chain of length, parents
+// and table entries in front of it is waited for once (64 x 8 beams: 20.5 us with CTAs a beam, two thirds of which found nothing to copy, 16.7 now).
+// Bound by memory: length % 16 rows of 80 bytes, layers x heads x 2 times, in and out.
+constexpr int kReorderThreads = 256, kReorderBatch = 8;  // 16-byte loads in flight a thread
 
-__global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenzo_kv4_cache c, int* table_out, const int* parent,
-                                                                      const int* length, int beams, int use_pdl) {
-    const int g = blockIdx.x / beams, i = blockIdx.x % beams, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenzo_kv4_cache c, int* table_out, const int* parent, const int* length, int beams,
+                                                                      int use_pdl) {
+    const int g = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
     const int* rows = c.block_table + (size_t)g * beams * c.table_stride;      // the group's
-    const int len = ld_l2(length + g), col = len / kK4Slots, filled = len < 0 ? 0 : len % kK4Slots;
     const bool mine = lane < beams;
+    const int len = ld_l2(length + g);
     int p = mine ? ld_l2(parent + (size_t)g * beams + lane) : lane;
+    const int col = len / kK4Slots, filled = len < 0 ? 0 : len % kK4Slots;
     const bool bad = (mine && (p < 0 || p >= beams)) || len < 0 || col + (filled > 0) > c.table_stride;
     const bool refused = __any_sync(0xffffffffu, bad);
     if (refused) {                                       // the group stays as it is
@@ -210,45 +213,54 @@ __global__ void __launch_bounds__(kReorderThreads) kv4_reorder_kernel(const tenz
     }
     const unsigned all = beams == 32 ? 0xffffffffu : (1u << beams) - 1u;
     const unsigned alike = __match_any_sync(0xffffffffu, p) & all, below = (1u << lane) - 1u;
-    const unsigned further = __ballot_sync(0xffffffffu, mine && (alike & below));
+    unsigned further = __ballot_sync(0xffffffffu, mine && (alike & below));
     const unsigned childless = all & ~__reduce_or_sync(0xffffffffu, mine ? 1u << p : 0u);
-    const int from = __shfl_sync(0xffffffffu, p, i);
-    const bool copies = filled > 0 && ((further >> i) & 1u);
-    int giver = filled > 0 ? from : i;                   // whose block the beam goes on filling
-    if (copies) {
-        unsigned left = childless;                       // as many beams are without children as there are further ones
-        for (int n = __popc(further & ((1u << i) - 1u)); n > 0; --n) left &= left - 1u;
+    if (filled == 0) further = 0;                        // there is no block being filled
+    int giver = filled > 0 ? p : lane;                   // whose block lane's beam goes on filling
+    if ((further >> lane) & 1u) {                        // the n-th further child gets the n-th beam's without children; there are as many
+        unsigned left = childless;
+        for (int n = __popc(further & below); n > 0; --n) left &= left - 1u;
         giver = __ffs((int)left) - 1;
     }
-    if (blockIdx.y == 0) {
+    // Every warp has all of this. The tables, a warp a row:
+    for (int i = blockIdx.y * (kReorderThreads / 32) + warp; i < beams; i += gridDim.y * (kReorderThreads / 32)) {
+        const int from = __shfl_sync(0xffffffffu, p, i), tail = __shfl_sync(0xffffffffu, giver, i);
         int* out = table_out + ((size_t)g * beams + i) * c.table_stride;
-        for (int x = threadIdx.x; x < c.table_stride; x += kReorderThreads)
-            out[x] = ld_l2(rows + (size_t)(refused ? i : x < col ? from : x == col ? giver : i) * c.table_stride + x);
+        for (int x = lane; x < c.table_stride; x += 32) out[x] = ld_l2(rows + (size_t)(refused ? i : x < col ? from : x == col ? tail : i) * c.table_stride + x);
     }
-    if (!copies) return;
-    const int source = ld_l2(rows + (size_t)from * c.table_stride + col), target = ld_l2(rows + (size_t)giver * c.table_stride + col);
-    if (source < 0 || source >= c.n_blocks || target < 0 || target >= c.n_blocks) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&g_kv4_rows_error, kK4ErrIndex);
-        return;
-    }
-    const unsigned halves = c.n_layers * c.n_kv * 2, units = filled * (kK4Row / 16), total = halves * units;         // 16-byte units of a half page, and in all
-    const unsigned by_units = 0xffffffffu / units + 1u;  // i / units for i below 2^32 / units
-    const uint4* src = reinterpret_cast<const uint4*>(c.pool + (size_t)source * halves * kK4Half);
-    uint4* dst = reinterpret_cast<uint4*>(c.pool + (size_t)target * halves * kK4Half);
-    constexpr unsigned kUnits = kK4Half / 16, kStep = kReorderParts * kReorderThreads;
-    constexpr int kBatch = 8;                            // loads in flight
-    for (unsigned i0 = blockIdx.y * kReorderThreads + threadIdx.x; i0 < total; i0 += kBatch * kStep) {
-        uint4 w[kBatch];
-        size_t at[kBatch];
-#pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-            const unsigned i = i0 + n * kStep, h = __umulhi(i, by_units);
-            at[n] = (size_t)h * kUnits + (i - h * units);
-            if (i < total) w[n] = ld_l2(src + at[n]);
+    if (!further) return;
+    // The blocks: lane's copy, if its beam is a further child (-1: none, or an entry out of range).
+    int source = -1, target = -1;
+    if ((further >> lane) & 1u) {
+        source = ld_l2(rows + (size_t)p * c.table_stride + col);
+        target = ld_l2(rows + (size_t)giver * c.table_stride + col);
+        if (source < 0 || source >= c.n_blocks || target < 0 || target >= c.n_blocks) {
+            if (warp == 0 && blockIdx.y == 0) atomicOr(&g_kv4_rows_error, kK4ErrIndex);
+            source = -1;
         }
+    }
+    const unsigned halves = c.n_layers * c.n_kv * 2, units = filled * (kK4Row / 16), total = halves * units;       // 16-byte units of a half page, and of a block
+    const unsigned by_units = 0xffffffffu / units + 1u;  // i / units for i below 2^32 / units
+    constexpr unsigned kUnits = kK4Half / 16;
+    const unsigned step = gridDim.y * kReorderThreads;
+    for (; further; further &= further - 1u) {
+        const int i = __ffs((int)further) - 1, s = __shfl_sync(0xffffffffu, source, i), t = __shfl_sync(0xffffffffu, target, i);
+        if (s < 0) continue;
+        const uint4* src = reinterpret_cast<const uint4*>(c.pool + (size_t)s * halves * kK4Half);
+        uint4* dst = reinterpret_cast<uint4*>(c.pool + (size_t)t * halves * kK4Half);
+        for (unsigned u0 = blockIdx.y * kReorderThreads + threadIdx.x; u0 < total; u0 += kReorderBatch * step) {
+            uint4 w[kReorderBatch];
+            size_t at[kReorderBatch];
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n)
-            if (i0 + n * kStep < total) dst[at[n]] = w[n];
+            for (int n = 0; n < kReorderBatch; ++n) {
+                const unsigned u = u0 + n * step, h = __umulhi(u, by_units);
+                at[n] = (size_t)h * kUnits + (u - h * units);
+                if (u < total) w[n] = ld_l2(src + at[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < kReorderBatch; ++n)
+                if (u0 + n * step < total) dst[at[n]] = w[n];
+        }
     }
 }
 
@@ -310,6 +322,11 @@ extern "C" int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_o
     if (!cache || !kv4_cache_ok(*cache) || !table_out || table_out == cache->block_table || !parent || !length || groups < 1) return -1;
     if (beams < 1 || beams > TENZO_BEAMS_MOST) return -5;
     if ((long long)groups * beams != cache->table_rows) return -1;
-    return kv4_launch(kv4_reorder_kernel, dim3((unsigned)(groups * beams), kReorderParts), kReorderThreads, 0, static_cast<cudaStream_t>(stream), use_pdl != 0, *cache,
-                      table_out, parent, length, beams, use_pdl != 0);
+    if ((long long)cache->n_layers * cache->n_kv > 16384) return -5;          // (a block's 16-byte units are numbered in 32 bits, and divided by multiplication)
+    // Parts of a group: six CTAs an SM in all (64 x 8 beams: 2 an SM 20.1 us, 3 18.2, 6 16.7, 16 16.6), and a batch of loads each at the most.
+    const long long units = (long long)cache->n_layers * cache->n_kv * 2 * (kK4Half / 16), most = (units + kReorderThreads * kReorderBatch - 1) / (kReorderThreads * kReorderBatch);
+    long long parts = 6 * 148 / groups;
+    parts = parts < 1 ? 1 : parts > most ? most : parts;
+    return kv4_launch(kv4_reorder_kernel, dim3((unsigned)groups, (unsigned)parts), kReorderThreads, 0, static_cast<cudaStream_t>(stream), use_pdl != 0, *cache, table_out, parent,
+                      length, beams, use_pdl != 0);
 }

@@ -64,6 +64,29 @@ def test_reorder_refuses_on_the_device(cuda_lib):
     assert np.array_equal(host(out), want_table) and np.array_equal(host(d_pool), want_pool)
 
 
+def test_selection_and_reordering_overlapped(cuda_lib):
+    """Selection, then the reordering that reads its parents, launched to overlap, many times over: nothing is read before the kernel in front has written it."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(2)
+    groups, beams, vocab = 2, 4, 211
+    table, pool = beams_setup(rng, groups, beams, 3, 1, 2)
+    d_table, d_pool, length = dev(table), dev(pool), torch.full((groups,), 21, dtype=torch.int32, device="cuda")
+    logits = [rng.standard_normal((groups * beams, vocab)).astype(np.float32) for _ in range(16)]
+    scores = np.zeros(groups * beams, np.float32)
+    want = []
+    for x in logits:
+        parent, token, _ = ref.select(x, scores, beams, beams)
+        want.append((parent, token, *ref.reorder(pool, table, parent.astype(np.int32), np.full(groups, 21))))
+    d_logits, d_scores = [dev(x) for x in logits], dev(scores)
+    got = []
+    for i in range(400):
+        p = d_pool.clone()
+        parent, token, _ = kernels.beam_select(d_logits[i % 16], d_scores, beams=beams, k=beams, use_pdl=True)
+        got.append((parent, token, kernels.kv4_reorder(p, d_table, parent, length, use_pdl=True), p))
+    for i, g in enumerate(got):
+        assert all(np.array_equal(host(a), b) for a, b in zip(g, want[i % 16])), i
+
+
 @pytest.mark.parametrize("pdl", [False, True])
 def test_beam_search(cuda_lib, pdl):
     """Two requests with four beams, prompts that end inside a block and at its end, 40 steps: the beams' tokens are those of a search that

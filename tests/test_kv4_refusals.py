@@ -55,10 +55,12 @@ def attention(**over):
 
 
 @pytest.mark.parametrize("over", [dict(q=None), dict(out=None), dict(pos=None), dict(layer=2), dict(layer=-1), dict(n_q=0), dict(n_q=7), dict(rows=-1), dict(max_len=0),
-                                  dict(max_len=81), dict(seq=None, rows=5), dict(rope_cos=P), dict(rope_sin=P), dict(rope_cos=P, rope_sin=P, rope_len=79),
+                                  dict(max_len=81), dict(max_len=(1 << 30) + 1), dict(seq=None, rows=5), dict(rope_cos=P), dict(rope_sin=P), dict(rope_cos=P, rope_sin=P, rope_len=79),
                                   dict(q_stride=767), dict(split_keys=-1), dict(out=P + 4), dict(split_keys=16), dict(split_keys=16, workspace=P + 8, workspace_bytes=1 << 30),
                                   dict(split_keys=16, max_len=80, workspace=P, workspace_bytes=10)], ids=str)
 def test_attention(lib, over):
+    if over.get("max_len") == (1 << 30) + 1:
+        over = dict(over, cache=cache(table_stride=1 << 27))
     if "split_keys" in over and over["split_keys"] == 16:
         over = dict(over, cache=cache(table_stride=100), max_len=1000)       # eight splits, and no room for them
     assert lib.tenzo_cuda_attention_kv4(C.byref(attention(**over)), None) == abi.ERR_INVALID
@@ -72,10 +74,10 @@ def test_attention_null_and_sizes(lib):
 
 
 @pytest.mark.parametrize("change,code", [(dict(out=None), -1), (dict(out=P), -1), (dict(parent=None), -1), (dict(length=None), -1), (dict(groups=0), -1), (dict(groups=-2), -1),
-                                         (dict(groups=3), -1), (dict(beams=0), -5), (dict(beams=33), -5)], ids=str)
+                                         (dict(groups=3), -1), (dict(beams=0), -5), (dict(beams=33), -5), (dict(layers=10000), -5)], ids=str)
 def test_reorder(lib, change, code):
-    a = dict(out=P + 4096, parent=P, length=P, groups=2, beams=2) | change
-    assert lib.tenzo_cuda_kv4_reorder(C.byref(cache()), a["out"], a["parent"], a["length"], a["groups"], a["beams"], 0, None) == code
+    a = dict(out=P + 4096, parent=P, length=P, groups=2, beams=2, layers=2) | change
+    assert lib.tenzo_cuda_kv4_reorder(C.byref(cache(n_layers=a["layers"])), a["out"], a["parent"], a["length"], a["groups"], a["beams"], 0, None) == code
     assert lib.tenzo_cuda_kv4_reorder(None, P, P, P, 2, 2, 0, None) == -1
 
 
