@@ -269,17 +269,27 @@ def kv4_read(pool, pos, *, layer, block_table, seq=None, use_pdl=False, k=None, 
     dev, n = _current_device(), len(pos)
     cache, n_kv, _, _ = _kv4_cache(pool, block_table, dev)
     if k is None and v is None:
-        k = torch.empty(n, n_kv * 128, dtype=torch.float32, device=pool.device)
-        v = torch.empty_like(k)
-    (kp, ks, m), (vp, vs, o) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
-    if n != m or n != o or (ks != vs and n > 1):
-        raise ValueError("k and v have one row for each position, equally far apart")
+        ks = n_kv * 128
+        both = torch.empty(2, n, ks, dtype=torch.float32, device=pool.device)
+        kp = both.data_ptr()
+        vp = kp + 4 * n * ks
+        k, v = both.unbind(0)
+    else:
+        (kp, ks, m), (vp, vs, o) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
+        if n != m or n != o or (ks != vs and n > 1):
+            raise ValueError("k and v have one row for each position, equally far apart")
     _ok(_beam_calls()[1](cache, layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, use_pdl, _raw_stream(dev)), "tenzo_cuda_kv4_read")
     return k, v
 
 
+@functools.lru_cache(1024)
 def attention_kv4_workspace_bytes(rows, n_q, n_kv, max_len) -> int:
     return _beam_calls()[5](rows, n_q, n_kv, max_len)
+
+
+@functools.lru_cache(1024)
+def beam_select_workspace_bytes(groups, beams, vocab, k) -> int:
+    return _beam_calls()[6](groups, beams, vocab, k)
 
 
 def attention_kv4(q, pool, pos, *, layer, n_q, block_table, seq=None, rope_cos=None, rope_sin=None, max_len=None, split_keys=0, use_pdl=False, out=None,
@@ -297,7 +307,7 @@ def attention_kv4(q, pool, pos, *, layer, n_q, block_table, seq=None, rope_cos=N
     elif out.shape != (rows, n_q * 128):
         raise ValueError(f"out is [{rows}, {n_q * 128}]")
     if workspace is None and (split_keys or max_len > 1024):       # (up to 1024 keys the call does as well without)
-        workspace = torch.empty(_beam_calls()[5](rows, n_q, n_kv, max_len), dtype=torch.uint8, device=q.device)
+        workspace = torch.empty(attention_kv4_workspace_bytes(rows, n_q, n_kv, max_len), dtype=torch.uint8, device=q.device)
     args = _KV4_ATTENTION.pack(qp, _arg(out, torch.float32, dev, "out"), *_KV4_CACHE.unpack(cache), _arg_entries(pos, rows, dev, "pos"), _arg_entries(seq, rows, dev, "seq"),
                                cos, sin, length, q_stride, layer, n_q, rows, max_len, split_keys, use_pdl, _arg(workspace, torch.uint8, dev, "workspace"),
                                0 if workspace is None else workspace.numel())
@@ -317,7 +327,7 @@ def beam_select(logits, scores, *, beams, k, finished=None, eos=0, use_pdl=False
     parent, token, score = torch.empty(3, groups, k, dtype=torch.int32, device=device).unbind(0)
     score = score.view(torch.float32)
     if workspace is None:
-        workspace = torch.empty(_beam_calls()[6](groups, beams, vocab, k), dtype=torch.uint8, device=device)
+        workspace = torch.empty(beam_select_workspace_bytes(groups, beams, vocab, k), dtype=torch.uint8, device=device)
     args = _BEAM_SELECT.pack(lp, _arg(scores, torch.float32, dev, "scores"), _arg_entries(finished, rows, dev, "finished"), eos, stride, groups, beams, vocab, k,
                              use_pdl, parent.data_ptr(), token.data_ptr(), score.data_ptr(), _arg(workspace, torch.uint8, dev, "workspace"), workspace.numel())
     _ok(_beam_calls()[4](args, _raw_stream(dev)), "tenzo_cuda_beam_select")
