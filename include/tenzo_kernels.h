@@ -270,7 +270,8 @@ TENZO_API int tenzo_cuda_kv4_read(const tenzo_kv4_cache* cache, int layer, float
  * pos[row] as above; query head h reads kv head h / (n_q / n_kv), any n_q that n_kv divides. Several rows may name one sequence
  * (a prompt's or a draft's rows, each with its own position). pos[row] < 0: zeros. A row whose position is max_len or more, or whose table row is
  * out of range, is not written and raises the flag; a table entry out of range leaves its 16 keys out and raises it. Sums and softmax in
- * fp32; products with the query and with the weights keep 22 bits (two fp16 parts), outputs agree with 64 bits to about 1e-6 of the output's norm. */
+ * fp32; the query is rounded to 23 bits of its head's largest number, products with the weights keep 22 bits (two fp16 parts), outputs agree with
+ * 64 bits to about 1e-6 of the output's norm where scores are not above a few tens. A NaN or an infinity in a head's query makes that head's output NaN. */
 typedef struct {
     const float* q;          /* [rows][q_stride], n_q*128 used, before rotation */
     float* out;              /* [rows][n_q*128] */
@@ -285,7 +286,7 @@ typedef struct {
     int split_keys;          /* keys a CTA takes (rounded up to 128); 0 = choose */
     int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
     void* workspace;         /* 16-byte aligned, contents need not be kept: partial results of splits. tenzo_cuda_attention_kv4_workspace_bytes(...) */
-    size_t workspace_bytes;  /* bytes; with less (or NULL) fewer splits are taken, and split_keys that need more are refused (-1) */
+    size_t workspace_bytes;  /* bytes; with less (or NULL) fewer splits are taken (few rows need none), and split_keys that need more are refused (-1) */
 } tenzo_attention_kv4_args;
 TENZO_API int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, void* stream);
 TENZO_API size_t tenzo_cuda_attention_kv4_workspace_bytes(int rows, int n_q, int n_kv, int max_len);
@@ -298,8 +299,8 @@ TENZO_API int tenzo_cuda_kv4_take_errors(void);
  * blocks are shared) and its own above j. The block being filled, entry j if r > 0, belongs to one beam alone (they must differ): the first child of a
  * parent takes its parent's; the n-th of the further children, by index, takes that of the n-th beam without children, and the r filled slots of all layers and heads are copied
  * into it. If r = 0, entry j stays the beam's own. No block is allocated or freed, and a prompt is forked the same way: parent 0 for
- * all. table_out [groups*beams][table_stride] must not overlap the table; groups*beams = table_rows, beams <= TENZO_BEAMS_MOST (-5 otherwise).
- * A group with a parent or a length out of range is copied as it is and raises the flag. */
+ * all. table_out [groups*beams][table_stride] must not overlap the table; groups*beams = table_rows, beams <= TENZO_BEAMS_MOST and
+ * n_layers*n_kv <= 16384 (-5 otherwise). A group with a parent or a length out of range is copied as it is and raises the flag. */
 enum { TENZO_BEAMS_MOST = 32 };
 TENZO_API int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_out, const int* parent, const int* length, int groups, int beams, int use_pdl,
                                      void* stream);
@@ -307,7 +308,8 @@ TENZO_API int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_ou
 /* ---- beam search: the k best continuations over beams x vocabulary -----------------------------------------
  * Beside the greedy argmax and the sampler (:1722-1807); the reference has no beam search. logits [groups*beams][row_stride] fp32,
  * scores [groups*beams] the beams' sums of log-probabilities. Per group, over all beams b and tokens t,
- *   score(b, t) = scores[b] + (x_t - log sum_u exp x_u)   in 64 bits,
+ *   score(b, t) = scores[b] + (x_t - log sum_u exp x_u)   in 64 bits
+ * (exponentials other than the largest ones' enter the sum with 32: its logarithm is good to some 1e-7, to 2e-6 at the worst),
  * the k best go to parent_out / token_out / score_out [groups][k], best first; of equal scores the lower beam, in a beam the larger logit, then the
  * lower token. score_out is rounded to fp32.
  * A finished beam (finished[row] != 0) has its end token `eos` alone, at scores[b]. -inf masks a token; NaN counts as -inf, +inf as the largest finite

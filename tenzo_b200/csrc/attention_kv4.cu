@@ -3,20 +3,27 @@
 //
 //   * The keys of a (row, kv head) are split over CTAs and, inside a CTA, over four warps that never wait for one another: each streams
 //     steps of 32 keys, two pages of 2560 bytes by one bulk copy each, through a ring of its own and keeps a running
-//     (maximum, sum, output) per query head. The triples meet by log-sum-exp, first the warps', then the splits' in a second kernel.
-//   * A nibble in the low bits of a 16-bit word is the fp16 number code * 2^-24, one field further up code * 2^-20; one packed multiplication
-//     makes two of them normal numbers. (The tensor cores take subnormal operands too, exactly, but line the products up by the
-//     exponent they are written with: sums lose the leading zeros' bits, 1e-5 instead of 4e-7 over 100 keys.) With
-//     value = minimum + scale * code per group of 32 dims,
+//     (maximum, sum, output) per query head. The triples meet by log-sum-exp, first the warps', then the splits': in shared memory of a
+//     thread-block cluster, or in a second kernel where there are too many.
+//   * With value = minimum + scale * code per group of 32 dims,
 //       q.k   = sum_g scale_g (q_g . c_g) + minimum_g (sum of q over g)
-//       p.v_d = sum_t (p_t scale_tg) c_td + sum_t p_t minimum_tg
-//     the products with codes are one chain of MMAs a group, whose sums (or weights) take the scale in fp32; the terms with the minima
-//     are one MMA more, over the parameters as they lie.
-//   * The other operands have 22 bits: queries and weights enter as two fp16 parts each (the query scaled to a maximum near 2^7, the
-//     weights to at most 2^14 with the largest scale of the values seen so far). Outputs agree with 64 bits to a few 1e-7.
-//   * S = Q K^T has heads as rows (rows 0-7 the first parts, 8-15 the second, so a lane adds the two itself) and its accumulators are, lane
-//     by lane, the weights' B operand of O^T = V^T P^T, whose columns are heads. Up to four heads a kv head, columns 4-7 carry the
-//     weights' second parts; with five to eight a second MMA does.
+//       p.v_d = sum_t (p_t scale_tg) (c_td - 8) + sum_t p_t (minimum_tg + 8 scale_tg)
+//     the products with codes run on the tensor cores, which see nothing but codes as they lie, and the scales go in fp32 to the sums (keys) or to the
+//     weights (values); the other terms are one MMA more, over the parameters.
+//   * Keys: whole numbers. A head's query is scaled to a maximum of 2^22 - 1 and rounded, and its three signed bytes are rows of the A operand (products of bytes and
+//     codes, 32 dims a chain: exact in 32 bits). Up to four heads a kv head, rows 0-3 have the first bytes, 4-7 the second and 8-11 the third, so one MMA does; with
+//     more a second one.
+//   * Values: fp16. A nibble in the low bits of a 16-bit word is the number code * 2^-24, one field further up code * 2^-20; one packed fused
+//     multiplication makes two of them normal numbers (code - 8) * 2^-9. (The tensor cores take subnormal operands too, exactly, but line the products up by the
+//     exponent they are written with: sums lose the leading zeros' bits, 1e-5 instead of 4e-7 over 100 keys. And they cut off what a sum's last bit
+//     does not hold, always towards zero: hence codes around zero, and accumulators of 32 keys that are added up in fp32.) The weights, up to 2^14 with the largest
+//     scale of the values seen so far, enter as two parts of eleven bits.
+//   * S = Q K^T has heads as rows, and its accumulators are, lane by lane, the weights' B operand of O^T = V^T P^T, whose columns are heads. Up to four heads a kv
+//     head, columns 4-7 carry the weights' second parts; with five to eight a second MMA does.
+// Outputs agree with 64 bits to a few 1e-7.
+//
+// 64 x 8192 keys of 20/5 heads: 114 us, 420 MB at 3.7 TB/s or 0.56 of the memory's rate. What bounds it is the issue of instructions: some 1100 slots for a step of 32 keys,
+// three quarters of them unpacking, scaling and converting around the 38 MMAs (110 us without the copies, 78 without the MMAs and what they need, 44 without either).
 #include "attn_common.cuh"
 #include "kv4.cuh"
 
@@ -460,7 +467,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
             l = __fmaf_rn(s_ml[w][h][1], x, l);
         }
         if (L.n_splits == 1) {
-            out[i] = l > 0.0f ? o / l : 0.0f;
+            out[i] = l == 0.0f ? 0.0f : o / l;
         } else if (L.cluster) {
             part[i] = o;
             if (d == 0) part_ml[h] = make_float2(m, l);
@@ -496,7 +503,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
                     l = __fmaf_rn(of(ml + 4, r), x, l);
                 }
             }
-            out[i] = l > 0.0f ? o / l : 0.0f;
+            out[i] = l == 0.0f ? 0.0f : o / l;
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");       // until all have read
     }
@@ -540,7 +547,7 @@ __global__ void __launch_bounds__(kA4Threads) attention_kv4_merge_kernel(const A
             l = __fmaf_rn(v[u].y, x, l);
         }
     }
-    const float r = l > 0.0f ? 1.0f / l : 0.0f;
+    const float r = l == 0.0f ? 0.0f : 1.0f / l;         // (a query with a NaN has a NaN here)
     reinterpret_cast<float4*>(a.out + ((size_t)row * a.n_q + head) * kA4Hd)[lane] = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
 }
 
@@ -565,6 +572,29 @@ static double a4_pick_split(long long items, int max_len, int most, double join,
         if (keys == 128) break;
     }
     return best;
+}
+
+// Splits, and who joins them, for CTAs of `hb` heads.
+static void a4_plan(A4Launch& L, int hb, size_t room) {
+    const tenzo_attention_kv4_args& a = L.a;
+    L.head_blocks = (L.group + hb - 1) / hb;
+    L.cluster = 0;
+    if (a.split_keys > 0) {
+        const long long keys = ((long long)a.split_keys + 127) / 128 * 128, all = ((long long)a.max_len + 127) / 128 * 128;
+        L.split_keys = (int)(keys < all ? keys : all);
+        L.n_splits = (a.max_len + L.split_keys - 1) / L.split_keys;
+        return;
+    }
+    const long long items = (long long)a.rows * a.cache.n_kv * L.head_blocks;
+    const double apart = a4_pick_split(items, a.max_len, room > 1 ? (int)(room < 64 ? room : 64) : 1, 300.0, &L.n_splits, &L.split_keys);
+    // Joined by clusters: 1 x 1000 keys 7.0 us and 9.2 by a second kernel, 12 x 8192 of 40/5 heads 36.3 and 38.1; but where CTAs come in several rounds
+    // a cluster waits for room for all of its own (256 x 4095 ragged: 218 and 174).
+    int splits, keys;
+    if (a4_pick_split(items, a.max_len, kA4Cluster, 100.0, &splits, &keys) < apart && splits > 1 && items * splits <= 148 * kA4Resident) {
+        L.n_splits = splits;
+        L.split_keys = keys;
+        L.cluster = 1;
+    }
 }
 
 template <int HB>
@@ -608,27 +638,16 @@ extern "C" int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, vo
     if (a.q_stride == 0) a.q_stride = a.n_q * kA4Hd;
     if (a.q_stride < a.n_q * kA4Hd) return -1;
     L.group = a.n_q / a.cache.n_kv;
-    const int hb = L.group <= 4 ? 4 : 8;
-    L.head_blocks = (L.group + hb - 1) / hb;
-    const long long items = (long long)a.rows * a.cache.n_kv * L.head_blocks;
-    if ((long long)a.cache.n_kv * L.head_blocks > 65535) return -1;
     const bool ws_ok = a.workspace && !(reinterpret_cast<uintptr_t>(a.workspace) & 15);
     const size_t room = ws_ok ? a.workspace_bytes / a4_part_bytes(a.rows, a.n_q) : 0;
-    if (a.split_keys > 0) {
-        L.split_keys = (int)(((long long)a.split_keys + 127) / 128 * 128 < a.max_len ? ((long long)a.split_keys + 127) / 128 * 128 : ((long long)a.max_len + 127) / 128 * 128);
-        L.n_splits = (a.max_len + L.split_keys - 1) / L.split_keys;
-        if (L.n_splits > 1 && room < (size_t)L.n_splits) return -1;
-    } else {
-        const double apart = a4_pick_split(items, a.max_len, room > 1 ? (int)(room < 64 ? room : 64) : 1, 300.0, &L.n_splits, &L.split_keys);
-        // Joined by clusters: 1 x 1000 keys 7.0 us and 9.2 by a second kernel, 12 x 8192 of 40/5 heads 36.3 and 38.1; but where CTAs come in several rounds
-        // a cluster waits for room for all of its own (256 x 4095 ragged: 218 and 174).
-        int splits, keys;
-        if (a4_pick_split(items, a.max_len, kA4Cluster, 100.0, &splits, &keys) < apart && splits > 1 && items * splits <= 148 * kA4Resident) {
-            L.n_splits = splits;
-            L.split_keys = keys;
-            L.cluster = 1;
-        }
-    }
+    // Heads a CTA takes: four, whose two parts of a weight share an MMA (64 x 8192 keys of 20/5 heads: 114 us, by eights 137); more than four heads a kv head by
+    // eights, so that fewer CTAs copy and unpack a key (64 x 4096 of 40/5: 86 us, by fours 118), unless by fours there are no more than two or three CTAs an
+    // SM, where an eight's longer way counts (1 x 1000 of 40/5: by fours 7.2 us, by eights 9.0; 4 x 1000: 9.4 and 10.2; but 16 x 1000: 16.9 and 15.0).
+    int hb = 4;
+    a4_plan(L, hb, room);
+    if (L.group > 4 && (long long)a.rows * a.cache.n_kv * L.head_blocks * L.n_splits > 148 * 5 / 2) a4_plan(L, hb = 8, room);
+    if (a.split_keys > 0 && L.n_splits > 1 && room < (size_t)L.n_splits) return -1;
+    if ((long long)a.cache.n_kv * L.head_blocks > 65535) return -1;
     if ((long long)a.rows * L.n_splits > 0x7fffffffLL) return -1;
     L.part_o = static_cast<float*>(a.workspace);
     L.part_ml = reinterpret_cast<float2*>(L.part_o + (size_t)a.rows * a.n_q * L.n_splits * kA4Hd);

@@ -274,6 +274,8 @@ def kv4_read(pool, pos, *, layer, block_table, seq=None, use_pdl=False, k=None, 
         kp = both.data_ptr()
         vp = kp + 4 * n * ks
         k, v = both.unbind(0)
+    elif k is None or v is None:
+        raise ValueError("k and v are given both or not at all")
     else:
         (kp, ks, m), (vp, vs, o) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
         if n != m or n != o or (ks != vs and n > 1):
@@ -320,9 +322,9 @@ def beam_select(logits, scores, *, beams, k, finished=None, eos=0, use_pdl=False
     fp32 [groups*beams]. Returns (parent, token, score), [groups, k], best first. finished int32 [groups*beams]: beams that only go on with `eos`."""
     dev, vocab = _current_device(), logits.shape[-1]
     lp, stride, rows = _arg_rows(logits, dev, vocab, "logits")
-    groups = rows // beams
-    if groups * beams != rows or scores.shape != (rows,):
-        raise ValueError(f"{rows} rows of logits are no groups of {beams} beams with one score each")
+    groups = rows // beams if beams > 0 else -1
+    if k < 1 or groups * beams != rows or scores.shape != (rows,):
+        raise ValueError(f"{rows} rows of logits are no groups of {beams} beams with one score each, or k = {k} is no number of candidates")
     device = logits.device
     parent, token, score = torch.empty(3, groups, k, dtype=torch.int32, device=device).unbind(0)
     score = score.view(torch.float32)

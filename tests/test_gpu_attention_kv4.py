@@ -221,6 +221,25 @@ def test_a_prompts_rows(cuda_lib, n_q, n_kv):
     check(out[some], q[some], pool, table, 0, pos[some], np.zeros(60, int), cos, sin)
 
 
+@pytest.mark.parametrize("n_q,n_kv,lens,split", [(4, 1, [90, 70], 0), (12, 2, [3000, 2500], 0), (8, 1, [900, 1000], 0), (8, 2, [700, 600], 128)])
+def test_a_query_that_is_not_finite(cuda_lib, n_q, n_kv, lens, split):
+    """NaN or infinity in one head of one row: NaN there, and the other heads' bits as before."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(n_q + split)
+    table, pool = setup(rng, lens, n_kv, (max(lens) + 15) // 16)
+    q = rng.standard_normal((2, n_q * 128)).astype(np.float32)
+    dp, dpos, dt = dev(pool), dev(np.array(lens, np.int32) - 1), dev(table)
+    call = lambda x: host(kernels.attention_kv4(dev(x), dp, dpos, layer=0, n_q=n_q, block_table=dt, split_keys=split)).reshape(2, n_q, 128)
+    want = call(q)
+    for bad in (np.nan, np.inf, -np.inf):
+        x = q.copy()
+        x[1, 2 * 128 + 17] = bad
+        got = call(x)
+        assert np.isnan(got[1, 2]).all()
+        got[1, 2] = want[1, 2]
+        assert np.array_equal(got, want)
+
+
 def test_two_at_once(cuda_lib):
     """Calls on two streams, joined by clusters, by a second kernel, and not at all; each with a workspace of its own."""
     from tenzo_b200 import kernels

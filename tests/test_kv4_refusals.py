@@ -137,3 +137,21 @@ def test_python_calls_refuse_tensors_of_the_host():
         with pytest.raises(Exception) as e:
             call()
         assert isinstance(e.value, (ValueError, RuntimeError))
+
+
+def test_python_calls_refuse_what_does_not_fit(monkeypatch):
+    monkeypatch.setattr(kernels, "_current_device", lambda: -1)              # where the host's tensors lie; nothing gets as far as a launch
+    pool, table, pos = torch.zeros(4, 1, 1, 2, 16, 80, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    rows, scores = torch.zeros(2, 128), torch.zeros(2)
+    for call in (lambda: kernels.kv4_read(pool, pos, layer=0, block_table=table, k=rows), lambda: kernels.kv4_read(pool, pos, layer=0, block_table=table, v=rows),
+                 lambda: kernels.kv4_read(pool, pos, layer=0, block_table=table, k=rows[:1], v=rows[:1]), lambda: kernels.kv4_append(rows, rows[:1], pool, pos, layer=0, block_table=table),
+                 lambda: kernels.kv4_append(rows, rows, pool, pos[:1], layer=0, block_table=table), lambda: kernels.kv4_append(rows.double(), rows, pool, pos, layer=0, block_table=table),
+                 lambda: kernels.kv4_append(rows, rows, pool.view(4, 1, 1, 2, 80, 16), pos, layer=0, block_table=table),
+                 lambda: kernels.attention_kv4(rows, pool, pos, layer=0, n_q=2, block_table=table), lambda: kernels.attention_kv4(rows, pool, pos.long(), layer=0, n_q=1, block_table=table),
+                 lambda: kernels.attention_kv4(rows, pool, pos, layer=0, n_q=1, block_table=table, rope_cos=torch.zeros(32, 64)),
+                 lambda: kernels.beam_select(rows, scores, beams=0, k=2), lambda: kernels.beam_select(rows, scores, beams=-1, k=2), lambda: kernels.beam_select(rows, scores, beams=2, k=0),
+                 lambda: kernels.beam_select(rows[:1], scores[:1], beams=2, k=2), lambda: kernels.beam_select(rows.half(), scores, beams=2, k=2),
+                 lambda: kernels.beam_select(rows, scores, beams=2, k=2, finished=pos[:1]), lambda: kernels.beam_select(rows.t(), scores, beams=2, k=2),
+                 lambda: kernels.kv4_reorder(pool, table, torch.zeros(1, 3, dtype=torch.int32), pos[:1]), lambda: kernels.kv4_reorder(pool, table, torch.zeros(1, 2, dtype=torch.int32), pos)):
+        with pytest.raises(ValueError):
+            call()
