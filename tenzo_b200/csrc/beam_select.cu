@@ -27,6 +27,7 @@ constexpr int kBsWindow = 8;                              // and up to so many t
 constexpr int kBsMostK = 2 * TENZO_BEAMS_MOST;
 constexpr int kBsMostPer = 32;                            // logits a thread holds at most
 constexpr int kBsList = (kBsMostK + kBsWindow) * kBsMostPer;      // candidates lie in that many threads' logits
+constexpr int kBsAhead = 148;                            // CTAs ahead whose logits are asked for into L2: one an SM
 constexpr int kBsMergeWarps = 16;                         // rows that the second kernel merges at a time
 constexpr int kBsHold = 1280;                             // entries of a row's lists that a warp keeps: 16 chunks of the most slots
 constexpr int kBsPicks = 96;                              // entries that are ranked; more than k + kBsWindow
@@ -104,6 +105,11 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
     if (out) return;
     if (tid == 0) {
         s_n = 0;
+        // Where CTAs come in waves, the logits of a later one on their way to L2 meanwhile (32 x 8 rows of 128256: 43.8 us without, 42.2 one CTA an SM ahead, 42.9 four)
+        if (VEC && !L.eager && blockIdx.x + kBsAhead < gridDim.x) {
+            const int r = (blockIdx.x + kBsAhead) / L.chunks, at = (blockIdx.x + kBsAhead) % L.chunks * kBsThreads * PER, n = min(a.vocab - at, kBsThreads * PER) & ~3;
+            if (n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.logits + (size_t)r * a.row_stride + at), "r"(4 * n) : "memory");
+        }
     }
     // ---- what counts: NaN as -infinity, infinity as the largest number; the largest of all ------------------------------------
     float top = -INFINITY;
