@@ -285,12 +285,15 @@ typedef struct {
     int max_len;             /* upper bound on pos + 1 (sizes the grid); at most 16 * table_stride */
     int split_keys;          /* keys a CTA takes (rounded up to 128); 0 = choose */
     int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
-    void* workspace;         /* 16-byte aligned, contents need not be kept: partial results of splits. tenzo_cuda_attention_kv4_workspace_bytes(...) */
-    size_t workspace_bytes;  /* bytes; with less (or NULL) fewer splits are taken (few rows need none), and split_keys that need more are refused (-1) */
+    void* workspace;         /* 16-byte aligned, contents need not be kept: partial results of splits; NULL: none */
+    size_t workspace_bytes;  /* rows * n_q * 520 a split; with less fewer splits are taken, and split_keys that need more are refused (-1). Enough for any split_keys:
+                                tenzo_cuda_attention_kv4_workspace_bytes(...); for split_keys 0: 520 * rows * n_q * tenzo_cuda_attention_kv4_splits(...), nothing at 1 */
 } tenzo_attention_kv4_args;
 TENZO_API int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, void* stream);
 TENZO_API size_t tenzo_cuda_attention_kv4_workspace_bytes(int rows, int n_q, int n_kv, int max_len);
-/* Error flags of the four calls above and below this one since the last call (bit 0: a bounded wait was given up, bit 1: an index out of range);
+/* Splits that the call's own choice (split_keys 0) wants room for; 1: none, 0: arguments that the call refuses. */
+TENZO_API int tenzo_cuda_attention_kv4_splits(int rows, int n_q, int n_kv, int max_len);
+/* Error flags of the calls above and below this one since the last call (bit 0: a bounded wait was given up, bit 1: an index out of range);
  * -1 if the query failed. Synchronises with the device. */
 TENZO_API int tenzo_cuda_kv4_take_errors(void);
 

@@ -112,7 +112,7 @@ KERNEL_SYMBOLS = [
     "tenzo_cuda_lm_head_static_max_batch", "tenzo_cuda_lm_head_take_timeouts", "tenzo_cuda_repetition_penalty",
     "tenzo_cuda_topk_candidates", "tenzo_cuda_topk_max_candidates",
     "tenzo_cuda_kv4_append", "tenzo_cuda_kv4_read", "tenzo_cuda_kv4_reorder", "tenzo_cuda_kv4_take_errors", "tenzo_cuda_attention_kv4",
-    "tenzo_cuda_attention_kv4_workspace_bytes", "tenzo_cuda_beam_select", "tenzo_cuda_beam_select_workspace_bytes",
+    "tenzo_cuda_attention_kv4_workspace_bytes", "tenzo_cuda_attention_kv4_splits", "tenzo_cuda_beam_select", "tenzo_cuda_beam_select_workspace_bytes",
 ]
 HAL_SYMBOLS = ["tenzo_hal_initialize", "tenzo_hal_bitlinear_tl1_host", "tenzo_hal_rmsnorm_host", "tenzo_hal_gemm_f32_host", "tenzo_hal_call_count"]
 
@@ -209,6 +209,7 @@ def declare_kernel_abi(L):
     L.tenzo_cuda_kv4_take_errors.restype, L.tenzo_cuda_kv4_take_errors.argtypes = i32, []
     L.tenzo_cuda_attention_kv4.restype, L.tenzo_cuda_attention_kv4.argtypes = i32, [C.POINTER(AttentionKv4Args), vp]
     L.tenzo_cuda_attention_kv4_workspace_bytes.restype, L.tenzo_cuda_attention_kv4_workspace_bytes.argtypes = sz, [i32, i32, i32, i32]
+    L.tenzo_cuda_attention_kv4_splits.restype, L.tenzo_cuda_attention_kv4_splits.argtypes = i32, [i32, i32, i32, i32]
     L.tenzo_cuda_beam_select.restype, L.tenzo_cuda_beam_select.argtypes = i32, [C.POINTER(BeamSelectArgs), vp]
     L.tenzo_cuda_beam_select_workspace_bytes.restype, L.tenzo_cuda_beam_select_workspace_bytes.argtypes = sz, [i32, i32, i32, i32]
     L.tenzo_cuda_lm_head_scratch_bytes.restype, L.tenzo_cuda_lm_head_scratch_bytes.argtypes = sz, [i32]

@@ -36,6 +36,7 @@ constexpr int kA4Step = 32;                              // keys a warp takes at
 constexpr int kA4Stages = 2, kA4StepBytes = 2 * kK4Page;
 constexpr int kA4Resident = 4;                           // CTAs an SM
 constexpr int kA4Cluster = 8;                            // splits that a cluster may take
+constexpr int kA4MostSplits = 64;                        // and a choice of its own, at most
 
 __device__ int g_kv4_attention_error = 0;
 
@@ -586,7 +587,7 @@ static void a4_plan(A4Launch& L, int hb, size_t room) {
         return;
     }
     const long long items = (long long)a.rows * a.cache.n_kv * L.head_blocks;
-    const double apart = a4_pick_split(items, a.max_len, room > 1 ? (int)(room < 64 ? room : 64) : 1, 300.0, &L.n_splits, &L.split_keys);
+    const double apart = a4_pick_split(items, a.max_len, room > 1 ? (int)(room < kA4MostSplits ? room : kA4MostSplits) : 1, 300.0, &L.n_splits, &L.split_keys);
     // Joined by clusters: 1 x 1000 keys 7.0 us and 9.2 by a second kernel, 12 x 8192 of 40/5 heads 36.3 and 38.1; but where CTAs come in several rounds
     // a cluster waits for room for all of its own (256 x 4095 ragged: 218 and 174).
     int splits, keys;
@@ -620,6 +621,20 @@ extern "C" size_t tenzo_cuda_attention_kv4_workspace_bytes(int rows, int n_q, in
     if (rows <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_len <= 0) return 0;
     const size_t splits = ((size_t)max_len + 127) / 128;     // the finest split that may be asked for
     return tz::a4_part_bytes(rows, n_q) * splits;
+}
+
+extern "C" int tenzo_cuda_attention_kv4_splits(int rows, int n_q, int n_kv, int max_len) {
+    using namespace tz;
+    if (rows <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_len <= 0 || max_len > 1 << 30) return 0;
+    A4Launch L = {};
+    L.a.rows = rows; L.a.n_q = n_q; L.a.cache.n_kv = n_kv; L.a.max_len = max_len;
+    L.group = n_q / n_kv;
+    int splits = 1;                                      // of the two plans that the call compares
+    for (int hb = 4; hb <= (L.group > 4 ? 8 : 4); hb += 4) {
+        a4_plan(L, hb, kA4MostSplits);
+        if (!L.cluster && L.n_splits > splits) splits = L.n_splits;
+    }
+    return splits;
 }
 
 extern "C" int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, void* stream) {

@@ -184,7 +184,7 @@ _PI, _PP, _PB = C.c_int, C.c_void_p, C.c_char_p
 @functools.cache
 def _beam_calls():
     """The entry points with prototypes of this module's own, whose structs are the bytes of a struct.Struct; tenzo_cuda_kv4_append, _read, _reorder,
-    tenzo_cuda_attention_kv4, tenzo_cuda_beam_select, and the two workspace sizes."""
+    tenzo_cuda_attention_kv4, tenzo_cuda_beam_select, the two workspace sizes, and the attention's choice of splits."""
     def fn(name, *argtypes, restype=C.c_int):
         f = load_library()[name]
         f.restype, f.argtypes = restype, list(argtypes)
@@ -194,7 +194,7 @@ def _beam_calls():
             fn("tenzo_cuda_kv4_reorder", _PB, _PP, _PP, _PP, _PI, _PI, _PI, _PP),
             fn("tenzo_cuda_attention_kv4", _PB, _PP), fn("tenzo_cuda_beam_select", _PB, _PP),
             fn("tenzo_cuda_attention_kv4_workspace_bytes", _PI, _PI, _PI, _PI, restype=C.c_size_t),
-            fn("tenzo_cuda_beam_select_workspace_bytes", _PI, _PI, _PI, _PI, restype=C.c_size_t))
+            fn("tenzo_cuda_beam_select_workspace_bytes", _PI, _PI, _PI, _PI, restype=C.c_size_t), fn("tenzo_cuda_attention_kv4_splits", _PI, _PI, _PI, _PI))
 
 
 # (These calls take as long as their kernels at small sizes: attributes of a tensor are read once, 0.05 us each, and the stream's handle comes from
@@ -286,7 +286,15 @@ def kv4_read(pool, pos, *, layer, block_table, seq=None, use_pdl=False, k=None, 
 
 @functools.lru_cache(1024)
 def attention_kv4_workspace_bytes(rows, n_q, n_kv, max_len) -> int:
+    """Enough for any split_keys."""
     return _beam_calls()[5](rows, n_q, n_kv, max_len)
+
+
+@functools.lru_cache(1024)
+def _attention_kv4_room(rows, n_q, n_kv, max_len, split_keys) -> int:
+    """What one call needs: splits of split_keys keys, or as many as it chooses itself."""
+    splits = -(-max_len // (-(-split_keys // 128) * 128)) if split_keys > 0 else _beam_calls()[7](rows, n_q, n_kv, max_len)
+    return rows * n_q * 520 * splits if splits > 1 else 0
 
 
 @functools.lru_cache(1024)
@@ -297,7 +305,8 @@ def beam_select_workspace_bytes(groups, beams, vocab, k) -> int:
 def attention_kv4(q, pool, pos, *, layer, n_q, block_table, seq=None, rope_cos=None, rope_sin=None, max_len=None, split_keys=0, use_pdl=False, out=None,
                   workspace=None):
     """GQA attention of the query rows q [rows, n_q*128] over the keys 0 .. pos[row] of their sequences in the 4-bit pool, the queries rotated first.
-    Returns out [rows, n_q*128]; zeros where pos is negative. max_len: an upper bound on pos + 1 (default: what the table has room for)."""
+    Returns out [rows, n_q*128]; zeros where pos is negative. max_len: an upper bound on pos + 1 (default: what the table has room for).
+    workspace: a uint8 tensor for partial results of splits (default: one is allocated if the call wants it)."""
     dev = _current_device()
     cache, n_kv, _, columns = _kv4_cache(pool, block_table, dev)
     qp, q_stride, rows = _arg_rows(q, dev, n_q * 128, "q")
@@ -308,8 +317,10 @@ def attention_kv4(q, pool, pos, *, layer, n_q, block_table, seq=None, rope_cos=N
         out = torch.empty(rows, n_q * 128, dtype=torch.float32, device=q.device)
     elif out.shape != (rows, n_q * 128):
         raise ValueError(f"out is [{rows}, {n_q * 128}]")
-    if workspace is None and (split_keys or max_len > 1024):       # (up to 1024 keys the call does as well without)
-        workspace = torch.empty(attention_kv4_workspace_bytes(rows, n_q, n_kv, max_len), dtype=torch.uint8, device=q.device)
+    if workspace is None:
+        size = _attention_kv4_room(rows, n_q, n_kv, max_len, split_keys)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
     args = _KV4_ATTENTION.pack(qp, _arg(out, torch.float32, dev, "out"), *_KV4_CACHE.unpack(cache), _arg_entries(pos, rows, dev, "pos"), _arg_entries(seq, rows, dev, "seq"),
                                cos, sin, length, q_stride, layer, n_q, rows, max_len, split_keys, use_pdl, _arg(workspace, torch.uint8, dev, "workspace"),
                                0 if workspace is None else workspace.numel())

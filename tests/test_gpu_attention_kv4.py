@@ -240,6 +240,19 @@ def test_a_query_that_is_not_finite(cuda_lib, n_q, n_kv, lens, split):
         assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("n_q,n_kv,lens", [(20, 5, [4000]), (40, 5, [6000, 5000]), (16, 1, [3000] * 9), (8, 2, [1500] * 40)])
+def test_room_for_the_chosen_splits_is_enough(cuda_lib, n_q, n_kv, lens):
+    """The workspace that a call takes by itself gives the same splits, and bits, as one with room for any."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(n_q)
+    table, pool = setup(rng, lens, n_kv, (max(lens) + 15) // 16, garbage=False)
+    q, dp, dpos, dt = dev(rng.standard_normal((len(lens), n_q * 128)).astype(np.float32)), dev(pool), dev(np.array(lens, np.int32) - 1), dev(table)
+    ws = torch.empty(kernels.attention_kv4_workspace_bytes(len(lens), n_q, n_kv, max(lens)), dtype=torch.uint8, device="cuda")
+    call = lambda **kw: kernels.attention_kv4(q, dp, dpos, layer=0, n_q=n_q, block_table=dt, max_len=max(lens), **kw)
+    assert torch.equal(call(), call(workspace=ws))
+    assert kernels.kv4_take_errors() == 0
+
+
 def test_two_at_once(cuda_lib):
     """Calls on two streams, joined by clusters, by a second kernel, and not at all; each with a workspace of its own."""
     from tenzo_b200 import kernels

@@ -73,6 +73,17 @@ def test_attention_null_and_sizes(lib):
     assert need(64, 20, 5, 8192) < need(128, 20, 5, 8192) and need(1, 4, 2, 1) > 0
 
 
+def test_attention_room_for_the_chosen_splits(lib):
+    splits = lib.tenzo_cuda_attention_kv4_splits
+    assert splits(0, 4, 2, 10) == splits(1, 0, 2, 10) == splits(1, 4, 0, 10) == splits(1, 5, 2, 10) == splits(1, 4, 2, 0) == splits(1, 4, 2, (1 << 30) + 1) == 0
+    assert splits(1, 20, 5, 100) == splits(1, 20, 5, 1000) == 1 and splits(1, 20, 5, 16384) > 8             # no room for one split, nor for a cluster's
+    for rows, n_q, n_kv, n in ((1, 40, 5, 16384), (64, 20, 5, 8192), (256, 20, 5, 131072), (3, 7, 1, 1 << 30), (100000, 32, 32, 4096)):
+        most = splits(rows, n_q, n_kv, n)
+        assert 1 <= most <= 64 and most * rows * n_q * 520 <= max(lib.tenzo_cuda_attention_kv4_workspace_bytes(rows, n_q, n_kv, n), rows * n_q * 520)
+        assert kernels._attention_kv4_room(rows, n_q, n_kv, n, 0) == (most * rows * n_q * 520 if most > 1 else 0)
+    assert kernels._attention_kv4_room(2, 4, 2, 1000, 128) == 8 * 2 * 4 * 520 and kernels._attention_kv4_room(2, 4, 2, 1000, 900) == 0       # 900: rounded up to 1024
+
+
 @pytest.mark.parametrize("change,code", [(dict(out=None), -1), (dict(out=P), -1), (dict(parent=None), -1), (dict(length=None), -1), (dict(groups=0), -1), (dict(groups=-2), -1),
                                          (dict(groups=3), -1), (dict(beams=0), -5), (dict(beams=33), -5), (dict(layers=10000), -5)], ids=str)
 def test_reorder(lib, change, code):
