@@ -253,6 +253,50 @@ def test_room_for_the_chosen_splits_is_enough(cuda_lib, n_q, n_kv, lens):
     assert kernels.kv4_take_errors() == 0
 
 
+@pytest.mark.parametrize("n_q,n_kv", [(5, 5), (8, 4), (9, 3), (20, 5), (2, 2)])
+@pytest.mark.parametrize("split", [0, 128])
+def test_rows_that_share_a_sequence(cuda_lib, n_q, n_kv, split):
+    """Many rows, in runs of one to twenty of the same sequence, at any positions; padding, and indices out of range, between them."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(n_q * 10 + n_kv)
+    lens = [int(n) for n in rng.integers(1, 600, 40)] + [1, 16, 33]
+    table, pool = setup(rng, lens, n_kv, 38, layers=2)
+    seq = np.concatenate([np.full(rng.integers(1, 21) if rng.random() < 0.5 else 1, s) for s in rng.permutation(len(lens))]).astype(np.int32)
+    pos = np.array([rng.integers(max(0, lens[s] - 8), lens[s]) if rng.random() < 0.7 else rng.integers(0, lens[s]) for s in seq], np.int32)
+    pos[rng.random(len(pos)) < 0.1] = -1
+    refused = rng.choice(len(pos), 8, replace=False)
+    q = rng.standard_normal((len(seq), n_q * 128)).astype(np.float32) * 2
+    cos, sin = ref.rope(608)
+    g = Guarded()
+    out = g.empty((len(seq), n_q * 128), torch.float32)
+    for bad in (False, True):
+        if bad:
+            pos[refused[:4]], seq[refused[4:]] = [608, 609, 1 << 30, 700], [-1, len(lens), 1 << 30, -5]
+        out.fill_(7.0)
+        kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=1, n_q=n_q, block_table=dev(table), seq=dev(seq), rope_cos=dev(cos), rope_sin=dev(sin), out=out, split_keys=split)
+        left = np.setdiff1d(np.arange(len(seq)), refused) if bad else np.arange(len(seq))
+        check(host(out)[left], q[left], pool, table, 1, pos[left], seq[left], cos, sin)
+        if bad:
+            assert (host(out)[refused] == 7.0).all()
+        g.check()
+        assert kernels.kv4_take_errors() == (2 if bad else 0)
+
+
+def test_long_rows_that_share_a_sequence(cuda_lib):
+    """Drafts of five rows over long contexts: splits joined by clusters and by a second kernel, and keys that only the later rows see."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(77)
+    for n_q, n_kv, lens in ((20, 5, [6000, 4096]), (16, 4, [1029, 1024, 900, 1027]), (8, 8, [3000, 2500, 2049])):
+        table, pool = setup(rng, lens, n_kv, (max(lens) + 15) // 16)
+        seq = np.arange(len(lens), dtype=np.int32).repeat(5)
+        pos = np.concatenate([n - 5 + rng.permutation(5) for n in lens]).astype(np.int32)
+        q = rng.standard_normal((len(seq), n_q * 128)).astype(np.float32)
+        for split in (0, 128, 256):
+            out = kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=n_q, block_table=dev(table), seq=dev(seq), split_keys=split, use_pdl=True)
+            check(host(out), q, pool, table, 0, pos, seq)
+    assert kernels.kv4_take_errors() == 0
+
+
 def test_two_at_once(cuda_lib):
     """Calls on two streams, joined by clusters, by a second kernel, and not at all; each with a workspace of its own."""
     from tenzo_b200 import kernels
