@@ -6,14 +6,16 @@
 //   1. A CTA takes a chunk of a row, each thread up to 32 logits in registers, read once. The k-th largest of the 256 threads' maxima is a
 //      lower bound of the chunk's k-th largest logit, and hardly more logits reach it: those are listed, and their exponentials are taken and summed
 //      in 64 bits. All others' (16 larger ones at least are on the list) are taken in 32, by the hardware's 2^x, and summed in 32 within a thread:
-//      nothing is lost where a few tokens have the weight, and where thousands share it the errors hardly add up: the logarithm of the whole was off by 3e-8
-//      at most in some ten thousand random rows, 9e-8 with logits that repeat, and cannot be by more than 2e-6. (An own 2^x good to 1e-8 costs
-//      thirteen instructions a logit where there are four now.)
+//      nothing is lost where a few tokens have the weight, and where thousands share it the errors hardly add up: the logarithm of the whole was off by some 1e-8
+//      in random rows, by up to 1e-7 with logits that repeat, and cannot be by more than 2e-6. (An own 2^x good to 1e-8 costs thirteen instructions a logit
+//      where there are two now.)
 //   2. A CTA a group, a warp a row: the k best of the lists, with their scores; then the rows' scores that reach a common border are ranked
 //      among one another.
 // Sums are taken in an order that the data alone decides, or as integers, so that equal rows get equal sums and tie.
 //
-// The first kernel reads 4 bytes a logit; what bounds it besides is some ten instructions and an ex2 (8 cycles of its unit a warp) for each.
+// 32 x 8 rows of 128256, k 16: 40.5 us. Loads alone take the first kernel 21 (131 MB at 6.2 TB/s), with everything else in it 32: some eight instructions and an ex2 a
+// logit, and the barriers around the bisection, are hidden by the other CTAs' loads for two thirds only. The second kernel is 9, a chain of a few thousand instructions
+// that run once.
 #include "common.cuh"
 #include "kv4.cuh"
 
@@ -33,6 +35,7 @@ constexpr int kBsHold = 1280;                             // entries of a row's 
 constexpr int kBsPicks = 96;                              // entries that are ranked; more than k + kBsWindow
 
 constexpr double kBsUnit = 281474976710656.0;             // 2^48
+constexpr float kLog2E = 1.4426950408889634f;
 
 typedef unsigned long long u64;
 
@@ -66,7 +69,7 @@ template <bool VEC, int PER>
 __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaunch L) {
     __shared__ uint32_t s_keys[kBsThreads];
     __shared__ u64 s_list[kBsList], s_sorted[kBsList];
-    __shared__ double s_sum[kBsWarps];
+    __shared__ double s_sum[kBsWarps], s_unit;
     __shared__ u64 s_listed[kBsWarps];
     __shared__ float s_red[kBsWarps];
     __shared__ uint32_t s_bound;
@@ -84,7 +87,14 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
     auto place = [&](int j) { return base + (VEC ? 4 * (tid + kBsThreads * (j >> 2)) + (j & 3) : tid + kBsThreads * j); };
     static_assert(PER <= 32, "one bit each");
     float v[PER];                                         // -infinity where there is nothing
-    if (VEC) {
+    if (VEC && base + kBsThreads * PER <= a.vocab) {
+        const float4* from = reinterpret_cast<const float4*>(x + base) + tid;
+#pragma unroll
+        for (int j = 0; j < PER; j += 4) {
+            const float4 f = ld_l2(from + kBsThreads * (j >> 2));
+            v[j] = f.x; v[j + 1] = f.y; v[j + 2] = f.z; v[j + 3] = f.w;
+        }
+    } else if (VEC) {
 #pragma unroll
         for (int j = 0; j < PER; j += 4) {
             float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -111,17 +121,14 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
             if (n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.logits + (size_t)r * a.row_stride + at), "r"(4 * n) : "memory");
         }
     }
-    // ---- what counts: NaN as -infinity, infinity as the largest number; the largest of all ------------------------------------
+    // ---- what counts: NaN as -infinity (below), infinity as the largest number; the largest of all ------------------------------
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        v[j] = fmaxf(v[j], -INFINITY);                    // (drops NaN)
-        top = fmaxf(top, v[j]);
-    }
+    for (int j = 0; j < PER; ++j) top = fmaxf(top, v[j]); // (drops NaN)
     if (top == INFINITY) {
         top = FLT_MAX;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = fminf(v[j], FLT_MAX);
+        for (int j = 0; j < PER; ++j) v[j] = fminf(fmaxf(v[j], -INFINITY), FLT_MAX);
     }
     s_keys[tid] = place(0) < a.vocab ? beam_key(top) : 0u;
     float most = warp_max(top);
@@ -187,22 +194,40 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
     }
     const int last = s_last;
     // ---- the others' exponentials, and the list of candidates -------------------------------------------------------------------
-    const float from = most == -INFINITY ? 0.0f : most;
+    // 2^(v log2(e) - shift) with one rounding: `shift` is most * log2(e), rounded, and what that rounding does to all of them alike is put right in the end. (log2(e) in
+    // 24 bits is 1.3e-8 off.) A shift near the end of the range, which masked rows have, would not be finite: there the difference comes first.
+    const float from = most == -INFINITY ? 0.0f : most, shift = -from * kLog2E;
+    const bool far = !(fabsf(from) < 1e37f);
+    auto power = [&](float c, bool difference_first) {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(difference_first ? (c - from) * kLog2E : __fmaf_rn(c, kLog2E, shift)));
+        return e;
+    };
     float rest = 0.0f;
     uint32_t reach_it = 0;                                // one bit a logit
+    if (!far) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const float d = v[j] - from;                      // times log2(e), whose second part is 1.9e-8
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmaf_rn(d, 1.4426950216293335f, d * 1.9259629911e-8f)));
-        if (v[j] >= bound) reach_it |= 1u << j; else rest += e;
+        for (int j = 0; j < PER; ++j) {
+            const float e = power(v[j], false);
+            if (v[j] >= bound) reach_it |= 1u << j; else rest += e;
+        }
+    }
+    if (far || rest != rest) {                            // a NaN among them
+        rest = 0.0f;
+        reach_it = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            v[j] = fmaxf(v[j], -INFINITY);
+            const float e = power(v[j], far);
+            if (v[j] >= bound) reach_it |= 1u << j; else rest += e;
+        }
     }
     for (const bool one = (reach_it & (reach_it - 1u)) == 0u; reach_it; reach_it &= reach_it - 1u) {
         const int i = place(__ffs((int)reach_it) - 1);
         if (i >= a.vocab) continue;
         const float c = one ? top : fminf(fmaxf(ld_l2(x + i), -INFINITY), FLT_MAX);      // (read again: a register's number is no variable)
         if (c == bound && i > last) {
-            rest += from == bound ? 1.0f : exp2f((c - from) * 1.4426950408889634f);
+            rest += power(c, far);
         } else {
             const int at = atomicAdd(&s_n, 1);
             if (at < kBsList) s_list[at] = beam_entry(beam_key(c), i);
@@ -225,6 +250,7 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
         for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         if (lane == 0) s_listed[warp] = mine;
     }
+    if (tid == kBsThreads - 1) s_unit = far ? 1.0 : exp2(-((double)from * (double)kLog2E + (double)shift));      // (the product is exact)
     if (n > L.slots) {                                    // (many large ones in few threads) the best k go on
         for (int i = tid; i < n; i += kBsThreads) {
             const u64 e = s_list[i];
@@ -242,9 +268,10 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
         BeamPart p;
         u64 listed = 0;
         for (int w = 0; w < kBsWarps && 32 * w < listed_n; ++w) listed += s_listed[w];
-        p.sum = (double)listed * (1.0 / kBsUnit);
+        double others = 0.0;
 #pragma unroll
-        for (int w = 0; w < kBsWarps; ++w) p.sum += s_sum[w];
+        for (int w = 0; w < kBsWarps; ++w) others += s_sum[w];
+        p.sum = (double)listed * (1.0 / kBsUnit) + others * s_unit;
         p.most = most;
         L.parts[(size_t)row * L.chunks + chunk] = p;
     }

@@ -22,9 +22,9 @@ def check(logits, scores, beams, k, finished=None, eos=0, logits_dev=None):
     both = np.isfinite(want_score)
     assert np.array_equal(both, np.isfinite(score)) and np.array_equal(score[~both], want_score[~both].astype(np.float32))
     # Rounded once to fp32 (2^-24), and the logarithm of the sum is good to 2^-19: an exponential that is taken in 32 bits counts where the logit is
-    # d <= ln(vocab) < 12 below the largest (those further off have no weight), so that d is rounded by 2^-21 at most (half a step between 8 and 16), its
-    # product with log2(e), below 18, by 2^-20 or 0.7 2^-20 of the exponential, and the hardware's 2^x by 2^-22. All that is 1.5 2^-20 if all logits went the
-    # same way, and half of it is the largest's weight at d = 12; below d = 8 it is 0.85 2^-20. A thread's sum of 32 is rounded 31 times by 2^-24
+    # d <= ln(vocab) < 12 below the largest (those further off have no weight), so that its exponent d log2(e), below 18, is rounded by 2^-20 or 0.7 2^-20 of the
+    # exponential, log2(e) in 24 bits is off by 1.4e-8 d or 0.2 2^-20, and the hardware's 2^x by 2^-22. All that is 1.2 2^-20 if all logits went the same
+    # way, and half of it is the largest's weight at d = 12; below d = 8 it is 0.8 2^-20. A thread's sum of 32 is rounded 31 times by 2^-24
     # of what has come together, half the sum on average: 1 2^-20 at most.
     assert (abs(score[both] - want_score[both]) <= 2.0 ** -24 * abs(want_score[both]) + 2.0 ** -19).all()
     return parent, token, score
