@@ -13,8 +13,8 @@
 //      among one another.
 // Sums are taken in an order that the data alone decides, or as integers, so that equal rows get equal sums and tie.
 //
-// 32 x 8 rows of 128256, k 16: 40.5 us. Loads alone take the first kernel 21 (131 MB at 6.2 TB/s), with everything else in it 32: some eight instructions and an ex2 a
-// logit, and the barriers around the bisection, are hidden by the other CTAs' loads for two thirds only. The second kernel is 9, a chain of a few thousand instructions
+// 32 x 8 rows of 128256, k 16: 38.7 us. Loads alone take the first kernel 21 (131 MB at 6.2 TB/s), with everything else in it 32: some eight instructions and an ex2 a
+// logit, and the barriers around the bisection, are hidden by the other CTAs' loads for two thirds only. The second kernel is 7, a chain of a few thousand instructions
 // that run once.
 #include "common.cuh"
 #include "kv4.cuh"
@@ -301,7 +301,6 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
     BeamGroup& G = *reinterpret_cast<BeamGroup*>(bs_smem);
     const tenzo_beam_select_args& a = L.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, k = a.k;
-    const unsigned below = (1u << lane) - 1u;
     u64* room = reinterpret_cast<u64*>(bs_smem + (sizeof(BeamGroup) + 15) / 16 * 16) + (size_t)warp * hold;
     pdl_launch_dependents();
     pdl_wait();
@@ -321,14 +320,19 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
         }
         // the row's entries, and each lane's two largest logits (of a row that was left out they mean nothing)
         uint32_t one = 0, two = 0;
-#pragma unroll 8
-        for (int i = lane; i < n / 2; i += 32) {
-            const uint4 e = ld_l2(reinterpret_cast<const uint4*>(list) + i);                       // two entries: token, logit, token, logit
-            if (hold) reinterpret_cast<uint4*>(room)[i] = e;
-            two = max(two, min(one, e.y));
-            one = max(one, e.y);
-            two = max(two, min(one, e.w));
-            one = max(one, e.w);
+#pragma unroll 1
+        for (int i0 = lane; i0 < n / 2; i0 += 8 * 32) {
+            uint4 e[8];                                   // two entries each: token, logit, token, logit
+#pragma unroll
+            for (int u = 0; u < 8; ++u) e[u] = i0 + 32 * u < n / 2 ? ld_l2(reinterpret_cast<const uint4*>(list) + i0 + 32 * u) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                if (hold && i0 + 32 * u < n / 2) reinterpret_cast<uint4*>(room)[i0 + 32 * u] = e[u];
+                two = max(two, min(one, e[u].y));
+                one = max(one, e[u].y);
+                two = max(two, min(one, e[u].w));
+                one = max(one, e[u].w);
+            }
         }
         const u64* entry = hold ? room : list;
         float most = -INFINITY;
@@ -382,20 +386,29 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
         int m;
 #pragma unroll 1
         for (;;) {
-            m = 0;
-#pragma unroll 2
-            for (int i0 = 0; i0 < n; i0 += 64) {          // two entries a lane
-                const int i = i0 + 2 * lane;
-                const ulonglong2 e = i < n ? *reinterpret_cast<const ulonglong2*>(entry + i) : make_ulonglong2(0, 0);
-                const unsigned in0 = __ballot_sync(0xffffffffu, e.x >= lo), in1 = __ballot_sync(0xffffffffu, e.y >= lo);
-                if (in0 | in1) {
-                    const int at0 = m + __popc(in0 & below), at1 = m + __popc(in0) + __popc(in1 & below);
-                    if (e.x >= lo && at0 < kBsPicks) G.pick[warp][at0] = e.x;
-                    if (e.y >= lo && at1 < kBsPicks) G.pick[warp][at1] = e.y;
-                    m += __popc(in0) + __popc(in1);
-                }
+            int mine = 0;                                 // counted, and placed behind those of the lanes below
+#pragma unroll 4
+            for (int i = 2 * lane; i < n; i += 64) {      // two entries a load
+                const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(entry + i);
+                mine += (e.x >= lo) + (e.y >= lo);
             }
-            if (m <= kBsPicks) break;
+            int at = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, at, o);
+                if (lane >= o) at += other;
+            }
+            m = __shfl_sync(0xffffffffu, at, 31);
+            at -= mine;
+            if (m <= kBsPicks) {
+#pragma unroll 4
+                for (int i = 2 * lane; i < n; i += 64) {
+                    const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(entry + i);
+                    if (e.x >= lo) G.pick[warp][at++] = e.x;
+                    if (e.y >= lo) G.pick[warp][at++] = e.y;
+                }
+                break;
+            }
 #pragma unroll 1
             for (int reach = m; reach > kBsPicks && hi - lo > 1;) {
                 const u64 mid = lo + (hi - lo) / 2;
@@ -424,21 +437,17 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
     }
     __syncthreads();
     // ---- a score that k entries reach: the worst of the rows' ceil(k / beams)-th, or the best of their k-th. What lies below is out. ----
-    u64 worst = ~0ull, best = 0, first = 0;
+    uint32_t worst = 0xffffffffu, best = 0, first = 0;    // (upper halves of the keys are enough)
     if (lane < a.beams) {
         const int each = (k + a.beams - 1) / a.beams, n = G.count[lane];
-        worst = n >= each ? G.score[lane][each - 1] : 0;
-        first = n ? G.score[lane][0] : 0;
-        if (n >= k) best = G.score[lane][k - 1];
+        worst = n >= each ? (uint32_t)(G.score[lane][each - 1] >> 32) : 0;
+        first = n ? (uint32_t)(G.score[lane][0] >> 32) : 0;
+        if (n >= k) best = (uint32_t)(G.score[lane][k - 1] >> 32);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 w = __shfl_xor_sync(0xffffffffu, worst, o), h = __shfl_xor_sync(0xffffffffu, best, o), f = __shfl_xor_sync(0xffffffffu, first, o);
-        worst = w < worst ? w : worst;
-        best = h > best ? h : best;
-        first = f > first ? f : first;
-    }
-    u64 border = worst > best ? worst : best, high = first + 1;
+    worst = __reduce_min_sync(0xffffffffu, worst);
+    best = __reduce_max_sync(0xffffffffu, best);
+    first = __reduce_max_sync(0xffffffffu, first);
+    u64 border = (u64)max(worst, best) << 32, high = ((u64)first + 1) << 32;
     // ... and closer to the k-th, by bisection over all (a place of the rows' lists a thread).
     auto place = [&](int i) { return i < a.beams * kBsMostK && i % kBsMostK < G.count[i / kBsMostK] ? G.score[i / kBsMostK][i % kBsMostK] : 0ull; };
     auto reaching = [&](u64 x) {
