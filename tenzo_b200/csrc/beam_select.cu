@@ -13,7 +13,7 @@
 //      among one another.
 // Sums are taken in an order that the data alone decides, or as integers, so that equal rows get equal sums and tie.
 //
-// 32 x 8 rows of 128256, k 16: 38.7 us. Loads alone take the first kernel 21 (131 MB at 6.2 TB/s), with everything else in it 32: some eight instructions and an ex2 a
+// 32 x 8 rows of 128256, k 16: 36.3 us. Loads alone take the first kernel 21 (131 MB at 6.2 TB/s), with everything else in it 29: some eight instructions and an ex2 a
 // logit, and the barriers around the bisection, are hidden by the other CTAs' loads for two thirds only. The second kernel is 7, a chain of a few thousand instructions
 // that run once.
 #include "common.cuh"
@@ -35,6 +35,7 @@ constexpr int kBsHold = 1280;                             // entries of a row's 
 constexpr int kBsPicks = 96;                              // entries that are ranked; more than k + kBsWindow
 
 constexpr double kBsUnit = 281474976710656.0;             // 2^48
+constexpr double kBsUnitOthers = 35184372088832.0;        // 2^45
 constexpr float kLog2E = 1.4426950408889634f;
 
 typedef unsigned long long u64;
@@ -68,9 +69,8 @@ __device__ __forceinline__ bool beam_finished(const tenzo_beam_select_args& a, i
 template <bool VEC, int PER>
 __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaunch L) {
     __shared__ uint32_t s_keys[kBsThreads];
-    __shared__ u64 s_list[kBsList], s_sorted[kBsList];
-    __shared__ double s_sum[kBsWarps], s_unit;
-    __shared__ u64 s_listed[kBsWarps];
+    __shared__ u64 s_list[kBsList], s_sum[kBsWarps], s_listed[kBsWarps];
+    __shared__ double s_unit;
     __shared__ float s_red[kBsWarps];
     __shared__ uint32_t s_bound;
     __shared__ int s_short, s_last, s_n;
@@ -195,9 +195,9 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
     const int last = s_last;
     // ---- the others' exponentials, and the list of candidates -------------------------------------------------------------------
     // 2^(v log2(e) - shift) with one rounding: `shift` is most * log2(e), rounded, and what that rounding does to all of them alike is put right in the end. (log2(e) in
-    // 24 bits is 1.3e-8 off.) A shift near the end of the range, which masked rows have, would not be finite: there the difference comes first.
+    // 24 bits is 1.3e-8 off.) That rounding is 2^-9 at most up to 32768; beyond, and where masked rows have the lowest number of all, the difference comes first.
     const float from = most == -INFINITY ? 0.0f : most, shift = -from * kLog2E;
-    const bool far = !(fabsf(from) < 1e37f);
+    const bool far = !(fabsf(from) < 32768.0f);
     auto power = [&](float c, bool difference_first) {
         float e;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(difference_first ? (c - from) * kLog2E : __fmaf_rn(c, kLog2E, shift)));
@@ -225,7 +225,12 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
     for (const bool one = (reach_it & (reach_it - 1u)) == 0u; reach_it; reach_it &= reach_it - 1u) {
         const int i = place(__ffs((int)reach_it) - 1);
         if (i >= a.vocab) continue;
-        const float c = one ? top : fminf(fmaxf(ld_l2(x + i), -INFINITY), FLT_MAX);      // (read again: a register's number is no variable)
+        float c = top;
+        if (!one) {                                       // (a register's number is no variable)
+            const int at = __ffs((int)reach_it) - 1;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) c = j == at ? v[j] : c;
+        }
         if (c == bound && i > last) {
             rest += power(c, far);
         } else {
@@ -233,45 +238,53 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
             if (at < kBsList) s_list[at] = beam_entry(beam_key(c), i);
         }
     }
-    double sum = (double)rest;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_sum[warp] = sum;
+    // Sums as whole numbers: up to 32 a thread, in units of 2^-21 and 2^-45, add up in two instructions a warp.
+    const float units = rest * 2097152.0f, whole = floorf(units);
+    const unsigned high = __reduce_add_sync(0xffffffffu, (unsigned)whole), low = __reduce_add_sync(0xffffffffu, (unsigned)((units - whole) * 16777216.0f));
+    if (lane == 0) s_sum[warp] = ((u64)high << 24) + low;
     __syncthreads();
-    const int listed_n = min(s_n, kBsList);
-    int n = listed_n;
-    const u64* list = s_list;
-    if (32 * warp < n) {                                  // the listed ones' exponentials, in units of 2^-48: whole numbers add up the same in any order
-        u64 mine = 0;
-#pragma unroll 1
-        for (int i = tid; i < n; i += kBsThreads)
-            if (most > -INFINITY) mine += (u64)__double2ll_rn(exp((double)entry_logit(s_list[i]) - (double)most) * kBsUnit);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        if (lane == 0) s_listed[warp] = mine;
-    }
-    if (tid == kBsThreads - 1) s_unit = far ? 1.0 : exp2(-((double)from * (double)kLog2E + (double)shift));      // (the product is exact)
-    if (n > L.slots) {                                    // (many large ones in few threads) the best k go on
+    const int n = min(s_n, kBsList);
+    u64* to = L.lists + ((size_t)row * L.chunks + chunk) * L.slots;
+    const bool few = n <= L.slots;
+    if (few) {
+        if (tid < L.slots) to[tid] = tid < n ? s_list[tid] : 0ull;
+    } else {                                              // (many large ones in few threads) the best k go on
         for (int i = tid; i < n; i += kBsThreads) {
             const u64 e = s_list[i];
             int before = 0;
             for (int j = 0; j < n; ++j) before += s_list[j] > e;
-            s_sorted[before] = e;
+            if (before < a.k) to[before] = e;
         }
-        n = a.k;
-        list = s_sorted;
+        if (tid >= a.k && tid < L.slots) to[tid] = 0ull;
     }
-    __syncthreads();
-    u64* to = L.lists + ((size_t)row * L.chunks + chunk) * L.slots;
-    if (tid < L.slots) to[tid] = tid < n ? list[tid] : 0ull;
+    if (few && warp > 0) return;
+    // The listed ones' exponentials, in units of 2^-48 (whole numbers add up the same in any order), by one warp or by all; and, as one more, the unit of the others.
+    u64 mine = 0;
+    double unit = 1.0;
+    const double off = far ? 0.0 : (double)from * (double)kLog2E + (double)shift;      // (the product is exact)
+#pragma unroll 1
+    for (int i = tid; i <= n; i += few ? 32 : kBsThreads) {
+        const double e = exp(i < n ? (double)entry_logit(s_list[i]) - (double)from : off * -0.69314718055994531);
+        if (i == n) unit = e;
+        else if (most > -INFINITY) mine += (u64)__double2ll_rn(e * kBsUnit);
+    }
+    const u64 listed = ((u64)__reduce_add_sync(0xffffffffu, (unsigned)(mine >> 26)) << 26) + __reduce_add_sync(0xffffffffu, (unsigned)mine & 0x3ffffffu);
+    if (few) {
+        unit = __shfl_sync(0xffffffffu, unit, n & 31);
+    } else {
+        if (tid == n % kBsThreads) s_unit = unit;
+        if (lane == 0) s_listed[warp] = listed;
+        __syncthreads();
+        unit = s_unit;
+    }
     if (tid == 0) {
         BeamPart p;
-        u64 listed = 0;
-        for (int w = 0; w < kBsWarps && 32 * w < listed_n; ++w) listed += s_listed[w];
-        double others = 0.0;
+        u64 all = listed, others = 0;
 #pragma unroll
         for (int w = 0; w < kBsWarps; ++w) others += s_sum[w];
-        p.sum = (double)listed * (1.0 / kBsUnit) + others * s_unit;
+        if (!few)
+            for (int w = 1; w < kBsWarps; ++w) all += s_listed[w];
+        p.sum = (double)all * (1.0 / kBsUnit) + (double)others * (unit / kBsUnitOthers);
         p.most = most;
         L.parts[(size_t)row * L.chunks + chunk] = p;
     }

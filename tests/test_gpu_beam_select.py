@@ -188,6 +188,16 @@ def test_logits_on_a_grid(cuda_lib, grid):
     check(flat, np.zeros(2, np.float32), 1, 4)
 
 
+@pytest.mark.parametrize("offset", [3e4, -3e4, 32768, 1e6, -1e9, 1e12, -1e20, 1e36, 2e38, -3e38])
+def test_logits_far_from_zero(cuda_lib, offset):
+    """Rows that lie around any number, and rows spread as widely: the largest counts for 1, whatever it is."""
+    rng = np.random.default_rng(3)
+    near = (offset + rng.standard_normal((4, 20000)) * 3).astype(np.float32)
+    wide = (rng.standard_normal((4, 20000)) * min(abs(offset), 6e37)).astype(np.float32)
+    for logits in (near, wide):
+        check(logits, np.array([0, -1, -2, -3], np.float32), 2, 6)
+
+
 def test_two_at_once(cuda_lib):
     """Calls on two streams, each with a workspace of its own."""
     from tenzo_b200 import kernels
