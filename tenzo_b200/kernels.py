@@ -218,20 +218,18 @@ def _arg(t: torch.Tensor | None, dtype, device: int, what: str) -> int:
 def _arg_rows(t: torch.Tensor, device: int, columns: int, what: str) -> tuple[int, int, int]:
     """Address, row stride and number of fp32 rows that may lie apart (a column slice of a wider buffer)."""
     shape, strides = t.shape, t.stride()
-    if t.dtype is not torch.float32 or t.get_device() != device or len(shape) != 2 or shape[1] != columns or (columns > 1 and strides[1] != 1):
-        _refuse(t, what, f"fp32 rows of {columns} values")
-    n = shape[0]
+    n = shape[0] if len(shape) == 2 else -1
+    if n < 0 or t.dtype is not torch.float32 or t.get_device() != device or shape[1] != columns or (columns > 1 and strides[1] != 1) or (n > 1 and strides[0] < columns):
+        _refuse(t, what, f"fp32 rows of {columns} values that do not overlap")
     return t.data_ptr(), strides[0] if n > 1 else max(strides[0], columns), n
 
 
 def _kv4_cache(pool: torch.Tensor, block_table: torch.Tensor, device: int):
-    """The bytes of abi.Kv4Cache, kv heads, table rows and columns."""
+    """The fields of abi.Kv4Cache."""
     shape, table = pool.shape, block_table.shape
     if len(shape) != 6 or len(table) != 2 or shape[3] != 2 or shape[4] != 16 or shape[5] != 80:
         raise ValueError(f"a pool [blocks, layers, kv heads, 2, 16, 80] and a table [rows, columns] are needed, not {tuple(shape)} and {tuple(table)}")
-    n_kv, (rows, columns) = shape[2], table
-    return (_KV4_CACHE.pack(_arg(pool, torch.uint8, device, "pool"), shape[0], shape[1], n_kv, _arg(block_table, torch.int32, device, "block_table"), rows, columns),
-            n_kv, rows, columns)
+    return _arg(pool, torch.uint8, device, "pool"), shape[0], shape[1], shape[2], _arg(block_table, torch.int32, device, "block_table"), table[0], table[1]
 
 
 def _arg_entries(t, n: int, device: int, what: str) -> int:
@@ -254,12 +252,13 @@ def kv4_append(k, v, pool, pos, *, layer, block_table, seq=None, rope_cos=None, 
     positions pos int32 [n] of the sequences seq int32 [n] (default: row i is sequence i) of block_table int32 [sequences, columns].
     A negative position marks a padding row, for which nothing is stored."""
     dev = _current_device()
-    cache, n_kv, _, _ = _kv4_cache(pool, block_table, dev)
+    cache = _kv4_cache(pool, block_table, dev)
+    n_kv = cache[3]
     (kp, ks, n), (vp, vs, m) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
     if n != m or (ks != vs and n > 1):
         raise ValueError("k and v have the same number of rows, equally far apart")
     cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
-    _ok(_beam_calls()[0](cache, layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, cos, sin, length, use_pdl, _raw_stream(dev)),
+    _ok(_beam_calls()[0](_KV4_CACHE.pack(*cache), layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, cos, sin, length, use_pdl, _raw_stream(dev)),
         "tenzo_cuda_kv4_append")
 
 
@@ -267,9 +266,9 @@ def kv4_read(pool, pos, *, layer, block_table, seq=None, use_pdl=False, k=None, 
     """The rows at positions pos int32 [n] of the sequences seq as the cache holds them: (k, v), fp32 [n, n_kv*128], the keys rotated; zeros for
     negative positions. k and v may be given (both) to be written into."""
     dev, n = _current_device(), len(pos)
-    cache, n_kv, _, _ = _kv4_cache(pool, block_table, dev)
+    cache = _kv4_cache(pool, block_table, dev)
+    ks = cache[3] * 128
     if k is None and v is None:
-        ks = n_kv * 128
         both = torch.empty(2, n, ks, dtype=torch.float32, device=pool.device)
         kp = both.data_ptr()
         vp = kp + 4 * n * ks
@@ -277,10 +276,10 @@ def kv4_read(pool, pos, *, layer, block_table, seq=None, use_pdl=False, k=None, 
     elif k is None or v is None:
         raise ValueError("k and v are given both or not at all")
     else:
-        (kp, ks, m), (vp, vs, o) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
+        (kp, ks, m), (vp, vs, o) = _arg_rows(k, dev, ks, "k"), _arg_rows(v, dev, ks, "v")
         if n != m or n != o or (ks != vs and n > 1):
             raise ValueError("k and v have one row for each position, equally far apart")
-    _ok(_beam_calls()[1](cache, layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, use_pdl, _raw_stream(dev)), "tenzo_cuda_kv4_read")
+    _ok(_beam_calls()[1](_KV4_CACHE.pack(*cache), layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, use_pdl, _raw_stream(dev)), "tenzo_cuda_kv4_read")
     return k, v
 
 
@@ -308,20 +307,21 @@ def attention_kv4(q, pool, pos, *, layer, n_q, block_table, seq=None, rope_cos=N
     Returns out [rows, n_q*128]; zeros where pos is negative. max_len: an upper bound on pos + 1 (default: what the table has room for).
     workspace: a uint8 tensor for partial results of splits (default: one is allocated if the call wants it)."""
     dev = _current_device()
-    cache, n_kv, _, columns = _kv4_cache(pool, block_table, dev)
+    cache = _kv4_cache(pool, block_table, dev)
+    n_kv, columns = cache[3], cache[6]
     qp, q_stride, rows = _arg_rows(q, dev, n_q * 128, "q")
     cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
     if max_len is None:
         max_len = min(columns * 16, length) if cos else columns * 16
     if out is None:
-        out = torch.empty(rows, n_q * 128, dtype=torch.float32, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != (rows, n_q * 128):
         raise ValueError(f"out is [{rows}, {n_q * 128}]")
     if workspace is None:
         size = _attention_kv4_room(rows, n_q, n_kv, max_len, split_keys)
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-    args = _KV4_ATTENTION.pack(qp, _arg(out, torch.float32, dev, "out"), *_KV4_CACHE.unpack(cache), _arg_entries(pos, rows, dev, "pos"), _arg_entries(seq, rows, dev, "seq"),
+    args = _KV4_ATTENTION.pack(qp, _arg(out, torch.float32, dev, "out"), *cache, _arg_entries(pos, rows, dev, "pos"), _arg_entries(seq, rows, dev, "seq"),
                                cos, sin, length, q_stride, layer, n_q, rows, max_len, split_keys, use_pdl, _arg(workspace, torch.uint8, dev, "workspace"),
                                0 if workspace is None else workspace.numel())
     _ok(_beam_calls()[3](args, _raw_stream(dev)), "tenzo_cuda_attention_kv4")
@@ -351,14 +351,15 @@ def kv4_reorder(pool, block_table, parent, length, *, out=None, use_pdl=False):
     """The block table of the beams that go on from parent int32 [groups, beams] of beams that hold length int32 [groups] tokens each. Full blocks are
     shared; the block being filled is copied within `pool` for the second and further children of a beam, into those of beams without children."""
     dev, (groups, beams) = _current_device(), parent.shape
-    cache, _, rows, _ = _kv4_cache(pool, block_table, dev)
+    cache = _kv4_cache(pool, block_table, dev)
+    rows = cache[5]
     if rows != groups * beams:
         raise ValueError(f"{groups} groups of {beams} beams need as many table rows, not {rows}")
     if out is None:
         out = torch.empty_like(block_table)
     elif out.shape != block_table.shape:
         raise ValueError("out has the table's shape")
-    _ok(_beam_calls()[2](cache, _arg(out, torch.int32, dev, "out"), _arg(parent, torch.int32, dev, "parent"), _arg_entries(length, groups, dev, "length"), groups, beams,
+    _ok(_beam_calls()[2](_KV4_CACHE.pack(*cache), _arg(out, torch.int32, dev, "out"), _arg(parent, torch.int32, dev, "parent"), _arg_entries(length, groups, dev, "length"), groups, beams,
                          use_pdl, _raw_stream(dev)), "tenzo_cuda_kv4_reorder")
     return out
 

@@ -161,6 +161,9 @@ def test_python_calls_refuse_what_does_not_fit(monkeypatch):
                  lambda: kernels.attention_kv4(rows, pool, pos, layer=0, n_q=2, block_table=table), lambda: kernels.attention_kv4(rows, pool, pos.long(), layer=0, n_q=1, block_table=table),
                  lambda: kernels.attention_kv4(rows, pool, pos, layer=0, n_q=1, block_table=table, rope_cos=torch.zeros(32, 64)),
                  lambda: kernels.beam_select(rows, scores, beams=0, k=2), lambda: kernels.beam_select(rows, scores, beams=-1, k=2), lambda: kernels.beam_select(rows, scores, beams=2, k=0),
+                 lambda: kernels.attention_kv4(rows[:1].expand(2, 128), pool, pos, layer=0, n_q=1, block_table=table), lambda: kernels.beam_select(rows[:1].expand(2, 128), scores, beams=2, k=2),
+                 lambda: kernels.kv4_append(rows, rows[:1].expand(2, 128), pool, pos, layer=0, block_table=table), lambda: kernels.attention_kv4(rows[0], pool, pos, layer=0, n_q=1, block_table=table),
+                 lambda: kernels.beam_select(rows.flatten().unfold(0, 128, 64), torch.zeros(3), beams=3, k=2), lambda: kernels.beam_select(rows[0], scores, beams=1, k=2),
                  lambda: kernels.beam_select(rows[:1], scores[:1], beams=2, k=2), lambda: kernels.beam_select(rows.half(), scores, beams=2, k=2),
                  lambda: kernels.beam_select(rows, scores, beams=2, k=2, finished=pos[:1]), lambda: kernels.beam_select(rows.t(), scores, beams=2, k=2),
                  lambda: kernels.kv4_reorder(pool, table, torch.zeros(1, 3, dtype=torch.int32), pos[:1]), lambda: kernels.kv4_reorder(pool, table, torch.zeros(1, 2, dtype=torch.int32), pos)):
