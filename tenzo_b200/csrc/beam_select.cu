@@ -14,8 +14,7 @@
 // Sums are taken in an order that the data alone decides, or as integers, so that equal rows get equal sums and tie.
 //
 // 32 x 8 rows of 128256, k 16: 36.3 us. Loads alone take the first kernel 21 (131 MB at 6.2 TB/s), with everything else in it 29: some eight instructions and an ex2 a
-// logit, and the barriers around the bisection, are hidden by the other CTAs' loads for two thirds only. The second kernel is 7, a chain of a few thousand instructions
-// that run once.
+// logit, and the barriers around the bisection, are hidden by the other CTAs' loads for two thirds only. The second kernel is 7, a chain of some 10 000 cycles.
 #include "common.cuh"
 #include "kv4.cuh"
 
@@ -307,8 +306,8 @@ struct BeamGroup {
     int n_live;
 };
 
-// Its loops are not unrolled further than their loads ask for: every instruction runs a few times only, and a kernel's first pass through its
-// code waits for the code. Dynamic shared memory: the group, then `hold` entries a warp (0: the lists are longer and read from L2).
+// Its loops are not unrolled further than their loads ask for: every instruction runs a few times only, and what runs once waits for its code (11 700 cycles at first, 10 200 when
+// all of it is in the caches). Dynamic shared memory: the group, then `hold` entries a warp (0: the lists are longer and read from L2).
 __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const BeamLaunch L, const int hold) {
     extern __shared__ __align__(16) unsigned char bs_smem[];
     BeamGroup& G = *reinterpret_cast<BeamGroup*>(bs_smem);
@@ -386,10 +385,13 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
                 if (at_least(least) >= k) low = least;
                 reach = at_least(low);
 #pragma unroll 1
-                while (reach > k + kBsWindow && high - low > 1) {
-                    const uint32_t mid = low + (high - low) / 2;
-                    const int m = at_least(mid);
-                    if (m >= k) { low = mid; reach = m; } else high = mid;
+                while (reach > k + kBsWindow && high - low > 1) {       // (in quarters: three counts take little longer than one)
+                    const uint32_t half = low + (high - low) / 2, first = low + (half - low) / 2, third = half + (high - half) / 2;
+                    const int m1 = at_least(first), m2 = at_least(half), m3 = at_least(third);
+                    if (m3 >= k) { low = third; reach = m3; }
+                    else if (m2 >= k) { low = half; reach = m2; high = third; }
+                    else if (m1 >= k) { low = first; reach = m1; high = half; }
+                    else high = first;
                 }
                 lo = (u64)low << 32;
             }
