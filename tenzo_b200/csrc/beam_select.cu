@@ -510,8 +510,8 @@ __global__ void __launch_bounds__(kBsMergeWarps * 32) beam_groups_kernel(const B
     }
 }
 
-// Logits a thread takes: 32, or fewer where that would leave SMs without a CTA.
-// (and lists would no longer be held in registers by the second kernel).
+// Logits a thread takes: 32, or fewer where that would leave SMs without a CTA, as long as the second kernel's warps can keep a row's lists (1 x 4 beams: 10.7 us, where they do
+// not 11.3; 8 x 32 beams with 64 candidates: 72.5 and 79.5).
 static int beam_chunks(int per, int vocab) { return (int)(((long long)vocab + kBsThreads * per - 1) / (kBsThreads * per)); }
 static int beam_slots(int k) { return ((k > kBsLeast ? k : kBsLeast) + 2 * kBsWindow + 1) / 2 * 2; }      // (even: they are read two at a time)
 static int beam_per(int rows, int vocab, int k) {
@@ -526,6 +526,9 @@ static_assert((sizeof(BeamGroup) + 15) / 16 * 16 + (size_t)kBsMergeWarps * kBsHo
 template <bool VEC>
 static int beam_rows_run(const BeamLaunch& L, cudaStream_t st) {
     auto* kernel = L.per == 32 ? beam_rows_kernel<VEC, 32> : L.per == 16 ? beam_rows_kernel<VEC, 16> : L.per == 8 ? beam_rows_kernel<VEC, 8> : beam_rows_kernel<VEC, 4>;
+    // Few CTAs: shared memory set up as the second kernel needs it, which otherwise waits until it is changed (5 x 12 rows of 50001: 15.7 us, 16.9 without). Many: as much of it for
+    // loads on their way as there is (32 x 8 of 128256: 36.1 us, 39.4 otherwise).
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, L.eager ? cudaSharedmemCarveoutMaxShared : cudaSharedmemCarveoutDefault)) return (int)e;
     return kv4_launch(kernel, dim3((unsigned)(L.a.groups * L.a.beams) * (unsigned)L.chunks), kBsThreads, 0, st, L.a.use_pdl != 0, L);
 }
 
@@ -555,7 +558,7 @@ extern "C" int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* 
     L.per = beam_per((int)rows, a.vocab, a.k);
     L.chunks = beam_chunks(L.per, a.vocab);
     L.slots = beam_slots(a.k);
-    L.eager = rows * L.chunks <= 592;
+    L.eager = rows * L.chunks <= 592;                     // one wave (logits of rows that are left out: 32 x 8 beams, one in ten finished: 37.9 us with them, 36.1 without)
     if (rows * L.chunks > 0x7fffffffLL || (long long)L.chunks * L.slots > 0x7fffffffLL || (long long)L.chunks * kBsThreads * L.per > 0x7fffffffLL) return -1;
     if (a.workspace_bytes < tenzo_cuda_beam_select_workspace_bytes(a.groups, a.beams, a.vocab, a.k)) return -1;
     L.parts = static_cast<BeamPart*>(a.workspace);
