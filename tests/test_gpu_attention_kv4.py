@@ -297,6 +297,31 @@ def test_long_rows_that_share_a_sequence(cuda_lib):
     assert kernels.kv4_take_errors() == 0
 
 
+@pytest.mark.parametrize("n_q,n_kv,most,split", [(8, 2, 1000, 0), (20, 5, 9000, 0), (3, 1, 300, 512)])
+def test_captured_once_for_growing_sequences(cuda_lib, n_q, n_kv, most, split):
+    """A graph captured with one set of lengths and replayed with others, queries and tables changed in place; nothing of an earlier replay stays."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(most)
+    columns = (most + 15) // 16
+    table, pool = setup(rng, [most, most], n_kv, columns)
+    d = dict(q=torch.zeros(2, n_q * 128, device="cuda"), pos=torch.full((2,), most - 1, dtype=torch.int32, device="cuda"), table=dev(table))
+    dp = dev(pool)
+    call = lambda: kernels.attention_kv4(d["q"], dp, d["pos"], layer=0, n_q=n_q, block_table=d["table"], max_len=most, split_keys=split, use_pdl=True)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for lens in ([1, most], [most // 2, 17], [0, 33], [most, most - 1]):
+        q, pos, swapped = rng.standard_normal((2, n_q * 128)).astype(np.float32), np.array(lens, np.int32) - 1, table[::-1].copy()
+        for name, x in (("q", q), ("pos", pos), ("table", swapped)):
+            d[name].copy_(dev(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(host(out), q, pool, swapped, 0, pos, range(2))
+    assert kernels.kv4_take_errors() == 0
+
+
 def test_two_at_once(cuda_lib):
     """Calls on two streams, joined by clusters, by a second kernel, and not at all; each with a workspace of its own."""
     from tenzo_b200 import kernels

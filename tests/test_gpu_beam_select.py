@@ -176,6 +176,20 @@ def test_odd_numbers_of_candidates(cuda_lib, k):
         check(logits, (-9 * rng.random(2 * beams)).astype(np.float32), beams, k)
 
 
+@pytest.mark.parametrize("beams,vocab,k", [(2, 400000, 64), (1, 1000003, 64), (3, 262144, 33)])
+def test_lists_longer_than_a_warp_keeps(cuda_lib, beams, vocab, k):
+    rng = np.random.default_rng(vocab)
+    logits = (rng.standard_normal((beams, vocab)) * 2).astype(np.float32)
+    check(logits, -np.arange(beams, dtype=np.float32), beams, k)
+    check(np.round(logits), -np.arange(beams, dtype=np.float32), beams, k)             # the border falls among many alike
+
+
+def test_many_groups(cuda_lib):
+    rng = np.random.default_rng(40)
+    logits, scores = rng.standard_normal((3000 * 2, 57)).astype(np.float32), (-5 * rng.random(6000)).astype(np.float32)
+    check(logits, scores, 2, 5, finished=(rng.random(6000) < 0.2).astype(np.int32), eos=56)
+
+
 @pytest.mark.parametrize("grid", [1.0, 0.5, 0.125])
 def test_logits_on_a_grid(cuda_lib, grid):
     """Logits of few different values, as those of a coarser type are: errors of their exponentials do not average out."""
