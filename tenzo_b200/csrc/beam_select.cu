@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
 #pragma unroll
             for (int j = PER - 1; j >= 0; --j)
                 if (v[j] == bound && place(j) < a.vocab) first = place(j);
+            if (bound == -INFINITY) first = place(0);     // (nothing but masks in these threads, and NaN is one: found by == or not)
         }
         __syncthreads();
         s_keys[tid] = (uint32_t)first;

@@ -235,3 +235,20 @@ def test_no_groups(cuda_lib):
     from tenzo_b200 import kernels
     parent, token, score = kernels.beam_select(torch.empty(0, 10, device="cuda"), torch.empty(0, device="cuda"), beams=2, k=3)
     assert parent.shape == token.shape == score.shape == (0, 3)
+
+
+@pytest.mark.parametrize("beams", [1, 4])
+@pytest.mark.parametrize("vocab,repeats", [(1000, 1), (8192, 1), (8192, 8), (20001, 3), (128256, 1)])
+def test_few_numbers_among_nan(cuda_lib, vocab, repeats, beams):
+    """Fewer finite logits than are asked for, at the front, in the middle, at the end and scattered, the rest NaN; NaN and -infinity in turns, at random and by the
+    threads that hold them: every finite one counts, then the lowest tokens of those that are masked. (Many rows: as many logits a thread as there can be.)"""
+    rng = np.random.default_rng(vocab + beams)
+    owner = np.arange(vocab) // 4 % 256
+    rests = [np.full(vocab, np.nan), np.where(rng.random(vocab) < 0.5, np.nan, -np.inf), np.where(owner % 2, np.nan, -np.inf), np.where(owner < 200, np.nan, -np.inf)]
+    for finite in (0, 1, 12, 15, 17):
+        places = [np.arange(finite), vocab // 2 + np.arange(finite), vocab - 1 - np.arange(finite), rng.choice(vocab, finite, replace=False)]
+        logits = np.stack([rest for rest in rests for _ in places] * repeats).astype(np.float32)
+        for row, at in zip(logits, places * len(rests) * repeats):
+            row[at] = np.round(rng.standard_normal(finite) * 8) / 4
+        for k in (8, 24):
+            check(logits, (-3 * rng.random(len(logits))).astype(np.float32), beams, k)
