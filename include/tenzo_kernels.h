@@ -294,7 +294,8 @@ TENZO_API size_t tenzo_cuda_attention_kv4_workspace_bytes(int rows, int n_q, int
 /* Splits that the call's own choice (split_keys 0) wants room for; 1: none, 0: arguments that the call refuses. */
 TENZO_API int tenzo_cuda_attention_kv4_splits(int rows, int n_q, int n_kv, int max_len);
 /* Error flags of the calls above and below this one since the last call (bit 0: a bounded wait was given up, bit 1: an index out of range);
- * -1 if the query failed. Synchronises with the device. */
+ * -1 if the query failed, which leaves the flags as they are. Synchronises with the device: waits for all of its streams, so it cannot be called while one is
+ * captured. */
 TENZO_API int tenzo_cuda_kv4_take_errors(void);
 
 /* The cache's half of a beam-search step. Table rows g*beams .. g*beams + beams - 1 are the beams of group g and hold length[g] tokens each; beam i goes

@@ -609,13 +609,11 @@ static int a4_run(const A4Launch& L, cudaStream_t st) {
     return kv4_launch_cluster(attention_kv4_kernel<HB>, grid, kA4Threads, L.cluster ? L.n_splits : 1, smem, st, L.a.use_pdl != 0, L);
 }
 
-int kv4_attention_take_error() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_kv4_attention_error, sizeof v) != cudaSuccess) return -1;
-    if (v) cudaMemcpyToSymbol(g_kv4_attention_error, &zero, sizeof zero);
-    return v;
+int* kv4_rows_flags();
+__global__ void kv4_clear_flags_kernel(int* rows, int rows_seen, int* attention, int attention_seen) {
+    atomicAnd(rows, ~rows_seen);
+    atomicAnd(attention, ~attention_seen);
 }
-int kv4_rows_take_error();
 
 }  // namespace tz
 
@@ -674,7 +672,15 @@ extern "C" int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, vo
     return kv4_launch(attention_kv4_merge_kernel, dim3((unsigned)a.rows, (unsigned)((a.n_q + kA4Warps - 1) / kA4Warps)), kA4Threads, 0, st, true, L);
 }
 
+// What runs on any stream is waited for, also on those that do not wait for the default one. Only bits that were seen are cleared: of what another thread's call raises
+// meanwhile a bit is in the result or stays.
 extern "C" int tenzo_cuda_kv4_take_errors(void) {
-    const int a = tz::kv4_rows_take_error(), b = tz::kv4_attention_take_error();
-    return a < 0 || b < 0 ? -1 : a | b;
+    using namespace tz;
+    int *rows = kv4_rows_flags(), *attention = nullptr, r = 0, a = 0;
+    if (!rows || cudaGetSymbolAddress(reinterpret_cast<void**>(&attention), g_kv4_attention_error) != cudaSuccess) return -1;
+    if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(&r, rows, sizeof r, cudaMemcpyDeviceToHost) != cudaSuccess ||
+        cudaMemcpy(&a, attention, sizeof a, cudaMemcpyDeviceToHost) != cudaSuccess)
+        return -1;
+    if ((r | a) && (kv4_launch(kv4_clear_flags_kernel, dim3(1), 1, 0, cudaStreamLegacy, false, rows, r, attention, a) || cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess)) return -1;
+    return r | a;
 }

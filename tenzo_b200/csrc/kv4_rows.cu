@@ -281,11 +281,9 @@ static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, co
 static int rows_a_warp(int rows, int n_kv) { return (long long)rows * n_kv >= 4LL * 148 * 16 ? 2 : 1; }
 static dim3 rows_grid(int rows, int n_kv, int r) { return dim3((unsigned)((((long long)rows + r - 1) / r * n_kv + kRowWarps - 1) / kRowWarps)); }
 
-int kv4_rows_take_error() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_kv4_rows_error, sizeof v) != cudaSuccess) return -1;
-    if (v) cudaMemcpyToSymbol(g_kv4_rows_error, &zero, sizeof zero);
-    return v;
+int* kv4_rows_flags() {
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, g_kv4_rows_error) == cudaSuccess ? static_cast<int*>(p) : nullptr;
 }
 
 }  // namespace tz

@@ -365,5 +365,6 @@ def kv4_reorder(pool, block_table, parent, length, *, out=None, use_pdl=False):
 
 
 def kv4_take_errors() -> int:
-    """Error flags of the 4-bit cache's kernels since the last call (1: a wait was given up, 2: an index out of range); synchronises."""
+    """Error flags of the 4-bit cache's kernels since the last call (1: a wait was given up, 2: an index out of range), -1 if the query failed; waits for
+    all streams of the device."""
     return int(load_library().tenzo_cuda_kv4_take_errors())

@@ -197,3 +197,23 @@ def test_on_a_side_stream_and_in_a_graph(cuda_lib):
     d.copy_(dev(pool))
     graph.replay()
     assert np.array_equal(host(d), expect(pool, table, 0, k + np.float32(1), v, pos, range(6), None, None))
+
+
+def test_errors_of_a_stream_that_is_still_running(cuda_lib):
+    """The query waits for streams that do not wait for the default stream, and reports what was raised there; each flag once."""
+    from tenzo_b200 import kernels
+    pool, table = torch.zeros(2, 1, 1, 2, 16, 80, dtype=torch.uint8, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    rows, beyond = torch.ones(1, 128, device="cuda"), torch.full((1,), 16, dtype=torch.int32, device="cuda")
+    calls = [lambda: kernels.kv4_append(rows, rows, pool, beyond, layer=0, block_table=table),
+             lambda: kernels.attention_kv4(rows, pool, beyond, layer=0, n_q=1, block_table=table, out=torch.empty_like(rows))]
+    for call in calls:                                                      # (both modules loaded before the query is to be quicker than the stream)
+        call()
+    torch.cuda.synchronize()
+    assert kernels.kv4_take_errors() == 2
+    for call in calls:
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)                                  # about 0.1 s
+            call()
+        assert kernels.kv4_take_errors() == 2
+        assert kernels.kv4_take_errors() == 0
