@@ -479,7 +479,9 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         }
     }
     if (L.cluster) {                                     // each CTA joins a share of the outputs, from all of the cluster's shared memory
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // (not .aligned: a share's last round leaves lanes out, and nothing says that a warp is together again after a loop)
+        auto cluster_sync = [] { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); };
+        cluster_sync();
         auto of = [](uint32_t at, int rank) {
             uint32_t r;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
             }
             out[i] = l == 0.0f ? 0.0f : o / l;
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");       // until all have read
+        cluster_sync();                                  // until all have read
     }
 }
 

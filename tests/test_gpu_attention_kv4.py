@@ -365,3 +365,25 @@ def test_pools_beyond_32_bits(cuda_lib):
     out = kernels.attention_kv4(dev(q), pool, dev(np.array([n - 1], np.int32)), layer=3, n_q=16, block_table=dt)
     check(host(out), q, small, np.arange(4)[None], 3, [n - 1], [0])
     assert kernels.kv4_take_errors() == 0
+
+
+@pytest.mark.parametrize("splits", [2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("rows,n_q,n_kv", [(2, 4, 1), (3, 3, 1), (1, 5, 5), (2, 20, 5), (2, 7, 1), (40, 8, 1), (45, 7, 1)])
+def test_clusters_of_every_size(cuda_lib, rows, n_q, n_kv, splits):
+    """Shares of the outputs that no number of warps divides; splits without keys, padding and refused rows beside full ones. (45 rows of 8 splits of seven heads a CTA.)"""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(splits * 100 + n_q)
+    most = 128 * splits
+    lens = [most] + [int(n) for n in rng.integers(1, most + 1, rows - 1)]
+    table, pool = setup(rng, lens, n_kv, most // 16)
+    q = rng.standard_normal((rows + 2, n_q * 128)).astype(np.float32)
+    seq, pos = np.r_[np.arange(rows), 0, 0].astype(np.int32), np.r_[np.array(lens) - 1, -1, most].astype(np.int32)
+    g = Guarded()
+    out = g.empty((rows + 2, n_q * 128), torch.float32)
+    out.fill_(7.0)
+    for pdl in (False, True):
+        kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=n_q, block_table=dev(table), seq=dev(seq), max_len=most, out=out, use_pdl=pdl)
+    check(host(out)[:-1], q[:-1], pool, table, 0, pos[:-1], seq[:-1])
+    assert (host(out)[-1] == 7.0).all()
+    g.check()
+    assert kernels.kv4_take_errors() == 2
