@@ -179,6 +179,7 @@ assert _KV4_CACHE.size == C.sizeof(abi.Kv4Cache) and _KV4_ATTENTION.size == C.si
 
 
 _PI, _PP, _PB = C.c_int, C.c_void_p, C.c_char_p
+_INT_MOST = 2 ** 31 - 1
 
 
 @functools.cache
@@ -221,7 +222,12 @@ def _arg_rows(t: torch.Tensor, device: int, columns: int, what: str) -> tuple[in
     n = shape[0] if len(shape) == 2 else -1
     if n < 0 or t.dtype is not torch.float32 or t.get_device() != device or shape[1] != columns or (columns > 1 and strides[1] != 1) or (n > 1 and strides[0] < columns):
         _refuse(t, what, f"fp32 rows of {columns} values that do not overlap")
-    return t.data_ptr(), strides[0] if n > 1 else max(strides[0], columns), n
+    stride = strides[0] if n > 1 else max(strides[0], columns)
+    if stride > _INT_MOST:
+        if n > 1:
+            _refuse(t, what, "rows that lie fewer than 2^31 values apart")
+        stride = columns                                        # one row: any
+    return t.data_ptr(), stride, n
 
 
 def _kv4_cache(pool: torch.Tensor, block_table: torch.Tensor, device: int):
@@ -230,6 +236,13 @@ def _kv4_cache(pool: torch.Tensor, block_table: torch.Tensor, device: int):
     if len(shape) != 6 or len(table) != 2 or shape[3] != 2 or shape[4] != 16 or shape[5] != 80:
         raise ValueError(f"a pool [blocks, layers, kv heads, 2, 16, 80] and a table [rows, columns] are needed, not {tuple(shape)} and {tuple(table)}")
     return _arg(pool, torch.uint8, device, "pool"), shape[0], shape[1], shape[2], _arg(block_table, torch.int32, device, "block_table"), table[0], table[1]
+
+
+def _arg_layer(layer: int) -> int:
+    """`layer` where it fits the prototype's C int, which takes larger ones modulo 2^32."""
+    if not -_INT_MOST <= layer <= _INT_MOST:
+        raise ValueError(f"there is no layer {layer}")
+    return layer
 
 
 def _arg_entries(t, n: int, device: int, what: str) -> int:
@@ -258,7 +271,7 @@ def kv4_append(k, v, pool, pos, *, layer, block_table, seq=None, rope_cos=None, 
     if n != m or (ks != vs and n > 1):
         raise ValueError("k and v have the same number of rows, equally far apart")
     cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
-    _ok(_beam_calls()[0](_KV4_CACHE.pack(*cache), layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, cos, sin, length, use_pdl, _raw_stream(dev)),
+    _ok(_beam_calls()[0](_KV4_CACHE.pack(*cache), _arg_layer(layer), kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, cos, sin, length, use_pdl, _raw_stream(dev)),
         "tenzo_cuda_kv4_append")
 
 
@@ -279,7 +292,7 @@ def kv4_read(pool, pos, *, layer, block_table, seq=None, use_pdl=False, k=None, 
         (kp, ks, m), (vp, vs, o) = _arg_rows(k, dev, ks, "k"), _arg_rows(v, dev, ks, "v")
         if n != m or n != o or (ks != vs and n > 1):
             raise ValueError("k and v have one row for each position, equally far apart")
-    _ok(_beam_calls()[1](_KV4_CACHE.pack(*cache), layer, kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, use_pdl, _raw_stream(dev)), "tenzo_cuda_kv4_read")
+    _ok(_beam_calls()[1](_KV4_CACHE.pack(*cache), _arg_layer(layer), kp, vp, ks, _arg_entries(pos, n, dev, "pos"), _arg_entries(seq, n, dev, "seq"), n, use_pdl, _raw_stream(dev)), "tenzo_cuda_kv4_read")
     return k, v
 
 

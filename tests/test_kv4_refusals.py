@@ -169,3 +169,20 @@ def test_python_calls_refuse_what_does_not_fit(monkeypatch):
                  lambda: kernels.kv4_reorder(pool, table, torch.zeros(1, 3, dtype=torch.int32), pos[:1]), lambda: kernels.kv4_reorder(pool, table, torch.zeros(1, 2, dtype=torch.int32), pos)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_numbers_beyond_a_c_int(monkeypatch):
+    """A layer or a distance of rows of 2^32 and something is refused, not taken modulo 2^32; how far from the next the only row would lie does not matter."""
+    monkeypatch.setattr(kernels, "_current_device", lambda: -1)
+    pool, table, pos = torch.zeros(4, 1, 1, 2, 16, 80, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    rows, far = torch.zeros(2, 128), torch.empty_strided((2, 128), (2 ** 32 + 128, 1), device="meta")
+    for layer in (2 ** 32, -2 ** 32, 2 ** 33 + 1, 2 ** 31):
+        for call in (lambda: kernels.kv4_append(rows, rows, pool, pos, layer=layer, block_table=table), lambda: kernels.kv4_read(pool, pos, layer=layer, block_table=table)):
+            with pytest.raises(ValueError):
+                call()
+    for call in (lambda: kernels.kv4_append(far, far, pool, pos, layer=0, block_table=table), lambda: kernels.kv4_read(pool, pos, layer=0, block_table=table, k=far, v=far),
+                 lambda: kernels.attention_kv4(far, pool, pos, layer=0, n_q=1, block_table=table), lambda: kernels.beam_select(far, torch.zeros(2), beams=2, k=2)):
+        with pytest.raises(ValueError):
+            call()
+    one = torch.zeros(200).as_strided((1, 128), (2 ** 32 + 64, 1))
+    assert kernels._arg_rows(one, -1, 128, "k") == (one.data_ptr(), 128, 1)
