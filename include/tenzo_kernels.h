@@ -303,7 +303,7 @@ TENZO_API int tenzo_cuda_kv4_take_errors(void);
  * blocks are shared) and its own above j. The block being filled, entry j if r > 0, belongs to one beam alone (they must differ): the first child of a
  * parent takes its parent's; the n-th of the further children, by index, takes that of the n-th beam without children, and the r filled slots of all layers and heads are copied
  * into it. If r = 0, entry j stays the beam's own. No block is allocated or freed, and a prompt is forked the same way: parent 0 for
- * all. table_out [groups*beams][table_stride] must not overlap the table; groups*beams = table_rows, beams <= TENZO_BEAMS_MOST and
+ * all. table_out [groups*beams][table_stride] must not overlap the table (-1); groups*beams = table_rows, beams <= TENZO_BEAMS_MOST and
  * n_layers*n_kv <= 16384 (-5 otherwise). A group with a parent or a length out of range is copied as it is and raises the flag. */
 enum { TENZO_BEAMS_MOST = 32 };
 TENZO_API int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_out, const int* parent, const int* length, int groups, int beams, int use_pdl,

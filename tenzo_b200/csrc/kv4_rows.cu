@@ -319,9 +319,11 @@ extern "C" int tenzo_cuda_kv4_read(const tenzo_kv4_cache* cache, int layer, floa
 extern "C" int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_out, const int* parent, const int* length, int groups, int beams, int use_pdl,
                                       void* stream) {
     using namespace tz;
-    if (!cache || !kv4_cache_ok(*cache) || !table_out || table_out == cache->block_table || !parent || !length || groups < 1) return -1;
+    if (!cache || !kv4_cache_ok(*cache) || !table_out || !parent || !length || groups < 1) return -1;
     if (beams < 1 || beams > TENZO_BEAMS_MOST) return -5;
     if ((long long)groups * beams != cache->table_rows) return -1;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(cache->block_table), to = reinterpret_cast<uintptr_t>(table_out), apart = from < to ? to - from : from - to;
+    if (apart < (size_t)cache->table_rows * cache->table_stride * sizeof(int)) return -1;           // a row would be read after another had been written over it
     if ((long long)cache->n_layers * cache->n_kv > 16384) return -5;          // (a block's 16-byte units are numbered in 32 bits, and divided by multiplication)
     // Parts of a group: six CTAs an SM in all (64 x 8 beams: 2 an SM 20.1 us, 3 18.2, 6 16.7, 16 16.6), and a batch of loads each at the most.
     const long long units = (long long)cache->n_layers * cache->n_kv * 2 * (kK4Half / 16), most = (units + kReorderThreads * kReorderBatch - 1) / (kReorderThreads * kReorderBatch);

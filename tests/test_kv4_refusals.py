@@ -186,3 +186,12 @@ def test_numbers_beyond_a_c_int(monkeypatch):
             call()
     one = torch.zeros(200).as_strided((1, 128), (2 ** 32 + 64, 1))
     assert kernels._arg_rows(one, -1, 128, "k") == (one.data_ptr(), 128, 1)
+
+
+@pytest.mark.parametrize("shift,code", [(0, -1), (4, -1), (16, -1), (76, -1), (-4, -1), (-76, -1)])
+def test_reorder_into_a_part_of_the_table_itself(lib, shift, code):
+    """A table of 4 rows of 5 entries is 80 bytes long."""
+    c = cache()
+    assert lib.tenzo_cuda_kv4_reorder(C.byref(c), P + shift, P, P, 2, 2, 0, None) == code
+    for beside in (80, -80):                             # (without a device the launch fails; on one it is not tried)
+        assert torch.cuda.is_available() or lib.tenzo_cuda_kv4_reorder(C.byref(c), P + beside, P, P, 2, 2, 0, None) > 0
