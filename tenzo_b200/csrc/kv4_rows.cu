@@ -269,7 +269,7 @@ static bool aligned16(const void* p) { return !(reinterpret_cast<uintptr_t>(p) &
 
 static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, const int* pos, const int* seq, int rows, RowsArgs* a) {
     if (!cache || !kv4_cache_ok(*cache) || layer < 0 || layer >= cache->n_layers || !pos || rows < 1 || (long long)rows * cache->n_kv > 0x7fffffffLL) return false;
-    if (kv_stride < cache->n_kv * 128) return false;
+    if (kv_stride < cache->n_kv * 128LL) return false;
     if (!seq && rows > cache->table_rows) return false;
     a->c = *cache;
     a->layer = layer; a->rows = rows; a->kv_stride = kv_stride; a->pos = pos; a->seq = seq;

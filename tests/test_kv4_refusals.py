@@ -195,3 +195,11 @@ def test_reorder_into_a_part_of_the_table_itself(lib, shift, code):
     assert lib.tenzo_cuda_kv4_reorder(C.byref(c), P + shift, P, P, 2, 2, 0, None) == code
     for beside in (80, -80):                             # (without a device the launch fails; on one it is not tried)
         assert torch.cuda.is_available() or lib.tenzo_cuda_kv4_reorder(C.byref(c), P + beside, P, P, 2, 2, 0, None) > 0
+
+
+@pytest.mark.parametrize("n_kv,stride", [(1 << 25, 0), (1 << 25, 128), (3 << 24, -(1 << 31)), ((1 << 25) + 1, 128)])
+def test_heads_whose_values_pass_32_bits(lib, n_kv, stride):
+    """n_kv * 128 is 2^32 and more: no stride holds that many values."""
+    c = cache(n_kv=n_kv)
+    assert lib.tenzo_cuda_kv4_append(C.byref(c), 0, P, P, stride, P, P, 1, None, None, 0, 0, None) == abi.ERR_INVALID
+    assert lib.tenzo_cuda_kv4_read(C.byref(c), 0, P, P, stride, P, P, 1, 0, None) == abi.ERR_INVALID
