@@ -627,7 +627,7 @@ extern "C" size_t tenzo_cuda_attention_kv4_workspace_bytes(int rows, int n_q, in
 
 extern "C" int tenzo_cuda_attention_kv4_splits(int rows, int n_q, int n_kv, int max_len) {
     using namespace tz;
-    if (rows <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_len <= 0 || max_len > 1 << 30) return 0;
+    if (rows <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || n_q > 4 * 65535 || n_kv > 65535 || max_len <= 0 || max_len > 1 << 30) return 0;
     A4Launch L = {};
     L.a.rows = rows; L.a.n_q = n_q; L.a.cache.n_kv = n_kv; L.a.max_len = max_len;
     L.group = n_q / n_kv;

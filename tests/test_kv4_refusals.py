@@ -203,3 +203,11 @@ def test_heads_whose_values_pass_32_bits(lib, n_kv, stride):
     c = cache(n_kv=n_kv)
     assert lib.tenzo_cuda_kv4_append(C.byref(c), 0, P, P, stride, P, P, 1, None, None, 0, 0, None) == abi.ERR_INVALID
     assert lib.tenzo_cuda_kv4_read(C.byref(c), 0, P, P, stride, P, P, 1, 0, None) == abi.ERR_INVALID
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(4 * 65535 + 1, 1), (65536, 65536), (4 * 65536, 65536)])
+def test_splits_of_more_heads_than_the_call_takes(lib, n_q, n_kv):
+    assert lib.tenzo_cuda_attention_kv4_splits(1, n_q, n_kv, 80) == 0
+    assert lib.tenzo_cuda_attention_kv4(C.byref(attention(n_q=n_q, cache=cache(n_kv=n_kv))), None) == abi.ERR_INVALID
+    for q, kv in ((4 * 65535, 1), (65535, 65535), (4 * 65535, 65535), (5 * 52428, 52428)):
+        assert lib.tenzo_cuda_attention_kv4_splits(1, q, kv, 80) >= 1
