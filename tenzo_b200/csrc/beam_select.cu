@@ -56,7 +56,6 @@ struct __align__(16) BeamPart {                           // of a chunk
 struct BeamLaunch {
     tenzo_beam_select_args a;
     int per, chunks, slots;                               // logits a thread takes, chunks a row, entries a chunk's list has room for
-    int eager;                                            // few CTAs: time counts, not the bytes of rows that are left out
     BeamPart* parts;                                      // [row][chunk]
     u64* lists;                                           // [row][chunk][slots], in any order; 0 where there is none
 };
@@ -65,7 +64,8 @@ struct BeamLaunch {
 __device__ __forceinline__ bool beam_dead(float cum) { return !(cum > -INFINITY); }
 __device__ __forceinline__ bool beam_finished(const tenzo_beam_select_args& a, int row) { return a.finished && ld_l2(a.finished + row) != 0; }
 
-template <bool VEC, int PER>
+// EAGER: few CTAs, so that time counts and not the bytes of rows that are left out.
+template <bool VEC, int PER, bool EAGER>
 __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaunch L) {
     __shared__ uint32_t s_keys[kBsThreads];
     __shared__ u64 s_list[kBsList], s_sum[kBsWarps], s_listed[kBsWarps];
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
     if (a.use_pdl) pdl_wait();
     const float cum = ld_l2(a.scores + row);
     const bool out = beam_finished(a, row) || beam_dead(cum);
-    if (!L.eager && out) return;                          // (eager: the logits are asked for meanwhile)
+    if (!EAGER && out) return;                            // (eager: the logits are asked for meanwhile)
     const float* x = a.logits + (size_t)row * a.row_stride;
     const int base = chunk * kBsThreads * PER;
     // place of the j-th logit of a thread: consecutive fours (or ones) go to consecutive threads
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(const BeamLaun
     if (tid == 0) {
         s_n = 0;
         // Where CTAs come in waves, the logits of a later one on their way to L2 meanwhile (32 x 8 rows of 128256: 43.8 us without, 42.2 one CTA an SM ahead, 42.9 four)
-        if (VEC && !L.eager && blockIdx.x + kBsAhead < gridDim.x) {
+        if (VEC && !EAGER && blockIdx.x + kBsAhead < gridDim.x) {
             const int r = (blockIdx.x + kBsAhead) / L.chunks, at = (blockIdx.x + kBsAhead) % L.chunks * kBsThreads * PER, n = min(a.vocab - at, kBsThreads * PER) & ~3;
             if (n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.logits + (size_t)r * a.row_stride + at), "r"(4 * n) : "memory");
         }
@@ -524,13 +524,22 @@ static int beam_per(int rows, int vocab, int k) {
 static size_t beam_groups_smem(int hold) { return (sizeof(BeamGroup) + 15) / 16 * 16 + (size_t)kBsMergeWarps * hold * sizeof(u64); }
 static_assert((sizeof(BeamGroup) + 15) / 16 * 16 + (size_t)kBsMergeWarps * kBsHold * sizeof(u64) <= kMaxSmem, "what an SM has");
 
+// One wave of CTAs (logits of rows that are left out: 32 x 8 beams, one in ten finished: 37.9 us with them, 36.1 without).
+static bool beam_eager(long long ctas) { return ctas <= 592; }
+
+template <bool VEC, int PER, bool EAGER>
+static int beam_rows_launch(const BeamLaunch& L, cudaStream_t st) {
+    auto* kernel = beam_rows_kernel<VEC, PER, EAGER>;
+    // Few CTAs: shared memory set up as the second kernel needs it, which otherwise waits until it is changed (5 x 12 rows of 50001: 15.7 us, 16.9 without). Many: as much of it for
+    // loads on their way as there is (32 x 8 of 128256: 36.1 us, 39.4 otherwise). As with allow_smem every host thread sets the same for a kernel: one of its own for either.
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, EAGER ? cudaSharedmemCarveoutMaxShared : cudaSharedmemCarveoutDefault)) return (int)e;
+    return kv4_launch(kernel, dim3((unsigned)(L.a.groups * L.a.beams) * (unsigned)L.chunks), kBsThreads, 0, st, L.a.use_pdl != 0, L);
+}
 template <bool VEC>
 static int beam_rows_run(const BeamLaunch& L, cudaStream_t st) {
-    auto* kernel = L.per == 32 ? beam_rows_kernel<VEC, 32> : L.per == 16 ? beam_rows_kernel<VEC, 16> : L.per == 8 ? beam_rows_kernel<VEC, 8> : beam_rows_kernel<VEC, 4>;
-    // Few CTAs: shared memory set up as the second kernel needs it, which otherwise waits until it is changed (5 x 12 rows of 50001: 15.7 us, 16.9 without). Many: as much of it for
-    // loads on their way as there is (32 x 8 of 128256: 36.1 us, 39.4 otherwise).
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, L.eager ? cudaSharedmemCarveoutMaxShared : cudaSharedmemCarveoutDefault)) return (int)e;
-    return kv4_launch(kernel, dim3((unsigned)(L.a.groups * L.a.beams) * (unsigned)L.chunks), kBsThreads, 0, st, L.a.use_pdl != 0, L);
+    if (!beam_eager((long long)L.a.groups * L.a.beams * L.chunks)) return beam_rows_launch<VEC, 32, false>(L, st);        // (fewer than 32 logits a thread: fewer than 256 CTAs)
+    return L.per == 32 ? beam_rows_launch<VEC, 32, true>(L, st) : L.per == 16 ? beam_rows_launch<VEC, 16, true>(L, st) : L.per == 8 ? beam_rows_launch<VEC, 8, true>(L, st)
+                                                                                                                                  : beam_rows_launch<VEC, 4, true>(L, st);
 }
 
 }  // namespace tz
@@ -559,7 +568,6 @@ extern "C" int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* 
     L.per = beam_per((int)rows, a.vocab, a.k);
     L.chunks = beam_chunks(L.per, a.vocab);
     L.slots = beam_slots(a.k);
-    L.eager = rows * L.chunks <= 592;                     // one wave (logits of rows that are left out: 32 x 8 beams, one in ten finished: 37.9 us with them, 36.1 without)
     if (rows * L.chunks > 0x7fffffffLL || (long long)L.chunks * L.slots > 0x7fffffffLL || (long long)L.chunks * kBsThreads * L.per > 0x7fffffffLL) return -1;
     if (a.workspace_bytes < tenzo_cuda_beam_select_workspace_bytes(a.groups, a.beams, a.vocab, a.k)) return -1;
     L.parts = static_cast<BeamPart*>(a.workspace);

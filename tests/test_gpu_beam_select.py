@@ -252,3 +252,33 @@ def test_few_numbers_among_nan(cuda_lib, vocab, repeats, beams):
             row[at] = np.round(rng.standard_normal(finite) * 8) / 4
         for k in (8, 24):
             check(logits, (-3 * rng.random(len(logits))).astype(np.float32), beams, k)
+
+
+def test_calls_of_many_and_few_rows_from_two_threads(cuda_lib):
+    """The sizes take kernels of their own, whose settings no other thread's call changes; each thread on its stream."""
+    import threading
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(50)
+    logits = [(rng.standard_normal((rows, 16384)) * 2).astype(np.float32) for rows in (512, 64)]              # 1024 chunks, and 128
+    want = [ref.select(x, np.zeros(len(x), np.float32), 4, 8) for x in logits]
+    d, scores = [dev(x) for x in logits], [torch.zeros(len(x), device="cuda") for x in logits]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    got[i].append(kernels.beam_select(d[i], scores[i], beams=4, k=8, use_pdl=True))
+        except Exception as e:                           # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for i in range(2):
+        for parent, token, _ in got[i]:
+            assert np.array_equal(host(parent), want[i][0]) and np.array_equal(host(token), want[i][1])
