@@ -282,3 +282,25 @@ def test_calls_of_many_and_few_rows_from_two_threads(cuda_lib):
     for i in range(2):
         for parent, token, _ in got[i]:
             assert np.array_equal(host(parent), want[i][0]) and np.array_equal(host(token), want[i][1])
+
+
+@pytest.mark.parametrize("groups,beams,vocab,stride,k", [(32, 8, 20004, 20004, 16), (32, 8, 32772, 32772, 5), (64, 4, 20002, 20016, 8), (10, 30, 16387, 16388, 32), (640, 1, 3001, 3004, 4)])
+def test_many_chunks_of_aligned_rows(cuda_lib, groups, beams, vocab, stride, k):
+    """More CTAs than run at a time, rows that start at 16 bytes: last chunks of a few logits, rows of a wider buffer, vocabularies of any remainder; finished and dead beams, whose rows nothing is
+    stored for, over a workspace of NaN."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(vocab)
+    wide = (rng.standard_normal((groups * beams, stride)) * 2.5).astype(np.float32)
+    wide[:, vocab:] = 1e30                               # (nobody's logits)
+    logits = wide[:, :vocab]
+    logits[:, 7::911] = -np.inf
+    logits[rng.random(logits.shape) < 1e-4] = np.nan
+    scores = (-20 - 3 * rng.random(groups * beams)).astype(np.float32)
+    scores[rng.random(groups * beams) < 0.05] = -np.inf
+    finished = (rng.random(groups * beams) < 0.1).astype(np.int32)
+    finished[-2:] = 1                                    # the last rows of the buffer
+    d = dev(wide)[:, :vocab]
+    got = check(logits, scores, beams, k, finished, 2, logits_dev=d)
+    ws = torch.full((kernels.beam_select_workspace_bytes(groups, beams, vocab, k),), 255, dtype=torch.uint8, device="cuda")
+    again = kernels.beam_select(d, dev(scores), beams=beams, k=k, finished=dev(finished), eos=2, workspace=ws, use_pdl=True)
+    assert all(np.array_equal(x, host(y)) for x, y in zip(got, again))

@@ -217,3 +217,60 @@ def test_errors_of_a_stream_that_is_still_running(cuda_lib):
             call()
         assert kernels.kv4_take_errors() == 2
         assert kernels.kv4_take_errors() == 0
+
+
+@pytest.mark.parametrize("n,n_kv,rotated,offset,broken", [
+    (1185, 8, True, 0, False), (1185, 8, True, 1, True), (9473, 1, True, 0, True), (9473, 1, False, 2, False), (2049, 5, False, 0, True), (9472, 1, True, 4, False), (4001, 3, True, 3, True),
+])
+def test_many_rows(cuda_lib, n, n_kv, rotated, offset, broken):
+    """As many rows and heads as two rows a warp are taken for: odd numbers of them; padding, and indices out of range, in either half of a pair and in the last row; rows of wider buffers, whether they
+    start at 16 bytes or not."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(n + offset)
+    assert n * n_kv >= 9472
+    n_seq, columns = 37, n // 37 // 16 + 2
+    table, pool = setup(rng, n_seq, columns, 2, n_kv)
+    place = rng.permutation(n_seq * columns * 16)[:n]    # no token twice
+    seq, pos = (place // (columns * 16)).astype(np.int32), (place % (columns * 16)).astype(np.int32)
+    pos[rng.random(n) < 0.2] = -1
+    want_pos, cos, sin = pos.copy(), *ref.rope(columns * 16)
+    if broken:
+        bad = rng.choice(n, n // 10, replace=False)
+        bad[0] = n - 1
+        for i, r in enumerate(bad):                      # past the table, no such sequence
+            seq[r], pos[r] = [(0, columns * 16), (n_seq, 3), (-1, 0), (1 << 30, 1 << 30)][i % 4]
+        want_pos[bad] = -1
+        table[5, :] = [-1 if c % 2 else len(pool) for c in range(columns)]
+        want_pos[seq == 5] = -1
+    width = n_kv * 128
+    wide = rng.standard_normal((n, 2 * width + 8 + offset)).astype(np.float32) * 3
+    k, v = wide[:, offset: offset + width], wide[:, offset + width + 4: offset + 4 + 2 * width]
+    d = dev(wide)
+    g = Guarded()
+    d_pool = g.empty(pool.shape, torch.uint8, dev(pool))
+    rope = dict(rope_cos=dev(cos), rope_sin=dev(sin)) if rotated else {}
+    kernels.kv4_append(d[:, offset: offset + width], d[:, offset + width + 4: offset + 4 + 2 * width], d_pool, dev(pos), layer=1, block_table=dev(table), seq=dev(seq), **rope)
+    rows = np.flatnonzero(want_pos >= 0)
+    keys = k.reshape(n, n_kv, 128)[rows]
+    if rotated:
+        keys = ref.rotate(keys, cos[want_pos[rows]][:, None], sin[want_pos[rows]][:, None])
+    want = pool.copy()
+    block, slot = table[seq[rows], want_pos[rows] // 16], want_pos[rows] % 16
+    want[block, 1, :, 0, slot], want[block, 1, :, 1, slot] = ref.quantise(keys), ref.quantise(v.reshape(n, n_kv, 128)[rows])
+    assert np.array_equal(host(d_pool), want)
+    assert kernels.kv4_take_errors() == (2 if broken else 0)
+    back = [g.empty((n, width), torch.float32) for _ in range(2)]
+    for to in back:
+        to.fill_(7.0)
+    apart = torch.full((n, 2 * width + 8 + offset), 7.0, device="cuda")
+    kernels.kv4_read(d_pool, dev(pos), layer=1, block_table=dev(table), seq=dev(seq), k=back[0], v=back[1])
+    kernels.kv4_read(d_pool, dev(pos), layer=1, block_table=dev(table), seq=dev(seq), k=apart[:, offset: offset + width], v=apart[:, offset + width + 4: offset + 4 + 2 * width], use_pdl=True)
+    stored = np.zeros((n, n_kv, 2, 128))
+    stored[rows] = ref.values(want[block, 1, :, :, slot])
+    for i, at in enumerate((offset, offset + width + 4)):
+        assert np.array_equal(host(back[i]), stored[:, :, i].reshape(n, -1).astype(np.float32))
+        assert torch.equal(apart[:, at: at + width], back[i])
+        apart[:, at: at + width] = 7.0
+    assert bool((apart == 7.0).all())
+    assert kernels.kv4_take_errors() == (2 if broken else 0)
+    g.check()
