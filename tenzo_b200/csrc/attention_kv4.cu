@@ -20,10 +20,12 @@
 //     scale of the values seen so far, enter as two parts of eleven bits.
 //   * S = Q K^T has heads as rows, and its accumulators are, lane by lane, the weights' B operand of O^T = V^T P^T, whose columns are heads. Up to four heads a kv
 //     head, columns 4-7 carry the weights' second parts; with five to eight a second MMA does.
-// Outputs agree with 64 bits to a few 1e-7.
+// In fewer bits than fp32: the query (whole numbers of 23 bits of its head's largest), the weights (two parts of eleven bits, cut off) and the centres of the values (two fp16 parts).
+// Outputs differ from 64 bits by 5e-7 to 1e-6 of their norm (1 x 1000 keys 4.7e-7, 256 ragged 6.3e-7, 64 x 8192 8.0e-7, 4 x 16000 9.9e-7; plain fp32 7.5e-7, 1.2e-6, 1.8e-6, 7.9e-7).
 //
-// 64 x 8192 keys of 20/5 heads: 114 us, 420 MB at 3.7 TB/s or 0.56 of the memory's rate. What bounds it is the issue of instructions: some 1100 slots for a step of 32 keys,
-// three quarters of them unpacking, scaling and converting around the 38 MMAs (110 us without the copies, 78 without the MMAs and what they need, 44 without either).
+// 64 x 8192 keys of 20/5 heads: 114 us, 420 MB at 3.7 TB/s or 0.56 of the memory's rate. What takes its time is instructions: some 1100 slots for a step of 32 keys,
+// three quarters of them unpacking, scaling and converting around the 38 MMAs (110 us without the copies, 78 without the MMAs and what they need, 44 without either); 56 % of
+// the issue slots are used, the rest is fixed latencies that three or four warps a scheduler do not cover.
 #include "attn_common.cuh"
 #include "kv4.cuh"
 

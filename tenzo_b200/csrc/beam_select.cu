@@ -1,7 +1,8 @@
 // The k best continuations of a group of beams over beams x vocabulary.
 //
-// score(beam, token) = cum[beam] + (x - log sum exp x), in 64 bits: sums of log-probabilities lie close together between beams, and 32
-// bits would order some of them wrongly (a score of -20 has steps of 2e-6). Within a row the order is that of the logits. Two kernels:
+// score(beam, token) = cum[beam] + (x - log sum exp x), in 64 bits: sums of log-probabilities lie close together between beams, and in 32
+// bits each score would be rounded by itself, to steps of 2e-6 at -20 and of 2e-3 at -30000. Only exponentials have fewer bits (below): their error is one number a row, which moves its
+// tokens together, by some 1e-8. Within a row the order is that of the logits. Two kernels:
 //
 //   1. A CTA takes a chunk of a row, each thread up to 32 logits in registers, read once. The k-th largest of the 256 threads' maxima is a
 //      lower bound of the chunk's k-th largest logit, and hardly more logits reach it: those are listed, and their exponentials are taken and summed
@@ -13,7 +14,7 @@
 //      among one another.
 // Sums are taken in an order that the data alone decides, or as integers, so that equal rows get equal sums and tie.
 //
-// 32 x 8 rows of 128256, k 16: 36.3 us. Loads alone take the first kernel 21 (131 MB at 6.2 TB/s), with everything else in it 29: some eight instructions and an ex2 a
+// 32 x 8 rows of 128256, k 16: 36 us. Loads alone take the first kernel 21 (131 MB at 6.2 TB/s), with everything else in it 29: some eight instructions and an ex2 a
 // logit, and the barriers around the bisection, are hidden by the other CTAs' loads for two thirds only. The second kernel is 7, a chain of some 10 000 cycles.
 #include "common.cuh"
 #include "kv4.cuh"

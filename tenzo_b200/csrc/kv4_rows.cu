@@ -6,7 +6,7 @@
 // fp32 in the order the header gives (a code next to a border must not depend on who computes it); only the two parameters are
 // rounded further, to fp16: at 32 dims a pair a third format of 32 bits would cost 10 % of the cache's bytes.
 // 1024 bytes in and 160 out a row and head: 8 x 1000 ragged rows of 8 heads 20.6 us, 14 of which are the loads alone; the quantiser's 150 instructions a row are the rest, the
-// stores cost nothing. (Registers for ten CTAs an SM: 20.6 us, as many as the compiler likes 21.3.) Read: 16.9 us, bound by memory.
+// stores cost nothing. (Registers for ten CTAs an SM: 20.6 us, as many as the compiler likes 21.3.) Read: 16.9 us, 0.6 of the memory's rate, nearly all of it stores.
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>
@@ -276,8 +276,11 @@ static bool rows_args(const tenzo_kv4_cache* cache, int layer, int kv_stride, co
     return true;
 }
 
-// Rows a warp takes: two where that still leaves every SM 16 warps (their loads are in flight together: read of 8000 rows of 8 heads 16.9 us, by ones 22.2; append
-// of 1537 rows of 5 heads 4.2 and 4.4), else one.
+// Rows a warp takes: two (their loads are in flight together) where that leaves every SM 32 warps, else one. Rows x heads by ones and by twos, over more than L2 holds, us:
+//            1537 x 5    1184 x 8    1600 x 8     3200 x 8     8000 x 8     20000 x 8
+//   append   5.5, 5.6    6.5, 6.0    7.2, 7.8    11.1, 11.3   23.0, 22.2   53.8, 50.6
+//   read     5.4, 4.9    6.3, 5.5    6.7, 5.9    10.1, 8.7    22.0, 17.3   53.4, 38.9
+// Reads gain on either side of the border, 9472; appends lose a little in places up to some 40000 and gain above.
 static int rows_a_warp(int rows, int n_kv) { return (long long)rows * n_kv >= 4LL * 148 * 16 ? 2 : 1; }
 static dim3 rows_grid(int rows, int n_kv, int r) { return dim3((unsigned)((((long long)rows + r - 1) / r * n_kv + kRowWarps - 1) / kRowWarps)); }
 
