@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kA4Threads, kA4Resident) attention_kv4_kernel(
         __syncwarp();                                    // every lane is done with the stage and the scales
         if (k + kA4Stages < my_steps) issue(k + kA4Stages);
     }
-    if (gave_up && lane == 0) atomicOr(&g_kv4_attention_error, kK4ErrWait);
+    if (gave_up) atomicOr(&g_kv4_attention_error, kK4ErrWait);                                // (any lane: each waits for itself)
     float l_run, l_other;
     unpack2(l_pair, l_run, l_other);
     l_run += l_other;
