@@ -241,6 +241,7 @@ TENZO_API int tenzo_cuda_topk_max_candidates(void);
  * No counterpart in the reference (its caches hold 8 bits). Pool: uint8 [block][layer][kv_head][K, V][16 slots][80], 16-byte
  * aligned. A row is 64 bytes of codes - dim d in nibble d % 2 of byte d / 2, the low nibble first - and four pairs (scale, minimum)
  * of fp16, one for each 32 dims; a value is minimum + scale * code. 160 bytes a token and kv head (the INT8 caches: 264).
+ * A pool that tenzo_cuda_kv4_append did not fill has finite parameters too, and |minimum + 8 scale| <= 65504: the attention holds that sum in fp16 parts.
  * Token t of table row s lives in block block_table[s * table_stride + t / 16], slot t % 16. head_dim is 128.
  *
  * A position outside its range, a table row outside [0, table_rows) or a table entry outside [0, n_blocks) touches no memory: that row is

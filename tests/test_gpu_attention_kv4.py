@@ -387,3 +387,23 @@ def test_clusters_of_every_size(cuda_lib, rows, n_q, n_kv, splits):
     assert (host(out)[-1] == 7.0).all()
     g.check()
     assert kernels.kv4_take_errors() == 2
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(4, 2), (8, 1)])
+def test_values_at_the_ends_of_fp16(cuda_lib, n_q, n_kv):
+    """Groups of 65504 alone, of -65504 alone, from one to the other, and clamped ones, as the quantiser leaves them: nothing overflows."""
+    from tenzo_b200 import kernels
+    rng = np.random.default_rng(n_q)
+    n, columns = 250, 16
+    x = np.clip(rng.standard_normal((columns, 1, n_kv, 2, 16, 128)) * 4e4, -65504, 65504).astype(np.float32)
+    x[:, :, :, 0] = rng.standard_normal(x[:, :, :, 0].shape)                # keys of ordinary size
+    some = rng.integers(0, 4, (columns, 1, n_kv, 16))
+    x[:, :, :, 1][some == 0], x[:, :, :, 1][some == 1] = 65504, -65504
+    x[:, :, :, 1, :, 96:] = 65504                                           # a group that no key leaves
+    pool, table = ref.quantise(x), rng.permutation(columns).astype(np.int32)[None]
+    q, pos = rng.standard_normal((1, n_q * 128)).astype(np.float32), np.array([n - 1], np.int32)
+    out = kernels.attention_kv4(dev(q), dev(pool), dev(pos), layer=0, n_q=n_q, block_table=dev(table))
+    k, v = ref.cached(pool, 0, table[0], n)
+    want, bound = ref.attention(q[0].reshape(n_q, 128), k, v)
+    err = abs(host(out)[0].reshape(n_q, 128).astype(np.float64) - want)
+    assert (err <= bound).all(), float((err / bound).max())
