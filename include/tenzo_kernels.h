@@ -335,6 +335,103 @@ typedef struct {
 TENZO_API int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* stream);
 TENZO_API size_t tenzo_cuda_beam_select_workspace_bytes(int groups, int beams, int vocab, int k);
 
+/* ---- INT8 caches: drafted trees, and caches of a bounded number of tokens ---------------------------------
+ * No counterpart in the reference, which decodes one token at a time and keeps every token. The caches are those of tenzo_cuda_attention_int8: int8
+ * [block][n_layers][n_kv][slots][128] for keys and for values and fp32 scales [block][n_layers][n_kv][slots] (a value is code * scale). The token at place t of table
+ * row s lies in block block_table[s * table_stride + t / slots], slot t % slots; slots is a multiple of 16. The paged_int8 pools have 16 slots; the contiguous
+ * cache [sequence][layer][kv_head][max_seq][128] is a pool of max_seq slots a block whose table has one entry a sequence. Caches and scales are 16-byte aligned and
+ * hold fewer than 2^31 rows; scales are not negative. head_dim is 128.
+ *
+ * Here a token's place is not its rotary position: nodes of a tree that lie side by side have the same position, and behind an eviction positions and places
+ * come apart for good. Calls that rotate take both.
+ * An index out of range (a place, a position, a table row or entry, a length) touches no memory: that row is left out and a flag is raised, which
+ * tenzo_cuda_kv8_take_errors() returns and clears. Calls on one device share the flags only. */
+typedef struct {
+    int8_t* k; int8_t* v;
+    float* scale_k; float* scale_v;
+    int n_blocks, n_layers, n_kv, slots;
+    const int* block_table;  /* device int32 [table_rows][table_stride] */
+    int table_rows, table_stride;
+} tenzo_kv8_cache;
+enum { TENZO_TREE_MOST = 256 };  /* nodes of a tree */
+
+/* Stores `rows` rows of keys and values: k, v [rows][kv_stride] fp32 (n_kv*128 used, kv_stride >= n_kv*128), row i at place place[i] of table row seq[i]
+ * (seq NULL: table row i). place[i] < 0 marks padding: nothing is stored. No two rows of a call may name the same token. Keys are rotated at rope_pos[i] (NULL: place[i];
+ * tables [rope_len][64], position < rope_len; both NULL: no rotation) as tenzo_cuda_attention_int8 does, then both are quantised: scale = max(max|x|, 1e-8) * (1/127),
+ * code = clamp(round(x * (1 / scale)), -128, 127), halves away from zero, each step rounded to fp32. (tenzo_cuda_attention_int8 divides by 127: its scales may differ in
+ * the last bit, and a code next to a border by one.) Values have to be finite.
+ * weight, position (either may be NULL), laid out as the scales: receive 0 and the row's rotary position, for the calls below. */
+TENZO_API int tenzo_cuda_kv8_append(const tenzo_kv8_cache* cache, int layer, const float* k, const float* v, int kv_stride, const int* place, const int* seq, int rows,
+                                    const int* rope_pos, const float* rope_cos, const float* rope_sin, int rope_len, float* weight, int* position, int use_pdl,
+                                    void* stream);
+
+/* Attention of the nodes of a tree, for each of `sequences` trees of up to `nodes` nodes (1 .. TENZO_TREE_MOST): sequence s holds start[s] tokens, and node i's key and
+ * value are stored at place start[s] + i already. Node i sees places 0 .. start[s] - 1, and node j if bit j % 32 of mask[(s*nodes + i)*mask_stride + j / 32] is
+ * set (itself too: any bits will do). mask NULL: nodes 0 .. i, a chain (a prompt's next rows, one decoded token with nodes = 1). count[s] (NULL: nodes): nodes that
+ * are there; the others are padding, are seen by none, and their rows of out are zeros. start[s] < 0: the whole sequence is padding.
+ *   out[s*nodes + i] = softmax(q K^T / sqrt(128)) V per query head h, over kv head h / (n_q / n_kv), the query rotated at rope_pos[s*nodes + i] (NULL: start[s] + i);
+ *   lse = log sum exp of the arguments (natural logarithm; -infinity and zeros in out where nothing is seen).
+ * Sums and softmax in fp32 or whole numbers; the query is rounded to 23 bits of its head's largest number, the weights to 24 bits or more of their row's largest so far: outputs agree with
+ * 64 bits to about 1e-6 of their norm. A NaN or an infinity in a head's query makes that head's outputs NaN; what lies in places that are not seen has no part.
+ * A sequence with start + count > max_len or a table row out of range, and a row whose position is, are not written and raise the flag; a table entry out
+ * of range leaves its block's keys out and raises it. */
+typedef struct {
+    const float* q;          /* [sequences*nodes][q_stride], n_q*128 used, before rotation */
+    float* out;              /* [sequences*nodes][n_q*128] */
+    float* lse;              /* [sequences*nodes][n_q], or NULL */
+    tenzo_kv8_cache cache;
+    const int* start;        /* [sequences] device */
+    const int* count;        /* [sequences] device, or NULL */
+    const int* seq;          /* [sequences] device: table rows, or NULL: table row s */
+    const int* mask;         /* [sequences*nodes][mask_stride] device, or NULL */
+    const int* rope_pos;     /* [sequences*nodes] device, or NULL */
+    const float* rope_cos; const float* rope_sin;   /* [rope_len][64]; both NULL: no rotation */
+    int rope_len;
+    int q_stride;            /* floats between rows; 0 = n_q*128 */
+    int mask_stride;         /* words between rows; 0 = ceil(nodes / 32) */
+    int layer, n_q, sequences, nodes;
+    int max_len;             /* upper bound on start + count (sizes the grid); at most slots * table_stride */
+    int split_keys;          /* keys a CTA takes (rounded up to 128); 0 = choose */
+    int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
+    void* workspace;         /* 16-byte aligned, contents need not be kept: partial results of splits; NULL: none */
+    size_t workspace_bytes;  /* sequences * nodes * n_q * 520 a split; with less fewer splits are taken, and split_keys that need more are refused (-1). Enough for any
+                                split_keys: tenzo_cuda_attention_tree_workspace_bytes(...); for split_keys 0: 520 * sequences * nodes * n_q *
+                                tenzo_cuda_attention_tree_splits(...), nothing at 1 */
+} tenzo_attention_tree_args;
+TENZO_API int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, void* stream);
+TENZO_API size_t tenzo_cuda_attention_tree_workspace_bytes(int sequences, int nodes, int n_q, int max_len);
+/* Splits that the call's own choice (split_keys 0) wants room for; 1: none, 0: arguments that the call refuses. */
+TENZO_API int tenzo_cuda_attention_tree_splits(int sequences, int nodes, int n_q, int n_kv, int max_len);
+
+/* The attention weight that each cached token receives: weight[token] += sum over the nodes that see it and the query heads of its kv head of exp(s - lse), s the
+ * argument of softmax above. args as for tenzo_cuda_attention_tree, whose lse this reads; out, workspace and split_keys are not used. weight is laid out as the scales.
+ * A row whose lse is not finite adds nothing. Every sum is taken in one order: equal calls give equal bits. No two sequences of a call may name the same table row. */
+TENZO_API int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float* weight, void* stream);
+
+/* Cuts caches back to `keep` tokens, for each layer and kv head on its own: table rows seq[s] (NULL: s) hold length[s] tokens at places 0 .. length[s] - 1, with the
+ * weight and position that tenzo_cuda_kv8_append and _weigh left. Where length[s] > keep, the `keep` heaviest stay; a token whose position is protect_from[s] or more counts as
+ * infinitely heavy (protect_from NULL: none does), NaN as -infinity, and of equal weights the lower place stays. Tokens that stay keep their places if those are below `keep`; the others
+ * move, in the order of their places, to the places below `keep` that became free, in the order of those, with scales, weight and position. (Order means nothing to
+ * attention over rotated keys: it takes one row's move a token evicted, not the whole cache's.) length_out[s] = min(length[s], keep), in
+ * memory of its own. No two sequences of a call may name the same table row.
+ * A negative length, one above max_len or a table row out of range leaves the sequence as it is, length_out with it, and raises the flag; a table entry out of range leaves all of
+ * the sequence's rows in their places, and raises it. max_len <= slots * table_stride; max_len <= 2^20 and sequences <= 65535 (-5 otherwise). */
+TENZO_API int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight, int* position, const int* length, const int* seq, const int* protect_from, int sequences,
+                                   int keep, int max_len, int* length_out, int use_pdl, void* stream);
+
+/* The nodes of drafted trees that the model agrees with, and their rows moved up behind the cached ones. token, parent, chosen [sequences][nodes]: node i's token, the node it
+ * goes on from (below i; node 0 is the root, a token that counts already), and the token that the model chose after node i (its argmax, or a draw). From the root, the next node is the first whose
+ * parent is the present one and whose token is the one chosen there, until there is none. path [sequences][nodes]: these nodes, root first, then -1; accepted[s]: how many; next[s]: the token
+ * chosen after the last. Row d of a path is moved from place start[s] + path[d] to start[s] + d in all layers, with scales and weight and position (either may be NULL).
+ * count, seq, start as for tenzo_cuda_attention_tree. A sequence of padding (start[s] < 0 or count[s] = 0) has accepted 0, next -1. So has one with start + count above slots * table_stride, with count
+ * out of range or a table row out of range, which raises the flag; a table entry out of range leaves the rows that need it where they are, and raises it. No two sequences of a call may
+ * name the same table row; sequences <= 65535, nodes <= TENZO_TREE_MOST (-5 otherwise). */
+TENZO_API int tenzo_cuda_kv8_accept(const tenzo_kv8_cache* cache, const int* token, const int* parent, const int* chosen, const int* start, const int* count, const int* seq,
+                                    int sequences, int nodes, int* accepted, int* next, int* path, float* weight, int* position, int use_pdl, void* stream);
+/* Error flags of the calls of this section since the last call (bit 0: a bounded wait was given up, bit 1: an index out of range); -1 if the query failed, which leaves the
+ * flags as they are. Synchronises with the device: waits for all of its streams, so it cannot be called while one is captured. */
+TENZO_API int tenzo_cuda_kv8_take_errors(void);
+
 /* ---- INT8 embedding row dequantisation ---------------------------------------------------------
  * Replaces embedding_lookup's int8 branch (:1299-1315): x = (float)W8[tok] * scale[tok].
  * vocab > 0: token ids outside [0, vocab) are read as row 0 rather than past the table; 0 = unchecked. */

@@ -1,0 +1,451 @@
+// Rows of the INT8 caches (kv8.cuh): storing them at places of their own, the accepted nodes of drafted trees, and the eviction of the tokens that received
+// least attention.
+#include "attn_common.cuh"
+#include "kv8.cuh"
+
+namespace tz {
+
+__device__ int g_kv8_rows_error = 0;
+int* kv8_rows_flags() {
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, g_kv8_rows_error) == cudaSuccess ? static_cast<int*>(p) : nullptr;
+}
+
+// ---- append ----------------------------------------------------------------------------------------------------------------
+// A warp takes one kv head of one row: lanes 0-15 the key, 16-31 the value, dims 4l .. 4l + 3 and 64 more a lane, so that the pairs that the
+// rotation turns lie in one lane.
+constexpr int kK8RowWarps = 4;
+
+struct K8RowsArgs {
+    tenzo_kv8_cache c;
+    int layer, rows, kv_stride, rope_len, use_pdl;
+    const int *place, *seq, *rope_pos;
+    const float *k, *v, *cs, *sn;
+    float* weight;
+    int* position;
+};
+
+template <bool VEC>
+__device__ __forceinline__ void k8_load4(const float* p, float* x) {
+    if (VEC) {
+        const float4 v = ld_l2(reinterpret_cast<const float4*>(p));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = ld_l2(p + j);
+    }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kK8RowWarps * 32) kv8_append_kernel(const K8RowsArgs a) {
+    const int lane = threadIdx.x & 31, is_v = lane >> 4, l = lane & 15;
+    const long long unit = (long long)blockIdx.x * kK8RowWarps + (threadIdx.x >> 5);
+    const int kvh = (int)(unit % a.c.n_kv);
+    const long long row = unit / a.c.n_kv;
+    if (a.use_pdl) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
+    if (row >= a.rows) return;
+    const int place = ld_l2(a.place + row), seq = a.seq ? ld_l2(a.seq + row) : (int)row, pos = a.rope_pos ? ld_l2(a.rope_pos + row) : place;
+    float x[8], c[4], s[4];
+    const float* p = (is_v ? a.v : a.k) + (size_t)row * a.kv_stride + kvh * kK8Hd + 4 * l;
+    k8_load4<VEC>(p, x);
+    k8_load4<VEC>(p + 64, x + 4);
+    if (place < 0) return;
+    bool there = seq >= 0 && seq < a.c.table_rows && place / a.c.slots < a.c.table_stride && (!a.cs || (pos >= 0 && pos < a.rope_len));
+    const int block = there ? kv8_block(a.c, seq, place) : -1;
+    if (block < 0) {
+        if (lane == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
+        return;
+    }
+    if (a.cs && !is_v) {
+        k8_load4<true>(a.cs + (size_t)pos * 64 + 4 * l, c);
+        k8_load4<true>(a.sn + (size_t)pos * 64 + 4 * l, s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rope_rotate(x[j], x[4 + j], true, c[j], s[j], x[j], x[4 + j]);
+    }
+    float amax = 1e-8f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float scale = amax * (1.0f / 127.0f), inv = 1.0f / scale;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float q = fminf(fmaxf(roundf(x[j] * inv), -128.0f), 127.0f);
+        w[j >> 2] |= ((uint32_t)(int)q & 255u) << (8 * (j & 3));
+    }
+    const size_t at = kv8_row(a.c, a.layer, kvh, block, place % a.c.slots);
+    uint32_t* to = reinterpret_cast<uint32_t*>((is_v ? a.c.v : a.c.k) + at * kK8Hd);
+    to[l] = w[0];
+    to[16 + l] = w[1];
+    if (l == 0) (is_v ? a.c.scale_v : a.c.scale_k)[at] = scale;
+    if (lane == 1 && a.weight) a.weight[at] = 0.0f;
+    if (lane == 2 && a.position) a.position[at] = pos;
+}
+
+// ---- moving rows: half a warp takes one row, sixteen bytes a lane, keys and values; four lanes take what is beside them ------------------------
+struct K8Row {
+    uint4 code;
+    uint32_t beside;
+};
+__device__ __forceinline__ uint32_t* k8_beside(const tenzo_kv8_cache& c, float* weight, int* position, int which) {
+    return which == 0 ? reinterpret_cast<uint32_t*>(c.scale_k) : which == 1 ? reinterpret_cast<uint32_t*>(c.scale_v) : which == 2 ? reinterpret_cast<uint32_t*>(weight)
+         : which == 3 ? reinterpret_cast<uint32_t*>(position) : nullptr;
+}
+__device__ __forceinline__ void k8_take(const tenzo_kv8_cache& c, const uint32_t* beside, size_t row, int l, K8Row& r) {
+    r.code = ld_l2(reinterpret_cast<const uint4*>((l & 8 ? c.v : c.k) + row * kK8Hd) + (l & 7));
+    if (beside) r.beside = ld_l2(beside + row);
+}
+__device__ __forceinline__ void k8_put(const tenzo_kv8_cache& c, uint32_t* beside, size_t row, int l, const K8Row& r) {
+    reinterpret_cast<uint4*>((l & 8 ? c.v : c.k) + row * kK8Hd)[l & 7] = r.code;
+    if (beside) beside[row] = r.beside;
+}
+
+// ---- accepted nodes ------------------------------------------------------------------------------------------------------------
+constexpr int kAcThreads = 256, kAcHalves = kAcThreads / 16, kAcBatch = 4;     // rows in flight a half warp
+
+struct AcceptArgs {
+    tenzo_kv8_cache c;
+    const int *token, *parent, *chosen, *start, *count, *seq;
+    int *accepted, *next, *path;
+    float* weight;
+    int* position;
+    int nodes, units, use_pdl;                           // (layer, kv head) pairs a CTA takes
+};
+
+__global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs a) {
+    __shared__ int s_next[TENZO_TREE_MOST], s_token[TENZO_TREE_MOST], s_chosen[TENZO_TREE_MOST], s_path[TENZO_TREE_MOST + 1];
+    __shared__ int2 s_at[TENZO_TREE_MOST][2];            // (block, slot) of a row's old place and of its new one
+    __shared__ int s_n;
+    const int tid = threadIdx.x, s = blockIdx.y;
+    if (a.use_pdl) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
+    const int start = ld_l2(a.start + s), count = a.count ? ld_l2(a.count + s) : a.nodes, seq = a.seq ? ld_l2(a.seq + s) : s;
+    const bool padding = start < 0 || count == 0;
+    const bool refused = !padding && (count < 0 || count > a.nodes || seq < 0 || seq >= a.c.table_rows || (long long)start + count > min((long long)a.c.table_stride * a.c.slots, 0x7fffffffLL));
+    if (refused && tid == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
+    const int n = padding || refused ? 0 : count;
+    int parent = -1;
+    if (tid < n) {
+        s_token[tid] = ld_l2(a.token + (size_t)s * a.nodes + tid);
+        s_chosen[tid] = ld_l2(a.chosen + (size_t)s * a.nodes + tid);
+        parent = ld_l2(a.parent + (size_t)s * a.nodes + tid);
+        s_next[tid] = 0x7fffffff;
+    }
+    __syncthreads();
+    if (tid < n && parent >= 0 && parent < tid && s_token[tid] == s_chosen[parent]) atomicMin(&s_next[parent], tid);     // the first that fits
+    __syncthreads();
+    if (tid == 0) {
+        int m = 0;
+        for (int i = 0; m < n && i < n; i = s_next[i]) s_path[m++] = i;       // (indices grow: it ends)
+        s_n = m;
+    }
+    __syncthreads();
+    const int m = s_n;
+    if (blockIdx.x == 0) {
+        for (int i = tid; i < a.nodes; i += kAcThreads) a.path[(size_t)s * a.nodes + i] = i < m ? s_path[i] : -1;
+        if (tid == 0) {
+            a.accepted[s] = m;
+            a.next[s] = m ? s_chosen[s_path[m - 1]] : -1;
+        }
+    }
+    int first = 0;                                       // rows in front of it are in their places
+    if (tid < m) {
+        const int from = start + s_path[tid], to = start + tid;
+        int2 x = make_int2(-1, 0), y = x;
+        if (from != to) {
+            x = make_int2(kv8_block(a.c, seq, from), from % a.c.slots);
+            y = make_int2(kv8_block(a.c, seq, to), to % a.c.slots);
+            if ((x.x < 0 || y.x < 0) && blockIdx.x == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
+        }
+        s_at[tid][0] = x;
+        s_at[tid][1] = y;
+    }
+    first = __syncthreads_count(tid < m && s_path[tid] == tid);
+    const int rows = m - first;
+    if (rows == 0) return;
+    // Row d goes from a node's place to one that is not behind it, and no later row comes from a place in front of its own number: rows are taken in their order,
+    // kAcHalves * kAcBatch at a time, and all of those are loaded before the first is stored.
+    const int unit0 = blockIdx.x * a.units, units = min(a.units, a.c.n_layers * a.c.n_kv - unit0), half = tid >> 4, l = tid & 15;
+    uint32_t* beside = k8_beside(a.c, a.weight, a.position, l);
+    for (int e0 = 0; e0 < units * rows; e0 += kAcHalves * kAcBatch) {
+        K8Row r[kAcBatch];
+        size_t to[kAcBatch];
+        bool moves[kAcBatch];
+#pragma unroll
+        for (int b = 0; b < kAcBatch; ++b) {
+            const int e = e0 + b * kAcHalves + half;
+            moves[b] = e < units * rows;
+            if (moves[b]) {
+                const int unit = unit0 + e / rows, d = first + e % rows, layer = unit / a.c.n_kv, kvh = unit % a.c.n_kv;
+                const int2 x = s_at[d][0], y = s_at[d][1];
+                moves[b] = x.x >= 0 && y.x >= 0;
+                if (moves[b]) {
+                    k8_take(a.c, beside, kv8_row(a.c, layer, kvh, x.x, x.y), l, r[b]);
+                    to[b] = kv8_row(a.c, layer, kvh, y.x, y.y);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < kAcBatch; ++b)
+            if (moves[b]) k8_put(a.c, beside, to[b], l, r[b]);
+    }
+}
+
+// ---- eviction -------------------------------------------------------------------------------------------------------------------
+// One CTA a (sequence, layer, kv head). The weights become whole numbers of the same order (the protected tokens' the largest) in shared memory; the `keep`-th largest is found by
+// counting, two bits a round; what stays is a bit a token; and the free places and the tokens that move into them are two lists, the i-th goes to the i-th.
+// Nothing that moves comes from a place that another moves to (those are below `keep`, these are not), so all rows move at once.
+constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32, kEvBatch = 4;
+constexpr int kEvHeld = 48 * 1024;                       // tokens whose numbers fit in shared memory
+constexpr int kEvMost = 1 << 20, kEvLists = 16 * 1024;   // tokens at most, and entries of both lists together where the numbers do not fit
+
+struct EvictArgs {
+    tenzo_kv8_cache c;
+    float* weight;
+    int* position;
+    const int *length, *seq, *protect_from;
+    int* length_out;
+    int keep, max_len, use_pdl;
+};
+
+// A number whose order is the weight's: NaN as -infinity, -0 as +0.
+__device__ __forceinline__ uint32_t ev_number(float w) {
+    w = w == w ? w + 0.0f : -INFINITY;
+    const uint32_t u = __float_as_uint(w);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// HELD: the numbers are kept in shared memory; otherwise they are read again each time, and the lists are made a part at a time.
+template <bool HELD>
+__global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a) {
+    extern __shared__ uint32_t ev_smem[];
+    __shared__ uint32_t s_count[2][kEvWarps][4];
+    __shared__ int s_warp[3][kEvWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.y, layer = blockIdx.x / a.c.n_kv, kvh = blockIdx.x % a.c.n_kv;
+    if (a.use_pdl) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
+    const int n = ld_l2(a.length + s), seq = a.seq ? ld_l2(a.seq + s) : s;
+    const bool refused = n < 0 || n > a.max_len || seq < 0 || seq >= a.c.table_rows;
+    if (refused || n <= a.keep) {
+        if (tid == 0 && blockIdx.x == 0) a.length_out[s] = n;
+        if (tid == 0 && refused) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
+        return;
+    }
+    const int from = a.protect_from ? ld_l2(a.protect_from + s) : 0;
+    const int words = (n + 31) / 32, chunks = (words + kEvWarps - 1) / kEvWarps;       // of the bits; a warp's share of them
+    uint32_t* s_keep = ev_smem;                          // [words]: what stays
+    uint32_t* s_num = ev_smem + (a.max_len + 31) / 32;   // [n], HELD only; later the two lists
+    bool bad = false;
+    auto load = [&](int t) -> uint32_t {
+        const int block = kv8_block(a.c, seq, t);
+        if (block < 0) {
+            bad = true;
+            return 0;
+        }
+        const size_t row = kv8_row(a.c, layer, kvh, block, t % a.c.slots);
+        return a.protect_from && ld_l2(a.position + row) >= from ? ev_number(INFINITY) : ev_number(ld_l2(a.weight + row));
+    };
+    uint32_t lo = 0xffffffffu, hi = 0;
+    for (int t = tid; t < n; t += kEvThreads) {
+        const uint32_t u = load(t);
+        if (HELD) s_num[t] = u;
+        lo = min(lo, u);
+        hi = max(hi, u);
+    }
+    if (tid == 0 && blockIdx.x == 0) a.length_out[s] = a.keep;
+    if (__syncthreads_or(bad)) {
+        if (tid == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
+        return;
+    }
+    auto number = [&](int t) { return HELD ? s_num[t] : load(t); };
+    // The largest number that `keep` tokens reach: bits from the top, those that all numbers share first.
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+        s_count[0][warp][0] = lo;
+        s_count[0][warp][1] = hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kEvWarps; ++w) {
+        lo = min(lo, s_count[0][w][0]);
+        hi = max(hi, s_count[0][w][1]);
+    }
+    int bits = 32 - __clz((int)(lo ^ hi));               // (0: all are equal)
+    bits += bits & 1;
+    uint32_t border = bits >= 32 ? 0u : lo >> bits << bits;
+    int above = 0;                                       // tokens over the border's present range
+    int round = 1;
+    while (bits > 0) {
+        bits -= 2;
+        const uint32_t t1 = border + (1u << bits), t2 = border + (2u << bits), t3 = border + (3u << bits);
+        int c1 = 0, c2 = 0, c3 = 0;
+        for (int t = tid; t < n; t += kEvThreads) {
+            const uint32_t u = number(t);
+            c1 += u >= t1;
+            c2 += u >= t2;
+            c3 += u >= t3;
+        }
+        c1 = __reduce_add_sync(0xffffffffu, c1);
+        c2 = __reduce_add_sync(0xffffffffu, c2);
+        c3 = __reduce_add_sync(0xffffffffu, c3);
+        uint32_t(*sc)[4] = s_count[round & 1];
+        if (lane == 0) {
+            sc[warp][0] = c1;
+            sc[warp][1] = c2;
+            sc[warp][2] = c3;
+        }
+        __syncthreads();
+        c1 = c2 = c3 = 0;
+#pragma unroll
+        for (int w = 0; w < kEvWarps; ++w) {
+            const uint4 v = *reinterpret_cast<const uint4*>(sc[w]);
+            c1 += v.x;
+            c2 += v.y;
+            c3 += v.z;
+        }
+        if (c3 >= a.keep) border = t3;
+        else if (c2 >= a.keep) border = t2, above = c3;
+        else if (c1 >= a.keep) border = t1, above = c2;
+        else above = c1;
+        ++round;
+    }
+    // `above` are over the border; of those that equal it the first `keep - above` stay too. (With all bits found, `above` is right: it was counted in the last round
+    // that had some over the border's range; before that none were.)
+    const int equal = a.keep - above;
+    const int w0 = warp * chunks, w1 = min(words, w0 + chunks);
+    int mine = 0;                                        // equal ones in the warp's share
+    for (int w = w0; w < w1; ++w) {
+        const int t = 32 * w + lane;
+        mine += __popc(__ballot_sync(0xffffffffu, t < n && number(t) == border));
+    }
+    if (lane == 0) s_warp[0][warp] = mine;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < warp; ++w) before += s_warp[0][w];
+    int holes = 0, far = 0;
+    for (int w = w0; w < w1; ++w) {
+        const int t = 32 * w + lane;
+        const uint32_t u = t < n ? number(t) : 0;
+        const unsigned same = __ballot_sync(0xffffffffu, t < n && u == border);
+        const bool stays = t < n && (u > border || (u == border && before + __popc(same & ((1u << lane) - 1)) < equal));
+        before += __popc(same);
+        const unsigned keep = __ballot_sync(0xffffffffu, stays);
+        holes += __popc(__ballot_sync(0xffffffffu, t < a.keep && !stays));
+        far += __popc(__ballot_sync(0xffffffffu, t >= a.keep && stays));
+        if (lane == 0) s_keep[w] = keep;
+    }
+    if (lane == 0) {
+        s_warp[1][warp] = holes;
+        s_warp[2][warp] = far;
+    }
+    __syncthreads();                                     // the numbers are no longer needed
+    int hole_at = 0, far_at = 0, moves = 0;
+    for (int w = 0; w < kEvWarps; ++w) {
+        if (w < warp) {
+            hole_at += s_warp[1][w];
+            far_at += s_warp[2][w];
+        }
+        moves += s_warp[1][w];
+    }
+    const int half = tid >> 4, l = tid & 15;
+    uint32_t* beside = k8_beside(a.c, a.weight, a.position, l);
+    const int room = HELD ? moves : kEvLists / 2;         // entries of a list
+    uint32_t *s_hole = s_num, *s_far = s_num + room;
+    for (int part = 0; part < moves; part += room) {
+        int h = hole_at, f = far_at;
+        for (int w = w0; w < w1; ++w) {
+            const int t = 32 * w + lane;
+            const bool stays = t < n && (s_keep[w] >> lane & 1);
+            const unsigned hm = __ballot_sync(0xffffffffu, t < a.keep && !stays), fm = __ballot_sync(0xffffffffu, t >= a.keep && stays), below = (1u << lane) - 1;
+            const int hi_ = h + __popc(hm & below) - part, fi = f + __popc(fm & below) - part;
+            if ((hm >> lane & 1) && hi_ >= 0 && hi_ < room) s_hole[hi_] = t;
+            if ((fm >> lane & 1) && fi >= 0 && fi < room) s_far[fi] = t;
+            h += __popc(hm);
+            f += __popc(fm);
+        }
+        __syncthreads();
+        const int these = min(room, moves - part);
+        for (int i0 = half; i0 < these; i0 += kEvThreads / 16 * kEvBatch) {
+            K8Row r[kEvBatch];
+#pragma unroll
+            for (int b = 0; b < kEvBatch; ++b) {
+                const int i = i0 + b * (kEvThreads / 16);
+                if (i < these) {
+                    const int t = s_far[i];
+                    k8_take(a.c, beside, kv8_row(a.c, layer, kvh, kv8_block(a.c, seq, t), t % a.c.slots), l, r[b]);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < kEvBatch; ++b) {
+                const int i = i0 + b * (kEvThreads / 16);
+                if (i < these) {
+                    const int t = s_hole[i];
+                    k8_put(a.c, beside, kv8_row(a.c, layer, kvh, kv8_block(a.c, seq, t), t % a.c.slots), l, r[b]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace tz
+
+extern "C" int tenzo_cuda_kv8_append(const tenzo_kv8_cache* cache, int layer, const float* k, const float* v, int kv_stride, const int* place, const int* seq, int rows,
+                                     const int* rope_pos, const float* rope_cos, const float* rope_sin, int rope_len, float* weight, int* position, int use_pdl, void* stream) {
+    using namespace tz;
+    if (!cache || !kv8_cache_ok(*cache) || layer < 0 || layer >= cache->n_layers || rows < 0) return -1;
+    if (rows == 0) return 0;
+    if (!k || !v || !place || kv_stride < (long long)cache->n_kv * kK8Hd || (!seq && rows > cache->table_rows)) return -1;
+    if ((rope_cos == nullptr) != (rope_sin == nullptr) || (rope_cos && (rope_len <= 0 || !kv8_aligned(rope_cos, 16) || !kv8_aligned(rope_sin, 16)))) return -1;
+    const long long ctas = ((long long)rows * cache->n_kv + kK8RowWarps - 1) / kK8RowWarps;
+    if (ctas > 0x7fffffffLL) return -5;
+    K8RowsArgs a = {*cache, layer, rows, kv_stride, rope_len, use_pdl, place, seq, rope_pos, k, v, rope_cos, rope_sin, weight, position};
+    const bool vec = kv8_aligned(k, 16) && kv8_aligned(v, 16) && kv_stride % 4 == 0;
+    return kv4_launch(vec ? kv8_append_kernel<true> : kv8_append_kernel<false>, dim3((unsigned)ctas), kK8RowWarps * 32, 0, static_cast<cudaStream_t>(stream), use_pdl != 0, a);
+}
+
+extern "C" int tenzo_cuda_kv8_accept(const tenzo_kv8_cache* cache, const int* token, const int* parent, const int* chosen, const int* start, const int* count, const int* seq,
+                                     int sequences, int nodes, int* accepted, int* next, int* path, float* weight, int* position, int use_pdl, void* stream) {
+    using namespace tz;
+    if (!cache || !kv8_cache_ok(*cache) || sequences < 0) return -1;
+    if (sequences == 0) return 0;
+    if (!token || !parent || !chosen || !start || !accepted || !next || !path || nodes <= 0 || (!seq && sequences > cache->table_rows)) return -1;
+    if (nodes > TENZO_TREE_MOST || sequences > 65535) return -5;
+    const long long units = (long long)cache->n_layers * cache->n_kv;
+    AcceptArgs a = {*cache, token, parent, chosen, start, count, seq, accepted, next, path, weight, position, nodes, 0, use_pdl};
+    a.units = (int)((units * sequences + 148 * 8 - 1) / (148 * 8));
+    if (a.units > units) a.units = (int)units;
+    if ((long long)a.units * nodes > 0x7fffffffLL) return -5;
+    return kv4_launch(kv8_accept_kernel, dim3((unsigned)((units + a.units - 1) / a.units), (unsigned)sequences), kAcThreads, 0, static_cast<cudaStream_t>(stream),
+                      use_pdl != 0, a);
+}
+
+extern "C" int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight, int* position, const int* length, const int* seq, const int* protect_from, int sequences,
+                                    int keep, int max_len, int* length_out, int use_pdl, void* stream) {
+    using namespace tz;
+    if (!cache || !kv8_cache_ok(*cache) || sequences < 0) return -1;
+    if (sequences == 0) return 0;
+    if (!weight || !position || !length || !length_out || length_out == length || keep <= 0 || max_len <= 0 || max_len > kv8_places(*cache) || (!seq && sequences > cache->table_rows)) return -1;
+    if (sequences > 65535 || max_len > kEvMost) return -5;
+    EvictArgs a = {*cache, weight, position, length, seq, protect_from, length_out, keep, max_len, use_pdl};
+    const bool held = max_len <= kEvHeld;
+    const size_t smem = ((size_t)(max_len + 31) / 32 + (size_t)(held ? max_len : kEvLists)) * 4;
+    constexpr size_t most = (kEvHeld / 32 + kEvHeld) * 4;
+    static_assert(most >= (kEvMost / 32 + kEvLists) * 4, "the larger of the two");
+    static_assert(most <= kMaxSmem - 2048, "bits of the longest and numbers of the longest that are held");
+    auto kernel = held ? kv8_evict_kernel<true> : kv8_evict_kernel<false>;
+    if (cudaError_t e = allow_smem(kernel, most)) return (int)e;
+    const long long ctas = (long long)cache->n_layers * cache->n_kv;
+    if (ctas > 0x7fffffffLL) return -5;
+    return kv4_launch(kernel, dim3((unsigned)ctas, (unsigned)sequences), kEvThreads, smem, static_cast<cudaStream_t>(stream), use_pdl != 0, a);
+}

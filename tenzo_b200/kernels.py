@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import struct
+from typing import NamedTuple
 
 import torch
 
@@ -381,3 +382,177 @@ def kv4_take_errors() -> int:
     """Error flags of the 4-bit cache's kernels since the last call (1: a wait was given up, 2: an index out of range), -1 if the query failed; waits for
     all streams of the device."""
     return int(load_library().tenzo_cuda_kv4_take_errors())
+
+
+# ---- INT8 caches: drafted trees, and caches of a bounded number of tokens ------------------------------------------------------------
+class Kv8Cache(NamedTuple):
+    """The INT8 caches of attention_int8 behind a block table: k, v int8 [blocks, layers, n_kv, slots, 128], scale_k, scale_v fp32 [blocks, layers, n_kv, slots],
+    block_table int32 [sequences, columns]; the token at place t of a sequence lies in block block_table[sequence, t / slots], slot t % slots. The paged_int8 pools
+    have 16 slots; the contiguous caches are blocks of max_seq slots (a multiple of 16) behind a table of one column, arange(sequences)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    scale_k: torch.Tensor
+    scale_v: torch.Tensor
+    block_table: torch.Tensor
+
+
+_KV8_CACHE = struct.Struct("@PPPPiiiiPii0P")                            # abi.Kv8Cache
+_ATTENTION_TREE = struct.Struct("@PPPPPPPiiiiPii0PPPPPPPPiiiiiiiiiiPN")    # abi.AttentionTreeArgs
+assert _KV8_CACHE.size == C.sizeof(abi.Kv8Cache) and _ATTENTION_TREE.size == C.sizeof(abi.AttentionTreeArgs)
+
+
+@functools.cache
+def _tree_calls():
+    """tenzo_cuda_kv8_append, _evict, _accept, tenzo_cuda_attention_tree, tenzo_cuda_kv8_weigh and the attention's choice of splits, with prototypes of this module's own,
+    whose structs are the bytes of a struct.Struct."""
+    def fn(name, *argtypes):
+        f = load_library()[name]
+        f.restype, f.argtypes = C.c_int, list(argtypes)
+        return f
+    return (fn("tenzo_cuda_kv8_append", _PB, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PP, _PP, _PP, _PI, _PP, _PP, _PI, _PP),
+            fn("tenzo_cuda_kv8_evict", _PB, _PP, _PP, _PP, _PP, _PP, _PI, _PI, _PI, _PP, _PI, _PP),
+            fn("tenzo_cuda_kv8_accept", _PB, _PP, _PP, _PP, _PP, _PP, _PP, _PI, _PI, _PP, _PP, _PP, _PP, _PP, _PI, _PP),
+            fn("tenzo_cuda_attention_tree", _PB, _PP), fn("tenzo_cuda_kv8_weigh", _PB, _PP, _PP), fn("tenzo_cuda_attention_tree_splits", _PI, _PI, _PI, _PI, _PI))
+
+
+def _kv8_cache(cache: Kv8Cache, device: int):
+    """The fields of abi.Kv8Cache."""
+    k, v, sk, sv, table = cache
+    shape, rows = k.shape, table.shape
+    if len(shape) != 5 or shape[4] != 128 or v.shape != shape or sk.shape != shape[:4] or sv.shape != shape[:4] or len(rows) != 2:
+        raise ValueError(f"caches [blocks, layers, kv heads, slots, 128], their scales and a table [rows, columns] are needed, not {tuple(shape)}, {tuple(v.shape)}, "
+                         f"{tuple(sk.shape)}, {tuple(sv.shape)} and {tuple(rows)}")
+    return (_arg(k, torch.int8, device, "k"), _arg(v, torch.int8, device, "v"), _arg(sk, torch.float32, device, "scale_k"), _arg(sv, torch.float32, device, "scale_v"),
+            shape[0], shape[1], shape[2], shape[3], _arg(table, torch.int32, device, "block_table"), rows[0], rows[1])
+
+
+def _arg_beside(t, cache: Kv8Cache, dtype, device: int, what: str) -> int:
+    """Address of what lies beside the scales; 0 for None."""
+    if t is not None and t.shape != cache.scale_k.shape:
+        raise ValueError(f"{what} has the scales' shape {tuple(cache.scale_k.shape)}, not {tuple(t.shape)}")
+    return _arg(t, dtype, device, what)
+
+
+def _arg_int(value: int, what: str) -> int:
+    """`value` where it fits the prototype's C int, which takes larger ones modulo 2^32."""
+    if not -_INT_MOST <= value <= _INT_MOST:
+        raise ValueError(f"{what} is {value}")
+    return value
+
+
+def kv8_append(k, v, cache, place, *, layer, seq=None, rope_pos=None, rope_cos=None, rope_sin=None, weight=None, position=None, use_pdl=False):
+    """Rotates the rows k [n, n_kv*128] at rope_pos int32 [n] (default: place), quantises k and v as attention_int8 does, and stores them at places place int32 [n] of the
+    sequences seq int32 [n] (default: row i is sequence i). A negative place marks a padding row, for which nothing is stored. weight fp32 and position int32, of the
+    scales' shape, receive 0 and the rotary position."""
+    dev = _current_device()
+    fields = _kv8_cache(cache, dev)
+    n_kv = fields[6]
+    (kp, ks, n), (vp, vs, m) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
+    if n != m or (ks != vs and n > 1):
+        raise ValueError("k and v have the same number of rows, equally far apart")
+    cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
+    _ok(_tree_calls()[0](_KV8_CACHE.pack(*fields), _arg_layer(layer), kp, vp, ks, _arg_entries(place, n, dev, "place"), _arg_entries(seq, n, dev, "seq"), n,
+                         _arg_entries(rope_pos, n, dev, "rope_pos"), cos, sin, length, _arg_beside(weight, cache, torch.float32, dev, "weight"),
+                         _arg_beside(position, cache, torch.int32, dev, "position"), use_pdl, _raw_stream(dev)), "tenzo_cuda_kv8_append")
+
+
+@functools.lru_cache(1024)
+def _attention_tree_room(sequences, nodes, n_q, n_kv, max_len, split_keys) -> int:
+    """What one call needs: splits of split_keys keys, or as many as it chooses itself."""
+    splits = -(-max_len // (-(-split_keys // 128) * 128)) if split_keys > 0 else _tree_calls()[5](sequences, nodes, n_q, n_kv, max_len)
+    return sequences * nodes * n_q * 520 * splits if splits > 1 else 0
+
+
+def _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev):
+    """The fields of abi.AttentionTreeArgs from cache to max_len, and what the calls ask further: the query's address and the number of rows."""
+    fields = _kv8_cache(cache, dev)
+    qp, q_stride, rows = _arg_rows(q, dev, n_q * 128, "q")
+    sequences = rows // nodes if nodes > 0 else -1
+    if sequences * nodes != rows:
+        raise ValueError(f"{rows} rows of q are no trees of {nodes} nodes")
+    mask_stride = 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] != rows or mask.shape[1] * 32 < nodes:
+            raise ValueError(f"mask has a row of at least {-(-nodes // 32)} words for each of {rows} nodes, not {tuple(mask.shape)}")
+        mask_stride = mask.shape[1]
+    cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
+    if max_len is None:
+        max_len = min(fields[7] * fields[10], _INT_MOST)
+    return qp, rows, sequences, (*fields, _arg_entries(start, sequences, dev, "start"), _arg_entries(count, sequences, dev, "count"), _arg_entries(seq, sequences, dev, "seq"),
+                                 _arg(mask, torch.int32, dev, "mask"), _arg_entries(rope_pos, rows, dev, "rope_pos"), cos, sin, length, q_stride, mask_stride,
+                                 _arg_layer(layer), n_q, sequences, nodes, _arg_int(max_len, "max_len"))
+
+
+def attention_tree(q, cache, start, *, layer, n_q, nodes, count=None, mask=None, seq=None, rope_pos=None, rope_cos=None, rope_sin=None, max_len=None, want_lse=False,
+                   split_keys=0, use_pdl=False, out=None, lse=None, workspace=None):
+    """Attention of the nodes of trees: q [sequences*nodes, n_q*128] over the tokens at places 0 .. start[s] - 1 of sequence s and, of the tree's own at start[s] + j, those
+    whose bit j % 32 of mask[row, j / 32] is set (int32 [rows, words]; default: nodes 0 .. i, a chain). start, count int32 [sequences]: tokens that are cached, and nodes
+    that are there (default: all); rope_pos int32 [rows]: the queries' rotary positions (default: start + i). Returns out [rows, n_q*128], zeros where nothing is seen;
+    with want_lse (out, lse [rows, n_q])."""
+    dev = _current_device()
+    qp, rows, sequences, fields = _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != (rows, n_q * 128):
+        raise ValueError(f"out is [{rows}, {n_q * 128}]")
+    if lse is None:
+        lse = torch.empty(rows, n_q, dtype=torch.float32, device=q.device) if want_lse else None
+    elif lse.shape != (rows, n_q):
+        raise ValueError(f"lse is [{rows}, {n_q}]")
+    if workspace is None:
+        size = _attention_tree_room(sequences, nodes, n_q, fields[6], fields[-1], split_keys)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    args = _ATTENTION_TREE.pack(qp, _arg(out, torch.float32, dev, "out"), _arg(lse, torch.float32, dev, "lse"), *fields, _arg_int(split_keys, "split_keys"), use_pdl,
+                                _arg(workspace, torch.uint8, dev, "workspace"), 0 if workspace is None else workspace.numel())
+    _ok(_tree_calls()[3](args, _raw_stream(dev)), "tenzo_cuda_attention_tree")
+    return out if lse is None else (out, lse)
+
+
+def kv8_weigh(q, lse, cache, weight, start, *, layer, n_q, nodes, count=None, mask=None, seq=None, rope_pos=None, rope_cos=None, rope_sin=None, max_len=None, use_pdl=False):
+    """Adds to weight (fp32, of the scales' shape) what each cached token received in attention_tree of the same arguments, whose lse [rows, n_q] this reads: the sum of
+    softmax's results over the nodes and the query heads of a kv head."""
+    dev = _current_device()
+    qp, rows, _, fields = _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev)
+    if lse.shape != (rows, n_q):
+        raise ValueError(f"lse is [{rows}, {n_q}], not {tuple(lse.shape)}")
+    args = _ATTENTION_TREE.pack(qp, 0, _arg(lse, torch.float32, dev, "lse"), *fields, 0, use_pdl, 0, 0)
+    _ok(_tree_calls()[4](args, _arg_beside(weight, cache, torch.float32, dev, "weight"), _raw_stream(dev)), "tenzo_cuda_kv8_weigh")
+
+
+def kv8_evict(cache, weight, position, length, *, keep, protect_from=None, seq=None, max_len=None, use_pdl=False):
+    """Cuts the sequences that hold length int32 [sequences] tokens back to `keep`, in all layers and for each kv head on its own: the tokens of least weight go, but
+    none whose position is protect_from[s] int32 [sequences] or more; those behind place keep - 1 that stay move to the places that became free. Returns the new lengths."""
+    dev, sequences = _current_device(), len(length)
+    fields = _kv8_cache(cache, dev)
+    if max_len is None:
+        max_len = min(fields[7] * fields[10], 1 << 20)
+    out = torch.empty_like(length)
+    _ok(_tree_calls()[1](_KV8_CACHE.pack(*fields), _arg_beside(weight, cache, torch.float32, dev, "weight"), _arg_beside(position, cache, torch.int32, dev, "position"),
+                         _arg_entries(length, sequences, dev, "length"), _arg_entries(seq, sequences, dev, "seq"), _arg_entries(protect_from, sequences, dev, "protect_from"),
+                         sequences, _arg_int(keep, "keep"), _arg_int(max_len, "max_len"), out.data_ptr(), use_pdl, _raw_stream(dev)), "tenzo_cuda_kv8_evict")
+    return out
+
+
+def kv8_accept(cache, token, parent, chosen, start, *, count=None, seq=None, weight=None, position=None, use_pdl=False):
+    """The nodes of drafted trees that the model agrees with, given the nodes' tokens, the nodes they go on from and the model's choice after each, int32
+    [sequences, nodes] (node 0 is the root); their rows are moved up behind the start[s] cached tokens in all layers. Returns (accepted [sequences], next [sequences],
+    path [sequences, nodes]): how many nodes, the root among them, the token chosen after the last, and which nodes, then -1."""
+    dev, shape = _current_device(), token.shape
+    if len(shape) != 2 or parent.shape != shape or chosen.shape != shape:
+        raise ValueError(f"token, parent and chosen are [sequences, nodes], not {tuple(shape)}, {tuple(parent.shape)} and {tuple(chosen.shape)}")
+    sequences, nodes = shape
+    fields = _kv8_cache(cache, dev)
+    both = torch.empty(sequences * (nodes + 2), dtype=torch.int32, device=token.device)
+    accepted, following, path = both[:sequences], both[sequences:2 * sequences], both[2 * sequences:].view(sequences, nodes)
+    _ok(_tree_calls()[2](_KV8_CACHE.pack(*fields), _arg(token, torch.int32, dev, "token"), _arg(parent, torch.int32, dev, "parent"), _arg(chosen, torch.int32, dev, "chosen"),
+                         _arg_entries(start, sequences, dev, "start"), _arg_entries(count, sequences, dev, "count"), _arg_entries(seq, sequences, dev, "seq"), sequences, nodes,
+                         accepted.data_ptr(), following.data_ptr(), path.data_ptr(), _arg_beside(weight, cache, torch.float32, dev, "weight"),
+                         _arg_beside(position, cache, torch.int32, dev, "position"), use_pdl, _raw_stream(dev)), "tenzo_cuda_kv8_accept")
+    return accepted, following, path
+
+
+def kv8_take_errors() -> int:
+    """Error flags of the kernels on trees and bounded caches since the last call (1: a wait was given up, 2: an index out of range), -1 if the query failed; waits for
+    all streams of the device."""
+    return int(load_library().tenzo_cuda_kv8_take_errors())

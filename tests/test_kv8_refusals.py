@@ -1,0 +1,156 @@
+"""What the calls on trees and bounded caches refuse, without a device: refusals come before any launch. And the packed arguments of the Python calls are
+the C structs."""
+import ctypes as C
+
+import pytest
+import torch
+from tenzo_b200 import abi, kernels, load_library
+
+P = 0x10000                                       # a 16-byte aligned address that nothing looks at
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return load_library()
+
+
+def cache(**over):
+    c = abi.Kv8Cache(k=P, v=P, scale_k=P, scale_v=P, n_blocks=10, n_layers=2, n_kv=3, slots=16, block_table=P, table_rows=4, table_stride=5)
+    for k, v in over.items():
+        setattr(c, k, v)
+    return c
+
+
+def tree(**over):
+    a = abi.AttentionTreeArgs(q=P, out=P, lse=P, cache=cache(), start=P, layer=0, n_q=6, sequences=4, nodes=7, max_len=80)
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+def append(lib, c, **over):
+    a = dict(layer=0, k=P, v=P, stride=384, place=P, seq=P, rows=4, rope_pos=None, cos=None, sin=None, length=0) | over
+    return lib.tenzo_cuda_kv8_append(c and C.byref(c), a["layer"], a["k"], a["v"], a["stride"], a["place"], a["seq"], a["rows"], a["rope_pos"], a["cos"], a["sin"], a["length"], P, P, 0,
+                                     None)
+
+
+def evict(lib, c, **over):
+    a = dict(weight=P, position=P, length=P, seq=P, sequences=4, keep=8, max_len=80, out=P + 64) | over
+    return lib.tenzo_cuda_kv8_evict(c and C.byref(c), a["weight"], a["position"], a["length"], a["seq"], None, a["sequences"], a["keep"], a["max_len"], a["out"], 0, None)
+
+
+def accept(lib, c, **over):
+    a = dict(token=P, parent=P, chosen=P, start=P, seq=P, sequences=4, nodes=7, accepted=P, next=P, path=P) | over
+    return lib.tenzo_cuda_kv8_accept(c and C.byref(c), a["token"], a["parent"], a["chosen"], a["start"], None, a["seq"], a["sequences"], a["nodes"], a["accepted"], a["next"], a["path"],
+                                     None, None, 0, None)
+
+
+BAD_CACHES = [dict(k=None), dict(v=None), dict(scale_k=None), dict(scale_v=None), dict(k=P + 8), dict(v=P + 4), dict(scale_k=P + 4), dict(scale_v=P + 8), dict(block_table=None),
+              dict(n_blocks=0), dict(n_layers=0), dict(n_kv=0), dict(slots=0), dict(slots=8), dict(slots=24), dict(slots=-16), dict(table_rows=0), dict(table_stride=0),
+              dict(n_blocks=1 << 20, n_layers=1 << 5, slots=1 << 6), dict(n_blocks=1 << 30, n_layers=1 << 30)]
+
+
+@pytest.mark.parametrize("over", BAD_CACHES, ids=str)
+def test_caches(lib, over):
+    c = cache(**over)
+    assert append(lib, c) == evict(lib, c) == accept(lib, c) == abi.ERR_INVALID
+    a = tree(cache=c)
+    assert lib.tenzo_cuda_attention_tree(C.byref(a), None) == lib.tenzo_cuda_kv8_weigh(C.byref(a), P, None) == abi.ERR_INVALID
+
+
+def test_null(lib):
+    assert append(lib, None) == evict(lib, None) == accept(lib, None) == lib.tenzo_cuda_attention_tree(None, None) == lib.tenzo_cuda_kv8_weigh(None, P, None) == abi.ERR_INVALID
+
+
+@pytest.mark.parametrize("over", [dict(layer=-1), dict(layer=2), dict(k=None), dict(v=None), dict(stride=383), dict(place=None), dict(rows=-1), dict(seq=None, rows=5), dict(cos=P),
+                                  dict(sin=P), dict(cos=P, sin=P, length=0), dict(cos=P + 4, sin=P, length=9), dict(cos=P, sin=P + 8, length=9)], ids=str)
+def test_append(lib, over):
+    assert append(lib, cache(), **over) == abi.ERR_INVALID
+
+
+TREE = [dict(q=None), dict(start=None), dict(layer=2), dict(layer=-1), dict(n_q=0), dict(n_q=7), dict(n_q=-6), dict(sequences=-1), dict(nodes=0), dict(nodes=-1), dict(max_len=0), dict(max_len=81),
+        dict(cache=cache(table_rows=3)), dict(rope_cos=P), dict(rope_sin=P), dict(rope_cos=P, rope_sin=P, rope_len=0), dict(q_stride=767), dict(q_stride=-768), dict(nodes=40, mask=P, mask_stride=1),
+        dict(mask=P, mask_stride=-1)]
+
+
+@pytest.mark.parametrize("over", TREE, ids=str)
+def test_tree_and_weigh(lib, over):
+    a = tree(**over)
+    assert lib.tenzo_cuda_attention_tree(C.byref(a), None) == abi.ERR_INVALID
+    assert lib.tenzo_cuda_kv8_weigh(C.byref(a), P, None) == abi.ERR_INVALID
+
+
+@pytest.mark.parametrize("over", [dict(out=None), dict(out=P + 4), dict(split_keys=-1)], ids=str)
+def test_tree_alone(lib, over):
+    assert lib.tenzo_cuda_attention_tree(C.byref(tree(**over)), None) == abi.ERR_INVALID
+
+
+def test_weigh_alone(lib):
+    assert lib.tenzo_cuda_kv8_weigh(C.byref(tree()), None, None) == abi.ERR_INVALID
+    assert lib.tenzo_cuda_kv8_weigh(C.byref(tree(lse=None)), P, None) == abi.ERR_INVALID
+
+
+def test_too_many_nodes(lib):
+    a = tree(nodes=257)
+    assert lib.tenzo_cuda_attention_tree(C.byref(a), None) == lib.tenzo_cuda_kv8_weigh(C.byref(a), P, None) == accept(lib, cache(), nodes=257) == abi.ERR_UNSUPPORTED
+
+
+def test_room_for_splits(lib):
+    splits, need = lib.tenzo_cuda_attention_tree_splits, lib.tenzo_cuda_attention_tree_workspace_bytes
+    assert splits(0, 4, 4, 2, 10) == splits(1, 0, 4, 2, 10) == splits(1, 257, 4, 2, 10) == splits(1, 4, 0, 2, 10) == splits(1, 4, 5, 2, 10) == splits(1, 4, 4, 2, 0) == 0
+    assert need(0, 4, 4, 10) == need(1, 0, 4, 10) == need(1, 4, 0, 10) == need(1, 4, 4, 0) == 0
+    for sequences, nodes, n_q, n_kv, n in ((1, 1, 20, 5, 30000), (1, 64, 20, 5, 16384), (64, 16, 20, 5, 4096), (3, 256, 7, 1, 1 << 20), (1, 1, 1, 1, 1), (5000, 3, 32, 32, 2000)):
+        most = splits(sequences, nodes, n_q, n_kv, n)
+        assert 1 <= most and (most == 1 or most * 520 * sequences * nodes * n_q <= need(sequences, nodes, n_q, n))
+        assert kernels._attention_tree_room(sequences, nodes, n_q, n_kv, n, 0) == (most * 520 * sequences * nodes * n_q if most > 1 else 0)
+    assert kernels._attention_tree_room(2, 3, 4, 2, 1000, 128) == 8 * 2 * 3 * 4 * 520 and kernels._attention_tree_room(2, 3, 4, 2, 1000, 900) == 0       # 900: rounded up to 1024
+
+
+@pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(length=None), -1), (dict(out=None), -1), (dict(out=P), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
+                                       (dict(max_len=0), -1), (dict(max_len=81), -1), (dict(sequences=-1), -1), (dict(seq=None, sequences=5), -1), (dict(sequences=65536), -5)], ids=str)
+def test_evict(lib, over, code):
+    assert evict(lib, cache(), **over) == code
+
+
+def test_evict_too_long(lib):
+    c = cache(table_stride=(1 << 16) + 1)
+    assert evict(lib, c, max_len=(1 << 20) + 1) == abi.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("over,code", [(dict(token=None), -1), (dict(parent=None), -1), (dict(chosen=None), -1), (dict(start=None), -1), (dict(accepted=None), -1), (dict(next=None), -1),
+                                       (dict(path=None), -1), (dict(nodes=0), -1), (dict(sequences=-1), -1), (dict(seq=None, sequences=5), -1), (dict(sequences=65536), -5)], ids=str)
+def test_accept(lib, over, code):
+    assert accept(lib, cache(), **over) == code
+
+
+def test_nothing_to_do_is_no_error(lib):
+    assert append(lib, cache(), rows=0, k=None, place=None) == 0
+    assert evict(lib, cache(), sequences=0, weight=None) == accept(lib, cache(), sequences=0, token=None) == 0
+    a = tree(sequences=0, q=None)
+    assert lib.tenzo_cuda_attention_tree(C.byref(a), None) == lib.tenzo_cuda_kv8_weigh(C.byref(a), P, None) == 0
+
+
+def _leaves(cls):
+    return [x for _, t in cls._fields_ for x in (_leaves(t) if issubclass(t, C.Structure) else [t])]
+
+
+def _flat(o):
+    return [x for n, t in o._fields_ for x in (_flat(getattr(o, n)) if issubclass(t, C.Structure) else [getattr(o, n)])]
+
+
+@pytest.mark.parametrize("cls,packer", [(abi.Kv8Cache, kernels._KV8_CACHE), (abi.AttentionTreeArgs, kernels._ATTENTION_TREE)], ids=lambda x: getattr(x, "__name__", ""))
+def test_packed_arguments_are_the_struct(cls, packer):
+    values = [1000 + i for i in range(len(_leaves(cls)))]
+    assert _flat(cls.from_buffer_copy(packer.pack(*values))) == values
+
+
+def test_python_calls_refuse_what_is_not_on_the_device():
+    c = kernels.Kv8Cache(*(torch.zeros(3, 1, 2, 16, 128, dtype=torch.int8) for _ in range(2)), *(torch.zeros(3, 1, 2, 16) for _ in range(2)), torch.zeros(1, 3, dtype=torch.int32))
+    ints = torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: kernels.kv8_append(torch.zeros(1, 256), torch.zeros(1, 256), c, ints, layer=0),
+                 lambda: kernels.attention_tree(torch.zeros(1, 512), c, ints, layer=0, n_q=4, nodes=1),
+                 lambda: kernels.kv8_weigh(torch.zeros(1, 512), torch.zeros(1, 4), c, c.scale_k, ints, layer=0, n_q=4, nodes=1),
+                 lambda: kernels.kv8_evict(c, c.scale_k, torch.zeros(3, 1, 2, 16, dtype=torch.int32), ints, keep=4),
+                 lambda: kernels.kv8_accept(c, ints[None], ints[None], ints[None], ints)):
+        with pytest.raises((ValueError, RuntimeError, AssertionError)):
+            call()
