@@ -20,6 +20,7 @@ constexpr int kTrTile = 128, kTrTileBytes = kTrTile * kK8Hd;          // keys a 
 constexpr int kTrMask = TENZO_TREE_MOST / 32;
 constexpr float kTrSlack = 4.0f, kTrOne = 134217728.0f;               // a weight of 1 is 2^27, weights up to 2^4 are let through
 constexpr float kTrLow = -1e30f;                                      // a reference that is not set
+constexpr uint32_t kTrShape = (2u << 4) | (1u << 7) | ((uint32_t)(kTrTile >> 4) << 24);      // of products: sums of 32 bits; codes, with a sign, as A; 128 rows
 constexpr int kTrFlush = 256;                                         // tiles after which the accumulators are moved on all the same: 2^15 keys * 128 * 255 < 2^31
 
 __device__ int g_tree_error = 0;
@@ -35,7 +36,7 @@ struct TreeLaunch {
 // R queries a CTA.
 template <int R>
 struct TreeShape {
-    static constexpr int warps = R / 4, threads = (warps + 2) * 32;   // four warps for sixteen queries; one that copies, one that issues products
+    static constexpr int warps = R / 4, threads = (warps + 3) * 32;   // four warps for sixteen queries; one that copies, two that issue products
     static constexpr int stages = R == 64 ? 3 : 2, resident = R == 64 ? 1 : 2;
     static constexpr int s_cols = 3 * R, o_cols = 4 * R, tmem_cols = R == 64 ? 512 : R == 32 ? 256 : 128;
     static constexpr int p_panels = R == 64 ? 2 : 1;                  // of 128 bytes: 32 queries
@@ -80,11 +81,23 @@ __device__ __forceinline__ bool tr_any(int barrier, int count, bool mine) {
 __device__ __forceinline__ uint64_t tr_desc_mn(uint32_t saddr, uint32_t panel) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// A query or key's sum from its three parts of a whole number (below 2^21 each): 2^23 * 1.5 with a part in its last bits is a float.
-__device__ __forceinline__ float tr_whole(uint32_t high, uint32_t mid, uint32_t low) {
+__device__ __forceinline__ f32x2 tr_mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 tr_fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+// The accumulators of the scores start at kTrBias, the bits of 2^23 * 1.5, so that a part of a sum (below 2^21 each) is read as the float 2^23 * 1.5 + part.
+// Two sums from their three parts; the lower two parts' share is rounded to 2^7 of some 2^29.
+constexpr uint32_t kTrBias = 0x4B400000u;
+__device__ __forceinline__ f32x2 tr_whole2(const uint32_t* high, const uint32_t* mid, const uint32_t* low) {
+    auto part = [](const uint32_t* v) { return pack2(__uint_as_float(v[0]), __uint_as_float(v[1])); };
     constexpr float base = 12582912.0f;
-    const float h = __uint_as_float(0x4B400000u + high) - base, m = __uint_as_float(0x4B400000u + mid) - base, l = __uint_as_float(0x4B400000u + low);
-    return __fmaf_rn(h, 65536.0f, __fmaf_rn(m, 256.0f, l)) - base;
+    return add2(tr_fma2(add2(part(high), pack2(-base, -base)), pack2(65536.0f, 65536.0f), tr_fma2(part(mid), pack2(256.0f, 256.0f), part(low))), pack2(-257.0f * base, -257.0f * base));
+}
+// The same value in N columns of the warp's 32 lanes.
+template <int N>
+__device__ __forceinline__ void tr_fill(uint32_t at, uint32_t v) {
+    static_assert(N % 16 == 0, "sixteen columns a store");
+#pragma unroll
+    for (int i = 0; i < N; i += 16)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(at + i), "r"(v) : "memory");
 }
 
 // What a sequence's numbers allow.
@@ -196,9 +209,11 @@ struct TreeCopies {
     }
 };
 
-// Arguments of 2^x of sixteen queries (columns col.. of each part) and the lane's key, whose scale is sk.
+// For sixteen queries (columns of each part), two by two, and the lane's key, whose scale is sk: arguments of 2^x less what `down` (with its sign turned) says. The
+// accumulators are left as they have to start.
 template <int R>
-__device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, float sk, float (&x)[16]) {
+__device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, const float* s_down, float sk, f32x2 (&w)[8]) {
+    const f32x2 sk2 = pack2(sk, sk);
 #pragma unroll
     for (int h = 0; h < 16; h += 8) {
         uint32_t d1[8], d2[8], d3[8];
@@ -210,12 +225,25 @@ __device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, fl
         tr_tie8(d3);
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(s_f + h + j);
-            x[h + j] = tr_whole(d1[j], d2[j], d3[j]) * (sk * f.x);
-            x[h + j + 1] = tr_whole(d1[j + 1], d2[j + 1], d3[j + 1]) * (sk * f.y);
-            x[h + j + 2] = tr_whole(d1[j + 2], d2[j + 2], d3[j + 2]) * (sk * f.z);
-            x[h + j + 3] = tr_whole(d1[j + 3], d2[j + 3], d3[j + 3]) * (sk * f.w);
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + h + j), m = *reinterpret_cast<const ulonglong2*>(s_down + h + j);
+            w[(h + j) / 2] = tr_fma2(tr_whole2(d1 + j, d2 + j, d3 + j), tr_mul2(sk2, f.x), m.x);
+            w[(h + j) / 2 + 1] = tr_fma2(tr_whole2(d1 + j + 2, d2 + j + 2, d3 + j + 2), tr_mul2(sk2, f.y), m.y);
         }
+    }
+#pragma unroll
+    for (int part = 0; part < 3; ++part) tr_fill<16>(tmem + part * R, kTrBias);
+    tmem_wait_st();
+}
+
+// Queries that do not see the lane's key: node j of the tree (below 0: a cached token, which all see), or `dead`, none.
+__device__ __forceinline__ void tr_hide(f32x2 (&w)[8], const uint32_t (*mask)[kTrMask], int j, bool dead) {
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+        float w0, w1;
+        unpack2(w[r / 2], w0, w1);
+        if (dead || (j >= 0 && !(mask[r][j >> 5] >> (j & 31) & 1u))) w0 = -INFINITY;
+        if (dead || (j >= 0 && !(mask[r + 1][j >> 5] >> (j & 31) & 1u))) w1 = -INFINITY;
+        w[r / 2] = pack2(w0, w1);
     }
 }
 
@@ -226,14 +254,13 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     using S = TreeShape<R>;
     const tenzo_attention_tree_args& a = L.a;
     extern __shared__ unsigned char tr_smem[];
-    __shared__ __align__(16) float s_f[R], s_ref[R], s_max[4][R], s_sum[4][R];
-    __shared__ float s_scale_max[4];
+    __shared__ __align__(16) float s_f[R], s_down[R], s_max[4][R], s_sum[4][R], s_scale_max[R / 16][4];      // (s_down: the references with their signs turned)
     __shared__ long long s_at[R];                        // [row][head] of a query; -1: none of this tree's, or refused; -2 - that: padding, zeros
     __shared__ uint32_t s_mask[R][kTrMask];
     __shared__ uint64_t s_full[S::stages], s_empty[S::stages], s_bar[4];
     __shared__ unsigned s_valid[S::stages];
-    __shared__ uint32_t s_tmem, s_fresh[2];
-    __shared__ float s_unit;                             // values' scales count up to this power of two
+    __shared__ uint32_t s_tmem, s_set[R / 16];           // queries that have a reference
+    __shared__ float s_unit[R / 16][2];                  // values' scales count up to this power of two; what a scale is multiplied by
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int tile = blockIdx.x % L.tiles, split = (int)(blockIdx.x / L.tiles) % L.n_splits, s = blockIdx.x / L.tiles / L.n_splits, kvh = blockIdx.y;
     if (a.use_pdl || L.n_splits > 1) pdl_launch_dependents();         // (the second kernel waits for this one whatever its neighbours do)
@@ -267,12 +294,15 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
             mbar_init(&s_full[i], 1);
             mbar_init(&s_empty[i], 1);
         }
-        mbar_init(b_scores, 1);
+        mbar_init(b_scores, 2);                          // the products, and the thread that has seen the copies land
         mbar_init(b_free, S::warps);
         mbar_init(b_weights, S::warps);
         mbar_init(b_values, 1);
         mbar_init_fence();
-        s_unit = 0.0f;
+        for (int g = 0; g < R / 16; ++g) {
+            s_unit[g][0] = s_unit[g][1] = 0.0f;
+            s_set[g] = 0;
+        }
     }
     if (warp == S::warps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::tmem_cols) : "memory");
@@ -289,42 +319,44 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
         const TreeCopies<S::stages, true> copies = {a, &kmap, &vmap, kvh, q.seq, c_begin, c_end, base, s_scales, s_full, s_empty, s_valid};
         ok = copies.run(n_tiles, n_tiles);
     } else if (warp == S::warps + 1) {
-        named_barrier_sync(2, kWithQueries);             // the queries are there
-        if (lane == 0) {
-            constexpr uint32_t shape = (2u << 4) | (1u << 7) | ((uint32_t)(kTrTile >> 4) << 24);      // sums of 32 bits; codes with a sign; 128 rows
-            constexpr uint32_t d_scores = shape | (1u << 10) | ((uint32_t)(S::s_cols >> 3) << 17);
-            constexpr uint32_t d_values = shape | (1u << 15) | (1u << 16) | ((uint32_t)(S::o_cols >> 3) << 17);        // both operands transposed
-            const uint64_t dq = umma_desc_sw128(smem_addr(s_q)), dp = tr_desc_mn(smem_addr(s_p), kTrTileBytes);
-            auto scores = [&](int i) {
+        named_barrier_sync(6, kWithQueries);             // the queries are there
+        if (lane == 0) {                                 // S^T = K Q^T
+            constexpr uint32_t shape = kTrShape | (1u << 10) | ((uint32_t)(S::s_cols >> 3) << 17);
+            const uint64_t dq = umma_desc_sw128(smem_addr(s_q));
+            for (int i = 0; i < n_tiles; ++i) {
                 const int st = i % S::stages;
-                ok = ok && mbar_spin_bounded(&s_full[st], (unsigned)(i / S::stages) & 1u) && (i == 0 || mbar_spin_bounded(b_free, (unsigned)(i - 1) & 1u));
-                if (!ok) return;
+                ok = mbar_spin_bounded(&s_full[st], (unsigned)(i / S::stages) & 1u) && (i == 0 || mbar_spin_bounded(b_free, (unsigned)(i - 1) & 1u));
+                if (!ok) break;
                 tc_fence_after();
                 const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * 2 * kTrTileBytes));
 #pragma unroll
-                for (int k = 0; k < kK8Hd / 32; ++k) umma_i8(tmem, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), d_scores, k > 0);
+                for (int k = 0; k < kK8Hd / 32; ++k) umma_i8(tmem, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), shape, 1u);
                 umma_commit(b_scores);
-            };
-            scores(0);
-            for (int i = 0; i < n_tiles && ok; ++i) {
-                if (i + 1 < n_tiles) scores(i + 1);
-                ok = ok && mbar_spin_bounded(b_weights, (unsigned)i & 1u);
+                mbar_arrive(b_scores);
+            }
+        }
+        __syncwarp();
+    } else if (warp == S::warps + 2) {
+        if (lane == 0) {                                 // O^T += V^T P^T
+            constexpr uint32_t shape = kTrShape | (1u << 15) | (1u << 16) | ((uint32_t)(S::o_cols >> 3) << 17);        // both operands transposed
+            const uint64_t dp = tr_desc_mn(smem_addr(s_p), kTrTileBytes);
+            for (int i = 0; i < n_tiles; ++i) {
+                const int st = i % S::stages;
+                ok = mbar_spin_bounded(&s_full[st], (unsigned)(i / S::stages) & 1u) && mbar_spin_bounded(b_weights, (unsigned)i & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                const int st = i % S::stages;
                 const uint64_t dv = tr_desc_mn(smem_addr(base + (size_t)st * 2 * kTrTileBytes + kTrTileBytes), kTrTileBytes);
-                const bool fresh = *reinterpret_cast<volatile uint32_t*>(&s_fresh[i & 1]) != 0;
 #pragma unroll
                 for (int k = 0; k < kTrTile / 32; ++k)
-                    umma_i8(tmem + S::s_cols, dv + (uint64_t)(k * (32 * kK8Hd >> 4)), dp + (uint64_t)(k * (32 * kK8Hd >> 4)), d_values, !fresh || k > 0);
-                umma_commit(&s_empty[st]);
+                    umma_i8(tmem + S::s_cols, dv + (uint64_t)(k * (32 * kK8Hd >> 4)), dp + (uint64_t)(k * (32 * kK8Hd >> 4)), shape, 1u);
                 umma_commit(b_values);
+                umma_commit(&s_empty[st]);
             }
         }
         __syncwarp();
     } else {
-        const int quarter = warp & 3, first = (warp >> 2) * 16;       // its keys of a tile, and its queries
-        constexpr int kAll = S::warps * 32;
+        const int quarter = warp & 3, group = warp >> 2, first = group * 16;      // its keys of a tile, and its queries
+        constexpr int kAll = S::warps * 32, kEvery = 7;              // threads, and their barrier (1 .. 4: those of sixteen queries)
         // ---- the queries ----
         for (int r = tid; r < R; r += kAll) {
             const int flat = flat0 + r, node = flat / L.group;
@@ -340,11 +372,11 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 }
             }
             s_at[r] = at;
-            s_ref[r] = kTrLow;
+            s_down[r] = 0.0f;
             for (int w = 0; w < (a.nodes + 31) / 32; ++w)
                 s_mask[r][w] = at < 0 ? 0u : a.mask ? (uint32_t)ld_l2(a.mask + row * a.mask_stride + w) : node >= 32 * w + 31 ? 0xffffffffu : node < 32 * w ? 0u : (2u << (node - 32 * w)) - 1u;
         }
-        named_barrier_sync(1, kAll);
+        named_barrier_sync(kEvery, kAll);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int r = warp + j * S::warps;
@@ -358,13 +390,21 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
             }
             if (lane == 0) s_f[r] = f;
         }
-        fence_proxy_async_smem();
-        named_barrier_sync(2, kWithQueries);
         const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_scores = t_lane + (uint32_t)first, t_values = t_lane + (uint32_t)(S::s_cols + 4 * first);
-        const int key = 32 * quarter + lane;
-        float o[16], l[16];                              // of dim `key` and of key `key`: outputs that were moved on, sums
+        tr_fill<64>(t_values, 0u);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[r] = l[r] = 0.0f;
+        for (int part = 0; part < 3; ++part) tr_fill<16>(t_scores + part * R, kTrBias);
+        tmem_wait_st();
+        tc_fence_before();
+        fence_proxy_async_smem();
+        named_barrier_sync(6, kWithQueries);
+        const int key = 32 * quarter + lane;
+        float o[16];                                     // of dim `key`: outputs that were moved on
+        f32x2 l[8];                                      // of key `key`: sums
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[r] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) l[r] = 0;
         // Adds the accumulators to o.
         auto move_on = [&](float unit) {
 #pragma unroll
@@ -381,7 +421,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
         };
         for (int i = 0; i < n_tiles; ++i) {
             const int st = i % S::stages, t = c_begin + i * kTrTile + key;
-            ok = ok && mbar_wait_bounded(&s_full[st], (unsigned)(i / S::stages) & 1u) && mbar_wait_bounded(b_scores, (unsigned)i & 1u);
+            ok = ok && mbar_wait_bounded(b_scores, (unsigned)i & 1u);
             __syncwarp();
             const unsigned valid = s_valid[st];
             const bool ragged = c_begin + (i + 1) * kTrTile > min(c_end, q.start) || valid != 0xffu;
@@ -392,77 +432,91 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 sk = __uint_as_float(0x7fc00000u);
             }
             tc_fence_after();
-            float x[16];
-            tr_arguments<R>(t_scores, s_f + first, sk, x);
+            f32x2 w[8];
+            tr_arguments<R>(t_scores, s_f + first, s_down + first, sk, w);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_free);
-            if (ragged) {
-                const int j = t - q.start;
+            if (ragged) tr_hide(w, s_mask + first, t - q.start, dead);
+            float over = -INFINITY;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (dead || (j >= 0 && !(s_mask[first + r][j >> 5] >> (j & 31) & 1u))) x[r] = -INFINITY;
+            for (int r = 0; r < 8; ++r) {
+                float w0, w1;
+                unpack2(w[r], w0, w1);
+                over = fmaxf(fmaxf(over, w0), w1);
             }
-            float w[16], over = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const float4 m = *reinterpret_cast<const float4*>(s_ref + first + r);
-                w[r] = x[r] - m.x;
-                w[r + 1] = x[r + 1] - m.y;
-                w[r + 2] = x[r + 2] - m.z;
-                w[r + 3] = x[r + 3] - m.w;
-                over = fmaxf(fmaxf(fmaxf(over, w[r]), fmaxf(w[r + 1], w[r + 2])), w[r + 3]);
-            }
-            float unit = s_unit;
-            const bool anew = tr_any(1, kAll, over > kTrSlack || sv > unit || (i + 1) % kTrFlush == 0);
+            const uint32_t set = s_set[group];
+            const bool anew = tr_any(1 + group, 128, over > kTrSlack || sv > s_unit[group][0] || set != 0xffffu || (i + 1) % kTrFlush == 0);
             if (anew) {
-                // ---- references anew, and accumulators moved on ----
-                float top = -INFINITY;                   // lane r: of query `first` + r
+                // ---- references of these sixteen queries anew, and their accumulators moved on ----
+                const float unit = s_unit[group][0];
+                float top = -INFINITY;                   // lane r: of query `first` + r, less the reference
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float m = tr_warp_max(x[r]);
-                    if (lane == r) top = m;
+                for (int r = 0; r < 16; r += 2) {
+                    float w0, w1;
+                    unpack2(w[r / 2], w0, w1);
+                    w0 = tr_warp_max(w0);
+                    w1 = tr_warp_max(w1);
+                    if (lane == r) top = w0;
+                    if (lane == r + 1) top = w1;
                 }
                 if (lane < 16) s_max[quarter][first + lane] = top;
                 const float most = tr_warp_max(sv);
-                if (warp < 4 && lane == 0) s_scale_max[quarter] = most;
-                named_barrier_sync(1, kAll);
-                const float scale_most = fmaxf(fmaxf(s_scale_max[0], s_scale_max[1]), fmaxf(s_scale_max[2], s_scale_max[3]));
-                const float now_unit = scale_most > unit ? __uint_as_float(min(max((__float_as_uint(scale_most) >> 23) + 1u, 67u), 254u) << 23) : unit;      // a power of two above it, at least 2^-60
+                if (lane == 0) s_scale_max[group][quarter] = most;
                 if (i > 0) {
                     ok = ok && mbar_wait_bounded(b_values, (unsigned)(i - 1) & 1u);
                     __syncwarp();
                     tc_fence_after();
                     move_on(unit * (1.0f / kTrOne));
+                    tr_fill<64>(t_values, 0u);
+                    tmem_wait_st();
                     tc_fence_before();
                 }
-                float now[16];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float old = s_ref[first + r];
-                    now[r] = fmaxf(fmaxf(fmaxf(s_max[0][first + r], s_max[1][first + r]), fmaxf(s_max[2][first + r], s_max[3][first + r])), old);
-                    const float down = tr_ex2(old - now[r]);
-                    o[r] *= down;
-                    l[r] *= down;
-                    w[r] = x[r] - now[r];
+                named_barrier_sync(1 + group, 128);
+                const float4 scales = *reinterpret_cast<const float4*>(s_scale_max[group]);
+                const float scale_most = fmaxf(fmaxf(scales.x, scales.y), fmaxf(scales.z, scales.w));
+                float up, by;                            // of query `first` + lane % 16: how far its reference goes up (the first one may go down), and what that leaves of its sums
+                {
+                    const int r = lane & 15;
+                    const bool was = set >> r & 1u;
+                    top = fmaxf(fmaxf(s_max[0][first + r], s_max[1][first + r]), fmaxf(s_max[2][first + r], s_max[3][first + r]));
+                    up = was ? fmaxf(top, 0.0f) : top == -INFINITY ? 0.0f : top;
+                    by = was ? tr_ex2(-up) : 0.0f;       // (there is nothing yet)
                 }
-                named_barrier_sync(1, kAll);             // all have read
-                if (quarter == 0 && lane == 0) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s_ref[first + r] = now[r];
+                const uint32_t now_set = set | (__ballot_sync(0xffffffffu, top != -INFINITY) & 0xffffu);
+                if (quarter == 0) {
+                    if (lane < 16) s_down[first + lane] -= up;
+                    if (lane == 0) {
+                        // a power of two above the largest scale, at least 2^-60
+                        const float now = scale_most > unit ? __uint_as_float(min(max((__float_as_uint(scale_most) >> 23) + 1u, 67u), 254u) << 23) : unit;
+                        s_unit[group][0] = now;
+                        s_unit[group][1] = now > 0.0f ? kTrOne / now : 0.0f;
+                        s_set[group] = now_set;
+                    }
                 }
-                if (tid == 0) s_unit = now_unit;
-                unit = now_unit;
-                named_barrier_sync(1, kAll);
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float u0 = __shfl_sync(0xffffffffu, up, r), u1 = __shfl_sync(0xffffffffu, up, r + 1);
+                    const float b0 = __shfl_sync(0xffffffffu, by, r), b1 = __shfl_sync(0xffffffffu, by, r + 1);
+                    o[r] *= b0;
+                    o[r + 1] *= b1;
+                    l[r / 2] = tr_mul2(l[r / 2], pack2(b0, b1));
+                    w[r / 2] = add2(w[r / 2], pack2(-u0, -u1));
+                }
+                named_barrier_sync(1 + group, 128);
             }
-            if (tid == 0) s_fresh[i & 1] = anew || i == 0;
-            const float by = sv * (unit > 0.0f ? kTrOne / unit : 0.0f);
+            const float by = sv * s_unit[group][1];
+            const f32x2 by2 = pack2(by, by);
             uint32_t word[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = tr_ex2(w[r]);
-                l[r] += p;
-                word[r] = __float2uint_rn(p * by);
+            for (int r = 0; r < 8; ++r) {
+                float p0, p1;
+                unpack2(w[r], p0, p1);
+                const f32x2 p = pack2(tr_ex2(p0), tr_ex2(p1));
+                l[r] = add2(l[r], p);
+                unpack2(tr_mul2(p, by2), p0, p1);
+                word[2 * r] = __float2uint_rn(p0);
+                word[2 * r + 1] = __float2uint_rn(p1);
             }
             if (i > 0 && !anew) ok = ok && mbar_wait_bounded(b_values, (unsigned)(i - 1) & 1u);        // (the weights in front were read)
             __syncwarp();
@@ -478,16 +532,21 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
         ok = ok && mbar_wait_bounded(b_values, (unsigned)(n_tiles - 1) & 1u);
         __syncwarp();
         tc_fence_after();
-        move_on(s_unit * (1.0f / kTrOne));
+        move_on(s_unit[group][0] * (1.0f / kTrOne));
         tc_fence_before();
         float mine = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float sum = warp_sum(l[r]);
-            if (lane == r) mine = sum;
+        for (int r = 0; r < 16; r += 2) {
+            float l0, l1;
+            unpack2(l[r / 2], l0, l1);
+            l0 = warp_sum(l0);
+            l1 = warp_sum(l1);
+            if (lane == r) mine = l0;
+            if (lane == r + 1) mine = l1;
         }
         if (lane < 16) s_sum[quarter][first + lane] = mine;
-        named_barrier_sync(1, kAll);
+        named_barrier_sync(1 + group, 128);
+        const uint32_t set = s_set[group];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const long long at = s_at[first + r];
@@ -495,13 +554,13 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
             if (L.n_splits > 1) {
                 if (at >= 0) {
                     L.part_o[((size_t)at * L.n_splits + split) * kK8Hd + key] = o[r];
-                    if (key == 0) L.part_ml[(size_t)at * L.n_splits + split] = make_float2(s_ref[first + r], sum);
+                    if (key == 0) L.part_ml[(size_t)at * L.n_splits + split] = make_float2(set >> r & 1u ? -s_down[first + r] : kTrLow, sum);
                 }
             } else if (at != -1) {
                 const size_t to = (size_t)(at >= 0 ? at : -2 - at);
                 const bool none = at < 0 || sum == 0.0f;
                 a.out[to * kK8Hd + key] = none ? 0.0f : o[r] / sum;
-                if (a.lse && key == 0) a.lse[to] = none ? -INFINITY : (s_ref[first + r] + tr_lg2(sum)) * 0.6931471805599453f;
+                if (a.lse && key == 0) a.lse[to] = none ? -INFINITY : (tr_lg2(sum) - s_down[first + r]) * 0.6931471805599453f;
             }
         }
     }
@@ -580,7 +639,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
     using S = WeighShape<R>;
     const tenzo_attention_tree_args& a = L.a;
     extern __shared__ unsigned char tr_smem[];
-    __shared__ __align__(16) float s_f[R], s_lse[R];
+    __shared__ __align__(16) float s_f[R], s_down[R];    // (the log-sum-exp with its sign turned)
     __shared__ uint32_t s_mask[R][kTrMask];
     __shared__ uint64_t s_full[S::stages], s_empty[S::stages], s_scores[2], s_free[2], s_query;
     __shared__ unsigned s_valid[S::stages];
@@ -609,7 +668,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
             mbar_init(&s_empty[i], S::warps + 1);        // the products, and the warps that read the scales
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_scores[i], 1);
+            mbar_init(&s_scores[i], 2);                  // the products, and the thread that has seen the copies land
             mbar_init(&s_free[i], S::warps);
         }
         mbar_init(&s_query, S::warps);
@@ -634,14 +693,15 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
             const uint64_t dq = umma_desc_sw128(smem_addr(s_q));
             for (int n = 0; n < steps && ok; ++n) {
                 const int st = n % S::stages, half = n & 1;
-                if (n % n_tiles == 0) ok = ok && mbar_spin_bounded(&s_query, (unsigned)(n / n_tiles) & 1u);
+                if (n % n_tiles == 0) ok = mbar_spin_bounded(&s_query, (unsigned)(n / n_tiles) & 1u);
                 ok = ok && mbar_spin_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n < 2 || mbar_spin_bounded(&s_free[half], (unsigned)(n / 2 - 1) & 1u));
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * kTrTileBytes));
 #pragma unroll
-                for (int k = 0; k < kK8Hd / 32; ++k) umma_i8(tmem + half * S::s_cols, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), d_scores, k > 0);
+                for (int k = 0; k < kK8Hd / 32; ++k) umma_i8(tmem + half * S::s_cols, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), d_scores, 1u);
                 umma_commit(&s_scores[half]);
+                mbar_arrive(&s_scores[half]);
                 umma_commit(&s_empty[st]);
             }
         }
@@ -651,6 +711,10 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
         constexpr int kAll = S::warps * 32;
         const uint32_t t_scores = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)first;
         float* sums = s_sum + (warp >> 2) * kTwTiles * kTrTile + key;
+#pragma unroll
+        for (int part = 0; part < 6; ++part) tr_fill<16>(t_scores + part * R, kTrBias);
+        tmem_wait_st();
+        tc_fence_before();
         for (int n = 0; n < steps; ++n) {
             const int i = n % n_tiles, pass = n / n_tiles, st = n % S::stages, half = n & 1;
             if (i == 0) {                                // the next queries; the products with the ones in front are done
@@ -667,7 +731,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                             if (!(fabsf(lse) < INFINITY)) lse = INFINITY;
                         }
                     }
-                    s_lse[r] = lse;
+                    s_down[r] = -lse;
                     for (int w = 0; w < (a.nodes + 31) / 32; ++w)
                         s_mask[r][w] = flat >= queries ? 0u : a.mask ? (uint32_t)ld_l2(a.mask + row * a.mask_stride + w) : node >= 32 * w + 31 ? 0xffffffffu : node < 32 * w ? 0u : (2u << (node - 32 * w)) - 1u;
                 }
@@ -677,7 +741,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                     const int r = warp + j * S::warps, flat = pass * R + r, node = flat / L.group;
                     const size_t row = (size_t)s * a.nodes + node;
                     float f = 0.0f;
-                    if (s_lse[r] < INFINITY) {
+                    if (s_down[r] > -INFINITY) {
                         f = tr_query<R>(a, row, kvh * L.group + flat % L.group, a.rope_pos ? ld_l2(a.rope_pos + row) : q.start + node, s_q, r);
                     } else {
                         for (int part = 0; part < 3; ++part) reinterpret_cast<uint32_t*>(s_q + (part * R + r) * kK8Hd)[lane] = 0;
@@ -688,7 +752,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                 named_barrier_sync(1, kAll);
                 if (lane == 0) mbar_arrive(&s_query);
             }
-            ok = ok && mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && mbar_wait_bounded(&s_scores[half], (unsigned)(n / 2) & 1u);
+            ok = ok && mbar_wait_bounded(&s_scores[half], (unsigned)(n / 2) & 1u);
             __syncwarp();
             const int t = c_begin + i * kTrTile + key;
             const unsigned valid = s_valid[st];
@@ -696,26 +760,25 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
             float sk = dead ? 0.0f : s_scales[st * kTrTile + key];
             if (!(fabsf(sk) < INFINITY)) sk = 0.0f;      // (no query that sees it has a finite lse)
             tc_fence_after();
-            float x[16];
-            tr_arguments<R>(t_scores + half * S::s_cols, s_f + first, sk, x);
+            f32x2 w[8];
+            tr_arguments<R>(t_scores + half * S::s_cols, s_f + first, s_down + first, sk, w);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&s_free[half]);
                 mbar_arrive(&s_empty[st]);
             }
-            if (ragged) {
-                const int j = t - q.start;
+            if (ragged) tr_hide(w, s_mask + first, t - q.start, dead);
+            f32x2 sum2 = 0;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (dead || (j >= 0 && !(s_mask[first + r][j >> 5] >> (j & 31) & 1u))) x[r] = -INFINITY;
+            for (int r = 0; r < 8; ++r) {
+                float w0, w1;
+                unpack2(w[r], w0, w1);
+                sum2 = add2(sum2, pack2(tr_ex2(w0), tr_ex2(w1)));
             }
-            float sum = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const float4 m = *reinterpret_cast<const float4*>(s_lse + first + r);
-                sum += (tr_ex2(x[r] - m.x) + tr_ex2(x[r + 1] - m.y)) + (tr_ex2(x[r + 2] - m.z) + tr_ex2(x[r + 3] - m.w));
-            }
+            float sum, other;
+            unpack2(sum2, sum, other);
+            sum += other;
             sums[i * kTrTile] = pass == 0 ? sum : sums[i * kTrTile] + sum;
         }
         named_barrier_sync(1, kAll);
