@@ -390,21 +390,19 @@ typedef struct {
     int q_stride;            /* floats between rows; 0 = n_q*128 */
     int mask_stride;         /* words between rows; 0 = ceil(nodes / 32) */
     int layer, n_q, sequences, nodes;
-    int max_len;             /* upper bound on start + count (sizes the grid); at most slots * table_stride */
-    int split_keys;          /* keys a CTA takes (rounded up to 128); 0 = choose */
+    int max_len;             /* upper bound on start + count; at most slots * table_stride, and 2^30 (-5) */
+    int shares;              /* equal shares that the keys of all sequences and kv heads are cut into, each of one CTA (or some, for many queries); 0 = choose, at most 65535 */
     int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
-    void* workspace;         /* 16-byte aligned, contents need not be kept: partial results of splits; NULL: none */
-    size_t workspace_bytes;  /* sequences * nodes * n_q * 520 a split; with less fewer splits are taken, and split_keys that need more are refused (-1). Enough for any
-                                split_keys: tenzo_cuda_attention_tree_workspace_bytes(...); for split_keys 0: 520 * sequences * nodes * n_q *
-                                tenzo_cuda_attention_tree_splits(...), nothing at 1 */
+    void* workspace;         /* 16-byte aligned, contents need not be kept: partial results where a cut goes through a sequence's keys */
+    size_t workspace_bytes;  /* tenzo_cuda_attention_tree_workspace_bytes(...), some MB whatever the lengths are. With less, or NULL, shares end with a sequence's kv head, which is
+                                slower for few sequences and for unequal ones; shares > 0 is refused then (-1) */
 } tenzo_attention_tree_args;
 TENZO_API int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, void* stream);
-TENZO_API size_t tenzo_cuda_attention_tree_workspace_bytes(int sequences, int nodes, int n_q, int max_len);
-/* Splits that the call's own choice (split_keys 0) wants room for; 1: none, 0: arguments that the call refuses. */
-TENZO_API int tenzo_cuda_attention_tree_splits(int sequences, int nodes, int n_q, int n_kv, int max_len);
+/* (0 for arguments that the call refuses.) */
+TENZO_API size_t tenzo_cuda_attention_tree_workspace_bytes(int sequences, int nodes, int n_q, int n_kv, int shares);
 
 /* The attention weight that each cached token receives: weight[token] += sum over the nodes that see it and the query heads of its kv head of exp(s - lse), s the
- * argument of softmax above. args as for tenzo_cuda_attention_tree, whose lse this reads; out, workspace and split_keys are not used. weight is laid out as the scales.
+ * argument of softmax above. args as for tenzo_cuda_attention_tree, whose lse this reads; out, workspace and shares are not used. weight is laid out as the scales.
  * A row whose lse is not finite adds nothing. Every sum is taken in one order: equal calls give equal bits. No two sequences of a call may name the same table row. */
 TENZO_API int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float* weight, void* stream);
 

@@ -93,7 +93,7 @@ class AttentionTreeArgs(C.Structure):
         ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("cache", Kv8Cache),
         ("start", C.c_void_p), ("count", C.c_void_p), ("seq", C.c_void_p), ("mask", C.c_void_p), ("rope_pos", C.c_void_p),
         ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rope_len", C.c_int), ("q_stride", C.c_int), ("mask_stride", C.c_int),
-        ("layer", C.c_int), ("n_q", C.c_int), ("sequences", C.c_int), ("nodes", C.c_int), ("max_len", C.c_int), ("split_keys", C.c_int), ("use_pdl", C.c_int),
+        ("layer", C.c_int), ("n_q", C.c_int), ("sequences", C.c_int), ("nodes", C.c_int), ("max_len", C.c_int), ("shares", C.c_int), ("use_pdl", C.c_int),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
@@ -128,7 +128,7 @@ KERNEL_SYMBOLS = [
     "tenzo_cuda_topk_candidates", "tenzo_cuda_topk_max_candidates",
     "tenzo_cuda_kv4_append", "tenzo_cuda_kv4_read", "tenzo_cuda_kv4_reorder", "tenzo_cuda_kv4_take_errors", "tenzo_cuda_attention_kv4",
     "tenzo_cuda_attention_kv4_workspace_bytes", "tenzo_cuda_attention_kv4_splits", "tenzo_cuda_beam_select", "tenzo_cuda_beam_select_workspace_bytes",
-    "tenzo_cuda_kv8_append", "tenzo_cuda_attention_tree", "tenzo_cuda_attention_tree_workspace_bytes", "tenzo_cuda_attention_tree_splits", "tenzo_cuda_kv8_weigh",
+    "tenzo_cuda_kv8_append", "tenzo_cuda_attention_tree", "tenzo_cuda_attention_tree_workspace_bytes", "tenzo_cuda_kv8_weigh",
     "tenzo_cuda_kv8_evict", "tenzo_cuda_kv8_accept", "tenzo_cuda_kv8_take_errors",
 ]
 HAL_SYMBOLS = ["tenzo_hal_initialize", "tenzo_hal_bitlinear_tl1_host", "tenzo_hal_rmsnorm_host", "tenzo_hal_gemm_f32_host", "tenzo_hal_call_count"]
@@ -235,8 +235,7 @@ def declare_kernel_abi(L):
     L.tenzo_cuda_kv8_evict.argtypes = [kv8, vp, vp, vp, vp, vp, i32, i32, i32, vp, i32, vp]
     L.tenzo_cuda_kv8_accept.argtypes = [kv8, vp, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, vp, i32, vp]
     L.tenzo_cuda_attention_tree.restype, L.tenzo_cuda_attention_tree.argtypes = i32, [tree, vp]
-    L.tenzo_cuda_attention_tree_workspace_bytes.restype, L.tenzo_cuda_attention_tree_workspace_bytes.argtypes = sz, [i32, i32, i32, i32]
-    L.tenzo_cuda_attention_tree_splits.restype, L.tenzo_cuda_attention_tree_splits.argtypes = i32, [i32, i32, i32, i32, i32]
+    L.tenzo_cuda_attention_tree_workspace_bytes.restype, L.tenzo_cuda_attention_tree_workspace_bytes.argtypes = sz, [i32, i32, i32, i32, i32]
     L.tenzo_cuda_kv8_weigh.restype, L.tenzo_cuda_kv8_weigh.argtypes = i32, [tree, vp, vp]
     L.tenzo_cuda_kv8_take_errors.restype, L.tenzo_cuda_kv8_take_errors.argtypes = i32, []
     L.tenzo_cuda_lm_head_scratch_bytes.restype, L.tenzo_cuda_lm_head_scratch_bytes.argtypes = sz, [i32]

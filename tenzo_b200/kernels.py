@@ -403,16 +403,17 @@ assert _KV8_CACHE.size == C.sizeof(abi.Kv8Cache) and _ATTENTION_TREE.size == C.s
 
 @functools.cache
 def _tree_calls():
-    """tenzo_cuda_kv8_append, _evict, _accept, tenzo_cuda_attention_tree, tenzo_cuda_kv8_weigh and the attention's choice of splits, with prototypes of this module's own,
-    whose structs are the bytes of a struct.Struct."""
-    def fn(name, *argtypes):
+    """tenzo_cuda_kv8_append, _evict, _accept, tenzo_cuda_attention_tree, tenzo_cuda_kv8_weigh and the attention's workspace, with prototypes of this module's own, whose structs
+    are the bytes of a struct.Struct."""
+    def fn(name, *argtypes, restype=C.c_int):
         f = load_library()[name]
-        f.restype, f.argtypes = C.c_int, list(argtypes)
+        f.restype, f.argtypes = restype, list(argtypes)
         return f
     return (fn("tenzo_cuda_kv8_append", _PB, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PP, _PP, _PP, _PI, _PP, _PP, _PI, _PP),
             fn("tenzo_cuda_kv8_evict", _PB, _PP, _PP, _PP, _PP, _PP, _PI, _PI, _PI, _PP, _PI, _PP),
             fn("tenzo_cuda_kv8_accept", _PB, _PP, _PP, _PP, _PP, _PP, _PP, _PI, _PI, _PP, _PP, _PP, _PP, _PP, _PI, _PP),
-            fn("tenzo_cuda_attention_tree", _PB, _PP), fn("tenzo_cuda_kv8_weigh", _PB, _PP, _PP), fn("tenzo_cuda_attention_tree_splits", _PI, _PI, _PI, _PI, _PI))
+            fn("tenzo_cuda_attention_tree", _PB, _PP), fn("tenzo_cuda_kv8_weigh", _PB, _PP, _PP),
+            fn("tenzo_cuda_attention_tree_workspace_bytes", _PI, _PI, _PI, _PI, _PI, restype=C.c_size_t))
 
 
 def _kv8_cache(cache: Kv8Cache, device: int):
@@ -457,10 +458,8 @@ def kv8_append(k, v, cache, place, *, layer, seq=None, rope_pos=None, rope_cos=N
 
 
 @functools.lru_cache(1024)
-def _attention_tree_room(sequences, nodes, n_q, n_kv, max_len, split_keys) -> int:
-    """What one call needs: splits of split_keys keys, or as many as it chooses itself."""
-    splits = -(-max_len // (-(-split_keys // 128) * 128)) if split_keys > 0 else _tree_calls()[5](sequences, nodes, n_q, n_kv, max_len)
-    return sequences * nodes * n_q * 520 * splits if splits > 1 else 0
+def attention_tree_workspace_bytes(sequences, nodes, n_q, n_kv, shares=0) -> int:
+    return _tree_calls()[5](sequences, nodes, n_q, n_kv, shares)
 
 
 def _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev):
@@ -484,7 +483,7 @@ def _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos,
 
 
 def attention_tree(q, cache, start, *, layer, n_q, nodes, count=None, mask=None, seq=None, rope_pos=None, rope_cos=None, rope_sin=None, max_len=None, want_lse=False,
-                   split_keys=0, use_pdl=False, out=None, lse=None, workspace=None):
+                   shares=0, use_pdl=False, out=None, lse=None, workspace=None):
     """Attention of the nodes of trees: q [sequences*nodes, n_q*128] over the tokens at places 0 .. start[s] - 1 of sequence s and, of the tree's own at start[s] + j, those
     whose bit j % 32 of mask[row, j / 32] is set (int32 [rows, words]; default: nodes 0 .. i, a chain). start, count int32 [sequences]: tokens that are cached, and nodes
     that are there (default: all); rope_pos int32 [rows]: the queries' rotary positions (default: start + i). Returns out [rows, n_q*128], zeros where nothing is seen;
@@ -500,11 +499,9 @@ def attention_tree(q, cache, start, *, layer, n_q, nodes, count=None, mask=None,
     elif lse.shape != (rows, n_q):
         raise ValueError(f"lse is [{rows}, {n_q}]")
     if workspace is None:
-        size = _attention_tree_room(sequences, nodes, n_q, fields[6], fields[-1], split_keys)
-        if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-    args = _ATTENTION_TREE.pack(qp, _arg(out, torch.float32, dev, "out"), _arg(lse, torch.float32, dev, "lse"), *fields, _arg_int(split_keys, "split_keys"), use_pdl,
-                                _arg(workspace, torch.uint8, dev, "workspace"), 0 if workspace is None else workspace.numel())
+        workspace = torch.empty(attention_tree_workspace_bytes(sequences, nodes, n_q, fields[6], shares), dtype=torch.uint8, device=q.device)
+    args = _ATTENTION_TREE.pack(qp, _arg(out, torch.float32, dev, "out"), _arg(lse, torch.float32, dev, "lse"), *fields, _arg_int(shares, "shares"), use_pdl,
+                                _arg(workspace, torch.uint8, dev, "workspace"), workspace.numel())
     _ok(_tree_calls()[3](args, _raw_stream(dev)), "tenzo_cuda_attention_tree")
     return out if lse is None else (out, lse)
 

@@ -119,26 +119,43 @@ def test_tree_and_weights(cuda_lib, starts, counts, nodes, n_q, n_kv, further):
     assert kernels.kv8_take_errors() == 0
 
 
-@pytest.mark.parametrize("nodes,n_q", [(1, 20), (12, 20), (64, 20)])
-@pytest.mark.parametrize("split_keys", [128, 384, 1000])
-def test_splits(cuda_lib, nodes, n_q, split_keys):
-    """Splits of any size give what one does, the ones behind a short sequence's end among them."""
+@pytest.mark.parametrize("nodes,n_q", [(1, 20), (8, 20), (12, 20), (64, 20), (40, 40)])
+@pytest.mark.parametrize("shares", [1, 2, 7, 13, 64, 1000])
+def test_shares(cuda_lib, nodes, n_q, shares):
+    """Cuts anywhere give what whole sequences do: several in one sequence's keys, several sequences between two, shares that nothing is left for."""
     from tenzo_b200 import kernels
-    case = Case(split_keys + nodes, [1500, 100, 640, 0], [nodes, nodes, max(1, nodes - 3), nodes], nodes, n_q, 5)
+    case = Case(shares + nodes, [1500, 100, -1, 640, 0, 3], [nodes, nodes, nodes, max(1, nodes - 3), nodes, 0], nodes, n_q, 5)
     cache, start, a = case.arguments()
-    out, lse = kernels.attention_tree(dev(case.q), cache, start, want_lse=True, split_keys=split_keys, **a)
+    out, lse = kernels.attention_tree(dev(case.q), cache, start, want_lse=True, shares=shares, **a)
     case.check(out, lse)
 
 
-def test_no_room_for_splits(cuda_lib):
+def test_many_sequences(cuda_lib):
+    """More sequences than a block has threads, most of them short, some empty."""
     from tenzo_b200 import kernels
-    case = Case(1, [3000], [4], 4, 20, 5)
+    rng = np.random.default_rng(5)
+    starts = [int(x) for x in rng.integers(-3, 40, 900)]
+    starts[700], starts[899] = 300, 200
+    case = Case(51, starts, [int(x) for x in rng.integers(0, 3, 900)], 2, 4, 2)
     cache, start, a = case.arguments()
-    for size in (0, 100, 520 * 4 * 20 * 3):
+    want = case.want()
+    for shares in (0, 5, 300):
+        out, lse = kernels.attention_tree(dev(case.q), cache, start, want_lse=True, shares=shares, **a)
+        case.check(out, lse, want)
+    weight = dev(case.c.weight)
+    kernels.kv8_weigh(dev(case.q), lse, cache, weight, start, **a)
+    assert abs(float(weight.double().sum()) - case.c.weight.astype(np.float64).sum() - (~np.isneginf(want[1])).sum()) < 1e-2
+
+
+def test_no_room_for_cuts(cuda_lib):
+    from tenzo_b200 import kernels
+    case = Case(1, [3000, 10, 400], [4, 4, 2], 4, 20, 5)
+    cache, start, a = case.arguments()
+    for size in (0, 100, 5000):
         out, lse = kernels.attention_tree(dev(case.q), cache, start, want_lse=True, workspace=torch.empty(size, dtype=torch.uint8, device="cuda"), **a)
         case.check(out, lse)
     with pytest.raises(RuntimeError):
-        kernels.attention_tree(dev(case.q), cache, start, split_keys=256, workspace=torch.empty(520 * 4 * 20 * 3, dtype=torch.uint8, device="cuda"), **a)
+        kernels.attention_tree(dev(case.q), cache, start, shares=20, workspace=torch.empty(5000, dtype=torch.uint8, device="cuda"), **a)
 
 
 def test_growing_scores(cuda_lib):

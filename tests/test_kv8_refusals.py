@@ -80,7 +80,8 @@ def test_tree_and_weigh(lib, over):
     assert lib.tenzo_cuda_kv8_weigh(C.byref(a), P, None) == abi.ERR_INVALID
 
 
-@pytest.mark.parametrize("over", [dict(out=None), dict(out=P + 4), dict(split_keys=-1)], ids=str)
+@pytest.mark.parametrize("over", [dict(out=None), dict(out=P + 4), dict(shares=-1), dict(shares=65536), dict(shares=3), dict(shares=3, workspace=P + 8, workspace_bytes=1 << 30),
+                                  dict(shares=3, workspace=P, workspace_bytes=100)], ids=str)
 def test_tree_alone(lib, over):
     assert lib.tenzo_cuda_attention_tree(C.byref(tree(**over)), None) == abi.ERR_INVALID
 
@@ -95,15 +96,14 @@ def test_too_many_nodes(lib):
     assert lib.tenzo_cuda_attention_tree(C.byref(a), None) == lib.tenzo_cuda_kv8_weigh(C.byref(a), P, None) == accept(lib, cache(), nodes=257) == abi.ERR_UNSUPPORTED
 
 
-def test_room_for_splits(lib):
-    splits, need = lib.tenzo_cuda_attention_tree_splits, lib.tenzo_cuda_attention_tree_workspace_bytes
-    assert splits(0, 4, 4, 2, 10) == splits(1, 0, 4, 2, 10) == splits(1, 257, 4, 2, 10) == splits(1, 4, 0, 2, 10) == splits(1, 4, 5, 2, 10) == splits(1, 4, 4, 2, 0) == 0
-    assert need(0, 4, 4, 10) == need(1, 0, 4, 10) == need(1, 4, 0, 10) == need(1, 4, 4, 0) == 0
-    for sequences, nodes, n_q, n_kv, n in ((1, 1, 20, 5, 30000), (1, 64, 20, 5, 16384), (64, 16, 20, 5, 4096), (3, 256, 7, 1, 1 << 20), (1, 1, 1, 1, 1), (5000, 3, 32, 32, 2000)):
-        most = splits(sequences, nodes, n_q, n_kv, n)
-        assert 1 <= most and (most == 1 or most * 520 * sequences * nodes * n_q <= need(sequences, nodes, n_q, n))
-        assert kernels._attention_tree_room(sequences, nodes, n_q, n_kv, n, 0) == (most * 520 * sequences * nodes * n_q if most > 1 else 0)
-    assert kernels._attention_tree_room(2, 3, 4, 2, 1000, 128) == 8 * 2 * 3 * 4 * 520 and kernels._attention_tree_room(2, 3, 4, 2, 1000, 900) == 0       # 900: rounded up to 1024
+def test_workspace(lib):
+    need = lib.tenzo_cuda_attention_tree_workspace_bytes
+    assert need(0, 4, 4, 2, 0) == need(1, 0, 4, 2, 0) == need(1, 257, 4, 2, 0) == need(1, 4, 0, 2, 0) == need(1, 4, 5, 2, 0) == need(1, 4, 4, 2, -1) == need(1, 4, 4, 2, 65536) == 0
+    for sequences, nodes, n_q, n_kv in ((1, 1, 20, 5), (1, 64, 20, 5), (64, 16, 20, 5), (3, 256, 7, 1), (1, 1, 1, 1), (5000, 3, 32, 32), (2, 256, 64, 1)):
+        room = need(sequences, nodes, n_q, n_kv, 0)
+        assert 0 < room - 8 * sequences * n_kv < 64 << 20 and room == kernels.attention_tree_workspace_bytes(sequences, nodes, n_q, n_kv)
+        assert need(sequences, nodes, n_q, n_kv, 7) < need(sequences, nodes, n_q, n_kv, 9)
+    assert need(2, 1, 4, 2, 10) == 48 + 10 * 2 * 16 * 520                       # 1 + 2 * 2 words, and two sets of sixteen rows a share
 
 
 @pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(length=None), -1), (dict(out=None), -1), (dict(out=P), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
