@@ -4,11 +4,11 @@
 //     the queries as columns: S^T = K Q^T and O^T = V^T P^T. A CTA takes 16, 32 or 64 of the queries and walks its keys in tiles of 128. With keys as rows a single
 //     query fills the tensor cores as well as many do, and one kernel serves a decode step and a tree of 64 nodes.
 //   * Both are products of whole numbers (tcgen05 kind::i8, sums of 32 bits), and the codes of the cache are operands as they lie: K and V tiles go from memory to shared
-//     memory to the tensor cores, nothing is unpacked or converted. A query is scaled to a maximum of 2^22 - 1 and rounded; its three signed bytes are three columns. A weight, p * scale of its
+//     memory to the tensor cores, nothing is unpacked or converted. A query is scaled to a maximum of 2^21 to 2^22 and rounded; its three signed bytes are three columns. A weight, p * scale of its
 //     value, is rounded to a whole number of 31 bits; its four bytes, as they lie in the register, are four columns. So P is stored as it is computed, 16 bytes for four queries, and its
-//     operand and V's are both read transposed (MN-major). Sums are exact: what rounds is the query (2^-23 of its largest number), the weights (2^-28 of a row's largest) and fp32 in between.
+//     operand and V's are both read transposed (MN-major). Sums are exact: what rounds is the query (2^-22 of its largest number), the weights (2^-27 of a row's largest) and fp32 in between.
 //   * softmax: a thread has one key and sixteen queries, so a row's maximum goes across lanes; and accumulators of whole numbers cannot be scaled down.
-//     Both are avoided: a row's weights are taken relative to a reference, the maximum when it was last set, and may grow to 2^4 of it. Only where a weight would pass that (one vote a
+//     Both are avoided: a row's weights are taken relative to a reference, the maximum when it was last set, and may grow to 2^5 of it. Only where a weight would pass that (one vote a
 //     tile; the first tile always) the references are set anew and the accumulators moved on into fp32.
 #include "attn_common.cuh"
 #include "kv8.cuh"
@@ -18,7 +18,7 @@ namespace tz {
 
 constexpr int kTrTile = 128, kTrTileBytes = kTrTile * kK8Hd;          // keys a step; bytes of their codes
 constexpr int kTrMask = TENZO_TREE_MOST / 32;
-constexpr float kTrSlack = 4.0f, kTrOne = 134217728.0f;               // a weight of 1 is 2^27, weights up to 2^4 are let through
+constexpr float kTrSlack = 5.0f, kTrOne = 67108864.0f;                // a weight of 1 is 2^26, weights up to 2^5 are let through
 constexpr float kTrLow = -1e30f;                                      // a reference that is not set
 constexpr uint32_t kTrShape = (2u << 4) | (1u << 7) | ((uint32_t)(kTrTile >> 4) << 24);      // of products: sums of 32 bits; codes, with a sign, as A; 128 rows
 constexpr int kTrFlush = 256;                                         // tiles after which the accumulators are moved on all the same: 2^15 keys * 128 * 255 < 2^31
@@ -32,6 +32,7 @@ struct TreeLaunch {
     tenzo_attention_tree_args a;
     int group, tiles, shares;                            // heads a kv head; CTAs for a tree's queries; shares of the keys
     int cut;                                             // shares end anywhere; otherwise with a pair
+    int aligned;                                         // queries and tables, to 16 bytes
     long long* head;                                     // [0]: tiles a share; [1 + pair]: the pair's first tile, -1 where no cut goes through it
     float* part_o;                                       // [share][tile][2][R][128]
     float2* part_ml;                                     // [share][tile][2][R]: reference (log2), sum
@@ -41,9 +42,13 @@ struct TreeLaunch {
 // R queries a CTA.
 template <int R>
 struct TreeShape {
-    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 3) * 32;      // four warps for sixteen queries; one that copies, two that issue products
+    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 4) * 32;      // four warps for sixteen queries; one that copies, two that issue products, and one to four of them
     static constexpr int stages = R > 32 ? 3 : 2, resident = R > 32 ? 1 : 2;
-    static constexpr int s_cols = 3 * R, o_cols = 4 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;
+    static constexpr int s_cols = 3 * R, o_cols = 4 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;       // and R for outputs that were moved on
+    static_assert(s_cols + o_cols + R <= tmem_cols, "tensor memory");
+    // Registers a thread: as the block is launched, and after the warps of the second line have given some to those of the first.
+    static constexpr int launched = R == 64 ? 96 : R == 48 ? 128 : R == 32 ? 80 : 128, most = R == 64 ? 112 : R == 48 ? 144 : R == 32 ? 104 : 168, least = R == 48 ? 40 : R == 16 ? 64 : 32;
+    static_assert(warps * most + 4 * least <= (warps + 4) * launched, "what is taken is there");
     static constexpr int p_panels = R > 32 ? 2 : 1;                   // of 128 bytes: 32 queries
     static constexpr int q_bytes = s_cols * kK8Hd, p_bytes = p_panels * kTrTileBytes;
     static constexpr size_t smem = 1024 + (size_t)stages * 2 * kTrTileBytes + q_bytes + p_bytes + stages * 2 * kTrTile * 4;
@@ -74,6 +79,10 @@ __device__ __forceinline__ void tr_wait8(uint32_t (&r)[8]) {
 }
 __device__ __forceinline__ void tr_tie8(uint32_t (&r)[8]) {
     asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
+__device__ __forceinline__ void tr_st8(uint32_t at, const float (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(at), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]) : "memory");
 }
 // Operand tiles that are contiguous along M or N (rows of 128 bytes, one for each k), 128-byte swizzle: eight k are 1024 bytes, `panel` bytes from one 128 to the next.
 __device__ __forceinline__ uint64_t tr_desc_mn(uint32_t saddr, uint32_t panel) {
@@ -218,36 +227,66 @@ struct TreeWalk {
 };
 
 // ---- the parts that both kernels have ------------------------------------------------------------------------------------------
-// Query `flat` = node * group + head of the group: rotated, rounded to whole numbers of 23 bits, its bytes as rows r, R + r, 2R + r of the operand (128 bytes each, swizzled). One
-// warp; returns what a unit of the products with the codes counts in the argument of 2^x (NaN for a query that is not finite).
-template <int R>
-__device__ __forceinline__ float tr_query(const tenzo_attention_tree_args& a, size_t row, int head, int pos, unsigned char* s_q, int r) {
-    const int lane = threadIdx.x & 31;
-    const float* q = a.q + row * a.q_stride + (size_t)head * kK8Hd + lane;
-    float x[4];
+// R queries of a block on their way to the operand, four by each of its R / 4 warps. A lane has dims 4 lane .. 4 lane + 3, and the lane sixteen on, or back, those that they are turned
+// with. A vector is turned, scaled by a power of two to a maximum between 2^21 and 2^22 and rounded; its signed bytes are rows r, R + r, 2R + r of the operand (128 bytes each, swizzled).
+// s_f: what a unit of the products with the codes counts in the argument of 2^x (NaN for a query that is not finite). from[r]: the vector in q, -1: none, zeros.
+// (Every load is made, of something, without a branch around it: where two ways meet the compiler copies what was loaded, and so waits for it. 3500 cycles for a block's loads that way, 900 this.)
+template <int R, bool VEC>
+__device__ __forceinline__ void tr_queries(const TreeLaunch& L, const long long* from, const int* pos, unsigned char* s_q, float* s_f) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool rotate = L.a.rope_cos != nullptr;
+    auto load4 = [](const float* p, float (&v)[4]) {
+        if (VEC) {
+            const float4 w = ld_l2(reinterpret_cast<const float4*>(p));
+            v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+        } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = ld_l2(q + 32 * j);             // dims lane + 32 j; pairs (0, 2) and (1, 3)
-    if (a.rope_cos) {
+            for (int j = 0; j < 4; ++j) v[j] = ld_l2(p + j);
+        }
+    };
+    float x[4][4], c[4][4], s[4][4];
+    long long at[4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float c = ld_l2(a.rope_cos + (size_t)pos * 64 + 32 * j + lane), s = ld_l2(a.rope_sin + (size_t)pos * 64 + 32 * j + lane);
-            rope_rotate(x[j], x[j + 2], true, c, s, x[j], x[j + 2]);
+    for (int i = 0; i < 4; ++i) at[i] = from[warp + i * (R / 4)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float* q = L.a.q + max(at[i], 0LL);
+        const size_t turn = (size_t)(at[i] < 0 ? 0 : pos[warp + i * (R / 4)]) * 64 + 4 * (lane & 15);
+        load4(q + 4 * lane, x[i]);
+        load4(rotate ? L.a.rope_cos + turn : q, c[i]);
+        load4(rotate ? L.a.rope_sin + turn : q, s[i]);
+    }
+    float most[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float other = __shfl_xor_sync(0xffffffffu, x[i][j], 16);
+            const float turned = lane < 16 ? __fmaf_rn(x[i][j], c[i][j], -(other * s[i][j])) : __fmaf_rn(other, s[i][j], x[i][j] * c[i][j]);
+            if (rotate) x[i][j] = turned;
         }
     }
-    const float most = fmaxf(tr_warp_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))), 1e-25f);
-    const bool bad = __any_sync(0xffffffffu, !(fabsf(x[0]) < INFINITY && fabsf(x[1]) < INFINITY && fabsf(x[2]) < INFINITY && fabsf(x[3]) < INFINITY));
-    const float up = 4194303.0f / most;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int v = bad ? 0 : __float2int_rn(x[j] * up), d3 = ((v + 128) & 255) - 128, m = (v - d3) >> 8, d2 = ((m + 128) & 255) - 128, d1 = (m - d2) >> 8;
-        const int d = lane + 32 * j, chunk = d >> 4;
+    for (int i = 0; i < 4; ++i) most[i] = fmaxf(tr_warp_max(fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])))), 1e-25f);
 #pragma unroll
-        for (int part = 0; part < 3; ++part) {
+    for (int i = 0; i < 4; ++i) {
+        const bool bad = __any_sync(0xffffffffu, !(fabsf(x[i][0]) < INFINITY && fabsf(x[i][1]) < INFINITY && fabsf(x[i][2]) < INFINITY && fabsf(x[i][3]) < INFINITY));
+        const int r = warp + i * (R / 4);
+        const uint32_t e = __float_as_uint(most[i]) >> 23;           // 43 .. 254
+        const float up = bad || at[i] < 0 ? 0.0f : __uint_as_float((275u - e) << 23);
+        int v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __float2int_rn(x[i][j] * up);          // (NaN: 0)
+#pragma unroll
+        for (int part = 2; part >= 0; --part) {          // the last byte, with its sign; what it leaves, in 256ths; again
             const int n = part * R + r;
-            s_q[n * kK8Hd + ((chunk ^ (n & 7)) << 4) + (d & 15)] = (unsigned char)(part == 0 ? d1 : part == 1 ? d2 : d3);
+            const uint32_t word = prmt(prmt((uint32_t)v[0], (uint32_t)v[1], 0x0040u), prmt((uint32_t)v[2], (uint32_t)v[3], 0x0040u), 0x5410u);
+            *reinterpret_cast<uint32_t*>(s_q + n * kK8Hd + (((lane >> 2) ^ (n & 7)) << 4) + 4 * (lane & 3)) = word;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (v[j] + 128) >> 8;
         }
+        if (lane == 0) s_f[r] = at[i] < 0 ? 0.0f : bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 21u) << 23) * (0.08838834764831845f * 1.4426950408889634f);
     }
-    return bad ? __uint_as_float(0x7fc00000u) : most * (1.0f / 4194303.0f) * (0.08838834764831845f * 1.4426950408889634f);
 }
 
 // The warp that copies: sixteen keys a lane of eight, a tile's codes and scales into one stage after the other. A block whose table entry is out of range is left out (its bit in s_valid
@@ -311,11 +350,20 @@ struct TreeCopies {
     }
 };
 
-// Row r of a block's queries: which bits of which nodes it sees.
-__device__ __forceinline__ void tr_masks(const tenzo_attention_tree_args& a, size_t row, int node, bool there, uint32_t (&mask)[kTrMask]) {
-    for (int w = 0; w < (a.nodes + 31) / 32; ++w)
-        mask[w] = !there ? 0u : a.mask ? (uint32_t)ld_l2(a.mask + row * a.mask_stride + w) : node >= 32 * w + 31 ? 0xffffffffu : node < 32 * w ? 0u : (2u << (node - 32 * w)) - 1u;
-}
+// What a row sees of its tree, word by word; nothing where it is not there.
+struct TreeMask {
+    uint32_t word[kTrMask];
+    __device__ __forceinline__ void load(const tenzo_attention_tree_args& a, size_t row, int node) {
+#pragma unroll
+        for (int w = 0; w < kTrMask; ++w)
+            if (32 * w < a.nodes) word[w] = a.mask ? (uint32_t)ld_l2(a.mask + row * a.mask_stride + w) : node >= 32 * w + 31 ? 0xffffffffu : node < 32 * w ? 0u : (2u << (node - 32 * w)) - 1u;
+    }
+    __device__ __forceinline__ void store(const tenzo_attention_tree_args& a, bool there, uint32_t (&mask)[kTrMask]) const {
+#pragma unroll
+        for (int w = 0; w < kTrMask; ++w)
+            if (32 * w < a.nodes) mask[w] = there ? word[w] : 0u;
+    }
+};
 
 // For sixteen queries (columns of each part), two by two, and the lane's key, whose scale is sk: arguments of 2^x less what `down` (with its sign turned) says. The
 // accumulators are left as they have to start.
@@ -343,6 +391,22 @@ __device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, co
     tmem_wait_st();
 }
 
+// Sums over the warp of sixteen numbers a lane: that of number lane / 2.
+__device__ __forceinline__ float tr_sums(const f32x2 (&l)[8]) {
+    float v[16];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) unpack2(l[r], v[2 * r], v[2 * r + 1]);
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 16; o > 1; o >>= 1) {                   // half of the numbers go to the other half of the lanes
+#pragma unroll
+        for (int r = 0; r < o / 2; ++r) {
+            const float keep = lane & o ? v[r + o / 2] : v[r], give = lane & o ? v[r] : v[r + o / 2];
+            v[r] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+}
 // Queries that do not see the lane's key: node j of the tree (below 0: a cached token, which all see), or `dead`, none.
 __device__ __forceinline__ void tr_hide(f32x2 (&w)[8], const uint32_t (*mask)[kTrMask], int j, bool dead) {
 #pragma unroll
@@ -363,8 +427,9 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     const tenzo_attention_tree_args& a = L.a;
     extern __shared__ unsigned char tr_smem[];
     __shared__ __align__(16) float s_f[R], s_down[R], s_max[4][R], s_sum[4][R], s_scale_max[S::groups][4];    // (s_down: the references with their signs turned)
-    __shared__ long long s_at[R];                        // [row][head] of a query; -1: none of this tree's, or refused
+    __shared__ long long s_at[R], s_from[R];             // [row][head] of a query, and its vector in q; -1: none of this tree's, or refused
     __shared__ uint32_t s_mask[R][kTrMask];
+    __shared__ int s_pos[R];
     __shared__ uint64_t s_full[S::stages], s_empty[S::stages], s_bar[4];
     __shared__ unsigned s_valid[S::stages];
     __shared__ uint32_t s_tmem, s_set[S::groups];        // queries that have a reference
@@ -404,7 +469,8 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     constexpr int kWithQueries = (S::warps + 1) * 32, kQueries = 6;  // threads that wait for a pair's queries, and their barrier
     bool ok = true;
 
-    if (idle) {
+    if (!idle && warp >= S::warps) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::least));
+    if (idle || warp == S::warps + 3) {
     } else if (warp == S::warps) {
         TreeCopies<S::stages, true> copies = {a, &kmap, &vmap, base, s_scales, s_full, s_empty, s_valid, 0};
         for (TreeWalk walk(L, at); ok && walk.next();) {
@@ -422,7 +488,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
             if (lane == 0) {
                 for (int i = walk.t0; ok && i < walk.t1; ++i, ++n) {
                     const int st = n % S::stages;
-                    ok = mbar_spin_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n == 0 || mbar_spin_bounded(b_free, (unsigned)(n - 1) & 1u));
+                    ok = mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n == 0 || mbar_wait_bounded(b_free, (unsigned)(n - 1) & 1u));
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * 2 * kTrTileBytes));
@@ -443,7 +509,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 if (flat0 >= walk.count * L.group) continue;
                 for (int i = walk.t0; ok && i < walk.t1; ++i, ++n) {
                     const int st = n % S::stages;
-                    ok = mbar_spin_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && mbar_spin_bounded(b_weights, (unsigned)n & 1u);
+                    ok = mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && mbar_wait_bounded(b_weights, (unsigned)n & 1u);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t dv = tr_desc_mn(smem_addr(base + (size_t)st * 2 * kTrTileBytes + kTrTileBytes), kTrTileBytes);
@@ -457,9 +523,11 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
         }
         __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::most));
         const int quarter = warp & 3, group = warp >> 2, first = group * 16, key = 32 * quarter + lane;      // its keys of a tile, and its queries
         constexpr int kAll = S::warps * 32, kEvery = 7;              // threads, and their barrier (1 .. 4: those of sixteen queries)
-        const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_scores = t_lane + (uint32_t)first, t_values = t_lane + (uint32_t)(S::s_cols + 4 * first);
+        const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_scores = t_lane + (uint32_t)first, t_values = t_lane + (uint32_t)(S::s_cols + 4 * first), t_moved = t_lane + (uint32_t)(S::s_cols + S::o_cols + first);
+        tr_fill<16>(t_moved, 0u);
         tr_fill<64>(t_values, 0u);
 #pragma unroll
         for (int part = 0; part < 3; ++part) tr_fill<16>(t_scores + part * R, kTrBias);
@@ -470,62 +538,55 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
             if (flat0 >= walk.count * L.group) continue;
             // ---- the queries ----
             named_barrier_sync(kEvery, kAll);            // (those in front are done with)
-            for (int r = tid; r < R; r += kAll) {
-                const int flat = flat0 + r, node = flat / L.group;
+            if (tid < R) {
+                const int flat = flat0 + tid, node = flat / L.group;
                 const size_t row = (size_t)walk.s * a.nodes + node;
                 long long to = -1;
+                int pos = -1;
+                TreeMask mask = {};
                 if (flat < walk.count * L.group) {
-                    to = (long long)(row * a.n_q + (size_t)walk.kvh * L.group + flat % L.group);
-                    if (tr_position_refused(a, a.rope_pos ? ld_l2(a.rope_pos + row) : walk.start + node)) {
+                    pos = a.rope_pos ? ld_l2(a.rope_pos + row) : walk.start + node;
+                    mask.load(a, row, node);
+                    to = (long long)(row * a.n_q + (size_t)walk.kvh * L.group + flat - node * L.group);
+                    if (tr_position_refused(a, pos)) {
                         atomicOr(&g_tree_error, kK8ErrIndex);
                         to = -1;
                     }
                 }
-                s_at[r] = to;
-                s_down[r] = 0.0f;
-                tr_masks(a, row, node, to >= 0, s_mask[r]);
+                s_at[tid] = to;
+                s_pos[tid] = pos;
+                s_from[tid] = to < 0 ? -1 : (long long)(row * a.q_stride + ((size_t)walk.kvh * L.group + flat - node * L.group) * kK8Hd);
+                s_down[tid] = 0.0f;
+                mask.store(a, to >= 0, s_mask[tid]);
             }
             if (lane == 0 && quarter == 0) {
                 s_unit[group][0] = s_unit[group][1] = 0.0f;
                 s_set[group] = 0;
             }
             named_barrier_sync(kEvery, kAll);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = warp + j * S::warps;
-                float f = 0.0f;
-                if (s_at[r] >= 0) {
-                    const int flat = flat0 + r, node = flat / L.group;
-                    const size_t row = (size_t)walk.s * a.nodes + node;
-                    f = tr_query<R>(a, row, walk.kvh * L.group + flat % L.group, a.rope_pos ? ld_l2(a.rope_pos + row) : walk.start + node, s_q, r);
-                } else {
-                    for (int part = 0; part < 3; ++part) reinterpret_cast<uint32_t*>(s_q + (part * R + r) * kK8Hd)[lane] = 0;
-                }
-                if (lane == 0) s_f[r] = f;
-            }
+            if (L.aligned) tr_queries<R, true>(L, s_from, s_pos, s_q, s_f);
+            else tr_queries<R, false>(L, s_from, s_pos, s_q, s_f);
             fence_proxy_async_smem();
             named_barrier_sync(kQueries, kWithQueries);
-            float o[16];                                 // of dim `key`: outputs that were moved on
             f32x2 l[8];                                  // of key `key`: sums
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[r] = 0.0f;
-#pragma unroll
             for (int r = 0; r < 8; ++r) l[r] = 0;
-            // Adds the accumulators to o, and sets them back.
-            auto move_on = [&](float unit) {
+            // Eight queries' outputs of dim `key`: what was moved on, and the accumulators.
+            auto moved = [&](int h, float unit, float (&o)[8]) {
+                uint32_t m[8];
+                tr_ld8(t_moved + h, m);
 #pragma unroll
-                for (int h = 0; h < 16; h += 2) {
+                for (int j = 0; j < 8; j += 2) {
                     uint32_t v[8];
-                    tr_ld8(t_values + 4 * h, v);
+                    tr_ld8(t_values + 4 * (h + j), v);
                     tr_wait8(v);
+                    if (j == 0) tr_tie8(m);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float hi = __fmaf_rn((float)(int)v[4 * j + 3], 256.0f, (float)(int)v[4 * j + 2]), lo = __fmaf_rn((float)(int)v[4 * j + 1], 256.0f, (float)(int)v[4 * j]);
-                        o[h + j] = __fmaf_rn(__fmaf_rn(hi, 65536.0f, lo), unit, o[h + j]);
+                    for (int k = 0; k < 2; ++k) {
+                        const float hi = __fmaf_rn((float)(int)v[4 * k + 3], 256.0f, (float)(int)v[4 * k + 2]), lo = __fmaf_rn((float)(int)v[4 * k + 1], 256.0f, (float)(int)v[4 * k]);
+                        o[j + k] = __fmaf_rn(__fmaf_rn(hi, 65536.0f, lo), unit, __uint_as_float(m[j + k]));
                     }
                 }
-                tr_fill<64>(t_values, 0u);
-                tmem_wait_st();
             };
             const int total = walk.start + walk.count;
             bool early = false;                          // the next scores were seen to be there
@@ -577,13 +638,6 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                     if (lane < 16) s_max[quarter][first + lane] = top;
                     const float most = tr_warp_max(sv);
                     if (lane == 0) s_scale_max[group][quarter] = most;
-                    if (i > walk.t0) {
-                        ok = ok && mbar_wait_bounded(b_values, (unsigned)(n - 1) & 1u);
-                        __syncwarp();
-                        tc_fence_after();
-                        move_on(unit * (1.0f / kTrOne));
-                        tc_fence_before();
-                    }
                     named_barrier_sync(1 + group, 128);
                     const float4 scales = *reinterpret_cast<const float4*>(s_scale_max[group]);
                     const float scale_most = fmaxf(fmaxf(scales.x, scales.y), fmaxf(scales.z, scales.w));
@@ -612,10 +666,24 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                         const float b0 = __shfl_sync(0xffffffffu, by, r), b1 = __shfl_sync(0xffffffffu, by, r + 1);
                         float w0, w1;
                         unpack2(w[r / 2], w0, w1);
-                        o[r] *= b0;
-                        o[r + 1] *= b1;
                         l[r / 2] = tr_mul2(l[r / 2], pack2(b0, b1));
                         p[r / 2] = pack2(tr_ex2(w0 - u0), tr_ex2(w1 - u1));
+                    }
+                    if (i > walk.t0) {
+                        ok = ok && mbar_wait_bounded(b_values, (unsigned)(n - 1) & 1u);
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll
+                        for (int h = 0; h < 16; h += 8) {
+                            float o[8];
+                            moved(h, unit * (1.0f / kTrOne), o);
+#pragma unroll
+                            for (int r = 0; r < 8; ++r) o[r] *= __shfl_sync(0xffffffffu, by, h + r);
+                            tr_st8(t_moved + h, o);
+                        }
+                        tr_fill<64>(t_values, 0u);
+                        tmem_wait_st();
+                        tc_fence_before();
                     }
                     named_barrier_sync(1 + group, 128);
                 }
@@ -645,37 +713,41 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
             ok = ok && mbar_wait_bounded(b_values, (unsigned)(n - 1) & 1u);
             __syncwarp();
             tc_fence_after();
-            move_on(s_unit[group][0] * (1.0f / kTrOne));
-            tc_fence_before();
-            float mine = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                float l0, l1;
-                unpack2(l[r / 2], l0, l1);
-                l0 = warp_sum(l0);
-                l1 = warp_sum(l1);
-                if (lane == r) mine = l0;
-                if (lane == r + 1) mine = l1;
-            }
-            if (lane < 16) s_sum[quarter][first + lane] = mine;
+            const float mine = tr_sums(l);
+            if (!(lane & 1)) s_sum[quarter][first + (lane >> 1)] = mine;
             named_barrier_sync(1 + group, 128);
             const bool whole = walk.whole();
             const size_t part = (((size_t)share * L.tiles + tile) * 2 + (walk.t0 > 0 ? 0 : 1)) * R + first;
             const uint32_t set = s_set[group];
-            if (L.cut && tile == 0 && walk.t0 == 0 && tid == 0) L.head[1 + (size_t)walk.s * a.cache.n_kv + walk.kvh] = whole ? -1 : walk.pair_begin();
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const long long to = s_at[first + r];
+            float inv, log_sum;                          // lane r: of query `first` + r
+            {
+                const int r = lane & 15;
                 const float sum = (s_sum[0][first + r] + s_sum[1][first + r]) + (s_sum[2][first + r] + s_sum[3][first + r]);
-                if (to < 0) continue;
-                if (!whole) {
-                    L.part_o[(part + r) * kK8Hd + key] = o[r];
-                    if (key == 0) L.part_ml[part + r] = make_float2(set >> r & 1u ? -s_down[first + r] : kTrLow, sum);
-                } else {
-                    a.out[(size_t)to * kK8Hd + key] = sum == 0.0f ? 0.0f : o[r] / sum;
-                    if (a.lse && key == 0) a.lse[to] = sum == 0.0f ? -INFINITY : (tr_lg2(sum) - s_down[first + r]) * 0.6931471805599453f;
+                inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+                log_sum = sum == 0.0f ? -INFINITY : (tr_lg2(sum) - s_down[first + r]) * 0.6931471805599453f;
+                const long long to = s_at[first + r];
+                if (quarter == 0 && lane < 16 && to >= 0) {
+                    if (!whole) L.part_ml[part + r] = make_float2(set >> r & 1u ? -s_down[first + r] : kTrLow, sum);
+                    else if (a.lse) a.lse[to] = log_sum;
                 }
             }
+            if (L.cut && tile == 0 && walk.t0 == 0 && tid == 0) L.head[1 + (size_t)walk.s * a.cache.n_kv + walk.kvh] = whole ? -1 : walk.pair_begin();
+#pragma unroll
+            for (int h = 0; h < 16; h += 8) {
+                float o[8];
+                moved(h, s_unit[group][0] * (1.0f / kTrOne), o);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const long long to = s_at[first + h + r];
+                    const float by = __shfl_sync(0xffffffffu, inv, h + r);
+                    float* out = whole ? a.out + (size_t)to * kK8Hd : L.part_o + (part + h + r) * kK8Hd;
+                    if (to >= 0) out[key] = o[r] * by;
+                }
+            }
+            tr_fill<16>(t_moved, 0u);                    // for the next pair
+            tr_fill<64>(t_values, 0u);
+            tmem_wait_st();
+            tc_fence_before();
         }
     }
     // Rows of padding, and sequences that are refused: a share of them to each block.
@@ -768,7 +840,9 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
     const tenzo_attention_tree_args& a = L.a;
     extern __shared__ unsigned char tr_smem[];
     __shared__ __align__(16) float s_f[R], s_down[R];    // (s_down: log-sum-exps with their signs turned)
+    __shared__ long long s_from[R];
     __shared__ uint32_t s_mask[R][kTrMask];
+    __shared__ int s_pos[R];
     __shared__ uint64_t s_full[S::stages], s_empty[S::stages], s_scores[2], s_free[2];
     __shared__ unsigned s_valid[S::stages];
     __shared__ uint32_t s_tmem;
@@ -823,7 +897,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                     if (lane == 0) {
                         for (int i = t0; ok && i < min(walk.t1, t0 + kTwTiles); ++i, ++n) {
                             const int st = n % S::stages, half = n & 1;
-                            ok = mbar_spin_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n < 2 || mbar_spin_bounded(&s_free[half], (unsigned)(n / 2 - 1) & 1u));
+                            ok = mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n < 2 || mbar_wait_bounded(&s_free[half], (unsigned)(n / 2 - 1) & 1u));
                             if (!ok) break;
                             tc_fence_after();
                             const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * kTrTileBytes));
@@ -851,34 +925,30 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                 const int t1 = min(walk.t1, t0 + kTwTiles), queries = walk.count * L.group, total = walk.start + walk.count;
                 for (int flat0 = 0; flat0 < queries; flat0 += R) {
                     named_barrier_sync(kEvery, kAll);    // (the queries in front, and the sums, are done with)
-                    for (int r = tid; r < R; r += kAll) {
-                        const int flat = flat0 + r, node = flat / L.group;
+                    if (tid < R) {
+                        const int flat = flat0 + tid, node = flat / L.group;
                         const size_t row = (size_t)walk.s * a.nodes + node;
                         float lse = INFINITY;            // of a query that does not count
+                        int pos = -1;
+                        TreeMask mask = {};
                         if (flat < queries) {
-                            if (tr_position_refused(a, a.rope_pos ? ld_l2(a.rope_pos + row) : walk.start + node)) {
+                            pos = a.rope_pos ? ld_l2(a.rope_pos + row) : walk.start + node;
+                            lse = ld_l2(a.lse + row * a.n_q + (size_t)walk.kvh * L.group + flat - node * L.group) * 1.4426950408889634f;
+                            mask.load(a, row, node);
+                            if (!(fabsf(lse) < INFINITY)) lse = INFINITY;
+                            if (tr_position_refused(a, pos)) {
                                 atomicOr(&g_tree_error, kK8ErrIndex);
-                            } else {
-                                lse = ld_l2(a.lse + row * a.n_q + (size_t)walk.kvh * L.group + flat % L.group) * 1.4426950408889634f;
-                                if (!(fabsf(lse) < INFINITY)) lse = INFINITY;
+                                lse = INFINITY;
                             }
                         }
-                        s_down[r] = -lse;
-                        tr_masks(a, row, node, lse < INFINITY, s_mask[r]);
+                        s_down[tid] = -lse;
+                        s_pos[tid] = pos;
+                        s_from[tid] = lse < INFINITY ? (long long)(row * a.q_stride + ((size_t)walk.kvh * L.group + flat - node * L.group) * kK8Hd) : -1;
+                        mask.store(a, lse < INFINITY, s_mask[tid]);
                     }
                     named_barrier_sync(kEvery, kAll);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = warp + j * S::warps, flat = flat0 + r, node = flat / L.group;
-                        const size_t row = (size_t)walk.s * a.nodes + node;
-                        float f = 0.0f;
-                        if (s_down[r] > -INFINITY) {
-                            f = tr_query<R>(a, row, walk.kvh * L.group + flat % L.group, a.rope_pos ? ld_l2(a.rope_pos + row) : walk.start + node, s_q, r);
-                        } else {
-                            for (int part = 0; part < 3; ++part) reinterpret_cast<uint32_t*>(s_q + (part * R + r) * kK8Hd)[lane] = 0;
-                        }
-                        if (lane == 0) s_f[r] = f;
-                    }
+                    if (L.aligned) tr_queries<R, true>(L, s_from, s_pos, s_q, s_f);
+            else tr_queries<R, false>(L, s_from, s_pos, s_q, s_f);
                     fence_proxy_async_smem();
                     named_barrier_sync(kQueries, kWithQueries);
                     for (int i = t0; i < t1; ++i, ++n) {
@@ -957,6 +1027,7 @@ static int tree_check(TreeLaunch& L) {
     if (a.mask_stride == 0) a.mask_stride = words;
     if (a.mask_stride < words) return -1;
     L.group = a.n_q / a.cache.n_kv;
+    L.aligned = kv8_aligned(a.q, 16) && a.q_stride % 4 == 0 && kv8_aligned(a.rope_cos, 16) && kv8_aligned(a.rope_sin, 16);
     return 0;
 }
 
@@ -987,6 +1058,12 @@ static size_t tree_room(const TreeLaunch& L) {
 template <int R>
 static int tree_run(const TreeLaunch& L, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
     if (cudaError_t e = allow_smem(attention_tree_kernel<R>, TreeShape<R>::smem)) return (int)e;
+    // With fewer registers than the warps ask of one another they would wait for good; the kernel's number is the compiler's.
+    static const bool registers_ok = [] {
+        cudaFuncAttributes f = {};
+        return cudaFuncGetAttributes(&f, attention_tree_kernel<R>) == cudaSuccess && f.numRegs == TreeShape<R>::launched;
+    }();
+    if (!registers_ok) return -4;
     return kv4_launch(attention_tree_kernel<R>, dim3((unsigned)(L.shares * L.tiles)), TreeShape<R>::threads, TreeShape<R>::smem, st, L.a.use_pdl != 0, L, kmap, vmap);
 }
 template <int R>

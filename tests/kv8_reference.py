@@ -110,13 +110,13 @@ def tree(q, caches, layer, n_q, start, sees, turn=None):
                 out[i, head] = e @ value[places] / e.sum()
                 lse[i, head] = top + np.log(e.sum())
                 weight[h, places] += e / e.sum()
-                # the query: half a step of 2^-22 of its largest; each product, sum and the exponential's argument: some steps of fp32 of the sum of magnitudes;
-                # a weight: half a step of 2^-27 of the largest, counted with scales that may be half the largest
+                # the query: half a step of 2^-21 of its largest; each product, sum and the exponential's argument: some steps of fp32 of the sum of magnitudes;
+                # a weight: half a step of 2^-26 of the largest, counted with scales that may be half the largest
                 reach = (np.abs(key[places]) @ np.abs(x[g])).max() / np.sqrt(128)
-                ds = 2.0 ** -23 * np.abs(x[g]).max() * np.abs(key[places]).sum(-1).max() / np.sqrt(128) + 24 * 2.0 ** -24 * (reach + 1)
+                ds = 2.0 ** -22 * np.abs(x[g]).max() * np.abs(key[places]).sum(-1).max() / np.sqrt(128) + 24 * 2.0 ** -24 * (reach + 1)
                 sums = (16 + len(places) / 16) * 2.0 ** -24
                 most = np.abs(value[places]).max()
-                bound[i, head] = most * (2 * ds + sums + len(places) * 2.0 ** -27)
+                bound[i, head] = most * (2 * ds + sums + len(places) * 2.0 ** -26)
                 lse_bound[i, head] = ds + sums + 4 * 2.0 ** -24 * (1 + abs(lse[i, head]))
     return out.reshape(len(q), -1), lse, np.repeat(bound, 128, 1), lse_bound, weight
 
