@@ -366,29 +366,30 @@ struct TreeMask {
 };
 
 // For sixteen queries (columns of each part), two by two, and the lane's key, whose scale is sk: arguments of 2^x less what `down` (with its sign turned) says. The
-// accumulators are left as they have to start.
+// accumulators are left as they have to start, once tmem_wait_st() has returned.
 template <int R>
 __device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, const float* s_down, float sk, f32x2 (&w)[8]) {
     const f32x2 sk2 = pack2(sk, sk);
+    uint32_t high[2][8], mid[2][8], low[2][8];
 #pragma unroll
-    for (int h = 0; h < 16; h += 8) {
-        uint32_t d1[8], d2[8], d3[8];
-        tr_ld8(tmem + h, d1);
-        tr_ld8(tmem + R + h, d2);
-        tr_ld8(tmem + 2 * R + h, d3);
-        tr_wait8(d1);
-        tr_tie8(d2);
-        tr_tie8(d3);
+    for (int h = 0; h < 2; ++h) {
+        tr_ld8(tmem + 8 * h, high[h]);
+        tr_ld8(tmem + R + 8 * h, mid[h]);
+        tr_ld8(tmem + 2 * R + 8 * h, low[h]);
+    }
+    tr_wait8(high[0]);
+    tr_tie8(mid[0]); tr_tie8(low[0]); tr_tie8(high[1]); tr_tie8(mid[1]); tr_tie8(low[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
-            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + h + j), m = *reinterpret_cast<const ulonglong2*>(s_down + h + j);
-            w[(h + j) / 2] = tr_fma2(tr_whole2(d1 + j, d2 + j, d3 + j), tr_mul2(sk2, f.x), m.x);
-            w[(h + j) / 2 + 1] = tr_fma2(tr_whole2(d1 + j + 2, d2 + j + 2, d3 + j + 2), tr_mul2(sk2, f.y), m.y);
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + 8 * h + j), m = *reinterpret_cast<const ulonglong2*>(s_down + 8 * h + j);
+            w[4 * h + j / 2] = tr_fma2(tr_whole2(high[h] + j, mid[h] + j, low[h] + j), tr_mul2(sk2, f.x), m.x);
+            w[4 * h + j / 2 + 1] = tr_fma2(tr_whole2(high[h] + j + 2, mid[h] + j + 2, low[h] + j + 2), tr_mul2(sk2, f.y), m.y);
         }
     }
 #pragma unroll
     for (int part = 0; part < 3; ++part) tr_fill<16>(tmem + part * R, kTrBias);
-    tmem_wait_st();
 }
 
 // Sums over the warp of sixteen numbers a lane: that of number lane / 2.
@@ -605,25 +606,31 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 tc_fence_after();
                 f32x2 w[8];
                 tr_arguments<R>(t_scores, s_f + first, s_down + first, sk, w);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b_free);
                 const bool values_early = n == 0 || mbar_test(b_values, (unsigned)(n - 1) & 1u);     // (looked at when the weights are ready to be stored)
                 if (ragged) tr_hide(w, s_mask + first, t - walk.start, dead);
                 float over = -INFINITY;
-                f32x2 p[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     float w0, w1;
                     unpack2(w[r], w0, w1);
                     over = fmaxf(fmaxf(over, w0), w1);
-                    p[r] = pack2(tr_ex2(w0), tr_ex2(w1));
                 }
                 const uint32_t set = s_set[group];
                 const float unit = s_unit[group][0];
                 if (over > kTrSlack || sv > unit || set != 0xffffu || (n + 1) % kTrFlush == 0) s_vote[group][n & 1] = n + 1;
+                tmem_wait_st();
+                tc_fence_before();
                 named_barrier_sync(1 + group, 128);
-                if (*reinterpret_cast<volatile int*>(&s_vote[group][n & 1]) == n + 1) {
+                if (lane == 0) mbar_arrive(b_free);
+                const int vote = *reinterpret_cast<volatile int*>(&s_vote[group][n & 1]);
+                f32x2 p[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    float w0, w1;
+                    unpack2(w[r], w0, w1);
+                    p[r] = pack2(tr_ex2(w0), tr_ex2(w1));
+                }
+                if (vote == n + 1) {
                     // ---- references of these sixteen queries anew, and their accumulators moved on ----
                     float top = -INFINITY;               // lane r: of query `first` + r, less the reference
 #pragma unroll
@@ -700,11 +707,11 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 }
                 if (!values_early) ok = ok && mbar_wait_bounded(b_values, (unsigned)(n - 1) & 1u);    // (the weights in front were read)
                 __syncwarp();
-                early = i + 1 < walk.t1 && mbar_test(b_scores, (unsigned)(n + 1) & 1u);
                 unsigned char* to = s_p + (first >> 5) * kTrTileBytes + key * kK8Hd;
                 const int chunk = (first & 31) >> 2;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(to + (((chunk + c) ^ (key & 7)) << 4)) = make_uint4(word[4 * c], word[4 * c + 1], word[4 * c + 2], word[4 * c + 3]);
+                early = i + 1 < walk.t1 && mbar_test(b_scores, (unsigned)(n + 1) & 1u);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(b_weights);
@@ -962,6 +969,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                         tc_fence_after();
                         f32x2 w[8];
                         tr_arguments<R>(t_scores + half * S::s_cols, s_f + first, s_down + first, sk, w);
+                        tmem_wait_st();
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
