@@ -42,15 +42,17 @@ struct TreeLaunch {
 // R queries a CTA.
 template <int R>
 struct TreeShape {
-    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 4) * 32;      // four warps for sixteen queries; one that copies, two that issue products, and one to four of them
+    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 4) * 32;      // four warps for sixteen queries; two that copy, one or two that issue products, four of these in all
+    // 64 queries are two lines of 32, which have the tiles in common and wait for nothing else of each other: the tensor cores work for the one while the other's warps make weights.
+    static constexpr int lines = R == 64 ? 2 : 1, line = R / lines, line_warps = line / 4;
     static constexpr int stages = R > 32 ? 3 : 2, resident = R > 32 ? 1 : 2;
-    static constexpr int s_cols = 3 * R, o_cols = 4 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;       // and R for outputs that were moved on
-    static_assert(s_cols + o_cols + R <= tmem_cols, "tensor memory");
+    static constexpr int s_cols = 3 * line, o_cols = 4 * line, all_s = 3 * R, all_o = 4 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;
+    static_assert(all_s + all_o + R <= tmem_cols, "tensor memory: scores, products with the values, outputs that were moved on");
     // Registers a thread: as the block is launched, and after the warps of the second line have given some to those of the first.
     static constexpr int launched = R == 64 ? 96 : R == 48 ? 128 : R == 32 ? 80 : 128, most = R == 64 ? 112 : R == 48 ? 144 : R == 32 ? 104 : 168, least = R == 48 ? 40 : R == 16 ? 64 : 32;
     static_assert(warps * most + 4 * least <= (warps + 4) * launched, "what is taken is there");
     static constexpr int p_panels = R > 32 ? 2 : 1;                   // of 128 bytes: 32 queries
-    static constexpr int q_bytes = s_cols * kK8Hd, p_bytes = p_panels * kTrTileBytes;
+    static constexpr int q_bytes = all_s * kK8Hd, p_bytes = p_panels * kTrTileBytes;
     static constexpr size_t smem = 1024 + (size_t)stages * 2 * kTrTileBytes + q_bytes + p_bytes + stages * 2 * kTrTile * 4;
 };
 
@@ -90,13 +92,9 @@ __device__ __forceinline__ uint64_t tr_desc_mn(uint32_t saddr, uint32_t panel) {
 }
 __device__ __forceinline__ f32x2 tr_mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 tr_fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-// The accumulators of the scores start at kTrBias, the bits of 2^23 * 1.5, so that a part of a sum (below 2^21 each) is read as the float 2^23 * 1.5 + part.
-// Two sums from their three parts; the lower two parts' share is rounded to 2^7 of some 2^29.
-constexpr uint32_t kTrBias = 0x4B400000u;
-__device__ __forceinline__ f32x2 tr_whole2(const uint32_t* high, const uint32_t* mid, const uint32_t* low) {
-    auto part = [](const uint32_t* v) { return pack2(__uint_as_float(v[0]), __uint_as_float(v[1])); };
-    constexpr float base = 12582912.0f;
-    return add2(tr_fma2(add2(part(high), pack2(-base, -base)), pack2(65536.0f, 65536.0f), tr_fma2(part(mid), pack2(256.0f, 256.0f), part(low))), pack2(-257.0f * base, -257.0f * base));
+// A sum from its three parts of a whole number (below 2^21 each).
+__device__ __forceinline__ float tr_whole(uint32_t high, uint32_t mid, uint32_t low) {
+    return __fmaf_rn((float)(int)high, 65536.0f, (float)((int)mid * 256 + (int)low));
 }
 // The same value in N columns of the warp's 32 lanes.
 template <int N>
@@ -228,10 +226,10 @@ struct TreeWalk {
 
 // ---- the parts that both kernels have ------------------------------------------------------------------------------------------
 // R queries of a block on their way to the operand, four by each of its R / 4 warps. A lane has dims 4 lane .. 4 lane + 3, and the lane sixteen on, or back, those that they are turned
-// with. A vector is turned, scaled by a power of two to a maximum between 2^21 and 2^22 and rounded; its signed bytes are rows r, R + r, 2R + r of the operand (128 bytes each, swizzled).
+// with. A vector is turned, scaled by a power of two to a maximum between 2^21 and 2^22 and rounded; its signed bytes are rows r, LINE + r, 2 LINE + r of its line's operand (128 bytes each, swizzled).
 // s_f: what a unit of the products with the codes counts in the argument of 2^x (NaN for a query that is not finite). from[r]: the vector in q, -1: none, zeros.
 // (Every load is made, of something, without a branch around it: where two ways meet the compiler copies what was loaded, and so waits for it. 3500 cycles for a block's loads that way, 900 this.)
-template <int R, bool VEC>
+template <int R, int LINE, bool VEC>
 __device__ __forceinline__ void tr_queries(const TreeLaunch& L, const long long* from, const int* pos, unsigned char* s_q, float* s_f) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool rotate = L.a.rope_cos != nullptr;
@@ -279,7 +277,7 @@ __device__ __forceinline__ void tr_queries(const TreeLaunch& L, const long long*
         for (int j = 0; j < 4; ++j) v[j] = __float2int_rn(x[i][j] * up);          // (NaN: 0)
 #pragma unroll
         for (int part = 2; part >= 0; --part) {          // the last byte, with its sign; what it leaves, in 256ths; again
-            const int n = part * R + r;
+            const int n = r / LINE * (3 * LINE) + part * LINE + r % LINE;
             const uint32_t word = prmt(prmt((uint32_t)v[0], (uint32_t)v[1], 0x0040u), prmt((uint32_t)v[2], (uint32_t)v[3], 0x0040u), 0x5410u);
             *reinterpret_cast<uint32_t*>(s_q + n * kK8Hd + (((lane >> 2) ^ (n & 7)) << 4) + 4 * (lane & 3)) = word;
 #pragma unroll
@@ -289,18 +287,19 @@ __device__ __forceinline__ void tr_queries(const TreeLaunch& L, const long long*
     }
 }
 
-// The warp that copies: sixteen keys a lane of eight, a tile's codes and scales into one stage after the other. A block whose table entry is out of range is left out (its bit in s_valid
-// is 0).
-template <int STAGES, bool VALUES>
+// A warp that copies keys, or values: a tile after the other into a ring of stages, the codes by tensor copies of sixteen rows, a lane of eight each, the scales by sixteen bytes a lane. A block
+// whose table entry is out of range is left out (its bit in s_valid is 0). (A warp issues its lanes' copies one by one: with both rings and the scales' copies, four a lane, in one warp 64 queries'
+// tiles took 3500 cycles and were waited for.)
+template <int STAGES>
 struct TreeCopies {
     const tenzo_attention_tree_args& a;
-    const CUtensorMap *kmap, *vmap;
-    unsigned char* stages;                               // [STAGES][K, V]
-    float* scales;                                       // [STAGES][K, V][128]
-    uint64_t *full, *empty;
-    unsigned* s_valid;
+    const CUtensorMap* map;
+    const float *scale_k, *scale_v;                      // (those of the values come with the keys; null: none)
+    unsigned char* stages;                               // [STAGES]
+    float* scales;                                       // [STAGES][2][128]
+    uint64_t *full, *empty;                              // [STAGES]; full: 33 arrivals and the copies' bytes
+    unsigned* s_valid;                                   // [STAGES], or null
     int n;                                               // tiles that were asked for
-    static constexpr int kPer = VALUES ? 2 : 1;
     // Tiles t0 .. t1 - 1 of a pair, `passes` times.
     __device__ __forceinline__ bool run(int seq, int kvh, int total, int t0, int t1, int passes) {
         const int lane = threadIdx.x & 31, n_tiles = t1 - t0, steps = n_tiles * passes, per = a.cache.slots / kK8Chunk;
@@ -322,24 +321,22 @@ struct TreeCopies {
                 now = next;
                 next = first_row(i + 4);
             }
+            const int mine = __shfl_sync(0xffffffffu, now, 8 * (i & 3) + (lane >> 2));           // row of the chunk whose scales 4 (lane % 4) .. the lane copies
+            const unsigned there = __ballot_sync(0xffffffffu, now >= 0) >> (8 * (i & 3)) & 0xffu;
             const bool ok = use == 0 || mbar_wait_bounded(&empty[st], (unsigned)(use - 1) & 1u);
             if (!__all_sync(0xffffffffu, ok)) return false;
-            const unsigned there = __ballot_sync(0xffffffffu, now >= 0) >> (8 * (i & 3)) & 0xffu;
+            auto copy = [&](const float* from, float* to) {
+                if (from && mine >= 0) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to + 4 * lane)), "l"(from + mine + 4 * (lane & 3)) : "memory");
+            };
+            copy(scale_k, scales + 2 * st * kTrTile);
+            copy(scale_v, scales + (2 * st + 1) * kTrTile);
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[st])) : "memory");
             if (lane == 0) {
-                s_valid[st] = there;
-                mbar_expect_tx(&full[st], (unsigned)__popc(there) * kPer * (kK8Chunk * kK8Hd + kK8Chunk * 4));
+                if (s_valid) s_valid[st] = there;
+                mbar_expect_tx(&full[st], (unsigned)__popc(there) * (kK8Chunk * kK8Hd));
             }
             __syncwarp();
-            if ((lane >> 3) == (i & 3) && now >= 0) {
-                unsigned char* to = stages + (size_t)st * kPer * kTrTileBytes + (lane & 7) * kK8Chunk * kK8Hd;
-                float* sc = scales + (size_t)st * kPer * kTrTile + (lane & 7) * kK8Chunk;
-                tma_load_2d(to, kmap, 0, now, &full[st]);
-                bulk_g2s(sc, a.cache.scale_k + now, kK8Chunk * 4, &full[st]);
-                if (VALUES) {
-                    tma_load_2d(to + kTrTileBytes, vmap, 0, now, &full[st]);
-                    bulk_g2s(sc + kTrTile, a.cache.scale_v + now, kK8Chunk * 4, &full[st]);
-                }
-            }
+            if ((lane >> 3) == (i & 3) && now >= 0) tma_load_2d(stages + (size_t)st * kTrTileBytes + (lane & 7) * kK8Chunk * kK8Hd, map, 0, now, &full[st]);
             __syncwarp();
         }
         return true;
@@ -365,8 +362,7 @@ struct TreeMask {
     }
 };
 
-// For sixteen queries (columns of each part), two by two, and the lane's key, whose scale is sk: arguments of 2^x less what `down` (with its sign turned) says. The
-// accumulators are left as they have to start, once tmem_wait_st() has returned.
+// For sixteen queries (columns of each part, R apart), two by two, and the lane's key, whose scale is sk: arguments of 2^x less what `down` (with its sign turned) says.
 template <int R>
 __device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, const float* s_down, float sk, f32x2 (&w)[8]) {
     const f32x2 sk2 = pack2(sk, sk);
@@ -384,12 +380,11 @@ __device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, co
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
             const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + 8 * h + j), m = *reinterpret_cast<const ulonglong2*>(s_down + 8 * h + j);
-            w[4 * h + j / 2] = tr_fma2(tr_whole2(high[h] + j, mid[h] + j, low[h] + j), tr_mul2(sk2, f.x), m.x);
-            w[4 * h + j / 2 + 1] = tr_fma2(tr_whole2(high[h] + j + 2, mid[h] + j + 2, low[h] + j + 2), tr_mul2(sk2, f.y), m.y);
+            auto whole = [&](int k) { return tr_whole(high[h][k], mid[h][k], low[h][k]); };
+            w[4 * h + j / 2] = tr_fma2(pack2(whole(j), whole(j + 1)), tr_mul2(sk2, f.x), m.x);
+            w[4 * h + j / 2 + 1] = tr_fma2(pack2(whole(j + 2), whole(j + 3)), tr_mul2(sk2, f.y), m.y);
         }
     }
-#pragma unroll
-    for (int part = 0; part < 3; ++part) tr_fill<16>(tmem + part * R, kTrBias);
 }
 
 // Sums over the warp of sixteen numbers a lane: that of number lane / 2.
@@ -431,7 +426,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     __shared__ long long s_at[R], s_from[R];             // [row][head] of a query, and its vector in q; -1: none of this tree's, or refused
     __shared__ uint32_t s_mask[R][kTrMask];
     __shared__ int s_pos[R];
-    __shared__ uint64_t s_full[S::stages], s_empty[S::stages], s_bar[4];
+    __shared__ uint64_t s_full[2 * S::stages], s_empty[2 * S::stages], s_bar[S::lines][4];     // rings of keys and of values
     __shared__ unsigned s_valid[S::stages];
     __shared__ uint32_t s_tmem, s_set[S::groups];        // queries that have a reference
     __shared__ int s_vote[S::groups][2], s_found;
@@ -441,16 +436,18 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     unsigned char* base = tr_smem + (((smem_addr(tr_smem) + 1023u) & ~1023u) - smem_addr(tr_smem));
     unsigned char *s_q = base + S::stages * 2 * kTrTileBytes, *s_p = s_q + S::q_bytes;
     float* s_scales = reinterpret_cast<float*>(s_p + S::p_bytes);
-    uint64_t *b_scores = s_bar, *b_free = s_bar + 1, *b_weights = s_bar + 2, *b_values = s_bar + 3;   // scores are there; were read; weights are there; their products are done
+    enum { kScores, kFree, kWeights, kValues };          // a line's scores are there; were read; weights are there; their products are done
     if (tid == 0) {
-        for (int i = 0; i < S::stages; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&s_empty[i], 1);
+        for (int i = 0; i < 2 * S::stages; ++i) {
+            mbar_init(&s_full[i], 33);
+            mbar_init(&s_empty[i], i < S::stages ? S::lines + S::warps : S::lines);       // products, and for the keys the warps that read the scales
         }
-        mbar_init(b_scores, 2);                          // the products, and the thread that has seen the copies land
-        mbar_init(b_free, S::warps);
-        mbar_init(b_weights, S::warps);
-        mbar_init(b_values, 1);
+        for (int i = 0; i < S::lines; ++i) {
+            mbar_init(&s_bar[i][kScores], 2);            // the products, and the thread that has seen the copies land
+            mbar_init(&s_bar[i][kFree], S::line_warps);
+            mbar_init(&s_bar[i][kWeights], S::line_warps);
+            mbar_init(&s_bar[i][kValues], 1);
+        }
         mbar_init_fence();
         for (int g = 0; g < S::groups; ++g) s_vote[g][0] = s_vote[g][1] = 0;
     }
@@ -467,71 +464,70 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
     if (L.cut && blockIdx.x == 0 && tid == 0) L.head[0] = at.tiles;
     const bool idle = at.first >= at.all;
-    constexpr int kWithQueries = (S::warps + 1) * 32, kQueries = 6;  // threads that wait for a pair's queries, and their barrier
+    constexpr int kWithQueries = (S::warps + S::lines) * 32, kQueries = 6;       // threads that wait for a pair's queries, and their barrier
     bool ok = true;
 
     if (!idle && warp >= S::warps) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::least));
-    if (idle || warp == S::warps + 3) {
-    } else if (warp == S::warps) {
-        TreeCopies<S::stages, true> copies = {a, &kmap, &vmap, base, s_scales, s_full, s_empty, s_valid, 0};
+    if (idle || warp > S::warps + 1 + S::lines) {
+    } else if (warp >= S::warps && warp <= S::warps + 1) {         // keys; values
+        const int ring = warp - S::warps;
+        TreeCopies<S::stages> copies = {a, ring ? &vmap : &kmap, ring ? nullptr : a.cache.scale_k, ring ? nullptr : a.cache.scale_v, base + (size_t)ring * S::stages * kTrTileBytes, s_scales,
+                                        s_full + ring * S::stages, s_empty + ring * S::stages, ring ? nullptr : s_valid, 0};
         for (TreeWalk walk(L, at); ok && walk.next();) {
             if (flat0 >= walk.count * L.group) continue;             // rows of padding alone
             ok = copies.run(walk.seq, walk.kvh, walk.start + walk.count, walk.t0, walk.t1, 1);
         }
         if (!ok) copies.drain();
-    } else if (warp == S::warps + 1) {                   // S^T = K Q^T
-        constexpr uint32_t shape = kTrShape | (1u << 10) | ((uint32_t)(S::s_cols >> 3) << 17);
-        const uint64_t dq = umma_desc_sw128(smem_addr(s_q));
-        int n = 0;
+    } else if (warp > S::warps + 1) {                    // the products of a line
+        constexpr uint32_t d_scores = kTrShape | (1u << 10) | ((uint32_t)(S::s_cols >> 3) << 17);                             // S^T = K Q^T
+        constexpr uint32_t d_values = kTrShape | (1u << 15) | (1u << 16) | ((uint32_t)(S::o_cols >> 3) << 17);                 // O^T += V^T P^T, both operands transposed
+        const int line = warp - S::warps - 2;
+        uint64_t* bar = s_bar[line];
+        const uint32_t t_scores = tmem + line * S::s_cols, t_values = tmem + S::all_s + line * S::o_cols;
+        const uint64_t dq = umma_desc_sw128(smem_addr(s_q) + line * S::s_cols * kK8Hd), dp = tr_desc_mn(smem_addr(s_p) + line * kTrTileBytes, kTrTileBytes);
+        int n = 0;                                       // tiles so far
+        auto scores = [&](int k) {                       // of the k-th tile
+            const int st = k % S::stages;
+            ok = mbar_wait_bounded(&s_full[st], (unsigned)(k / S::stages) & 1u) && (k == 0 || mbar_wait_bounded(&bar[kFree], (unsigned)(k - 1) & 1u));
+            if (!ok) return;
+            tc_fence_after();
+            const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * kTrTileBytes));
+#pragma unroll
+            for (int i = 0; i < kK8Hd / 32; ++i) umma_i8(t_scores, dk + (uint64_t)(2 * i), dq + (uint64_t)(2 * i), d_scores, i > 0);
+            umma_commit(&bar[kScores]);
+            umma_commit(&s_empty[st]);
+            mbar_arrive(&bar[kScores]);
+        };
         for (TreeWalk walk(L, at); walk.next();) {
             if (flat0 >= walk.count * L.group) continue;
             named_barrier_sync(kQueries, kWithQueries);
-            if (lane == 0) {
+            if (lane == 0 && ok) {
+                scores(n);
                 for (int i = walk.t0; ok && i < walk.t1; ++i, ++n) {
+                    if (i + 1 < walk.t1) scores(n + 1);
                     const int st = n % S::stages;
-                    ok = mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n == 0 || mbar_wait_bounded(b_free, (unsigned)(n - 1) & 1u));
+                    ok = ok && mbar_wait_bounded(&s_full[S::stages + st], (unsigned)(n / S::stages) & 1u) && mbar_wait_bounded(&bar[kWeights], (unsigned)n & 1u);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * 2 * kTrTileBytes));
+                    const uint64_t dv = tr_desc_mn(smem_addr(base + (size_t)(S::stages + st) * kTrTileBytes), kTrTileBytes);
 #pragma unroll
-                    for (int k = 0; k < kK8Hd / 32; ++k) umma_i8(tmem, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), shape, 1u);
-                    umma_commit(b_scores);
-                    mbar_arrive(b_scores);
+                    for (int k = 0; k < kTrTile / 32; ++k) umma_i8(t_values, dv + (uint64_t)(k * (32 * kK8Hd >> 4)), dp + (uint64_t)(k * (32 * kK8Hd >> 4)), d_values, 1u);
+                    umma_commit(&bar[kValues]);
+                    umma_commit(&s_empty[S::stages + st]);
                 }
             }
             __syncwarp();
         }
-    } else if (warp == S::warps + 2) {                   // O^T += V^T P^T
-        if (lane == 0) {
-            constexpr uint32_t shape = kTrShape | (1u << 15) | (1u << 16) | ((uint32_t)(S::o_cols >> 3) << 17);        // both operands transposed
-            const uint64_t dp = tr_desc_mn(smem_addr(s_p), kTrTileBytes);
-            int n = 0;
-            for (TreeWalk walk(L, at); ok && walk.next();) {
-                if (flat0 >= walk.count * L.group) continue;
-                for (int i = walk.t0; ok && i < walk.t1; ++i, ++n) {
-                    const int st = n % S::stages;
-                    ok = mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && mbar_wait_bounded(b_weights, (unsigned)n & 1u);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t dv = tr_desc_mn(smem_addr(base + (size_t)st * 2 * kTrTileBytes + kTrTileBytes), kTrTileBytes);
-#pragma unroll
-                    for (int k = 0; k < kTrTile / 32; ++k)
-                        umma_i8(tmem + S::s_cols, dv + (uint64_t)(k * (32 * kK8Hd >> 4)), dp + (uint64_t)(k * (32 * kK8Hd >> 4)), shape, 1u);
-                    umma_commit(b_values);
-                    umma_commit(&s_empty[st]);
-                }
-            }
-        }
-        __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::most));
         const int quarter = warp & 3, group = warp >> 2, first = group * 16, key = 32 * quarter + lane;      // its keys of a tile, and its queries
         constexpr int kAll = S::warps * 32, kEvery = 7;              // threads, and their barrier (1 .. 4: those of sixteen queries)
-        const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_scores = t_lane + (uint32_t)first, t_values = t_lane + (uint32_t)(S::s_cols + 4 * first), t_moved = t_lane + (uint32_t)(S::s_cols + S::o_cols + first);
+        const int line = first / S::line, in_line = first % S::line;
+        uint64_t* bar = s_bar[line];
+        const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_scores = t_lane + (uint32_t)(line * S::s_cols + in_line),
+                       t_values = t_lane + (uint32_t)(S::all_s + 4 * first), t_moved = t_lane + (uint32_t)(S::all_s + S::all_o + first);
         tr_fill<16>(t_moved, 0u);
         tr_fill<64>(t_values, 0u);
-#pragma unroll
-        for (int part = 0; part < 3; ++part) tr_fill<16>(t_scores + part * R, kTrBias);
         tmem_wait_st();
         tc_fence_before();
         int n = 0;                                       // tiles so far
@@ -565,8 +561,8 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 s_set[group] = 0;
             }
             named_barrier_sync(kEvery, kAll);
-            if (L.aligned) tr_queries<R, true>(L, s_from, s_pos, s_q, s_f);
-            else tr_queries<R, false>(L, s_from, s_pos, s_q, s_f);
+            if (L.aligned) tr_queries<R, S::line, true>(L, s_from, s_pos, s_q, s_f);
+            else tr_queries<R, S::line, false>(L, s_from, s_pos, s_q, s_f);
             fence_proxy_async_smem();
             named_barrier_sync(kQueries, kWithQueries);
             f32x2 l[8];                                  // of key `key`: sums
@@ -593,7 +589,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
             bool early = false;                          // the next scores were seen to be there
             for (int i = walk.t0; i < walk.t1; ++i, ++n) {
                 const int st = n % S::stages, t = i * kTrTile + key;
-                if (!early) ok = ok && mbar_wait_bounded(b_scores, (unsigned)n & 1u);
+                if (!early) ok = ok && mbar_wait_bounded(&bar[kScores], (unsigned)n & 1u);
                 __syncwarp();
                 const unsigned valid = s_valid[st];
                 const bool ragged = (i + 1) * kTrTile > walk.start || valid != 0xffu;
@@ -605,8 +601,14 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 }
                 tc_fence_after();
                 f32x2 w[8];
-                tr_arguments<R>(t_scores, s_f + first, s_down + first, sk, w);
-                const bool values_early = n == 0 || mbar_test(b_values, (unsigned)(n - 1) & 1u);     // (looked at when the weights are ready to be stored)
+                tr_arguments<S::line>(t_scores, s_f + first, s_down + first, sk, w);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&bar[kFree]);
+                    mbar_arrive(&s_empty[st]);
+                }
+                const bool values_early = n == 0 || mbar_test(&bar[kValues], (unsigned)(n - 1) & 1u);     // (looked at when the weights are ready to be stored)
                 if (ragged) tr_hide(w, s_mask + first, t - walk.start, dead);
                 float over = -INFINITY;
 #pragma unroll
@@ -618,10 +620,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 const uint32_t set = s_set[group];
                 const float unit = s_unit[group][0];
                 if (over > kTrSlack || sv > unit || set != 0xffffu || (n + 1) % kTrFlush == 0) s_vote[group][n & 1] = n + 1;
-                tmem_wait_st();
-                tc_fence_before();
                 named_barrier_sync(1 + group, 128);
-                if (lane == 0) mbar_arrive(b_free);
                 const int vote = *reinterpret_cast<volatile int*>(&s_vote[group][n & 1]);
                 f32x2 p[8];
 #pragma unroll
@@ -677,7 +676,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                         p[r / 2] = pack2(tr_ex2(w0 - u0), tr_ex2(w1 - u1));
                     }
                     if (i > walk.t0) {
-                        ok = ok && mbar_wait_bounded(b_values, (unsigned)(n - 1) & 1u);
+                        ok = ok && mbar_wait_bounded(&bar[kValues], (unsigned)(n - 1) & 1u);
                         __syncwarp();
                         tc_fence_after();
 #pragma unroll
@@ -705,19 +704,19 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                     word[2 * r] = __float2uint_rn(p0);
                     word[2 * r + 1] = __float2uint_rn(p1);
                 }
-                if (!values_early) ok = ok && mbar_wait_bounded(b_values, (unsigned)(n - 1) & 1u);    // (the weights in front were read)
+                if (!values_early) ok = ok && mbar_wait_bounded(&bar[kValues], (unsigned)(n - 1) & 1u);    // (the weights in front were read)
                 __syncwarp();
                 unsigned char* to = s_p + (first >> 5) * kTrTileBytes + key * kK8Hd;
                 const int chunk = (first & 31) >> 2;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(to + (((chunk + c) ^ (key & 7)) << 4)) = make_uint4(word[4 * c], word[4 * c + 1], word[4 * c + 2], word[4 * c + 3]);
-                early = i + 1 < walk.t1 && mbar_test(b_scores, (unsigned)(n + 1) & 1u);
+                early = i + 1 < walk.t1 && mbar_test(&bar[kScores], (unsigned)(n + 1) & 1u);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(b_weights);
+                if (lane == 0) mbar_arrive(&bar[kWeights]);
             }
             // ---- the outputs ----
-            ok = ok && mbar_wait_bounded(b_values, (unsigned)(n - 1) & 1u);
+            ok = ok && mbar_wait_bounded(&bar[kValues], (unsigned)(n - 1) & 1u);
             __syncwarp();
             tc_fence_after();
             const float mine = tr_sums(l);
@@ -838,7 +837,7 @@ struct WeighShape {
     static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 2) * 32, stages = 4, resident = R > 32 ? 1 : 2;
     static constexpr int s_cols = 3 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;         // two sets of scores
     static constexpr int q_bytes = s_cols * kK8Hd;
-    static constexpr size_t smem = 1024 + (size_t)stages * kTrTileBytes + q_bytes + stages * kTrTile * 4 + groups * kTwTiles * kTrTile * 4;
+    static constexpr size_t smem = 1024 + (size_t)stages * kTrTileBytes + q_bytes + stages * 2 * kTrTile * 4 + groups * kTwTiles * kTrTile * 4;
 };
 
 template <int R>
@@ -858,10 +857,10 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned char* base = tr_smem + (((smem_addr(tr_smem) + 1023u) & ~1023u) - smem_addr(tr_smem));
     unsigned char* s_q = base + S::stages * kTrTileBytes;
-    float *s_scales = reinterpret_cast<float*>(s_q + S::q_bytes), *s_sum = s_scales + S::stages * kTrTile;
+    float *s_scales = reinterpret_cast<float*>(s_q + S::q_bytes), *s_sum = s_scales + 2 * S::stages * kTrTile;
     if (tid == 0) {
         for (int i = 0; i < S::stages; ++i) {
-            mbar_init(&s_full[i], 1);
+            mbar_init(&s_full[i], 33);
             mbar_init(&s_empty[i], S::warps + 1);        // the products, and the warps that read the scales
         }
         for (int i = 0; i < 2; ++i) {
@@ -888,7 +887,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
 
     if (at.first >= at.all) {
     } else if (warp == S::warps) {
-        TreeCopies<S::stages, false> copies = {a, &kmap, nullptr, base, s_scales, s_full, s_empty, s_valid, 0};
+        TreeCopies<S::stages> copies = {a, &kmap, a.cache.scale_k, nullptr, base, s_scales, s_full, s_empty, s_valid, 0};
         for (TreeWalk walk(L, at); ok && walk.next();)
             for (int t0 = walk.t0; ok && t0 < walk.t1; t0 += kTwTiles)
                 ok = copies.run(walk.seq, walk.kvh, walk.start + walk.count, t0, min(walk.t1, t0 + kTwTiles), (walk.count * L.group + R - 1) / R);
@@ -909,7 +908,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                             tc_fence_after();
                             const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * kTrTileBytes));
 #pragma unroll
-                            for (int k = 0; k < kK8Hd / 32; ++k) umma_i8(tmem + half * S::s_cols, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), shape, 1u);
+                            for (int k = 0; k < kK8Hd / 32; ++k) umma_i8(tmem + half * S::s_cols, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), shape, k > 0);
                             umma_commit(&s_scores[half]);
                             umma_commit(&s_empty[st]);
                             mbar_arrive(&s_scores[half]);
@@ -921,10 +920,6 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
         const int quarter = warp & 3, group = warp >> 2, first = group * 16, key = 32 * quarter + lane;
         constexpr int kAll = S::warps * 32, kEvery = 7;
         const uint32_t t_scores = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)first;
-#pragma unroll
-        for (int part = 0; part < 6; ++part) tr_fill<16>(t_scores + part * R, kTrBias);
-        tmem_wait_st();
-        tc_fence_before();
         float* sums = s_sum + group * kTwTiles * kTrTile + key;
         int n = 0;
         for (TreeWalk walk(L, at); walk.next();)
@@ -954,8 +949,8 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                         mask.store(a, lse < INFINITY, s_mask[tid]);
                     }
                     named_barrier_sync(kEvery, kAll);
-                    if (L.aligned) tr_queries<R, true>(L, s_from, s_pos, s_q, s_f);
-            else tr_queries<R, false>(L, s_from, s_pos, s_q, s_f);
+                    if (L.aligned) tr_queries<R, R, true>(L, s_from, s_pos, s_q, s_f);
+                    else tr_queries<R, R, false>(L, s_from, s_pos, s_q, s_f);
                     fence_proxy_async_smem();
                     named_barrier_sync(kQueries, kWithQueries);
                     for (int i = t0; i < t1; ++i, ++n) {
@@ -964,12 +959,11 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                         __syncwarp();
                         const unsigned valid = s_valid[st];
                         const bool ragged = (i + 1) * kTrTile > walk.start || valid != 0xffu, dead = ragged && (t >= total || !(valid >> (key >> 4) & 1u));
-                        float sk = dead ? 0.0f : s_scales[st * kTrTile + key];
+                        float sk = dead ? 0.0f : s_scales[2 * st * kTrTile + key];
                         if (!(fabsf(sk) < INFINITY)) sk = 0.0f;      // (no query that sees it has a finite lse)
                         tc_fence_after();
                         f32x2 w[8];
                         tr_arguments<R>(t_scores + half * S::s_cols, s_f + first, s_down + first, sk, w);
-                        tmem_wait_st();
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
