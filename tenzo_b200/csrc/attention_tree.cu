@@ -86,6 +86,20 @@ __device__ __forceinline__ void tr_st8(uint32_t at, const float (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  ::"r"(at), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]) : "memory");
 }
+// What one lane of a warp does that is together: which, and a product and a commit of it. (From a branch that one lane takes, the same products start 93 cycles apart and those of 256
+// columns take 169; like this 77 and 128, which is what the multiplications take.)
+__device__ __forceinline__ uint32_t tr_elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void tr_mma(uint32_t elected, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
+}
+__device__ __forceinline__ void tr_commit(uint32_t elected, uint64_t* bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)), "r"(elected) : "memory");
+}
 // Operand tiles that are contiguous along M or N (rows of 128 bytes, one for each k), 128-byte swizzle: eight k are 1024 bytes, `panel` bytes from one 128 to the next.
 __device__ __forceinline__ uint64_t tr_desc_mn(uint32_t saddr, uint32_t panel) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -485,38 +499,41 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
         uint64_t* bar = s_bar[line];
         const uint32_t t_scores = tmem + line * S::s_cols, t_values = tmem + S::all_s + line * S::o_cols;
         const uint64_t dq = umma_desc_sw128(smem_addr(s_q) + line * S::s_cols * kK8Hd), dp = tr_desc_mn(smem_addr(s_p) + line * kTrTileBytes, kTrTileBytes);
+        const uint32_t one = tr_elect();
         int n = 0;                                       // tiles so far
+        auto wait = [&](uint64_t* b, int k) { ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(b, (unsigned)k & 1u)); };
         auto scores = [&](int k) {                       // of the k-th tile
             const int st = k % S::stages;
-            ok = mbar_wait_bounded(&s_full[st], (unsigned)(k / S::stages) & 1u) && (k == 0 || mbar_wait_bounded(&bar[kFree], (unsigned)(k - 1) & 1u));
+            wait(&s_full[st], k / S::stages);
+            if (k > 0) wait(&bar[kFree], k - 1);
             if (!ok) return;
             tc_fence_after();
             const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * kTrTileBytes));
 #pragma unroll
-            for (int i = 0; i < kK8Hd / 32; ++i) umma_i8(t_scores, dk + (uint64_t)(2 * i), dq + (uint64_t)(2 * i), d_scores, i > 0);
-            umma_commit(&bar[kScores]);
-            umma_commit(&s_empty[st]);
-            mbar_arrive(&bar[kScores]);
+            for (int i = 0; i < kK8Hd / 32; ++i) tr_mma(one, t_scores, dk + (uint64_t)(2 * i), dq + (uint64_t)(2 * i), d_scores, i > 0);
+            tr_commit(one, &bar[kScores]);
+            tr_commit(one, &s_empty[st]);
+            if (one) mbar_arrive(&bar[kScores]);
         };
         for (TreeWalk walk(L, at); walk.next();) {
             if (flat0 >= walk.count * L.group) continue;
-            named_barrier_sync(kQueries, kWithQueries);
-            if (lane == 0 && ok) {
-                scores(n);
-                for (int i = walk.t0; ok && i < walk.t1; ++i, ++n) {
-                    if (i + 1 < walk.t1) scores(n + 1);
-                    const int st = n % S::stages;
-                    ok = ok && mbar_wait_bounded(&s_full[S::stages + st], (unsigned)(n / S::stages) & 1u) && mbar_wait_bounded(&bar[kWeights], (unsigned)n & 1u);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t dv = tr_desc_mn(smem_addr(base + (size_t)(S::stages + st) * kTrTileBytes), kTrTileBytes);
-#pragma unroll
-                    for (int k = 0; k < kTrTile / 32; ++k) umma_i8(t_values, dv + (uint64_t)(k * (32 * kK8Hd >> 4)), dp + (uint64_t)(k * (32 * kK8Hd >> 4)), d_values, 1u);
-                    umma_commit(&bar[kValues]);
-                    umma_commit(&s_empty[S::stages + st]);
-                }
-            }
             __syncwarp();
+            named_barrier_sync(kQueries, kWithQueries);
+            if (!ok) continue;
+            scores(n);
+            for (int i = walk.t0; ok && i < walk.t1; ++i, ++n) {
+                if (i + 1 < walk.t1) scores(n + 1);
+                const int st = n % S::stages;
+                wait(&s_full[S::stages + st], n / S::stages);
+                wait(&bar[kWeights], n);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t dv = tr_desc_mn(smem_addr(base + (size_t)(S::stages + st) * kTrTileBytes), kTrTileBytes);
+#pragma unroll
+                for (int k = 0; k < kTrTile / 32; ++k) tr_mma(one, t_values, dv + (uint64_t)(k * (32 * kK8Hd >> 4)), dp + (uint64_t)(k * (32 * kK8Hd >> 4)), d_values, 1u);
+                tr_commit(one, &bar[kValues]);
+                tr_commit(one, &s_empty[S::stages + st]);
+            }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::most));
@@ -895,26 +912,25 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
     } else if (warp == S::warps + 1) {
         constexpr uint32_t shape = kTrShape | (1u << 10) | ((uint32_t)(S::s_cols >> 3) << 17);
         const uint64_t dq = umma_desc_sw128(smem_addr(s_q));
+        const uint32_t one = tr_elect();
         int n = 0;
         for (TreeWalk walk(L, at); walk.next();)
             for (int t0 = walk.t0; t0 < walk.t1; t0 += kTwTiles)
                 for (int flat0 = 0; flat0 < walk.count * L.group; flat0 += R) {
-                    named_barrier_sync(kQueries, kWithQueries);
-                    if (lane == 0) {
-                        for (int i = t0; ok && i < min(walk.t1, t0 + kTwTiles); ++i, ++n) {
-                            const int st = n % S::stages, half = n & 1;
-                            ok = mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n < 2 || mbar_wait_bounded(&s_free[half], (unsigned)(n / 2 - 1) & 1u));
-                            if (!ok) break;
-                            tc_fence_after();
-                            const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * kTrTileBytes));
-#pragma unroll
-                            for (int k = 0; k < kK8Hd / 32; ++k) umma_i8(tmem + half * S::s_cols, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), shape, k > 0);
-                            umma_commit(&s_scores[half]);
-                            umma_commit(&s_empty[st]);
-                            mbar_arrive(&s_scores[half]);
-                        }
-                    }
                     __syncwarp();
+                    named_barrier_sync(kQueries, kWithQueries);
+                    for (int i = t0; ok && i < min(walk.t1, t0 + kTwTiles); ++i, ++n) {
+                        const int st = n % S::stages, half = n & 1;
+                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n < 2 || mbar_wait_bounded(&s_free[half], (unsigned)(n / 2 - 1) & 1u)));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t dk = umma_desc_sw128(smem_addr(base + (size_t)st * kTrTileBytes));
+#pragma unroll
+                        for (int k = 0; k < kK8Hd / 32; ++k) tr_mma(one, tmem + half * S::s_cols, dk + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), shape, k > 0);
+                        tr_commit(one, &s_scores[half]);
+                        tr_commit(one, &s_empty[st]);
+                        if (one) mbar_arrive(&s_scores[half]);
+                    }
                 }
     } else {
         const int quarter = warp & 3, group = warp >> 2, first = group * 16, key = 32 * quarter + lane;
