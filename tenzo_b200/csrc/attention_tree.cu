@@ -313,6 +313,7 @@ struct TreeCopies {
     float* scales;                                       // [STAGES][2][128]
     uint64_t *full, *empty;                              // [STAGES]; full: 33 arrivals and the copies' bytes
     unsigned* s_valid;                                   // [STAGES], or null
+    int *rows, rows_most;                                // null, or where the rows of the last tiles' chunks are remembered: [tile % rows_most][8]
     int n;                                               // tiles that were asked for
     // Tiles t0 .. t1 - 1 of a pair, `passes` times.
     __device__ __forceinline__ bool run(int seq, int kvh, int total, int t0, int t1, int passes) {
@@ -344,7 +345,9 @@ struct TreeCopies {
             };
             copy(scale_k, scales + 2 * st * kTrTile);
             copy(scale_v, scales + (2 * st + 1) * kTrTile);
+            if (rows && (lane >> 3) == (i & 3)) rows[n % rows_most * 8 + (lane & 7)] = now;
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[st])) : "memory");
+            __syncwarp();                                // (lane 0's arrival says that the rows are written)
             if (lane == 0) {
                 if (s_valid) s_valid[st] = there;
                 mbar_expect_tx(&full[st], (unsigned)__popc(there) * (kK8Chunk * kK8Hd));
@@ -486,7 +489,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     } else if (warp >= S::warps && warp <= S::warps + 1) {         // keys; values
         const int ring = warp - S::warps;
         TreeCopies<S::stages> copies = {a, ring ? &vmap : &kmap, ring ? nullptr : a.cache.scale_k, ring ? nullptr : a.cache.scale_v, base + (size_t)ring * S::stages * kTrTileBytes, s_scales,
-                                        s_full + ring * S::stages, s_empty + ring * S::stages, ring ? nullptr : s_valid, 0};
+                                        s_full + ring * S::stages, s_empty + ring * S::stages, ring ? nullptr : s_valid, nullptr, 0, 0};
         for (TreeWalk walk(L, at); ok && walk.next();) {
             if (flat0 >= walk.count * L.group) continue;             // rows of padding alone
             ok = copies.run(walk.seq, walk.kvh, walk.start + walk.count, walk.t0, walk.t1, 1);
@@ -844,17 +847,16 @@ __global__ void __launch_bounds__(kTrMergeWarps * 32) attention_tree_merge_kerne
 }
 
 // ---- the weight that keys receive -------------------------------------------------------------------------------------------------
-// The same scores, for up to kTwTiles tiles of a pair's keys at a time and all its queries, R of them a pass: a thread has one key, so its sum over sixteen queries needs no other
+// The same scores, for some tiles of a pair's keys at a time (as many as there is room for sums) and all its queries, R of them a pass: a thread has one key, so its sum over sixteen queries needs no other
 // lane, and the sums lie in shared memory, each thread's own, until all passes are done. No key has two CTAs: one order of summation, no atomics. Nothing holds the warps together but the
 // scores, of which there are two sets.
-constexpr int kTwTiles = 16;
 
 template <int R>
 struct WeighShape {
-    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 2) * 32, stages = 4, resident = R > 32 ? 1 : 2;
+    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 2) * 32, stages = 4, most = 64 / groups, rows_most = most + 2 * stages, resident = R > 32 ? 1 : 2;
     static constexpr int s_cols = 3 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;         // two sets of scores
     static constexpr int q_bytes = s_cols * kK8Hd;
-    static constexpr size_t smem = 1024 + (size_t)stages * kTrTileBytes + q_bytes + stages * 2 * kTrTile * 4 + groups * kTwTiles * kTrTile * 4;
+    static constexpr size_t smem = 1024 + (size_t)stages * kTrTileBytes + q_bytes + stages * 2 * kTrTile * 4 + groups * most * kTrTile * 4;
 };
 
 template <int R>
@@ -869,7 +871,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
     __shared__ uint64_t s_full[S::stages], s_empty[S::stages], s_scores[2], s_free[2];
     __shared__ unsigned s_valid[S::stages];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_found;
+    __shared__ int s_found, s_rows[S::rows_most * 8];    // rows of the chunks of the last tiles
     __shared__ long long s_scan[S::threads / 32 + 2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned char* base = tr_smem + (((smem_addr(tr_smem) + 1023u) & ~1023u) - smem_addr(tr_smem));
@@ -904,10 +906,10 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
 
     if (at.first >= at.all) {
     } else if (warp == S::warps) {
-        TreeCopies<S::stages> copies = {a, &kmap, a.cache.scale_k, nullptr, base, s_scales, s_full, s_empty, s_valid, 0};
+        TreeCopies<S::stages> copies = {a, &kmap, a.cache.scale_k, nullptr, base, s_scales, s_full, s_empty, s_valid, s_rows, S::rows_most, 0};
         for (TreeWalk walk(L, at); ok && walk.next();)
-            for (int t0 = walk.t0; ok && t0 < walk.t1; t0 += kTwTiles)
-                ok = copies.run(walk.seq, walk.kvh, walk.start + walk.count, t0, min(walk.t1, t0 + kTwTiles), (walk.count * L.group + R - 1) / R);
+            for (int t0 = walk.t0; ok && t0 < walk.t1; t0 += S::most)
+                ok = copies.run(walk.seq, walk.kvh, walk.start + walk.count, t0, min(walk.t1, t0 + S::most), (walk.count * L.group + R - 1) / R);
         if (!ok) copies.drain();
     } else if (warp == S::warps + 1) {
         constexpr uint32_t shape = kTrShape | (1u << 10) | ((uint32_t)(S::s_cols >> 3) << 17);
@@ -915,11 +917,11 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
         const uint32_t one = tr_elect();
         int n = 0;
         for (TreeWalk walk(L, at); walk.next();)
-            for (int t0 = walk.t0; t0 < walk.t1; t0 += kTwTiles)
+            for (int t0 = walk.t0; t0 < walk.t1; t0 += S::most)
                 for (int flat0 = 0; flat0 < walk.count * L.group; flat0 += R) {
                     __syncwarp();
                     named_barrier_sync(kQueries, kWithQueries);
-                    for (int i = t0; ok && i < min(walk.t1, t0 + kTwTiles); ++i, ++n) {
+                    for (int i = t0; ok && i < min(walk.t1, t0 + S::most); ++i, ++n) {
                         const int st = n % S::stages, half = n & 1;
                         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[st], (unsigned)(n / S::stages) & 1u) && (n < 2 || mbar_wait_bounded(&s_free[half], (unsigned)(n / 2 - 1) & 1u)));
                         if (!ok) break;
@@ -936,11 +938,11 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
         const int quarter = warp & 3, group = warp >> 2, first = group * 16, key = 32 * quarter + lane;
         constexpr int kAll = S::warps * 32, kEvery = 7;
         const uint32_t t_scores = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)first;
-        float* sums = s_sum + group * kTwTiles * kTrTile + key;
+        float* sums = s_sum + group * S::most * kTrTile + key;
         int n = 0;
         for (TreeWalk walk(L, at); walk.next();)
-            for (int t0 = walk.t0; t0 < walk.t1; t0 += kTwTiles) {
-                const int t1 = min(walk.t1, t0 + kTwTiles), queries = walk.count * L.group, total = walk.start + walk.count;
+            for (int t0 = walk.t0; t0 < walk.t1; t0 += S::most) {
+                const int t1 = min(walk.t1, t0 + S::most), queries = walk.count * L.group, total = walk.start + walk.count;
                 for (int flat0 = 0; flat0 < queries; flat0 += R) {
                     named_barrier_sync(kEvery, kAll);    // (the queries in front, and the sums, are done with)
                     if (tid < R) {
@@ -974,6 +976,10 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                         ok = ok && mbar_wait_bounded(&s_scores[half], (unsigned)(n / 2) & 1u);
                         __syncwarp();
                         const unsigned valid = s_valid[st];
+                        if (flat0 == 0 && group == 0 && (lane & 15) == 0) {       // the weights, which are wanted when the last pass is done
+                            const int row = s_rows[n % S::rows_most * 8 + (key >> 4)];
+                            if (row >= 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(L.weight + row));
+                        }
                         const bool ragged = (i + 1) * kTrTile > walk.start || valid != 0xffu, dead = ragged && (t >= total || !(valid >> (key >> 4) & 1u));
                         float sk = dead ? 0.0f : s_scales[2 * st * kTrTile + key];
                         if (!(fabsf(sk) < INFINITY)) sk = 0.0f;      // (no query that sees it has a finite lse)
@@ -1001,14 +1007,28 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                     }
                 }
                 named_barrier_sync(kEvery, kAll);
-                for (int k = tid; k < (t1 - t0) * kTrTile; k += kAll) {
-                    const int t = t0 * kTrTile + k, id = t < total ? kv8_block(a.cache, walk.seq, t) : -1;
-                    if (id < 0) continue;
-                    float sum = 0.0f;
+                // the last t1 - t0 tiles' rows are remembered (behind n the copies are at most `stages` tiles)
+                constexpr int kBatch = 8;                // loads in flight
+                for (int k0 = tid; k0 < (t1 - t0) * kTrTile; k0 += kBatch * kAll) {
+                    int row[kBatch];
+                    float old[kBatch];
 #pragma unroll
-                    for (int g = 0; g < S::groups; ++g) sum += s_sum[g * kTwTiles * kTrTile + k];
-                    float* to = L.weight + kv8_row(a.cache, a.layer, walk.kvh, id, t % a.cache.slots);
-                    *to = ld_l2(to) + sum;
+                    for (int u = 0; u < kBatch; ++u) {
+                        const int k = k0 + u * kAll, i = k / kTrTile;
+                        const bool there = k < (t1 - t0) * kTrTile && t0 * kTrTile + k < total;
+                        row[u] = there ? s_rows[(n - (t1 - t0) + i) % S::rows_most * 8 + (k % kTrTile) / kK8Chunk] : -1;
+                        if (row[u] >= 0) row[u] += k % kK8Chunk;
+                    }
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) old[u] = ld_l2(L.weight + max(row[u], 0));           // (something, where there is none)
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) {
+                        float sum = 0.0f;
+                        if (row[u] < 0) continue;
+#pragma unroll
+                        for (int g = 0; g < S::groups; ++g) sum += s_sum[g * S::most * kTrTile + k0 + u * kAll];
+                        L.weight[row[u]] = old[u] + sum;
+                    }
                 }
             }
     }
