@@ -407,7 +407,7 @@ TENZO_API size_t tenzo_cuda_attention_tree_workspace_bytes(int sequences, int no
 TENZO_API int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float* weight, void* stream);
 
 /* Cuts caches back to `keep` tokens, for each layer and kv head on its own: table rows seq[s] (NULL: s) hold length[s] tokens at places 0 .. length[s] - 1, with the
- * weight and position that tenzo_cuda_kv8_append and _weigh left. Where length[s] > keep, the `keep` heaviest stay; a token whose position is protect_from[s] or more counts as
+ * weight and position (16-byte aligned) that tenzo_cuda_kv8_append and _weigh left. Where length[s] > keep, the `keep` heaviest stay; a token whose position is protect_from[s] or more counts as
  * infinitely heavy (protect_from NULL: none does), NaN as -infinity, and of equal weights the lower place stays. Tokens that stay keep their places if those are below `keep`; the others
  * move, in the order of their places, to the places below `keep` that became free, in the order of those, with scales, weight and position. (Order means nothing to
  * attention over rotated keys: it takes one row's move a token evicted, not the whole cache's.) length_out[s] = min(length[s], keep), in

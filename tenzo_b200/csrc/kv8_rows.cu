@@ -12,9 +12,11 @@ int* kv8_rows_flags() {
 }
 
 // ---- append ----------------------------------------------------------------------------------------------------------------
-// A warp takes one kv head of one row: lanes 0-15 the key, 16-31 the value, dims 4l .. 4l + 3 and 64 more a lane, so that the pairs that the
-// rotation turns lie in one lane.
+// A warp takes HB kv heads of one row: lanes 0-15 the keys, 16-31 the values, dims 4l .. 4l + 3 and 64 more a lane, so that the pairs that the rotation turns lie in one lane. Four heads
+// where there are warps enough: what names the row, its place in the table and the rotation's coefficients are asked for once, and four times the bytes are on their way
+// meanwhile (8 x 1000 ragged rows of 8 heads: 16.2 us by fours, 23.4 by ones, 11 of which are the bytes; 512 rows of 5 heads: 3.2 by ones, 3.9 by fours).
 constexpr int kK8RowWarps = 4;
+constexpr long long kK8Many = 148 * 64;                  // (row, head) pairs from which on a warp takes four heads: as many warps as the machine holds
 
 struct K8RowsArgs {
     tenzo_kv8_cache c;
@@ -36,54 +38,64 @@ __device__ __forceinline__ void k8_load4(const float* p, float* x) {
     }
 }
 
-template <bool VEC>
+template <bool VEC, int HB>
 __global__ void __launch_bounds__(kK8RowWarps * 32) kv8_append_kernel(const K8RowsArgs a) {
-    const int lane = threadIdx.x & 31, is_v = lane >> 4, l = lane & 15;
-    const long long unit = (long long)blockIdx.x * kK8RowWarps + (threadIdx.x >> 5);
-    const int kvh = (int)(unit % a.c.n_kv);
-    const long long row = unit / a.c.n_kv;
+    const int lane = threadIdx.x & 31, is_v = lane >> 4, l = lane & 15, blocks = (a.c.n_kv + HB - 1) / HB;
+    const long long unit = (long long)blockIdx.x * kK8RowWarps + (threadIdx.x >> 5), row = unit / blocks;
+    const int head0 = (int)(unit % blocks) * HB;
     if (a.use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
     if (row >= a.rows) return;
     const int place = ld_l2(a.place + row), seq = a.seq ? ld_l2(a.seq + row) : (int)row, pos = a.rope_pos ? ld_l2(a.rope_pos + row) : place;
-    float x[8], c[4], s[4];
-    const float* p = (is_v ? a.v : a.k) + (size_t)row * a.kv_stride + kvh * kK8Hd + 4 * l;
-    k8_load4<VEC>(p, x);
-    k8_load4<VEC>(p + 64, x + 4);
+    float x[HB][8];
+    const float* p = (is_v ? a.v : a.k) + (size_t)row * a.kv_stride + 4 * l;
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {                       // (the last block's missing heads read its first one again)
+        const int head = HB == 1 || head0 + h < a.c.n_kv ? head0 + h : head0;
+        k8_load4<VEC>(p + head * kK8Hd, x[h]);
+        k8_load4<VEC>(p + head * kK8Hd + 64, x[h] + 4);
+    }
     if (place < 0) return;
-    bool there = seq >= 0 && seq < a.c.table_rows && place / a.c.slots < a.c.table_stride && (!a.cs || (pos >= 0 && pos < a.rope_len));
-    const int block = there ? kv8_block(a.c, seq, place) : -1;
-    if (block < 0) {
+    const bool there = seq >= 0 && seq < a.c.table_rows && place / a.c.slots < a.c.table_stride && (!a.cs || (pos >= 0 && pos < a.rope_len));
+    const int id = there ? ld_l2(a.c.block_table + (size_t)seq * a.c.table_stride + place / a.c.slots) : -1;
+    float c[4] = {1, 1, 1, 1}, s[4] = {0, 0, 0, 0};
+    if (a.cs && there) {
+        k8_load4<true>(a.cs + (size_t)pos * 64 + 4 * l, c);
+        k8_load4<true>(a.sn + (size_t)pos * 64 + 4 * l, s);
+    }
+    if (id < 0 || id >= a.c.n_blocks) {
         if (lane == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
         return;
     }
-    if (a.cs && !is_v) {
-        k8_load4<true>(a.cs + (size_t)pos * 64 + 4 * l, c);
-        k8_load4<true>(a.sn + (size_t)pos * 64 + 4 * l, s);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) rope_rotate(x[j], x[4 + j], true, c[j], s[j], x[j], x[4 + j]);
+    for (int h = 0; h < HB; ++h) {
+        if (a.cs && !is_v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) rope_rotate(x[h][j], x[h][4 + j], true, c[j], s[j], x[h][j], x[h][4 + j]);
+        }
+        float amax = 1e-8f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[h][j]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const float scale = amax * (1.0f / 127.0f), inv = 1.0f / scale;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float q = fminf(fmaxf(roundf(x[h][j] * inv), -128.0f), 127.0f);
+            w[j >> 2] |= ((uint32_t)(int)q & 255u) << (8 * (j & 3));
+        }
+        if (HB > 1 && head0 + h >= a.c.n_kv) break;      // (the whole warp)
+        const size_t at = kv8_row(a.c, a.layer, head0 + h, id, place % a.c.slots);
+        uint32_t* to = reinterpret_cast<uint32_t*>((is_v ? a.c.v : a.c.k) + at * kK8Hd);
+        to[l] = w[0];
+        to[16 + l] = w[1];
+        if (l == 0) (is_v ? a.c.scale_v : a.c.scale_k)[at] = scale;
+        if (lane == 1 && a.weight) a.weight[at] = 0.0f;
+        if (lane == 2 && a.position) a.position[at] = pos;
     }
-    float amax = 1e-8f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float scale = amax * (1.0f / 127.0f), inv = 1.0f / scale;
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float q = fminf(fmaxf(roundf(x[j] * inv), -128.0f), 127.0f);
-        w[j >> 2] |= ((uint32_t)(int)q & 255u) << (8 * (j & 3));
-    }
-    const size_t at = kv8_row(a.c, a.layer, kvh, block, place % a.c.slots);
-    uint32_t* to = reinterpret_cast<uint32_t*>((is_v ? a.c.v : a.c.k) + at * kK8Hd);
-    to[l] = w[0];
-    to[16 + l] = w[1];
-    if (l == 0) (is_v ? a.c.scale_v : a.c.scale_k)[at] = scale;
-    if (lane == 1 && a.weight) a.weight[at] = 0.0f;
-    if (lane == 2 && a.position) a.position[at] = pos;
 }
 
 // ---- moving rows: half a warp takes one row, sixteen bytes a lane, keys and values; four lanes take what is beside them ------------------------
@@ -91,13 +103,14 @@ struct K8Row {
     uint4 code;
     uint32_t beside;
 };
+// What lane `which` of a row's sixteen moves beside its codes, and whether it does; those that do not read the keys' scale, for nothing.
 __device__ __forceinline__ uint32_t* k8_beside(const tenzo_kv8_cache& c, float* weight, int* position, int which) {
     return which == 0 ? reinterpret_cast<uint32_t*>(c.scale_k) : which == 1 ? reinterpret_cast<uint32_t*>(c.scale_v) : which == 2 ? reinterpret_cast<uint32_t*>(weight)
          : which == 3 ? reinterpret_cast<uint32_t*>(position) : nullptr;
 }
 __device__ __forceinline__ void k8_take(const tenzo_kv8_cache& c, const uint32_t* beside, size_t row, int l, K8Row& r) {
     r.code = ld_l2(reinterpret_cast<const uint4*>((l & 8 ? c.v : c.k) + row * kK8Hd) + (l & 7));
-    if (beside) r.beside = ld_l2(beside + row);
+    r.beside = ld_l2((beside ? beside : reinterpret_cast<const uint32_t*>(c.scale_k)) + row);
 }
 __device__ __forceinline__ void k8_put(const tenzo_kv8_cache& c, uint32_t* beside, size_t row, int l, const K8Row& r) {
     reinterpret_cast<uint4*>((l & 8 ? c.v : c.k) + row * kK8Hd)[l & 7] = r.code;
@@ -178,18 +191,12 @@ __global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs
         size_t to[kAcBatch];
         bool moves[kAcBatch];
 #pragma unroll
-        for (int b = 0; b < kAcBatch; ++b) {
-            const int e = e0 + b * kAcHalves + half;
-            moves[b] = e < units * rows;
-            if (moves[b]) {
-                const int unit = unit0 + e / rows, d = first + e % rows, layer = unit / a.c.n_kv, kvh = unit % a.c.n_kv;
-                const int2 x = s_at[d][0], y = s_at[d][1];
-                moves[b] = x.x >= 0 && y.x >= 0;
-                if (moves[b]) {
-                    k8_take(a.c, beside, kv8_row(a.c, layer, kvh, x.x, x.y), l, r[b]);
-                    to[b] = kv8_row(a.c, layer, kvh, y.x, y.y);
-                }
-            }
+        for (int b = 0; b < kAcBatch; ++b) {             // (something is read, where there is none, and not stored)
+            const int e = min(e0 + b * kAcHalves + half, units * rows - 1), unit = unit0 + e / rows, d = first + e % rows, layer = unit / a.c.n_kv, kvh = unit % a.c.n_kv;
+            const int2 x = s_at[d][0], y = s_at[d][1];
+            moves[b] = e0 + b * kAcHalves + half < units * rows && x.x >= 0 && y.x >= 0;
+            k8_take(a.c, beside, kv8_row(a.c, layer, kvh, max(x.x, 0), x.y), l, r[b]);
+            to[b] = kv8_row(a.c, layer, kvh, max(y.x, 0), y.y);
         }
         __syncthreads();
 #pragma unroll
@@ -200,9 +207,9 @@ __global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs
 
 // ---- eviction -------------------------------------------------------------------------------------------------------------------
 // One CTA a (sequence, layer, kv head). The weights become whole numbers of the same order (the protected tokens' the largest) in shared memory; the `keep`-th largest is found by
-// counting, two bits a round; what stays is a bit a token; and the free places and the tokens that move into them are two lists, the i-th goes to the i-th.
+// counting, two bits a round, and only those in the range that is left once these are few; what stays is a bit a token; and the free places and the tokens that move into them are two lists, the i-th goes to the i-th.
 // Nothing that moves comes from a place that another moves to (those are below `keep`, these are not), so all rows move at once.
-constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32, kEvBatch = 4;
+constexpr int kEvThreads = 256, kEvWarps = kEvThreads / 32, kEvResident = 4, kEvBatch = 4, kEvLoads = 4;
 constexpr int kEvHeld = 48 * 1024;                       // tokens whose numbers fit in shared memory
 constexpr int kEvMost = 1 << 20, kEvLists = 16 * 1024;   // tokens at most, and entries of both lists together where the numbers do not fit
 
@@ -224,10 +231,11 @@ __device__ __forceinline__ uint32_t ev_number(float w) {
 
 // HELD: the numbers are kept in shared memory; otherwise they are read again each time, and the lists are made a part at a time.
 template <bool HELD>
-__global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a) {
-    extern __shared__ uint32_t ev_smem[];
+__global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(const EvictArgs a) {
+    extern __shared__ __align__(16) uint32_t ev_smem[];
     __shared__ uint32_t s_count[2][kEvWarps][4];
-    __shared__ int s_warp[3][kEvWarps];
+    __shared__ int s_warp[3][kEvWarps], s_listed;
+    __shared__ uint32_t s_list[2 * kEvThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.y, layer = blockIdx.x / a.c.n_kv, kvh = blockIdx.x % a.c.n_kv;
     if (a.use_pdl) {
         pdl_launch_dependents();
@@ -243,30 +251,54 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a
     const int from = a.protect_from ? ld_l2(a.protect_from + s) : 0;
     const int words = (n + 31) / 32, chunks = (words + kEvWarps - 1) / kEvWarps;       // of the bits; a warp's share of them
     uint32_t* s_keep = ev_smem;                          // [words]: what stays
-    uint32_t* s_num = ev_smem + (a.max_len + 31) / 32;   // [n], HELD only; later the two lists
+    uint32_t* s_num = ev_smem + ((a.max_len + 31) / 32 + 3) / 4 * 4;          // [n to 4], HELD only; later the two lists
+    // Numbers of four tokens from 4 g on, and of so many from 4 (g + step) .., 0 behind the last; four tokens lie in one block and are one load. All loads of one kind are in front of the first
+    // that is waited for, and of something where there is nothing (where two ways meet the compiler copies what was loaded, and so waits for it).
     bool bad = false;
-    auto load = [&](int t) -> uint32_t {
-        const int block = kv8_block(a.c, seq, t);
-        if (block < 0) {
-            bad = true;
-            return 0;
+    auto load = [&](int g, int step, uint32_t (&num)[kEvLoads][4]) {
+        size_t row[kEvLoads];
+        int id[kEvLoads];
+        uint4 w[kEvLoads], pos[kEvLoads];
+#pragma unroll
+        for (int u = 0; u < kEvLoads; ++u) id[u] = ld_l2(a.c.block_table + (size_t)seq * a.c.table_stride + min(4 * (g + u * step), n - 1) / a.c.slots);
+#pragma unroll
+        for (int u = 0; u < kEvLoads; ++u) {
+            const bool there = id[u] >= 0 && id[u] < a.c.n_blocks;
+            bad |= !there;
+            row[u] = kv8_row(a.c, layer, kvh, there ? id[u] : 0, min(4 * (g + u * step), (n - 1) & ~3) % a.c.slots);
+            w[u] = ld_l2(reinterpret_cast<const uint4*>(a.weight + row[u]));
         }
-        const size_t row = kv8_row(a.c, layer, kvh, block, t % a.c.slots);
-        return a.protect_from && ld_l2(a.position + row) >= from ? ev_number(INFINITY) : ev_number(ld_l2(a.weight + row));
+#pragma unroll
+        for (int u = 0; u < kEvLoads; ++u) pos[u] = ld_l2(reinterpret_cast<const uint4*>(a.position + row[u]));
+#pragma unroll
+        for (int u = 0; u < kEvLoads; ++u) {
+            const uint32_t wx[4] = {w[u].x, w[u].y, w[u].z, w[u].w}, px[4] = {pos[u].x, pos[u].y, pos[u].z, pos[u].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                num[u][j] = 4 * (g + u * step) + j >= n ? 0u : ev_number(a.protect_from && (int)px[j] >= from ? INFINITY : __uint_as_float(wx[j]));
+        }
     };
     uint32_t lo = 0xffffffffu, hi = 0;
-    for (int t = tid; t < n; t += kEvThreads) {
-        const uint32_t u = load(t);
-        if (HELD) s_num[t] = u;
-        lo = min(lo, u);
-        hi = max(hi, u);
+    for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kEvThreads) {
+        uint32_t num[kEvLoads][4];
+        load(g0 + tid, kEvThreads, num);
+#pragma unroll
+        for (int u = 0; u < kEvLoads; ++u) {
+            const int g = g0 + u * kEvThreads + tid;
+            if (4 * g >= n) break;
+            if (HELD) *reinterpret_cast<uint4*>(s_num + 4 * g) = make_uint4(num[u][0], num[u][1], num[u][2], num[u][3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                lo = num[u][j] ? min(lo, num[u][j]) : lo;
+                hi = max(hi, num[u][j]);
+            }
+        }
     }
     if (tid == 0 && blockIdx.x == 0) a.length_out[s] = a.keep;
     if (__syncthreads_or(bad)) {
         if (tid == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
         return;
     }
-    auto number = [&](int t) { return HELD ? s_num[t] : load(t); };
     // The largest number that `keep` tokens reach: bits from the top, those that all numbers share first.
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
@@ -283,17 +315,67 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a
     int bits = 32 - __clz((int)(lo ^ hi));               // (0: all are equal)
     bits += bits & 1;
     uint32_t border = bits >= 32 ? 0u : lo >> bits << bits;
-    int above = 0;                                       // tokens over the border's present range
-    int round = 1;
+    int above = 0, reach = n;                            // tokens over the border's present range, and those that are not below it
+    int round = 1, base = -1;                            // once few are in the range: the tokens over it then,
+    uint32_t mine0 = 0, mine1 = 0;                       // and the thread's two of those
     while (bits > 0) {
+        if (base < 0 && reach - above <= 2 * kEvThreads) {
+            if (tid == 0) s_listed = 0;
+            __syncthreads();
+            auto list = [&](uint32_t u) {
+                if (u >= border && (bits >= 32 || u - border < 1u << bits) && u != 0) s_list[atomicAdd(&s_listed, 1)] = u;      // (in any order: they are only counted)
+            };
+            if (HELD) {
+                for (int g = tid; 4 * g < n; g += kEvThreads) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(s_num + 4 * g);
+                    list(v.x);
+                    list(v.y);
+                    list(v.z);
+                    list(v.w);
+                }
+            } else {
+                for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kEvThreads) {
+                    uint32_t num[kEvLoads][4];
+                    load(g0 + tid, kEvThreads, num);
+#pragma unroll
+                    for (int u = 0; u < kEvLoads; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) list(num[u][j]);
+                }
+            }
+            __syncthreads();
+            base = above;
+            mine0 = tid < s_listed ? s_list[tid] : 0u;
+            mine1 = tid + kEvThreads < s_listed ? s_list[tid + kEvThreads] : 0u;
+        }
         bits -= 2;
         const uint32_t t1 = border + (1u << bits), t2 = border + (2u << bits), t3 = border + (3u << bits);
-        int c1 = 0, c2 = 0, c3 = 0;
-        for (int t = tid; t < n; t += kEvThreads) {
-            const uint32_t u = number(t);
+        int c1 = 0, c2 = 0, c3 = 0;                      // (border > 0 or a token's number is: ev_number is never 0)
+        auto count = [&](uint32_t u) {
             c1 += u >= t1;
             c2 += u >= t2;
             c3 += u >= t3;
+        };
+        if (base >= 0) {
+            count(mine0);
+            count(mine1);
+        } else if (HELD) {
+            for (int g = tid; 4 * g < n; g += kEvThreads) {
+                const uint4 v = *reinterpret_cast<const uint4*>(s_num + 4 * g);
+                count(v.x);
+                count(v.y);
+                count(v.z);
+                count(v.w);
+            }
+        } else {
+            for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kEvThreads) {
+                uint32_t num[kEvLoads][4];
+                load(g0 + tid, kEvThreads, num);
+#pragma unroll
+                for (int u = 0; u < kEvLoads; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) count(num[u][j]);
+            }
         }
         c1 = __reduce_add_sync(0xffffffffu, c1);
         c2 = __reduce_add_sync(0xffffffffu, c2);
@@ -305,7 +387,7 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a
             sc[warp][2] = c3;
         }
         __syncthreads();
-        c1 = c2 = c3 = 0;
+        c1 = c2 = c3 = max(base, 0);
 #pragma unroll
         for (int w = 0; w < kEvWarps; ++w) {
             const uint4 v = *reinterpret_cast<const uint4*>(sc[w]);
@@ -313,9 +395,9 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a
             c2 += v.y;
             c3 += v.z;
         }
-        if (c3 >= a.keep) border = t3;
-        else if (c2 >= a.keep) border = t2, above = c3;
-        else if (c1 >= a.keep) border = t1, above = c2;
+        if (c3 >= a.keep) border = t3, reach = c3;
+        else if (c2 >= a.keep) border = t2, reach = c2, above = c3;
+        else if (c1 >= a.keep) border = t1, reach = c1, above = c2;
         else above = c1;
         ++round;
     }
@@ -323,11 +405,20 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a
     // that had some over the border's range; before that none were.)
     const int equal = a.keep - above;
     const int w0 = warp * chunks, w1 = min(words, w0 + chunks);
+    // Number of a word's token `lane` (0 behind the last). Not held, the four tokens of the lane's eighth are loaded, and the eight lanes that have the word's take turns.
+    auto number = [&](int w) -> uint32_t {
+        if (HELD) return 32 * w + lane < n ? s_num[32 * w + lane] : 0u;
+        uint32_t num[kEvLoads][4], r = 0;
+        load(8 * w + (lane & 7), 0, num);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t v = __shfl_sync(0xffffffffu, num[0][j], lane >> 2);
+            if ((lane & 3) == j) r = v;
+        }
+        return r;
+    };
     int mine = 0;                                        // equal ones in the warp's share
-    for (int w = w0; w < w1; ++w) {
-        const int t = 32 * w + lane;
-        mine += __popc(__ballot_sync(0xffffffffu, t < n && number(t) == border));
-    }
+    for (int w = w0; w < w1; ++w) mine += __popc(__ballot_sync(0xffffffffu, number(w) == border));
     if (lane == 0) s_warp[0][warp] = mine;
     __syncthreads();
     int before = 0;
@@ -335,9 +426,9 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a
     int holes = 0, far = 0;
     for (int w = w0; w < w1; ++w) {
         const int t = 32 * w + lane;
-        const uint32_t u = t < n ? number(t) : 0;
-        const unsigned same = __ballot_sync(0xffffffffu, t < n && u == border);
-        const bool stays = t < n && (u > border || (u == border && before + __popc(same & ((1u << lane) - 1)) < equal));
+        const uint32_t u = number(w);
+        const unsigned same = __ballot_sync(0xffffffffu, u == border);
+        const bool stays = u > border || (u == border && before + __popc(same & ((1u << lane) - 1)) < equal);
         before += __popc(same);
         const unsigned keep = __ballot_sync(0xffffffffu, stays);
         holes += __popc(__ballot_sync(0xffffffffu, t < a.keep && !stays));
@@ -377,22 +468,20 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(const EvictArgs a
         const int these = min(room, moves - part);
         for (int i0 = half; i0 < these; i0 += kEvThreads / 16 * kEvBatch) {
             K8Row r[kEvBatch];
+            int id[kEvBatch][2], t[kEvBatch][2];
 #pragma unroll
-            for (int b = 0; b < kEvBatch; ++b) {
-                const int i = i0 + b * (kEvThreads / 16);
-                if (i < these) {
-                    const int t = s_far[i];
-                    k8_take(a.c, beside, kv8_row(a.c, layer, kvh, kv8_block(a.c, seq, t), t % a.c.slots), l, r[b]);
-                }
+            for (int b = 0; b < kEvBatch; ++b) {         // (the last row again, where there is none)
+                const int i = min(i0 + b * (kEvThreads / 16), these - 1);
+                t[b][0] = s_far[i];
+                t[b][1] = s_hole[i];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) id[b][e] = ld_l2(a.c.block_table + (size_t)seq * a.c.table_stride + t[b][e] / a.c.slots);
             }
 #pragma unroll
-            for (int b = 0; b < kEvBatch; ++b) {
-                const int i = i0 + b * (kEvThreads / 16);
-                if (i < these) {
-                    const int t = s_hole[i];
-                    k8_put(a.c, beside, kv8_row(a.c, layer, kvh, kv8_block(a.c, seq, t), t % a.c.slots), l, r[b]);
-                }
-            }
+            for (int b = 0; b < kEvBatch; ++b) k8_take(a.c, beside, kv8_row(a.c, layer, kvh, id[b][0], t[b][0] % a.c.slots), l, r[b]);
+#pragma unroll
+            for (int b = 0; b < kEvBatch; ++b)
+                if (i0 + b * (kEvThreads / 16) < these) k8_put(a.c, beside, kv8_row(a.c, layer, kvh, id[b][1], t[b][1] % a.c.slots), l, r[b]);
         }
         __syncthreads();
     }
@@ -407,11 +496,13 @@ extern "C" int tenzo_cuda_kv8_append(const tenzo_kv8_cache* cache, int layer, co
     if (rows == 0) return 0;
     if (!k || !v || !place || kv_stride < (long long)cache->n_kv * kK8Hd || (!seq && rows > cache->table_rows)) return -1;
     if ((rope_cos == nullptr) != (rope_sin == nullptr) || (rope_cos && (rope_len <= 0 || !kv8_aligned(rope_cos, 16) || !kv8_aligned(rope_sin, 16)))) return -1;
-    const long long ctas = ((long long)rows * cache->n_kv + kK8RowWarps - 1) / kK8RowWarps;
+    const int hb = cache->n_kv > 1 && (long long)rows * cache->n_kv > kK8Many ? 4 : 1;
+    const long long ctas = ((long long)rows * ((cache->n_kv + hb - 1) / hb) + kK8RowWarps - 1) / kK8RowWarps;
     if (ctas > 0x7fffffffLL) return -5;
     K8RowsArgs a = {*cache, layer, rows, kv_stride, rope_len, use_pdl, place, seq, rope_pos, k, v, rope_cos, rope_sin, weight, position};
     const bool vec = kv8_aligned(k, 16) && kv8_aligned(v, 16) && kv_stride % 4 == 0;
-    return kv4_launch(vec ? kv8_append_kernel<true> : kv8_append_kernel<false>, dim3((unsigned)ctas), kK8RowWarps * 32, 0, static_cast<cudaStream_t>(stream), use_pdl != 0, a);
+    auto kernel = hb == 4 ? (vec ? kv8_append_kernel<true, 4> : kv8_append_kernel<false, 4>) : (vec ? kv8_append_kernel<true, 1> : kv8_append_kernel<false, 1>);
+    return kv4_launch(kernel, dim3((unsigned)ctas), kK8RowWarps * 32, 0, static_cast<cudaStream_t>(stream), use_pdl != 0, a);
 }
 
 extern "C" int tenzo_cuda_kv8_accept(const tenzo_kv8_cache* cache, const int* token, const int* parent, const int* chosen, const int* start, const int* count, const int* seq,
@@ -435,16 +526,17 @@ extern "C" int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight,
     using namespace tz;
     if (!cache || !kv8_cache_ok(*cache) || sequences < 0) return -1;
     if (sequences == 0) return 0;
-    if (!weight || !position || !length || !length_out || length_out == length || keep <= 0 || max_len <= 0 || max_len > kv8_places(*cache) || (!seq && sequences > cache->table_rows)) return -1;
+    if (!weight || !position || !kv8_aligned(weight, 16) || !kv8_aligned(position, 16) || !length || !length_out || length_out == length || keep <= 0 || max_len <= 0 || max_len > kv8_places(*cache) || (!seq && sequences > cache->table_rows)) return -1;
     if (sequences > 65535 || max_len > kEvMost) return -5;
     EvictArgs a = {*cache, weight, position, length, seq, protect_from, length_out, keep, max_len, use_pdl};
     const bool held = max_len <= kEvHeld;
-    const size_t smem = ((size_t)(max_len + 31) / 32 + (size_t)(held ? max_len : kEvLists)) * 4;
+    const size_t smem = (((size_t)(max_len + 31) / 32 + 3) / 4 * 4 + (size_t)(held ? (max_len + 3) / 4 * 4 : kEvLists)) * 4;
     constexpr size_t most = (kEvHeld / 32 + kEvHeld) * 4;
     static_assert(most >= (kEvMost / 32 + kEvLists) * 4, "the larger of the two");
     static_assert(most <= kMaxSmem - 2048, "bits of the longest and numbers of the longest that are held");
     auto kernel = held ? kv8_evict_kernel<true> : kv8_evict_kernel<false>;
-    if (cudaError_t e = allow_smem(kernel, most)) return (int)e;
+    if (smem > 40 * 1024)
+        if (cudaError_t e = allow_smem(kernel, most)) return (int)e;
     const long long ctas = (long long)cache->n_layers * cache->n_kv;
     if (ctas > 0x7fffffffLL) return -5;
     return kv4_launch(kernel, dim3((unsigned)ctas, (unsigned)sequences), kEvThreads, smem, static_cast<cudaStream_t>(stream), use_pdl != 0, a);

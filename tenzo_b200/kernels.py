@@ -419,17 +419,20 @@ def _tree_calls():
 def _kv8_cache(cache: Kv8Cache, device: int):
     """The fields of abi.Kv8Cache."""
     k, v, sk, sv, table = cache
-    shape, rows = k.shape, table.shape
-    if len(shape) != 5 or shape[4] != 128 or v.shape != shape or sk.shape != shape[:4] or sv.shape != shape[:4] or len(rows) != 2:
+    shape, scales, rows = k.shape, sk.shape, table.shape
+    if len(shape) != 5 or shape[4] != 128 or v.shape != shape or scales != shape[:4] or sv.shape != scales or len(rows) != 2:
         raise ValueError(f"caches [blocks, layers, kv heads, slots, 128], their scales and a table [rows, columns] are needed, not {tuple(shape)}, {tuple(v.shape)}, "
                          f"{tuple(sk.shape)}, {tuple(sv.shape)} and {tuple(rows)}")
+    blocks, layers, n_kv, slots, _ = shape
     return (_arg(k, torch.int8, device, "k"), _arg(v, torch.int8, device, "v"), _arg(sk, torch.float32, device, "scale_k"), _arg(sv, torch.float32, device, "scale_v"),
-            shape[0], shape[1], shape[2], shape[3], _arg(table, torch.int32, device, "block_table"), rows[0], rows[1])
+            blocks, layers, n_kv, slots, _arg(table, torch.int32, device, "block_table"), *rows)
 
 
 def _arg_beside(t, cache: Kv8Cache, dtype, device: int, what: str) -> int:
     """Address of what lies beside the scales; 0 for None."""
-    if t is not None and t.shape != cache.scale_k.shape:
+    if t is None:
+        return 0
+    if t.shape != cache[2].shape:
         raise ValueError(f"{what} has the scales' shape {tuple(cache.scale_k.shape)}, not {tuple(t.shape)}")
     return _arg(t, dtype, device, what)
 
@@ -492,16 +495,26 @@ def attention_tree(q, cache, start, *, layer, n_q, nodes, count=None, mask=None,
     qp, rows, sequences, fields = _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        op = out.data_ptr()
     elif out.shape != (rows, n_q * 128):
         raise ValueError(f"out is [{rows}, {n_q * 128}]")
-    if lse is None:
-        lse = torch.empty(rows, n_q, dtype=torch.float32, device=q.device) if want_lse else None
-    elif lse.shape != (rows, n_q):
-        raise ValueError(f"lse is [{rows}, {n_q}]")
+    else:
+        op = _arg(out, torch.float32, dev, "out")
+    lp = 0
+    if lse is not None:
+        if lse.shape != (rows, n_q):
+            raise ValueError(f"lse is [{rows}, {n_q}]")
+        lp = _arg(lse, torch.float32, dev, "lse")
+    elif want_lse:
+        lse = q.new_empty(rows, n_q)
+        lp = lse.data_ptr()
     if workspace is None:
-        workspace = torch.empty(attention_tree_workspace_bytes(sequences, nodes, n_q, fields[6], shares), dtype=torch.uint8, device=q.device)
-    args = _ATTENTION_TREE.pack(qp, _arg(out, torch.float32, dev, "out"), _arg(lse, torch.float32, dev, "lse"), *fields, _arg_int(shares, "shares"), use_pdl,
-                                _arg(workspace, torch.uint8, dev, "workspace"), workspace.numel())
+        size = attention_tree_workspace_bytes(sequences, nodes, n_q, fields[6], shares)
+        workspace = q.new_empty(-(-size // 4))
+        wp = workspace.data_ptr()
+    else:
+        wp, size = _arg(workspace, torch.uint8, dev, "workspace"), workspace.numel()
+    args = _ATTENTION_TREE.pack(qp, op, lp, *fields, _arg_int(shares, "shares"), use_pdl, wp, size)
     _ok(_tree_calls()[3](args, _raw_stream(dev)), "tenzo_cuda_attention_tree")
     return out if lse is None else (out, lse)
 
@@ -540,9 +553,9 @@ def kv8_accept(cache, token, parent, chosen, start, *, count=None, seq=None, wei
         raise ValueError(f"token, parent and chosen are [sequences, nodes], not {tuple(shape)}, {tuple(parent.shape)} and {tuple(chosen.shape)}")
     sequences, nodes = shape
     fields = _kv8_cache(cache, dev)
-    both = torch.empty(sequences * (nodes + 2), dtype=torch.int32, device=token.device)
-    accepted, following, path = both[:sequences], both[sequences:2 * sequences], both[2 * sequences:].view(sequences, nodes)
-    _ok(_tree_calls()[2](_KV8_CACHE.pack(*fields), _arg(token, torch.int32, dev, "token"), _arg(parent, torch.int32, dev, "parent"), _arg(chosen, torch.int32, dev, "chosen"),
+    tokens = _arg(token, torch.int32, dev, "token")
+    accepted, following, path = token.new_empty(sequences), token.new_empty(sequences), torch.empty_like(token)
+    _ok(_tree_calls()[2](_KV8_CACHE.pack(*fields), tokens, _arg(parent, torch.int32, dev, "parent"), _arg(chosen, torch.int32, dev, "chosen"),
                          _arg_entries(start, sequences, dev, "start"), _arg_entries(count, sequences, dev, "count"), _arg_entries(seq, sequences, dev, "seq"), sequences, nodes,
                          accepted.data_ptr(), following.data_ptr(), path.data_ptr(), _arg_beside(weight, cache, torch.float32, dev, "weight"),
                          _arg_beside(position, cache, torch.int32, dev, "position"), use_pdl, _raw_stream(dev)), "tenzo_cuda_kv8_accept")

@@ -106,7 +106,7 @@ def test_workspace(lib):
     assert need(2, 1, 4, 2, 10) == 48 + 10 * 2 * 16 * 520                       # 1 + 2 * 2 words, and two sets of sixteen rows a share
 
 
-@pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(length=None), -1), (dict(out=None), -1), (dict(out=P), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
+@pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(weight=P + 4), -1), (dict(position=P + 8), -1), (dict(length=None), -1), (dict(out=None), -1), (dict(out=P), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
                                        (dict(max_len=0), -1), (dict(max_len=81), -1), (dict(sequences=-1), -1), (dict(seq=None, sequences=5), -1), (dict(sequences=65536), -5)], ids=str)
 def test_evict(lib, over, code):
     assert evict(lib, cache(), **over) == code
