@@ -403,7 +403,8 @@ TENZO_API size_t tenzo_cuda_attention_tree_workspace_bytes(int sequences, int no
 
 /* The attention weight that each cached token receives: weight[token] += sum over the nodes that see it and the query heads of its kv head of exp(s - lse), s the
  * argument of softmax above. args as for tenzo_cuda_attention_tree, whose lse this reads; out, workspace and shares are not used. weight is laid out as the scales.
- * A row whose lse is not finite adds nothing. Every sum is taken in one order: equal calls give equal bits. No two sequences of a call may name the same table row. */
+ * A row whose lse is not finite adds nothing. Every sum is taken in one order: equal calls give equal bits. No two sequences of a call may name
+ * the same table row, or blocks in common (a token would lose what one of them adds); attention reads common blocks as well as others. */
 TENZO_API int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float* weight, void* stream);
 
 /* Cuts caches back to `keep` tokens, for each layer and kv head on its own: table rows seq[s] (NULL: s) hold length[s] tokens at places 0 .. length[s] - 1, with the
@@ -411,9 +412,9 @@ TENZO_API int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float*
  * infinitely heavy (protect_from NULL: none does), NaN as -infinity, and of equal weights the lower place stays. Tokens that stay keep their places if those are below `keep`; the others
  * move, in the order of their places, to the places below `keep` that became free, in the order of those, with scales, weight and position. (Order means nothing to
  * attention over rotated keys: it takes one row's move a token evicted, not the whole cache's.) length_out[s] = min(length[s], keep), in
- * memory of its own. No two sequences of a call may name the same table row.
- * A negative length, one above max_len or a table row out of range leaves the sequence as it is, length_out with it, and raises the flag; a table entry out of range leaves all of
- * the sequence's rows in their places, and raises it. max_len <= slots * table_stride; max_len <= 2^20 and sequences <= 65535 (-5 otherwise). */
+ * memory of its own. No two sequences of a call may name the same table row, or blocks in common.
+ * A negative length, one above max_len, a table row out of range or a table entry out of range leaves the sequence as it is, with length_out[s] = length[s], and raises the
+ * flag. max_len <= slots * table_stride; max_len <= 2^20 and sequences <= 65535 (-5 otherwise). */
 TENZO_API int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight, int* position, const int* length, const int* seq, const int* protect_from, int sequences,
                                    int keep, int max_len, int* length_out, int use_pdl, void* stream);
 
@@ -423,7 +424,7 @@ TENZO_API int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight, 
  * chosen after the last. Row d of a path is moved from place start[s] + path[d] to start[s] + d in all layers, with scales and weight and position (either may be NULL).
  * count, seq, start as for tenzo_cuda_attention_tree. A sequence of padding (start[s] < 0 or count[s] = 0) has accepted 0, next -1. So has one with start + count above slots * table_stride, with count
  * out of range or a table row out of range, which raises the flag; a table entry out of range leaves the rows that need it where they are, and raises it. No two sequences of a call may
- * name the same table row; sequences <= 65535, nodes <= TENZO_TREE_MOST (-5 otherwise). */
+ * name the same table row, or have blocks in common; sequences <= 65535, nodes <= TENZO_TREE_MOST (-5 otherwise). */
 TENZO_API int tenzo_cuda_kv8_accept(const tenzo_kv8_cache* cache, const int* token, const int* parent, const int* chosen, const int* start, const int* count, const int* seq,
                                     int sequences, int nodes, int* accepted, int* next, int* path, float* weight, int* position, int use_pdl, void* stream);
 /* Error flags of the calls of this section since the last call (bit 0: a bounded wait was given up, bit 1: an index out of range); -1 if the query failed, which leaves the

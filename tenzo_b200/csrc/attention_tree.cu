@@ -106,9 +106,11 @@ __device__ __forceinline__ uint64_t tr_desc_mn(uint32_t saddr, uint32_t panel) {
 }
 __device__ __forceinline__ f32x2 tr_mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 tr_fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-// A sum from its three parts of a whole number (below 2^21 each).
-__device__ __forceinline__ float tr_whole(uint32_t high, uint32_t mid, uint32_t low) {
-    return __fmaf_rn((float)(int)high, 65536.0f, (float)((int)mid * 256 + (int)low));
+// Two sums from the three parts of whole numbers (below 2^21 each). The high part is made a float by adding 1.5 * 2^23 to its bits, as the units that convert are those of 2^x too.
+__device__ __forceinline__ f32x2 tr_whole(const uint32_t* high, const uint32_t* mid, const uint32_t* low) {
+    constexpr float kMagic = 12582912.0f;
+    const f32x2 hi = add2(pack2(__uint_as_float(high[0] + 0x4b400000u), __uint_as_float(high[1] + 0x4b400000u)), pack2(-kMagic, -kMagic));
+    return tr_fma2(hi, pack2(65536.0f, 65536.0f), pack2((float)((int)mid[0] * 256 + (int)low[0]), (float)((int)mid[1] * 256 + (int)low[1])));
 }
 // The same value in N columns of the warp's 32 lanes.
 template <int N>
@@ -397,9 +399,8 @@ __device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, co
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
             const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + 8 * h + j), m = *reinterpret_cast<const ulonglong2*>(s_down + 8 * h + j);
-            auto whole = [&](int k) { return tr_whole(high[h][k], mid[h][k], low[h][k]); };
-            w[4 * h + j / 2] = tr_fma2(pack2(whole(j), whole(j + 1)), tr_mul2(sk2, f.x), m.x);
-            w[4 * h + j / 2 + 1] = tr_fma2(pack2(whole(j + 2), whole(j + 3)), tr_mul2(sk2, f.y), m.y);
+            w[4 * h + j / 2] = tr_fma2(tr_whole(high[h] + j, mid[h] + j, low[h] + j), tr_mul2(sk2, f.x), m.x);
+            w[4 * h + j / 2 + 1] = tr_fma2(tr_whole(high[h] + j + 2, mid[h] + j + 2, low[h] + j + 2), tr_mul2(sk2, f.y), m.y);
         }
     }
 }
@@ -1058,7 +1059,7 @@ static int tree_check(TreeLaunch& L) {
     if (a.layer < 0 || a.layer >= a.cache.n_layers || a.n_q <= 0 || a.n_q % a.cache.n_kv || a.sequences < 0 || a.nodes <= 0 || a.max_len <= 0) return -1;
     if (a.max_len > kv8_places(a.cache) || (!a.seq && a.sequences > a.cache.table_rows)) return -1;
     if ((a.rope_cos == nullptr) != (a.rope_sin == nullptr) || (a.rope_cos && a.rope_len <= 0)) return -1;
-    if (a.nodes > TENZO_TREE_MOST || a.n_q > 1 << 20 || a.cache.n_kv > 65535 || a.max_len > 1 << 30) return -5;
+    if (a.nodes > TENZO_TREE_MOST || a.n_q > 1 << 17 || a.cache.n_kv > 65535 || a.max_len > 1 << 30) return -5;
     if (a.q_stride == 0) a.q_stride = a.n_q * kK8Hd;
     if (a.q_stride < a.n_q * kK8Hd) return -1;
     const int words = (a.nodes + 31) / 32;
@@ -1073,10 +1074,22 @@ static int tree_map(CUtensorMap* map, const tenzo_kv8_cache& c, const int8_t* co
     return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, kK8Hd, (uint64_t)c.n_blocks * c.n_layers * c.n_kv * c.slots, kK8Hd, kK8Hd, kK8Chunk, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Queries a CTA: all of a kv head's, up to 64; more in CTAs of 48 or 64, whichever wastes less (a tile of 48 takes some 0.85 of one of 64).
+// Queries a CTA of the attention: the width at which the CTAs that a tree's queries take cost least, one of 16, 32 and 48 as this much of one of 64. Measured, sequences x 4096 keys:
+// 64 x 24 queries 87 us at 32, 104 at 16, 119 at 48; 32 x 48: 71 at 48, 81 at 64, 85 at 32; 32 x 64: 83 at 64, 87 at 32; 32 x 80: 121 at 32, 126 at 48, 143 at 64; 16 x 128: 81 at
+// 64, 86 at 32; 16 x 144: 97 at 48, 104 at 32, 110 at 64; 4 x 1000: 147 at 64, 154 at 48, 156 at 32; and 64 x 4 queries of 8192 keys 122 at 16, 141 at 32.
 static int tree_queries_a_cta(long long queries) {
-    if (queries <= 64) return queries <= 16 ? 16 : (int)((queries + 15) / 16 * 16);
-    return 0.85 * (double)((queries + 47) / 48) < (double)((queries + 63) / 64) ? 48 : 64;
+    constexpr int width[4] = {64, 48, 32, 16};
+    constexpr double cost[4] = {1.0, 0.80, 0.53, 0.32};
+    int best = 0;
+    for (int i = 1; i < 4; ++i)
+        if (cost[i] * (double)((queries + width[i] - 1) / width[i]) < cost[best] * (double)((queries + width[best] - 1) / width[best])) best = i;
+    return width[best];
+}
+// Queries a pass over the keys whose weights are summed, of which a CTA makes as many as there are: 16, twice if that is enough (64 sequences of 24 or 32 queries, 4096 keys: 70 us; in one of 48, 79);
+// then 48 (32 x 48: 45 us, three of 16 52, one of 64 51; 32 x 80: 74, 79 and 88) or 64, of which a pass of 48 costs 0.87 (16 x 128: 48 us at 64, 60 at 48; 4 x 1000: 174 and 190).
+static int weigh_queries_a_pass(long long queries) {
+    if (queries <= 32) return 16;
+    return 0.87 * (double)((queries + 47) / 48) < (double)((queries + 63) / 64) ? 48 : 64;
 }
 
 // Shares of the keys, with CTAs for every SM.
@@ -1101,7 +1114,7 @@ static int tree_run(const TreeLaunch& L, const CUtensorMap& kmap, const CUtensor
         cudaFuncAttributes f = {};
         return cudaFuncGetAttributes(&f, attention_tree_kernel<R>) == cudaSuccess && f.numRegs == TreeShape<R>::launched;
     }();
-    if (!registers_ok) return -4;
+    if (!registers_ok) return (int)cudaErrorLaunchOutOfResources;
     return kv4_launch(attention_tree_kernel<R>, dim3((unsigned)(L.shares * L.tiles)), TreeShape<R>::threads, TreeShape<R>::smem, st, L.a.use_pdl != 0, L, kmap, vmap);
 }
 template <int R>
@@ -1113,7 +1126,7 @@ static int weigh_run(TreeLaunch L, const CUtensorMap& kmap, cudaStream_t st) {
 }
 
 static bool tree_sizes_ok(int sequences, int nodes, int n_q, int n_kv) {
-    return sequences > 0 && nodes > 0 && nodes <= TENZO_TREE_MOST && n_q > 0 && n_kv > 0 && n_q % n_kv == 0 && n_q <= 1 << 20 && n_kv <= 65535;
+    return sequences > 0 && nodes > 0 && nodes <= TENZO_TREE_MOST && n_q > 0 && n_kv > 0 && n_q % n_kv == 0 && n_q <= 1 << 17 && n_kv <= 65535;
 }
 
 }  // namespace tz
@@ -1168,8 +1181,8 @@ extern "C" int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float
     CUtensorMap kmap;
     if (int rc = tree_map(&kmap, a.cache, a.cache.k)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int r = tree_queries_a_cta((long long)a.nodes * L.group);
-    return r == 16 ? weigh_run<16>(L, kmap, st) : r == 32 ? weigh_run<32>(L, kmap, st) : r == 48 ? weigh_run<48>(L, kmap, st) : weigh_run<64>(L, kmap, st);
+    const int r = weigh_queries_a_pass((long long)a.nodes * L.group);
+    return r == 16 ? weigh_run<16>(L, kmap, st) : r == 48 ? weigh_run<48>(L, kmap, st) : weigh_run<64>(L, kmap, st);
 }
 
 // What runs on any stream is waited for, also on those that do not wait for the default one. Only bits that were seen are cleared: of what another thread's call raises

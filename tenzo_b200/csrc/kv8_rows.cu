@@ -12,9 +12,10 @@ int* kv8_rows_flags() {
 }
 
 // ---- append ----------------------------------------------------------------------------------------------------------------
-// A warp takes HB kv heads of one row: lanes 0-15 the keys, 16-31 the values, dims 4l .. 4l + 3 and 64 more a lane, so that the pairs that the rotation turns lie in one lane. Four heads
-// where there are warps enough: what names the row, its place in the table and the rotation's coefficients are asked for once, and four times the bytes are on their way
-// meanwhile (8 x 1000 ragged rows of 8 heads: 16.2 us by fours, 23.4 by ones, 11 of which are the bytes; 512 rows of 5 heads: 3.2 by ones, 3.9 by fours).
+// A warp takes HB kv heads of one row: lanes 0-15 the keys, 16-31 the values, dims 4l .. 4l + 3 and 64 more a lane, so that the pairs that the rotation turns lie in one lane. Bound
+// by the bytes (5 of 6 read) in long calls and by the chain of loads (place, table, row) in short ones. Four heads a warp where there are warps enough: what names the row, its place in the
+// table and the rotation's coefficients are asked for once, and four times the bytes are on their way meanwhile (8000 rows of 8 heads: 19.0 us by fours, 26.6 by ones; of 4 heads 10.9 and 14.4;
+// 1600 rows of 8: 6.4 and 7.3; 1024: both 5.4; 512 rows of 5 heads: 3.9 and 3.2; 9000 rows of 2 heads: 9.3 and 9.1).
 constexpr int kK8RowWarps = 4;
 constexpr long long kK8Many = 148 * 64;                  // (row, head) pairs from which on a warp takes four heads: as many warps as the machine holds
 
@@ -209,6 +210,8 @@ __global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs
 // One CTA a (sequence, layer, kv head). The weights become whole numbers of the same order (the protected tokens' the largest) in shared memory; the `keep`-th largest is found by
 // counting, two bits a round, and only those in the range that is left once these are few; what stays is a bit a token; and the free places and the tokens that move into them are two lists, the i-th goes to the i-th.
 // Nothing that moves comes from a place that another moves to (those are below `keep`, these are not), so all rows move at once.
+// Threads, CTAs an SM, and loads in flight, measured at 64 x 20 heads of 4224 tokens, and 150 of 2176 (both cold): 256, 4, and 4 of numbers and of rows: 63 and 22.5 us; 128 and 8: 57 and
+// 26.6; 512 and 2: 100 and 30.7; two and eight loads of numbers: 61 and 23.4, 72 and 26.6; of rows: 70 and 24.6, 71 and 24.6.
 constexpr int kEvThreads = 256, kEvWarps = kEvThreads / 32, kEvResident = 4, kEvBatch = 4, kEvLoads = 4;
 constexpr int kEvHeld = 48 * 1024;                       // tokens whose numbers fit in shared memory
 constexpr int kEvMost = 1 << 20, kEvLists = 16 * 1024;   // tokens at most, and entries of both lists together where the numbers do not fit
@@ -294,8 +297,9 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
             }
         }
     }
-    if (tid == 0 && blockIdx.x == 0) a.length_out[s] = a.keep;
-    if (__syncthreads_or(bad)) {
+    bad = __syncthreads_or(bad);
+    if (tid == 0 && blockIdx.x == 0) a.length_out[s] = bad ? n : a.keep;
+    if (bad) {
         if (tid == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
         return;
     }
@@ -496,7 +500,7 @@ extern "C" int tenzo_cuda_kv8_append(const tenzo_kv8_cache* cache, int layer, co
     if (rows == 0) return 0;
     if (!k || !v || !place || kv_stride < (long long)cache->n_kv * kK8Hd || (!seq && rows > cache->table_rows)) return -1;
     if ((rope_cos == nullptr) != (rope_sin == nullptr) || (rope_cos && (rope_len <= 0 || !kv8_aligned(rope_cos, 16) || !kv8_aligned(rope_sin, 16)))) return -1;
-    const int hb = cache->n_kv > 1 && (long long)rows * cache->n_kv > kK8Many ? 4 : 1;
+    const int hb = cache->n_kv > 2 && (long long)rows * cache->n_kv > kK8Many ? 4 : 1;
     const long long ctas = ((long long)rows * ((cache->n_kv + hb - 1) / hb) + kK8RowWarps - 1) / kK8RowWarps;
     if (ctas > 0x7fffffffLL) return -5;
     K8RowsArgs a = {*cache, layer, rows, kv_stride, rope_len, use_pdl, place, seq, rope_pos, k, v, rope_cos, rope_sin, weight, position};
@@ -516,7 +520,7 @@ extern "C" int tenzo_cuda_kv8_accept(const tenzo_kv8_cache* cache, const int* to
     AcceptArgs a = {*cache, token, parent, chosen, start, count, seq, accepted, next, path, weight, position, nodes, 0, use_pdl};
     a.units = (int)((units * sequences + 148 * 8 - 1) / (148 * 8));
     if (a.units > units) a.units = (int)units;
-    if ((long long)a.units * nodes > 0x7fffffffLL) return -5;
+    if ((long long)a.units * nodes > 1 << 30) return -5;
     return kv4_launch(kv8_accept_kernel, dim3((unsigned)((units + a.units - 1) / a.units), (unsigned)sequences), kAcThreads, 0, static_cast<cudaStream_t>(stream),
                       use_pdl != 0, a);
 }
