@@ -33,7 +33,7 @@ struct TreeLaunch {
     int group, tiles, shares;                            // heads a kv head; CTAs for a tree's queries; shares of the keys
     int cut;                                             // shares end anywhere; otherwise with a pair
     int aligned;                                         // queries and tables, to 16 bytes
-    long long* head;                                     // [0]: tiles a share; [1 + pair]: the pair's first tile, -1 where no cut goes through it
+    int2* head;                                          // [pair]: the share that its first tile is in, and the shares that it has a part of; 0 where no cut goes through it
     float* part_o;                                       // [share][tile][2][R][128]
     float2* part_ml;                                     // [share][tile][2][R]: reference (log2), sum
     float* weight;
@@ -237,7 +237,6 @@ struct TreeWalk {
         return true;
     }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
-    __device__ __forceinline__ long long pair_begin() const { return u - t1; }
 };
 
 // ---- the parts that both kernels have ------------------------------------------------------------------------------------------
@@ -480,7 +479,6 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
-    if (L.cut && blockIdx.x == 0 && tid == 0) L.head[0] = at.tiles;
     const bool idle = at.first >= at.all;
     constexpr int kWithQueries = (S::warps + S::lines) * 32, kQueries = 6;       // threads that wait for a pair's queries, and their barrier
     bool ok = true;
@@ -758,7 +756,8 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                     else if (a.lse) a.lse[to] = log_sum;
                 }
             }
-            if (L.cut && tile == 0 && walk.t0 == 0 && tid == 0) L.head[1 + (size_t)walk.s * a.cache.n_kv + walk.kvh] = whole ? -1 : walk.pair_begin();
+            if (L.cut && tile == 0 && walk.t0 == 0 && tid == 0)      // (what this share leaves goes to the next ones, at.tiles each)
+                L.head[(size_t)walk.s * a.cache.n_kv + walk.kvh] = make_int2(share, whole ? 0 : 1 + (int)((walk.tiles - walk.t1 + at.tiles - 1) / at.tiles));
 #pragma unroll
             for (int h = 0; h < 16; h += 8) {
                 float o[8];
@@ -808,32 +807,40 @@ __global__ void __launch_bounds__(kTrMergeWarps * 32) attention_tree_merge_kerne
     pdl_launch_dependents();
     pdl_wait();
     if (head >= a.n_q) return;
-    const int s = (int)(row / a.nodes), node = (int)(row % a.nodes), kvh = head / L.group, flat = node * L.group + head % L.group;
+    const int s = (int)blockIdx.x / a.nodes, node = (int)blockIdx.x - s * a.nodes, kvh = head / L.group, flat = node * L.group + head - kvh * L.group;
+    // (Everything is asked for that does not hang on something else, then the first eight parts and what they count: two ways to memory. One after the other these were 4.6 us of tree 1 x 8's 14.)
+    const unsigned long long pair = ld_l2(reinterpret_cast<const unsigned long long*>(L.head) + (size_t)s * a.cache.n_kv + kvh);
+    const int given = ld_l2(a.rope_pos ? a.rope_pos + row : a.start + s);
     const TreeSequence q(a, s);
-    if (q.refused || q.padding || node >= q.count) return;
-    if (tr_position_refused(a, a.rope_pos ? ld_l2(a.rope_pos + row) : q.start + node)) return;
-    const long long share = ld_l2(reinterpret_cast<const unsigned long long*>(L.head)), begin = ld_l2(reinterpret_cast<const unsigned long long*>(L.head) + 1 + (size_t)s * a.cache.n_kv + kvh);
-    if (begin < 0) return;
-    const int first = (int)(begin / share), parts = (int)((begin + tr_tiles(q) - 1) / share) - first + 1;
+    const int first = (int)(uint32_t)pair, parts = (int)(pair >> 32), pos = a.rope_pos ? given : given + node;
+    if (q.refused || q.padding || node >= q.count || tr_position_refused(a, pos) || parts == 0) return;
     // part i is of share first + i: its second, for the first of them (the pair begins in that share, or at its begin), the first one of the others
     const size_t at = ((size_t)first * L.tiles + flat / queries) * 2 * queries + flat % queries, step = (size_t)L.tiles * 2 * queries;
     auto where = [&](int i) { return at + i * step + (i == 0 ? queries : 0); };
+    constexpr int kBatch = 8;                            // loads in flight
+    float2 v[kBatch];
+    float4 p[kBatch];
+    auto load = [&](int i0) {                            // (the last part again, where there is none)
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const size_t from = where(min(i0 + u, parts - 1));
+            v[u] = ld_l2(L.part_ml + from);
+            p[u] = ld_l2(reinterpret_cast<const float4*>(L.part_o + from * kK8Hd) + lane);
+        }
+    };
+    load(0);
     float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, ld_l2(L.part_ml + where(i)).x);
+    for (int i = kBatch + lane; i < parts; i += 32) m = fmaxf(m, ld_l2(L.part_ml + where(i)).x);
     m = warp_max(m);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) m = fmaxf(m, v[u].x);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float l = 0.0f;
-    constexpr int kBatch = 8;                            // loads in flight
     for (int i0 = 0; i0 < parts; i0 += kBatch) {
-        float2 v[kBatch];
-        float4 p[kBatch];
+        if (i0 > 0) load(i0);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            v[u] = i0 + u < parts ? ld_l2(L.part_ml + where(i0 + u)) : make_float2(kTrLow, 0.0f);
-            p[u] = i0 + u < parts ? ld_l2(reinterpret_cast<const float4*>(L.part_o + where(i0 + u) * kK8Hd) + lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
+            if (i0 + u >= parts) break;
             const float x = tr_ex2(v[u].x - m);
             o.x = __fmaf_rn(p[u].x, x, o.x);
             o.y = __fmaf_rn(p[u].y, x, o.y);
@@ -1102,7 +1109,7 @@ static void tree_plan(TreeLaunch& L) {
 }
 static size_t tree_room(const TreeLaunch& L) {
     const int r = tree_queries_a_cta((long long)L.a.nodes * L.group);
-    const size_t head = ((1 + (size_t)L.a.sequences * L.a.cache.n_kv) * sizeof(long long) + 15) & ~(size_t)15;
+    const size_t head = ((size_t)L.a.sequences * L.a.cache.n_kv * sizeof(int2) + 15) & ~(size_t)15;
     return head + (size_t)L.shares * L.tiles * 2 * r * (kK8Hd + 2) * sizeof(float);
 }
 
@@ -1155,8 +1162,8 @@ extern "C" int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, 
     if (a.shares > 0 && !L.cut) return -1;
     if ((long long)L.shares * L.tiles > 0x7fffffffLL || (long long)a.sequences * a.nodes > 0x7fffffffLL) return -5;
     const int r = tree_queries_a_cta((long long)a.nodes * L.group);
-    L.head = static_cast<long long*>(a.workspace);
-    L.part_o = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + (((1 + (size_t)a.sequences * a.cache.n_kv) * sizeof(long long) + 15) & ~(size_t)15));
+    L.head = static_cast<int2*>(a.workspace);
+    L.part_o = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + (((size_t)a.sequences * a.cache.n_kv * sizeof(int2) + 15) & ~(size_t)15));
     L.part_ml = reinterpret_cast<float2*>(L.part_o + (size_t)L.shares * L.tiles * 2 * r * kK8Hd);
     CUtensorMap kmap, vmap;
     if (int rc = tree_map(&kmap, a.cache, a.cache.k)) return rc;

@@ -71,6 +71,25 @@ class Case:
         assert norm == 0 or np.linalg.norm(out - want_out) <= 4e-6 * norm, np.linalg.norm(out - want_out) / norm      # (the bound above is the worst of all cases)
 
 
+def check_weights(case, q, lse, cache, start, a, want):
+    from tenzo_b200 import kernels
+    weight = dev(case.c.weight)
+    kernels.kv8_weigh(q, lse, cache, weight, start, **a)
+    expect, slack = case.c.weight.astype(np.float64), np.zeros(case.c.weight.shape)
+    for s, w in enumerate(want[4]):
+        if w is None:
+            continue
+        b, o = case.c.at(s, np.arange(w.shape[1]))
+        for h in range(case.c.n_kv):
+            expect[b, case.layer, h, o] += w[h]
+            # an exponential is off by what its argument is off; sums of up to nodes * group numbers and the old weight in fp32
+            slack[b, case.layer, h, o] += w[h] * (2 * want[3].max() + (16 + case.nodes * case.n_q / case.c.n_kv / 8) * 2.0 ** -24)
+    got = host(weight).astype(np.float64)
+    assert (np.abs(got - expect) <= slack + 2.0 ** -23 * np.abs(expect)).all()
+    assert np.array_equal(got[slack == 0], case.c.weight[slack == 0])                       # nothing else is touched
+    assert kernels.kv8_take_errors() == 0
+
+
 CASES = [
     # starts, counts, nodes, n_q, n_kv, further
     ([0], [1], 1, 1, 1, {}),
@@ -102,21 +121,20 @@ def test_tree_and_weights(cuda_lib, starts, counts, nodes, n_q, n_kv, further):
     out, lse = kernels.attention_tree(q, cache, start, want_lse=True, **a)
     want = case.want()
     case.check(out, lse, want)
-    weight = dev(case.c.weight)
-    kernels.kv8_weigh(q, lse, cache, weight, start, **a)
-    expect, slack = case.c.weight.astype(np.float64), np.zeros(case.c.weight.shape)
-    for s, w in enumerate(want[4]):
-        if w is None:
-            continue
-        b, o = case.c.at(s, np.arange(w.shape[1]))
-        for h in range(n_kv):
-            expect[b, case.layer, h, o] += w[h]
-            # an exponential is off by what its argument is off; sums of up to nodes * group numbers and the old weight in fp32
-            slack[b, case.layer, h, o] += w[h] * (2 * want[3].max() + (16 + nodes * n_q / n_kv / 8) * 2.0 ** -24)
-    got = host(weight).astype(np.float64)
-    assert (np.abs(got - expect) <= slack + 2.0 ** -23 * np.abs(expect)).all()
-    assert np.array_equal(got[slack == 0], case.c.weight[slack == 0])                       # nothing else is touched
-    assert kernels.kv8_take_errors() == 0
+    check_weights(case, q, lse, cache, start, a, want)
+
+
+@pytest.mark.parametrize("starts,nodes,n_q,n_kv", [([3300, 2700, 1999, 3500, 900, 3111, 2048], 70, 16, 8), ([5000, 4000, 6000, 2500], 1, 16, 16), ([2000, 3000, 1500, 2300], 100, 32, 16)])
+def test_weights_of_long_shares(cuda_lib, starts, nodes, n_q, n_kv):
+    """Enough keys that every CTA has many tiles, with queries of one pass, of five and of seven, the last of which take two walks."""
+    from tenzo_b200 import kernels
+    case = Case(nodes + 7, starts, [max(1, nodes - 3 * s) for s in range(len(starts))], nodes, n_q, n_kv)
+    cache, start, a = case.arguments()
+    q = dev(case.q)
+    out, lse = kernels.attention_tree(q, cache, start, want_lse=True, **a)
+    want = case.want()
+    case.check(out, lse, want)
+    check_weights(case, q, lse, cache, start, a, want)
 
 
 @pytest.mark.parametrize("nodes,n_q", [(1, 20), (8, 20), (12, 20), (64, 20), (40, 40)])

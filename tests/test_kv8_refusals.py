@@ -103,7 +103,7 @@ def test_workspace(lib):
         room = need(sequences, nodes, n_q, n_kv, 0)
         assert 0 < room - 8 * sequences * n_kv < 64 << 20 and room == kernels.attention_tree_workspace_bytes(sequences, nodes, n_q, n_kv)
         assert need(sequences, nodes, n_q, n_kv, 7) < need(sequences, nodes, n_q, n_kv, 9)
-    assert need(2, 1, 4, 2, 10) == 48 + 10 * 2 * 16 * 520                       # 1 + 2 * 2 words, and two sets of sixteen rows a share
+    assert need(2, 1, 4, 2, 10) == 32 + 10 * 2 * 16 * 520                       # 2 * 2 words, and two sets of sixteen rows a share
 
 
 @pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(weight=P + 4), -1), (dict(position=P + 8), -1), (dict(length=None), -1), (dict(out=None), -1), (dict(out=P), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
