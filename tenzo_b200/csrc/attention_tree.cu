@@ -266,38 +266,42 @@ __device__ __forceinline__ void tr_queries(const TreeLaunch& L, const long long*
         const float* q = L.a.q + max(at[i], 0LL);
         const size_t turn = (size_t)(at[i] < 0 ? 0 : pos[warp + i * (R / 4)]) * 64 + 4 * (lane & 15);
         load4(q + 4 * lane, x[i]);
-        load4(rotate ? L.a.rope_cos + turn : q, c[i]);
-        load4(rotate ? L.a.rope_sin + turn : q, s[i]);
+        load4(rotate ? (lane < 16 ? L.a.rope_cos : L.a.rope_sin) + turn : q, c[i]);
+        load4(rotate ? (lane < 16 ? L.a.rope_sin : L.a.rope_cos) + turn : q, s[i]);
     }
-    float most[4];
+    if (rotate) {                                        // x c - other s in the lower half, other s + x c in the upper one, whose tables were taken the other way round
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float other = __shfl_xor_sync(0xffffffffu, x[i][j], 16);
+                x[i][j] = __fmaf_rn(lane < 16 ? x[i][j] : other, c[i][j], (lane < 16 ? -other : x[i][j]) * s[i][j]);
+            }
+    }
+    uint32_t most[4];                                    // bits of the largest magnitude: infinity's and above where one is not finite
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        uint32_t m = 0x15f79688u;                        // (1e-25)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float other = __shfl_xor_sync(0xffffffffu, x[i][j], 16);
-            const float turned = lane < 16 ? __fmaf_rn(x[i][j], c[i][j], -(other * s[i][j])) : __fmaf_rn(other, s[i][j], x[i][j] * c[i][j]);
-            if (rotate) x[i][j] = turned;
-        }
+        for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(x[i][j]) & 0x7fffffffu);
+        most[i] = __reduce_max_sync(0xffffffffu, m);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) most[i] = fmaxf(tr_warp_max(fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])))), 1e-25f);
-#pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const bool bad = __any_sync(0xffffffffu, !(fabsf(x[i][0]) < INFINITY && fabsf(x[i][1]) < INFINITY && fabsf(x[i][2]) < INFINITY && fabsf(x[i][3]) < INFINITY));
         const int r = warp + i * (R / 4);
-        const uint32_t e = __float_as_uint(most[i]) >> 23;           // 43 .. 254
+        const bool bad = most[i] >= 0x7f800000u;         // (its bytes are anything, as those of a vector that is not there)
+        const uint32_t e = most[i] >> 23;                // 43 .. 254
         const float up = bad || at[i] < 0 ? 0.0f : __uint_as_float((275u - e) << 23);
-        int v[4];
+        // Rounded as the low bits of 1.5 * 2^23; with 128 added to every byte, carries and all, the bytes are the three signed ones and 128 each.
+        uint32_t v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __float2int_rn(x[i][j] * up);          // (NaN: 0)
+        for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(__fmaf_rn(x[i][j], up, 12582912.0f)) - 0x4b400000u + 0x808080u;
+        const uint32_t two0 = prmt(v[0], v[1], 0x5140u), two1 = prmt(v[2], v[3], 0x5140u), top0 = prmt(v[0], v[1], 0x0062u), top1 = prmt(v[2], v[3], 0x0062u);
+        const uint32_t part[3] = {prmt(top0, top1, 0x5410u), prmt(two0, two1, 0x7632u), prmt(two0, two1, 0x5410u)};
+        static_assert(LINE % 8 == 0, "the parts of a vector are swizzled alike");
+        unsigned char* to = s_q + (r / LINE * (3 * LINE) + r % LINE) * kK8Hd + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3);
 #pragma unroll
-        for (int part = 2; part >= 0; --part) {          // the last byte, with its sign; what it leaves, in 256ths; again
-            const int n = r / LINE * (3 * LINE) + part * LINE + r % LINE;
-            const uint32_t word = prmt(prmt((uint32_t)v[0], (uint32_t)v[1], 0x0040u), prmt((uint32_t)v[2], (uint32_t)v[3], 0x0040u), 0x5410u);
-            *reinterpret_cast<uint32_t*>(s_q + n * kK8Hd + (((lane >> 2) ^ (n & 7)) << 4) + 4 * (lane & 3)) = word;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = (v[j] + 128) >> 8;
-        }
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(to + k * LINE * kK8Hd) = part[k] ^ 0x80808080u;
         if (lane == 0) s_f[r] = at[i] < 0 ? 0.0f : bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 21u) << 23) * (0.08838834764831845f * 1.4426950408889634f);
     }
 }
@@ -861,7 +865,7 @@ __global__ void __launch_bounds__(kTrMergeWarps * 32) attention_tree_merge_kerne
 
 template <int R>
 struct WeighShape {
-    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 2) * 32, stages = 4, most = 64 / groups, rows_most = most + 2 * stages, resident = R > 32 ? 1 : 2;
+    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 2) * 32, stages = R == 16 ? 3 : 4, most = R == 16 ? 16 : 128 / groups, rows_most = most + 2 * stages, resident = R == 16 ? 3 : 1;
     static constexpr int s_cols = 3 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;         // two sets of scores
     static constexpr int q_bytes = s_cols * kK8Hd;
     static constexpr size_t smem = 1024 + (size_t)stages * kTrTileBytes + q_bytes + stages * 2 * kTrTile * 4 + groups * most * kTrTile * 4;
@@ -1160,6 +1164,9 @@ extern "C" int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, 
     tree_plan(L);
     L.cut = a.workspace && kv8_aligned(a.workspace, 16) && a.workspace_bytes >= tree_room(L);
     if (a.shares > 0 && !L.cut) return -1;
+    // Up to four tiles are not cut: what the cut saves the second kernel takes again (8 nodes, 500 keys: one sequence 13.5 us whole, 13.4 cut, 16 17.3 and 18.5, 64 29.5 and 35.0; 1000 keys: 17.8 and
+    // 13.2, 24.2 and 26.7, 43.4 and 44.0; 64 nodes, one sequence of 500: 17.2 and 15.6), and the call is one launch.
+    if (a.shares == 0 && a.max_len <= 4 * kTrTile) L.cut = 0;
     if ((long long)L.shares * L.tiles > 0x7fffffffLL || (long long)a.sequences * a.nodes > 0x7fffffffLL) return -5;
     const int r = tree_queries_a_cta((long long)a.nodes * L.group);
     L.head = static_cast<int2*>(a.workspace);
