@@ -859,16 +859,21 @@ __global__ void __launch_bounds__(kTrMergeWarps * 32) attention_tree_merge_kerne
 }
 
 // ---- the weight that keys receive -------------------------------------------------------------------------------------------------
-// The same scores, for some tiles of a pair's keys at a time (as many as there is room for sums) and all its queries, R of them a pass: a thread has one key, so its sum over sixteen queries needs no other
-// lane, and the sums lie in shared memory, each thread's own, until all passes are done. No key has two CTAs: one order of summation, no atomics. Nothing holds the warps together but the
-// scores, of which there are two sets.
-
+// The same scores, R queries a pass: a thread has one key, so its sum over sixteen queries needs no other lane. With sixteen a CTA it is added to the key's weight at once, without a wait (one
+// tile belongs to one CTA, a second pass's addition comes from the same thread behind the first: one order of summation). With more, four warps' sums of a key have to come together: they lie in
+// shared memory, for as many tiles at a time as there is room for, until all passes over these are done. Nothing holds the warps together but the scores, of which there are two sets.
+// Bound by the bytes of the keys for single tokens (64 sequences of 8192 keys, 5 kv heads: 69 us, 54 at the memory's rate), behind a start of some 14000 cycles; for trees by the
+// chain of a pass's queries (5000 cycles, which a CTA's few tiles do not hide: 7 x 33 nodes, 8 x 4 heads, 6001 keys: 50 us) and 1200 cycles a tile of 48 queries.
+// Measured: sums of single tokens in shared memory as well 42.5 us (64 x 4096 keys; at once 40.0); two CTAs an SM of 16 queries and four stages 70.5 (64 x 24 queries; three of three stages 67.2);
+// 64 tiles a block instead of 128 at 48 queries 41.6 (32 x 48; 40.1); eight of sixteen queries left out where there are four: no difference.
 template <int R>
 struct WeighShape {
-    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 2) * 32, stages = R == 16 ? 3 : 4, most = R == 16 ? 16 : 128 / groups, rows_most = most + 2 * stages, resident = R == 16 ? 3 : 1;
+    static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 2) * 32, stages = R == 16 ? 3 : 4, resident = R == 16 ? 3 : 1;
+    static constexpr bool direct = groups == 1;                       // a key has one thread: its sums go to its weight at once
+    static constexpr int most = direct ? 1 << 30 : 128 / groups, rows_most = direct ? stages : most + 2 * stages;
     static constexpr int s_cols = 3 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;         // two sets of scores
     static constexpr int q_bytes = s_cols * kK8Hd;
-    static constexpr size_t smem = 1024 + (size_t)stages * kTrTileBytes + q_bytes + stages * 2 * kTrTile * 4 + groups * most * kTrTile * 4;
+    static constexpr size_t smem = 1024 + (size_t)stages * kTrTileBytes + q_bytes + stages * 2 * kTrTile * 4 + (direct ? 0 : groups * most * kTrTile * 4);
 };
 
 template <int R>
@@ -988,7 +993,8 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                         ok = ok && mbar_wait_bounded(&s_scores[half], (unsigned)(n / 2) & 1u);
                         __syncwarp();
                         const unsigned valid = s_valid[st];
-                        if (flat0 == 0 && group == 0 && (lane & 15) == 0) {       // the weights, which are wanted when the last pass is done
+                        const int direct = S::direct ? s_rows[n % S::rows_most * 8 + (key >> 4)] : -1;
+                        if (!S::direct && flat0 == 0 && group == 0 && (lane & 15) == 0) {     // the weights, which are wanted when the last pass is done
                             const int row = s_rows[n % S::rows_most * 8 + (key >> 4)];
                             if (row >= 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(L.weight + row));
                         }
@@ -1015,9 +1021,11 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                         float sum, other;
                         unpack2(sum2, sum, other);
                         sum += other;
-                        sums[(i - t0) * kTrTile] = flat0 == 0 ? sum : sums[(i - t0) * kTrTile] + sum;
+                        if (!S::direct) sums[(i - t0) * kTrTile] = flat0 == 0 ? sum : sums[(i - t0) * kTrTile] + sum;
+                        else if (ok && !dead) atomicAdd(L.weight + direct + (key & (kK8Chunk - 1)), sum);      // (sums below 2^-126 are 0)
                     }
                 }
+                if (S::direct) continue;
                 named_barrier_sync(kEvery, kAll);
                 // the last t1 - t0 tiles' rows are remembered (behind n the copies are at most `stages` tiles)
                 constexpr int kBatch = 8;                // loads in flight
