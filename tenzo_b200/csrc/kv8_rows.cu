@@ -210,9 +210,10 @@ __global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs
 // One CTA a (sequence, layer, kv head). The weights become whole numbers of the same order (the protected tokens' the largest) in shared memory; the `keep`-th largest is found by
 // counting, two bits a round, and only those in the range that is left once these are few; what stays is a bit a token; and the free places and the tokens that move into them are two lists, the i-th goes to the i-th.
 // Nothing that moves comes from a place that another moves to (those are below `keep`, these are not), so all rows move at once.
-// Threads, CTAs an SM, and loads in flight, measured at 64 x 20 heads of 4224 tokens, and 150 of 2176 (both cold): 256, 4, and 4 of numbers and of rows: 63 and 22.5 us; 128 and 8: 57 and
-// 26.6; 512 and 2: 100 and 30.7; two and eight loads of numbers: 61 and 23.4, 72 and 26.6; of rows: 70 and 24.6, 71 and 24.6.
-constexpr int kEvThreads = 256, kEvWarps = kEvThreads / 32, kEvResident = 4, kEvBatch = 4, kEvLoads = 4;
+// T threads a CTA, 1024 / T CTAs an SM: 256, or 128 where there are more CTAs than that leaves room for at once and shared memory has room for eight an SM (64 x 20 heads of 4224 tokens: 38.3 us of
+// selection by 256, 32.3 by 128; 150 heads of 2176: 5.6 and 6.7; 512 threads, cold and with the moves: 100 and 30.7 us, where 256 take 63 and 22.5). Four loads in flight of numbers and of rows
+// (cold, with the moves: two of numbers 61 and 23.4, eight 72 and 26.6; two of rows 70 and 24.6, eight 71 and 24.6).
+constexpr int kEvBatch = 4, kEvLoads = 4;
 constexpr int kEvHeld = 48 * 1024;                       // tokens whose numbers fit in shared memory
 constexpr int kEvMost = 1 << 20, kEvLists = 16 * 1024;   // tokens at most, and entries of both lists together where the numbers do not fit
 
@@ -233,12 +234,13 @@ __device__ __forceinline__ uint32_t ev_number(float w) {
 }
 
 // HELD: the numbers are kept in shared memory; otherwise they are read again each time, and the lists are made a part at a time.
-template <bool HELD>
-__global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(const EvictArgs a) {
+template <bool HELD, int T>
+__global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const EvictArgs a) {
+    constexpr int kThreads = T, kWarps = T / 32;
     extern __shared__ __align__(16) uint32_t ev_smem[];
-    __shared__ uint32_t s_count[2][kEvWarps][4];
-    __shared__ int s_warp[3][kEvWarps], s_listed;
-    __shared__ uint32_t s_list[2 * kEvThreads];
+    __shared__ uint32_t s_count[2][kWarps][4];
+    __shared__ int s_warp[3][kWarps], s_listed;
+    __shared__ uint32_t s_list[2 * kThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.y, layer = blockIdx.x / a.c.n_kv, kvh = blockIdx.x % a.c.n_kv;
     if (a.use_pdl) {
         pdl_launch_dependents();
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
         return;
     }
     const int from = a.protect_from ? ld_l2(a.protect_from + s) : 0;
-    const int words = (n + 31) / 32, chunks = (words + kEvWarps - 1) / kEvWarps;       // of the bits; a warp's share of them
+    const int words = (n + 31) / 32, chunks = (words + kWarps - 1) / kWarps;       // of the bits; a warp's share of them
     uint32_t* s_keep = ev_smem;                          // [words]: what stays
     uint32_t* s_num = ev_smem + ((a.max_len + 31) / 32 + 3) / 4 * 4;          // [n to 4], HELD only; later the two lists
     // Numbers of four tokens from 4 g on, and of so many from 4 (g + step) .., 0 behind the last; four tokens lie in one block and are one load. All loads of one kind are in front of the first
@@ -282,12 +284,12 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
         }
     };
     uint32_t lo = 0xffffffffu, hi = 0;
-    for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kEvThreads) {
+    for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kThreads) {
         uint32_t num[kEvLoads][4];
-        load(g0 + tid, kEvThreads, num);
+        load(g0 + tid, kThreads, num);
 #pragma unroll
         for (int u = 0; u < kEvLoads; ++u) {
-            const int g = g0 + u * kEvThreads + tid;
+            const int g = g0 + u * kThreads + tid;
             if (4 * g >= n) break;
             if (HELD) *reinterpret_cast<uint4*>(s_num + 4 * g) = make_uint4(num[u][0], num[u][1], num[u][2], num[u][3]);
 #pragma unroll
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kEvWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
         lo = min(lo, s_count[0][w][0]);
         hi = max(hi, s_count[0][w][1]);
     }
@@ -323,14 +325,14 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
     int round = 1, base = -1;                            // once few are in the range: the tokens over it then,
     uint32_t mine0 = 0, mine1 = 0;                       // and the thread's two of those
     while (bits > 0) {
-        if (base < 0 && reach - above <= 2 * kEvThreads) {
+        if (base < 0 && reach - above <= 2 * kThreads) {
             if (tid == 0) s_listed = 0;
             __syncthreads();
             auto list = [&](uint32_t u) {
                 if (u >= border && (bits >= 32 || u - border < 1u << bits) && u != 0) s_list[atomicAdd(&s_listed, 1)] = u;      // (in any order: they are only counted)
             };
             if (HELD) {
-                for (int g = tid; 4 * g < n; g += kEvThreads) {
+                for (int g = tid; 4 * g < n; g += kThreads) {
                     const uint4 v = *reinterpret_cast<const uint4*>(s_num + 4 * g);
                     list(v.x);
                     list(v.y);
@@ -338,9 +340,9 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
                     list(v.w);
                 }
             } else {
-                for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kEvThreads) {
+                for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kThreads) {
                     uint32_t num[kEvLoads][4];
-                    load(g0 + tid, kEvThreads, num);
+                    load(g0 + tid, kThreads, num);
 #pragma unroll
                     for (int u = 0; u < kEvLoads; ++u)
 #pragma unroll
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
             __syncthreads();
             base = above;
             mine0 = tid < s_listed ? s_list[tid] : 0u;
-            mine1 = tid + kEvThreads < s_listed ? s_list[tid + kEvThreads] : 0u;
+            mine1 = tid + kThreads < s_listed ? s_list[tid + kThreads] : 0u;
         }
         bits -= 2;
         const uint32_t t1 = border + (1u << bits), t2 = border + (2u << bits), t3 = border + (3u << bits);
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
             count(mine0);
             count(mine1);
         } else if (HELD) {
-            for (int g = tid; 4 * g < n; g += kEvThreads) {
+            for (int g = tid; 4 * g < n; g += kThreads) {
                 const uint4 v = *reinterpret_cast<const uint4*>(s_num + 4 * g);
                 count(v.x);
                 count(v.y);
@@ -372,9 +374,9 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
                 count(v.w);
             }
         } else {
-            for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kEvThreads) {
+            for (int g0 = 0; 4 * g0 < n; g0 += kEvLoads * kThreads) {
                 uint32_t num[kEvLoads][4];
-                load(g0 + tid, kEvThreads, num);
+                load(g0 + tid, kThreads, num);
 #pragma unroll
                 for (int u = 0; u < kEvLoads; ++u)
 #pragma unroll
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
         __syncthreads();
         c1 = c2 = c3 = max(base, 0);
 #pragma unroll
-        for (int w = 0; w < kEvWarps; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
             const uint4 v = *reinterpret_cast<const uint4*>(sc[w]);
             c1 += v.x;
             c2 += v.y;
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
     }
     __syncthreads();                                     // the numbers are no longer needed
     int hole_at = 0, far_at = 0, moves = 0;
-    for (int w = 0; w < kEvWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
         if (w < warp) {
             hole_at += s_warp[1][w];
             far_at += s_warp[2][w];
@@ -470,12 +472,12 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
         }
         __syncthreads();
         const int these = min(room, moves - part);
-        for (int i0 = half; i0 < these; i0 += kEvThreads / 16 * kEvBatch) {
+        for (int i0 = half; i0 < these; i0 += kThreads / 16 * kEvBatch) {
             K8Row r[kEvBatch];
             int id[kEvBatch][2], t[kEvBatch][2];
 #pragma unroll
             for (int b = 0; b < kEvBatch; ++b) {         // (the last row again, where there is none)
-                const int i = min(i0 + b * (kEvThreads / 16), these - 1);
+                const int i = min(i0 + b * (kThreads / 16), these - 1);
                 t[b][0] = s_far[i];
                 t[b][1] = s_hole[i];
 #pragma unroll
@@ -485,7 +487,7 @@ __global__ void __launch_bounds__(kEvThreads, kEvResident) kv8_evict_kernel(cons
             for (int b = 0; b < kEvBatch; ++b) k8_take(a.c, beside, kv8_row(a.c, layer, kvh, id[b][0], t[b][0] % a.c.slots), l, r[b]);
 #pragma unroll
             for (int b = 0; b < kEvBatch; ++b)
-                if (i0 + b * (kEvThreads / 16) < these) k8_put(a.c, beside, kv8_row(a.c, layer, kvh, id[b][1], t[b][1] % a.c.slots), l, r[b]);
+                if (i0 + b * (kThreads / 16) < these) k8_put(a.c, beside, kv8_row(a.c, layer, kvh, id[b][1], t[b][1] % a.c.slots), l, r[b]);
         }
         __syncthreads();
     }
@@ -538,10 +540,11 @@ extern "C" int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight,
     constexpr size_t most = (kEvHeld / 32 + kEvHeld) * 4;
     static_assert(most >= (kEvMost / 32 + kEvLists) * 4, "the larger of the two");
     static_assert(most <= kMaxSmem - 2048, "bits of the longest and numbers of the longest that are held");
-    auto kernel = held ? kv8_evict_kernel<true> : kv8_evict_kernel<false>;
-    if (smem > 40 * 1024)
-        if (cudaError_t e = allow_smem(kernel, most)) return (int)e;
     const long long ctas = (long long)cache->n_layers * cache->n_kv;
     if (ctas > 0x7fffffffLL) return -5;
-    return kv4_launch(kernel, dim3((unsigned)ctas, (unsigned)sequences), kEvThreads, smem, static_cast<cudaStream_t>(stream), use_pdl != 0, a);
+    const bool many = ctas * sequences > 148 * 4 && 8 * (smem + 3072) <= kMaxSmem;
+    auto kernel = many ? kv8_evict_kernel<true, 128> : held ? kv8_evict_kernel<true, 256> : kv8_evict_kernel<false, 256>;
+    if (smem > 40 * 1024)
+        if (cudaError_t e = allow_smem(kernel, most)) return (int)e;
+    return kv4_launch(kernel, dim3((unsigned)ctas, (unsigned)sequences), many ? 128 : 256, smem, static_cast<cudaStream_t>(stream), use_pdl != 0, a);
 }

@@ -131,6 +131,8 @@ def evict_case(rng, lengths, layers, n_kv, slots, levels=None):
     ([33, 65, 64], 32, 40, 1, 2, 80, 2),
     ([2177], 2048, 256, 1, 5, 16, None),
     ([5000, 1], 4999, 3, 1, 1, 16, 3),
+    ([33 + 37 * s % 90 for s in range(40)], 40, 6, 5, 3, 16, 40),             # (more CTAs than the GPU holds of the larger ones)
+    ([700 + 97 * s % 900 for s in range(40)], 690, 64, 5, 3, 16, None),
 ])
 def test_evict(cuda_lib, lengths, keep, recent, layers, n_kv, slots, levels):
     from tenzo_b200 import kernels
