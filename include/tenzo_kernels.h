@@ -361,9 +361,17 @@ enum { TENZO_TREE_MOST = 256 };  /* nodes of a tree */
  * code = clamp(round(x * (1 / scale)), -128, 127), halves away from zero, each step rounded to fp32. (tenzo_cuda_attention_int8 divides by 127: its scales may differ in
  * the last bit, and a code next to a border by one.) Values have to be finite.
  * weight, position (either may be NULL), laid out as the scales: receive 0 and the row's rotary position, for the calls below. */
-TENZO_API int tenzo_cuda_kv8_append(const tenzo_kv8_cache* cache, int layer, const float* k, const float* v, int kv_stride, const int* place, const int* seq, int rows,
-                                    const int* rope_pos, const float* rope_cos, const float* rope_sin, int rope_len, float* weight, int* position, int use_pdl,
-                                    void* stream);
+typedef struct {
+    tenzo_kv8_cache cache;
+    const float* k; const float* v;                 /* [rows][kv_stride] */
+    const int* place;                               /* [rows] device */
+    const int* seq; const int* rope_pos;            /* [rows] device, or NULL */
+    const float* rope_cos; const float* rope_sin;   /* [rope_len][64], 16-byte aligned; both NULL: no rotation */
+    float* weight; int* position;                   /* or NULL */
+    int layer, kv_stride, rows, rope_len;
+    int use_pdl;
+} tenzo_kv8_append_args;
+TENZO_API int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* stream);
 
 /* Attention of the nodes of a tree, for each of `sequences` trees of up to `nodes` nodes (1 .. TENZO_TREE_MOST): sequence s holds start[s] tokens, and node i's key and
  * value are stored at place start[s] + i already. Node i sees places 0 .. start[s] - 1, and node j if bit j % 32 of mask[(s*nodes + i)*mask_stride + j / 32] is
@@ -395,7 +403,8 @@ typedef struct {
     int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
     void* workspace;         /* 16-byte aligned, contents need not be kept: partial results where a cut goes through a sequence's keys */
     size_t workspace_bytes;  /* tenzo_cuda_attention_tree_workspace_bytes(...), some MB whatever the lengths are. With less, or NULL, shares end with a sequence's kv head, which is
-                                slower for few sequences and for unequal ones; shares > 0 is refused then (-1) */
+                                slower for few sequences and for unequal ones; shares > 0 is refused then (-1). With
+                                shares = 0 it is not used where max_len <= 512 */
 } tenzo_attention_tree_args;
 TENZO_API int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, void* stream);
 /* (0 for arguments that the call refuses.) */
@@ -415,8 +424,16 @@ TENZO_API int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float*
  * memory of its own. No two sequences of a call may name the same table row, or blocks in common.
  * A negative length, one above max_len, a table row out of range or a table entry out of range leaves the sequence as it is, with length_out[s] = length[s], and raises the
  * flag. max_len <= slots * table_stride; max_len <= 2^20 and sequences <= 65535 (-5 otherwise). */
-TENZO_API int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight, int* position, const int* length, const int* seq, const int* protect_from, int sequences,
-                                   int keep, int max_len, int* length_out, int use_pdl, void* stream);
+typedef struct {
+    tenzo_kv8_cache cache;
+    float* weight; int* position;
+    const int* length;                              /* [sequences] device */
+    const int* seq; const int* protect_from;        /* [sequences] device, or NULL */
+    int* length_out;                                /* [sequences] device */
+    int sequences, keep, max_len;
+    int use_pdl;
+} tenzo_kv8_evict_args;
+TENZO_API int tenzo_cuda_kv8_evict(const tenzo_kv8_evict_args* args, void* stream);
 
 /* The nodes of drafted trees that the model agrees with, and their rows moved up behind the cached ones. token, parent, chosen [sequences][nodes]: node i's token, the node it
  * goes on from (below i; node 0 is the root, a token that counts already), and the token that the model chose after node i (its argmax, or a draw). From the root, the next node is the first whose
@@ -425,8 +442,17 @@ TENZO_API int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight, 
  * count, seq, start as for tenzo_cuda_attention_tree. A sequence of padding (start[s] < 0 or count[s] = 0) has accepted 0, next -1. So has one with start + count above slots * table_stride, with count
  * out of range or a table row out of range, which raises the flag; a table entry out of range leaves the rows that need it where they are, and raises it. No two sequences of a call may
  * name the same table row, or have blocks in common; sequences <= 65535, nodes <= TENZO_TREE_MOST (-5 otherwise). */
-TENZO_API int tenzo_cuda_kv8_accept(const tenzo_kv8_cache* cache, const int* token, const int* parent, const int* chosen, const int* start, const int* count, const int* seq,
-                                    int sequences, int nodes, int* accepted, int* next, int* path, float* weight, int* position, int use_pdl, void* stream);
+typedef struct {
+    tenzo_kv8_cache cache;
+    const int* token; const int* parent; const int* chosen;   /* [sequences][nodes] device */
+    const int* start;                               /* [sequences] device */
+    const int* count; const int* seq;               /* [sequences] device, or NULL */
+    int* accepted; int* next; int* path;            /* device: [sequences], [sequences], [sequences][nodes] */
+    float* weight; int* position;                   /* or NULL */
+    int sequences, nodes;
+    int use_pdl;
+} tenzo_kv8_accept_args;
+TENZO_API int tenzo_cuda_kv8_accept(const tenzo_kv8_accept_args* args, void* stream);
 /* Error flags of the calls of this section since the last call (bit 0: a bounded wait was given up, bit 1: an index out of range); -1 if the query failed, which leaves the
  * flags as they are. Synchronises with the device: waits for all of its streams, so it cannot be called while one is captured. */
 TENZO_API int tenzo_cuda_kv8_take_errors(void);

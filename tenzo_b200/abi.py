@@ -88,6 +88,23 @@ class Kv8Cache(C.Structure):
                 ("slots", C.c_int), ("block_table", C.c_void_p), ("table_rows", C.c_int), ("table_stride", C.c_int)]
 
 
+class Kv8AppendArgs(C.Structure):
+    _fields_ = [("cache", Kv8Cache), ("k", C.c_void_p), ("v", C.c_void_p), ("place", C.c_void_p), ("seq", C.c_void_p), ("rope_pos", C.c_void_p), ("rope_cos", C.c_void_p),
+                ("rope_sin", C.c_void_p), ("weight", C.c_void_p), ("position", C.c_void_p), ("layer", C.c_int), ("kv_stride", C.c_int), ("rows", C.c_int), ("rope_len", C.c_int),
+                ("use_pdl", C.c_int)]
+
+
+class Kv8EvictArgs(C.Structure):
+    _fields_ = [("cache", Kv8Cache), ("weight", C.c_void_p), ("position", C.c_void_p), ("length", C.c_void_p), ("seq", C.c_void_p), ("protect_from", C.c_void_p),
+                ("length_out", C.c_void_p), ("sequences", C.c_int), ("keep", C.c_int), ("max_len", C.c_int), ("use_pdl", C.c_int)]
+
+
+class Kv8AcceptArgs(C.Structure):
+    _fields_ = [("cache", Kv8Cache), ("token", C.c_void_p), ("parent", C.c_void_p), ("chosen", C.c_void_p), ("start", C.c_void_p), ("count", C.c_void_p), ("seq", C.c_void_p),
+                ("accepted", C.c_void_p), ("next", C.c_void_p), ("path", C.c_void_p), ("weight", C.c_void_p), ("position", C.c_void_p), ("sequences", C.c_int), ("nodes", C.c_int),
+                ("use_pdl", C.c_int)]
+
+
 class AttentionTreeArgs(C.Structure):
     _fields_ = [
         ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("cache", Kv8Cache),
@@ -229,11 +246,9 @@ def declare_kernel_abi(L):
     L.tenzo_cuda_attention_kv4_splits.restype, L.tenzo_cuda_attention_kv4_splits.argtypes = i32, [i32, i32, i32, i32]
     L.tenzo_cuda_beam_select.restype, L.tenzo_cuda_beam_select.argtypes = i32, [C.POINTER(BeamSelectArgs), vp]
     L.tenzo_cuda_beam_select_workspace_bytes.restype, L.tenzo_cuda_beam_select_workspace_bytes.argtypes = sz, [i32, i32, i32, i32]
-    kv8, tree = C.POINTER(Kv8Cache), C.POINTER(AttentionTreeArgs)
-    L.tenzo_cuda_kv8_append.restype = L.tenzo_cuda_kv8_evict.restype = L.tenzo_cuda_kv8_accept.restype = i32
-    L.tenzo_cuda_kv8_append.argtypes = [kv8, i32, vp, vp, i32, vp, vp, i32, vp, vp, vp, i32, vp, vp, i32, vp]
-    L.tenzo_cuda_kv8_evict.argtypes = [kv8, vp, vp, vp, vp, vp, i32, i32, i32, vp, i32, vp]
-    L.tenzo_cuda_kv8_accept.argtypes = [kv8, vp, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, vp, i32, vp]
+    for name, args in (("append", Kv8AppendArgs), ("evict", Kv8EvictArgs), ("accept", Kv8AcceptArgs)):
+        getattr(L, "tenzo_cuda_kv8_" + name).restype, getattr(L, "tenzo_cuda_kv8_" + name).argtypes = i32, [C.POINTER(args), vp]
+    tree = C.POINTER(AttentionTreeArgs)
     L.tenzo_cuda_attention_tree.restype, L.tenzo_cuda_attention_tree.argtypes = i32, [tree, vp]
     L.tenzo_cuda_attention_tree_workspace_bytes.restype, L.tenzo_cuda_attention_tree_workspace_bytes.argtypes = sz, [i32, i32, i32, i32, i32]
     L.tenzo_cuda_kv8_weigh.restype, L.tenzo_cuda_kv8_weigh.argtypes = i32, [tree, vp, vp]

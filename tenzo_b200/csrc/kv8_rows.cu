@@ -19,15 +19,6 @@ int* kv8_rows_flags() {
 constexpr int kK8RowWarps = 4;
 constexpr long long kK8Many = 148 * 64;                  // (row, head) pairs from which on a warp takes four heads: as many warps as the machine holds
 
-struct K8RowsArgs {
-    tenzo_kv8_cache c;
-    int layer, rows, kv_stride, rope_len, use_pdl;
-    const int *place, *seq, *rope_pos;
-    const float *k, *v, *cs, *sn;
-    float* weight;
-    int* position;
-};
-
 template <bool VEC>
 __device__ __forceinline__ void k8_load4(const float* p, float* x) {
     if (VEC) {
@@ -40,8 +31,8 @@ __device__ __forceinline__ void k8_load4(const float* p, float* x) {
 }
 
 template <bool VEC, int HB>
-__global__ void __launch_bounds__(kK8RowWarps * 32) kv8_append_kernel(const K8RowsArgs a) {
-    const int lane = threadIdx.x & 31, is_v = lane >> 4, l = lane & 15, blocks = (a.c.n_kv + HB - 1) / HB;
+__global__ void __launch_bounds__(kK8RowWarps * 32) kv8_append_kernel(const tenzo_kv8_append_args a) {
+    const int lane = threadIdx.x & 31, is_v = lane >> 4, l = lane & 15, blocks = (a.cache.n_kv + HB - 1) / HB;
     const long long unit = (long long)blockIdx.x * kK8RowWarps + (threadIdx.x >> 5), row = unit / blocks;
     const int head0 = (int)(unit % blocks) * HB;
     if (a.use_pdl) {
@@ -54,25 +45,25 @@ __global__ void __launch_bounds__(kK8RowWarps * 32) kv8_append_kernel(const K8Ro
     const float* p = (is_v ? a.v : a.k) + (size_t)row * a.kv_stride + 4 * l;
 #pragma unroll
     for (int h = 0; h < HB; ++h) {                       // (the last block's missing heads read its first one again)
-        const int head = HB == 1 || head0 + h < a.c.n_kv ? head0 + h : head0;
+        const int head = HB == 1 || head0 + h < a.cache.n_kv ? head0 + h : head0;
         k8_load4<VEC>(p + head * kK8Hd, x[h]);
         k8_load4<VEC>(p + head * kK8Hd + 64, x[h] + 4);
     }
     if (place < 0) return;
-    const bool there = seq >= 0 && seq < a.c.table_rows && place / a.c.slots < a.c.table_stride && (!a.cs || (pos >= 0 && pos < a.rope_len));
-    const int id = there ? ld_l2(a.c.block_table + (size_t)seq * a.c.table_stride + place / a.c.slots) : -1;
+    const bool there = seq >= 0 && seq < a.cache.table_rows && place / a.cache.slots < a.cache.table_stride && (!a.rope_cos || (pos >= 0 && pos < a.rope_len));
+    const int id = there ? ld_l2(a.cache.block_table + (size_t)seq * a.cache.table_stride + place / a.cache.slots) : -1;
     float c[4] = {1, 1, 1, 1}, s[4] = {0, 0, 0, 0};
-    if (a.cs && there) {
-        k8_load4<true>(a.cs + (size_t)pos * 64 + 4 * l, c);
-        k8_load4<true>(a.sn + (size_t)pos * 64 + 4 * l, s);
+    if (a.rope_cos && there) {
+        k8_load4<true>(a.rope_cos + (size_t)pos * 64 + 4 * l, c);
+        k8_load4<true>(a.rope_sin + (size_t)pos * 64 + 4 * l, s);
     }
-    if (id < 0 || id >= a.c.n_blocks) {
+    if (id < 0 || id >= a.cache.n_blocks) {
         if (lane == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
         return;
     }
 #pragma unroll
     for (int h = 0; h < HB; ++h) {
-        if (a.cs && !is_v) {
+        if (a.rope_cos && !is_v) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) rope_rotate(x[h][j], x[h][4 + j], true, c[j], s[j], x[h][j], x[h][4 + j]);
         }
@@ -88,12 +79,12 @@ __global__ void __launch_bounds__(kK8RowWarps * 32) kv8_append_kernel(const K8Ro
             const float q = fminf(fmaxf(roundf(x[h][j] * inv), -128.0f), 127.0f);
             w[j >> 2] |= ((uint32_t)(int)q & 255u) << (8 * (j & 3));
         }
-        if (HB > 1 && head0 + h >= a.c.n_kv) break;      // (the whole warp)
-        const size_t at = kv8_row(a.c, a.layer, head0 + h, id, place % a.c.slots);
-        uint32_t* to = reinterpret_cast<uint32_t*>((is_v ? a.c.v : a.c.k) + at * kK8Hd);
+        if (HB > 1 && head0 + h >= a.cache.n_kv) break;      // (the whole warp)
+        const size_t at = kv8_row(a.cache, a.layer, head0 + h, id, place % a.cache.slots);
+        uint32_t* to = reinterpret_cast<uint32_t*>((is_v ? a.cache.v : a.cache.k) + at * kK8Hd);
         to[l] = w[0];
         to[16 + l] = w[1];
-        if (l == 0) (is_v ? a.c.scale_v : a.c.scale_k)[at] = scale;
+        if (l == 0) (is_v ? a.cache.scale_v : a.cache.scale_k)[at] = scale;
         if (lane == 1 && a.weight) a.weight[at] = 0.0f;
         if (lane == 2 && a.position) a.position[at] = pos;
     }
@@ -121,16 +112,7 @@ __device__ __forceinline__ void k8_put(const tenzo_kv8_cache& c, uint32_t* besid
 // ---- accepted nodes ------------------------------------------------------------------------------------------------------------
 constexpr int kAcThreads = 256, kAcHalves = kAcThreads / 16, kAcBatch = 4;     // rows in flight a half warp
 
-struct AcceptArgs {
-    tenzo_kv8_cache c;
-    const int *token, *parent, *chosen, *start, *count, *seq;
-    int *accepted, *next, *path;
-    float* weight;
-    int* position;
-    int nodes, units, use_pdl;                           // (layer, kv head) pairs a CTA takes
-};
-
-__global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs a) {
+__global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const tenzo_kv8_accept_args a, const int many) {
     __shared__ int s_next[TENZO_TREE_MOST], s_token[TENZO_TREE_MOST], s_chosen[TENZO_TREE_MOST], s_path[TENZO_TREE_MOST + 1];
     __shared__ int2 s_at[TENZO_TREE_MOST][2];            // (block, slot) of a row's old place and of its new one
     __shared__ int s_n;
@@ -141,7 +123,7 @@ __global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs
     }
     const int start = ld_l2(a.start + s), count = a.count ? ld_l2(a.count + s) : a.nodes, seq = a.seq ? ld_l2(a.seq + s) : s;
     const bool padding = start < 0 || count == 0;
-    const bool refused = !padding && (count < 0 || count > a.nodes || seq < 0 || seq >= a.c.table_rows || (long long)start + count > min((long long)a.c.table_stride * a.c.slots, 0x7fffffffLL));
+    const bool refused = !padding && (count < 0 || count > a.nodes || seq < 0 || seq >= a.cache.table_rows || (long long)start + count > min((long long)a.cache.table_stride * a.cache.slots, 0x7fffffffLL));
     if (refused && tid == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
     const int n = padding || refused ? 0 : count;
     int parent = -1;
@@ -173,8 +155,8 @@ __global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs
         const int from = start + s_path[tid], to = start + tid;
         int2 x = make_int2(-1, 0), y = x;
         if (from != to) {
-            x = make_int2(kv8_block(a.c, seq, from), from % a.c.slots);
-            y = make_int2(kv8_block(a.c, seq, to), to % a.c.slots);
+            x = make_int2(kv8_block(a.cache, seq, from), from % a.cache.slots);
+            y = make_int2(kv8_block(a.cache, seq, to), to % a.cache.slots);
             if ((x.x < 0 || y.x < 0) && blockIdx.x == 0) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
         }
         s_at[tid][0] = x;
@@ -185,24 +167,24 @@ __global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const AcceptArgs
     if (rows == 0) return;
     // Row d goes from a node's place to one that is not behind it, and no later row comes from a place in front of its own number: rows are taken in their order,
     // kAcHalves * kAcBatch at a time, and all of those are loaded before the first is stored.
-    const int unit0 = blockIdx.x * a.units, units = min(a.units, a.c.n_layers * a.c.n_kv - unit0), half = tid >> 4, l = tid & 15;
-    uint32_t* beside = k8_beside(a.c, a.weight, a.position, l);
+    const int unit0 = blockIdx.x * many, units = min(many, a.cache.n_layers * a.cache.n_kv - unit0), half = tid >> 4, l = tid & 15;
+    uint32_t* beside = k8_beside(a.cache, a.weight, a.position, l);
     for (int e0 = 0; e0 < units * rows; e0 += kAcHalves * kAcBatch) {
         K8Row r[kAcBatch];
         size_t to[kAcBatch];
         bool moves[kAcBatch];
 #pragma unroll
         for (int b = 0; b < kAcBatch; ++b) {             // (something is read, where there is none, and not stored)
-            const int e = min(e0 + b * kAcHalves + half, units * rows - 1), unit = unit0 + e / rows, d = first + e % rows, layer = unit / a.c.n_kv, kvh = unit % a.c.n_kv;
+            const int e = min(e0 + b * kAcHalves + half, units * rows - 1), unit = unit0 + e / rows, d = first + e % rows, layer = unit / a.cache.n_kv, kvh = unit % a.cache.n_kv;
             const int2 x = s_at[d][0], y = s_at[d][1];
             moves[b] = e0 + b * kAcHalves + half < units * rows && x.x >= 0 && y.x >= 0;
-            k8_take(a.c, beside, kv8_row(a.c, layer, kvh, max(x.x, 0), x.y), l, r[b]);
-            to[b] = kv8_row(a.c, layer, kvh, max(y.x, 0), y.y);
+            k8_take(a.cache, beside, kv8_row(a.cache, layer, kvh, max(x.x, 0), x.y), l, r[b]);
+            to[b] = kv8_row(a.cache, layer, kvh, max(y.x, 0), y.y);
         }
         __syncthreads();
 #pragma unroll
         for (int b = 0; b < kAcBatch; ++b)
-            if (moves[b]) k8_put(a.c, beside, to[b], l, r[b]);
+            if (moves[b]) k8_put(a.cache, beside, to[b], l, r[b]);
     }
 }
 
@@ -217,15 +199,6 @@ constexpr int kEvBatch = 4, kEvLoads = 4;
 constexpr int kEvHeld = 48 * 1024;                       // tokens whose numbers fit in shared memory
 constexpr int kEvMost = 1 << 20, kEvLists = 16 * 1024;   // tokens at most, and entries of both lists together where the numbers do not fit
 
-struct EvictArgs {
-    tenzo_kv8_cache c;
-    float* weight;
-    int* position;
-    const int *length, *seq, *protect_from;
-    int* length_out;
-    int keep, max_len, use_pdl;
-};
-
 // A number whose order is the weight's: NaN as -infinity, -0 as +0.
 __device__ __forceinline__ uint32_t ev_number(float w) {
     w = w == w ? w + 0.0f : -INFINITY;
@@ -235,19 +208,19 @@ __device__ __forceinline__ uint32_t ev_number(float w) {
 
 // HELD: the numbers are kept in shared memory; otherwise they are read again each time, and the lists are made a part at a time.
 template <bool HELD, int T>
-__global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const tenzo_kv8_evict_args a) {
     constexpr int kThreads = T, kWarps = T / 32;
     extern __shared__ __align__(16) uint32_t ev_smem[];
     __shared__ uint32_t s_count[2][kWarps][4];
     __shared__ int s_warp[3][kWarps], s_listed;
     __shared__ uint32_t s_list[2 * kThreads];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.y, layer = blockIdx.x / a.c.n_kv, kvh = blockIdx.x % a.c.n_kv;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.y, layer = blockIdx.x / a.cache.n_kv, kvh = blockIdx.x % a.cache.n_kv;
     if (a.use_pdl) {
         pdl_launch_dependents();
         pdl_wait();
     }
     const int n = ld_l2(a.length + s), seq = a.seq ? ld_l2(a.seq + s) : s;
-    const bool refused = n < 0 || n > a.max_len || seq < 0 || seq >= a.c.table_rows;
+    const bool refused = n < 0 || n > a.max_len || seq < 0 || seq >= a.cache.table_rows;
     if (refused || n <= a.keep) {
         if (tid == 0 && blockIdx.x == 0) a.length_out[s] = n;
         if (tid == 0 && refused) atomicOr(&g_kv8_rows_error, kK8ErrIndex);
@@ -265,12 +238,12 @@ __global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const EvictArgs 
         int id[kEvLoads];
         uint4 w[kEvLoads], pos[kEvLoads];
 #pragma unroll
-        for (int u = 0; u < kEvLoads; ++u) id[u] = ld_l2(a.c.block_table + (size_t)seq * a.c.table_stride + min(4 * (g + u * step), n - 1) / a.c.slots);
+        for (int u = 0; u < kEvLoads; ++u) id[u] = ld_l2(a.cache.block_table + (size_t)seq * a.cache.table_stride + min(4 * (g + u * step), n - 1) / a.cache.slots);
 #pragma unroll
         for (int u = 0; u < kEvLoads; ++u) {
-            const bool there = id[u] >= 0 && id[u] < a.c.n_blocks;
+            const bool there = id[u] >= 0 && id[u] < a.cache.n_blocks;
             bad |= !there;
-            row[u] = kv8_row(a.c, layer, kvh, there ? id[u] : 0, min(4 * (g + u * step), (n - 1) & ~3) % a.c.slots);
+            row[u] = kv8_row(a.cache, layer, kvh, there ? id[u] : 0, min(4 * (g + u * step), (n - 1) & ~3) % a.cache.slots);
             w[u] = ld_l2(reinterpret_cast<const uint4*>(a.weight + row[u]));
         }
 #pragma unroll
@@ -455,7 +428,7 @@ __global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const EvictArgs 
         moves += s_warp[1][w];
     }
     const int half = tid >> 4, l = tid & 15;
-    uint32_t* beside = k8_beside(a.c, a.weight, a.position, l);
+    uint32_t* beside = k8_beside(a.cache, a.weight, a.position, l);
     const int room = HELD ? moves : kEvLists / 2;         // entries of a list
     uint32_t *s_hole = s_num, *s_far = s_num + room;
     for (int part = 0; part < moves; part += room) {
@@ -481,13 +454,13 @@ __global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const EvictArgs 
                 t[b][0] = s_far[i];
                 t[b][1] = s_hole[i];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) id[b][e] = ld_l2(a.c.block_table + (size_t)seq * a.c.table_stride + t[b][e] / a.c.slots);
+                for (int e = 0; e < 2; ++e) id[b][e] = ld_l2(a.cache.block_table + (size_t)seq * a.cache.table_stride + t[b][e] / a.cache.slots);
             }
 #pragma unroll
-            for (int b = 0; b < kEvBatch; ++b) k8_take(a.c, beside, kv8_row(a.c, layer, kvh, id[b][0], t[b][0] % a.c.slots), l, r[b]);
+            for (int b = 0; b < kEvBatch; ++b) k8_take(a.cache, beside, kv8_row(a.cache, layer, kvh, id[b][0], t[b][0] % a.cache.slots), l, r[b]);
 #pragma unroll
             for (int b = 0; b < kEvBatch; ++b)
-                if (i0 + b * (kThreads / 16) < these) k8_put(a.c, beside, kv8_row(a.c, layer, kvh, id[b][1], t[b][1] % a.c.slots), l, r[b]);
+                if (i0 + b * (kThreads / 16) < these) k8_put(a.cache, beside, kv8_row(a.cache, layer, kvh, id[b][1], t[b][1] % a.cache.slots), l, r[b]);
         }
         __syncthreads();
     }
@@ -495,56 +468,55 @@ __global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const EvictArgs 
 
 }  // namespace tz
 
-extern "C" int tenzo_cuda_kv8_append(const tenzo_kv8_cache* cache, int layer, const float* k, const float* v, int kv_stride, const int* place, const int* seq, int rows,
-                                     const int* rope_pos, const float* rope_cos, const float* rope_sin, int rope_len, float* weight, int* position, int use_pdl, void* stream) {
+extern "C" int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* stream) {
     using namespace tz;
-    if (!cache || !kv8_cache_ok(*cache) || layer < 0 || layer >= cache->n_layers || rows < 0) return -1;
-    if (rows == 0) return 0;
-    if (!k || !v || !place || kv_stride < (long long)cache->n_kv * kK8Hd || (!seq && rows > cache->table_rows)) return -1;
-    if ((rope_cos == nullptr) != (rope_sin == nullptr) || (rope_cos && (rope_len <= 0 || !kv8_aligned(rope_cos, 16) || !kv8_aligned(rope_sin, 16)))) return -1;
-    const int hb = cache->n_kv > 2 && (long long)rows * cache->n_kv > kK8Many ? 4 : 1;
-    const long long ctas = ((long long)rows * ((cache->n_kv + hb - 1) / hb) + kK8RowWarps - 1) / kK8RowWarps;
+    if (!args) return -1;
+    const tenzo_kv8_append_args& a = *args;
+    if (!kv8_cache_ok(a.cache) || a.layer < 0 || a.layer >= a.cache.n_layers || a.rows < 0) return -1;
+    if (a.rows == 0) return 0;
+    if (!a.k || !a.v || !a.place || a.kv_stride < (long long)a.cache.n_kv * kK8Hd || (!a.seq && a.rows > a.cache.table_rows)) return -1;
+    if ((a.rope_cos == nullptr) != (a.rope_sin == nullptr) || (a.rope_cos && (a.rope_len <= 0 || !kv8_aligned(a.rope_cos, 16) || !kv8_aligned(a.rope_sin, 16)))) return -1;
+    const int hb = a.cache.n_kv > 2 && (long long)a.rows * a.cache.n_kv > kK8Many ? 4 : 1;
+    const long long ctas = ((long long)a.rows * ((a.cache.n_kv + hb - 1) / hb) + kK8RowWarps - 1) / kK8RowWarps;
     if (ctas > 0x7fffffffLL) return -5;
-    K8RowsArgs a = {*cache, layer, rows, kv_stride, rope_len, use_pdl, place, seq, rope_pos, k, v, rope_cos, rope_sin, weight, position};
-    const bool vec = kv8_aligned(k, 16) && kv8_aligned(v, 16) && kv_stride % 4 == 0;
+    const bool vec = kv8_aligned(a.k, 16) && kv8_aligned(a.v, 16) && a.kv_stride % 4 == 0;
     auto kernel = hb == 4 ? (vec ? kv8_append_kernel<true, 4> : kv8_append_kernel<false, 4>) : (vec ? kv8_append_kernel<true, 1> : kv8_append_kernel<false, 1>);
-    return kv4_launch(kernel, dim3((unsigned)ctas), kK8RowWarps * 32, 0, static_cast<cudaStream_t>(stream), use_pdl != 0, a);
+    return kv4_launch(kernel, dim3((unsigned)ctas), kK8RowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl != 0, a);
 }
 
-extern "C" int tenzo_cuda_kv8_accept(const tenzo_kv8_cache* cache, const int* token, const int* parent, const int* chosen, const int* start, const int* count, const int* seq,
-                                     int sequences, int nodes, int* accepted, int* next, int* path, float* weight, int* position, int use_pdl, void* stream) {
+extern "C" int tenzo_cuda_kv8_accept(const tenzo_kv8_accept_args* args, void* stream) {
     using namespace tz;
-    if (!cache || !kv8_cache_ok(*cache) || sequences < 0) return -1;
-    if (sequences == 0) return 0;
-    if (!token || !parent || !chosen || !start || !accepted || !next || !path || nodes <= 0 || (!seq && sequences > cache->table_rows)) return -1;
-    if (nodes > TENZO_TREE_MOST || sequences > 65535) return -5;
-    const long long units = (long long)cache->n_layers * cache->n_kv;
-    AcceptArgs a = {*cache, token, parent, chosen, start, count, seq, accepted, next, path, weight, position, nodes, 0, use_pdl};
-    a.units = (int)((units * sequences + 148 * 8 - 1) / (148 * 8));
-    if (a.units > units) a.units = (int)units;
-    if ((long long)a.units * nodes > 1 << 30) return -5;
-    return kv4_launch(kv8_accept_kernel, dim3((unsigned)((units + a.units - 1) / a.units), (unsigned)sequences), kAcThreads, 0, static_cast<cudaStream_t>(stream),
-                      use_pdl != 0, a);
+    if (!args) return -1;
+    const tenzo_kv8_accept_args& a = *args;
+    if (!kv8_cache_ok(a.cache) || a.sequences < 0) return -1;
+    if (a.sequences == 0) return 0;
+    if (!a.token || !a.parent || !a.chosen || !a.start || !a.accepted || !a.next || !a.path || a.nodes <= 0 || (!a.seq && a.sequences > a.cache.table_rows)) return -1;
+    if (a.nodes > TENZO_TREE_MOST || a.sequences > 65535) return -5;
+    const long long units = (long long)a.cache.n_layers * a.cache.n_kv, share = (units * a.sequences + 148 * 8 - 1) / (148 * 8);
+    const int many = (int)(share < units ? share : units);           // (layer, kv head) pairs a CTA takes
+    if ((long long)many * a.nodes > 1 << 30) return -5;
+    return kv4_launch(kv8_accept_kernel, dim3((unsigned)((units + many - 1) / many), (unsigned)a.sequences), kAcThreads, 0, static_cast<cudaStream_t>(stream), a.use_pdl != 0, a, many);
 }
 
-extern "C" int tenzo_cuda_kv8_evict(const tenzo_kv8_cache* cache, float* weight, int* position, const int* length, const int* seq, const int* protect_from, int sequences,
-                                    int keep, int max_len, int* length_out, int use_pdl, void* stream) {
+extern "C" int tenzo_cuda_kv8_evict(const tenzo_kv8_evict_args* args, void* stream) {
     using namespace tz;
-    if (!cache || !kv8_cache_ok(*cache) || sequences < 0) return -1;
-    if (sequences == 0) return 0;
-    if (!weight || !position || !kv8_aligned(weight, 16) || !kv8_aligned(position, 16) || !length || !length_out || length_out == length || keep <= 0 || max_len <= 0 || max_len > kv8_places(*cache) || (!seq && sequences > cache->table_rows)) return -1;
-    if (sequences > 65535 || max_len > kEvMost) return -5;
-    EvictArgs a = {*cache, weight, position, length, seq, protect_from, length_out, keep, max_len, use_pdl};
-    const bool held = max_len <= kEvHeld;
-    const size_t smem = (((size_t)(max_len + 31) / 32 + 3) / 4 * 4 + (size_t)(held ? (max_len + 3) / 4 * 4 : kEvLists)) * 4;
+    if (!args) return -1;
+    const tenzo_kv8_evict_args& a = *args;
+    if (!kv8_cache_ok(a.cache) || a.sequences < 0) return -1;
+    if (a.sequences == 0) return 0;
+    if (!a.weight || !a.position || !kv8_aligned(a.weight, 16) || !kv8_aligned(a.position, 16) || !a.length || !a.length_out || a.length_out == a.length) return -1;
+    if (a.keep <= 0 || a.max_len <= 0 || a.max_len > kv8_places(a.cache) || (!a.seq && a.sequences > a.cache.table_rows)) return -1;
+    if (a.sequences > 65535 || a.max_len > kEvMost) return -5;
+    const bool held = a.max_len <= kEvHeld;
+    const size_t smem = (((size_t)(a.max_len + 31) / 32 + 3) / 4 * 4 + (size_t)(held ? (a.max_len + 3) / 4 * 4 : kEvLists)) * 4;
     constexpr size_t most = (kEvHeld / 32 + kEvHeld) * 4;
     static_assert(most >= (kEvMost / 32 + kEvLists) * 4, "the larger of the two");
-    static_assert(most <= kMaxSmem - 2048, "bits of the longest and numbers of the longest that are held");
-    const long long ctas = (long long)cache->n_layers * cache->n_kv;
+    static_assert(most <= kMaxSmem - 3072, "bits of the longest and numbers of the longest that are held");
+    const long long ctas = (long long)a.cache.n_layers * a.cache.n_kv;
     if (ctas > 0x7fffffffLL) return -5;
-    const bool many = ctas * sequences > 148 * 4 && 8 * (smem + 3072) <= kMaxSmem;
+    const bool many = ctas * a.sequences > 148 * 4 && 8 * (smem + 3072) <= kMaxSmem;
     auto kernel = many ? kv8_evict_kernel<true, 128> : held ? kv8_evict_kernel<true, 256> : kv8_evict_kernel<false, 256>;
     if (smem > 40 * 1024)
         if (cudaError_t e = allow_smem(kernel, most)) return (int)e;
-    return kv4_launch(kernel, dim3((unsigned)ctas, (unsigned)sequences), many ? 128 : 256, smem, static_cast<cudaStream_t>(stream), use_pdl != 0, a);
+    return kv4_launch(kernel, dim3((unsigned)ctas, (unsigned)a.sequences), many ? 128 : 256, smem, static_cast<cudaStream_t>(stream), a.use_pdl != 0, a);
 }

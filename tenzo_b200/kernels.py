@@ -398,7 +398,13 @@ class Kv8Cache(NamedTuple):
 
 _KV8_CACHE = struct.Struct("@PPPPiiiiPii0P")                            # abi.Kv8Cache
 _ATTENTION_TREE = struct.Struct("@PPPPPPPiiiiPii0PPPPPPPPiiiiiiiiiiPN")    # abi.AttentionTreeArgs
-assert _KV8_CACHE.size == C.sizeof(abi.Kv8Cache) and _ATTENTION_TREE.size == C.sizeof(abi.AttentionTreeArgs)
+_F32, _I32, _I8, _U8 = torch.float32, torch.int32, torch.int8, torch.uint8
+_TREE_WHOLE = 512                                                      # max_len to which the attention cuts no sequence, and needs no workspace
+_KV8_APPEND = struct.Struct("@PPPPiiiiPiiPPPPPPPPPiiiii0P")            # abi.Kv8AppendArgs
+_KV8_EVICT = struct.Struct("@PPPPiiiiPiiPPPPPPiiii0P")                # abi.Kv8EvictArgs
+_KV8_ACCEPT = struct.Struct("@PPPPiiiiPiiPPPPPPPPPPPiii0P")            # abi.Kv8AcceptArgs
+for _packer, _struct in ((_KV8_CACHE, abi.Kv8Cache), (_ATTENTION_TREE, abi.AttentionTreeArgs), (_KV8_APPEND, abi.Kv8AppendArgs), (_KV8_EVICT, abi.Kv8EvictArgs), (_KV8_ACCEPT, abi.Kv8AcceptArgs)):
+    assert _packer.size == C.sizeof(_struct)
 
 
 @functools.cache
@@ -409,31 +415,31 @@ def _tree_calls():
         f = load_library()[name]
         f.restype, f.argtypes = restype, list(argtypes)
         return f
-    return (fn("tenzo_cuda_kv8_append", _PB, _PI, _PP, _PP, _PI, _PP, _PP, _PI, _PP, _PP, _PP, _PI, _PP, _PP, _PI, _PP),
-            fn("tenzo_cuda_kv8_evict", _PB, _PP, _PP, _PP, _PP, _PP, _PI, _PI, _PI, _PP, _PI, _PP),
-            fn("tenzo_cuda_kv8_accept", _PB, _PP, _PP, _PP, _PP, _PP, _PP, _PI, _PI, _PP, _PP, _PP, _PP, _PP, _PI, _PP),
+    return (fn("tenzo_cuda_kv8_append", _PB, _PP), fn("tenzo_cuda_kv8_evict", _PB, _PP), fn("tenzo_cuda_kv8_accept", _PB, _PP),
             fn("tenzo_cuda_attention_tree", _PB, _PP), fn("tenzo_cuda_kv8_weigh", _PB, _PP, _PP),
             fn("tenzo_cuda_attention_tree_workspace_bytes", _PI, _PI, _PI, _PI, _PI, restype=C.c_size_t))
 
 
 def _kv8_cache(cache: Kv8Cache, device: int):
-    """The fields of abi.Kv8Cache."""
+    """The fields of abi.Kv8Cache, and the shape of the scales."""
     k, v, sk, sv, table = cache
-    shape, scales, rows = k.shape, sk.shape, table.shape
-    if len(shape) != 5 or shape[4] != 128 or v.shape != shape or scales != shape[:4] or sv.shape != scales or len(rows) != 2:
-        raise ValueError(f"caches [blocks, layers, kv heads, slots, 128], their scales and a table [rows, columns] are needed, not {tuple(shape)}, {tuple(v.shape)}, "
-                         f"{tuple(sk.shape)}, {tuple(sv.shape)} and {tuple(rows)}")
-    blocks, layers, n_kv, slots, _ = shape
-    return (_arg(k, torch.int8, device, "k"), _arg(v, torch.int8, device, "v"), _arg(sk, torch.float32, device, "scale_k"), _arg(sv, torch.float32, device, "scale_v"),
-            blocks, layers, n_kv, slots, _arg(table, torch.int32, device, "block_table"), *rows)
+    shape, rows = k.shape, table.shape
+    if len(shape) == 5 and len(rows) == 2:
+        blocks, layers, n_kv, slots, dims = shape
+        scales = (blocks, layers, n_kv, slots)
+        if dims == 128 and v.shape == shape and sk.shape == scales and sv.shape == scales:
+            return (_arg(k, _I8, device, "k"), _arg(v, _I8, device, "v"), _arg(sk, _F32, device, "scale_k"), _arg(sv, _F32, device, "scale_v"),
+                    blocks, layers, n_kv, slots, _arg(table, _I32, device, "block_table"), *rows), scales
+    raise ValueError(f"caches [blocks, layers, kv heads, slots, 128], their scales and a table [rows, columns] are needed, not {tuple(shape)}, {tuple(v.shape)}, "
+                     f"{tuple(sk.shape)}, {tuple(sv.shape)} and {tuple(rows)}")
 
 
-def _arg_beside(t, cache: Kv8Cache, dtype, device: int, what: str) -> int:
+def _arg_beside(t, scales: tuple, dtype, device: int, what: str) -> int:
     """Address of what lies beside the scales; 0 for None."""
     if t is None:
         return 0
-    if t.shape != cache[2].shape:
-        raise ValueError(f"{what} has the scales' shape {tuple(cache.scale_k.shape)}, not {tuple(t.shape)}")
+    if t.shape != scales:
+        raise ValueError(f"{what} has the scales' shape {scales}, not {tuple(t.shape)}")
     return _arg(t, dtype, device, what)
 
 
@@ -449,15 +455,15 @@ def kv8_append(k, v, cache, place, *, layer, seq=None, rope_pos=None, rope_cos=N
     sequences seq int32 [n] (default: row i is sequence i). A negative place marks a padding row, for which nothing is stored. weight fp32 and position int32, of the
     scales' shape, receive 0 and the rotary position."""
     dev = _current_device()
-    fields = _kv8_cache(cache, dev)
+    fields, scales = _kv8_cache(cache, dev)
     n_kv = fields[6]
     (kp, ks, n), (vp, vs, m) = _arg_rows(k, dev, n_kv * 128, "k"), _arg_rows(v, dev, n_kv * 128, "v")
     if n != m or (ks != vs and n > 1):
         raise ValueError("k and v have the same number of rows, equally far apart")
     cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
-    _ok(_tree_calls()[0](_KV8_CACHE.pack(*fields), _arg_layer(layer), kp, vp, ks, _arg_entries(place, n, dev, "place"), _arg_entries(seq, n, dev, "seq"), n,
-                         _arg_entries(rope_pos, n, dev, "rope_pos"), cos, sin, length, _arg_beside(weight, cache, torch.float32, dev, "weight"),
-                         _arg_beside(position, cache, torch.int32, dev, "position"), use_pdl, _raw_stream(dev)), "tenzo_cuda_kv8_append")
+    args = _KV8_APPEND.pack(*fields, kp, vp, _arg_entries(place, n, dev, "place"), _arg_entries(seq, n, dev, "seq"), _arg_entries(rope_pos, n, dev, "rope_pos"), cos, sin,
+                            _arg_beside(weight, scales, _F32, dev, "weight"), _arg_beside(position, scales, _I32, dev, "position"), _arg_layer(layer), ks, n, length, use_pdl)
+    _ok(_tree_calls()[0](args, _raw_stream(dev)), "tenzo_cuda_kv8_append")
 
 
 @functools.lru_cache(1024)
@@ -466,8 +472,8 @@ def attention_tree_workspace_bytes(sequences, nodes, n_q, n_kv, shares=0) -> int
 
 
 def _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev):
-    """The fields of abi.AttentionTreeArgs from cache to max_len, and what the calls ask further: the query's address and the number of rows."""
-    fields = _kv8_cache(cache, dev)
+    """The fields of abi.AttentionTreeArgs from cache to max_len, and what the calls ask further: the query's address, the numbers of rows and sequences, and the scales' shape."""
+    fields, scales = _kv8_cache(cache, dev)
     qp, q_stride, rows = _arg_rows(q, dev, n_q * 128, "q")
     sequences = rows // nodes if nodes > 0 else -1
     if sequences * nodes != rows:
@@ -480,8 +486,8 @@ def _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos,
     cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
     if max_len is None:
         max_len = min(fields[7] * fields[10], _INT_MOST)
-    return qp, rows, sequences, (*fields, _arg_entries(start, sequences, dev, "start"), _arg_entries(count, sequences, dev, "count"), _arg_entries(seq, sequences, dev, "seq"),
-                                 _arg(mask, torch.int32, dev, "mask"), _arg_entries(rope_pos, rows, dev, "rope_pos"), cos, sin, length, q_stride, mask_stride,
+    return qp, rows, sequences, scales, (*fields, _arg_entries(start, sequences, dev, "start"), _arg_entries(count, sequences, dev, "count"), _arg_entries(seq, sequences, dev, "seq"),
+                                 _arg(mask, _I32, dev, "mask"), _arg_entries(rope_pos, rows, dev, "rope_pos"), cos, sin, length, q_stride, mask_stride,
                                  _arg_layer(layer), n_q, sequences, nodes, _arg_int(max_len, "max_len"))
 
 
@@ -492,28 +498,30 @@ def attention_tree(q, cache, start, *, layer, n_q, nodes, count=None, mask=None,
     that are there (default: all); rope_pos int32 [rows]: the queries' rotary positions (default: start + i). Returns out [rows, n_q*128], zeros where nothing is seen;
     with want_lse (out, lse [rows, n_q])."""
     dev = _current_device()
-    qp, rows, sequences, fields = _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev)
+    qp, rows, sequences, _, fields = _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         op = out.data_ptr()
     elif out.shape != (rows, n_q * 128):
         raise ValueError(f"out is [{rows}, {n_q * 128}]")
     else:
-        op = _arg(out, torch.float32, dev, "out")
+        op = _arg(out, _F32, dev, "out")
     lp = 0
     if lse is not None:
         if lse.shape != (rows, n_q):
             raise ValueError(f"lse is [{rows}, {n_q}]")
-        lp = _arg(lse, torch.float32, dev, "lse")
+        lp = _arg(lse, _F32, dev, "lse")
     elif want_lse:
         lse = q.new_empty(rows, n_q)
         lp = lse.data_ptr()
-    if workspace is None:
+    if workspace is None and shares == 0 and fields[-1] <= _TREE_WHOLE:
+        wp = size = 0
+    elif workspace is None:
         size = attention_tree_workspace_bytes(sequences, nodes, n_q, fields[6], shares)
         workspace = q.new_empty(-(-size // 4))
         wp = workspace.data_ptr()
     else:
-        wp, size = _arg(workspace, torch.uint8, dev, "workspace"), workspace.numel()
+        wp, size = _arg(workspace, _U8, dev, "workspace"), workspace.numel()
     args = _ATTENTION_TREE.pack(qp, op, lp, *fields, _arg_int(shares, "shares"), use_pdl, wp, size)
     _ok(_tree_calls()[3](args, _raw_stream(dev)), "tenzo_cuda_attention_tree")
     return out if lse is None else (out, lse)
@@ -523,24 +531,25 @@ def kv8_weigh(q, lse, cache, weight, start, *, layer, n_q, nodes, count=None, ma
     """Adds to weight (fp32, of the scales' shape) what each cached token received in attention_tree of the same arguments, whose lse [rows, n_q] this reads: the sum of
     softmax's results over the nodes and the query heads of a kv head."""
     dev = _current_device()
-    qp, rows, _, fields = _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev)
+    qp, rows, _, scales, fields = _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev)
     if lse.shape != (rows, n_q):
         raise ValueError(f"lse is [{rows}, {n_q}], not {tuple(lse.shape)}")
-    args = _ATTENTION_TREE.pack(qp, 0, _arg(lse, torch.float32, dev, "lse"), *fields, 0, use_pdl, 0, 0)
-    _ok(_tree_calls()[4](args, _arg_beside(weight, cache, torch.float32, dev, "weight"), _raw_stream(dev)), "tenzo_cuda_kv8_weigh")
+    args = _ATTENTION_TREE.pack(qp, 0, _arg(lse, _F32, dev, "lse"), *fields, 0, use_pdl, 0, 0)
+    _ok(_tree_calls()[4](args, _arg_beside(weight, scales, _F32, dev, "weight"), _raw_stream(dev)), "tenzo_cuda_kv8_weigh")
 
 
 def kv8_evict(cache, weight, position, length, *, keep, protect_from=None, seq=None, max_len=None, use_pdl=False):
     """Cuts the sequences that hold length int32 [sequences] tokens back to `keep`, in all layers and for each kv head on its own: the tokens of least weight go, but
     none whose position is protect_from[s] int32 [sequences] or more; those behind place keep - 1 that stay move to the places that became free. Returns the new lengths."""
     dev, sequences = _current_device(), len(length)
-    fields = _kv8_cache(cache, dev)
+    fields, scales = _kv8_cache(cache, dev)
     if max_len is None:
         max_len = min(fields[7] * fields[10], 1 << 20)
     out = torch.empty_like(length)
-    _ok(_tree_calls()[1](_KV8_CACHE.pack(*fields), _arg_beside(weight, cache, torch.float32, dev, "weight"), _arg_beside(position, cache, torch.int32, dev, "position"),
-                         _arg_entries(length, sequences, dev, "length"), _arg_entries(seq, sequences, dev, "seq"), _arg_entries(protect_from, sequences, dev, "protect_from"),
-                         sequences, _arg_int(keep, "keep"), _arg_int(max_len, "max_len"), out.data_ptr(), use_pdl, _raw_stream(dev)), "tenzo_cuda_kv8_evict")
+    args = _KV8_EVICT.pack(*fields, _arg_beside(weight, scales, _F32, dev, "weight"), _arg_beside(position, scales, _I32, dev, "position"),
+                           _arg_entries(length, sequences, dev, "length"), _arg_entries(seq, sequences, dev, "seq"), _arg_entries(protect_from, sequences, dev, "protect_from"),
+                           out.data_ptr(), sequences, _arg_int(keep, "keep"), _arg_int(max_len, "max_len"), use_pdl)
+    _ok(_tree_calls()[1](args, _raw_stream(dev)), "tenzo_cuda_kv8_evict")
     return out
 
 
@@ -552,13 +561,13 @@ def kv8_accept(cache, token, parent, chosen, start, *, count=None, seq=None, wei
     if len(shape) != 2 or parent.shape != shape or chosen.shape != shape:
         raise ValueError(f"token, parent and chosen are [sequences, nodes], not {tuple(shape)}, {tuple(parent.shape)} and {tuple(chosen.shape)}")
     sequences, nodes = shape
-    fields = _kv8_cache(cache, dev)
-    tokens = _arg(token, torch.int32, dev, "token")
+    fields, scales = _kv8_cache(cache, dev)
+    tokens = _arg(token, _I32, dev, "token")
     accepted, following, path = token.new_empty(sequences), token.new_empty(sequences), torch.empty_like(token)
-    _ok(_tree_calls()[2](_KV8_CACHE.pack(*fields), tokens, _arg(parent, torch.int32, dev, "parent"), _arg(chosen, torch.int32, dev, "chosen"),
-                         _arg_entries(start, sequences, dev, "start"), _arg_entries(count, sequences, dev, "count"), _arg_entries(seq, sequences, dev, "seq"), sequences, nodes,
-                         accepted.data_ptr(), following.data_ptr(), path.data_ptr(), _arg_beside(weight, cache, torch.float32, dev, "weight"),
-                         _arg_beside(position, cache, torch.int32, dev, "position"), use_pdl, _raw_stream(dev)), "tenzo_cuda_kv8_accept")
+    args = _KV8_ACCEPT.pack(*fields, tokens, _arg(parent, _I32, dev, "parent"), _arg(chosen, _I32, dev, "chosen"), _arg_entries(start, sequences, dev, "start"),
+                            _arg_entries(count, sequences, dev, "count"), _arg_entries(seq, sequences, dev, "seq"), accepted.data_ptr(), following.data_ptr(), path.data_ptr(),
+                            _arg_beside(weight, scales, _F32, dev, "weight"), _arg_beside(position, scales, _I32, dev, "position"), sequences, nodes, use_pdl)
+    _ok(_tree_calls()[2](args, _raw_stream(dev)), "tenzo_cuda_kv8_accept")
     return accepted, following, path
 
 

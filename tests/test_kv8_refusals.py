@@ -28,21 +28,22 @@ def tree(**over):
     return a
 
 
+def call(name, cls, c, a):
+    if c is None:
+        return getattr(load_library(), name)(None, None)
+    return getattr(load_library(), name)(C.byref(cls(cache=c, **a)), None)
+
+
 def append(lib, c, **over):
-    a = dict(layer=0, k=P, v=P, stride=384, place=P, seq=P, rows=4, rope_pos=None, cos=None, sin=None, length=0) | over
-    return lib.tenzo_cuda_kv8_append(c and C.byref(c), a["layer"], a["k"], a["v"], a["stride"], a["place"], a["seq"], a["rows"], a["rope_pos"], a["cos"], a["sin"], a["length"], P, P, 0,
-                                     None)
+    return call("tenzo_cuda_kv8_append", abi.Kv8AppendArgs, c, dict(layer=0, k=P, v=P, kv_stride=384, place=P, seq=P, rows=4, weight=P, position=P) | over)
 
 
 def evict(lib, c, **over):
-    a = dict(weight=P, position=P, length=P, seq=P, sequences=4, keep=8, max_len=80, out=P + 64) | over
-    return lib.tenzo_cuda_kv8_evict(c and C.byref(c), a["weight"], a["position"], a["length"], a["seq"], None, a["sequences"], a["keep"], a["max_len"], a["out"], 0, None)
+    return call("tenzo_cuda_kv8_evict", abi.Kv8EvictArgs, c, dict(weight=P, position=P, length=P, seq=P, sequences=4, keep=8, max_len=80, length_out=P + 64) | over)
 
 
 def accept(lib, c, **over):
-    a = dict(token=P, parent=P, chosen=P, start=P, seq=P, sequences=4, nodes=7, accepted=P, next=P, path=P) | over
-    return lib.tenzo_cuda_kv8_accept(c and C.byref(c), a["token"], a["parent"], a["chosen"], a["start"], None, a["seq"], a["sequences"], a["nodes"], a["accepted"], a["next"], a["path"],
-                                     None, None, 0, None)
+    return call("tenzo_cuda_kv8_accept", abi.Kv8AcceptArgs, c, dict(token=P, parent=P, chosen=P, start=P, seq=P, sequences=4, nodes=7, accepted=P, next=P, path=P) | over)
 
 
 BAD_CACHES = [dict(k=None), dict(v=None), dict(scale_k=None), dict(scale_v=None), dict(k=P + 8), dict(v=P + 4), dict(scale_k=P + 4), dict(scale_v=P + 8), dict(block_table=None),
@@ -62,8 +63,8 @@ def test_null(lib):
     assert append(lib, None) == evict(lib, None) == accept(lib, None) == lib.tenzo_cuda_attention_tree(None, None) == lib.tenzo_cuda_kv8_weigh(None, P, None) == abi.ERR_INVALID
 
 
-@pytest.mark.parametrize("over", [dict(layer=-1), dict(layer=2), dict(k=None), dict(v=None), dict(stride=383), dict(place=None), dict(rows=-1), dict(seq=None, rows=5), dict(cos=P),
-                                  dict(sin=P), dict(cos=P, sin=P, length=0), dict(cos=P + 4, sin=P, length=9), dict(cos=P, sin=P + 8, length=9)], ids=str)
+@pytest.mark.parametrize("over", [dict(layer=-1), dict(layer=2), dict(k=None), dict(v=None), dict(kv_stride=383), dict(place=None), dict(rows=-1), dict(seq=None, rows=5), dict(rope_cos=P),
+                                  dict(rope_sin=P), dict(rope_cos=P, rope_sin=P, rope_len=0), dict(rope_cos=P + 4, rope_sin=P, rope_len=9), dict(rope_cos=P, rope_sin=P + 8, rope_len=9)], ids=str)
 def test_append(lib, over):
     assert append(lib, cache(), **over) == abi.ERR_INVALID
 
@@ -106,7 +107,7 @@ def test_workspace(lib):
     assert need(2, 1, 4, 2, 10) == 32 + 10 * 2 * 16 * 520                       # 2 * 2 words, and two sets of sixteen rows a share
 
 
-@pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(weight=P + 4), -1), (dict(position=P + 8), -1), (dict(length=None), -1), (dict(out=None), -1), (dict(out=P), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
+@pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(weight=P + 4), -1), (dict(position=P + 8), -1), (dict(length=None), -1), (dict(length_out=None), -1), (dict(length_out=P), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
                                        (dict(max_len=0), -1), (dict(max_len=81), -1), (dict(sequences=-1), -1), (dict(seq=None, sequences=5), -1), (dict(sequences=65536), -5)], ids=str)
 def test_evict(lib, over, code):
     assert evict(lib, cache(), **over) == code
@@ -138,7 +139,8 @@ def _flat(o):
     return [x for n, t in o._fields_ for x in (_flat(getattr(o, n)) if issubclass(t, C.Structure) else [getattr(o, n)])]
 
 
-@pytest.mark.parametrize("cls,packer", [(abi.Kv8Cache, kernels._KV8_CACHE), (abi.AttentionTreeArgs, kernels._ATTENTION_TREE)], ids=lambda x: getattr(x, "__name__", ""))
+@pytest.mark.parametrize("cls,packer", [(abi.Kv8Cache, kernels._KV8_CACHE), (abi.AttentionTreeArgs, kernels._ATTENTION_TREE), (abi.Kv8AppendArgs, kernels._KV8_APPEND),
+                                        (abi.Kv8EvictArgs, kernels._KV8_EVICT), (abi.Kv8AcceptArgs, kernels._KV8_ACCEPT)], ids=lambda x: getattr(x, "__name__", ""))
 def test_packed_arguments_are_the_struct(cls, packer):
     values = [1000 + i for i in range(len(_leaves(cls)))]
     assert _flat(cls.from_buffer_copy(packer.pack(*values))) == values
