@@ -1,7 +1,7 @@
 // Attention of drafted trees over the INT8 caches (kv8.cuh), and the weight that each cached token receives.
 //
 //   * All query vectors of a kv head (nodes x heads of the group) read the same keys, so both products are matrix products with the keys, then the dims, as rows of 128 and
-//     the queries as columns: S^T = K Q^T and O^T = V^T P^T. A CTA takes 16, 32 or 64 of the queries and walks its keys in tiles of 128. With keys as rows a single
+//     the queries as columns: S^T = K Q^T and O^T = V^T P^T. A CTA takes 16, 32, 48 or 64 of the queries and walks its keys in tiles of 128. With keys as rows a single
 //     query fills the tensor cores as well as many do, and one kernel serves a decode step and a tree of 64 nodes.
 //   * Both are products of whole numbers (tcgen05 kind::i8, sums of 32 bits), and the codes of the cache are operands as they lie: K and V tiles go from memory to shared
 //     memory to the tensor cores, nothing is unpacked or converted. A query is scaled to a maximum of 2^21 to 2^22 and rounded; its three signed bytes are three columns. A weight, p * scale of its
@@ -10,6 +10,10 @@
 //   * softmax: a thread has one key and sixteen queries, so a row's maximum goes across lanes; and accumulators of whole numbers cannot be scaled down.
 //     Both are avoided: a row's weights are taken relative to a reference, the maximum when it was last set, and may grow to 2^5 of it. Only where a weight would pass that (one vote a
 //     tile; the first tile always) the references are set anew and the accumulators moved on into fp32.
+//   * Bound: single tokens by the bytes (64 sequences of 8192 keys, 20 heads over 5: 118 us on the device, 106 at the memory's measured rate), trees by the instructions of the warps that make
+//     weights, some 415 for 32 keys and sixteen queries (16 trees of 64 nodes, 8192 keys: 227 us, 2600 cycles a tile of 64 queries, 64 % of the issue slots; tensor cores 32 %, memory 10 %); small
+//     calls by the chain share, queries, tile, outputs, join (8 nodes, 1000 keys: 13.4 us). Going on to the next pair takes some 9000 cycles, 4300 of them 64 queries'.
+//     The same 64 queries as one line of 64, whose products wait for all warps, took 282 us, plain fp32 instead of packed pairs 248.
 #include "attn_common.cuh"
 #include "kv8.cuh"
 #include "umma.cuh"
@@ -243,7 +247,8 @@ struct TreeWalk {
 // R queries of a block on their way to the operand, four by each of its R / 4 warps. A lane has dims 4 lane .. 4 lane + 3, and the lane sixteen on, or back, those that they are turned
 // with. A vector is turned, scaled by a power of two to a maximum between 2^21 and 2^22 and rounded; its signed bytes are rows r, LINE + r, 2 LINE + r of its line's operand (128 bytes each, swizzled).
 // s_f: what a unit of the products with the codes counts in the argument of 2^x (NaN for a query that is not finite). from[r]: the vector in q, -1: none, zeros.
-// (Every load is made, of something, without a branch around it: where two ways meet the compiler copies what was loaded, and so waits for it. 3500 cycles for a block's loads that way, 900 this.)
+// (Every load is made, of something, without a branch around it: where two ways meet the compiler copies what was loaded, and so waits for it. Bytes cut off one after another, by shifts, made the
+// weights of 4 x 250 nodes, which are mostly this, 178 us; like this 168.)
 template <int R, int LINE, bool VEC>
 __device__ __forceinline__ void tr_queries(const TreeLaunch& L, const long long* from, const int* pos, unsigned char* s_q, float* s_f) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
