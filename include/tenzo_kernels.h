@@ -385,7 +385,7 @@ TENZO_API int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* str
  * of range leaves its block's keys out and raises it. */
 typedef struct {
     const float* q;          /* [sequences*nodes][q_stride], n_q*128 used, before rotation */
-    float* out;              /* [sequences*nodes][n_q*128] */
+    float* out;              /* [sequences*nodes][n_q*128], 16-byte aligned, apart from q */
     float* lse;              /* [sequences*nodes][n_q], or NULL */
     tenzo_kv8_cache cache;
     const int* start;        /* [sequences] device */
@@ -397,11 +397,12 @@ typedef struct {
     int rope_len;
     int q_stride;            /* floats between rows; 0 = n_q*128 */
     int mask_stride;         /* words between rows; 0 = ceil(nodes / 32) */
-    int layer, n_q, sequences, nodes;
+    int layer, n_q, sequences, nodes;    /* n_q at most 2^17, n_kv at most 65535 (-5) */
     int max_len;             /* upper bound on start + count; at most slots * table_stride, and 2^30 (-5) */
     int shares;              /* equal shares that the keys of all sequences and kv heads are cut into, each of one CTA (or some, for many queries); 0 = choose, at most 65535 */
     int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
-    void* workspace;         /* 16-byte aligned, contents need not be kept: partial results where a cut goes through a sequence's keys */
+    void* workspace;         /* 16-byte aligned, contents need not be kept, of one call at a time (two graphs that may run together have two): partial results where a
+                                cut goes through a sequence's keys */
     size_t workspace_bytes;  /* tenzo_cuda_attention_tree_workspace_bytes(...), some MB whatever the lengths are. With less, or NULL, shares end with a sequence's kv head, which is
                                 slower for few sequences and for unequal ones; shares > 0 is refused then (-1). With
                                 shares = 0 it is not used where max_len <= 512 */
@@ -447,7 +448,7 @@ typedef struct {
     const int* token; const int* parent; const int* chosen;   /* [sequences][nodes] device */
     const int* start;                               /* [sequences] device */
     const int* count; const int* seq;               /* [sequences] device, or NULL */
-    int* accepted; int* next; int* path;            /* device: [sequences], [sequences], [sequences][nodes] */
+    int* accepted; int* next; int* path;            /* device: [sequences], [sequences], [sequences][nodes], in memory of their own */
     float* weight; int* position;                   /* or NULL */
     int sequences, nodes;
     int use_pdl;

@@ -1174,6 +1174,11 @@ extern "C" int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, 
     if (a.sequences == 0) return 0;
     if (int rc = tree_check(L)) return rc;
     if (!a.out || !kv8_aligned(a.out, 16) || a.shares < 0 || a.shares > 65535) return -1;
+    {                                                    // (a query is read by every CTA that has some of its keys)
+        const size_t row = (size_t)a.n_q * kK8Hd, rows = (size_t)a.sequences * a.nodes;
+        const uintptr_t q0 = reinterpret_cast<uintptr_t>(a.q), q1 = q0 + ((rows - 1) * a.q_stride + row) * sizeof(float), o0 = reinterpret_cast<uintptr_t>(a.out), o1 = o0 + rows * row * sizeof(float);
+        if (q0 < o1 && o0 < q1) return -1;
+    }
     tree_plan(L);
     L.cut = a.workspace && kv8_aligned(a.workspace, 16) && a.workspace_bytes >= tree_room(L);
     if (a.shares > 0 && !L.cut) return -1;

@@ -495,6 +495,9 @@ extern "C" int tenzo_cuda_kv8_accept(const tenzo_kv8_accept_args* args, void* st
     if (!kv8_cache_ok(a.cache) || a.sequences < 0) return -1;
     if (a.sequences == 0) return 0;
     if (!a.token || !a.parent || !a.chosen || !a.start || !a.accepted || !a.next || !a.path || a.nodes <= 0 || (!a.seq && a.sequences > a.cache.table_rows)) return -1;
+    const int* const written[3] = {a.accepted, a.next, a.path};
+    for (const int* to : written)                                    // (what other CTAs of the sequence still read)
+        if (to == a.token || to == a.parent || to == a.chosen || to == a.start || to == a.count || to == a.seq) return -1;
     if (a.nodes > TENZO_TREE_MOST || a.sequences > 65535) return -5;
     const long long units = (long long)a.cache.n_layers * a.cache.n_kv, share = (units * a.sequences + 148 * 8 - 1) / (148 * 8);
     const int many = (int)(share < units ? share : units);           // (layer, kv head) pairs a CTA takes
@@ -508,7 +511,8 @@ extern "C" int tenzo_cuda_kv8_evict(const tenzo_kv8_evict_args* args, void* stre
     const tenzo_kv8_evict_args& a = *args;
     if (!kv8_cache_ok(a.cache) || a.sequences < 0) return -1;
     if (a.sequences == 0) return 0;
-    if (!a.weight || !a.position || !kv8_aligned(a.weight, 16) || !kv8_aligned(a.position, 16) || !a.length || !a.length_out || a.length_out == a.length) return -1;
+    if (!a.weight || !a.position || !kv8_aligned(a.weight, 16) || !kv8_aligned(a.position, 16) || !a.length || !a.length_out) return -1;
+    if (a.length_out == a.length || a.length_out == a.seq || a.length_out == a.protect_from) return -1;      // (which other CTAs still read)
     if (a.keep <= 0 || a.max_len <= 0 || a.max_len > kv8_places(a.cache) || (!a.seq && a.sequences > a.cache.table_rows)) return -1;
     if (a.sequences > 65535 || a.max_len > kEvMost) return -5;
     const bool held = a.max_len <= kEvHeld;

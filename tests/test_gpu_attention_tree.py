@@ -109,6 +109,7 @@ CASES = [
     ([30, -1, 40], [3, 3, 2], 3, 64, 1, {}),
     ([64], [64], 64, 3, 1, dict(scale=8.0)),
     ([4000], [2], 2, 20, 5, dict(scale=0.01)),
+    ([40], [256], 256, 32, 1, {}),                                            # 8192 queries of one kv head
 ]
 
 
@@ -248,8 +249,54 @@ def test_table_rows_and_strided_queries(cuda_lib):
     order = [2, 0, 1]
     back = np.argsort(order)
     shuffled = kernels.Kv8Cache(*cache[:4], cache.block_table[torch.tensor(back, device="cuda")].contiguous())
-    out, lse = kernels.attention_tree(wide[:, 3: 3 + 2560], shuffled, start, seq=dev(np.array(order, np.int32)), want_lse=True, **a)
-    case.check(out, lse)
+    seq = dev(np.array(order, np.int32))
+    out, lse = kernels.attention_tree(wide[:, 3: 3 + 2560], shuffled, start, seq=seq, want_lse=True, **a)
+    want = case.want()
+    case.check(out, lse, want)
+    check_weights(case, wide[:, 3: 3 + 2560], lse, shuffled, start, a | dict(seq=seq), want)
+
+
+@pytest.mark.parametrize("starts,counts,nodes", [([100, 7], [12, 9], 12), ([1500, 900], [1, 1], 1)])
+def test_positions_by_default(cuda_lib, starts, counts, nodes):
+    """Without rope_pos a node's position is its place."""
+    from tenzo_b200 import kernels
+    case = Case(nodes, starts, counts, nodes, 20, 5)
+    case.pos = (np.array(starts)[:, None] + np.arange(nodes)).astype(np.int32).flatten()
+    cache, start, a = case.arguments()
+    del a["rope_pos"]
+    q = dev(case.q)
+    out, lse = kernels.attention_tree(q, cache, start, want_lse=True, **a)
+    want = case.want()
+    case.check(out, lse, want)
+    check_weights(case, q, lse, cache, start, a, want)
+
+
+def test_one_table_row_for_several_sequences(cuda_lib):
+    """Drafts of one sequence that end at different tokens, and a table whose rows share blocks: attention reads what others read too."""
+    from tenzo_b200 import kernels
+    case = Case(17, [300, 300, 300], [6, 6, 6], 6, 20, 5)
+    cache, start, a = case.arguments()
+    q = dev(case.q)
+    table = cache.block_table.clone()
+    table[1] = table[2] = table[0]
+    seq = torch.zeros(3, dtype=torch.int32, device="cuda")
+    got = [kernels.attention_tree(q, kernels.Kv8Cache(*cache[:4], t), start, seq=s, want_lse=True, **a) for t, s in ((table, None), (cache.block_table, seq))]
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    case.c.table[1] = case.c.table[2] = case.c.table[0]
+    case.check(*got[0])
+
+
+def test_nothing_to_do(cuda_lib):
+    from tenzo_b200 import kernels
+    case = Case(19, [20], [4], 4, 20, 5)
+    cache, start, a = case.arguments()
+    none = {n: x[:0] if n in ("count", "mask", "rope_pos") else x for n, x in a.items()}
+    out, lse = kernels.attention_tree(dev(case.q)[:0], cache, start[:0], want_lse=True, **none)
+    assert out.shape == (0, 2560) and lse.shape == (0, 20)
+    kernels.kv8_weigh(dev(case.q)[:0], lse, cache, dev(case.c.weight), start[:0], **none)
+    with pytest.raises(RuntimeError):
+        q = dev(case.q)
+        kernels.attention_tree(q, cache, start, out=q, **a)
 
 
 def test_out_of_range(cuda_lib):

@@ -22,7 +22,7 @@ def cache(**over):
 
 
 def tree(**over):
-    a = abi.AttentionTreeArgs(q=P, out=P, lse=P, cache=cache(), start=P, layer=0, n_q=6, sequences=4, nodes=7, max_len=80)
+    a = abi.AttentionTreeArgs(q=P, out=P + (1 << 20), lse=P, cache=cache(), start=P, layer=0, n_q=6, sequences=4, nodes=7, max_len=80)
     for k, v in over.items():
         setattr(a, k, v)
     return a
@@ -43,7 +43,7 @@ def evict(lib, c, **over):
 
 
 def accept(lib, c, **over):
-    return call("tenzo_cuda_kv8_accept", abi.Kv8AcceptArgs, c, dict(token=P, parent=P, chosen=P, start=P, seq=P, sequences=4, nodes=7, accepted=P, next=P, path=P) | over)
+    return call("tenzo_cuda_kv8_accept", abi.Kv8AcceptArgs, c, dict(token=P, parent=P, chosen=P, start=P, seq=P, sequences=4, nodes=7, accepted=P + 64, next=P + 128, path=P + 256) | over)
 
 
 BAD_CACHES = [dict(k=None), dict(v=None), dict(scale_k=None), dict(scale_v=None), dict(k=P + 8), dict(v=P + 4), dict(scale_k=P + 4), dict(scale_v=P + 8), dict(block_table=None),
@@ -81,7 +81,7 @@ def test_tree_and_weigh(lib, over):
     assert lib.tenzo_cuda_kv8_weigh(C.byref(a), P, None) == abi.ERR_INVALID
 
 
-@pytest.mark.parametrize("over", [dict(out=None), dict(out=P + 4), dict(shares=-1), dict(shares=65536), dict(shares=3), dict(shares=3, workspace=P + 8, workspace_bytes=1 << 30),
+@pytest.mark.parametrize("over", [dict(out=None), dict(out=P + (1 << 20) + 4), dict(out=P), dict(out=P + 27 * 768 * 4), dict(out=P, q=P + 27 * 768 * 4), dict(out=P + (27 * 800 + 764) * 4, q=P, q_stride=800), dict(shares=-1), dict(shares=65536), dict(shares=3), dict(shares=3, workspace=P + 8, workspace_bytes=1 << 30),
                                   dict(shares=3, workspace=P, workspace_bytes=100)], ids=str)
 def test_tree_alone(lib, over):
     assert lib.tenzo_cuda_attention_tree(C.byref(tree(**over)), None) == abi.ERR_INVALID
@@ -107,7 +107,7 @@ def test_workspace(lib):
     assert need(2, 1, 4, 2, 10) == 32 + 10 * 2 * 16 * 520                       # 2 * 2 words, and two sets of sixteen rows a share
 
 
-@pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(weight=P + 4), -1), (dict(position=P + 8), -1), (dict(length=None), -1), (dict(length_out=None), -1), (dict(length_out=P), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
+@pytest.mark.parametrize("over,code", [(dict(weight=None), -1), (dict(position=None), -1), (dict(weight=P + 4), -1), (dict(position=P + 8), -1), (dict(length=None), -1), (dict(length_out=None), -1), (dict(length_out=P), -1), (dict(length_out=P + 128, seq=P + 128), -1), (dict(length_out=P + 128, protect_from=P + 128), -1), (dict(keep=0), -1), (dict(keep=-3), -1),
                                        (dict(max_len=0), -1), (dict(max_len=81), -1), (dict(sequences=-1), -1), (dict(seq=None, sequences=5), -1), (dict(sequences=65536), -5)], ids=str)
 def test_evict(lib, over, code):
     assert evict(lib, cache(), **over) == code
@@ -119,7 +119,7 @@ def test_evict_too_long(lib):
 
 
 @pytest.mark.parametrize("over,code", [(dict(token=None), -1), (dict(parent=None), -1), (dict(chosen=None), -1), (dict(start=None), -1), (dict(accepted=None), -1), (dict(next=None), -1),
-                                       (dict(path=None), -1), (dict(nodes=0), -1), (dict(sequences=-1), -1), (dict(seq=None, sequences=5), -1), (dict(sequences=65536), -5)], ids=str)
+                                       (dict(path=None), -1), (dict(accepted=P), -1), (dict(next=P), -1), (dict(path=P), -1), (dict(count=P + 64), -1), (dict(nodes=0), -1), (dict(sequences=-1), -1), (dict(seq=None, sequences=5), -1), (dict(sequences=65536), -5)], ids=str)
 def test_accept(lib, over, code):
     assert accept(lib, cache(), **over) == code
 
