@@ -256,9 +256,10 @@ def _arg_entries(t, n: int, device: int, what: str) -> int:
 def _arg_rope(cos, sin, device: int) -> tuple[int, int, int]:
     if cos is None and sin is None:
         return 0, 0, 0
-    if cos is None or sin is None or cos.dim() != 2 or cos.shape[1] != 64 or sin.shape != cos.shape:
+    shape = None if cos is None or sin is None else cos.shape
+    if shape is None or len(shape) != 2 or shape[1] != 64 or sin.shape != shape:
         raise ValueError("rope_cos and rope_sin are tables of the same number of rows of 64")
-    return _arg(cos, torch.float32, device, "rope_cos"), _arg(sin, torch.float32, device, "rope_sin"), cos.shape[0]
+    return _arg(cos, torch.float32, device, "rope_cos"), _arg(sin, torch.float32, device, "rope_sin"), shape[0]
 
 
 def kv4_append(k, v, pool, pos, *, layer, block_table, seq=None, rope_cos=None, rope_sin=None, use_pdl=False):
@@ -480,9 +481,10 @@ def _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos,
         raise ValueError(f"{rows} rows of q are no trees of {nodes} nodes")
     mask_stride = 0
     if mask is not None:
-        if mask.dim() != 2 or mask.shape[0] != rows or mask.shape[1] * 32 < nodes:
-            raise ValueError(f"mask has a row of at least {-(-nodes // 32)} words for each of {rows} nodes, not {tuple(mask.shape)}")
-        mask_stride = mask.shape[1]
+        shape = mask.shape
+        if len(shape) != 2 or shape[0] != rows or shape[1] * 32 < nodes:
+            raise ValueError(f"mask has a row of at least {-(-nodes // 32)} words for each of {rows} nodes, not {tuple(shape)}")
+        mask_stride = shape[1]
     cos, sin, length = _arg_rope(rope_cos, rope_sin, dev)
     if max_len is None:
         max_len = min(fields[7] * fields[10], _INT_MOST)
