@@ -448,9 +448,11 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     using S = TreeShape<R>;
     const tenzo_attention_tree_args& a = L.a;
     extern __shared__ unsigned char tr_smem[];
-    __shared__ __align__(16) float s_f[R], s_down[R], s_max[4][R], s_sum[4][R], s_scale_max[S::groups][4];    // (s_down: the references with their signs turned)
+    __shared__ __align__(16) float s_f[R];
+    __shared__ __align__(16) float s_down[R];            // the references with their signs turned
+    __shared__ __align__(16) float s_max[4][R], s_sum[4][R], s_scale_max[S::groups][4];
     __shared__ long long s_at[R], s_from[R];             // [row][head] of a query, and its vector in q; -1: none of this tree's, or refused
-    __shared__ uint32_t s_mask[R][kTrMask];
+    __shared__ __align__(16) uint32_t s_mask[R][kTrMask];
     __shared__ int s_pos[R];
     __shared__ uint64_t s_full[2 * S::stages], s_empty[2 * S::stages], s_bar[S::lines][4];     // rings of keys and of values
     __shared__ unsigned s_valid[S::stages];
@@ -886,9 +888,10 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
     using S = WeighShape<R>;
     const tenzo_attention_tree_args& a = L.a;
     extern __shared__ unsigned char tr_smem[];
-    __shared__ __align__(16) float s_f[R], s_down[R];    // (s_down: log-sum-exps with their signs turned)
+    __shared__ __align__(16) float s_f[R];
+    __shared__ __align__(16) float s_down[R];            // log-sum-exps with their signs turned
     __shared__ long long s_from[R];
-    __shared__ uint32_t s_mask[R][kTrMask];
+    __shared__ __align__(16) uint32_t s_mask[R][kTrMask];
     __shared__ int s_pos[R];
     __shared__ uint64_t s_full[S::stages], s_empty[S::stages], s_scores[2], s_free[2];
     __shared__ unsigned s_valid[S::stages];

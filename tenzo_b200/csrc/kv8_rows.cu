@@ -215,7 +215,7 @@ template <bool HELD, int T>
 __global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const tenzo_kv8_evict_args a) {
     constexpr int kThreads = T, kWarps = T / 32;
     extern __shared__ __align__(16) uint32_t ev_smem[];
-    __shared__ uint32_t s_count[2][kWarps][4];
+    __shared__ __align__(16) uint32_t s_count[2][kWarps][4];                     // (read four at a time)
     __shared__ int s_warp[3][kWarps], s_listed;
     __shared__ uint32_t s_list[2 * kThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.y, layer = blockIdx.x / a.cache.n_kv, kvh = blockIdx.x % a.cache.n_kv;
