@@ -1093,6 +1093,7 @@ static int tree_check(TreeLaunch& L) {
     if (a.mask_stride == 0) a.mask_stride = words;
     if (a.mask_stride < words) return -1;
     L.group = a.n_q / a.cache.n_kv;
+    // (Vectors of four where all rows allow it: 16 trees of 64 nodes, 8192 keys, 222 us, by single numbers 225; their weights 145 and 154.)
     L.aligned = kv8_aligned(a.q, 16) && a.q_stride % 4 == 0 && kv8_aligned(a.rope_cos, 16) && kv8_aligned(a.rope_sin, 16);
     return 0;
 }
@@ -1112,8 +1113,9 @@ static int tree_queries_a_cta(long long queries) {
         if (cost[i] * (double)((queries + width[i] - 1) / width[i]) < cost[best] * (double)((queries + width[best] - 1) / width[best])) best = i;
     return width[best];
 }
-// Queries a pass over the keys whose weights are summed, of which a CTA makes as many as there are: 16, twice if that is enough (64 sequences of 24 or 32 queries, 4096 keys: 70 us; in one of 48, 79);
-// then 48 (32 x 48: 45 us, three of 16 52, one of 64 51; 32 x 80: 74, 79 and 88) or 64, of which a pass of 48 costs 0.87 (16 x 128: 48 us at 64, 60 at 48; 4 x 1000: 174 and 190).
+// Queries a pass over the keys whose weights are summed, of which a CTA makes as many as there are: 16, twice if that is enough (64 sequences of 20 or 32 queries, 4096 keys: 62 and 63 us; in one of
+// 48, 75); then 48 (32 x 48: 41 us, three of 16 47, one of 64 49; 32 x 80: 69, 73 and 85) or 64, of which a pass of 48 costs 0.87 (32 x 64: 50 us at 64, 60 at 16, 72 at 48; 16 x 128: 48 at 64,
+// 58 at 48; 4 x 1000: 171 and 186).
 static int weigh_queries_a_pass(long long queries) {
     if (queries <= 32) return 16;
     return 0.87 * (double)((queries + 47) / 48) < (double)((queries + 63) / 64) ? 48 : 64;
