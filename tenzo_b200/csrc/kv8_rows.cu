@@ -520,10 +520,10 @@ extern "C" int tenzo_cuda_kv8_evict(const tenzo_kv8_evict_args* args, void* stre
     const size_t smem = (((size_t)(a.max_len + 31) / 32 + 3) / 4 * 4 + (size_t)(held ? (a.max_len + 3) / 4 * 4 : kEvLists)) * 4;
     constexpr size_t most = (kEvHeld / 32 + kEvHeld) * 4;
     static_assert(most >= (kEvMost / 32 + kEvLists) * 4, "the larger of the two");
-    static_assert(most <= kMaxSmem - 3072, "bits of the longest and numbers of the longest that are held");
+    static_assert(most <= kMaxSmem - 4096, "bits of the longest and numbers of the longest that are held");
     const long long ctas = (long long)a.cache.n_layers * a.cache.n_kv;
     if (ctas > 0x7fffffffLL) return -5;
-    const bool many = ctas * a.sequences > 148 * 4 && 8 * (smem + 3072) <= kMaxSmem;
+    const bool many = ctas * a.sequences > 148 * 4 && 8 * (smem + 4096) <= kMaxSmem;
     auto kernel = many ? kv8_evict_kernel<true, 128> : held ? kv8_evict_kernel<true, 256> : kv8_evict_kernel<false, 256>;
     if (smem > 40 * 1024)
         if (cudaError_t e = allow_smem(kernel, most)) return (int)e;
