@@ -17,6 +17,7 @@
 #include "attn_common.cuh"
 #include "kv8.cuh"
 #include "umma.cuh"
+#include "weigh_sums.cuh"
 
 namespace tz {
 
@@ -896,13 +897,14 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
     __shared__ uint64_t s_full[S::stages], s_empty[S::stages], s_scores[2], s_free[2];
     __shared__ unsigned s_valid[S::stages];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_found, s_rows[S::rows_most * 8];    // rows of the chunks of the last tiles
+    __shared__ int s_found, s_given_up, s_rows[S::rows_most * 8];    // (s_rows: rows of the chunks of the last tiles)
     __shared__ long long s_scan[S::threads / 32 + 2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned char* base = tr_smem + (((smem_addr(tr_smem) + 1023u) & ~1023u) - smem_addr(tr_smem));
     unsigned char* s_q = base + S::stages * kTrTileBytes;
     float *s_scales = reinterpret_cast<float*>(s_q + S::q_bytes), *s_sum = s_scales + 2 * S::stages * kTrTile;
     if (tid == 0) {
+        s_given_up = 0;
         for (int i = 0; i < S::stages; ++i) {
             mbar_init(&s_full[i], 33);
             mbar_init(&s_empty[i], S::warps + 1);        // the products, and the warps that read the scales
@@ -1002,7 +1004,7 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                         __syncwarp();
                         const unsigned valid = s_valid[st];
                         const int direct = S::direct ? s_rows[n % S::rows_most * 8 + (key >> 4)] : -1;
-                        if (!S::direct && flat0 == 0 && group == 0 && (lane & 15) == 0) {     // the weights, which are wanted when the last pass is done
+                        if (!S::direct && ok && flat0 == 0 && group == 0 && (lane & 15) == 0) {     // the weights, which are wanted when the last pass is done
                             const int row = s_rows[n % S::rows_most * 8 + (key >> 4)];
                             if (row >= 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(L.weight + row));
                         }
@@ -1034,30 +1036,10 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
                     }
                 }
                 if (S::direct) continue;
+                if (!ok) s_given_up = 1;
                 named_barrier_sync(kEvery, kAll);
-                // the last t1 - t0 tiles' rows are remembered (behind n the copies are at most `stages` tiles)
-                constexpr int kBatch = 8;                // loads in flight
-                for (int k0 = tid; k0 < (t1 - t0) * kTrTile; k0 += kBatch * kAll) {
-                    int row[kBatch];
-                    float old[kBatch];
-#pragma unroll
-                    for (int u = 0; u < kBatch; ++u) {
-                        const int k = k0 + u * kAll, i = k / kTrTile;
-                        const bool there = k < (t1 - t0) * kTrTile && t0 * kTrTile + k < total;
-                        row[u] = there ? s_rows[(n - (t1 - t0) + i) % S::rows_most * 8 + (k % kTrTile) / kK8Chunk] : -1;
-                        if (row[u] >= 0) row[u] += k % kK8Chunk;
-                    }
-#pragma unroll
-                    for (int u = 0; u < kBatch; ++u) old[u] = ld_l2(L.weight + max(row[u], 0));           // (something, where there is none)
-#pragma unroll
-                    for (int u = 0; u < kBatch; ++u) {
-                        float sum = 0.0f;
-                        if (row[u] < 0) continue;
-#pragma unroll
-                        for (int g = 0; g < S::groups; ++g) sum += s_sum[g * S::most * kTrTile + k0 + u * kAll];
-                        L.weight[row[u]] = old[u] + sum;
-                    }
-                }
+                // (behind n the copies are at most `stages` tiles)
+                weigh_add<S::groups, S::most, S::rows_most, kAll, kTrTile, kK8Chunk>(*reinterpret_cast<volatile int*>(&s_given_up) != 0, tid, n, t0, t1, total, s_rows, s_sum, L.weight);
             }
     }
     if (blockIdx.x == 0)
