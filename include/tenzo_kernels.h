@@ -386,7 +386,7 @@ TENZO_API int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* str
 typedef struct {
     const float* q;          /* [sequences*nodes][q_stride], n_q*128 used, before rotation */
     float* out;              /* [sequences*nodes][n_q*128], 16-byte aligned, apart from q */
-    float* lse;              /* [sequences*nodes][n_q], or NULL */
+    float* lse;              /* [sequences*nodes][n_q], or NULL; apart from q and out where it is written */
     tenzo_kv8_cache cache;
     const int* start;        /* [sequences] device */
     const int* count;        /* [sequences] device, or NULL */
@@ -422,7 +422,7 @@ TENZO_API int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float*
  * infinitely heavy (protect_from NULL: none does), NaN as -infinity, and of equal weights the lower place stays. Tokens that stay keep their places if those are below `keep`; the others
  * move, in the order of their places, to the places below `keep` that became free, in the order of those, with scales, weight and position. (Order means nothing to
  * attention over rotated keys: it takes one row's move a token evicted, not the whole cache's.) length_out[s] = min(length[s], keep), in
- * memory of its own. No two sequences of a call may name the same table row, or blocks in common.
+ * memory of its own (-1 where it has bytes in common with what the call reads). No two sequences of a call may name the same table row, or blocks in common.
  * A negative length, one above max_len, a table row out of range or a table entry out of range leaves the sequence as it is, with length_out[s] = length[s], and raises the
  * flag. max_len <= slots * table_stride; max_len <= 2^20 and sequences <= 65535 (-5 otherwise). */
 typedef struct {
@@ -448,7 +448,7 @@ typedef struct {
     const int* token; const int* parent; const int* chosen;   /* [sequences][nodes] device */
     const int* start;                               /* [sequences] device */
     const int* count; const int* seq;               /* [sequences] device, or NULL */
-    int* accepted; int* next; int* path;            /* device: [sequences], [sequences], [sequences][nodes], in memory of their own */
+    int* accepted; int* next; int* path;            /* device: [sequences], [sequences], [sequences][nodes], in memory of their own (-1 otherwise) */
     float* weight; int* position;                   /* or NULL */
     int sequences, nodes;
     int use_pdl;

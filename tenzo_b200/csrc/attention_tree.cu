@@ -1161,10 +1161,10 @@ extern "C" int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, 
     if (a.sequences == 0) return 0;
     if (int rc = tree_check(L)) return rc;
     if (!a.out || !kv8_aligned(a.out, 16) || a.shares < 0 || a.shares > 65535) return -1;
-    {                                                    // (a query is read by every CTA that has some of its keys)
-        const size_t row = (size_t)a.n_q * kK8Hd, rows = (size_t)a.sequences * a.nodes;
-        const uintptr_t q0 = reinterpret_cast<uintptr_t>(a.q), q1 = q0 + ((rows - 1) * a.q_stride + row) * sizeof(float), o0 = reinterpret_cast<uintptr_t>(a.out), o1 = o0 + rows * row * sizeof(float);
-        if (q0 < o1 && o0 < q1) return -1;
+    {                                                    // (a query, and what names it, is read by every CTA that has some of its keys)
+        const size_t row = (size_t)a.n_q * kK8Hd, rows = (size_t)a.sequences * a.nodes, q_bytes = ((rows - 1) * a.q_stride + row) * sizeof(float);
+        const size_t out_bytes = rows * row * sizeof(float), lse_bytes = rows * a.n_q * sizeof(float);
+        if (kv8_overlap(a.q, q_bytes, a.out, out_bytes) || kv8_overlap(a.q, q_bytes, a.lse, lse_bytes) || kv8_overlap(a.out, out_bytes, a.lse, lse_bytes)) return -1;
     }
     tree_plan(L);
     L.cut = a.workspace && kv8_aligned(a.workspace, 16) && a.workspace_bytes >= tree_room(L);

@@ -27,6 +27,13 @@ inline bool kv8_cache_ok(const tenzo_kv8_cache& c) {
     // (a row's number is an int in the copies' coordinates; the quotients never pass 64 bits)
     return (long long)c.n_blocks * c.n_layers <= 0x7fffffffLL && (long long)c.n_kv * c.slots <= 0x7fffffffLL / ((long long)c.n_blocks * c.n_layers);
 }
+// Whether two ranges of memory have bytes in common (a null range has none).
+inline bool kv8_overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+inline size_t kv8_table_bytes(const tenzo_kv8_cache& c) { return (size_t)c.table_rows * c.table_stride * sizeof(int); }
+inline size_t kv8_rows(const tenzo_kv8_cache& c) { return (size_t)c.n_blocks * c.n_layers * c.n_kv * c.slots; }
 inline long long kv8_places(const tenzo_kv8_cache& c) { return (long long)c.table_stride * c.slots; }
 
 }  // namespace tz

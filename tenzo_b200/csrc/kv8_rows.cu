@@ -470,6 +470,27 @@ __global__ void __launch_bounds__(T, 1024 / T) kv8_evict_kernel(const tenzo_kv8_
     }
 }
 
+// ---- the calls ------------------------------------------------------------------------------------------------------------------
+// Results that lie in what is read, anywhere in it, would be written under the eyes of CTAs that come later: such calls are refused.
+struct K8Range {
+    const void* at;
+    size_t bytes;
+};
+template <int W, int N>
+static bool k8_apart(const K8Range (&written)[W], const K8Range (&read)[N], const tenzo_kv8_cache& c) {
+    const size_t rows = kv8_rows(c);
+    const K8Range pools[4] = {{c.k, rows * kK8Hd}, {c.v, rows * kK8Hd}, {c.scale_k, rows * sizeof(float)}, {c.scale_v, rows * sizeof(float)}};
+    for (int i = 0; i < W; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (kv8_overlap(written[i].at, written[i].bytes, written[j].at, written[j].bytes)) return false;
+        for (const K8Range& r : read)
+            if (kv8_overlap(written[i].at, written[i].bytes, r.at, r.bytes)) return false;
+        for (const K8Range& r : pools)
+            if (kv8_overlap(written[i].at, written[i].bytes, r.at, r.bytes)) return false;
+    }
+    return true;
+}
+
 }  // namespace tz
 
 extern "C" int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* stream) {
@@ -496,10 +517,13 @@ extern "C" int tenzo_cuda_kv8_accept(const tenzo_kv8_accept_args* args, void* st
     if (!kv8_cache_ok(a.cache) || a.sequences < 0) return -1;
     if (a.sequences == 0) return 0;
     if (!a.token || !a.parent || !a.chosen || !a.start || !a.accepted || !a.next || !a.path || a.nodes <= 0 || (!a.seq && a.sequences > a.cache.table_rows)) return -1;
-    const int* const written[3] = {a.accepted, a.next, a.path};
-    for (const int* to : written)                                    // (what other CTAs of the sequence still read)
-        if (to == a.token || to == a.parent || to == a.chosen || to == a.start || to == a.count || to == a.seq) return -1;
     if (a.nodes > TENZO_TREE_MOST || a.sequences > 65535) return -5;
+    {                                                                // results apart from each other, and from what other CTAs of the sequence still read
+        const size_t one = (size_t)a.sequences * sizeof(int), all = one * a.nodes, beside = kv8_rows(a.cache) * sizeof(int);
+        const K8Range written[3] = {{a.accepted, one}, {a.next, one}, {a.path, all}};
+        const K8Range read[9] = {{a.token, all}, {a.parent, all}, {a.chosen, all}, {a.start, one}, {a.count, one}, {a.seq, one}, {a.cache.block_table, kv8_table_bytes(a.cache)}, {a.weight, beside}, {a.position, beside}};
+        if (!k8_apart(written, read, a.cache)) return -1;
+    }
     const long long units = (long long)a.cache.n_layers * a.cache.n_kv, share = (units * a.sequences + 148 * 8 - 1) / (148 * 8);
     const int many = (int)(share < units ? share : units);           // (layer, kv head) pairs a CTA takes
     if ((long long)many * a.nodes > 1 << 30) return -5;
@@ -513,9 +537,14 @@ extern "C" int tenzo_cuda_kv8_evict(const tenzo_kv8_evict_args* args, void* stre
     if (!kv8_cache_ok(a.cache) || a.sequences < 0) return -1;
     if (a.sequences == 0) return 0;
     if (!a.weight || !a.position || !kv8_aligned(a.weight, 16) || !kv8_aligned(a.position, 16) || !a.length || !a.length_out) return -1;
-    if (a.length_out == a.length || a.length_out == a.seq || a.length_out == a.protect_from) return -1;      // (which other CTAs still read)
     if (a.keep <= 0 || a.max_len <= 0 || a.max_len > kv8_places(a.cache) || (!a.seq && a.sequences > a.cache.table_rows)) return -1;
     if (a.sequences > 65535 || a.max_len > kEvMost) return -5;
+    {                                                                // apart from what other CTAs still read
+        const size_t one = (size_t)a.sequences * sizeof(int), beside = kv8_rows(a.cache) * sizeof(int);
+        const K8Range written[1] = {{a.length_out, one}};
+        const K8Range read[6] = {{a.length, one}, {a.seq, one}, {a.protect_from, one}, {a.cache.block_table, kv8_table_bytes(a.cache)}, {a.weight, beside}, {a.position, beside}};
+        if (!k8_apart(written, read, a.cache)) return -1;
+    }
     const bool held = a.max_len <= kEvHeld;
     const size_t smem = (((size_t)(a.max_len + 31) / 32 + 3) / 4 * 4 + (size_t)(held ? (a.max_len + 3) / 4 * 4 : kEvLists)) * 4;
     constexpr size_t most = (kEvHeld / 32 + kEvHeld) * 4;
