@@ -379,8 +379,9 @@ TENZO_API int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* str
  * are there; the others are padding, are seen by none, and their rows of out are zeros. start[s] < 0: the whole sequence is padding.
  *   out[s*nodes + i] = softmax(q K^T / sqrt(128)) V per query head h, over kv head h / (n_q / n_kv), the query rotated at rope_pos[s*nodes + i] (NULL: start[s] + i);
  *   lse = log sum exp of the arguments (natural logarithm; -infinity and zeros in out where nothing is seen).
- * Sums and softmax in fp32 or whole numbers; the query is rounded to 22 bits and a sign of its head's largest number, the weights to 26 bits of their row's largest when it was last looked for: outputs agree with
- * 64 bits to about 1e-6 of their norm. A NaN or an infinity in a head's query makes that head's outputs NaN; what lies in places that are not seen has no part.
+ * Sums and softmax in fp32 or whole numbers; the query is rounded to 22 bits and a sign of its head's largest number, a weight times its value's scale to 26 bits of the largest such product that the row
+ * had met when it was last looked for: outputs agree with 64 bits to about 1e-6 of their norm where no dim of a query is far larger than the others (2^-22 of the largest number, times the key's sum of magnitudes, is
+ * what the argument may be off by), with scales of values up to 2^60 apart and from 2^-60 on. A NaN or an infinity in a head's query makes that head's outputs NaN; what lies in places that are not seen has no part.
  * A sequence with start + count > max_len or a table row out of range, and a row whose position is, are not written and raise the flag; a table entry out
  * of range leaves its block's keys out and raises it. */
 typedef struct {

@@ -6,10 +6,11 @@
 //   * Both are products of whole numbers (tcgen05 kind::i8, sums of 32 bits), and the codes of the cache are operands as they lie: K and V tiles go from memory to shared
 //     memory to the tensor cores, nothing is unpacked or converted. A query is scaled to a maximum of 2^21 to 2^22 and rounded; its three signed bytes are three columns. A weight, p * scale of its
 //     value, is rounded to a whole number of 31 bits; its four bytes, as they lie in the register, are four columns. So P is stored as it is computed, 16 bytes for four queries, and its
-//     operand and V's are both read transposed (MN-major). Sums are exact: what rounds is the query (2^-22 of its largest number), the weights (2^-27 of a row's largest) and fp32 in between.
+//     operand and V's are both read transposed (MN-major). Sums are exact: what rounds is the query (2^-22 of its largest number), the products of weight and scale (2^-27 of a row's largest) and fp32 in between.
 //   * softmax: a thread has one key and sixteen queries, so a row's maximum goes across lanes; and accumulators of whole numbers cannot be scaled down.
-//     Both are avoided: a row's weights are taken relative to a reference, the maximum when it was last set, and may grow to 2^5 of it. Only where a weight would pass that (one vote a
-//     tile; the first tile always) the references are set anew and the accumulators moved on into fp32.
+//     Both are avoided: a row's weights are taken relative to a reference, set so that the largest product of weight and scale is 1, and these products may grow to 2^5. Only where one would pass
+//     that (one vote a tile; the first tile always) the references are set anew and the accumulators moved on into fp32. The reference goes by the product, which a thread has as a sum with its scale's
+//     logarithm, and by the row's own keys: neither a key of most weight and small values, as a first token often is, nor one of large values that others see leaves a row fewer bits.
 //   * Bound: single tokens by the bytes (64 sequences of 8192 keys, 20 heads over 5: 118 us on the device, 106 at the memory's measured rate), trees by the instructions of the warps that make
 //     weights, some 415 for 32 keys and sixteen queries (16 trees of 64 nodes, 8192 keys: 227 us, 2600 cycles a tile of 64 queries, 64 % of the issue slots; tensor cores 32 %, memory 10 %); small
 //     calls by the chain share, queries, tile, outputs, join (8 nodes, 1000 keys: 13.4 us). Going on to the next pair takes some 9000 cycles, 4300 of them 64 queries'.
@@ -23,7 +24,9 @@ namespace tz {
 
 constexpr int kTrTile = 128, kTrTileBytes = kTrTile * kK8Hd;          // keys a step; bytes of their codes
 constexpr int kTrMask = TENZO_TREE_MOST / 32;
-constexpr float kTrSlack = 5.0f, kTrOne = 67108864.0f;                // a weight of 1 is 2^26, weights up to 2^5 are let through
+constexpr int kTrOne = 26;                                            // a row's largest product of weight and scale is 2^26
+constexpr float kTrSlack = 5.0f;                                      // when it was looked for; up to 2^5 of that is let through
+constexpr float kTrScales = 60.0f;                                    // a scale below 2^-60 of the others is taken as that where references are set
 constexpr float kTrLow = -1e30f;                                      // a reference that is not set
 constexpr uint32_t kTrShape = (2u << 4) | (1u << 7) | ((uint32_t)(kTrTile >> 4) << 24);      // of products: sums of 32 bits; codes, with a sign, as A; 128 rows
 constexpr int kTrFlush = 256;                                         // tiles after which the accumulators are moved on all the same: 2^15 keys * 128 * 255 < 2^31
@@ -452,6 +455,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     __shared__ __align__(16) float s_f[R];
     __shared__ __align__(16) float s_down[R];            // the references with their signs turned
     __shared__ __align__(16) float s_max[4][R], s_sum[4][R], s_scale_max[S::groups][4];
+    __shared__ __align__(16) float4 s_unit[S::groups];   // of these queries' weights: log2 of a scale that is as good as 1, that and the slack, 2^26 over it, it over 2^26
     __shared__ long long s_at[R], s_from[R];             // [row][head] of a query, and its vector in q; -1: none of this tree's, or refused
     __shared__ __align__(16) uint32_t s_mask[R][kTrMask];
     __shared__ int s_pos[R];
@@ -459,7 +463,6 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     __shared__ unsigned s_valid[S::stages];
     __shared__ uint32_t s_tmem, s_set[S::groups];        // queries that have a reference
     __shared__ int s_vote[S::groups][2], s_found;
-    __shared__ float s_unit[S::groups][2];               // values' scales count up to this power of two; what a scale is multiplied by
     __shared__ long long s_scan[S::threads / 32 + 2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, tile = (int)blockIdx.x % L.tiles, share = (int)blockIdx.x / L.tiles, flat0 = tile * R;
     unsigned char* base = tr_smem + (((smem_addr(tr_smem) + 1023u) & ~1023u) - smem_addr(tr_smem));
@@ -588,7 +591,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                 mask.store(a, to >= 0, s_mask[tid]);
             }
             if (lane == 0 && quarter == 0) {
-                s_unit[group][0] = s_unit[group][1] = 0.0f;
+                s_unit[group] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 s_set[group] = 0;
             }
             named_barrier_sync(kEvery, kAll);
@@ -649,8 +652,9 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                     over = fmaxf(fmaxf(over, w0), w1);
                 }
                 const uint32_t set = s_set[group];
-                const float unit = s_unit[group][0];
-                if (over > kTrSlack || sv > unit || set != 0xffffu || (n + 1) % kTrFlush == 0) s_vote[group][n & 1] = n + 1;
+                const float4 unit = s_unit[group];
+                const float log_scale = fmaxf(tr_lg2(sv), unit.x - kTrScales);
+                if (over + log_scale > unit.y || set != 0xffffu || (n + 1) % kTrFlush == 0) s_vote[group][n & 1] = n + 1;
                 named_barrier_sync(1 + group, 128);
                 const int vote = *reinterpret_cast<volatile int*>(&s_vote[group][n & 1]);
                 f32x2 p[8];
@@ -667,22 +671,25 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                     for (int r = 0; r < 16; r += 2) {
                         float w0, w1;
                         unpack2(w[r / 2], w0, w1);
-                        w0 = tr_warp_max(w0);
-                        w1 = tr_warp_max(w1);
+                        w0 = tr_warp_max(w0 + log_scale);
+                        w1 = tr_warp_max(w1 + log_scale);
                         if (lane == r) top = w0;
                         if (lane == r + 1) top = w1;
                     }
                     if (lane < 16) s_max[quarter][first + lane] = top;
-                    const float most = tr_warp_max(sv);
+                    const float most = tr_warp_max(over > -INFINITY ? sv : 0.0f);      // (a key that none of these queries sees does not count)
                     if (lane == 0) s_scale_max[group][quarter] = most;
                     named_barrier_sync(1 + group, 128);
                     const float4 scales = *reinterpret_cast<const float4*>(s_scale_max[group]);
+                    // The unit is set with the first references: a power of two above the largest scale there, 2^-60 to 2^30 (1, where all of them are 0).
                     const float scale_most = fmaxf(fmaxf(scales.x, scales.y), fmaxf(scales.z, scales.w));
+                    const int bits = scale_most > 0.0f ? (int)min(max((__float_as_uint(scale_most) >> 23) + 1u, 67u), 157u) : 127;
+                    const float log_unit = set ? unit.x : (float)(bits - 127);
                     float up, by;                        // of query `first` + lane % 16: how far its reference goes up (the first one may go down), and what that leaves of its sums
                     {
                         const int r = lane & 15;
                         const bool was = set >> r & 1u;
-                        top = fmaxf(fmaxf(s_max[0][first + r], s_max[1][first + r]), fmaxf(s_max[2][first + r], s_max[3][first + r]));
+                        top = fmaxf(fmaxf(s_max[0][first + r], s_max[1][first + r]), fmaxf(s_max[2][first + r], s_max[3][first + r])) - log_unit;
                         up = was ? fmaxf(top, 0.0f) : top == -INFINITY ? 0.0f : top;
                         by = was ? tr_ex2(-up) : 0.0f;   // (there is nothing yet)
                     }
@@ -690,10 +697,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                     if (quarter == 0) {
                         if (lane < 16) s_down[first + lane] -= up;
                         if (lane == 0) {
-                            // a power of two above the largest scale, at least 2^-60
-                            const float now = scale_most > unit ? __uint_as_float(min(max((__float_as_uint(scale_most) >> 23) + 1u, 67u), 254u) << 23) : unit;
-                            s_unit[group][0] = now;
-                            s_unit[group][1] = now > 0.0f ? kTrOne / now : 0.0f;
+                            if (!set && now_set) s_unit[group] = make_float4(log_unit, log_unit + kTrSlack, __uint_as_float((uint32_t)(254 + kTrOne - bits) << 23), __uint_as_float((uint32_t)(bits - kTrOne) << 23));
                             s_set[group] = now_set;
                         }
                     }
@@ -713,7 +717,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
 #pragma unroll
                         for (int h = 0; h < 16; h += 8) {
                             float o[8];
-                            moved(h, unit * (1.0f / kTrOne), o);
+                            moved(h, unit.w, o);
 #pragma unroll
                             for (int r = 0; r < 8; ++r) o[r] *= __shfl_sync(0xffffffffu, by, h + r);
                             tr_st8(t_moved + h, o);
@@ -724,7 +728,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                     }
                     named_barrier_sync(1 + group, 128);
                 }
-                const float by = sv * s_unit[group][1];
+                const float by = sv * s_unit[group].z;
                 const f32x2 by2 = pack2(by, by);
                 uint32_t word[16];
 #pragma unroll
@@ -773,7 +777,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
 #pragma unroll
             for (int h = 0; h < 16; h += 8) {
                 float o[8];
-                moved(h, s_unit[group][0] * (1.0f / kTrOne), o);
+                moved(h, s_unit[group].w, o);
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     const long long to = s_at[first + h + r];
