@@ -4,9 +4,9 @@
 //     the queries as columns: S^T = K Q^T and O^T = V^T P^T. A CTA takes 16, 32, 48 or 64 of the queries and walks its keys in tiles of 128. With keys as rows a single
 //     query fills the tensor cores as well as many do, and one kernel serves a decode step and a tree of 64 nodes.
 //   * Both are products of whole numbers (tcgen05 kind::i8, sums of 32 bits), and the codes of the cache are operands as they lie: K and V tiles go from memory to shared
-//     memory to the tensor cores, nothing is unpacked or converted. A query is scaled to a maximum of 2^21 to 2^22 and rounded; its three signed bytes are three columns. A weight, p * scale of its
+//     memory to the tensor cores, nothing is unpacked or converted. A query is scaled to a maximum of 2^29 to 2^30 and rounded; its four signed bytes are four columns. A weight, p * scale of its
 //     value, is rounded to a whole number of 31 bits; its four bytes, as they lie in the register, are four columns. So P is stored as it is computed, 16 bytes for four queries, and its
-//     operand and V's are both read transposed (MN-major). Sums are exact: what rounds is the query (2^-22 of its largest number), the products of weight and scale (2^-27 of a row's largest) and fp32 in between.
+//     operand and V's are both read transposed (MN-major). Sums are exact: what rounds is the query (2^-30 of its largest number; with three bytes, 2^-22, a query with one large dim lost its others, and 16 trees of 64 nodes took 231 us instead of 235), the products of weight and scale (2^-27 of a row's largest) and fp32 in between.
 //   * softmax: a thread has one key and sixteen queries, so a row's maximum goes across lanes; and accumulators of whole numbers cannot be scaled down.
 //     Both are avoided: a row's weights are taken relative to a reference, set so that the largest product of weight and scale is 1, and these products may grow to 2^5. Only where one would pass
 //     that (one vote a tile; the first tile always) the references are set anew and the accumulators moved on into fp32. The reference goes by the product, which a thread has as a sum with its scale's
@@ -54,14 +54,15 @@ struct TreeShape {
     // 64 queries are two lines of 32, which have the tiles in common and wait for nothing else of each other: the tensor cores work for the one while the other's warps make weights.
     static constexpr int lines = R == 64 ? 2 : 1, line = R / lines, line_warps = line / 4;
     static constexpr int stages = R > 32 ? 3 : 2, resident = R > 32 ? 1 : 2;
-    static constexpr int s_cols = 3 * line, o_cols = 4 * line, all_s = 3 * R, all_o = 4 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;
-    static_assert(all_s + all_o + R <= tmem_cols, "tensor memory: scores, products with the values, outputs that were moved on");
+    static constexpr int s_cols = 4 * line, o_cols = 4 * line, all_s = 4 * R, all_o = 4 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;
+    static_assert(all_s + all_o <= tmem_cols, "tensor memory: scores, products with the values");
     // Registers a thread: as the block is launched, and after the warps of the second line have given some to those of the first.
     static constexpr int launched = R == 64 ? 96 : R == 48 ? 128 : R == 32 ? 80 : 128, most = R == 64 ? 112 : R == 48 ? 144 : R == 32 ? 104 : 168, least = R == 48 ? 40 : R == 16 ? 64 : 32;
     static_assert(warps * most + 4 * least <= (warps + 4) * launched, "what is taken is there");
     static constexpr int p_panels = R > 32 ? 2 : 1;                   // of 128 bytes: 32 queries
     static constexpr int q_bytes = all_s * kK8Hd, p_bytes = p_panels * kTrTileBytes;
-    static constexpr size_t smem = 1024 + (size_t)stages * 2 * kTrTileBytes + q_bytes + p_bytes + stages * 2 * kTrTile * 4;
+    static constexpr bool kept_shared = R != 32;                      // outputs that were moved on lie in shared memory; of two CTAs of 32 queries there is no room for them, and they are the threads' own
+    static constexpr size_t smem = 1024 + (size_t)stages * 2 * kTrTileBytes + q_bytes + p_bytes + stages * 2 * kTrTile * 4 + (kept_shared ? R * kTrTile * 4 : 0);
 };
 
 __device__ __forceinline__ float tr_ex2(float x) {
@@ -90,10 +91,6 @@ __device__ __forceinline__ void tr_wait8(uint32_t (&r)[8]) {
 __device__ __forceinline__ void tr_tie8(uint32_t (&r)[8]) {
     asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
 }
-__device__ __forceinline__ void tr_st8(uint32_t at, const float (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 ::"r"(at), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]) : "memory");
-}
 // What one lane of a warp does that is together: which, and a product and a commit of it. (From a branch that one lane takes, the same products start 93 cycles apart and those of 256
 // columns take 169; like this 77 and 128, which is what the multiplications take.)
 __device__ __forceinline__ uint32_t tr_elect() {
@@ -114,11 +111,10 @@ __device__ __forceinline__ uint64_t tr_desc_mn(uint32_t saddr, uint32_t panel) {
 }
 __device__ __forceinline__ f32x2 tr_mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 tr_fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-// Two sums from the three parts of whole numbers (below 2^21 each). The high part is made a float by adding 1.5 * 2^23 to its bits, as the units that convert are those of 2^x too.
-__device__ __forceinline__ f32x2 tr_whole(const uint32_t* high, const uint32_t* mid, const uint32_t* low) {
-    constexpr float kMagic = 12582912.0f;
-    const f32x2 hi = add2(pack2(__uint_as_float(high[0] + 0x4b400000u), __uint_as_float(high[1] + 0x4b400000u)), pack2(-kMagic, -kMagic));
-    return tr_fma2(hi, pack2(65536.0f, 65536.0f), pack2((float)((int)mid[0] * 256 + (int)low[0]), (float)((int)mid[1] * 256 + (int)low[1])));
+// Two sums from the four parts of whole numbers (below 2^21 each), highest first.
+__device__ __forceinline__ f32x2 tr_whole(const uint32_t* a, const uint32_t* b, const uint32_t* c, const uint32_t* d) {
+    const f32x2 high = pack2((float)((int)a[0] * 256 + (int)b[0]), (float)((int)a[1] * 256 + (int)b[1]));
+    return tr_fma2(high, pack2(65536.0f, 65536.0f), pack2((float)((int)c[0] * 256 + (int)d[0]), (float)((int)c[1] * 256 + (int)d[1])));
 }
 // The same value in N columns of the warp's 32 lanes.
 template <int N>
@@ -249,7 +245,7 @@ struct TreeWalk {
 
 // ---- the parts that both kernels have ------------------------------------------------------------------------------------------
 // R queries of a block on their way to the operand, four by each of its R / 4 warps. A lane has dims 4 lane .. 4 lane + 3, and the lane sixteen on, or back, those that they are turned
-// with. A vector is turned, scaled by a power of two to a maximum between 2^21 and 2^22 and rounded; its signed bytes are rows r, LINE + r, 2 LINE + r of its line's operand (128 bytes each, swizzled).
+// with. A vector is turned, scaled by a power of two to a maximum between 2^29 and 2^30 and rounded; its signed bytes are rows r, LINE + r, .., 3 LINE + r of its line's operand (128 bytes each, swizzled).
 // s_f: what a unit of the products with the codes counts in the argument of 2^x (NaN for a query that is not finite). from[r]: the vector in q, -1: none, zeros.
 // (Every load is made, of something, without a branch around it: where two ways meet the compiler copies what was loaded, and so waits for it. Bytes cut off one after another, by shifts, made the
 // weights of 4 x 250 nodes, which are mostly this, 178 us; like this 168.)
@@ -300,18 +296,17 @@ __device__ __forceinline__ void tr_queries(const TreeLaunch& L, const long long*
         const int r = warp + i * (R / 4);
         const bool bad = most[i] >= 0x7f800000u;         // (its bytes are anything, as those of a vector that is not there)
         const uint32_t e = most[i] >> 23;                // 43 .. 254
-        const float up = bad || at[i] < 0 ? 0.0f : __uint_as_float((275u - e) << 23);
-        // Rounded as the low bits of 1.5 * 2^23; with 128 added to every byte, carries and all, the bytes are the three signed ones and 128 each.
-        uint32_t v[4];
+        const float up = bad || at[i] < 0 ? 0.0f : __uint_as_float((283u - e) << 23);
+        uint32_t v[4];                                   // with 128 added to every byte, carries and all, the bytes are the four signed ones and 128 each
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(__fmaf_rn(x[i][j], up, 12582912.0f)) - 0x4b400000u + 0x808080u;
-        const uint32_t two0 = prmt(v[0], v[1], 0x5140u), two1 = prmt(v[2], v[3], 0x5140u), top0 = prmt(v[0], v[1], 0x0062u), top1 = prmt(v[2], v[3], 0x0062u);
-        const uint32_t part[3] = {prmt(top0, top1, 0x5410u), prmt(two0, two1, 0x7632u), prmt(two0, two1, 0x5410u)};
+        for (int j = 0; j < 4; ++j) v[j] = (uint32_t)__float2int_rn(x[i][j] * up) + 0x80808080u;
+        const uint32_t low0 = prmt(v[0], v[1], 0x5140u), low1 = prmt(v[2], v[3], 0x5140u), top0 = prmt(v[0], v[1], 0x7362u), top1 = prmt(v[2], v[3], 0x7362u);
+        const uint32_t part[4] = {prmt(top0, top1, 0x7632u), prmt(top0, top1, 0x5410u), prmt(low0, low1, 0x7632u), prmt(low0, low1, 0x5410u)};
         static_assert(LINE % 8 == 0, "the parts of a vector are swizzled alike");
-        unsigned char* to = s_q + (r / LINE * (3 * LINE) + r % LINE) * kK8Hd + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3);
+        unsigned char* to = s_q + (r / LINE * (4 * LINE) + r % LINE) * kK8Hd + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(to + k * LINE * kK8Hd) = part[k] ^ 0x80808080u;
-        if (lane == 0) s_f[r] = at[i] < 0 ? 0.0f : bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 21u) << 23) * (0.08838834764831845f * 1.4426950408889634f);
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint32_t*>(to + k * LINE * kK8Hd) = part[k] ^ 0x80808080u;
+        if (lane == 0) s_f[r] = at[i] < 0 ? 0.0f : bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 29u) << 23) * (0.08838834764831845f * 1.4426950408889634f);
     }
 }
 
@@ -397,22 +392,18 @@ struct TreeMask {
 template <int R>
 __device__ __forceinline__ void tr_arguments(uint32_t tmem, const float* s_f, const float* s_down, float sk, f32x2 (&w)[8]) {
     const f32x2 sk2 = pack2(sk, sk);
-    uint32_t high[2][8], mid[2][8], low[2][8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        tr_ld8(tmem + 8 * h, high[h]);
-        tr_ld8(tmem + R + 8 * h, mid[h]);
-        tr_ld8(tmem + 2 * R + 8 * h, low[h]);
-    }
-    tr_wait8(high[0]);
-    tr_tie8(mid[0]); tr_tie8(low[0]); tr_tie8(high[1]); tr_tie8(mid[1]); tr_tie8(low[1]);
+        uint32_t part[4][8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+        for (int k = 0; k < 4; ++k) tr_ld8(tmem + k * R + 8 * h, part[k]);
+        tr_wait8(part[0]);
+        tr_tie8(part[1]); tr_tie8(part[2]); tr_tie8(part[3]);
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
             const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + 8 * h + j), m = *reinterpret_cast<const ulonglong2*>(s_down + 8 * h + j);
-            w[4 * h + j / 2] = tr_fma2(tr_whole(high[h] + j, mid[h] + j, low[h] + j), tr_mul2(sk2, f.x), m.x);
-            w[4 * h + j / 2 + 1] = tr_fma2(tr_whole(high[h] + j + 2, mid[h] + j + 2, low[h] + j + 2), tr_mul2(sk2, f.y), m.y);
+            w[4 * h + j / 2] = tr_fma2(tr_whole(part[0] + j, part[1] + j, part[2] + j, part[3] + j), tr_mul2(sk2, f.x), m.x);
+            w[4 * h + j / 2 + 1] = tr_fma2(tr_whole(part[0] + j + 2, part[1] + j + 2, part[2] + j + 2, part[3] + j + 2), tr_mul2(sk2, f.y), m.y);
         }
     }
 }
@@ -467,7 +458,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, tile = (int)blockIdx.x % L.tiles, share = (int)blockIdx.x / L.tiles, flat0 = tile * R;
     unsigned char* base = tr_smem + (((smem_addr(tr_smem) + 1023u) & ~1023u) - smem_addr(tr_smem));
     unsigned char *s_q = base + S::stages * 2 * kTrTileBytes, *s_p = s_q + S::q_bytes;
-    float* s_scales = reinterpret_cast<float*>(s_p + S::p_bytes);
+    float *s_scales = reinterpret_cast<float*>(s_p + S::p_bytes), *s_kept = s_scales + S::stages * 2 * kTrTile;
     enum { kScores, kFree, kWeights, kValues };          // a line's scores are there; were read; weights are there; their products are done
     if (tid == 0) {
         for (int i = 0; i < 2 * S::stages; ++i) {
@@ -559,8 +550,10 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
         const int line = first / S::line, in_line = first % S::line;
         uint64_t* bar = s_bar[line];
         const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16), t_scores = t_lane + (uint32_t)(line * S::s_cols + in_line),
-                       t_values = t_lane + (uint32_t)(S::all_s + 4 * first), t_moved = t_lane + (uint32_t)(S::all_s + S::all_o + first);
-        tr_fill<16>(t_moved, 0u);
+                       t_values = t_lane + (uint32_t)(S::all_s + 4 * first);
+        // Outputs of dim `key` that were moved on, seldom looked at.
+        float* kept = s_kept + first * kTrTile + key;
+        volatile float kept_own[S::kept_shared ? 1 : 16];
         tr_fill<64>(t_values, 0u);
         tmem_wait_st();
         tc_fence_before();
@@ -602,21 +595,27 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
             f32x2 l[8];                                  // of key `key`: sums
 #pragma unroll
             for (int r = 0; r < 8; ++r) l[r] = 0;
+            bool has = false;                            // kept_own has something
+            if (S::kept_shared) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) kept[j * kTrTile] = 0.0f;
+            }
             // Eight queries' outputs of dim `key`: what was moved on, and the accumulators.
             auto moved = [&](int h, float unit, float (&o)[8]) {
-                uint32_t m[8];
-                tr_ld8(t_moved + h, m);
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     uint32_t v[8];
                     tr_ld8(t_values + 4 * (h + j), v);
                     tr_wait8(v);
-                    if (j == 0) tr_tie8(m);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const float hi = __fmaf_rn((float)(int)v[4 * k + 3], 256.0f, (float)(int)v[4 * k + 2]), lo = __fmaf_rn((float)(int)v[4 * k + 1], 256.0f, (float)(int)v[4 * k]);
-                        o[j + k] = __fmaf_rn(__fmaf_rn(hi, 65536.0f, lo), unit, __uint_as_float(m[j + k]));
+                        o[j + k] = __fmaf_rn(__fmaf_rn(hi, 65536.0f, lo), unit, S::kept_shared ? kept[(h + j + k) * kTrTile] : 0.0f);
                     }
+                }
+                if (has) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) o[j] += kept_own[S::kept_shared ? 0 : h + j];
                 }
             };
             const int total = walk.start + walk.count;
@@ -719,9 +718,12 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                             float o[8];
                             moved(h, unit.w, o);
 #pragma unroll
-                            for (int r = 0; r < 8; ++r) o[r] *= __shfl_sync(0xffffffffu, by, h + r);
-                            tr_st8(t_moved + h, o);
+                            for (int r = 0; r < 8; ++r) {
+                                o[r] *= __shfl_sync(0xffffffffu, by, h + r);
+                                if (S::kept_shared) kept[(h + r) * kTrTile] = o[r]; else kept_own[S::kept_shared ? 0 : h + r] = o[r];
+                            }
                         }
+                        has = !S::kept_shared;
                         tr_fill<64>(t_values, 0u);
                         tmem_wait_st();
                         tc_fence_before();
@@ -786,8 +788,7 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
                     if (to >= 0) out[key] = o[r] * by;
                 }
             }
-            tr_fill<16>(t_moved, 0u);                    // for the next pair
-            tr_fill<64>(t_values, 0u);
+            tr_fill<64>(t_values, 0u);                   // for the next pair
             tmem_wait_st();
             tc_fence_before();
         }
@@ -883,7 +884,7 @@ struct WeighShape {
     static constexpr int groups = R / 16, warps = R / 4, threads = (warps + 2) * 32, stages = R == 16 ? 3 : 4, resident = R == 16 ? 3 : 1;
     static constexpr bool direct = groups == 1;                       // a key has one thread: its sums go to its weight at once
     static constexpr int most = direct ? 1 << 30 : 128 / groups, rows_most = direct ? stages : most + 2 * stages;
-    static constexpr int s_cols = 3 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;         // two sets of scores
+    static constexpr int s_cols = 4 * R, tmem_cols = R > 32 ? 512 : R == 32 ? 256 : 128;         // two sets of scores
     static constexpr int q_bytes = s_cols * kK8Hd;
     static constexpr size_t smem = 1024 + (size_t)stages * kTrTileBytes + q_bytes + stages * 2 * kTrTile * 4 + (direct ? 0 : groups * most * kTrTile * 4);
 };

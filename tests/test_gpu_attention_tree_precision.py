@@ -1,4 +1,5 @@
-"""How good attention over drafted trees is where the numbers are of unlike sizes: values' scales far apart, keys that have most of the weight and small values. Against 64 bits, by the norm of each head's output.
+"""How good attention over drafted trees is where the numbers are of unlike sizes: values' scales far apart, keys that have most of the weight and small values, queries with single large dims. Against
+64 bits, by the norm of each head's output.
 
 The tolerance counts roundings. An argument of the exponential (s, natural units) is a product of four factors, each rounded once to fp32 (2^-24), minus a reference and plus a scale's logarithm, rounded once
 as it is (w, in halvings), and the exponential is off by 2^-22: together d = 2^-24 (3 |s| + |w| + 4 + 4) at most, which moves a weight by itself and all others by way of the sum: 2 d, for the largest |s| and |w|
@@ -108,6 +109,29 @@ def test_one_key_apart_from_all_others(cuda_lib, nodes, n_q, place, above, value
     case.c.sk[b, 0, 0, o] = np.float32(abs(above) / 100 / np.sqrt(128))
     case.c.sv[b, 0, 0, o] *= np.float32(value)
     check(case)
+
+
+@pytest.mark.parametrize("dim,times,there", [(3, 100, 0.05), (64, 1000, 0.0), (127, 30, 1.0), (0, 1e5, 0.0)])
+@pytest.mark.parametrize("nodes,n_q,n_kv", [(1, 4, 1), (9, 8, 2), (33, 6, 3), (64, 4, 1)])
+def test_queries_with_one_large_dim(cuda_lib, nodes, n_q, n_kv, dim, times, there):
+    """Where the keys are small, the other dims decide."""
+    case = Case(nodes + dim, [2000], [nodes], nodes, n_q, n_kv, rotated=False, scale=1.0)
+    q = case.q.reshape(nodes, n_q, 128)
+    q[:, :, dim] = times * np.sign(q[:, :, dim])
+    case.c.k[..., dim] = np.rint(case.c.k[..., dim] * there)
+    check(case)
+
+
+@pytest.mark.parametrize("step", [0.02, 0.5, 6.0])
+def test_growing_scores_and_scales(cuda_lib, step):
+    """The largest argument moves on from tile to tile, values' scales grow or fall meanwhile."""
+    for ratio in (1.5, 1 / 1.5):
+        case = Case(7, [1300], [16], 16, 20, 5, rotated=False, masked=False)
+        b, o = case.c.at(0, np.arange(1316))
+        case.c.k[b, 0, :, o] = np.sign(case.q[3].reshape(5, 4, 128)[:, 0]).astype(np.int8) * 20
+        case.c.sk[b, 0, :, o] = (0.02 * step * (1 + np.arange(1316) // 100) * (1 + 0.01 * np.random.default_rng(3).random(1316)))[:, None]
+        case.c.sv[b, 0, :, o] = (0.001 * ratio ** (np.arange(1316) // 90))[:, None]
+        check(case)
 
 
 def test_scales_of_zero(cuda_lib):
