@@ -381,116 +381,7 @@ TENZO_API int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* str
  *   lse = log sum exp of the arguments (natural logarithm; -infinity and zeros in out where nothing is seen).
  * Sums and softmax in fp32 or whole numbers; the query is rounded to 2^-30 of its head's largest number, a weight times its value's scale to 2^-26 of the largest such product that the row
  * had met when it was last looked for: outputs agree with 64 bits as plain fp32 does, to about 1e-6 of their norm with arguments of ordinary size. (What an argument may be off by is some 2^-22 of itself, and 2^-30 of the
- * query's largest number times the key's sum of magnitudes / sqrt(128).) Scales of values are within 2^60 of each other where rows see them, and from 2^-60 on; smaller ones count as 0. A NaN or an infinity in a head's query makes that head's output NaN. */
-typedef struct {
-    const float* q;          /* [rows][q_stride], n_q*128 used, before rotation */
-    float* out;              /* [rows][n_q*128] */
-    tenzo_kv4_cache cache;
-    const int* pos;          /* [rows] device */
-    const int* seq;          /* [rows] device, or NULL */
-    const float* rope_cos; const float* rope_sin;   /* [rope_len][64], rope_len >= max_len; both NULL: no rotation */
-    int rope_len;
-    int q_stride;            /* floats between rows; 0 = n_q*128 */
-    int layer, n_q, rows;
-    int max_len;             /* upper bound on pos + 1 (sizes the grid); at most 16 * table_stride */
-    int split_keys;          /* keys a CTA takes (rounded up to 128); 0 = choose */
-    int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
-    void* workspace;         /* 16-byte aligned, contents need not be kept: partial results of splits; NULL: none */
-    size_t workspace_bytes;  /* rows * n_q * 520 a split; with less fewer splits are taken, and split_keys that need more are refused (-1). Enough for any split_keys:
-                                tenzo_cuda_attention_kv4_workspace_bytes(...); for split_keys 0: 520 * rows * n_q * tenzo_cuda_attention_kv4_splits(...), nothing at 1 */
-} tenzo_attention_kv4_args;
-TENZO_API int tenzo_cuda_attention_kv4(const tenzo_attention_kv4_args* args, void* stream);
-TENZO_API size_t tenzo_cuda_attention_kv4_workspace_bytes(int rows, int n_q, int n_kv, int max_len);
-/* Splits that the call's own choice (split_keys 0) wants room for; 1: none, 0: arguments that the call refuses. */
-TENZO_API int tenzo_cuda_attention_kv4_splits(int rows, int n_q, int n_kv, int max_len);
-/* Error flags of the calls above and below this one since the last call (bit 0: a bounded wait was given up, bit 1: an index out of range);
- * -1 if the query failed, which leaves the flags as they are. Synchronises with the device: waits for all of its streams, so it cannot be called while one is
- * captured. */
-TENZO_API int tenzo_cuda_kv4_take_errors(void);
-
-/* The cache's half of a beam-search step. Table rows g*beams .. g*beams + beams - 1 are the beams of group g and hold length[g] tokens each; beam i goes
- * on from beam parent[g*beams + i] (0 .. beams - 1). With j = length / 16 and r = length % 16, row i of table_out gets its parent's entries below j (full
- * blocks are shared) and its own above j. The block being filled, entry j if r > 0, belongs to one beam alone (they must differ): the first child of a
- * parent takes its parent's; the n-th of the further children, by index, takes that of the n-th beam without children, and the r filled slots of all layers and heads are copied
- * into it. If r = 0, entry j stays the beam's own. No block is allocated or freed, and a prompt is forked the same way: parent 0 for
- * all. table_out [groups*beams][table_stride] must not overlap the table (-1); groups*beams = table_rows, beams <= TENZO_BEAMS_MOST and
- * n_layers*n_kv <= 16384 (-5 otherwise). A group with a parent or a length out of range is copied as it is and raises the flag. */
-enum { TENZO_BEAMS_MOST = 32 };
-TENZO_API int tenzo_cuda_kv4_reorder(const tenzo_kv4_cache* cache, int* table_out, const int* parent, const int* length, int groups, int beams, int use_pdl,
-                                     void* stream);
-
-/* ---- beam search: the k best continuations over beams x vocabulary -----------------------------------------
- * Beside the greedy argmax and the sampler (:1722-1807); the reference has no beam search. logits [groups*beams][row_stride] fp32,
- * scores [groups*beams] the beams' sums of log-probabilities. Per group, over all beams b and tokens t,
- *   score(b, t) = scores[b] + (x_t - log sum_u exp x_u)   in 64 bits
- * (exponentials other than the largest ones' enter the sum with 32: its logarithm is good to some 1e-7, to 2e-6 at the worst),
- * the k best go to parent_out / token_out / score_out [groups][k], best first; of equal scores the lower beam, in a beam the larger logit, then the
- * lower token. score_out is rounded to fp32.
- * A finished beam (finished[row] != 0) has its end token `eos` alone, at scores[b]. -inf masks a token; NaN counts as -inf, +inf as the largest finite
- * number. A beam with score -inf or NaN, or with no token left, has score -inf for every token (chosen only when nothing else is left, lowest index
- * first). beams <= TENZO_BEAMS_MOST and k <= 2 * TENZO_BEAMS_MOST (-5 otherwise); k <= beams * vocab. */
-typedef struct {
-    const float* logits;
-    const float* scores;
-    const int* finished;     /* [groups*beams] device, or NULL */
-    int eos;                 /* used with `finished` only */
-    int row_stride;          /* floats between rows of logits; 0 = vocab */
-    int groups, beams, vocab, k;
-    int use_pdl;
-    int* parent_out; int* token_out; float* score_out;
-    void* workspace;         /* tenzo_cuda_beam_select_workspace_bytes(...) bytes, 16-byte aligned, contents need not be kept */
-    size_t workspace_bytes;
-} tenzo_beam_select_args;
-TENZO_API int tenzo_cuda_beam_select(const tenzo_beam_select_args* args, void* stream);
-TENZO_API size_t tenzo_cuda_beam_select_workspace_bytes(int groups, int beams, int vocab, int k);
-
-/* ---- INT8 caches: drafted trees, and caches of a bounded number of tokens ---------------------------------
- * No counterpart in the reference, which decodes one token at a time and keeps every token. The caches are those of tenzo_cuda_attention_int8: int8
- * [block][n_layers][n_kv][slots][128] for keys and for values and fp32 scales [block][n_layers][n_kv][slots] (a value is code * scale). The token at place t of table
- * row s lies in block block_table[s * table_stride + t / slots], slot t % slots; slots is a multiple of 16. The paged_int8 pools have 16 slots; the contiguous
- * cache [sequence][layer][kv_head][max_seq][128] is a pool of max_seq slots a block whose table has one entry a sequence. Caches and scales are 16-byte aligned and
- * hold fewer than 2^31 rows; scales are not negative. head_dim is 128.
- *
- * Here a token's place is not its rotary position: nodes of a tree that lie side by side have the same position, and behind an eviction positions and places
- * come apart for good. Calls that rotate take both.
- * An index out of range (a place, a position, a table row or entry, a length) touches no memory: that row is left out and a flag is raised, which
- * tenzo_cuda_kv8_take_errors() returns and clears. Calls on one device share the flags only. */
-typedef struct {
-    int8_t* k; int8_t* v;
-    float* scale_k; float* scale_v;
-    int n_blocks, n_layers, n_kv, slots;
-    const int* block_table;  /* device int32 [table_rows][table_stride] */
-    int table_rows, table_stride;
-} tenzo_kv8_cache;
-enum { TENZO_TREE_MOST = 256 };  /* nodes of a tree */
-
-/* Stores `rows` rows of keys and values: k, v [rows][kv_stride] fp32 (n_kv*128 used, kv_stride >= n_kv*128), row i at place place[i] of table row seq[i]
- * (seq NULL: table row i). place[i] < 0 marks padding: nothing is stored. No two rows of a call may name the same token. Keys are rotated at rope_pos[i] (NULL: place[i];
- * tables [rope_len][64], position < rope_len; both NULL: no rotation) as tenzo_cuda_attention_int8 does, then both are quantised: scale = max(max|x|, 1e-8) * (1/127),
- * code = clamp(round(x * (1 / scale)), -128, 127), halves away from zero, each step rounded to fp32. (tenzo_cuda_attention_int8 divides by 127: its scales may differ in
- * the last bit, and a code next to a border by one.) Values have to be finite.
- * weight, position (either may be NULL), laid out as the scales: receive 0 and the row's rotary position, for the calls below. */
-typedef struct {
-    tenzo_kv8_cache cache;
-    const float* k; const float* v;                 /* [rows][kv_stride] */
-    const int* place;                               /* [rows] device */
-    const int* seq; const int* rope_pos;            /* [rows] device, or NULL */
-    const float* rope_cos; const float* rope_sin;   /* [rope_len][64], 16-byte aligned; both NULL: no rotation */
-    float* weight; int* position;                   /* or NULL */
-    int layer, kv_stride, rows, rope_len;
-    int use_pdl;
-} tenzo_kv8_append_args;
-TENZO_API int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* stream);
-
-/* Attention of the nodes of a tree, for each of `sequences` trees of up to `nodes` nodes (1 .. TENZO_TREE_MOST): sequence s holds start[s] tokens, and node i's key and
- * value are stored at place start[s] + i already. Node i sees places 0 .. start[s] - 1, and node j if bit j % 32 of mask[(s*nodes + i)*mask_stride + j / 32] is
- * set (itself too: any bits will do). mask NULL: nodes 0 .. i, a chain (a prompt's next rows, one decoded token with nodes = 1). count[s] (NULL: nodes): nodes that
- * are there; the others are padding, are seen by none, and their rows of out are zeros. start[s] < 0: the whole sequence is padding.
- *   out[s*nodes + i] = softmax(q K^T / sqrt(128)) V per query head h, over kv head h / (n_q / n_kv), the query rotated at rope_pos[s*nodes + i] (NULL: start[s] + i);
- *   lse = log sum exp of the arguments (natural logarithm; -infinity and zeros in out where nothing is seen).
- * Sums and softmax in fp32 or whole numbers; the query is rounded to 22 bits and a sign of its head's largest number, a weight times its value's scale to 26 bits of the largest such product that the row
- * had met when it was last looked for: outputs agree with 64 bits to about 1e-6 of their norm where no dim of a query is far larger than the others (2^-22 of the largest number, times the key's sum of magnitudes, is
- * what the argument may be off by), with scales of values up to 2^60 apart and from 2^-60 on. A NaN or an infinity in a head's query makes that head's outputs NaN; what lies in places that are not seen has no part.
+ * query's largest number times the key's sum of magnitudes / sqrt(128).) Scales of values are within 2^60 of each other where rows see them, and from 2^-60 on; smaller ones count as 0. A NaN or an infinity in a head's query makes that head's outputs NaN; what lies in places that are not seen has no part.
  * A sequence with start + count > max_len or a table row out of range, and a row whose position is, are not written and raise the flag; a table entry out
  * of range leaves its block's keys out and raises it. */
 typedef struct {
