@@ -404,7 +404,7 @@ typedef struct {
     int use_pdl;             /* launch with programmatic stream serialisation; nothing is read before the wait for the kernel in front */
     void* workspace;         /* 16-byte aligned, contents need not be kept, of one call at a time (two graphs that may run together have two): partial results where a
                                 cut goes through a sequence's keys */
-    size_t workspace_bytes;  /* tenzo_cuda_attention_tree_workspace_bytes(...), some MB whatever the lengths are. With less, or NULL, shares end with a sequence's kv head, which is
+    size_t workspace_bytes;  /* tenzo_cuda_attention_tree_workspace_bytes(...), with shares = 0 10 MB and 8 bytes a sequence and kv head at most, whatever the lengths are. With less, or NULL, shares end with a sequence's kv head, which is
                                 slower for few sequences and for unequal ones; shares > 0 is refused then (-1). With
                                 shares = 0 it is not used where max_len <= 512 */
 } tenzo_attention_tree_args;

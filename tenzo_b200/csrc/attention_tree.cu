@@ -1116,10 +1116,11 @@ static void tree_plan(TreeLaunch& L) {
     L.tiles = (int)((queries + r - 1) / r);
     L.shares = a.shares > 0 ? a.shares : L.tiles < places ? places / L.tiles : 1;
 }
+// Bytes for what cuts leave: nothing is cut where there is one share, as with queries for half of the SMs and more (a few bytes all the same: 0 is the answer to arguments that are refused).
 static size_t tree_room(const TreeLaunch& L) {
     const int r = tree_queries_a_cta((long long)L.a.nodes * L.group);
     const size_t head = ((size_t)L.a.sequences * L.a.cache.n_kv * sizeof(int2) + 15) & ~(size_t)15;
-    return head + (size_t)L.shares * L.tiles * 2 * r * (kK8Hd + 2) * sizeof(float);
+    return head + (L.shares == 1 ? 16 : (size_t)L.shares * L.tiles * 2 * r * (kK8Hd + 2) * sizeof(float));
 }
 
 template <int R>
@@ -1176,7 +1177,7 @@ extern "C" int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, 
     if (a.shares > 0 && !L.cut) return -1;
     // Up to four tiles are not cut: what the cut saves the second kernel takes again (8 nodes, 500 keys: one sequence 13.5 us whole, 13.4 cut, 16 17.3 and 18.5, 64 29.5 and 35.0; 1000 keys: 17.8 and
     // 13.2, 24.2 and 26.7, 43.4 and 44.0; 64 nodes, one sequence of 500: 17.2 and 15.6), and the call is one launch.
-    if (a.shares == 0 && a.max_len <= 4 * kTrTile) L.cut = 0;
+    if (L.shares == 1 || (a.shares == 0 && a.max_len <= 4 * kTrTile)) L.cut = 0;
     if ((long long)L.shares * L.tiles > 0x7fffffffLL || (long long)a.sequences * a.nodes > 0x7fffffffLL) return -5;
     const int r = tree_queries_a_cta((long long)a.nodes * L.group);
     L.head = static_cast<int2*>(a.workspace);
