@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import subprocess
 import sys
 from pathlib import Path
@@ -24,6 +25,20 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-fmad=false", "-Xcompiler", "-fPIC,-fvisibility=hidden,-O2", "-Xptxas", "-v",
 ]
+
+
+# Kernels whose warps hand registers to one another by fixed numbers (setmaxnreg): registers a thread that each has to be launched with, and may be. With others its launches
+# would be refused, so the build is.
+LAUNCHED_REGISTERS = {"attention_tree_kernelILi64E": (96, 112), "attention_tree_kernelILi48E": (128, 144), "attention_tree_kernelILi32E": (80, 104), "attention_tree_kernelILi16E": (128, 168)}
+
+
+def check_registers(log: str) -> None:
+    """Raises where ptxas gave one of LAUNCHED_REGISTERS another number, or `log` does not name it."""
+    for kernel, (least, most) in LAUNCHED_REGISTERS.items():
+        used = re.search(rf"Compiling entry function '[^']*{kernel}[^']*'.*?Used (\d+) registers", log, re.S)
+        if not used or not least <= -(-int(used[1]) // 8) * 8 <= most:
+            raise RuntimeError(f"{kernel} has to have {least} to {most} registers a thread, and this compiler gave it {used[1] if used else 'none that it says'}: "
+                               "the numbers that its warps hand on (TreeShape in attention_tree.cu, and here) have to be set anew")
 
 
 def nvcc_path() -> str:
@@ -63,6 +78,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             raise RuntimeError(f"nvcc failed on {src}")
         objs.append(str(obj))
     (PKG / "lib" / "ptxas.log").write_text("\n".join(log))
+    check_registers("\n".join(log))
     if verbose:
         print("\n".join(log))
     link = [nvcc, "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", str(LIB), *objs, "-cudart", "static"]

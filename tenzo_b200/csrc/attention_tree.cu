@@ -59,6 +59,7 @@ struct TreeShape {
     // Registers a thread: as the block is launched, and after the warps of the second line have given some to those of the first.
     static constexpr int launched = R == 64 ? 96 : R == 48 ? 128 : R == 32 ? 80 : 128, most = R == 64 ? 112 : R == 48 ? 144 : R == 32 ? 104 : 168, least = R == 48 ? 40 : R == 16 ? 64 : 32;
     static_assert(warps * most + 4 * least <= (warps + 4) * launched, "what is taken is there");
+    static_assert(launched == 65536 / (threads * resident) / 8 * 8, "as many as the launch bounds leave, which the compiler takes where warps hand registers on; the build checks that it has");
     static constexpr int p_panels = R > 32 ? 2 : 1;                   // of 128 bytes: 32 queries
     static constexpr int q_bytes = all_s * kK8Hd, p_bytes = p_panels * kTrTileBytes;
     static constexpr bool kept_shared = R != 32;                      // outputs that were moved on lie in shared memory; of two CTAs of 32 queries there is no room for them, and they are the threads' own
@@ -1126,10 +1127,10 @@ static size_t tree_room(const TreeLaunch& L) {
 template <int R>
 static int tree_run(const TreeLaunch& L, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
     if (cudaError_t e = allow_smem(attention_tree_kernel<R>, TreeShape<R>::smem)) return (int)e;
-    // With fewer registers than the warps ask of one another they would wait for good; the kernel's number is the compiler's.
+    // With fewer registers than the warps ask of one another they would wait for good; the kernel's number is the compiler's. (Registers are given out by eights.)
     static const bool registers_ok = [] {
         cudaFuncAttributes f = {};
-        return cudaFuncGetAttributes(&f, attention_tree_kernel<R>) == cudaSuccess && f.numRegs == TreeShape<R>::launched;
+        return cudaFuncGetAttributes(&f, attention_tree_kernel<R>) == cudaSuccess && (f.numRegs + 7) / 8 * 8 >= TreeShape<R>::launched && f.numRegs <= TreeShape<R>::most;
     }();
     if (!registers_ok) return (int)cudaErrorLaunchOutOfResources;
     return kv4_launch(attention_tree_kernel<R>, dim3((unsigned)(L.shares * L.tiles)), TreeShape<R>::threads, TreeShape<R>::smem, st, L.a.use_pdl != 0, L, kmap, vmap);
