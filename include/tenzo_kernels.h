@@ -414,6 +414,8 @@ TENZO_API size_t tenzo_cuda_attention_tree_workspace_bytes(int sequences, int no
 
 /* The attention weight that each cached token receives: weight[token] += sum over the nodes that see it and the query heads of its kv head of exp(s - lse), s the
  * argument of softmax above. args as for tenzo_cuda_attention_tree, whose lse this reads; out, workspace and shares are not used. weight is laid out as the scales.
+ * All nodes count, also those of a draft that are refused later. To leave these out, call it behind tenzo_cuda_kv8_accept for the accepted ones, whose rows are a chain there: q, lse and rope_pos
+ * gathered by path (anything where that is -1), count = accepted, mask NULL, start as it was; nodes and the arrays may be as long as before.
  * A row whose lse is not finite adds nothing; weights and sums below 2^-126 may count as 0. Every sum is taken in one order: equal calls give equal bits. No two sequences of a call may name
  * the same table row, or blocks in common (a token would lose what one of them adds); attention reads common blocks as well as others. */
 TENZO_API int tenzo_cuda_kv8_weigh(const tenzo_attention_tree_args* args, float* weight, void* stream);

@@ -531,7 +531,8 @@ def attention_tree(q, cache, start, *, layer, n_q, nodes, count=None, mask=None,
 
 def kv8_weigh(q, lse, cache, weight, start, *, layer, n_q, nodes, count=None, mask=None, seq=None, rope_pos=None, rope_cos=None, rope_sin=None, max_len=None, use_pdl=False):
     """Adds to weight (fp32, of the scales' shape) what each cached token received in attention_tree of the same arguments, whose lse [rows, n_q] this reads: the sum of
-    softmax's results over the nodes and the query heads of a kv head."""
+    softmax's results over the nodes and the query heads of a kv head. Nodes that are refused later count like others; to leave them out, call it behind kv8_accept for the accepted ones,
+    which are a chain there: q, lse and rope_pos gathered by its path (anything where that is -1), count=accepted, no mask, the same start."""
     dev = _current_device()
     qp, rows, _, scales, fields = _tree_fields(q, cache, start, layer, n_q, nodes, count, mask, seq, rope_pos, rope_cos, rope_sin, max_len, dev)
     if lse.shape != (rows, n_q):
