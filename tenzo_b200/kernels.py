@@ -452,9 +452,9 @@ def _arg_int(value: int, what: str) -> int:
 
 
 def kv8_append(k, v, cache, place, *, layer, seq=None, rope_pos=None, rope_cos=None, rope_sin=None, weight=None, position=None, use_pdl=False):
-    """Rotates the rows k [n, n_kv*128] at rope_pos int32 [n] (default: place), quantises k and v as attention_int8 does, and stores them at places place int32 [n] of the
-    sequences seq int32 [n] (default: row i is sequence i). A negative place marks a padding row, for which nothing is stored. weight fp32 and position int32, of the
-    scales' shape, receive 0 and the rotary position."""
+    """Rotates the rows k [n, n_kv*128] at rope_pos int32 [n] (default: place), quantises k and v to int8, and stores them at places place int32 [n] of the
+    sequences seq int32 [n] (default: row i is sequence i). A scale is max|x| * (1/127), where attention_int8 divides by 127: scales may differ from its own in the last bit, and a code next to a
+    border by one. A negative place marks a padding row, for which nothing is stored. weight fp32 and position int32, of the scales' shape, receive 0 and the rotary position."""
     dev = _current_device()
     fields, scales = _kv8_cache(cache, dev)
     n_kv = fields[6]
