@@ -478,8 +478,10 @@ attention_tree_kernel(const TreeLaunch L, const __grid_constant__ CUtensorMap km
     if (warp == S::warps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        // Kernels behind this one may come in only when the block has its tensor memory: one that allocates all of it, and then waits for this one, would otherwise be waited for by the allocation above
+        // where the kernel in front still holds some. (The second kernel waits for this one whatever its neighbours do.)
+        if (a.use_pdl || L.cut) pdl_launch_dependents();
     }
-    if (a.use_pdl || L.cut) pdl_launch_dependents();     // (the second kernel waits for this one whatever its neighbours do)
     if (a.use_pdl) pdl_wait();
     tc_fence_before();
     const TreeShareAt at = tr_share<S::threads>(L, share, s_scan, s_found);
@@ -924,11 +926,9 @@ __global__ void __launch_bounds__(WeighShape<R>::threads, WeighShape<R>::residen
     if (warp == S::warps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (a.use_pdl) pdl_launch_dependents();          // (as in the attention: only with the block's tensor memory)
     }
-    if (a.use_pdl) {
-        pdl_launch_dependents();
-        pdl_wait();
-    }
+    if (a.use_pdl) pdl_wait();
     tc_fence_before();
     const TreeShareAt at = tr_share<S::threads>(L, (int)blockIdx.x, s_scan, s_found);
     __syncthreads();
