@@ -1176,8 +1176,10 @@ extern "C" int tenzo_cuda_attention_tree(const tenzo_attention_tree_args* args, 
     tree_plan(L);
     L.cut = a.workspace && kv8_aligned(a.workspace, 16) && a.workspace_bytes >= tree_room(L);
     if (a.shares > 0 && !L.cut) return -1;
-    // Up to four tiles are not cut: what the cut saves the second kernel takes again (8 nodes, 500 keys: one sequence 13.5 us whole, 13.4 cut, 16 17.3 and 18.5, 64 29.5 and 35.0; 1000 keys: 17.8 and
-    // 13.2, 24.2 and 26.7, 43.4 and 44.0; 64 nodes, one sequence of 500: 17.2 and 15.6), and the call is one launch.
+    // Up to four tiles are not cut, and the call is one launch: what the cut saves the second kernel takes again. Whole and cut, 20 heads over 5, us: 8 nodes, 500 keys, one sequence 13.4 and 12.4, 16
+    // sequences 18.2 and 19.6, 64 33.3 and 37.2; 64 nodes 17.2 and 17.8, 41.6 and 49.5, 120 and 157. Beyond that the rule goes by one sequence, which gains most (1000 keys: 19.6 and 12.7, 22.6 and 19.4);
+    // many sequences of some eight tiles are slower cut (8 nodes: 16 sequences 25.2 and 28.6, 64 46.5 and 45.9; 64 nodes: 58.5 and 61.9, 168 and 204; of 2000 keys 38.2 and 32.4, 72.1 and 62.5, 91.2
+    // and 90.6, 265 and 298): a call without a workspace leaves them whole.
     if (L.shares == 1 || (a.shares == 0 && a.max_len <= 4 * kTrTile)) L.cut = 0;
     if ((long long)L.shares * L.tiles > 0x7fffffffLL || (long long)a.sequences * a.nodes > 0x7fffffffLL) return -5;
     const int r = tree_queries_a_cta((long long)a.nodes * L.group);
