@@ -11,10 +11,10 @@
 //     Both are avoided: a row's weights are taken relative to a reference, set so that the largest product of weight and scale is 1, and these products may grow to 2^5. Only where one would pass
 //     that (one vote a tile; the first tile always) the references are set anew and the accumulators moved on into fp32. The reference goes by the product, which a thread has as a sum with its scale's
 //     logarithm, and by the row's own keys: neither a key of most weight and small values, as a first token often is, nor one of large values that others see leaves a row fewer bits.
-//   * Bound: single tokens by the bytes (64 sequences of 8192 keys, 20 heads over 5: 118 us on the device, 106 at the memory's measured rate), trees by the instructions of the warps that make
-//     weights, some 415 for 32 keys and sixteen queries (16 trees of 64 nodes, 8192 keys: 227 us, 2600 cycles a tile of 64 queries, 64 % of the issue slots; tensor cores 32 %, memory 10 %); small
-//     calls by the chain share, queries, tile, outputs, join (8 nodes, 1000 keys: 13.4 us). Going on to the next pair takes some 9000 cycles, 4300 of them 64 queries'.
-//     The same 64 queries as one line of 64, whose products wait for all warps, took 282 us, plain fp32 instead of packed pairs 248.
+//   * Bound (times of calls back to back in a graph): single tokens by the bytes (64 sequences of 8192 keys, 20 heads over 5: 120 us, 106 at the memory's measured rate), trees by the instructions of the
+//     warps that make weights, some 470 for 32 keys and sixteen queries with all that lies around them (16 trees of 64 nodes, 8192 keys: 235 us, 66 % of the issue slots; tensor cores 36 %, memory 11 %);
+//     small calls by the chain share, queries, tile, outputs, join (8 nodes, 1000 keys: 12.7 us). Going on to the next pair takes some 9000 cycles, half of them 64 queries'.
+//     With queries of three bytes, 227 us then: the same 64 queries as one line of 64, whose products wait for all warps, 282, plain fp32 instead of packed pairs 248.
 #include "attn_common.cuh"
 #include "kv8.cuh"
 #include "umma.cuh"
@@ -249,7 +249,7 @@ struct TreeWalk {
 // with. A vector is turned, scaled by a power of two to a maximum between 2^29 and 2^30 and rounded; its signed bytes are rows r, LINE + r, .., 3 LINE + r of its line's operand (128 bytes each, swizzled).
 // s_f: what a unit of the products with the codes counts in the argument of 2^x (NaN for a query that is not finite). from[r]: the vector in q, -1: none, zeros.
 // (Every load is made, of something, without a branch around it: where two ways meet the compiler copies what was loaded, and so waits for it. Bytes cut off one after another, by shifts, made the
-// weights of 4 x 250 nodes, which are mostly this, 178 us; like this 168.)
+// weights of 4 x 250 nodes, which are mostly this, 178 us, like this 168, with three bytes; with four 180.)
 template <int R, int LINE, bool VEC>
 __device__ __forceinline__ void tr_queries(const TreeLaunch& L, const long long* from, const int* pos, unsigned char* s_q, float* s_f) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -879,8 +879,8 @@ __global__ void __launch_bounds__(kTrMergeWarps * 32) attention_tree_merge_kerne
 // tile belongs to one CTA, a second pass's addition comes from the same thread behind the first: one order of summation). With more, four warps' sums of a key have to come together: they lie in
 // shared memory, for as many tiles at a time as there is room for, until all passes over these are done. Nothing holds the warps together but the scores, of which there are two sets.
 // Bound by the bytes of the keys for single tokens (64 sequences of 8192 keys, 5 kv heads: 69 us, 54 at the memory's rate), behind a start of some 14000 cycles; for trees by the
-// chain of a pass's queries (5000 cycles, which a CTA's few tiles do not hide: 7 x 33 nodes, 8 x 4 heads, 6001 keys: 50 us) and 1200 cycles a tile of 48 queries.
-// Measured: sums of single tokens in shared memory as well 42.5 us (64 x 4096 keys; at once 40.0); two CTAs an SM of 16 queries and four stages 70.5 (64 x 24 queries; three of three stages 67.2);
+// chain of a pass's queries (5000 cycles, which a CTA's few tiles do not hide: 7 x 33 nodes, 8 x 4 heads, 6001 keys: 52 us) and 1200 cycles a tile of 48 queries.
+// Measured, with queries of three bytes: sums of single tokens in shared memory as well 42.5 us (64 x 4096 keys; at once 40.0, with four bytes 38.8); two CTAs an SM of 16 queries and four stages 70.5 (64 x 24 queries; three of three stages 67.2);
 // 64 tiles a block instead of 128 at 48 queries 41.6 (32 x 48; 40.1); eight of sixteen queries left out where there are four: no difference.
 template <int R>
 struct WeighShape {
@@ -1081,7 +1081,7 @@ static int tree_check(TreeLaunch& L) {
     if (a.mask_stride == 0) a.mask_stride = words;
     if (a.mask_stride < words) return -1;
     L.group = a.n_q / a.cache.n_kv;
-    // (Vectors of four where all rows allow it: 16 trees of 64 nodes, 8192 keys, 222 us, by single numbers 225; their weights 145 and 154.)
+    // (Vectors of four where all rows allow it: 16 trees of 64 nodes, 8192 keys, 234 us, by single numbers 250; their weights 162 and 202.)
     L.aligned = kv8_aligned(a.q, 16) && a.q_stride % 4 == 0 && kv8_aligned(a.rope_cos, 16) && kv8_aligned(a.rope_sin, 16);
     return 0;
 }
@@ -1091,19 +1091,19 @@ static int tree_map(CUtensorMap* map, const tenzo_kv8_cache& c, const int8_t* co
 }
 
 // Queries a CTA of the attention: the width at which the CTAs that a tree's queries take cost least, one of 16, 32 and 48 as this much of one of 64. Measured, sequences x 4096 keys:
-// 64 x 24 queries 87 us at 32, 104 at 16, 119 at 48; 32 x 48: 71 at 48, 81 at 64, 85 at 32; 32 x 64: 83 at 64, 87 at 32; 32 x 80: 121 at 32, 126 at 48, 143 at 64; 16 x 128: 81 at
-// 64, 86 at 32; 16 x 144: 97 at 48, 104 at 32, 110 at 64; 4 x 1000: 147 at 64, 154 at 48, 156 at 32; and 64 x 4 queries of 8192 keys 122 at 16, 141 at 32.
+// 64 x 24 queries 91 us at 32, 103 at 16, 117 at 48; 32 x 48: 69 at 48, 80 at 64, 90 at 32; 32 x 64: 82 at 64, 92 at 32; 32 x 80: 123 at 48, 129 at 32, 142 at 64; 16 x 128: 79 at
+// 64, 89 at 32; 16 x 144: 95 at 48, 109 at 32 and 64; 4 x 1000: 144 at 64, 152 at 48, 163 at 32; and 64 x 4 queries of 8192 keys 121 at 16, 144 at 32.
 static int tree_queries_a_cta(long long queries) {
     constexpr int width[4] = {64, 48, 32, 16};
-    constexpr double cost[4] = {1.0, 0.80, 0.53, 0.32};
+    constexpr double cost[4] = {1.0, 0.80, 0.54, 0.32};
     int best = 0;
     for (int i = 1; i < 4; ++i)
         if (cost[i] * (double)((queries + width[i] - 1) / width[i]) < cost[best] * (double)((queries + width[best] - 1) / width[best])) best = i;
     return width[best];
 }
-// Queries a pass over the keys whose weights are summed, of which a CTA makes as many as there are: 16, twice if that is enough (64 sequences of 20 or 32 queries, 4096 keys: 62 and 63 us; in one of
-// 48, 75); then 48 (32 x 48: 41 us, three of 16 47, one of 64 49; 32 x 80: 69, 73 and 85) or 64, of which a pass of 48 costs 0.87 (32 x 64: 50 us at 64, 60 at 16, 72 at 48; 16 x 128: 48 at 64,
-// 58 at 48; 4 x 1000: 171 and 186).
+// Queries a pass over the keys whose weights are summed, of which a CTA makes as many as there are: 16, twice if that is enough (64 sequences of 20 or 32 queries, 4096 keys: 63 and 64 us; in one of
+// 48, 78); then 48 (32 x 48: 43 us, three of 16 48, one of 64 50; 32 x 80: 73, 75 and 88) or 64, of which a pass of 48 costs 0.87 (32 x 64: 51 us at 64, 62 at 16, 73 at 48; 16 x 128: 50 at 64,
+// 61 at 48; 4 x 1000: 180 and 195).
 static int weigh_queries_a_pass(long long queries) {
     if (queries <= 32) return 16;
     return 0.87 * (double)((queries + 47) / 48) < (double)((queries + 63) / 64) ? 48 : 64;

@@ -14,8 +14,8 @@ int* kv8_rows_flags() {
 // ---- append ----------------------------------------------------------------------------------------------------------------
 // A warp takes HB kv heads of one row: lanes 0-15 the keys, 16-31 the values, dims 4l .. 4l + 3 and 64 more a lane, so that the pairs that the rotation turns lie in one lane. Bound
 // by the bytes (5 of 6 read) in long calls and by the chain of loads (place, table, row) in short ones. Four heads a warp where there are warps enough: what names the row, its place in the
-// table and the rotation's coefficients are asked for once, and four times the bytes are on their way meanwhile (8000 rows of 8 heads: 19.0 us by fours, 26.6 by ones; of 4 heads 10.9 and 14.4;
-// 1600 rows of 8: 6.4 and 7.3; 1024: both 5.4; 512 rows of 5 heads: 3.9 and 3.2; 9000 rows of 2 heads: 9.3 and 9.1).
+// table and the rotation's coefficients are asked for once, and four times the bytes are on their way meanwhile (calls back to back in a graph; 8000 rows of 8 heads: 18.5 us by fours, 26.2 by ones; of 4 heads 10.3 and 13.9;
+// 1600 rows of 8: 6.1 and 7.2; 1024: 5.3 and 5.2; 512 rows of 5 heads: 4.2 and 3.5; 9000 rows of 2 heads: 9.3 and 9.0).
 constexpr int kK8RowWarps = 4;
 constexpr long long kK8Many = 148 * 64;                  // (row, head) pairs from which on a warp takes four heads: as many warps as the machine holds
 
@@ -194,10 +194,10 @@ __global__ void __launch_bounds__(kAcThreads) kv8_accept_kernel(const tenzo_kv8_
 // One CTA a (sequence, layer, kv head). The weights become whole numbers of the same order (the protected tokens' the largest) in shared memory; the `keep`-th largest is found by
 // counting, two bits a round, and only those in the range that is left once these are few; what stays is a bit a token; and the free places and the tokens that move into them are two lists, the i-th goes to the i-th.
 // Nothing that moves comes from a place that another moves to (those are below `keep`, these are not), so all rows move at once.
-// Bound by the chain of loads, counts and barriers where CTAs are few (150 heads of 2176 tokens: 17 us with the moves, all of it cold; 5.5 where nothing moves), by the rows' scattered pieces
-// (128 bytes of codes twice, four of four) where they are many: 64 x 20 heads of 4224 tokens 54 us, 32 without moves, 10.4 at the memory's rate.
-// T threads a CTA, 1024 / T CTAs an SM: 256, or 128 where there are more CTAs than that leaves room for at once and shared memory has room for eight an SM (64 x 20 heads of 4224 tokens: 38.3 us of
-// selection by 256, 32.3 by 128; 150 heads of 2176: 5.6 and 6.7; 512 threads, cold and with the moves: 100 and 30.7 us, where 256 take 63 and 22.5). Four loads in flight of numbers and of rows
+// Bound by the chain of loads, counts and barriers where CTAs are few (150 heads of 2176 tokens: 22 us with the moves, a single call with its launch, nothing in L2; 5.6 where nothing moves, in a graph), by the
+// rows' scattered pieces (128 bytes of codes twice, four of four) where they are many: 64 x 20 heads of 4224 tokens 57 us, 30 without moves, 10.4 at the memory's rate.
+// T threads a CTA, 1024 / T CTAs an SM: 256, or 128 where there are more CTAs than that leaves room for at once and shared memory has room for eight an SM (64 x 20 heads of 4224 tokens: 34.5 us of
+// selection by 256, 29.7 by 128; 150 heads of 2176: 5.6 and 6.7; 512 threads, cold and with the moves: 100 and 30.7 us, where 256 take 63 and 22.5). Four loads in flight of numbers and of rows
 // (cold, with the moves: two of numbers 61 and 23.4, eight 72 and 26.6; two of rows 70 and 24.6, eight 71 and 24.6).
 constexpr int kEvBatch = 4, kEvLoads = 4;
 constexpr int kEvHeld = 48 * 1024;                       // tokens whose numbers fit in shared memory
@@ -504,7 +504,7 @@ extern "C" int tenzo_cuda_kv8_append(const tenzo_kv8_append_args* args, void* st
     const int hb = a.cache.n_kv > 2 && (long long)a.rows * a.cache.n_kv > kK8Many ? 4 : 1;
     const long long ctas = ((long long)a.rows * ((a.cache.n_kv + hb - 1) / hb) + kK8RowWarps - 1) / kK8RowWarps;
     if (ctas > 0x7fffffffLL) return -5;
-    // Vectors of four where all rows allow it: 8000 rows of 8 heads 16.4 us, by single numbers 21.8.
+    // Vectors of four where all rows allow it: 8000 rows of 8 heads 18.5 us, by single numbers 22.6.
     const bool vec = kv8_aligned(a.k, 16) && kv8_aligned(a.v, 16) && a.kv_stride % 4 == 0;
     auto kernel = hb == 4 ? (vec ? kv8_append_kernel<true, 4> : kv8_append_kernel<false, 4>) : (vec ? kv8_append_kernel<true, 1> : kv8_append_kernel<false, 1>);
     return kv4_launch(kernel, dim3((unsigned)ctas), kK8RowWarps * 32, 0, static_cast<cudaStream_t>(stream), a.use_pdl != 0, a);
