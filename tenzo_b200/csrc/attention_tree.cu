@@ -1092,10 +1092,11 @@ static int tree_map(CUtensorMap* map, const tenzo_kv8_cache& c, const int8_t* co
 
 // Queries a CTA of the attention: the width at which the CTAs that a tree's queries take cost least, one of 16, 32 and 48 as this much of one of 64. Measured, sequences x 4096 keys:
 // 64 x 24 queries 91 us at 32, 103 at 16, 117 at 48; 32 x 48: 69 at 48, 80 at 64, 90 at 32; 32 x 64: 82 at 64, 92 at 32; 32 x 80: 123 at 48, 129 at 32, 142 at 64; 16 x 128: 79 at
-// 64, 89 at 32; 16 x 144: 95 at 48, 109 at 32 and 64; 4 x 1000: 144 at 64, 152 at 48, 163 at 32; and 64 x 4 queries of 8192 keys 121 at 16, 144 at 32.
+// 64, 89 at 32; 16 x 144: 95 at 48, 109 at 32 and 64; 4 x 1000: 144 at 64, 152 at 48, 163 at 32; and 64 x 4 queries of 8192 keys 121 at 16, 144 at 32. (80 queries take 32: short
+// sequences pay for a change of pair, 26 x 270 queries of 51 keys 14.3 at 32, 18.6 at 48.)
 static int tree_queries_a_cta(long long queries) {
     constexpr int width[4] = {64, 48, 32, 16};
-    constexpr double cost[4] = {1.0, 0.80, 0.54, 0.32};
+    constexpr double cost[4] = {1.0, 0.80, 0.53, 0.32};
     int best = 0;
     for (int i = 1; i < 4; ++i)
         if (cost[i] * (double)((queries + width[i] - 1) / width[i]) < cost[best] * (double)((queries + width[best] - 1) / width[best])) best = i;
